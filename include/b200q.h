@@ -368,6 +368,50 @@ int b200q_gguf_repack(const void* blocks, int gguf_type, int64_t n_blocks, uint3
                       void* biases, void* stream);
 
 /*
+ * Microscaled 4-bit floating point (the modes mxfp4 and nvfp4 of the reference's quantize, dequantize and qqmm:
+ * mlx/ops.cpp:5036-5099,5208-5340).  Codes are E2M1 (sign, two exponent bits, one mantissa bit; magnitudes 0, .5, 1, 1.5, 2,
+ * 3, 4, 6), eight to a word, first value in the lowest bits; one scale byte per group of consecutive values of a row:
+ *   B200Q_MXFP4  groups of 32, scale 2^(code - 127): floor(log2(largest magnitude)) - 2, at least -127
+ *   B200Q_NVFP4  groups of 16, scale an E4M3 number (sign 0): largest magnitude / (6 G) to the nearest even, at most 448;
+ *                G = global_scale, an fp32 number on the device, > 0 (NULL: 1)
+ * A code is the E2M1 number nearest to value / scale (/ (scale G)), ties to the even code, beyond 6: 6.  All operations are
+ * fp32, rounded once each.  A group with a NaN or an infinity has the scale's NaN (0xFF, 0x7F) and codes 0.
+ *   w / out [rows, K] dtype, wq [rows, K/8], scales [rows, K/group] bytes; global_scale[r / rows_per_scale] is row r's.
+ * Requires K a multiple of the group; wq 8-byte aligned.
+ */
+#define B200Q_MXFP4 0
+#define B200Q_NVFP4 1
+int b200q_fp4_quantize(const void* w, int dtype, int64_t rows, int64_t K, int mode, const float* global_scale,
+                       int64_t rows_per_scale, uint32_t* wq, uint8_t* scales, void* stream);
+int b200q_fp4_dequantize(const uint32_t* wq, const uint8_t* scales, int mode, const float* global_scale, int64_t rows_per_scale,
+                         int dtype, int64_t rows, int64_t K, void* out, void* stream);
+
+/*
+ * Products of rows sorted by group (expert): rows [first_e, first_e + sizes[e]) of x belong to group e, first_e being the
+ * sum of the sizes before it.
+ *   sizes  [E] integers of size_bytes (4 or 8) on the device, read by the kernel only.  Rows past their sum give zeros; a
+ *          negative size counts as 0, groups that reach past row T end there, and both set the status word (code 9).
+ *   b200q_grouped_mm     y[t] = x[t] w[e]^T (transpose: w [E, N, K]) or x[t] w[e] (w [E, K, N]);  bf16 and f16.  The gradient
+ *                        with respect to x is the same call on dy with `transpose` inverted and N, K exchanged.
+ *   b200q_grouped_mm_dw  dw[e] = sum over the rows of e of dy[t]^T x[t]  [E, N, K] (dy [T, N], x [T, K]): the gradient of
+ *                        transpose-form weights; with dy and x (and N, K) exchanged that of the others.  No rows: zeros.
+ *   b200q_grouped_qqmm   y[t] = Gx Gw[e] (quantized x[t]) (wq[e], scales[e])^T: x is quantized on the way in the weights'
+ *                        mode (b200q_fp4_quantize) and both go through the 4-bit tensor cores; every dtype.  sizes NULL and
+ *                        E == 1: the dense product.  scale_per_group: global_scale_w has E entries, else one.
+ * Sums are fp32, results are rounded once.  x, dy and w 16-byte aligned (qqmm: wq only); at most 4096 groups.
+ */
+size_t b200q_grouped_mm_workspace_bytes(int64_t T, int64_t E, int64_t N, int64_t K, int transpose);
+int b200q_grouped_mm(const void* x, const void* w, const void* sizes, int size_bytes, void* y, int dtype, int64_t T, int64_t E,
+                     int64_t N, int64_t K, int transpose, void* ws, size_t ws_bytes, void* stream);
+size_t b200q_grouped_mm_dw_workspace_bytes(int64_t T, int64_t N, int64_t K);
+int b200q_grouped_mm_dw(const void* dy, const void* x, const void* sizes, int size_bytes, void* dw, int dtype, int64_t T, int64_t E,
+                        int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
+size_t b200q_grouped_qqmm_workspace_bytes(int64_t T, int64_t E, int64_t N, int64_t K, int mode);
+int b200q_grouped_qqmm(const void* x, const uint32_t* wq, const uint8_t* scales, const void* sizes, int size_bytes, void* y, int dtype,
+                       int64_t T, int64_t E, int64_t N, int64_t K, int mode, const float* global_scale_x,
+                       const float* global_scale_w, int scale_per_group, void* ws, size_t ws_bytes, void* stream);
+
+/*
  * Introspection for tests and benchmarks: name of the kernel family b200q_qmm would
  * launch for this problem ("qmv_rows", "qmv_mma", "qmm_tcgen05", "qvm",
  * "qmm_generic").

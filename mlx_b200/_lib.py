@@ -12,6 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libb200q.so")
 
 F32, F16, BF16 = 0, 1, 2
+MXFP4, NVFP4 = 0, 1
 OK = 0
 ERR_INVALID_ARGUMENT = -1
 ERR_UNSUPPORTED = -2
@@ -59,6 +60,14 @@ SIGNATURES = {
     "b200q_ipc_close": (_i, [_vp]),
     "b200q_ipc_free": (_i, [_vp]),
     "b200q_gguf_repack": (_i, [_vp, _i, _i64, _vp, _vp, _vp, _vp]),
+    "b200q_fp4_quantize": (_i, [_vp, _i, _i64, _i64, _i, _vp, _i64, _vp, _vp, _vp]),
+    "b200q_fp4_dequantize": (_i, [_vp, _vp, _i, _vp, _i64, _i, _i64, _i64, _vp, _vp]),
+    "b200q_grouped_mm_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i]),
+    "b200q_grouped_mm": (_i, [_vp, _vp, _vp, _i, _vp, _i, _i64, _i64, _i64, _i64, _i, _vp, _sz, _vp]),
+    "b200q_grouped_mm_dw_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "b200q_grouped_mm_dw": (_i, [_vp, _vp, _vp, _i, _vp, _i, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "b200q_grouped_qqmm_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i]),
+    "b200q_grouped_qqmm": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _i64, _i64, _i64, _i64, _i, _vp, _vp, _i, _vp, _sz, _vp]),
     "b200q_qmm_kernel_name": (ctypes.c_char_p, [_i, _i64, _i64, _i64, _i64, _i, _i, _i]),
     "b200q_launch_count": (ctypes.c_uint64, []),
     "b200q_set_weights_constant": (None, [_i]),

@@ -1,0 +1,274 @@
+// Microscaled 4-bit floating point: quantisation and back.
+//
+// E2M1, the 4-bit type: sign, two exponent bits, one mantissa bit; magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6.  Eight to a 32-bit
+// word, first value in the lowest bits; one 8-bit scale per group:
+//   mxfp4, 32 values: 2^e, e = floor(log2(amax)) - 2 (at least -127), stored as e + 127: the largest value comes to lie in
+//          [4, 8) and what is beyond 6 becomes 6; scaling is exact
+//   nvfp4, 16 values: E4M3 s = amax / (6 G) to the nearest even, at most 448; a value is divided by s G.  G is one fp32
+//          number per tensor (or per matrix of a stack): without it, weights of 0.02 would have scales of two or three bits
+// Codes are the nearest, ties to the even one.  Every operation is fp32, rounded once, so that any fp32 program that follows
+// the formulas gets the same codes.  A group with a NaN or an infinity has the scale's NaN (0xFF, 0x7F) and codes 0.
+#include <type_traits>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace b200q {
+namespace {
+
+constexpr int kUnit = 16;   // consecutive values of a thread: a whole nvfp4 group, half an mxfp4 one
+
+// 16 values at `at` (which is 16-byte aligned: ALIGNED; else aligned to its type only).
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void load_unit(const T* at, float (&v)[kUnit]) {
+  if constexpr (ALIGNED) {
+    uint4 raw[sizeof(T)];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * i + j] = __uint_as_float(w[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const T* e = reinterpret_cast<const T*>(&w[j]);
+          v[8 * i + 2 * j] = Elem<T>::to_float(e[0]);
+          v[8 * i + 2 * j + 1] = Elem<T>::to_float(e[1]);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) v[i] = Elem<T>::to_float(at[i]);
+  }
+}
+
+// Eight codes, lowest bits first.
+__device__ __forceinline__ uint32_t e2m1x8(const float* v) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+// The values of two codes (the low byte's low and high half).
+__device__ __forceinline__ float2 e2m1x2_value(uint32_t byte) {
+  uint32_t h;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(h) : "r"(byte));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+__device__ __forceinline__ uint32_t e4m3(float v) {   // v >= 0; beyond 448: 448
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.0f), "f"(v));
+  return r & 0xFFu;
+}
+__device__ __forceinline__ float e4m3_value(uint32_t code) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)code));
+  return __low2float(*reinterpret_cast<const __half2*>(&h));
+}
+__device__ __forceinline__ float e8m0_value(uint32_t code) {
+  return __uint_as_float(code == 255u ? 0x7FC00000u : (code == 0u ? 0x00400000u : code << 23));
+}
+
+// Scale code and codes of a thread's 16 values.  MX: lanes 2i and 2i + 1 share a group; the whole warp calls.
+template <bool MX>
+__device__ __forceinline__ uint32_t quantize_unit(float (&v)[kUnit], float G, uint32_t (&codes)[2]) {
+  // The largest magnitude by its bits, which are ordered as the numbers are, infinities and NaNs last.
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kUnit; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  if constexpr (MX) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+  const bool odd = top >= 0x7F800000u;
+  uint32_t s;
+  if constexpr (MX) {
+    const int f = (int)(top >> 23) - 2;   // biased exponent; subnormal numbers count as 0
+    s = f < 0 ? 0u : (uint32_t)f;
+    const float inv = __uint_as_float((254u - min(s, 252u)) << 23);   // 1 / scale, exact
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) v[i] *= inv;
+    if (odd) s = 255u;
+  } else {
+    s = e4m3(fminf(__fdiv_rn(__uint_as_float(top), 6.0f * G), 448.0f));
+    const float d = e4m3_value(s) * G;
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) v[i] = d == 0.0f ? copysignf(0.0f, v[i]) : __fdiv_rn(v[i], d);
+    if (odd) s = 0x7Fu;
+  }
+  codes[0] = odd ? 0u : e2m1x8(v);
+  codes[1] = odd ? 0u : e2m1x8(v + 8);
+  return s;
+}
+
+constexpr int kQuantThreads = 256;
+
+template <typename T, bool MX, bool ALIGNED>
+__global__ void __launch_bounds__(kQuantThreads)
+fp4_quantize_kernel(const T* __restrict__ w, int64_t units, const float* __restrict__ global, int64_t units_per_global,
+                    uint2* __restrict__ wq, uint8_t* __restrict__ scales) {
+  const int64_t u = (int64_t)blockIdx.x * kQuantThreads + threadIdx.x;
+  const bool in = u < units;
+  float v[kUnit];
+  if (in) load_unit<T, ALIGNED>(w + u * kUnit, v);
+  else
+    for (int i = 0; i < kUnit; ++i) v[i] = 0.0f;
+  const float G = !MX && global && in ? __ldg(global + u / units_per_global) : 1.0f;
+  uint32_t codes[2];
+  const uint32_t s = quantize_unit<MX>(v, G, codes);
+  if (!in) return;
+  wq[u] = make_uint2(codes[0], codes[1]);
+  if (!MX) scales[u] = (uint8_t)s;
+  else if ((u & 1) == 0) scales[u >> 1] = (uint8_t)s;
+}
+
+// Activations: a block has up to kQuantThreads units of one row.
+template <typename T, bool MX, bool ALIGNED>
+__global__ void __launch_bounds__(kQuantThreads)
+fp4_quantize_rows_kernel(const T* __restrict__ x, int64_t K, int blocks_per_row, const float* __restrict__ global,
+                         uint8_t* __restrict__ codes_out, int64_t code_pitch, uint8_t* __restrict__ scales, int64_t sf_pitch) {
+  const int64_t row = blockIdx.x / blocks_per_row;
+  const int64_t u = (int64_t)(blockIdx.x - row * blocks_per_row) * kQuantThreads + threadIdx.x, k = u * kUnit;
+  const bool in = k < K;
+  float v[kUnit];
+  if (in) load_unit<T, ALIGNED>(x + row * K + k, v);
+  else
+    for (int i = 0; i < kUnit; ++i) v[i] = 0.0f;
+  const float G = !MX && global ? __ldg(global) : 1.0f;
+  uint32_t codes[2];
+  const uint32_t s = quantize_unit<MX>(v, G, codes);
+  if (in) *reinterpret_cast<uint2*>(codes_out + row * code_pitch + k / 2) = make_uint2(codes[0], codes[1]);
+  const int64_t at = MX ? u >> 1 : u;
+  if (at < sf_pitch && (!MX || (u & 1) == 0)) scales[row * sf_pitch + at] = in ? (uint8_t)s : (uint8_t)0;
+}
+
+template <typename T, bool MX, bool ALIGNED>
+__global__ void __launch_bounds__(kQuantThreads)
+fp4_dequantize_kernel(const uint2* __restrict__ wq, const uint8_t* __restrict__ scales, int64_t units,
+                      const float* __restrict__ global, int64_t units_per_global, T* __restrict__ out) {
+  const int64_t u = (int64_t)blockIdx.x * kQuantThreads + threadIdx.x;
+  if (u >= units) return;
+  const uint2 c = __ldg(wq + u);
+  const uint32_t code = __ldg(scales + (MX ? u >> 1 : u));
+  const float s = MX ? e8m0_value(code) : e4m3_value(code), G = !MX && global ? __ldg(global + u / units_per_global) : 1.0f;
+  alignas(16) T r[kUnit];
+#pragma unroll
+  for (int i = 0; i < kUnit / 2; ++i) {
+    const float2 q = e2m1x2_value((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+    r[2 * i] = Elem<T>::from_float(q.x * s * G);
+    r[2 * i + 1] = Elem<T>::from_float(q.y * s * G);
+  }
+  T* at = out + u * kUnit;
+  if constexpr (ALIGNED) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) reinterpret_cast<uint4*>(at)[i] = reinterpret_cast<const uint4*>(r)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) at[i] = r[i];
+  }
+}
+
+// A thread makes 16 bytes of a destination row from the aligned words that hold them.
+__global__ void __launch_bounds__(256) repack_rows_kernel(const uint8_t* __restrict__ src, int64_t src_bytes, uint8_t* __restrict__ dst,
+                                                          int64_t dst_pitch, int64_t pieces_per_row, int64_t pieces) {
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (u >= pieces) return;
+  const int64_t row = u / pieces_per_row, at = (u - row * pieces_per_row) * 16;
+  const uint8_t* from = src + row * src_bytes + at;
+  const int64_t left = src_bytes - at;   // bytes of the row from here on
+  const int sh = (int)(reinterpret_cast<uintptr_t>(from) & 3);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(from - sh);
+  uint32_t v[5], r[4];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) v[i] = 4 * i - sh < left && 4 * i - sh < 16 ? __ldg(w + i) : 0u;   // words that hold a byte of the piece
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t n = left - 4 * i;
+    r[i] = __funnelshift_r(v[i], v[i + 1], 8 * sh);
+    if (n < 4) r[i] = n <= 0 ? 0u : r[i] & (0xFFFFFFFFu >> (32 - 8 * (int)n));
+  }
+  *reinterpret_cast<uint4*>(dst + row * dst_pitch + at) = make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <class F>
+int with_type(int dtype, F f) {
+  switch (dtype) {
+    case B200Q_F32: return f(float{});
+    case B200Q_F16: return f(__half{});
+    default: return f(__nv_bfloat16{});
+  }
+}
+template <class F>
+int with_flags(int mode, bool aligned, F f) {
+  using Y = std::true_type;
+  using N = std::false_type;
+  if (mode == B200Q_MXFP4) return aligned ? f(Y{}, Y{}) : f(Y{}, N{});
+  return aligned ? f(N{}, Y{}) : f(N{}, N{});
+}
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+constexpr int64_t kMostBlocks = INT32_MAX;
+
+}  // namespace
+
+int fp4_quantize(const void* w, int dtype, int64_t rows, int64_t K, int mode, const float* global, int64_t rows_per_global,
+                 uint32_t* wq, uint8_t* scales, cudaStream_t st) {
+  const int64_t units = rows * (K / kUnit), blocks = (units + kQuantThreads - 1) / kQuantThreads;
+  if (blocks > kMostBlocks) return fail(B200Q_ERR_UNSUPPORTED, "[quantize] No implementation for problem shape: too many values");
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    return with_flags(mode, aligned16(w), [&](auto mx, auto al) {
+      fp4_quantize_kernel<T, decltype(mx)::value, decltype(al)::value><<<(unsigned)blocks, kQuantThreads, 0, st>>>(
+          static_cast<const T*>(w), units, global, rows_per_global * (K / kUnit), reinterpret_cast<uint2*>(wq), scales);
+      B200Q_LAUNCH_OK("fp4_quantize_kernel");
+      return B200Q_OK;
+    });
+  });
+}
+
+int fp4_dequantize(const uint32_t* wq, const uint8_t* scales, int mode, const float* global, int64_t rows_per_global, int dtype,
+                   int64_t rows, int64_t K, void* out, cudaStream_t st) {
+  const int64_t units = rows * (K / kUnit), blocks = (units + kQuantThreads - 1) / kQuantThreads;
+  if (blocks > kMostBlocks) return fail(B200Q_ERR_UNSUPPORTED, "[dequantize] No implementation for problem shape: too many values");
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    return with_flags(mode, aligned16(out), [&](auto mx, auto al) {
+      fp4_dequantize_kernel<T, decltype(mx)::value, decltype(al)::value><<<(unsigned)blocks, kQuantThreads, 0, st>>>(
+          reinterpret_cast<const uint2*>(wq), scales, units, global, rows_per_global * (K / kUnit), static_cast<T*>(out));
+      B200Q_LAUNCH_OK("fp4_dequantize_kernel");
+      return B200Q_OK;
+    });
+  });
+}
+
+int fp4_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int mode, const float* global, uint8_t* codes,
+                      int64_t code_pitch, uint8_t* scales, int64_t sf_pitch, cudaStream_t st) {
+  const int64_t units = sf_pitch * (mode == B200Q_MXFP4 ? 2 : 1), bpr = (units + kQuantThreads - 1) / kQuantThreads;
+  if (rows * bpr > kMostBlocks) return fail(B200Q_ERR_UNSUPPORTED, "[qqmm] No implementation for problem shape: too many values");
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    return with_flags(mode, aligned16(x), [&](auto mx, auto al) {
+      fp4_quantize_rows_kernel<T, decltype(mx)::value, decltype(al)::value><<<(unsigned)(rows * bpr), kQuantThreads, 0, st>>>(
+          static_cast<const T*>(x), K, (int)bpr, global, codes, code_pitch, scales, sf_pitch);
+      B200Q_LAUNCH_OK("fp4_quantize_rows_kernel");
+      return B200Q_OK;
+    });
+  });
+}
+
+int repack_rows(const void* src, int64_t src_bytes, void* dst, int64_t dst_pitch, int64_t rows, cudaStream_t st) {
+  const int64_t per = dst_pitch / 16, pieces = per * rows, blocks = (pieces + 255) / 256;
+  if (blocks > kMostBlocks) return fail(B200Q_ERR_UNSUPPORTED, "[grouped product] No implementation for problem shape: too many values");
+  repack_rows_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const uint8_t*>(src), src_bytes, static_cast<uint8_t*>(dst), dst_pitch,
+                                                       per, pieces);
+  B200Q_LAUNCH_OK("repack_rows_kernel");
+  return B200Q_OK;
+}
+
+}  // namespace b200q

@@ -372,6 +372,233 @@ PyObject* py_swiglu(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- microscaled 4-bit modes
+// Mode argument: its code and group size; group_size and bits, where given, have to be the mode's.
+bool fp4_mode(PyObject* mode, PyObject* group_size, PyObject* bits, int* code, int* group) {
+  if (!PyUnicode_Check(mode)) return false;
+  if (PyUnicode_CompareWithASCIIString(mode, "mxfp4") == 0) { *code = B200Q_MXFP4; *group = 32; }
+  else if (PyUnicode_CompareWithASCIIString(mode, "nvfp4") == 0) { *code = B200Q_NVFP4; *group = 16; }
+  else return false;
+  int g, b;
+  return integer(group_size, *group, &g) && integer(bits, 4, &b) && g == *group && b == 4;
+}
+// A global scale: None, or a contiguous float32 tensor of one element or of `each`.
+bool global_arg(PyObject* o, int mode, int64_t each, at::Device dev, const float** out, bool* per_matrix) {
+  *out = nullptr;
+  *per_matrix = false;
+  if (o == Py_None) return true;
+  const Tensor* t = tensor(o);
+  if (!t || mode != B200Q_NVFP4 || t->scalar_type() != at::kFloat || t->device() != dev || !t->is_contiguous()) return false;
+  if (t->numel() != 1 && (t->numel() != each || each < 1)) return false;
+  *per_matrix = t->numel() != 1;
+  *out = static_cast<const float*>(t->data_ptr());
+  return true;
+}
+bool on16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+bool fp4_weights(const Tensor& w, const Tensor& s, int group, at::Device dev) {
+  if (w.scalar_type() != at::kUInt32 || s.scalar_type() != at::kByte || w.device() != dev || s.device() != dev) return false;
+  const int64_t nd = w.dim();
+  if (nd < 2 || s.dim() != nd || w.size(nd - 1) * 8 != s.size(nd - 1) * group) return false;
+  for (int64_t i = 0; i < nd - 1; ++i)
+    if (s.size(i) != w.size(i)) return false;
+  return w.is_contiguous() && s.is_contiguous() && on16(w);
+}
+int64_t matrices(const Tensor& w) { return product(w.sizes().slice(0, w.dim() - 2)); }
+
+PyObject* py_fp4_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {   // (w, group_size, bits, mode, global_scale)
+  HANDLE_TH_ERRORS
+  const Tensor* w;
+  int mode, group;
+  if (n != 5 || !(w = tensor(a[0])) || !fp4_mode(a[3], a[1], a[2], &mode, &group)) return none();
+  const int dt = dtype_code(w->scalar_type());
+  const at::Device dev = w->device();
+  if (dt < 0 || !current(dev) || w->dim() < 2 || !w->is_contiguous() || w->numel() == 0) return none();
+  const int64_t K = w->size(-1), rows = w->numel() / K;
+  const float* g;
+  bool each;
+  if (K % group != 0 || !global_arg(a[4], mode, matrices(*w), dev, &g, &each)) return none();
+  c10::SmallVector<int64_t, 6> size(w->sizes().begin(), w->sizes().end());
+  size.back() = K / 8;
+  Tensor wq = at::detail::empty_cuda(size, at::kUInt32, dev, std::nullopt);
+  size.back() = K / group;
+  Tensor s = at::detail::empty_cuda(size, at::kByte, dev, std::nullopt);
+  void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  if (b200q_fp4_quantize(w->data_ptr(), dt, rows, K, mode, g, each ? w->size(-2) : rows, static_cast<uint32_t*>(wq.data_ptr()),
+                         static_cast<uint8_t*>(s.data_ptr()), stream) != B200Q_OK)
+    return none();
+  PyObject* out = PyTuple_New(2);
+  if (!out) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(wq)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(s)));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_fp4_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {   // (w, scales, group_size, bits, mode, dtype code, global_scale)
+  HANDLE_TH_ERRORS
+  const Tensor *w, *s;
+  int mode, group, dt;
+  if (n != 7 || !(w = tensor(a[0])) || !(s = tensor(a[1])) || !fp4_mode(a[4], a[2], a[3], &mode, &group) || !integer(a[5], -1, &dt))
+    return none();
+  const at::Device dev = w->device();
+  const float* g;
+  bool each;
+  if (dt < 0 || dt > B200Q_BF16 || !current(dev) || !fp4_weights(*w, *s, group, dev) || w->numel() == 0 ||
+      !global_arg(a[6], mode, matrices(*w), dev, &g, &each))
+    return none();
+  const int64_t K = w->size(-1) * 8, rows = w->numel() / w->size(-1);
+  c10::SmallVector<int64_t, 6> size(w->sizes().begin(), w->sizes().end());
+  size.back() = K;
+  Tensor out = at::detail::empty_cuda(size, dt == B200Q_F32 ? at::kFloat : (dt == B200Q_F16 ? at::kHalf : at::kBFloat16), dev, std::nullopt);
+  void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  if (b200q_fp4_dequantize(static_cast<const uint32_t*>(w->data_ptr()), static_cast<const uint8_t*>(s->data_ptr()), mode, g,
+                           each ? w->size(-2) : rows, dt, rows, K, out.data_ptr(), stream) != B200Q_OK)
+    return none();
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- products grouped by expert
+bool sizes_ok(const Tensor& t, int64_t E, at::Device dev) {
+  return (t.scalar_type() == at::kLong || t.scalar_type() == at::kInt) && t.dim() == 1 && t.size(0) == E && t.device() == dev && t.is_contiguous();
+}
+
+// (x, w, scales, sizes or None, group_size, bits, mode, global_scale_x, global_scale_w)
+PyObject* py_qqmm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *x, *w, *s, *sizes;
+  int mode, group;
+  if (n != 9 || !(x = tensor(a[0])) || !(w = tensor(a[1])) || !(s = tensor(a[2])) || !index_arg(a[3], &sizes) ||
+      !fp4_mode(a[6], a[4], a[5], &mode, &group))
+    return none();
+  const at::ScalarType t = x->scalar_type();
+  const int dt = dtype_code(t);
+  const at::Device dev = x->device();
+  if (dt < 0 || !current(dev) || !x->is_contiguous() || !fp4_weights(*w, *s, group, dev) || checked()) return none();
+  if (sizes ? x->dim() != 2 || w->dim() != 3 : x->dim() < 1 || w->dim() != 2) return none();
+  const int64_t E = sizes ? w->size(0) : 1, N = w->size(-2), K = w->size(-1) * 8;
+  const float *gx, *gw;
+  bool each_x, each_w;
+  if (x->size(-1) != K || x->numel() == 0 || N == 0 || E == 0 || (sizes && !sizes_ok(*sizes, E, dev)) ||
+      !global_arg(a[7], mode, 1, dev, &gx, &each_x) || !global_arg(a[8], mode, E, dev, &gw, &each_w))
+    return none();
+  const int64_t T = x->numel() / K;
+  void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const Scratch* ws = find_scratch(dev.index(), stream, 2, b200q_grouped_qqmm_workspace_bytes(T, E, N, K, mode));
+  if (!ws) return none();
+  c10::SmallVector<int64_t, 6> size(x->sizes().begin(), x->sizes().end());
+  size.back() = N;
+  Tensor y = at::detail::empty_cuda(size, t, dev, std::nullopt);
+  if (b200q_grouped_qqmm(x->data_ptr(), static_cast<const uint32_t*>(w->data_ptr()), static_cast<const uint8_t*>(s->data_ptr()),
+                         sizes ? sizes->data_ptr() : nullptr, sizes && sizes->scalar_type() == at::kLong ? 8 : 4, y.data_ptr(), dt, T, E,
+                         N, K, mode, gx, gw, each_w, ws->ptr, ws->bytes, stream) != B200Q_OK)
+    return none();
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+bool grouped_run(const Tensor& x, const Tensor& w, const Tensor& sizes, bool transpose, Tensor* y) {
+  const at::ScalarType t = x.scalar_type();
+  const at::Device dev = x.device();
+  if ((t != at::kHalf && t != at::kBFloat16) || w.scalar_type() != t || w.device() != dev || !current(dev) || x.dim() != 2 || w.dim() != 3 ||
+      !x.is_contiguous() || !w.is_contiguous() || !on16(x) || !on16(w) || checked())
+    return false;
+  const int64_t E = w.size(0), N = w.size(transpose ? 1 : 2), K = w.size(transpose ? 2 : 1), T = x.size(0);
+  if (x.size(1) != K || T == 0 || N == 0 || K == 0 || E == 0 || !sizes_ok(sizes, E, dev)) return false;
+  void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const Scratch* ws = find_scratch(dev.index(), stream, 2, b200q_grouped_mm_workspace_bytes(T, E, N, K, transpose));
+  if (!ws) return false;
+  *y = at::detail::empty_cuda({T, N}, t, dev, std::nullopt);
+  return b200q_grouped_mm(x.data_ptr(), w.data_ptr(), sizes.data_ptr(), sizes.scalar_type() == at::kLong ? 8 : 4, y->data_ptr(),
+                          dtype_code(t), T, E, N, K, transpose, ws->ptr, ws->bytes, stream) == B200Q_OK;
+}
+bool grouped_dw_run(const Tensor& dy, const Tensor& x, const Tensor& sizes, bool transpose, Tensor* dw) {
+  const at::ScalarType t = x.scalar_type();
+  const at::Device dev = x.device();
+  if ((t != at::kHalf && t != at::kBFloat16) || dy.scalar_type() != t || dy.device() != dev || !current(dev) || x.dim() != 2 ||
+      dy.dim() != 2 || sizes.dim() != 1 || !x.is_contiguous() || !dy.is_contiguous() || !on16(x) || !on16(dy) || checked())
+    return false;
+  const Tensor &a = transpose ? dy : x, &b = transpose ? x : dy;
+  const int64_t E = sizes.size(0), N = a.size(1), K = b.size(1), T = x.size(0);
+  if (dy.size(0) != T || T == 0 || N == 0 || K == 0 || E == 0 || !sizes_ok(sizes, E, dev)) return false;
+  void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const Scratch* ws = find_scratch(dev.index(), stream, 2, b200q_grouped_mm_dw_workspace_bytes(T, N, K));
+  if (!ws) return false;
+  *dw = at::detail::empty_cuda({E, N, K}, t, dev, std::nullopt);
+  return b200q_grouped_mm_dw(a.data_ptr(), b.data_ptr(), sizes.data_ptr(), sizes.scalar_type() == at::kLong ? 8 : 4, dw->data_ptr(),
+                             dtype_code(t), T, E, N, K, ws->ptr, ws->bytes, stream) == B200Q_OK;
+}
+bool boolean(PyObject* o, bool* out) {
+  *out = o == Py_True;
+  return PyBool_Check(o);
+}
+
+PyObject* py_grouped_mm(PyObject*, PyObject* const* a, Py_ssize_t n) {   // (x, w, sizes, transpose)
+  HANDLE_TH_ERRORS
+  const Tensor *x, *w, *sizes;
+  bool transpose;
+  Tensor y;
+  if (n != 4 || !(x = tensor(a[0])) || !(w = tensor(a[1])) || !(sizes = tensor(a[2])) || !boolean(a[3], &transpose)) return none();
+  if (!grouped_run(*x, *w, *sizes, transpose, &y)) return none();
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_grouped_mm_dw(PyObject*, PyObject* const* a, Py_ssize_t n) {   // (dy, x, sizes, transpose)
+  HANDLE_TH_ERRORS
+  const Tensor *dy, *x, *sizes;
+  bool transpose;
+  Tensor dw;
+  if (n != 4 || !(dy = tensor(a[0])) || !(x = tensor(a[1])) || !(sizes = tensor(a[2])) || !boolean(a[3], &transpose)) return none();
+  if (!grouped_dw_run(*dy, *x, *sizes, transpose, &dw)) return none();
+  return THPVariable_Wrap(std::move(dw));
+  END_HANDLE_TH_ERRORS
+}
+
+// grouped_mm with gradients for x and w
+struct GroupedFn : public torch::autograd::Function<GroupedFn> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& sizes, bool transpose, Tensor* y) {
+    ctx->save_for_backward({x, w, sizes});
+    ctx->saved_data["transpose"] = transpose;
+    ctx->saved_data["dx"] = x.requires_grad();
+    ctx->saved_data["dw"] = w.requires_grad();
+    return *y;   // by address: a result passed as a tensor would come back as a view of itself
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &sizes = saved[2];
+    const bool transpose = ctx->saved_data["transpose"].toBool();
+    Tensor dx, dw;
+    if (!grads[0].defined()) return {dx, dw, Tensor(), Tensor(), Tensor()};
+    const Tensor dy = grads[0].contiguous();
+    pybind11::gil_scoped_acquire gil;   // the scratch table, and the Python forms
+    at::AutoDispatchBelowAutograd below;
+    auto python = [&](const char* name, const Tensor& p, const Tensor& q, bool t) {
+      const auto ops = pybind11::module_::import("mlx_b200.ops");
+      auto wrap = [](const Tensor& v) { return pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(v)); };
+      pybind11::object r = ops.attr(name)(wrap(p), wrap(q), wrap(sizes), t);
+      return Tensor(THPVariable_Unpack(r.ptr()));
+    };
+    if (ctx->saved_data["dx"].toBool() && !grouped_run(dy, w, sizes, !transpose, &dx)) dx = python("grouped_mm", dy, w, !transpose);
+    if (ctx->saved_data["dw"].toBool() && !grouped_dw_run(dy, x, sizes, transpose, &dw)) dw = python("grouped_mm_dw", dy, x, transpose);
+    return {dx, dw, Tensor(), Tensor(), Tensor()};
+  }
+};
+PyObject* py_grouped_mm_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {   // (x, w, sizes, transpose)
+  HANDLE_TH_ERRORS
+  const Tensor *x, *w, *sizes;
+  bool transpose;
+  Tensor y;
+  if (n != 4 || !(x = tensor(a[0])) || !(w = tensor(a[1])) || !(sizes = tensor(a[2])) || !boolean(a[3], &transpose)) return none();
+  if (x->_fw_grad(0).defined() || w->_fw_grad(0).defined()) return none();   // the Python form says that it has no forward mode
+  {
+    at::AutoDispatchBelowAutograd below;
+    if (!grouped_run(*x, *w, *sizes, transpose, &y)) return none();
+  }
+  if ((x->requires_grad() || w->requires_grad()) && at::GradMode::is_enabled()) y = GroupedFn::apply(*x, *w, *sizes, transpose, &y);
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
 // (device index, stream, operator, address, bytes): ops._workspaces has a new buffer
 PyObject* py_scratch(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 5) { PyErr_SetString(PyExc_TypeError, "scratch takes five arguments"); return nullptr; }
@@ -390,6 +617,12 @@ PyMethodDef methods[] = {
     {"dequantize", (PyCFunction)(void (*)(void))py_dequantize, METH_FASTCALL, nullptr},
     {"gather", (PyCFunction)(void (*)(void))py_gather, METH_FASTCALL, nullptr},
     {"swiglu", (PyCFunction)(void (*)(void))py_swiglu, METH_FASTCALL, nullptr},
+    {"fp4_quantize", (PyCFunction)(void (*)(void))py_fp4_quantize, METH_FASTCALL, nullptr},
+    {"fp4_dequantize", (PyCFunction)(void (*)(void))py_fp4_dequantize, METH_FASTCALL, nullptr},
+    {"qqmm", (PyCFunction)(void (*)(void))py_qqmm, METH_FASTCALL, nullptr},
+    {"grouped_mm", (PyCFunction)(void (*)(void))py_grouped_mm, METH_FASTCALL, nullptr},
+    {"grouped_mm_dw", (PyCFunction)(void (*)(void))py_grouped_mm_dw, METH_FASTCALL, nullptr},
+    {"grouped_mm_grad", (PyCFunction)(void (*)(void))py_grouped_mm_grad, METH_FASTCALL, nullptr},
     {"scratch", (PyCFunction)(void (*)(void))py_scratch, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_front", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,930 @@
+// Products over groups of rows with ragged sizes, on the 5th-generation tensor cores.  Rows of group e are consecutive:
+//   KK   out[t, i] = sum_k a[e, i, k] b[t, k]      the weights' reduced dimension is contiguous
+//   MK   out[t, i] = sum_k a[e, k, i] b[t, k]      the weights' output dimension is contiguous
+//   MM   out[e, j, i] = sum_t a[t, i] b[t, j]      gradient of the weights: the sum goes over the group's rows
+//   Mx, Nv  as KK, a and b in microscaled 4-bit floating point (fp4.cuh), times the operands' global scales
+// One group without sizes is the dense product.
+//
+// D[i, j] has the output's contiguous dimension on the accumulator's lanes (256 over a pair of thread blocks, cta_group::2)
+// and up to 256 rows of the output as columns: a tile costs what its rows cost, in steps of 16, so ragged groups and
+// single tokens need no other kernel.  Each block of the pair fetches 128 of the i and half of the j; 16-bit operands need
+// 64 bytes per clock and SM that way, the L2's rate, where a block of its own would need 94.
+//
+//   warp 0      TMA: both operands of a stage (128 bytes of k per row; MM and MK: 64 k)
+//   warp 1      tcgen05.mma, and for 4 bits tcgen05.cp of the stage's scales (leader block, one thread)
+//   warp 2      MM only: the stage that a group ends in has its foreign rows zeroed in shared memory (both operands: a foreign
+//               infinity times zero would be NaN)
+//   warps 4-7   4 bits only: scales from global memory (row-major, any alignment) into the order that tensor memory wants
+//   warps 8-15  epilogue: accumulator -> rounding -> stmatrix staging -> 16-byte stores
+//
+// The table of groups (first row, first tile, first step) is built in shared memory by every block from `sizes`, which the
+// host never reads: no launch in front and no synchronisation.
+//
+// Tiles are dealt to the pairs in whole waves.  What is left over is laid end to end and cut into equal ranges of K where
+// that gains more than the partial sums cost; the last pair to arrive adds a tile's parts in order (no atomics on values,
+// the same bits every time), and nobody waits for another pair.
+//
+// Every wait is bounded: when one runs out, the role raises the block's abort flag and the status word, all roles leave, tensor
+// memory is freed and the kernel ends.
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "tc_ptx.cuh"
+
+namespace b200q {
+namespace {
+
+using namespace tc;
+
+enum class Kind { KK, MK, MM, Mx, Nv };
+template <Kind K> constexpr bool kFp4 = K == Kind::Mx || K == Kind::Nv;
+
+constexpr int kLanes = 128;          // i per block
+constexpr int kTileI = 2 * kLanes;
+constexpr int kMaxNT = 256;
+constexpr int kStageA = kLanes * 128;
+constexpr int kMaxStages = 12;
+constexpr int kSfSlots = 4;          // chunks of scales: 32 bytes per row each
+constexpr int kWarps = 16, kThreads = 32 * kWarps;
+constexpr int kScaleWarp0 = 4, kScaleWarps = 4, kEpiWarp0 = 8, kEpiWarps = 8;
+constexpr int kStageOut = 2048;      // epilogue staging per warp: 32 rows of 64 bytes
+constexpr int kSfColumns = 96;       // two buffers of 16 (a) + 32 (b) columns
+constexpr size_t kSmemMax = 227 * 1024;
+
+// k per stage, and stages per step: the unit in which K is cut (4 bits: what a chunk of scales covers)
+template <Kind K> constexpr int kStageK = kFp4<K> ? 256 : 64;
+template <Kind K> constexpr int kSpc = K == Kind::Mx ? 4 : (K == Kind::Nv ? 2 : 1);
+
+struct Maps {
+  CUtensorMap a;
+  CUtensorMap b[5];   // boxes of 128, 64, 32, 16 and 8 rows (MM: the first only, 64 x 64)
+};
+
+struct Params {
+  const void* sizes;       // null: one group of T rows
+  int size_bytes;          // 4 or 8
+  int E, T;
+  int I, J, K;             // output width; MM: output rows per group; length of the sum (MM: unused)
+  int NT, i_tiles, stages;
+  int sfb_chunk;           // 4 bits: bytes of a chunk of b's scales
+  void* out;
+  int vec;                 // rows of the output start on 16-byte boundaries
+  const uint8_t* sfa;      // scales [E * I, sf_row] and [T, sfb_pitch]
+  const uint8_t* sfb;
+  int sf_row, sfb_pitch;
+  int sfa16;               // rows of sfa on 16-byte boundaries
+  const float* ga;         // global scales: one, or (ga_each) one per group
+  const float* gb;
+  int ga_each;
+  float* partial;          // [2 * pairs][block of the pair][NT][128]; null: no tile is cut
+  uint32_t* counters;      // [pairs][block of the pair]
+  int cut_gain, cut_cost;  // cycles of a step, and what a cut tile costs beyond its steps
+  uint32_t* status;
+};
+
+struct __align__(8) Bars {
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  uint64_t landed[kMaxStages];                     // MM: this block's tiles are there, foreign rows and all
+  uint64_t sf_full[kSfSlots], sf_empty[kSfSlots];
+  uint64_t acc_full[2], acc_empty[2];
+  uint32_t tmem_base;
+  int abort_flag, last, seen[2];
+  // schedule
+  int full_units, cut_pairs, cut_steps;   // tiles in whole waves; pairs and steps of the rest
+  int cut_base;                           // step at which the rest begins
+  int rows;                               // rows that belong to a group
+};
+
+// The table of groups: entry e is where group e begins.
+struct Table {
+  int* row;
+  int* unit;
+  int* step;
+};
+
+struct Piece {
+  int e, i0;          // group; first i of the pair
+  int row0, rows;     // first output row (MM: row of b's columns) and how many are valid
+  int neff;           // the same, rounded up to what the MMA takes
+  int t0, len;        // MM: first row of the group and their number
+  int ks0, ks1;       // stages
+  int parts, part, j0;   // of a cut tile: number of parts, this one's number, first part's pair
+};
+
+template <Kind KIND>
+__device__ __forceinline__ int group_steps(const Params& p, int len) {
+  const int st = KIND == Kind::MM ? max(1, (len + kStageK<KIND> - 1) / kStageK<KIND>) : (p.K + kStageK<KIND> - 1) / kStageK<KIND>;
+  return (st + kSpc<KIND> - 1) / kSpc<KIND>;
+}
+// Rows per tile of a group: as even as multiples of 16 allow.
+__device__ __forceinline__ int tile_rows(int len, int nt) {
+  const int n = (len + nt - 1) / nt;
+  return n == 0 ? nt : ((len + n - 1) / n + 15) & ~15;
+}
+template <Kind KIND>
+__device__ __forceinline__ int tiles_j(const Params& p, int len) {
+  if (KIND == Kind::MM) return (p.J + p.NT - 1) / p.NT;
+  const int tr = tile_rows(len, p.NT);
+  return (len + tr - 1) / tr;
+}
+
+// Walks over a pair's pieces; every role has one.
+template <Kind KIND>
+struct Walk {
+  const Params& p;
+  const Bars& b;
+  const Table& tab;
+  int pair, pairs;
+  int u;             // next whole tile
+  int pos, end;      // next step of the pair's range, and its end
+  __device__ Walk(const Params& p_, const Bars& b_, const Table& t_) : p(p_), b(b_), tab(t_), pair(blockIdx.x >> 1), pairs(gridDim.x >> 1) {
+    u = pair;
+    pos = end = 0;
+    if (pair < b.cut_pairs) {
+      pos = b.cut_base + (int)((long long)b.cut_steps * pair / b.cut_pairs);
+      end = b.cut_base + (int)((long long)b.cut_steps * (pair + 1) / b.cut_pairs);
+    }
+  }
+  __device__ __forceinline__ int find(const int* first, int v) const {   // the last group that begins at or before v (and is not empty)
+    int lo = 0, hi = p.E;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (first[mid] <= v) lo = mid; else hi = mid;
+    }
+    return lo;
+  }
+  __device__ __forceinline__ int owner(int at) const {   // pair whose range holds step `at`
+    return (int)((((long long)(at - b.cut_base) + 1) * b.cut_pairs - 1) / b.cut_steps);
+  }
+  __device__ bool next(Piece& c) {
+    int v, k0, k1, e, steps;
+    c.parts = 1;
+    if (u < b.full_units) {
+      e = find(tab.unit, u);
+      v = u - tab.unit[e];
+      u += pairs;
+      steps = group_steps<KIND>(p, tab.row[e + 1] - tab.row[e]);
+      k0 = 0;
+      k1 = steps;
+    } else if (pos < end) {
+      e = find(tab.step, pos);
+      steps = group_steps<KIND>(p, tab.row[e + 1] - tab.row[e]);
+      const int off = pos - tab.step[e];
+      v = off / steps;
+      k0 = off - v * steps;
+      const int first = pos - k0;
+      k1 = min(steps, end - first);
+      c.j0 = owner(first);
+      c.parts = owner(first + steps - 1) - c.j0 + 1;
+      c.part = pair - c.j0;
+      pos = first + k1;
+    } else {
+      return false;
+    }
+    const int len = tab.row[e + 1] - tab.row[e], nj = tiles_j<KIND>(p, len), it = v / nj, jt = v - it * nj;
+    c.e = e;
+    c.i0 = it * kTileI;
+    c.t0 = tab.row[e];
+    c.len = len;
+    if (KIND == Kind::MM) {
+      c.row0 = jt * p.NT;
+      c.rows = min(p.NT, p.J - c.row0);
+      c.neff = (c.rows + 127) & ~127;
+    } else {
+      const int tr = tile_rows(len, p.NT);
+      c.row0 = c.t0 + jt * tr;
+      c.rows = min(tr, c.t0 + len - c.row0);
+      c.neff = (c.rows + 15) & ~15;
+    }
+    const int st = KIND == Kind::MM ? max(1, (len + kStageK<KIND> - 1) / kStageK<KIND>) : (p.K + kStageK<KIND> - 1) / kStageK<KIND>;
+    c.ks0 = k0 * kSpc<KIND>;
+    c.ks1 = min(st, k1 * kSpc<KIND>);
+    return true;
+  }
+};
+
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
+// Into this block's shared memory, counted on the pair leader's barrier.
+__device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t leader_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(leader_bar)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_release_cluster(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+// Bounded wait of the MMA thread for what the other block's threads have written too.
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  for (uint32_t i = 0; i < kSpinLimit * 4u; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((i & 1023) == 1023 && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 128-byte-swizzled operand tile.  K-major: rows of 128 bytes of k, 8-row groups 1024 bytes apart.  M-major: rows of 64
+// i (or j), one per k, 8-k groups 1024 bytes apart, blocks of 64 i 8192 bytes apart.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, bool mn_major) {
+  const uint32_t lbo = mn_major ? 8192 : 16;
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// 32 rows of 16 bytes of scales, not swizzled: 8-row groups 128 bytes apart.
+__device__ __forceinline__ uint64_t scales_desc(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+// The 512 bytes of 128 rows' scales, from each block's shared memory into all four lane quarters of its tensor memory.
+__device__ __forceinline__ void tcgen05_cp_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+template <Kind KIND>
+__device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
+  if constexpr (KIND == Kind::Nv)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+        : "memory");
+}
+// Instruction descriptors, without N (and without the place of the scales in their word).
+template <typename T, Kind KIND>
+__device__ __forceinline__ uint32_t make_idesc(int n) {
+  const uint32_t shape = ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileI >> 4) << 24);
+  if constexpr (kFp4<KIND>) return shape | (1u << 7) | (1u << 10) | (KIND == Kind::Mx ? 1u << 23 : 0u);   // E2M1; scales UE8M0 or UE4M3
+  constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return shape | (1u << 4) | (fmt << 7) | (fmt << 10) | (KIND != Kind::KK ? 1u << 15 : 0u) | (KIND == Kind::MM ? 1u << 16 : 0u);
+}
+
+// 16 bytes at any address, of which those before `end` are read (and the rest are zeros).
+__device__ __forceinline__ uint4 load16_any(const uint8_t* at, const uint8_t* end) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(at);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
+  const int sh = (int)(a & 3) * 8;
+  const uint32_t* stop = reinterpret_cast<const uint32_t*>((reinterpret_cast<uintptr_t>(end) + 3) & ~uintptr_t(3));
+  uint32_t v[5];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) v[i] = w + i < stop ? __ldg(w + i) : 0u;
+  uint32_t r[4];
+  const long long left = end - at;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[i] = __funnelshift_r(v[i], v[i + 1], sh);
+    const long long n = left - 4 * i;
+    if (n < 4) r[i] = n <= 0 ? 0u : r[i] & (0xFFFFFFFFu >> (32 - 8 * (int)n));
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+__device__ __forceinline__ void sts32(uint32_t at, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+__device__ __forceinline__ void lds128(uint32_t at, uint4& v) {
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+}
+// A chunk's word k of row r: blocks of 128 rows x 4 bytes of k, in which row r has word (r % 32) * 4 + r / 32.
+__device__ __forceinline__ void store_scales(uint32_t base, uint32_t k_stride, int r, int half, const uint4& v) {
+  const uint32_t at = base + (r >> 7) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + half * 4 * k_stride;
+  sts32(at, v.x);
+  sts32(at + k_stride, v.y);
+  sts32(at + 2 * k_stride, v.z);
+  sts32(at + 3 * k_stride, v.w);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  uint32_t d;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+  return d;
+}
+// 32 lanes x 16 columns of the accumulator, as mma fragments.
+__device__ __forceinline__ void load_16(uint32_t tmem, uint32_t (&r)[16]) {
+  tcgen05_ld_16x16(tmem, r);
+  tcgen05_ld_16x16(tmem + (16u << 16), r + 8);
+}
+
+// Element (row, i) of the output, of type T.
+template <typename T, Kind KIND>
+__device__ __forceinline__ T* out_row(const Params& p, const Piece& c, int row) {
+  const long long r = (KIND == Kind::MM ? (long long)c.e * p.J : 0) + c.row0 + row;
+  return static_cast<T*>(p.out) + r * p.I;
+}
+// Four consecutive i of one row.
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, int left, bool vec, float a, float b, float c, float d) {
+  if (vec && left >= 4) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = make_float4(a, b, c, d);
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(a, b), pack2<T>(c, d));
+  } else {
+    const float v[4] = {a, b, c, d};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) dst[i] = Elem<T>::from_float(v[i]);
+  }
+}
+
+template <typename T, Kind KIND>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+  constexpr bool kSf = kFp4<KIND>, kSum = KIND == Kind::MM;
+  constexpr int kSb = KIND == Kind::Mx ? 8 : 16;   // bytes of scales per row and stage
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t stage_bytes = kStageA + (uint32_t)p.NT * 64u;
+  unsigned char* ring_sf = smem + (size_t)p.stages * stage_bytes;
+  const uint32_t sf_bytes = kSf ? 4096u + (uint32_t)p.sfb_chunk : 0u;
+  unsigned char* staging = ring_sf + kSfSlots * sf_bytes;
+  Bars* bars = reinterpret_cast<Bars*>(staging + (sizeof(T) == 2 ? kEpiWarps * kStageOut : 0));
+  Table tab;
+  tab.row = reinterpret_cast<int*>(bars + 1);
+  tab.unit = tab.row + p.E + 1;
+  tab.step = tab.unit + p.E + 1;
+  volatile int* abort_flag = &bars->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_rank();
+
+  if (warp == 0) {
+    if (lane < p.stages) {
+      mbar_init(smem_u32(&bars->full[lane]), kSum ? 2 : 1);
+      mbar_init(smem_u32(&bars->empty[lane]), 1);
+      mbar_init(smem_u32(&bars->landed[lane]), 1);
+    }
+    if (lane < kSfSlots) { mbar_init(smem_u32(&bars->sf_full[lane]), 2); mbar_init(smem_u32(&bars->sf_empty[lane]), 1); }
+    if (lane < 2) { mbar_init(smem_u32(&bars->acc_full[lane]), 1); mbar_init(smem_u32(&bars->acc_empty[lane]), 2 * kEpiWarps); }
+    if (lane == 0) bars->abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
+  } else if (warp == 1) {
+    tcgen05_alloc(smem_u32(&bars->tmem_base), 512);
+    tcgen05_relinquish();
+  } else if (warp == 2) {
+    // The table: a lane takes E / 32 consecutive groups.
+    if (lane == 0) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.b[4]) : "memory");
+    }
+    const int per = (p.E + 31) / 32, lo = min(p.E, lane * per), hi = min(p.E, lo + per);
+    bool bad = false;
+    long long rows = 0;
+    auto size_of = [&](int e) -> long long {
+      if (!p.sizes) return p.T;
+      const long long n = p.size_bytes == 8 ? static_cast<const long long*>(p.sizes)[e] : static_cast<const int*>(p.sizes)[e];
+      bad |= n < 0 || n > p.T;
+      return n < 0 ? 0 : (n > p.T ? p.T : n);
+    };
+    for (int e = lo; e < hi; ++e) rows += size_of(e);
+    long long before = rows;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const long long v = __shfl_up_sync(0xFFFFFFFFu, before, d);
+      if (lane >= d) before += v;
+    }
+    before -= rows;
+    bad |= before + rows > p.T;
+    int units = 0, steps = 0;
+    long long at = before;
+    for (int e = lo; e < hi; ++e) {
+      const int r0 = (int)min(at, (long long)p.T);
+      at += size_of(e);
+      const int len = (int)min(at, (long long)p.T) - r0, n = tiles_j<KIND>(p, len) * p.i_tiles;
+      tab.row[e] = r0;
+      tab.unit[e] = units;
+      tab.step[e] = steps;
+      units += n;
+      steps += n * group_steps<KIND>(p, len);
+    }
+    int u0 = units, s0 = steps;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int a = __shfl_up_sync(0xFFFFFFFFu, u0, d), b = __shfl_up_sync(0xFFFFFFFFu, s0, d);
+      if (lane >= d) { u0 += a; s0 += b; }
+    }
+    const int total = __shfl_sync(0xFFFFFFFFu, u0, 31), all_steps = __shfl_sync(0xFFFFFFFFu, s0, 31);
+    u0 -= units;
+    s0 -= steps;
+    for (int e = lo; e < hi; ++e) { tab.unit[e] += u0; tab.step[e] += s0; }
+    const int last_row = (int)min(__shfl_sync(0xFFFFFFFFu, at, 31), (long long)p.T);
+    bad = __any_sync(0xFFFFFFFFu, bad);
+    __syncwarp();
+    if (lane == 0) {
+      tab.row[p.E] = last_row;
+      tab.unit[p.E] = total;
+      tab.step[p.E] = all_steps;
+      bars->rows = last_row;
+      const int pairs = gridDim.x >> 1;
+      int full = total - total % pairs, cut_pairs = 0, base = 0, rest = 0;
+      if (full < total && p.partial) {
+        int e = 0, h = p.E;   // the group in which the rest begins
+        while (h - e > 1) { const int m = (e + h) >> 1; if (tab.unit[m] <= full) e = m; else h = m; }
+        base = tab.step[e] + (full - tab.unit[e]) * group_steps<KIND>(p, tab.row[e + 1] - tab.row[e]);
+        rest = all_steps - base;
+        cut_pairs = min(pairs, rest);
+        // a whole wave takes as long as one tile, the cut one its share
+        if ((long long)rest * p.cut_gain / (total - full) - (long long)rest * p.cut_gain / cut_pairs <= p.cut_cost) cut_pairs = 0;
+      }
+      bars->full_units = cut_pairs ? full : total;
+      bars->cut_pairs = cut_pairs;
+      bars->cut_steps = rest;
+      bars->cut_base = base;
+      if (bad && blockIdx.x == 0) atomicMax(p.status, 9u);
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tcgen05_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  const int nacc = 2 * p.NT + (kSf ? kSfColumns : 0) <= 512 ? 2 : 1;
+  const uint32_t tmem_sf = tmem + nacc * p.NT;
+  const uint32_t ring = smem_u32(smem);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ operands
+    if (elect_one()) {
+      const uint32_t full = smem_u32(&bars->full[0]), lfull = leader_addr(full), empty = smem_u32(&bars->empty[0]), landed = smem_u32(&bars->landed[0]);
+      Walk<KIND> walk(p, *bars, tab);
+      Piece c;
+      uint32_t s = 0, ph = 1;
+      bool ok = true;
+      while (ok && walk.next(c)) {
+        const int half = c.neff >> 1;
+        const uint32_t mine = kStageA + (uint32_t)half * 128u;
+        for (int ks = c.ks0; ks < c.ks1; ++ks) {
+          if (!mbar_nap<20>(empty + s * 8, ph, abort_flag)) { ok = false; break; }
+          const uint32_t a = ring + s * stage_bytes, b = a + kStageA;
+          if constexpr (kSum) {
+            const uint32_t bar = landed + s * 8;
+            const int t = c.t0 + ks * 64;
+            mbar_expect_tx(bar, mine);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) tma_3d(a + h * 8192, &maps.a, c.i0 + rank * kLanes + 64 * h, t, 0, bar);
+            for (int h = 0; h < half / 64; ++h) tma_3d(b + h * 8192, &maps.b[0], c.row0 + rank * half + 64 * h, t, 0, bar);
+          } else {
+            const uint32_t bar = lfull + s * 8;
+            const int k = ks * (kSf ? 128 : 64);
+            if (rank == 0) mbar_expect_tx(full + s * 8, 2 * mine);
+            if constexpr (KIND == Kind::MK) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) tma_3d_pair(a + h * 8192, &maps.a, c.i0 + rank * kLanes + 64 * h, k, c.e, bar);
+            } else {
+              tma_3d_pair(a, &maps.a, k, c.i0 + rank * kLanes, c.e, bar);
+            }
+            int r = 0;
+            const int row = c.row0 + rank * half;
+#pragma unroll
+            for (int i = 0; i < 5; ++i) {
+              const int box = 128 >> i;
+              if (half & box) {
+                tma_3d_pair(b + r * 128, &maps.b[i], k, row + r, 0, bar);
+                r += box;
+              }
+            }
+          }
+          if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; }
+        }
+      }
+      if (!ok) for (int i = 0; i < 100; ++i) __nanosleep(1000);   // copies in flight land before the block ends
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMAs (leader)
+    if (rank == 0 && elect_one()) {
+      const uint32_t full = smem_u32(&bars->full[0]), empty = smem_u32(&bars->empty[0]);
+      const uint32_t sf_full = smem_u32(&bars->sf_full[0]), sf_empty = smem_u32(&bars->sf_empty[0]), sf_ring = smem_u32(ring_sf);
+      Walk<KIND> walk(p, *bars, tab);
+      Piece c;
+      uint32_t s = 0, ph = 0, sq = 0, sph = 0, n_piece = 0, n_stage = 0;
+      bool ok = true;
+      while (ok && walk.next(c)) {
+        const uint32_t idesc = make_idesc<T, KIND>(c.neff);
+        const uint32_t ab = nacc == 2 ? n_piece & 1 : 0, an = nacc == 2 ? n_piece >> 1 : n_piece;
+        const uint32_t acc = tmem + ab * p.NT;
+        ++n_piece;
+        if (!mbar_wait_spin(smem_u32(&bars->acc_empty[ab]), (an & 1) ^ 1, abort_flag)) break;
+        uint32_t first = 0;
+        for (int ks = c.ks0; ks < c.ks1; ++ks) {
+          const int in_chunk = kSf ? (ks - c.ks0) % kSpc<KIND> : 0;
+          if (kSf && in_chunk == 0 && !wait_cluster(sf_full + sq * 8, sph, abort_flag)) { ok = false; break; }
+          if (!wait_cluster(full + s * 8, ph, abort_flag)) { ok = false; break; }
+          tcgen05_fence_after();
+          const uint64_t da = sw128_desc(ring + s * stage_bytes, KIND == Kind::MK || kSum);
+          const uint64_t db = sw128_desc(ring + s * stage_bytes + kStageA, kSum);
+          if constexpr (kSf) {
+            constexpr int kWords = kSb / 4;
+            const uint32_t kb = p.sfb_chunk / 8;   // bytes per word of k of b's scales: 512 or 1024
+            const uint32_t ta = tmem_sf + (n_stage & 1) * 48, tb = ta + 16;
+            const uint32_t sa = sf_ring + sq * sf_bytes + in_chunk * kWords * 512, sb = sf_ring + sq * sf_bytes + 4096 + in_chunk * kWords * kb;
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) {
+              tcgen05_cp_scales(ta + 4 * w, scales_desc(sa + 512 * w));
+              tcgen05_cp_scales(tb + 8 * w, scales_desc(sb + kb * w));
+              if (c.neff > 128) tcgen05_cp_scales(tb + 8 * w + 4, scales_desc(sb + kb * w + 512));
+            }
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              const int w = KIND == Kind::Mx ? kk >> 1 : kk, id = KIND == Kind::Mx ? (kk & 1) * 2 : 0;
+              mma_fp4<KIND>(acc, da + 2 * kk, db + 2 * kk, idesc | (uint32_t)id << 29 | (uint32_t)id << 4, ta + 4 * w, tb + 8 * w, kk ? 1u : first);
+            }
+            if (in_chunk == kSpc<KIND> - 1 || ks + 1 == c.ks1) {
+              tcgen05_commit_pair(sf_empty + sq * 8);
+              if (++sq == kSfSlots) { sq = 0; sph ^= 1; }
+            }
+          } else {
+            const int a_step = KIND == Kind::KK ? 2 : 128, b_step = kSum ? 128 : 2;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) tcgen05_mma_ss(acc, da + a_step * kk, db + b_step * kk, idesc, kk ? 1u : first);
+          }
+          first = 1;
+          ++n_stage;
+          tcgen05_commit_pair(empty + s * 8);
+          if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; }
+        }
+        tcgen05_commit_pair(smem_u32(&bars->acc_full[ab]));
+      }
+    }
+  } else if (kSum && warp == 2) {
+    // ------------------------------------------------------------ rows of other groups are zeroed; the leader hears that a stage is there
+    const uint32_t landed = smem_u32(&bars->landed[0]), lfull = leader_addr(smem_u32(&bars->full[0]));
+    Walk<KIND> walk(p, *bars, tab);
+    Piece c;
+    uint32_t s = 0, ph = 0;
+    bool ok = true;
+    while (ok && walk.next(c)) {
+      const int blocks = 2 + (c.neff >> 7);   // of 64 columns: two of a, one or two of b
+      for (int ks = c.ks0; ks < c.ks1; ++ks) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_nap<20>(landed + s * 8, ph, abort_flag));
+        if (!ok) break;
+        const int valid = c.len - ks * 64;
+        if (valid < 64) {
+          const uint32_t a = ring + s * stage_bytes;
+          for (int h = 0; h < blocks; ++h)
+            for (uint32_t at = max(valid, 0) * 128 + lane * 16; at < 8192; at += 512)
+              asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(a + h * 8192 + at), "r"(0u) : "memory");
+          fence_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) arrive_release_cluster(lfull + s * 8);
+        if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; }
+      }
+    }
+  } else if (kSf && warp >= kScaleWarp0 && warp < kScaleWarp0 + kScaleWarps) {
+    // ------------------------------------------------------------ scales: warps take chunks in turn
+    const uint32_t sf_ring = smem_u32(ring_sf), lsf = leader_addr(smem_u32(&bars->sf_full[0])), sf_empty = smem_u32(&bars->sf_empty[0]);
+    const uint32_t kb = p.sfb_chunk / 8;
+    const int half = lane & 1, r0 = lane >> 1;   // a lane has 16 of a row's 32 bytes
+    Walk<KIND> walk(p, *bars, tab);
+    Piece c;
+    uint32_t chunk = 0;
+    bool ok = true;
+    while (ok && walk.next(c)) {
+      for (int ks = c.ks0; ks < c.ks1; ks += kSpc<KIND>, ++chunk) {
+        if ((chunk & (kScaleWarps - 1)) != (uint32_t)(warp - kScaleWarp0)) continue;
+        const int byte = ks * kSb + 16 * half, left = p.sf_row - byte;
+        uint4 va[kLanes / 16];
+#pragma unroll
+        for (int i = 0; i < kLanes / 16; ++i) {
+          const int n = c.i0 + rank * kLanes + r0 + 16 * i;
+          va[i] = make_uint4(0, 0, 0, 0);
+          if (n < p.I && left > 0) {
+            const uint8_t* at = p.sfa + ((long long)c.e * p.I + n) * p.sf_row + byte;
+            if (p.sfa16) va[i] = __ldg(reinterpret_cast<const uint4*>(at));
+            else va[i] = load16_any(at, at + min(left, 16));
+          }
+        }
+        const uint32_t sl = chunk % kSfSlots, at = sf_ring + sl * sf_bytes;
+        ok = __all_sync(0xFFFFFFFFu, mbar_nap<20>(sf_empty + sl * 8, ((chunk / kSfSlots) & 1) ^ 1, abort_flag));
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < kLanes / 16; ++i) store_scales(at, 512, r0 + 16 * i, half, va[i]);
+        // b: rows of the tile, of x's own scales (rows past the end of x: the last row's, for columns that nobody stores)
+#pragma unroll
+        for (int i0 = 0; i0 < kMaxNT / 16; i0 += 4) {
+          if (16 * i0 >= c.neff) break;
+          uint4 vb[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = min(c.row0 + r0 + 16 * (i0 + i), p.T - 1);
+            vb[i] = *reinterpret_cast<const uint4*>(p.sfb + (long long)r * p.sfb_pitch + byte);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * (i0 + i) < c.neff) store_scales(at + 4096, kb, r0 + 16 * (i0 + i), half, vb[i]);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) arrive_release_cluster(lsf + sl * 8);
+      }
+    }
+  } else if (warp >= kEpiWarp0) {
+    // ------------------------------------------------------------ epilogue
+    const int w = warp - kEpiWarp0, quad = warp & 3, chalf = w >> 2;
+    const uint32_t stg = smem_u32(staging) + w * kStageOut;
+    const uint32_t lane_field = (uint32_t)(quad * 32) << 16;
+    if (!kSum && bars->rows < p.T) {   // rows that belong to no group
+      T* z = static_cast<T*>(p.out) + (long long)bars->rows * p.I;
+      const long long n = (long long)(p.T - bars->rows) * p.I, step = (long long)gridDim.x * kEpiWarps * 32;
+      for (long long i = ((long long)blockIdx.x * kEpiWarps + w) * 32 + lane; i < n; i += step) z[i] = Elem<T>::from_float(0.0f);
+    }
+    Walk<KIND> walk(p, *bars, tab);
+    Piece c;
+    uint32_t n_piece = 0;
+    while (walk.next(c)) {
+      const uint32_t ab = nacc == 2 ? n_piece & 1 : 0, an = nacc == 2 ? n_piece >> 1 : n_piece;
+      // One warp looks and all go by what it found: the abort flag may be raised between two warps' looks.
+      if (w == 0) {
+        const bool seen = __all_sync(0xFFFFFFFFu, mbar_nap<50>(smem_u32(&bars->acc_full[ab]), an & 1, abort_flag));
+        if (lane == 0) bars->seen[n_piece & 1] = seen;
+        __syncwarp();
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+      if (!bars->seen[n_piece & 1]) break;
+      ++n_piece;
+      tcgen05_fence_after();
+      float alpha = 1.0f;
+      if constexpr (kSf) {
+        if (p.ga) alpha = __ldg(p.ga + (p.ga_each ? c.e : 0));
+        if (p.gb) alpha *= __ldg(p.gb);
+      }
+      const uint32_t acc = tmem + ab * p.NT + lane_field;
+      const int i_warp = c.i0 + rank * kLanes + quad * 32;
+      auto release = [&]() {
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(leader_addr(smem_u32(&bars->acc_empty[ab])));
+      };
+      // this warp's columns: half of them, in pieces of 32
+      const int pieces = (c.neff + 31) / 32, p0 = chalf ? (pieces + 1) / 2 : 0, p1 = chalf ? pieces : (pieces + 1) / 2;
+      if (c.parts > 1) {
+        const int slot = c.part == 0 ? 2 * c.j0 + 1 : 2 * (c.j0 + c.part);
+        float* part = p.partial + ((size_t)slot * 2 + rank) * ((size_t)p.NT * kLanes) + quad * 32 + lane;
+        for (int q = p0; q < p1; ++q) {
+          uint32_t v[32];
+          tcgen05_ld_x32(acc + 32 * q, v);
+          tcgen05_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (32 * q + j < c.rows) __stcg(part + (size_t)(32 * q + j) * kLanes, __uint_as_float(v[j]));
+        }
+        release();
+        __threadfence();
+        asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+        if (w == 0 && lane == 0) {
+          uint32_t* ctr = p.counters + c.j0 * 2 + rank;
+          const bool last = atomicAdd(ctr, 1u) == (uint32_t)c.parts - 1;
+          if (last) *ctr = 0;
+          bars->last = last;
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+        if (bars->last) {
+          __threadfence();
+          const size_t pitch = 2 * (size_t)p.NT * kLanes / 4;   // slot to slot
+          const float4* base = reinterpret_cast<const float4*>(p.partial + (size_t)rank * ((size_t)p.NT * kLanes)) + lane;
+          const int i = c.i0 + rank * kLanes + 4 * lane;
+          for (int r = w; r < c.rows; r += kEpiWarps) {
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int s = 0; s < c.parts; s += 4) {
+              float4 v[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int q = s + k;
+                if (q < c.parts) v[k] = __ldcg(base + (size_t)(q == 0 ? 2 * c.j0 + 1 : 2 * (c.j0 + q)) * pitch + (size_t)r * (kLanes / 4));
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (s + k < c.parts) { sum.x += v[k].x; sum.y += v[k].y; sum.z += v[k].z; sum.w += v[k].w; }
+            }
+            if (i < p.I)
+              store4(out_row<T, KIND>(p, c, r) + i, p.I - i, p.vec != 0, sum.x * alpha, sum.y * alpha, sum.z * alpha, sum.w * alpha);
+          }
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");   // `last` may be written again
+        continue;
+      }
+      if constexpr (sizeof(T) == 2) {
+        if (p.vec) {
+          for (int q = p0; q < p1; ++q) {
+            uint32_t r[2][16];
+            load_16(acc + 32 * q, r[0]);
+            const bool two = 32 * q + 16 < c.neff;
+            if (two) load_16(acc + 32 * q + 16, r[1]);
+            tcgen05_wait_ld16(r[0]);
+            if (two) tcgen05_wait_ld16(r[1]);
+            if (q + 1 == p1) release();
+  #pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (h == 1 && !two) break;
+              // 16 rows of 64 bytes, 16-byte chunks xor-ed with row / 2
+              const uint32_t row = lane & 7, at = stg + h * 1024 + row * 64 + ((((uint32_t)lane >> 3) ^ (row >> 1)) << 4);
+              auto f = [&](int k) { return __uint_as_float(r[h][k]) * alpha; };
+  #pragma unroll
+              for (int x = 0; x < 2; ++x)
+                stmatrix_x4_trans(at + x * 512, pack2<T>(f(4 * x), f(4 * x + 1)), pack2<T>(f(4 * x + 2), f(4 * x + 3)),
+                                  pack2<T>(f(8 + 4 * x), f(8 + 4 * x + 1)), pack2<T>(f(8 + 4 * x + 2), f(8 + 4 * x + 3)));
+            }
+            __syncwarp();
+            const int i = i_warp + (lane & 3) * 8;
+            if (i < p.I) {   // (whole chunks: rows on 16-byte boundaries are whole eights long)
+              for (int tok = lane >> 2; tok < min(32, c.rows - 32 * q); tok += 8) {
+                uint4 v;
+                lds128(stg + tok * 64 + (((lane & 3) ^ ((tok >> 1) & 3)) << 4), v);
+                *reinterpret_cast<uint4*>(out_row<T, KIND>(p, c, 32 * q + tok) + i) = v;
+              }
+            }
+            __syncwarp();
+          }
+          if (p0 == p1) release();
+          continue;
+        }
+      }
+      // f32, or rows of any alignment: a lane per i, the warp stores 64 (f32: 128) contiguous bytes per row
+      const int i = i_warp + lane;
+      for (int q = p0; q < p1; ++q) {
+        uint32_t v[32];
+        tcgen05_ld_x32(acc + 32 * q, v);
+        tcgen05_wait_ld();
+        if (q + 1 == p1) release();
+        if (i < p.I) {
+          T* y = out_row<T, KIND>(p, c, 32 * q) + i;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (32 * q + j < c.rows) y[(long long)j * p.I] = Elem<T>::from_float(__uint_as_float(v[j]) * alpha);
+        }
+        __syncwarp();
+      }
+      if (p0 == p1) release();
+    }
+  }
+
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) atomicMax(p.status, 8u);
+  __syncwarp();
+  cluster_sync();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tcgen05_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) == cudaSuccess &&
+                    qres == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<EncodeFn>(sym) : nullptr;
+  }();
+  return fn;
+}
+int sm_pairs() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 74;
+  if (!cached[dev]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 2) n = 148;
+    cached[dev] = n / 2;
+  }
+  return cached[dev];
+}
+
+// Rows of `cols` elements (bytes where esize is 1), `mid` of them per matrix; boxes of `box0` x `box1`.
+int encode(CUtensorMap* m, int dtype, int esize, const void* base, int64_t cols, int64_t pitch, int64_t mid, int64_t outer, int box0, int box1) {
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)mid, (cuuint64_t)outer};
+  const cuuint64_t strides[2] = {(cuuint64_t)pitch, (cuuint64_t)pitch * mid};
+  const cuuint32_t box[3] = {(cuuint32_t)box0, (cuuint32_t)box1, 1}, one[3] = {1, 1, 1};
+  const CUtensorMapDataType t = esize == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                : dtype == B200Q_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult r = encode_fn()(m, t, 3, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B200Q_OK : fail(B200Q_ERR_CUDA, "[grouped product] a tensor map could not be encoded (%d)", (int)r);
+}
+
+// Once per kernel, device and thread.
+int allow_smem(const void* kernel) {
+  constexpr int kMost = 16;   // instantiations: 12
+  static thread_local const void* done[64][kMost];
+  static thread_local int count[64];
+  int dev = 0;
+  B200Q_CUDA_OK(cudaGetDevice(&dev));
+  const bool known = dev >= 0 && dev < 64;
+  for (int i = 0; known && i < count[dev]; ++i)
+    if (done[dev][i] == kernel) return B200Q_OK;
+  B200Q_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax));
+  if (known && count[dev] < kMost) done[dev][count[dev]++] = kernel;
+  return B200Q_OK;
+}
+
+template <typename T, Kind KIND>
+int launch(const Maps& m, Params& p, cudaStream_t st) {
+  const size_t stage = kStageA + (size_t)p.NT * 64;
+  const size_t fixed = 1024 + (kFp4<KIND> ? kSfSlots * (4096 + (size_t)p.sfb_chunk) : 0) + (sizeof(T) == 2 ? kEpiWarps * kStageOut : 0) +
+                       sizeof(Bars) + (size_t)(p.E + 1) * 12;
+  p.stages = (int)((kSmemMax - fixed) / stage);
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  size_t smem = fixed + p.stages * stage;
+  // One block per SM: the allocation of all of tensor memory never waits for another block of this kernel.
+  if (smem < 120 * 1024) smem = 120 * 1024;
+  auto kernel = grouped_tc_kernel<T, KIND>;
+  if (int rc = allow_smem((const void*)kernel)) return rc;
+  kernel<<<2 * sm_pairs(), kThreads, smem, st>>>(m, p);
+  B200Q_LAUNCH_OK("grouped_tc_kernel");
+  return B200Q_OK;
+}
+
+template <Kind KIND>
+int launch_t(int dtype, const Maps& m, Params& p, cudaStream_t st) {
+  if (dtype == B200Q_BF16) return launch<__nv_bfloat16, KIND>(m, p, st);
+  if (dtype == B200Q_F16) return launch<__half, KIND>(m, p, st);
+  if constexpr (kFp4<KIND>) return launch<float, KIND>(m, p, st);
+  return fail(B200Q_ERR_UNSUPPORTED, "[grouped product] only bfloat16 and float16 are supported");
+}
+
+int tile_columns(int64_t rows) { return (int)(rows >= kMaxNT ? kMaxNT : (rows + 15) / 16 * 16); }
+constexpr size_t kCounterBytes = 2048;   // [pairs][2] words, 148 SMs and more
+
+}  // namespace
+
+// The product's own part of the workspace: counters, then partial sums.
+size_t grouped_tc_bytes(int64_t rows, bool sum) {
+  return kCounterBytes + 2 * (size_t)sm_pairs() * 2 * (size_t)(sum ? kMaxNT : tile_columns(rows)) * kLanes * 4;
+}
+
+int grouped_tc(const GroupedTcArgs& a, cudaStream_t st) {
+  if (!encode_fn()) return fail(B200Q_ERR_CUDA, "[grouped product] cuTensorMapEncodeTiled is not available");
+  if (int rc = bind_context()) return rc;
+  Maps m;
+  Params p{};
+  p.sizes = a.sizes; p.size_bytes = a.size_bytes;
+  p.E = (int)a.E; p.T = (int)a.T; p.I = (int)a.I; p.J = (int)a.J; p.K = (int)a.K;
+  p.i_tiles = (p.I + kTileI - 1) / kTileI;
+  const bool sum = a.form == GroupedForm::Sum, fp4 = a.form == GroupedForm::Mx || a.form == GroupedForm::Nv;
+  p.NT = sum ? (a.J > 128 ? 256 : 128) : tile_columns(a.T);
+  const int es = a.dtype == B200Q_F32 ? 4 : 2;
+  p.out = a.out;
+  p.vec = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.I * es)) & 15) == 0;
+  p.counters = static_cast<uint32_t*>(a.ws);
+  p.partial = reinterpret_cast<float*>(static_cast<char*>(a.ws) + kCounterBytes);
+  p.status = a.status;
+  p.sfb_chunk = p.NT > 128 ? 8192 : 4096;
+  p.sfa = a.sfa; p.sfb = a.sfb; p.sf_row = (int)a.sf_row; p.sfb_pitch = (int)a.sfb_pitch;
+  p.sfa16 = ((reinterpret_cast<uintptr_t>(a.sfa) | (uintptr_t)a.sf_row) & 15) == 0;
+  p.ga = a.ga; p.gb = a.gb; p.ga_each = a.ga_each;
+  // number of tiles and steps in 32 bits
+  const int64_t tiles = ((sum ? (a.J + p.NT - 1) / p.NT * a.E : a.T / p.NT + a.E + 1)) * p.i_tiles;
+  const int64_t steps = sum ? (a.T / 64 + 2 * a.E) * ((a.J + p.NT - 1) / p.NT) * p.i_tiles : tiles * ((a.K + 63) / 64);
+  if (tiles >= INT32_MAX || steps >= INT32_MAX)
+    return fail(B200Q_ERR_UNSUPPORTED, "[grouped product] No implementation for problem shape: too many tiles");
+  const int stage = 2 * p.NT > 700 ? 2 * p.NT : 700;
+  p.cut_gain = a.form == GroupedForm::Mx ? 4 * stage : (a.form == GroupedForm::Nv ? 2 * stage : stage);
+  p.cut_cost = 4000 + 16 * p.NT;
+
+  const int e_a = fp4 ? 1 : 2;
+  const int64_t ka = fp4 ? a.K / 2 : a.K;
+  int rc = B200Q_OK;
+  if (sum) {
+    rc = encode(&m.a, a.dtype, 2, a.a, a.I, a.a_pitch, a.T, 1, 64, 64);
+    if (!rc) rc = encode(&m.b[0], a.dtype, 2, a.b, a.J, a.b_pitch, a.T, 1, 64, 64);
+  } else {
+    const int box = fp4 ? 128 : 64;
+    if (a.form == GroupedForm::MK) rc = encode(&m.a, a.dtype, 2, a.a, a.I, a.a_pitch, a.K, a.E, 64, 64);
+    else rc = encode(&m.a, a.dtype, e_a, a.a, ka, a.a_pitch, a.I, a.E, box, kLanes);
+    for (int i = 0; i < 5 && !rc; ++i)
+      if ((128 >> i) <= p.NT / 2) rc = encode(&m.b[i], a.dtype, e_a, a.b, ka, a.b_pitch, a.T, 1, box, 128 >> i);
+  }
+  if (rc) return rc;
+  switch (a.form) {
+    case GroupedForm::KK: return launch_t<Kind::KK>(a.dtype, m, p, st);
+    case GroupedForm::MK: return launch_t<Kind::MK>(a.dtype, m, p, st);
+    case GroupedForm::Sum: return launch_t<Kind::MM>(a.dtype, m, p, st);
+    case GroupedForm::Mx: return launch_t<Kind::Mx>(a.dtype, m, p, st);
+    default: return launch_t<Kind::Nv>(a.dtype, m, p, st);
+  }
+}
+
+}  // namespace b200q

@@ -6,6 +6,8 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "../../include/b200q.h"
+
 namespace b200q {
 
 // Output replicated into the buffers of several GPUs (N-sharded linear with the all_gather
@@ -162,5 +164,40 @@ bool qmm_tc_supported(const QmmArgs& a);
 size_t qmm_tc_workspace_bytes(const QmmArgs& a);
 int qmm_tc(const QmmArgs& a, cudaStream_t st);
 int qmm_tc_grouped(const GroupedArgs& a, cudaStream_t st);
+
+// grouped_tc.cu : products over groups of rows with ragged sizes (forms: see there).  Bases and pitches of a and b are
+// multiples of 16 bytes; T, I, K >= 1 (Sum: T, I, J >= 1).
+enum class GroupedForm { KK, MK, Sum, Mx, Nv };
+struct GroupedTcArgs {
+  GroupedForm form;
+  const void* a;            // [E, I, K], MK: [E, K, I], Sum: [T, I]; rows a_pitch bytes apart
+  const void* b;            // [T, K], Sum: [T, J]
+  int64_t a_pitch, b_pitch;
+  const void* sizes;        // device, [E] of size_bytes each; null: one group of T rows
+  int size_bytes;
+  void* out;                // [T, I], Sum: [E, J, I]
+  int dtype;                // of out (and of 16-bit operands)
+  int64_t T, E, I, J, K;
+  const uint8_t *sfa, *sfb;         // 4 bits: scales, rows sf_row and sfb_pitch bytes apart (sfb: padded with zeros to whole 32s, 16-byte aligned)
+  int64_t sf_row, sfb_pitch;
+  const float *ga, *gb;             // global scales (null: 1); ga_each: one per group
+  int ga_each;
+  void* ws;                 // grouped_tc_bytes, zeroed once
+  uint32_t* status;
+};
+size_t grouped_tc_bytes(int64_t rows, bool sum);
+int grouped_tc(const GroupedTcArgs& a, cudaStream_t st);
+
+// fp4.cu : microscaled 4-bit floating point
+constexpr int fp4_group(int mode) { return mode == B200Q_MXFP4 ? 32 : 16; }
+int fp4_quantize(const void* w, int dtype, int64_t rows, int64_t K, int mode, const float* global, int64_t rows_per_global,
+                 uint32_t* wq, uint8_t* scales, cudaStream_t st);
+int fp4_dequantize(const uint32_t* wq, const uint8_t* scales, int mode, const float* global, int64_t rows_per_global, int dtype,
+                   int64_t rows, int64_t K, void* out, cudaStream_t st);
+// Activations for grouped_tc: rows of codes and of scales with pitches of their own, scales padded with zeros to sf_pitch.
+int fp4_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int mode, const float* global, uint8_t* codes,
+                      int64_t code_pitch, uint8_t* scales, int64_t sf_pitch, cudaStream_t st);
+// dst rows of dst_pitch bytes (a multiple of 16) from src rows of src_bytes, padded with zeros.
+int repack_rows(const void* src, int64_t src_bytes, void* dst, int64_t dst_pitch, int64_t rows, cudaStream_t st);
 
 }  // namespace b200q

@@ -124,3 +124,31 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: t
     lhs_indices, rhs_indices = torch.broadcast_tensors(lhs_indices.to(dev), rhs_indices.to(dev))
     return _GatherQmmFn.apply(x, w, scales, biases, lhs_indices.contiguous(), rhs_indices.contiguous(), transpose,
                               group_size, bits)
+
+
+class _GroupedMmFn(torch.autograd.Function):
+    """y[t] = w_e x[t] over the rows of every expert e: d x is the same product with the matrices the other way round,
+    d w_e the sum over e's rows of dy[t] x[t]^T (zeros for an expert without rows)."""
+
+    @staticmethod
+    def forward(ctx, x, w, sizes, transpose):
+        ctx.save_for_backward(x, w, sizes)
+        ctx.transpose = transpose
+        return ops.grouped_mm(x, w, sizes, transpose)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, sizes = ctx.saved_tensors
+        dy = dy.to(x.dtype)
+        dx = ops.grouped_mm(dy, w, sizes, not ctx.transpose) if ctx.needs_input_grad[0] else None
+        dw = ops.grouped_mm_dw(dy, x, sizes, ctx.transpose) if ctx.needs_input_grad[1] else None
+        return dx, dw, None, None
+
+
+def grouped_mm(x: torch.Tensor, w: torch.Tensor, sizes: torch.Tensor, transpose: bool = True) -> torch.Tensor:
+    """ops.grouped_mm with autograd support for x and w."""
+    y = ops._front.grouped_mm_grad(x, w, sizes, transpose)
+    if y is not None:
+        return y
+    return _GroupedMmFn.apply(x, w, sizes, bool(transpose))

@@ -1,9 +1,11 @@
-"""Host-side mirror of the reference operator front-end for the affine quantized path.
+"""Host-side mirror of the reference operator front-end for the quantized path.
 
 Same names, argument meaning and error behaviour as ``mlx.core.quantize``,
 ``dequantize``, ``quantized_matmul`` and ``gather_qmm`` (reference: mlx/ops.cpp:4784-4834
 quantized_matmul, :5208-5245 quantize, :5465-5517 dequantize, :5553-5629 gather_qmm;
-validation helpers :110-181, :4704-4754).  Arrays are ``torch`` CUDA tensors: torch only
+validation helpers :110-181, :4704-4754) in the affine mode.  ``quantize``, ``dequantize`` and ``qqmm`` have the
+microscaled 4-bit modes ``mxfp4`` and ``nvfp4`` too; ``grouped_mm`` and ``grouped_qqmm`` are products of rows that are
+already sorted by expert, with one size per expert.  Arrays are ``torch`` CUDA tensors: torch only
 supplies device memory and streams, every computation is a call into libb200q.so.
 Invalid arguments raise ``ValueError`` (the reference's std::invalid_argument).
 """
@@ -20,9 +22,10 @@ from . import _lib
 _lib.load()   # with its symbols present, and its message if it is not built
 from . import _front  # noqa: E402  (the native form of the ordinary calls: csrc/front.cpp)
 
-_SCRATCH_OPS = {"qmm": 0, "gather": 1}
+_SCRATCH_OPS = {"qmm": 0, "gather": 1, "grouped": 2}
 _DT = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _MODES = ("affine", "mxfp4", "mxfp8", "nvfp4")
+_FP4 = {"mxfp4": (_lib.MXFP4, 32), "nvfp4": (_lib.NVFP4, 16)}   # mode -> (its code, its group size)
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -52,9 +55,9 @@ def _as_u32(w: torch.Tensor, tag: str) -> torch.Tensor:
 class _Workspaces:
     """One zero-initialised scratch buffer per (device, stream, operator); it only grows.
 
-    quantized_matmul and gather_qmm keep separate buffers: the matmul kernels rely on
-    counters that start at zero and are left at zero, while gather_qmm uses its buffer as
-    plain scratch (sorted indices, tile table, gathered rows).
+    quantized_matmul, gather_qmm and the grouped products keep separate buffers: the matmul kernels rely on
+    counters that start at zero and are left at zero (those of the grouped products lie elsewhere than
+    quantized_matmul's), while gather_qmm uses its buffer as plain scratch (sorted indices, tile table, gathered rows).
 
     A buffer that has become too small is kept: a CUDA graph captured before goes on using it.
     Every new one is at least twice as large, so that the old ones never add up to more than it."""
@@ -92,6 +95,8 @@ _STATUS_TEXT = {
     5: "bounded wait expired in the TMA ring of the stream decode kernel",
     6: "bounded wait for a peer GPU's completion flag expired: the gathered output is incomplete",
     7: "bounded wait expired in the row-owning decode kernel",
+    8: "bounded wait expired in the grouped tensor-core kernel",
+    9: "a group size was negative, or the groups reach past the last row (they end there)",
 }
 
 
@@ -140,7 +145,8 @@ def _mode_params(mode: str, group_size, bits, tag: str) -> Tuple[int, int]:
     if mode not in _MODES:
         raise ValueError(f"[{tag}] Invalid quantization mode '{mode}'.")
     if mode != "affine":
-        raise NotImplementedError(f"[{tag}] only the affine mode is built; '{mode}' is out of scope")
+        raise NotImplementedError(f"[{tag}] only the affine mode is built; '{mode}' is out of scope"
+                                  + ("" if mode not in _FP4 else " (quantize, dequantize, qqmm and grouped_qqmm have it)"))
     return (64 if group_size is None else int(group_size), 4 if bits is None else int(bits))
 
 
@@ -199,8 +205,17 @@ def _extract_dims(tag, x, w, scales, biases, transpose, group_size, bits):
 
 # --------------------------------------------------------------------------- quantize
 def quantize(w: torch.Tensor, group_size: Optional[int] = None, bits: Optional[int] = None,
-             mode: str = "affine"):
-    """-> (w_q uint32 [..., K*bits/32], scales [..., K/g], biases [..., K/g]); mlx/ops.cpp:5208."""
+             mode: str = "affine", global_scale: Optional[torch.Tensor] = None):
+    """-> (w_q uint32 [..., K*bits/32], scales [..., K/g], biases [..., K/g]); mlx/ops.cpp:5208.
+
+    mode "mxfp4" (groups of 32) or "nvfp4" (groups of 16): -> (w_q uint32 [..., K/8], scales uint8 [..., K/g]), 4-bit
+    floating-point codes under a power of two or an E4M3 number per group; see b200q_fp4_quantize in include/b200q.h for
+    the rounding.  global_scale (nvfp4): what every scale is relative to, a float32 tensor with one element or one per
+    matrix of a stack; largest magnitude / (448 * 6) is the usual choice."""
+    if mode in _FP4:
+        return _fp4_quantize(w, group_size, bits, mode, global_scale)
+    if global_scale is not None:
+        raise ValueError(f"[quantize] a global scale belongs to the nvfp4 mode, not to '{mode}'.")
     q = _front.quantize(w, group_size, bits, mode)
     if q is not None:
         return q
@@ -243,8 +258,13 @@ def quantize(w: torch.Tensor, group_size: Optional[int] = None, bits: Optional[i
 
 def dequantize(w: torch.Tensor, scales: torch.Tensor, biases: Optional[torch.Tensor] = None,
                group_size: Optional[int] = None, bits: Optional[int] = None, mode: str = "affine",
-               dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """mlx/ops.cpp:5465-5517 (+ affine_dequantize :5258-5340)."""
+               dtype: Optional[torch.dtype] = None, global_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """mlx/ops.cpp:5465-5517 (+ affine_dequantize :5258-5340).  The microscaled modes have no biases; their values come
+    in `dtype`, bfloat16 if it is not given."""
+    if mode in _FP4:
+        return _fp4_dequantize(w, scales, biases, group_size, bits, mode, dtype, global_scale)
+    if global_scale is not None:
+        raise ValueError(f"[dequantize] a global scale belongs to the nvfp4 mode, not to '{mode}'.")
     if dtype is None or dtype == scales.dtype:
         out = _front.dequantize(w, scales, biases, group_size, bits, mode)
         if out is not None:
@@ -283,6 +303,100 @@ def dequantize(w: torch.Tensor, scales: torch.Tensor, biases: Optional[torch.Ten
                                           group_size, bits, _ptr(out), _stream(w))
     _lib.check(rc)
     return out if out.dtype == out_type else out.to(out_type)
+
+
+# ------------------------------------------------------------------- microscaled 4-bit modes
+def _fp4_params(tag, mode, group_size, bits):
+    if mode not in _MODES:
+        raise ValueError(f"[{tag}] Invalid quantization mode '{mode}'.")
+    if mode not in _FP4:
+        raise NotImplementedError(f"[{tag}] mode '{mode}' is not built; 'mxfp4' and 'nvfp4' are")
+    code, group = _FP4[mode]
+    if (group if group_size is None else group_size) != group or (4 if bits is None else bits) != 4:
+        raise ValueError(f"[{tag}] mode '{mode}' has 4 bits in groups of {group}, not {bits} in groups of {group_size}.")
+    return code, group
+
+
+def _fp4_global(tag, mode, g, counts, dev):
+    """A global scale as a contiguous float32 tensor on `dev`, or None; `counts`: how many elements it may have."""
+    if g is None:
+        return None
+    if mode != "nvfp4":
+        raise ValueError(f"[{tag}] a global scale belongs to the nvfp4 mode, not to '{mode}'.")
+    if not isinstance(g, torch.Tensor) or not g.dtype.is_floating_point or g.numel() not in counts:
+        raise ValueError(f"[{tag}] a global scale is a floating-point tensor of {' or '.join(str(c) for c in sorted(set(counts)))} element(s).")
+    if g.device != dev:
+        raise ValueError(f"[{tag}] all tensors must be on the same device")
+    return g.detach().to(torch.float32).contiguous()
+
+
+def _fp4_weights(tag, w, scales, group):
+    _as_u32(w, tag)
+    if scales.dtype != torch.uint8:
+        raise ValueError(f"[{tag}] The scales should be uint8 but received {scales.dtype}")
+    if w.ndim < 2 or scales.ndim != w.ndim or w.shape[:-1] != scales.shape[:-1] or w.shape[-1] * 8 != scales.shape[-1] * group:
+        raise ValueError(f"[{tag}] The shapes of the weight and scales are incompatible: w.shape() == {tuple(w.shape)} and "
+                         f"scales.shape() == {tuple(scales.shape)} with 4 bits in groups of {group}")
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and on a 16-byte boundary."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _matrices(shape) -> int:
+    return torch.Size(shape[:-2]).numel()
+
+
+def _fp4_quantize(w, group_size, bits, mode, global_scale):
+    q = _front.fp4_quantize(w, group_size, bits, mode, global_scale)
+    if q is not None:
+        return q
+    code, group = _fp4_params("quantize", mode, group_size, bits)
+    if w.dtype not in _DT:
+        raise ValueError(f"[quantize] Only real floating types can be quantized but w has type {w.dtype}.")
+    if w.ndim < 2:
+        raise ValueError(f"[quantize] The matrix to be quantized must have at least 2 dimension but it has only {w.ndim}.")
+    if w.shape[-1] % group != 0:
+        raise ValueError("[quantize] The last dimension of the matrix needs to be divisible by the quantization group "
+                         f"size {group}. However the provided matrix has shape {tuple(w.shape)}")
+    dev = _require_cuda("quantize", w)
+    n_mat = _matrices(w.shape)
+    g = _fp4_global("quantize", mode, global_scale, (1, max(n_mat, 1)), dev)
+    w = w.detach().contiguous()
+    K, rows, lead = w.shape[-1], torch.Size(w.shape[:-1]).numel(), tuple(w.shape[:-1])
+    with torch.cuda.device(dev):
+        wq = torch.empty(lead + (K // 8,), dtype=torch.uint32, device=dev)
+        scales = torch.empty(lead + (K // group,), dtype=torch.uint8, device=dev)
+        per = max(rows if g is None or g.numel() == 1 else w.shape[-2], 1)
+        rc = _lib.load().b200q_fp4_quantize(_ptr(w), _DT[w.dtype], rows, K, code, _ptr(g), per, _ptr(wq), _ptr(scales), _stream(w))
+    _lib.check(rc)
+    return wq, scales
+
+
+def _fp4_dequantize(w, scales, biases, group_size, bits, mode, dtype, global_scale):
+    if biases is None:
+        v = _front.fp4_dequantize(w, scales, group_size, bits, mode, _DT.get(torch.bfloat16 if dtype is None else dtype, -1), global_scale)
+        if v is not None:
+            return v
+    code, group = _fp4_params("dequantize", mode, group_size, bits)
+    if biases is not None:
+        raise ValueError(f"[dequantize] Biases must be null for quantization mode '{mode}'.")
+    dtype = torch.bfloat16 if dtype is None else dtype
+    if dtype not in _DT:
+        raise ValueError(f"[dequantize] Only real floating types are supported but output dtype == {dtype}.")
+    _fp4_weights("dequantize", w, scales, group)
+    dev = _require_cuda("dequantize", w, scales)
+    g = _fp4_global("dequantize", mode, global_scale, (1, max(_matrices(w.shape), 1)), dev)
+    w, scales = _aligned(w), scales.contiguous()
+    K, rows = w.shape[-1] * 8, torch.Size(w.shape[:-1]).numel()
+    with torch.cuda.device(dev):
+        out = torch.empty(tuple(w.shape[:-1]) + (K,), dtype=dtype, device=dev)
+        per = max(rows if g is None or g.numel() == 1 else w.shape[-2], 1)
+        rc = _lib.load().b200q_fp4_dequantize(_ptr(w), _ptr(scales), code, _ptr(g), per, _DT[dtype], rows, K, _ptr(out), _stream(w))
+    _lib.check(rc)
+    return out
 
 
 def quantized_embedding(ids: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
@@ -557,3 +671,134 @@ def gather_qmm_swiglu(x: torch.Tensor, gate, up, down, rhs_indices: torch.Tensor
                                          group_size, bits, _ptr(ws), ws.numel(), _stream(x))
     _lib.check(rc)
     return y
+
+
+# ------------------------------------------------------------------- microscaled products, products grouped by expert
+def _group_sizes(tag, sizes, E, dev):
+    if sizes.dtype.is_floating_point or sizes.dtype.is_complex or sizes.dtype == torch.bool:
+        raise ValueError(f"[{tag}] Group sizes must be integral but are {sizes.dtype}.")
+    if sizes.ndim != 1 or sizes.shape[0] != E:
+        raise ValueError(f"[{tag}] One group size per expert is needed: sizes.shape() == {tuple(sizes.shape)} with {E} experts.")
+    if sizes.device != dev:
+        raise ValueError(f"[{tag}] all tensors must be on the same device")
+    return (sizes if sizes.dtype in (torch.int32, torch.int64) else sizes.to(torch.int64)).contiguous()
+
+
+def _qqmm(tag, x, w, scales, sizes, group_size, bits, mode, gx, gw):
+    code, group = _fp4_params(tag, mode, group_size, bits)
+    if x.dtype not in _DT:
+        raise ValueError(f"[{tag}] Only real floating types are supported but x.dtype() == {x.dtype}.")
+    _fp4_weights(tag, w, scales, group)
+    if sizes is None and (w.ndim != 2 or x.ndim < 1):
+        raise ValueError(f"[{tag}] x must have at least one dimension and w two, but they have {x.ndim} and {w.ndim}.")
+    if sizes is not None and (w.ndim != 3 or x.ndim != 2):
+        raise ValueError(f"[{tag}] x must have two dimensions and w three, but they have {x.ndim} and {w.ndim}.")
+    E, N, K = (1 if w.ndim == 2 else w.shape[0]), w.shape[-2], w.shape[-1] * 8
+    if x.shape[-1] != K:
+        raise ValueError(f"[{tag}] Last dimension of first input with shape (..., {x.shape[-1]}) does not match the expanded "
+                         f"quantized matrix ({K}, {N}) computed from shape {tuple(w.shape)}")
+    dev = _require_cuda(tag, x, w, scales)
+    if sizes is not None:
+        sizes = _group_sizes(tag, sizes, E, dev)
+    gx, gw = _fp4_global(tag, mode, gx, (1,), dev), _fp4_global(tag, mode, gw, (1, max(E, 1)), dev)
+    x, w, scales = x.detach().contiguous(), _aligned(w), scales.contiguous()
+    T = torch.Size(x.shape[:-1]).numel()
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        y = torch.empty(tuple(x.shape[:-1]) + (N,), dtype=x.dtype, device=dev)
+        ws = _workspaces.get(dev, lib.b200q_grouped_qqmm_workspace_bytes(T, E, N, K, code), "grouped")
+        rc = lib.b200q_grouped_qqmm(_ptr(x), _ptr(w), _ptr(scales), _ptr(sizes), 0 if sizes is None else sizes.element_size(), _ptr(y),
+                                    _DT[x.dtype], T, E, N, K, code, _ptr(gx), _ptr(gw), int(gw is not None and gw.numel() > 1),
+                                    _ptr(ws), ws.numel(), _stream(x))
+    _lib.check(rc)
+    if _checked():
+        read_workspace_status(ws, torch.cuda.current_stream(dev).cuda_stream, "grouped")
+    return y
+
+
+def qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, group_size: Optional[int] = None, bits: Optional[int] = None,
+         mode: str = "nvfp4", global_scale_x: Optional[torch.Tensor] = None,
+         global_scale_w: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x [..., K] times the transpose of a quantized matrix (w uint32 [N, K/8], scales uint8 [N, K/g]), both in 4-bit
+    floating point: x is quantized on the way, as quantize(x, mode=mode, global_scale=global_scale_x) does, and the codes of
+    both go through the 4-bit tensor cores with their scales.  Sums in float32, the result [..., N] in x's type.
+    global_scale_w: what `w` was quantized with.  (QQMatmul of the reference, mlx/backend/cuda/quantized/qqmm.cpp.)"""
+    y = _front.qqmm(x, w, scales, None, group_size, bits, mode, global_scale_x, global_scale_w)
+    return y if y is not None else _qqmm("qqmm", x, w, scales, None, group_size, bits, mode, global_scale_x, global_scale_w)
+
+
+def grouped_qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, sizes: torch.Tensor, group_size: Optional[int] = None,
+                 bits: Optional[int] = None, mode: str = "nvfp4", global_scale_x: Optional[torch.Tensor] = None,
+                 global_scale_w: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """qqmm of rows sorted by expert: of x [T, K] the first sizes[0] rows multiply w[0] [N, K/8], the next sizes[1] rows w[1]
+    and so on.  sizes: integers on the device, never read by the host; rows past their sum give zeros.  global_scale_w: one
+    element, or one per expert."""
+    y = _front.qqmm(x, w, scales, sizes, group_size, bits, mode, global_scale_x, global_scale_w)
+    return y if y is not None else _qqmm("grouped_qqmm", x, w, scales, sizes, group_size, bits, mode, global_scale_x, global_scale_w)
+
+
+def _grouped_operands(tag, x, w, sizes, transpose):
+    if x.dtype not in (torch.float16, torch.bfloat16) or w.dtype != x.dtype:
+        raise ValueError(f"[{tag}] x and w must both be float16 or bfloat16 but are {x.dtype} and {w.dtype}.")
+    if x.ndim != 2 or w.ndim != 3:
+        raise ValueError(f"[{tag}] x must have two dimensions and w three, but they have {x.ndim} and {w.ndim}.")
+    E, N, K = w.shape[0], w.shape[1 if transpose else 2], w.shape[2 if transpose else 1]
+    if x.shape[1] != K:
+        raise ValueError(f"[{tag}] Last dimension of first input with shape {tuple(x.shape)} does not match the matrices "
+                         f"({K}, {N}) of w with shape {tuple(w.shape)} and transpose={transpose}")
+    dev = _require_cuda(tag, x, w)
+    return dev, _group_sizes(tag, sizes, E, dev), E, N, K
+
+
+def grouped_mm(x: torch.Tensor, w: torch.Tensor, sizes: torch.Tensor, transpose: bool = True) -> torch.Tensor:
+    """Rows sorted by expert through 16-bit weights: of x [T, K] the first sizes[0] rows multiply the transpose of w[0]
+    (w [E, N, K]; transpose=False: w[0] of w [E, K, N]), the next sizes[1] rows that of w[1] and so on; out [T, N].  sizes:
+    integers on the device, never read by the host; rows past their sum give zeros.  bfloat16 and float16, sums in float32.
+    grad.grouped_mm is the same with gradients."""
+    y = _front.grouped_mm(x, w, sizes, transpose)
+    if y is not None:
+        return y
+    transpose = bool(transpose)
+    dev, sizes, E, N, K = _grouped_operands("grouped_mm", x, w, sizes, transpose)
+    x, w = _aligned(x.detach()), _aligned(w.detach())
+    T = x.shape[0]
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        y = torch.empty((T, N), dtype=x.dtype, device=dev)
+        ws = _workspaces.get(dev, lib.b200q_grouped_mm_workspace_bytes(T, E, N, K, int(transpose)), "grouped")
+        rc = lib.b200q_grouped_mm(_ptr(x), _ptr(w), _ptr(sizes), sizes.element_size(), _ptr(y), _DT[x.dtype], T, E, N, K,
+                                  int(transpose), _ptr(ws), ws.numel(), _stream(x))
+    _lib.check(rc)
+    if _checked():
+        read_workspace_status(ws, torch.cuda.current_stream(dev).cuda_stream, "grouped")
+    return y
+
+
+def grouped_mm_dw(dy: torch.Tensor, x: torch.Tensor, sizes: torch.Tensor, transpose: bool = True) -> torch.Tensor:
+    """The gradient of grouped_mm with respect to w, in w's layout: for every expert the sum over its rows of dy[t]^T x[t]
+    ([E, N, K]; transpose=False: x[t]^T dy[t], [E, K, N]).  An expert without rows gets zeros."""
+    dw = _front.grouped_mm_dw(dy, x, sizes, transpose)
+    if dw is not None:
+        return dw
+    if x.dtype not in (torch.float16, torch.bfloat16) or dy.dtype != x.dtype:
+        raise ValueError(f"[grouped_mm_dw] dy and x must both be float16 or bfloat16 but are {dy.dtype} and {x.dtype}.")
+    if x.ndim != 2 or dy.ndim != 2 or x.shape[0] != dy.shape[0]:
+        raise ValueError(f"[grouped_mm_dw] dy and x must be matrices with as many rows, but have shapes {tuple(dy.shape)} and {tuple(x.shape)}.")
+    dev = _require_cuda("grouped_mm_dw", dy, x)
+    if sizes.ndim != 1:
+        raise ValueError(f"[grouped_mm_dw] sizes must have one dimension but has shape {tuple(sizes.shape)}.")
+    E, T = sizes.shape[0], x.shape[0]
+    sizes = _group_sizes("grouped_mm_dw", sizes, E, dev)
+    dy, x = _aligned(dy.detach()), _aligned(x.detach())
+    a, b = (dy, x) if transpose else (x, dy)
+    N, K = a.shape[1], b.shape[1]
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        dw = torch.empty((E, N, K), dtype=x.dtype, device=dev)
+        ws = _workspaces.get(dev, lib.b200q_grouped_mm_dw_workspace_bytes(T, N, K), "grouped")
+        rc = lib.b200q_grouped_mm_dw(_ptr(a), _ptr(b), _ptr(sizes), sizes.element_size(), _ptr(dw), _DT[x.dtype], T, E, N, K, _ptr(ws),
+                                     ws.numel(), _stream(x))
+    _lib.check(rc)
+    if _checked():
+        read_workspace_status(ws, torch.cuda.current_stream(dev).cuda_stream, "grouped")
+    return dw
