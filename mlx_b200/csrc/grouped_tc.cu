@@ -52,6 +52,7 @@ constexpr int kWarps = 16, kThreads = 32 * kWarps;
 constexpr int kScaleWarp0 = 4, kScaleWarps = 4, kEpiWarp0 = 8, kEpiWarps = 8;
 constexpr int kStageOut = 2048;      // epilogue staging per warp: 32 rows of 64 bytes
 constexpr int kSfColumns = 96;       // two buffers of 16 (a) + 32 (b) columns
+constexpr int kCutCycles = 3000;     // what a cut tile costs beside its sums: fences, the counter, latencies
 constexpr size_t kSmemMax = 227 * 1024;
 
 // k per stage, and stages per step: the unit in which K is cut (4 bits: what a chunk of scales covers)
@@ -81,7 +82,7 @@ struct Params {
   int ga_each;
   float* partial;          // [2 * pairs][block of the pair][NT][128]; null: no tile is cut
   uint32_t* counters;      // [pairs][block of the pair]
-  int cut_gain, cut_cost;  // cycles of a step, and what a cut tile costs beyond its steps
+  int step_cycles;         // estimate of a step's time
   uint32_t* status;
 };
 
@@ -439,9 +440,13 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
         while (h - e > 1) { const int m = (e + h) >> 1; if (tab.unit[m] <= full) e = m; else h = m; }
         base = tab.step[e] + (full - tab.unit[e]) * group_steps<KIND>(p, tab.row[e + 1] - tab.row[e]);
         rest = all_steps - base;
-        cut_pairs = min(pairs, rest);
-        // a whole wave takes as long as one tile, the cut one its share
-        if ((long long)rest * p.cut_gain / (total - full) - (long long)rest * p.cut_gain / cut_pairs <= p.cut_cost) cut_pairs = 0;
+        // A whole wave takes as long as a tile.  Cut in s parts, a tile takes its share, and whoever comes last reads s partial
+        // sums at about 64 bytes per clock: least at s = sqrt(tile / sum of one part).
+        const float n = (float)(total - full), tile = (float)rest / n * (float)p.step_cycles, part = 8.0f * (float)p.NT;
+        const float share = fminf((float)pairs, floorf(n * fmaxf(1.0f, sqrtf(tile / part))));
+        cut_pairs = min((int)share, rest);
+        const float cut = tile * n / (float)cut_pairs + (ceilf((float)cut_pairs / n) + 1.0f) * part + (float)kCutCycles;
+        if (cut_pairs < 2 || cut >= tile) cut_pairs = 0;
       }
       bars->full_units = cut_pairs ? full : total;
       bars->cut_pairs = cut_pairs;
@@ -700,21 +705,31 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
           const size_t pitch = 2 * (size_t)p.NT * kLanes / 4;   // slot to slot
           const float4* base = reinterpret_cast<const float4*>(p.partial + (size_t)rank * ((size_t)p.NT * kLanes)) + lane;
           const int i = c.i0 + rank * kLanes + 4 * lane;
-          for (int r = w; r < c.rows; r += kEpiWarps) {
-            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int s = 0; s < c.parts; s += 4) {
-              float4 v[4];
+          const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          // two rows and up to eight parts of each in flight
+          for (int r = w; r < c.rows; r += 2 * kEpiWarps) {
+            const int rows = r + kEpiWarps < c.rows ? 2 : 1;
+            const float4* at = base + (size_t)r * (kLanes / 4);
+            float4 sum[2] = {zero, zero};
+            for (int s = 0; s < c.parts; s += 8) {
+              float4 v[2][8];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int q = s + k;
-                if (q < c.parts) v[k] = __ldcg(base + (size_t)(q == 0 ? 2 * c.j0 + 1 : 2 * (c.j0 + q)) * pitch + (size_t)r * (kLanes / 4));
-              }
+              for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (s + k < c.parts) { sum.x += v[k].x; sum.y += v[k].y; sum.z += v[k].z; sum.w += v[k].w; }
+                for (int k = 0; k < 8; ++k) {
+                  const int q = s + k;
+                  v[h][k] = h < rows && q < c.parts
+                                ? __ldcg(at + h * (kEpiWarps * kLanes / 4) + (size_t)(q == 0 ? 2 * c.j0 + 1 : 2 * (c.j0 + q)) * pitch) : zero;
+                }
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) { sum[h].x += v[h][k].x; sum[h].y += v[h][k].y; sum[h].z += v[h][k].z; sum[h].w += v[h][k].w; }
             }
-            if (i < p.I)
-              store4(out_row<T, KIND>(p, c, r) + i, p.I - i, p.vec != 0, sum.x * alpha, sum.y * alpha, sum.z * alpha, sum.w * alpha);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (h < rows && i < p.I)
+                store4(out_row<T, KIND>(p, c, r + h * kEpiWarps) + i, p.I - i, p.vec != 0, sum[h].x * alpha, sum[h].y * alpha, sum[h].z * alpha, sum[h].w * alpha);
           }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");   // `last` may be written again
@@ -900,9 +915,8 @@ int grouped_tc(const GroupedTcArgs& a, cudaStream_t st) {
   const int64_t steps = sum ? (a.T / 64 + 2 * a.E) * ((a.J + p.NT - 1) / p.NT) * p.i_tiles : tiles * ((a.K + 63) / 64);
   if (tiles >= INT32_MAX || steps >= INT32_MAX)
     return fail(B200Q_ERR_UNSUPPORTED, "[grouped product] No implementation for problem shape: too many tiles");
-  const int stage = 2 * p.NT > 700 ? 2 * p.NT : 700;
-  p.cut_gain = a.form == GroupedForm::Mx ? 4 * stage : (a.form == GroupedForm::Nv ? 2 * stage : stage);
-  p.cut_cost = 4000 + 16 * p.NT;
+  // A stage: its MMAs (2 cycles per row), or 16 KB of weights at an SM's share of HBM.
+  p.step_cycles = (2 * p.NT > 700 ? 2 * p.NT : 700) * (a.form == GroupedForm::Mx ? kSpc<Kind::Mx> : (a.form == GroupedForm::Nv ? kSpc<Kind::Nv> : 1));
 
   const int e_a = fp4 ? 1 : 2;
   const int64_t ka = fp4 ? a.K / 2 : a.K;
