@@ -13,7 +13,8 @@
 //   warp 0      TMA: both operands of a stage (128 bytes of k per row; MM and MK: 64 k)
 //   warp 1      tcgen05.mma, and for 4 bits tcgen05.cp of the stage's scales (leader block, one thread)
 //   warp 2      MM only: the stage that a group ends in has its foreign rows zeroed in shared memory (both operands: a foreign
-//               infinity times zero would be NaN)
+//               infinity times zero would be NaN).  Only those stages go through this warp: with all of them handed on by it
+//               a step of the ring took 1600 cycles instead of 700
 //   warps 4-7   4 bits only: scales from global memory (row-major, any alignment) into the order that tensor memory wants
 //   warps 8-15  epilogue: accumulator -> rounding -> stmatrix staging -> 16-byte stores
 //
@@ -88,7 +89,7 @@ struct Params {
 
 struct __align__(8) Bars {
   uint64_t full[kMaxStages], empty[kMaxStages];
-  uint64_t landed[kMaxStages];                     // MM: this block's tiles are there, foreign rows and all
+  uint64_t landed[kMaxStages], fixed[kMaxStages];  // MM, a group's last stage: this block's tiles are there; and without foreign rows, in both
   uint64_t sf_full[kSfSlots], sf_empty[kSfSlots];
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem_base;
@@ -367,9 +368,9 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
 
   if (warp == 0) {
     if (lane < p.stages) {
-      mbar_init(smem_u32(&bars->full[lane]), kSum ? 2 : 1);
+      mbar_init(smem_u32(&bars->full[lane]), 1);
       mbar_init(smem_u32(&bars->empty[lane]), 1);
-      mbar_init(smem_u32(&bars->landed[lane]), 1);
+      if (kSum) { mbar_init(smem_u32(&bars->landed[lane]), 1); mbar_init(smem_u32(&bars->fixed[lane]), 2); }
     }
     if (lane < kSfSlots) { mbar_init(smem_u32(&bars->sf_full[lane]), 2); mbar_init(smem_u32(&bars->sf_empty[lane]), 1); }
     if (lane < 2) { mbar_init(smem_u32(&bars->acc_full[lane]), 1); mbar_init(smem_u32(&bars->acc_empty[lane]), 2 * kEpiWarps); }
@@ -476,15 +477,23 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
         const int half = c.neff >> 1;
         const uint32_t mine = kStageA + (uint32_t)half * 128u;
         for (int ks = c.ks0; ks < c.ks1; ++ks) {
-          if (!mbar_nap<20>(empty + s * 8, ph, abort_flag)) { ok = false; break; }
+          if (!mbar_wait_spin(empty + s * 8, ph, abort_flag)) { ok = false; break; }
           const uint32_t a = ring + s * stage_bytes, b = a + kStageA;
           if constexpr (kSum) {
-            const uint32_t bar = landed + s * 8;
             const int t = c.t0 + ks * 64;
-            mbar_expect_tx(bar, mine);
+            if (c.len - ks * 64 >= 64) {
+              const uint32_t bar = lfull + s * 8;
+              if (rank == 0) mbar_expect_tx(full + s * 8, 2 * mine);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) tma_3d(a + h * 8192, &maps.a, c.i0 + rank * kLanes + 64 * h, t, 0, bar);
-            for (int h = 0; h < half / 64; ++h) tma_3d(b + h * 8192, &maps.b[0], c.row0 + rank * half + 64 * h, t, 0, bar);
+              for (int h = 0; h < 2; ++h) tma_3d_pair(a + h * 8192, &maps.a, c.i0 + rank * kLanes + 64 * h, t, 0, bar);
+              for (int h = 0; h < half / 64; ++h) tma_3d_pair(b + h * 8192, &maps.b[0], c.row0 + rank * half + 64 * h, t, 0, bar);
+            } else {
+              const uint32_t bar = landed + s * 8;
+              mbar_expect_tx(bar, mine);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) tma_3d(a + h * 8192, &maps.a, c.i0 + rank * kLanes + 64 * h, t, 0, bar);
+              for (int h = 0; h < half / 64; ++h) tma_3d(b + h * 8192, &maps.b[0], c.row0 + rank * half + 64 * h, t, 0, bar);
+            }
           } else {
             const uint32_t bar = lfull + s * 8;
             const int k = ks * (kSf ? 128 : 64);
@@ -518,7 +527,9 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       const uint32_t sf_full = smem_u32(&bars->sf_full[0]), sf_empty = smem_u32(&bars->sf_empty[0]), sf_ring = smem_u32(ring_sf);
       Walk<KIND> walk(p, *bars, tab);
       Piece c;
-      uint32_t s = 0, ph = 0, sq = 0, sph = 0, n_piece = 0, n_stage = 0;
+      const uint32_t fixed = smem_u32(&bars->fixed[0]);
+      // A bit per slot: the phase that its barriers `full` and `fixed` are in (MM uses one or the other)
+      uint32_t s = 0, full_ph = 0, fixed_ph = 0, sq = 0, sph = 0, n_piece = 0, n_stage = 0;
       bool ok = true;
       while (ok && walk.next(c)) {
         const uint32_t idesc = make_idesc<T, KIND>(c.neff);
@@ -530,7 +541,9 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
         for (int ks = c.ks0; ks < c.ks1; ++ks) {
           const int in_chunk = kSf ? (ks - c.ks0) % kSpc<KIND> : 0;
           if (kSf && in_chunk == 0 && !wait_cluster(sf_full + sq * 8, sph, abort_flag)) { ok = false; break; }
-          if (!wait_cluster(full + s * 8, ph, abort_flag)) { ok = false; break; }
+          const bool ends = kSum && c.len - ks * 64 < 64;
+          if (!wait_cluster((ends ? fixed : full) + s * 8, ((ends ? fixed_ph : full_ph) >> s) & 1, abort_flag)) { ok = false; break; }
+          if (ends) fixed_ph ^= 1u << s; else full_ph ^= 1u << s;
           tcgen05_fence_after();
           const uint64_t da = sw128_desc(ring + s * stage_bytes, KIND == Kind::MK || kSum);
           const uint64_t db = sw128_desc(ring + s * stage_bytes + kStageA, kSum);
@@ -562,35 +575,32 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
           first = 1;
           ++n_stage;
           tcgen05_commit_pair(empty + s * 8);
-          if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; }
+          if (++s == (uint32_t)p.stages) s = 0;
         }
         tcgen05_commit_pair(smem_u32(&bars->acc_full[ab]));
       }
     }
   } else if (kSum && warp == 2) {
-    // ------------------------------------------------------------ rows of other groups are zeroed; the leader hears that a stage is there
-    const uint32_t landed = smem_u32(&bars->landed[0]), lfull = leader_addr(smem_u32(&bars->full[0]));
+    // ------------------------------------------------------------ rows of other groups are zeroed
+    const uint32_t landed = smem_u32(&bars->landed[0]), lfixed = leader_addr(smem_u32(&bars->fixed[0]));
     Walk<KIND> walk(p, *bars, tab);
     Piece c;
-    uint32_t s = 0, ph = 0;
-    bool ok = true;
-    while (ok && walk.next(c)) {
+    uint32_t at = 0, ph = 0;   // stages so far; a bit per slot
+    while (walk.next(c)) {
+      at += c.ks1 - c.ks0;
+      const int valid = c.len - (c.ks1 - 1) * 64;
+      if (valid >= 64) continue;
+      const uint32_t s = (at - 1) % (uint32_t)p.stages;
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait_spin(landed + s * 8, (ph >> s) & 1, abort_flag))) break;
+      ph ^= 1u << s;
       const int blocks = 2 + (c.neff >> 7);   // of 64 columns: two of a, one or two of b
-      for (int ks = c.ks0; ks < c.ks1; ++ks) {
-        ok = __all_sync(0xFFFFFFFFu, mbar_nap<20>(landed + s * 8, ph, abort_flag));
-        if (!ok) break;
-        const int valid = c.len - ks * 64;
-        if (valid < 64) {
-          const uint32_t a = ring + s * stage_bytes;
-          for (int h = 0; h < blocks; ++h)
-            for (uint32_t at = max(valid, 0) * 128 + lane * 16; at < 8192; at += 512)
-              asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(a + h * 8192 + at), "r"(0u) : "memory");
-          fence_async_smem();
-        }
-        __syncwarp();
-        if (lane == 0) arrive_release_cluster(lfull + s * 8);
-        if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; }
-      }
+      const uint32_t tile = ring + s * stage_bytes;
+      for (int h = 0; h < blocks; ++h)
+        for (uint32_t o = max(valid, 0) * 128 + lane * 16; o < 8192; o += 512)
+          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(tile + h * 8192 + o), "r"(0u) : "memory");
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) arrive_release_cluster(lfixed + s * 8);
     }
   } else if (kSf && warp >= kScaleWarp0 && warp < kScaleWarp0 + kScaleWarps) {
     // ------------------------------------------------------------ scales: warps take chunks in turn
@@ -617,7 +627,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
           }
         }
         const uint32_t sl = chunk % kSfSlots, at = sf_ring + sl * sf_bytes;
-        ok = __all_sync(0xFFFFFFFFu, mbar_nap<20>(sf_empty + sl * 8, ((chunk / kSfSlots) & 1) ^ 1, abort_flag));
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_spin(sf_empty + sl * 8, ((chunk / kSfSlots) & 1) ^ 1, abort_flag));
         if (!ok) break;
 #pragma unroll
         for (int i = 0; i < kLanes / 16; ++i) store_scales(at, 512, r0 + 16 * i, half, va[i]);
@@ -657,7 +667,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       const uint32_t ab = nacc == 2 ? n_piece & 1 : 0, an = nacc == 2 ? n_piece >> 1 : n_piece;
       // One warp looks and all go by what it found: the abort flag may be raised between two warps' looks.
       if (w == 0) {
-        const bool seen = __all_sync(0xFFFFFFFFu, mbar_nap<50>(smem_u32(&bars->acc_full[ab]), an & 1, abort_flag));
+        const bool seen = __all_sync(0xFFFFFFFFu, mbar_wait_spin(smem_u32(&bars->acc_full[ab]), an & 1, abort_flag));
         if (lane == 0) bars->seen[n_piece & 1] = seen;
         __syncwarp();
       }
