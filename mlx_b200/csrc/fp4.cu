@@ -129,11 +129,12 @@ fp4_quantize_kernel(const T* __restrict__ w, int64_t units, const float* __restr
   else if ((u & 1) == 0) scales[u >> 1] = (uint8_t)s;
 }
 
-// Activations: a block has up to kQuantThreads units of one row.
+// Activations: a block has up to kQuantThreads units of one row; four scales become one word of scales[word][row].
 template <typename T, bool MX, bool ALIGNED>
 __global__ void __launch_bounds__(kQuantThreads)
-fp4_quantize_rows_kernel(const T* __restrict__ x, int64_t K, int blocks_per_row, const float* __restrict__ global,
-                         uint8_t* __restrict__ codes_out, int64_t code_pitch, uint8_t* __restrict__ scales, int64_t sf_pitch) {
+fp4_quantize_rows_kernel(const T* __restrict__ x, int64_t K, int64_t rows, int blocks_per_row, const float* __restrict__ global,
+                         uint8_t* __restrict__ codes_out, int64_t code_pitch, uint32_t* __restrict__ scales, int64_t words) {
+  asm volatile("griddepcontrol.launch_dependents;");   // the product may set itself up; it waits for this grid before it reads
   const int64_t row = blockIdx.x / blocks_per_row;
   const int64_t u = (int64_t)(blockIdx.x - row * blocks_per_row) * kQuantThreads + threadIdx.x, k = u * kUnit;
   const bool in = k < K;
@@ -143,10 +144,14 @@ fp4_quantize_rows_kernel(const T* __restrict__ x, int64_t K, int blocks_per_row,
     for (int i = 0; i < kUnit; ++i) v[i] = 0.0f;
   const float G = !MX && global ? __ldg(global) : 1.0f;
   uint32_t codes[2];
-  const uint32_t s = quantize_unit<MX>(v, G, codes);
+  uint32_t s = quantize_unit<MX>(v, G, codes);
   if (in) *reinterpret_cast<uint2*>(codes_out + row * code_pitch + k / 2) = make_uint2(codes[0], codes[1]);
-  const int64_t at = MX ? u >> 1 : u;
-  if (at < sf_pitch && (!MX || (u & 1) == 0)) scales[row * sf_pitch + at] = in ? (uint8_t)s : (uint8_t)0;
+  else s = 0;
+  constexpr int kLanes = MX ? 8 : 4;   // that share a word
+  if (MX) s |= __shfl_down_sync(0xFFFFFFFFu, s, 2) << 8;
+  else s |= __shfl_down_sync(0xFFFFFFFFu, s, 1) << 8;
+  s |= __shfl_down_sync(0xFFFFFFFFu, s, kLanes / 2) << 16;
+  if (threadIdx.x % kLanes == 0 && u / kLanes < words) scales[(u / kLanes) * rows + row] = s;
 }
 
 template <typename T, bool MX, bool ALIGNED>
@@ -248,14 +253,14 @@ int fp4_dequantize(const uint32_t* wq, const uint8_t* scales, int mode, const fl
 }
 
 int fp4_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int mode, const float* global, uint8_t* codes,
-                      int64_t code_pitch, uint8_t* scales, int64_t sf_pitch, cudaStream_t st) {
-  const int64_t units = sf_pitch * (mode == B200Q_MXFP4 ? 2 : 1), bpr = (units + kQuantThreads - 1) / kQuantThreads;
+                      int64_t code_pitch, uint32_t* scales, int64_t words, cudaStream_t st) {
+  const int64_t units = words * (mode == B200Q_MXFP4 ? 8 : 4), bpr = (units + kQuantThreads - 1) / kQuantThreads;
   if (rows * bpr > kMostBlocks) return fail(B200Q_ERR_UNSUPPORTED, "[qqmm] No implementation for problem shape: too many values");
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     return with_flags(mode, aligned16(x), [&](auto mx, auto al) {
       fp4_quantize_rows_kernel<T, decltype(mx)::value, decltype(al)::value><<<(unsigned)(rows * bpr), kQuantThreads, 0, st>>>(
-          static_cast<const T*>(x), K, (int)bpr, global, codes, code_pitch, scales, sf_pitch);
+          static_cast<const T*>(x), K, rows, (int)bpr, global, codes, code_pitch, scales, words);
       B200Q_LAUNCH_OK("fp4_quantize_rows_kernel");
       return B200Q_OK;
     });

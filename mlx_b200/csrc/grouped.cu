@@ -5,7 +5,7 @@
 namespace b200q {
 namespace {
 
-constexpr int64_t kMostGroups = 4096;   // the table of groups is in shared memory (12 bytes each)
+constexpr int64_t kMostGroups = 4096;   // the table of groups is in shared memory (16 bytes each)
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
@@ -61,10 +61,11 @@ int check_ws(const char* tag, const void* ws, size_t have, size_t need) {
 }
 uint32_t* status_word(void* ws, size_t bytes) { return reinterpret_cast<uint32_t*>(static_cast<char*>(ws) + bytes - kStatusBytes); }
 
-int64_t sf_pitch(int64_t K, int mode) { return (K / fp4_group(mode) + 31) / 32 * 32; }
+// Words of four scales per row of x, a multiple of 8.
+int64_t sf_words(int64_t K, int mode) { return (K / fp4_group(mode) + 31) / 32 * 8; }
 
 size_t qqmm_bytes(int64_t T, int64_t E, int64_t N, int64_t K, int mode) {
-  return up(grouped_tc_bytes(T, false)) + up((size_t)T * up16(K / 2)) + up((size_t)T * sf_pitch(K, mode)) + packed_bytes(E * N, K / 2) + kStatusBytes;
+  return up(grouped_tc_bytes(T, false)) + up((size_t)T * up16(K / 2)) + up((size_t)T * sf_words(K, mode) * 4) + packed_bytes(E * N, K / 2) + kStatusBytes;
 }
 size_t grouped_bytes(int64_t T, int64_t E, int64_t N, int64_t K, bool transpose) {
   return up(grouped_tc_bytes(T, false)) + packed_bytes(T, 2 * K) + (transpose ? packed_bytes(E * N, 2 * K) : packed_bytes(E * K, 2 * N)) + kStatusBytes;
@@ -136,11 +137,11 @@ extern "C" int b200q_grouped_qqmm(const void* x, const uint32_t* wq, const uint8
   char* at = static_cast<char*>(ws) + up(grouped_tc_bytes(T, false));
   uint8_t* codes = reinterpret_cast<uint8_t*>(at);
   at += up((size_t)T * up16(K / 2));
-  uint8_t* sfx = reinterpret_cast<uint8_t*>(at);
-  at += up((size_t)T * sf_pitch(K, mode));
+  uint32_t* sfx = reinterpret_cast<uint32_t*>(at);
+  at += up((size_t)T * sf_words(K, mode) * 4);
   Operand w;
   if (int rc = pack(wq, E * N, K / 2, at, &w, st)) return rc;
-  if (int rc = fp4_quantize_rows(x, dtype, T, K, mode, global_scale_x, codes, up16(K / 2), sfx, sf_pitch(K, mode), st)) return rc;
+  if (int rc = fp4_quantize_rows(x, dtype, T, K, mode, global_scale_x, codes, up16(K / 2), sfx, sf_words(K, mode), st)) return rc;
   GroupedTcArgs a{};
   a.form = mode == B200Q_MXFP4 ? GroupedForm::Mx : GroupedForm::Nv;
   a.a = w.at; a.a_pitch = w.pitch;
@@ -149,7 +150,7 @@ extern "C" int b200q_grouped_qqmm(const void* x, const uint32_t* wq, const uint8
   a.out = y; a.dtype = dtype;
   a.T = T; a.E = E; a.I = N; a.K = K;
   a.sfa = scales; a.sf_row = K / fp4_group(mode);
-  a.sfb = sfx; a.sfb_pitch = sf_pitch(K, mode);
+  a.sfb = sfx;
   a.ga = global_scale_w; a.gb = global_scale_x; a.ga_each = scale_per_group;
   a.ws = ws; a.status = status_word(ws, ws_bytes);
   return grouped_tc(a, st);

@@ -15,8 +15,9 @@
 //   warp 2      MM only: the stage that a group ends in has its foreign rows zeroed in shared memory (both operands: a foreign
 //               infinity times zero would be NaN).  Only those stages go through this warp: with all of them handed on by it
 //               a step of the ring took 1600 cycles instead of 700
-//   warps 4-7   4 bits only: scales from global memory (row-major, any alignment) into the order that tensor memory wants
-//   warps 8-15  epilogue: accumulator -> rounding -> stmatrix staging -> 16-byte stores
+//   warps 4-11  epilogue: accumulator -> rounding -> stmatrix staging -> 16-byte stores
+//   warps 12-15 4 bits only: scales from global memory (row-major, a's at any alignment) into the order that tensor memory
+//               wants, word by word with cp.async, two warps for each operand
 //
 // The table of groups (first row, first tile, first step) is built in shared memory by every block from `sizes`, which the
 // host never reads: no launch in front and no synchronisation.
@@ -49,11 +50,12 @@ constexpr int kMaxNT = 256;
 constexpr int kStageA = kLanes * 128;
 constexpr int kMaxStages = 12;
 constexpr int kSfSlots = 4;          // chunks of scales: 32 bytes per row each
-constexpr int kWarps = 16, kThreads = 32 * kWarps;
-constexpr int kScaleWarp0 = 4, kScaleWarps = 4, kEpiWarp0 = 8, kEpiWarps = 8;
+constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
+constexpr int kScaleWarp0 = 12, kScaleWarps = 2;   // of each operand's scales
+constexpr int kMaxWarps = kScaleWarp0 + 2 * kScaleWarps;
+template <Kind K> constexpr int kThreads = 32 * (kFp4<K> ? kScaleWarp0 + 2 * kScaleWarps : kScaleWarp0);
 constexpr int kStageOut = 2048;      // epilogue staging per warp: 32 rows of 64 bytes
 constexpr int kSfColumns = 96;       // two buffers of 16 (a) + 32 (b) columns
-constexpr int kCutCycles = 3000;     // what a cut tile costs beside its sums: fences, the counter, latencies
 constexpr size_t kSmemMax = 227 * 1024;
 
 // k per stage, and stages per step: the unit in which K is cut (4 bits: what a chunk of scales covers)
@@ -74,20 +76,35 @@ struct Params {
   int sfb_chunk;           // 4 bits: bytes of a chunk of b's scales
   void* out;
   int vec;                 // rows of the output start on 16-byte boundaries
-  const uint8_t* sfa;      // scales [E * I, sf_row] and [T, sfb_pitch]
-  const uint8_t* sfb;
-  int sf_row, sfb_pitch;
-  int sfa16;               // rows of sfa on 16-byte boundaries
+  const uint8_t* sfa;      // scales [E * I, sf_row], and words of four of them [.., T]
+  const uint32_t* sfb;
+  int sf_row;
+  int sfa4;                // rows of sfa on 4-byte boundaries
   const float* ga;         // global scales: one, or (ga_each) one per group
   const float* gb;
   int ga_each;
   float* partial;          // [2 * pairs][block of the pair][NT][128]; null: no tile is cut
   uint32_t* counters;      // [pairs][block of the pair]
-  int step_cycles;         // estimate of a step's time
   uint32_t* status;
 };
 
-struct __align__(8) Bars {
+struct Piece {
+  int e, i0;          // group; first i of the pair
+  int row0, rows;     // first output row (MM: row of b's columns) and how many are valid
+  int neff;           // the same, rounded up to what the MMA takes
+  int t0, len;        // first row of the group and their number
+  int ks0, ks1;       // stages
+  int parts, part, j0;   // of a cut tile: number of parts, this one's number, first part's pair
+};
+
+// A warp's way through its pair's pieces.
+struct __align__(16) Walk {
+  Piece c;        // where it is
+  int u;          // next whole tile
+  int pos, end;   // next step of the pair's range, and its end
+};
+
+struct __align__(16) Bars {
   uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t landed[kMaxStages], fixed[kMaxStages];  // MM, a group's last stage: this block's tiles are there; and without foreign rows, in both
   uint64_t sf_full[kSfSlots], sf_empty[kSfSlots];
@@ -98,115 +115,114 @@ struct __align__(8) Bars {
   int full_units, cut_pairs, cut_steps;   // tiles in whole waves; pairs and steps of the rest
   int cut_base;                           // step at which the rest begins
   int rows;                               // rows that belong to a group
+  Walk walk[kMaxWarps];
 };
 
-// The table of groups: entry e is where group e begins.
-struct Table {
-  int* row;
-  int* unit;
-  int* step;
-};
+// Entry e of the table of groups: first row, first tile and first step of group e; number of tiles of its rows and rows per
+// tile (nj << 9 | tr).  The last entry is where everything ends.
+using Group = int4;
 
-struct Piece {
-  int e, i0;          // group; first i of the pair
-  int row0, rows;     // first output row (MM: row of b's columns) and how many are valid
-  int neff;           // the same, rounded up to what the MMA takes
-  int t0, len;        // MM: first row of the group and their number
-  int ks0, ks1;       // stages
-  int parts, part, j0;   // of a cut tile: number of parts, this one's number, first part's pair
-};
-
+template <Kind KIND>
+__device__ __forceinline__ int group_stages(const Params& p, int len) {
+  return KIND == Kind::MM ? max(1, (len + kStageK<KIND> - 1) / kStageK<KIND>) : (p.K + kStageK<KIND> - 1) / kStageK<KIND>;
+}
 template <Kind KIND>
 __device__ __forceinline__ int group_steps(const Params& p, int len) {
-  const int st = KIND == Kind::MM ? max(1, (len + kStageK<KIND> - 1) / kStageK<KIND>) : (p.K + kStageK<KIND> - 1) / kStageK<KIND>;
-  return (st + kSpc<KIND> - 1) / kSpc<KIND>;
+  return (group_stages<KIND>(p, len) + kSpc<KIND> - 1) / kSpc<KIND>;
 }
-// Rows per tile of a group: as even as multiples of 16 allow.
-__device__ __forceinline__ int tile_rows(int len, int nt) {
-  const int n = (len + nt - 1) / nt;
-  return n == 0 ? nt : ((len + n - 1) / n + 15) & ~15;
-}
+// Rows per tile of a group, as even as multiples of 16 allow, and the number of tiles.
 template <Kind KIND>
-__device__ __forceinline__ int tiles_j(const Params& p, int len) {
-  if (KIND == Kind::MM) return (p.J + p.NT - 1) / p.NT;
-  const int tr = tile_rows(len, p.NT);
-  return (len + tr - 1) / tr;
+__device__ __forceinline__ int2 tiles_j(const Params& p, int len) {
+  if (KIND == Kind::MM) return make_int2(p.NT, (p.J + p.NT - 1) / p.NT);
+  if (len <= p.NT) return make_int2((len + 15) & ~15, len > 0);
+  const int n = (int)((uint32_t)(len + p.NT - 1) / (uint32_t)p.NT), tr = ((int)((uint32_t)(len + n - 1) / (uint32_t)n) + 15) & ~15;
+  return make_int2(tr, (int)((uint32_t)(len + tr - 1) / (uint32_t)tr));
 }
 
-// Walks over a pair's pieces; every role has one.
+// Number of pairs that the n tiles (`rest` steps, `rows` rows each on average) left over from whole waves are cut for; 0: not
+// cut.  In cycles: a stage of n busy pairs takes its MMAs, its 16 KB of weights at their share of HBM, or at least 300; a cut
+// tile costs its writes (36 a row), the last arriver's reads (20 a row and part) and 4000 of fences and latencies.
 template <Kind KIND>
-struct Walk {
-  const Params& p;
-  const Bars& b;
-  const Table& tab;
-  int pair, pairs;
-  int u;             // next whole tile
-  int pos, end;      // next step of the pair's range, and its end
-  __device__ Walk(const Params& p_, const Bars& b_, const Table& t_) : p(p_), b(b_), tab(t_), pair(blockIdx.x >> 1), pairs(gridDim.x >> 1) {
-    u = pair;
-    pos = end = 0;
-    if (pair < b.cut_pairs) {
-      pos = b.cut_base + (int)((long long)b.cut_steps * pair / b.cut_pairs);
-      end = b.cut_base + (int)((long long)b.cut_steps * (pair + 1) / b.cut_pairs);
-    }
+__device__ __forceinline__ int cut_for(const Params& p, int n, int rest, int rows, int pairs) {
+  if ((long long)rest * (pairs + 1) >= INT32_MAX) return 0;
+  const float r = (float)max(rows, 16), tile = (float)(rest * kSpc<KIND>) / (float)n;   // stages
+  auto stage = [&](float busy) { return fmaxf(fmaxf(2.0f * r, 700.0f * busy / (float)pairs), 300.0f); };
+  const float whole = tile * stage((float)n);
+  float best = whole;
+  int cut = 0;
+#pragma unroll 1
+  for (int s = 2; s <= 8; ++s) {
+    const int busy = min(min(n * s, pairs), rest);
+    const float t = tile * (float)n / (float)busy * stage((float)busy) + r * (36.0f + 20.0f * ((float)busy / (float)n + (n * s > pairs ? 1.0f : 0.0f))) + 4000.0f;
+    if (t < best) { best = t; cut = busy; }
+    if (n * s >= pairs) break;
   }
-  __device__ __forceinline__ int find(const int* first, int v) const {   // the last group that begins at or before v (and is not empty)
-    int lo = 0, hi = p.E;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (first[mid] <= v) lo = mid; else hi = mid;
-    }
-    return lo;
+  return cut;
+}
+
+__device__ __forceinline__ void walk_begin(const Bars& b, Walk& w) {
+  const uint32_t pair = blockIdx.x >> 1;
+  w.u = (int)pair;
+  w.pos = w.end = 0;
+  if ((int)pair < b.cut_pairs) {   // (cut_steps * pairs stays below 2^31)
+    w.pos = b.cut_base + (int)((uint32_t)b.cut_steps * pair / (uint32_t)b.cut_pairs);
+    w.end = b.cut_base + (int)((uint32_t)b.cut_steps * (pair + 1) / (uint32_t)b.cut_pairs);
   }
-  __device__ __forceinline__ int owner(int at) const {   // pair whose range holds step `at`
-    return (int)((((long long)(at - b.cut_base) + 1) * b.cut_pairs - 1) / b.cut_steps);
+}
+// One thread: the next piece; false: there is none.  Out of line and through shared memory, so that all roles share its
+// instructions and none has a stack: with a copy in each role five of them had to come from memory before the first load
+// could start, and what is left of L1 beside the rings keeps no stack.
+template <Kind KIND>
+__device__ __noinline__ bool walk_next(const Params& p, const Bars& b, const Group* tab, Walk& w) {
+  const bool whole = w.u < b.full_units;
+  if (!whole && w.pos >= w.end) return false;
+  const int at = whole ? w.u : w.pos;
+  int e = 0, hi = p.E;   // the last group that begins at or before `at` is not empty
+  while (hi - e > 1) {
+    const int mid = (e + hi) >> 1;
+    if ((whole ? tab[mid].y : tab[mid].z) <= at) e = mid; else hi = mid;
   }
-  __device__ bool next(Piece& c) {
-    int v, k0, k1, e, steps;
-    c.parts = 1;
-    if (u < b.full_units) {
-      e = find(tab.unit, u);
-      v = u - tab.unit[e];
-      u += pairs;
-      steps = group_steps<KIND>(p, tab.row[e + 1] - tab.row[e]);
-      k0 = 0;
-      k1 = steps;
-    } else if (pos < end) {
-      e = find(tab.step, pos);
-      steps = group_steps<KIND>(p, tab.row[e + 1] - tab.row[e]);
-      const int off = pos - tab.step[e];
-      v = off / steps;
-      k0 = off - v * steps;
-      const int first = pos - k0;
-      k1 = min(steps, end - first);
-      c.j0 = owner(first);
-      c.parts = owner(first + steps - 1) - c.j0 + 1;
-      c.part = pair - c.j0;
-      pos = first + k1;
-    } else {
-      return false;
-    }
-    const int len = tab.row[e + 1] - tab.row[e], nj = tiles_j<KIND>(p, len), it = v / nj, jt = v - it * nj;
-    c.e = e;
-    c.i0 = it * kTileI;
-    c.t0 = tab.row[e];
-    c.len = len;
-    if (KIND == Kind::MM) {
-      c.row0 = jt * p.NT;
-      c.rows = min(p.NT, p.J - c.row0);
-      c.neff = (c.rows + 127) & ~127;
-    } else {
-      const int tr = tile_rows(len, p.NT);
-      c.row0 = c.t0 + jt * tr;
-      c.rows = min(tr, c.t0 + len - c.row0);
-      c.neff = (c.rows + 15) & ~15;
-    }
-    const int st = KIND == Kind::MM ? max(1, (len + kStageK<KIND> - 1) / kStageK<KIND>) : (p.K + kStageK<KIND> - 1) / kStageK<KIND>;
-    c.ks0 = k0 * kSpc<KIND>;
-    c.ks1 = min(st, k1 * kSpc<KIND>);
-    return true;
+  const Group g = tab[e];
+  const int len = tab[e + 1].x - g.x, steps = group_steps<KIND>(p, len), nj = g.w >> 9, tr = g.w & 511;
+  uint32_t v;
+  int k0 = 0, k1 = steps;
+  Piece& c = w.c;
+  c.parts = 1;
+  if (whole) {
+    v = (uint32_t)(at - g.y);
+    w.u += gridDim.x >> 1;
+  } else {
+    const uint32_t off = (uint32_t)(at - g.z);
+    v = off / (uint32_t)steps;
+    k0 = (int)(off - v * (uint32_t)steps);
+    const int first = at - k0;
+    k1 = min(steps, w.end - first);
+    // the pair whose range holds step s (counted from cut_base) is ((s + 1) cut_pairs - 1) / cut_steps
+    const uint32_t s0 = (uint32_t)(first - b.cut_base), s1 = s0 + (uint32_t)steps - 1, n = (uint32_t)b.cut_pairs, all = (uint32_t)b.cut_steps;
+    c.j0 = (int)(((s0 + 1) * n - 1) / all);
+    c.parts = (int)(((s1 + 1) * n - 1) / all) - c.j0 + 1;
+    c.part = (int)(blockIdx.x >> 1) - c.j0;
+    w.pos = first + k1;
   }
-};
+  const uint32_t it = nj == 1 ? v : v / (uint32_t)nj;
+  const int jt = (int)(v - it * (uint32_t)nj);
+  c.e = e;
+  c.i0 = (int)it * kTileI;
+  c.t0 = g.x;
+  c.len = len;
+  if (KIND == Kind::MM) {
+    c.row0 = jt * tr;
+    c.rows = min(tr, p.J - c.row0);
+    c.neff = (c.rows + 127) & ~127;
+  } else {
+    c.row0 = g.x + jt * tr;
+    c.rows = min(tr, g.x + len - c.row0);
+    c.neff = (c.rows + 15) & ~15;
+  }
+  c.ks0 = k0 * kSpc<KIND>;
+  c.ks1 = min(group_stages<KIND>(p, len), k1 * kSpc<KIND>);
+  return true;
+}
 
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
   asm volatile(
@@ -224,22 +240,44 @@ __device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap* map
 __device__ __forceinline__ void arrive_release_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
-// Bounded wait of the MMA thread for what the other block's threads have written too.
-__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  for (uint32_t i = 0; i < kSpinLimit * 4u; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if ((i & 1023) == 1023 && *abort_flag) return false;
+// Bounded waits.  try_wait holds the thread back in hardware: a dozen warps that look again and again take issue slots and
+// shared-memory cycles from the tensor core's operands.
+constexpr long long kWaitMost = 1ll << 30;   // cycles, about half a second
+__device__ __forceinline__ bool wait_local(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try(bar, parity)) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > kWaitMost) {
+      *abort_flag = 1;
+      return false;
+    }
   }
-  *abort_flag = 1;
-  return false;
+  return true;
+}
+// Of the MMA thread, for what the other block's threads have written too.
+__device__ __forceinline__ bool try_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (try_cluster(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!try_cluster(bar, parity)) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > kWaitMost) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -281,37 +319,28 @@ __device__ __forceinline__ uint32_t make_idesc(int n) {
   return shape | (1u << 4) | (fmt << 7) | (fmt << 10) | (KIND != Kind::KK ? 1u << 15 : 0u) | (KIND == Kind::MM ? 1u << 16 : 0u);
 }
 
-// 16 bytes at any address, of which those before `end` are read (and the rest are zeros).
-__device__ __forceinline__ uint4 load16_any(const uint8_t* at, const uint8_t* end) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(at);
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
-  const int sh = (int)(a & 3) * 8;
-  const uint32_t* stop = reinterpret_cast<const uint32_t*>((reinterpret_cast<uintptr_t>(end) + 3) & ~uintptr_t(3));
-  uint32_t v[5];
-#pragma unroll
-  for (int i = 0; i < 5; ++i) v[i] = w + i < stop ? __ldg(w + i) : 0u;
-  uint32_t r[4];
-  const long long left = end - at;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    r[i] = __funnelshift_r(v[i], v[i + 1], sh);
-    const long long n = left - 4 * i;
-    if (n < 4) r[i] = n <= 0 ? 0u : r[i] & (0xFFFFFFFFu >> (32 - 8 * (int)n));
-  }
-  return make_uint4(r[0], r[1], r[2], r[3]);
+// 4 bytes at any address, of which `left` >= 1 are there (and the rest are zeros): from the one or two words that hold them.
+__device__ __forceinline__ uint32_t load4_any(const uint8_t* at, int left) {
+  const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(at) & 3);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(at - sh);
+  const uint32_t lo = __ldg(w), hi = sh && sh + min(left, 4) > 4 ? __ldg(w + 1) : 0u;
+  const uint32_t v = __funnelshift_r(lo, hi, 8 * sh);
+  return left >= 4 ? v : v & (0xFFFFFFFFu >> (32 - 8 * left));
 }
 __device__ __forceinline__ void sts32(uint32_t at, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
 __device__ __forceinline__ void lds128(uint32_t at, uint4& v) {
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
 }
-// A chunk's word k of row r: blocks of 128 rows x 4 bytes of k, in which row r has word (r % 32) * 4 + r / 32.
-__device__ __forceinline__ void store_scales(uint32_t base, uint32_t k_stride, int r, int half, const uint4& v) {
-  const uint32_t at = base + (r >> 7) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + half * 4 * k_stride;
-  sts32(at, v.x);
-  sts32(at + k_stride, v.y);
-  sts32(at + 2 * k_stride, v.z);
-  sts32(at + 3 * k_stride, v.w);
+// Where a chunk has the 4 scales `word` of row r: per word blocks of 128 rows, in which row r is at (r % 32) * 4 + r / 32.
+__device__ __forceinline__ uint32_t scales_at(uint32_t base, uint32_t word_stride, int r, int word) {
+  return base + word * word_stride + (r >> 7) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4;
 }
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool read) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(read ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -347,7 +376,7 @@ __device__ __forceinline__ void store4(T* dst, int left, bool vec, float a, floa
 }
 
 template <typename T, Kind KIND>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<KIND>, 1)
 grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   constexpr bool kSf = kFp4<KIND>, kSum = KIND == Kind::MM;
   constexpr int kSb = KIND == Kind::Mx ? 8 : 16;   // bytes of scales per row and stage
@@ -358,10 +387,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
   const uint32_t sf_bytes = kSf ? 4096u + (uint32_t)p.sfb_chunk : 0u;
   unsigned char* staging = ring_sf + kSfSlots * sf_bytes;
   Bars* bars = reinterpret_cast<Bars*>(staging + (sizeof(T) == 2 ? kEpiWarps * kStageOut : 0));
-  Table tab;
-  tab.row = reinterpret_cast<int*>(bars + 1);
-  tab.unit = tab.row + p.E + 1;
-  tab.step = tab.unit + p.E + 1;
+  Group* tab = reinterpret_cast<Group*>(bars + 1);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
@@ -372,7 +398,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       mbar_init(smem_u32(&bars->empty[lane]), 1);
       if (kSum) { mbar_init(smem_u32(&bars->landed[lane]), 1); mbar_init(smem_u32(&bars->fixed[lane]), 2); }
     }
-    if (lane < kSfSlots) { mbar_init(smem_u32(&bars->sf_full[lane]), 2); mbar_init(smem_u32(&bars->sf_empty[lane]), 1); }
+    if (lane < kSfSlots) { mbar_init(smem_u32(&bars->sf_full[lane]), 4); mbar_init(smem_u32(&bars->sf_empty[lane]), 1); }
     if (lane < 2) { mbar_init(smem_u32(&bars->acc_full[lane]), 1); mbar_init(smem_u32(&bars->acc_empty[lane]), 2 * kEpiWarps); }
     if (lane == 0) bars->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -409,12 +435,11 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
     for (int e = lo; e < hi; ++e) {
       const int r0 = (int)min(at, (long long)p.T);
       at += size_of(e);
-      const int len = (int)min(at, (long long)p.T) - r0, n = tiles_j<KIND>(p, len) * p.i_tiles;
-      tab.row[e] = r0;
-      tab.unit[e] = units;
-      tab.step[e] = steps;
-      units += n;
-      steps += n * group_steps<KIND>(p, len);
+      const int len = (int)min(at, (long long)p.T) - r0;
+      const int2 tr = tiles_j<KIND>(p, len);
+      tab[e] = make_int4(r0, units, steps, tr.y << 9 | tr.x);
+      units += tr.y * p.i_tiles;
+      steps += tr.y * p.i_tiles * group_steps<KIND>(p, len);
     }
     int u0 = units, s0 = steps;
 #pragma unroll
@@ -425,30 +450,24 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
     const int total = __shfl_sync(0xFFFFFFFFu, u0, 31), all_steps = __shfl_sync(0xFFFFFFFFu, s0, 31);
     u0 -= units;
     s0 -= steps;
-    for (int e = lo; e < hi; ++e) { tab.unit[e] += u0; tab.step[e] += s0; }
-    const int last_row = (int)min(__shfl_sync(0xFFFFFFFFu, at, 31), (long long)p.T);
+    for (int e = lo; e < hi; ++e) { tab[e].y += u0; tab[e].z += s0; }
+    const int rows_end = (int)min(__shfl_sync(0xFFFFFFFFu, at, 31), (long long)p.T);
     bad = __any_sync(0xFFFFFFFFu, bad);
     __syncwarp();
     if (lane == 0) {
-      tab.row[p.E] = last_row;
-      tab.unit[p.E] = total;
-      tab.step[p.E] = all_steps;
-      bars->rows = last_row;
+      tab[p.E] = make_int4(rows_end, total, all_steps, 0);
       const int pairs = gridDim.x >> 1;
-      int full = total - total % pairs, cut_pairs = 0, base = 0, rest = 0;
-      if (full < total && p.partial) {
+      const int full = (int)((uint32_t)total / (uint32_t)pairs) * pairs;
+      int cut_pairs = 0, base = 0, rest = 0;
+      if (full < total) {
         int e = 0, h = p.E;   // the group in which the rest begins
-        while (h - e > 1) { const int m = (e + h) >> 1; if (tab.unit[m] <= full) e = m; else h = m; }
-        base = tab.step[e] + (full - tab.unit[e]) * group_steps<KIND>(p, tab.row[e + 1] - tab.row[e]);
+        while (h - e > 1) { const int m = (e + h) >> 1; if (tab[m].y <= full) e = m; else h = m; }
+        const int x1 = tab[e + 1].x;
+        base = tab[e].z + (full - tab[e].y) * group_steps<KIND>(p, x1 - tab[e].x);
         rest = all_steps - base;
-        // A whole wave takes as long as a tile.  Cut in s parts, a tile takes its share, and whoever comes last reads s partial
-        // sums at about 64 bytes per clock: least at s = sqrt(tile / sum of one part).
-        const float n = (float)(total - full), tile = (float)rest / n * (float)p.step_cycles, part = 8.0f * (float)p.NT;
-        const float share = fminf((float)pairs, floorf(n * fmaxf(1.0f, sqrtf(tile / part))));
-        cut_pairs = min((int)share, rest);
-        const float cut = tile * n / (float)cut_pairs + (ceilf((float)cut_pairs / n) + 1.0f) * part + (float)kCutCycles;
-        if (cut_pairs < 2 || cut >= tile) cut_pairs = 0;
+        cut_pairs = cut_for<KIND>(p, total - full, rest, KIND == Kind::MM ? p.NT : (int)__fdividef((float)rows_end * (float)p.i_tiles, (float)total), pairs);
       }
+      bars->rows = rows_end;
       bars->full_units = cut_pairs ? full : total;
       bars->cut_pairs = cut_pairs;
       bars->cut_steps = rest;
@@ -464,60 +483,86 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
   const int nacc = 2 * p.NT + (kSf ? kSfColumns : 0) <= 512 ? 2 : 1;
   const uint32_t tmem_sf = tmem + nacc * p.NT;
   const uint32_t ring = smem_u32(smem);
+  Walk& walk = bars->walk[warp];
+  if (lane == 0) walk_begin(*bars, walk);
+  __syncwarp();
+  auto next_of_warp = [&]() -> bool {
+    __syncwarp();   // everybody has read the last piece
+    bool more = false;
+    if (lane == 0) more = walk_next<KIND>(p, *bars, tab, walk);
+    return __shfl_sync(0xFFFFFFFFu, more, 0);
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ operands
     if (elect_one()) {
       const uint32_t full = smem_u32(&bars->full[0]), lfull = leader_addr(full), empty = smem_u32(&bars->empty[0]), landed = smem_u32(&bars->landed[0]);
-      Walk<KIND> walk(p, *bars, tab);
-      Piece c;
       uint32_t s = 0, ph = 1;
       bool ok = true;
-      while (ok && walk.next(c)) {
-        const int half = c.neff >> 1;
-        const uint32_t mine = kStageA + (uint32_t)half * 128u;
-        for (int ks = c.ks0; ks < c.ks1; ++ks) {
-          if (!mbar_wait_spin(empty + s * 8, ph, abort_flag)) { ok = false; break; }
-          const uint32_t a = ring + s * stage_bytes, b = a + kStageA;
+      bool begun = !kSf;
+      while (ok && walk_next<KIND>(p, *bars, tab, walk)) {
+        const Piece c = walk.c;
+        auto load_a = [&](int ks) {
+          const uint32_t a = ring + s * stage_bytes, bar = lfull + s * 8;
+          const int k = ks * (kSf ? 128 : 64);
+          if (rank == 0) mbar_expect_tx(full + s * 8, 2 * kStageA + (uint32_t)c.neff * 128u);
+          if constexpr (KIND == Kind::MK) {
+  #pragma unroll
+            for (int h = 0; h < 2; ++h) tma_3d_pair(a + h * 8192, &maps.a, c.i0 + rank * kLanes + 64 * h, k, c.e, bar);
+          } else {
+            tma_3d_pair(a, &maps.a, k, c.i0 + rank * kLanes, c.e, bar);
+          }
+        };
+        auto load_b = [&](int ks, uint32_t slot) {
+          const uint32_t b = ring + slot * stage_bytes + kStageA, bar = lfull + slot * 8;
+          const int k = ks * (kSf ? 128 : 64), half = c.neff >> 1, row = c.row0 + rank * half;
+          int r = 0;
+  #pragma unroll
+          for (int i = 0; i < 5; ++i) {
+            const int box = 128 >> i;
+            if (half & box) {
+              tma_3d_pair(b + r * 128, &maps.b[i], k, row + r, 0, bar);
+              r += box;
+            }
+          }
+        };
+        int ks = c.ks0;
+        if (!begun) {
+          // 4 bits: the kernel that quantizes b may still be running.  The first stages' weights are requested before it is
+          // waited for.
+          begun = true;
+          const int n = min(p.stages, c.ks1 - c.ks0);
+          for (; ks < c.ks0 + n; ++ks, ++s) load_a(ks);
+          asm volatile("griddepcontrol.wait;" ::: "memory");
+          for (int i = 0; i < n; ++i) load_b(c.ks0 + i, (uint32_t)i);
+          if (s == (uint32_t)p.stages) { s = 0; ph ^= 1; }
+        }
+        for (; ks < c.ks1; ++ks) {
+          if (!wait_local(empty + s * 8, ph, abort_flag)) { ok = false; break; }
           if constexpr (kSum) {
-            const int t = c.t0 + ks * 64;
+            const uint32_t a = ring + s * stage_bytes, b = a + kStageA;
+            const int t = c.t0 + ks * 64, half = c.neff >> 1, i = c.i0 + rank * kLanes, j = c.row0 + rank * half;
             if (c.len - ks * 64 >= 64) {
               const uint32_t bar = lfull + s * 8;
-              if (rank == 0) mbar_expect_tx(full + s * 8, 2 * mine);
+              if (rank == 0) mbar_expect_tx(full + s * 8, 2 * kStageA + (uint32_t)c.neff * 128u);
 #pragma unroll
-              for (int h = 0; h < 2; ++h) tma_3d_pair(a + h * 8192, &maps.a, c.i0 + rank * kLanes + 64 * h, t, 0, bar);
-              for (int h = 0; h < half / 64; ++h) tma_3d_pair(b + h * 8192, &maps.b[0], c.row0 + rank * half + 64 * h, t, 0, bar);
+              for (int h = 0; h < 2; ++h) tma_3d_pair(a + h * 8192, &maps.a, i + 64 * h, t, 0, bar);
+              for (int h = 0; h < half / 64; ++h) tma_3d_pair(b + h * 8192, &maps.b[0], j + 64 * h, t, 0, bar);
             } else {
               const uint32_t bar = landed + s * 8;
-              mbar_expect_tx(bar, mine);
+              mbar_expect_tx(bar, kStageA + (uint32_t)half * 128u);
 #pragma unroll
-              for (int h = 0; h < 2; ++h) tma_3d(a + h * 8192, &maps.a, c.i0 + rank * kLanes + 64 * h, t, 0, bar);
-              for (int h = 0; h < half / 64; ++h) tma_3d(b + h * 8192, &maps.b[0], c.row0 + rank * half + 64 * h, t, 0, bar);
+              for (int h = 0; h < 2; ++h) tma_3d(a + h * 8192, &maps.a, i + 64 * h, t, 0, bar);
+              for (int h = 0; h < half / 64; ++h) tma_3d(b + h * 8192, &maps.b[0], j + 64 * h, t, 0, bar);
             }
           } else {
-            const uint32_t bar = lfull + s * 8;
-            const int k = ks * (kSf ? 128 : 64);
-            if (rank == 0) mbar_expect_tx(full + s * 8, 2 * mine);
-            if constexpr (KIND == Kind::MK) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h) tma_3d_pair(a + h * 8192, &maps.a, c.i0 + rank * kLanes + 64 * h, k, c.e, bar);
-            } else {
-              tma_3d_pair(a, &maps.a, k, c.i0 + rank * kLanes, c.e, bar);
-            }
-            int r = 0;
-            const int row = c.row0 + rank * half;
-#pragma unroll
-            for (int i = 0; i < 5; ++i) {
-              const int box = 128 >> i;
-              if (half & box) {
-                tma_3d_pair(b + r * 128, &maps.b[i], k, row + r, 0, bar);
-                r += box;
-              }
-            }
+            load_a(ks);
+            load_b(ks, s);
           }
           if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; }
         }
       }
+      if (!begun) asm volatile("griddepcontrol.wait;" ::: "memory");   // no block ends before that kernel has
       if (!ok) for (int i = 0; i < 100; ++i) __nanosleep(1000);   // copies in flight land before the block ends
     }
   } else if (warp == 1) {
@@ -525,18 +570,17 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
     if (rank == 0 && elect_one()) {
       const uint32_t full = smem_u32(&bars->full[0]), empty = smem_u32(&bars->empty[0]);
       const uint32_t sf_full = smem_u32(&bars->sf_full[0]), sf_empty = smem_u32(&bars->sf_empty[0]), sf_ring = smem_u32(ring_sf);
-      Walk<KIND> walk(p, *bars, tab);
-      Piece c;
       const uint32_t fixed = smem_u32(&bars->fixed[0]);
       // A bit per slot: the phase that its barriers `full` and `fixed` are in (MM uses one or the other)
       uint32_t s = 0, full_ph = 0, fixed_ph = 0, sq = 0, sph = 0, n_piece = 0, n_stage = 0;
       bool ok = true;
-      while (ok && walk.next(c)) {
+      while (ok && walk_next<KIND>(p, *bars, tab, walk)) {
+        const Piece c = walk.c;
         const uint32_t idesc = make_idesc<T, KIND>(c.neff);
         const uint32_t ab = nacc == 2 ? n_piece & 1 : 0, an = nacc == 2 ? n_piece >> 1 : n_piece;
         const uint32_t acc = tmem + ab * p.NT;
         ++n_piece;
-        if (!mbar_wait_spin(smem_u32(&bars->acc_empty[ab]), (an & 1) ^ 1, abort_flag)) break;
+        if (!wait_local(smem_u32(&bars->acc_empty[ab]), (an & 1) ^ 1, abort_flag)) break;
         uint32_t first = 0;
         for (int ks = c.ks0; ks < c.ks1; ++ks) {
           const int in_chunk = kSf ? (ks - c.ks0) % kSpc<KIND> : 0;
@@ -583,15 +627,14 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
   } else if (kSum && warp == 2) {
     // ------------------------------------------------------------ rows of other groups are zeroed
     const uint32_t landed = smem_u32(&bars->landed[0]), lfixed = leader_addr(smem_u32(&bars->fixed[0]));
-    Walk<KIND> walk(p, *bars, tab);
-    Piece c;
     uint32_t at = 0, ph = 0;   // stages so far; a bit per slot
-    while (walk.next(c)) {
+    while (next_of_warp()) {
+      const Piece c = walk.c;
       at += c.ks1 - c.ks0;
       const int valid = c.len - (c.ks1 - 1) * 64;
       if (valid >= 64) continue;
       const uint32_t s = (at - 1) % (uint32_t)p.stages;
-      if (!__all_sync(0xFFFFFFFFu, mbar_wait_spin(landed + s * 8, (ph >> s) & 1, abort_flag))) break;
+      if (!__all_sync(0xFFFFFFFFu, wait_local(landed + s * 8, (ph >> s) & 1, abort_flag))) break;
       ph ^= 1u << s;
       const int blocks = 2 + (c.neff >> 7);   // of 64 columns: two of a, one or two of b
       const uint32_t tile = ring + s * stage_bytes;
@@ -602,55 +645,67 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       __syncwarp();
       if (lane == 0) arrive_release_cluster(lfixed + s * 8);
     }
-  } else if (kSf && warp >= kScaleWarp0 && warp < kScaleWarp0 + kScaleWarps) {
-    // ------------------------------------------------------------ scales: warps take chunks in turn
-    const uint32_t sf_ring = smem_u32(ring_sf), lsf = leader_addr(smem_u32(&bars->sf_full[0])), sf_empty = smem_u32(&bars->sf_empty[0]);
-    const uint32_t kb = p.sfb_chunk / 8;
-    const int half = lane & 1, r0 = lane >> 1;   // a lane has 16 of a row's 32 bytes
-    Walk<KIND> walk(p, *bars, tab);
-    Piece c;
-    uint32_t chunk = 0;
+  } else if (kSf && warp >= kScaleWarp0) {
+    // ------------------------------------------------------------ scales: an operand's two warps take chunks in turn
+    const bool of_b = warp >= kScaleWarp0 + kScaleWarps;
+    const uint32_t mine = warp & 1, lsf = leader_addr(smem_u32(&bars->sf_full[0])), sf_empty = smem_u32(&bars->sf_empty[0]);
+    const uint32_t stride = of_b ? p.sfb_chunk / 8 : 512, base = smem_u32(ring_sf) + (of_b ? 4096 : 0);
+    const int word = lane & 7, r0 = lane >> 3;   // a lane has 4 of a row's 32 bytes
+    uint32_t chunk = 0, oldest = mine, pending = 0;
+    // The oldest chunk on its way is there: the tensor core may read it.
+    auto finish = [&]() {
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) arrive_release_cluster(lsf + oldest % kSfSlots * 8);
+      oldest += kScaleWarps;
+      --pending;
+    };
     bool ok = true;
-    while (ok && walk.next(c)) {
+    if (of_b) asm volatile("griddepcontrol.wait;" ::: "memory");
+    while (ok && next_of_warp()) {
+      const Piece c = walk.c;
       for (int ks = c.ks0; ks < c.ks1; ks += kSpc<KIND>, ++chunk) {
-        if ((chunk & (kScaleWarps - 1)) != (uint32_t)(warp - kScaleWarp0)) continue;
-        const int byte = ks * kSb + 16 * half, left = p.sf_row - byte;
-        uint4 va[kLanes / 16];
-#pragma unroll
-        for (int i = 0; i < kLanes / 16; ++i) {
-          const int n = c.i0 + rank * kLanes + r0 + 16 * i;
-          va[i] = make_uint4(0, 0, 0, 0);
-          if (n < p.I && left > 0) {
-            const uint8_t* at = p.sfa + ((long long)c.e * p.I + n) * p.sf_row + byte;
-            if (p.sfa16) va[i] = __ldg(reinterpret_cast<const uint4*>(at));
-            else va[i] = load16_any(at, at + min(left, 16));
-          }
+        if ((chunk & (kScaleWarps - 1)) != mine) continue;
+        const uint32_t sl = chunk % kSfSlots, ph = (chunk / kSfSlots & 1) ^ 1, at = base + sl * sf_bytes;
+        if (pending && !__all_sync(0xFFFFFFFFu, mbar_test(sf_empty + sl * 8, ph))) {
+          // nobody waits for a slot while others wait for what is on its way
+          if (pending == 2) { cp_async_wait<1>(); finish(); }
+          cp_async_wait<0>();
+          finish();
         }
-        const uint32_t sl = chunk % kSfSlots, at = sf_ring + sl * sf_bytes;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait_spin(sf_empty + sl * 8, ((chunk / kSfSlots) & 1) ^ 1, abort_flag));
+        ok = __all_sync(0xFFFFFFFFu, wait_local(sf_empty + sl * 8, ph, abort_flag));
         if (!ok) break;
+        const int byte = ks * kSb + 4 * word;
+        if (of_b) {
+          // rows of the tile, 32 at a time (past the end of b: the last row's, for columns that nobody stores)
+          const uint32_t* from = p.sfb + (long long)(ks * kSb / 4) * p.T + c.row0;
+          const int most = p.T - 1 - c.row0;
+          for (int r = lane; r < ((c.neff + 31) & ~31); r += 32) {
+            const uint32_t* of_row = from + min(r, most);
 #pragma unroll
-        for (int i = 0; i < kLanes / 16; ++i) store_scales(at, 512, r0 + 16 * i, half, va[i]);
-        // b: rows of the tile, of x's own scales (rows past the end of x: the last row's, for columns that nobody stores)
-#pragma unroll
-        for (int i0 = 0; i0 < kMaxNT / 16; i0 += 4) {
-          if (16 * i0 >= c.neff) break;
-          uint4 vb[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = min(c.row0 + r0 + 16 * (i0 + i), p.T - 1);
-            vb[i] = *reinterpret_cast<const uint4*>(p.sfb + (long long)r * p.sfb_pitch + byte);
+            for (int k = 0; k < 8; ++k) cp_async4(scales_at(at, stride, r, k), of_row + (long long)k * p.T, true);
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (16 * (i0 + i) < c.neff) store_scales(at + 4096, kb, r0 + 16 * (i0 + i), half, vb[i]);
+        } else {
+          const int n0 = c.i0 + rank * kLanes, rows = p.I - n0, left = p.sf_row - byte;
+          const uint8_t* from = p.sfa + ((long long)c.e * p.I + n0) * p.sf_row + byte;
+          if (p.sfa4) {
+#pragma unroll 8
+            for (int r = r0; r < kLanes; r += 4) {
+              const bool in = r < rows && left > 0;
+              cp_async4(scales_at(at, 512, r, word), in ? from + (long long)r * p.sf_row : p.sfa, in);
+            }
+          } else {
+#pragma unroll 8
+            for (int r = r0; r < kLanes; r += 4)
+              sts32(scales_at(at, 512, r, word), r < rows && left > 0 ? load4_any(from + (long long)r * p.sf_row, left) : 0u);
+          }
         }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) arrive_release_cluster(lsf + sl * 8);
+        cp_async_commit();
+        if (++pending == 2) { cp_async_wait<1>(); finish(); }
       }
     }
-  } else if (warp >= kEpiWarp0) {
+    if (pending) { cp_async_wait<0>(); finish(); }
+  } else if (warp >= kEpiWarp0 && warp < kEpiWarp0 + kEpiWarps) {
     // ------------------------------------------------------------ epilogue
     const int w = warp - kEpiWarp0, quad = warp & 3, chalf = w >> 2;
     const uint32_t stg = smem_u32(staging) + w * kStageOut;
@@ -660,14 +715,13 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       const long long n = (long long)(p.T - bars->rows) * p.I, step = (long long)gridDim.x * kEpiWarps * 32;
       for (long long i = ((long long)blockIdx.x * kEpiWarps + w) * 32 + lane; i < n; i += step) z[i] = Elem<T>::from_float(0.0f);
     }
-    Walk<KIND> walk(p, *bars, tab);
-    Piece c;
     uint32_t n_piece = 0;
-    while (walk.next(c)) {
+    while (next_of_warp()) {
+      const Piece c = walk.c;
       const uint32_t ab = nacc == 2 ? n_piece & 1 : 0, an = nacc == 2 ? n_piece >> 1 : n_piece;
       // One warp looks and all go by what it found: the abort flag may be raised between two warps' looks.
       if (w == 0) {
-        const bool seen = __all_sync(0xFFFFFFFFu, mbar_wait_spin(smem_u32(&bars->acc_full[ab]), an & 1, abort_flag));
+        const bool seen = __all_sync(0xFFFFFFFFu, wait_local(smem_u32(&bars->acc_full[ab]), an & 1, abort_flag));
         if (lane == 0) bars->seen[n_piece & 1] = seen;
         __syncwarp();
       }
@@ -747,35 +801,54 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       }
       if constexpr (sizeof(T) == 2) {
         if (p.vec) {
-          for (int q = p0; q < p1; ++q) {
-            uint32_t r[2][16];
-            load_16(acc + 32 * q, r[0]);
-            const bool two = 32 * q + 16 < c.neff;
-            if (two) load_16(acc + 32 * q + 16, r[1]);
-            tcgen05_wait_ld16(r[0]);
-            if (two) tcgen05_wait_ld16(r[1]);
-            if (q + 1 == p1) release();
-  #pragma unroll
+          const uint32_t row = lane & 7, put = stg + row * 64 + ((((uint32_t)lane >> 3) ^ (row >> 1)) << 4);
+          const uint32_t get = stg + (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
+          const int i = i_warp + (lane & 3) * 8;
+          T* dst = out_row<T, KIND>(p, c, 32 * p0 + (lane >> 2)) + i;
+          uint32_t r0[2][16], r1[2][16];
+          auto load = [&](int q, uint32_t (&v)[2][16]) {
+            load_16(acc + 32 * q, v[0]);
+            if (32 * q + 16 < c.neff) load_16(acc + 32 * q + 16, v[1]);
+          };
+          auto piece = [&](int q, uint32_t (&v)[2][16]) {
+#pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (h == 1 && !two) break;
+              if (h == 1 && 32 * q + 16 >= c.neff) break;
               // 16 rows of 64 bytes, 16-byte chunks xor-ed with row / 2
-              const uint32_t row = lane & 7, at = stg + h * 1024 + row * 64 + ((((uint32_t)lane >> 3) ^ (row >> 1)) << 4);
-              auto f = [&](int k) { return __uint_as_float(r[h][k]) * alpha; };
-  #pragma unroll
+              auto f = [&](int k) { return __uint_as_float(v[h][k]) * alpha; };
+#pragma unroll
               for (int x = 0; x < 2; ++x)
-                stmatrix_x4_trans(at + x * 512, pack2<T>(f(4 * x), f(4 * x + 1)), pack2<T>(f(4 * x + 2), f(4 * x + 3)),
+                stmatrix_x4_trans(put + h * 1024 + x * 512, pack2<T>(f(4 * x), f(4 * x + 1)), pack2<T>(f(4 * x + 2), f(4 * x + 3)),
                                   pack2<T>(f(8 + 4 * x), f(8 + 4 * x + 1)), pack2<T>(f(8 + 4 * x + 2), f(8 + 4 * x + 3)));
             }
             __syncwarp();
-            const int i = i_warp + (lane & 3) * 8;
             if (i < p.I) {   // (whole chunks: rows on 16-byte boundaries are whole eights long)
-              for (int tok = lane >> 2; tok < min(32, c.rows - 32 * q); tok += 8) {
-                uint4 v;
-                lds128(stg + tok * 64 + (((lane & 3) ^ ((tok >> 1) & 3)) << 4), v);
-                *reinterpret_cast<uint4*>(out_row<T, KIND>(p, c, 32 * q + tok) + i) = v;
+              const int n = c.rows - 32 * q - (lane >> 2);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint4 o;
+                lds128(get + k * 512, o);
+                if (8 * k < n) *reinterpret_cast<uint4*>(dst + (long long)(8 * k) * p.I) = o;
               }
             }
+            dst += (long long)32 * p.I;
             __syncwarp();
+          };
+          // the next piece is on its way while one is stored
+          if (p0 < p1) load(p0, r0);
+          for (int q = p0; q < p1; q += 2) {
+            tcgen05_wait_ld16(r0[0]);
+            tcgen05_wait_ld16(r0[1]);
+            if (q + 1 < p1) load(q + 1, r1);
+            else release();
+            piece(q, r0);
+            if (q + 1 < p1) {
+              tcgen05_wait_ld16(r1[0]);
+              tcgen05_wait_ld16(r1[1]);
+              if (q + 2 < p1) load(q + 2, r0);
+              else release();
+              piece(q + 1, r1);
+            }
           }
           if (p0 == p1) release();
           continue;
@@ -869,7 +942,7 @@ template <typename T, Kind KIND>
 int launch(const Maps& m, Params& p, cudaStream_t st) {
   const size_t stage = kStageA + (size_t)p.NT * 64;
   const size_t fixed = 1024 + (kFp4<KIND> ? kSfSlots * (4096 + (size_t)p.sfb_chunk) : 0) + (sizeof(T) == 2 ? kEpiWarps * kStageOut : 0) +
-                       sizeof(Bars) + (size_t)(p.E + 1) * 12;
+                       sizeof(Bars) + (size_t)(p.E + 1) * sizeof(Group);
   p.stages = (int)((kSmemMax - fixed) / stage);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   size_t smem = fixed + p.stages * stage;
@@ -877,7 +950,18 @@ int launch(const Maps& m, Params& p, cudaStream_t st) {
   if (smem < 120 * 1024) smem = 120 * 1024;
   auto kernel = grouped_tc_kernel<T, KIND>;
   if (int rc = allow_smem((const void*)kernel)) return rc;
-  kernel<<<2 * sm_pairs(), kThreads, smem, st>>>(m, p);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * sm_pairs());
+  cfg.blockDim = dim3(kThreads<KIND>);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  // 4 bits: starts beside the kernel that quantizes b, which is always the one before it on the stream
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = kFp4<KIND> ? 1 : 0;
+  B200Q_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, m, p));
   B200Q_LAUNCH_OK("grouped_tc_kernel");
   return B200Q_OK;
 }
@@ -917,17 +1001,14 @@ int grouped_tc(const GroupedTcArgs& a, cudaStream_t st) {
   p.partial = reinterpret_cast<float*>(static_cast<char*>(a.ws) + kCounterBytes);
   p.status = a.status;
   p.sfb_chunk = p.NT > 128 ? 8192 : 4096;
-  p.sfa = a.sfa; p.sfb = a.sfb; p.sf_row = (int)a.sf_row; p.sfb_pitch = (int)a.sfb_pitch;
-  p.sfa16 = ((reinterpret_cast<uintptr_t>(a.sfa) | (uintptr_t)a.sf_row) & 15) == 0;
+  p.sfa = a.sfa; p.sfb = a.sfb; p.sf_row = (int)a.sf_row;
+  p.sfa4 = ((reinterpret_cast<uintptr_t>(a.sfa) | (uintptr_t)a.sf_row) & 3) == 0;
   p.ga = a.ga; p.gb = a.gb; p.ga_each = a.ga_each;
   // number of tiles and steps in 32 bits
   const int64_t tiles = ((sum ? (a.J + p.NT - 1) / p.NT * a.E : a.T / p.NT + a.E + 1)) * p.i_tiles;
   const int64_t steps = sum ? (a.T / 64 + 2 * a.E) * ((a.J + p.NT - 1) / p.NT) * p.i_tiles : tiles * ((a.K + 63) / 64);
   if (tiles >= INT32_MAX || steps >= INT32_MAX)
     return fail(B200Q_ERR_UNSUPPORTED, "[grouped product] No implementation for problem shape: too many tiles");
-  // A stage: its MMAs (2 cycles per row), or 16 KB of weights at an SM's share of HBM.
-  p.step_cycles = (2 * p.NT > 700 ? 2 * p.NT : 700) * (a.form == GroupedForm::Mx ? kSpc<Kind::Mx> : (a.form == GroupedForm::Nv ? kSpc<Kind::Nv> : 1));
-
   const int e_a = fp4 ? 1 : 2;
   const int64_t ka = fp4 ? a.K / 2 : a.K;
   int rc = B200Q_OK;

@@ -178,8 +178,9 @@ struct GroupedTcArgs {
   void* out;                // [T, I], Sum: [E, J, I]
   int dtype;                // of out (and of 16-bit operands)
   int64_t T, E, I, J, K;
-  const uint8_t *sfa, *sfb;         // 4 bits: scales, rows sf_row and sfb_pitch bytes apart (sfb: padded with zeros to whole 32s, 16-byte aligned)
-  int64_t sf_row, sfb_pitch;
+  const uint8_t* sfa;               // 4 bits: scales, rows sf_row bytes apart
+  const uint32_t* sfb;              // and words of four consecutive ones: [words][T], zeros after the last up to a multiple of 8 words
+  int64_t sf_row;
   const float *ga, *gb;             // global scales (null: 1); ga_each: one per group
   int ga_each;
   void* ws;                 // grouped_tc_bytes, zeroed once
@@ -194,9 +195,9 @@ int fp4_quantize(const void* w, int dtype, int64_t rows, int64_t K, int mode, co
                  uint32_t* wq, uint8_t* scales, cudaStream_t st);
 int fp4_dequantize(const uint32_t* wq, const uint8_t* scales, int mode, const float* global, int64_t rows_per_global, int dtype,
                    int64_t rows, int64_t K, void* out, cudaStream_t st);
-// Activations for grouped_tc: rows of codes and of scales with pitches of their own, scales padded with zeros to sf_pitch.
+// Activations for grouped_tc: rows of codes with a pitch of their own, scales as [words][rows] words of four, zeros after the last.
 int fp4_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int mode, const float* global, uint8_t* codes,
-                      int64_t code_pitch, uint8_t* scales, int64_t sf_pitch, cudaStream_t st);
+                      int64_t code_pitch, uint32_t* scales, int64_t words, cudaStream_t st);
 // dst rows of dst_pitch bytes (a multiple of 16) from src rows of src_bytes, padded with zeros.
 int repack_rows(const void* src, int64_t src_bytes, void* dst, int64_t dst_pitch, int64_t rows, cudaStream_t st);
 
