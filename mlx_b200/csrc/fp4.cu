@@ -154,29 +154,41 @@ fp4_quantize_rows_kernel(const T* __restrict__ x, int64_t K, int64_t rows, int b
   if (threadIdx.x % kLanes == 0 && u / kLanes < words) scales[(u / kLanes) * rows + row] = s;
 }
 
+// A thread takes kAhead pieces of 8 values, kQuantThreads apart, whose codes and scales are all on their way before the first is
+// used: 16-byte stores, whole lines per warp.  (A thread per 16 values: 28672 x 8192 bf16 in 122 us.)
+constexpr int kAhead = 4;
 template <typename T, bool MX, bool ALIGNED>
 __global__ void __launch_bounds__(kQuantThreads)
-fp4_dequantize_kernel(const uint2* __restrict__ wq, const uint8_t* __restrict__ scales, int64_t units,
-                      const float* __restrict__ global, int64_t units_per_global, T* __restrict__ out) {
-  const int64_t u = (int64_t)blockIdx.x * kQuantThreads + threadIdx.x;
-  if (u >= units) return;
-  const uint2 c = __ldg(wq + u);
-  const uint32_t code = __ldg(scales + (MX ? u >> 1 : u));
-  const float s = MX ? e8m0_value(code) : e4m3_value(code), G = !MX && global ? __ldg(global + u / units_per_global) : 1.0f;
-  alignas(16) T r[kUnit];
+fp4_dequantize_kernel(const uint32_t* __restrict__ wq, const uint8_t* __restrict__ scales, int64_t pieces,
+                      const float* __restrict__ global, int64_t pieces_per_global, T* __restrict__ out) {
+  const int64_t p0 = (int64_t)blockIdx.x * (kQuantThreads * kAhead) + threadIdx.x;
+  uint32_t c[kAhead], code[kAhead];
 #pragma unroll
-  for (int i = 0; i < kUnit / 2; ++i) {
-    const float2 q = e2m1x2_value((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
-    r[2 * i] = Elem<T>::from_float(q.x * s * G);
-    r[2 * i + 1] = Elem<T>::from_float(q.y * s * G);
+  for (int j = 0; j < kAhead; ++j) {
+    const int64_t p = p0 + j * kQuantThreads;
+    c[j] = p < pieces ? __ldg(wq + p) : 0u;
+    code[j] = p < pieces ? __ldg(scales + (MX ? p >> 2 : p >> 1)) : 0u;
   }
-  T* at = out + u * kUnit;
-  if constexpr (ALIGNED) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T); ++i) reinterpret_cast<uint4*>(at)[i] = reinterpret_cast<const uint4*>(r)[i];
-  } else {
+  for (int j = 0; j < kAhead; ++j) {
+    const int64_t p = p0 + j * kQuantThreads;
+    if (p >= pieces) return;
+    const float s = MX ? e8m0_value(code[j]) : e4m3_value(code[j]), G = !MX && global ? __ldg(global + p / pieces_per_global) : 1.0f;
+    alignas(16) T r[8];
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i) at[i] = r[i];
+    for (int i = 0; i < 4; ++i) {
+      const float2 q = e2m1x2_value(c[j] >> (8 * i));
+      r[2 * i] = Elem<T>::from_float(q.x * s * G);
+      r[2 * i + 1] = Elem<T>::from_float(q.y * s * G);
+    }
+    T* at = out + p * 8;
+    if constexpr (ALIGNED) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(at)[i] = reinterpret_cast<const uint4*>(r)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) at[i] = r[i];
+    }
   }
 }
 
@@ -239,13 +251,13 @@ int fp4_quantize(const void* w, int dtype, int64_t rows, int64_t K, int mode, co
 
 int fp4_dequantize(const uint32_t* wq, const uint8_t* scales, int mode, const float* global, int64_t rows_per_global, int dtype,
                    int64_t rows, int64_t K, void* out, cudaStream_t st) {
-  const int64_t units = rows * (K / kUnit), blocks = (units + kQuantThreads - 1) / kQuantThreads;
+  const int64_t pieces = rows * (K / 8), blocks = (pieces + kQuantThreads * kAhead - 1) / (kQuantThreads * kAhead);
   if (blocks > kMostBlocks) return fail(B200Q_ERR_UNSUPPORTED, "[dequantize] No implementation for problem shape: too many values");
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     return with_flags(mode, aligned16(out), [&](auto mx, auto al) {
       fp4_dequantize_kernel<T, decltype(mx)::value, decltype(al)::value><<<(unsigned)blocks, kQuantThreads, 0, st>>>(
-          reinterpret_cast<const uint2*>(wq), scales, units, global, rows_per_global * (K / kUnit), static_cast<T*>(out));
+          wq, scales, pieces, global, rows_per_global * (K / 8), static_cast<T*>(out));
       B200Q_LAUNCH_OK("fp4_dequantize_kernel");
       return B200Q_OK;
     });

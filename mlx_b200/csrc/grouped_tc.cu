@@ -10,7 +10,7 @@
 // single tokens need no other kernel.  Each block of the pair fetches 128 of the i and half of the j; 16-bit operands need
 // 64 bytes per clock and SM that way, the L2's rate, where a block of its own would need 94.
 //
-//   warp 0      TMA: both operands of a stage (128 bytes of k per row; MM and MK: 64 k)
+//   warps 0, 3  TMA: a's and b's tile of a stage (128 bytes of k per row; MM and MK: 64 k)
 //   warp 1      tcgen05.mma, and for 4 bits tcgen05.cp of the stage's scales (leader block, one thread)
 //   warp 2      MM only: the stage that a group ends in has its foreign rows zeroed in shared memory (both operands: a foreign
 //               infinity times zero would be NaN).  Only those stages go through this warp: with all of them handed on by it
@@ -73,13 +73,15 @@ struct Params {
   int E, T;
   int I, J, K;             // output width; MM: output rows per group; length of the sum (MM: unused)
   int NT, i_tiles, stages;
+  int b_bytes;             // of a stage's b tile
+  int blocks;              // MK, MM: a (b) comes in whole blocks of 64 columns, two in one copy (bit 0: a, bit 1: b)
   int sfb_chunk;           // 4 bits: bytes of a chunk of b's scales
   void* out;
   int vec;                 // rows of the output start on 16-byte boundaries
   const uint8_t* sfa;      // scales [E * I, sf_row], and words of four of them [.., T]
   const uint32_t* sfb;
   int sf_row;
-  int sfa4;                // rows of sfa on 4-byte boundaries
+  int sfa_align;           // rows of sfa start on multiples of 16, of 8, or anywhere (1)
   const float* ga;         // global scales: one, or (ga_each) one per group
   const float* gb;
   int ga_each;
@@ -96,6 +98,17 @@ struct Piece {
   int ks0, ks1;       // stages
   int parts, part, j0;   // of a cut tile: number of parts, this one's number, first part's pair
 };
+
+// Rows of b that are fetched for `half` (a multiple of 8) of them: two boxes at most, since a copy costs its thread more than
+// 100 cycles and four of them more than a stage's MMAs.
+__host__ __device__ __forceinline__ int box_rows(int half, int* first) {
+  int a = 8;
+  while (2 * a <= half) a *= 2;
+  int b = half > a ? 8 : 0;
+  while (b && b < half - a) b *= 2;
+  *first = b == a ? 2 * a : a;
+  return a + b;
+}
 
 // A warp's way through its pair's pieces.
 struct __align__(16) Walk {
@@ -142,22 +155,22 @@ __device__ __forceinline__ int2 tiles_j(const Params& p, int len) {
 // Number of pairs that the n tiles (`rest` steps, `rows` rows each on average) left over from whole waves are cut for; 0: not
 // cut.  In cycles: a stage of n busy pairs takes its MMAs, its 16 KB of weights at their share of HBM, or at least 300; a cut
 // tile costs its writes (36 a row), the last arriver's reads (20 a row and part) and 4000 of fences and latencies.
+// The lanes of a warp try lane + 1 parts per tile (most: 8).
 template <Kind KIND>
-__device__ __forceinline__ int cut_for(const Params& p, int n, int rest, int rows, int pairs) {
+__device__ __forceinline__ int cut_for(int lane, int n, int rest, int rows, int pairs) {
   if ((long long)rest * (pairs + 1) >= INT32_MAX) return 0;
-  const float r = (float)max(rows, 16), tile = (float)(rest * kSpc<KIND>) / (float)n;   // stages
-  auto stage = [&](float busy) { return fmaxf(fmaxf(2.0f * r, 700.0f * busy / (float)pairs), 300.0f); };
-  const float whole = tile * stage((float)n);
-  float best = whole;
-  int cut = 0;
-#pragma unroll 1
-  for (int s = 2; s <= 8; ++s) {
-    const int busy = min(min(n * s, pairs), rest);
-    const float t = tile * (float)n / (float)busy * stage((float)busy) + r * (36.0f + 20.0f * ((float)busy / (float)n + (n * s > pairs ? 1.0f : 0.0f))) + 4000.0f;
-    if (t < best) { best = t; cut = busy; }
-    if (n * s >= pairs) break;
-  }
-  return cut;
+  const float r = (float)max(rows, 16), steps = (float)(rest * kSpc<KIND>);   // stages of all of them
+  const int s = lane + 1, busy = min(min(n * s, pairs), rest);
+  const float stage = fmaxf(fmaxf(2.0f * r, 700.0f * (float)busy / (float)pairs), 300.0f);
+  float t = __fdividef(steps, (float)busy) * stage;
+  if (s > 1) t += r * (36.0f + 20.0f * (__fdividef((float)busy, (float)n) + (n * s > pairs ? 1.0f : 0.0f))) + 4000.0f;
+  if (s > 8 || n * (s - 1) >= pairs) t = 3.0e38f;
+  // the least time, with the fewest parts
+  uint32_t best = (__float_as_uint(t) & ~31u) | (uint32_t)lane;
+#pragma unroll
+  for (int d = 16; d; d /= 2) best = min(best, __shfl_xor_sync(0xFFFFFFFFu, best, d));
+  const int parts = (int)(best & 31u) + 1;
+  return parts == 1 ? 0 : min(min(n * parts, pairs), rest);
 }
 
 __device__ __forceinline__ void walk_begin(const Bars& b, Walk& w) {
@@ -236,6 +249,31 @@ __device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
       ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(leader_bar)
       : "memory");
+}
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_4d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t leader_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(leader_bar)
+      : "memory");
+}
+// n blocks of 64 columns and 64 rows, from column `col` and row `k` of matrix e: one copy where the map has blocks as a
+// dimension of their own (and the box both of them).
+__device__ __forceinline__ void load_columns(uint32_t dst, const CUtensorMap* map, bool blocks, int n, int col, int k, int e, uint32_t bar, bool own) {
+  if (blocks) {
+    if (own) tma_4d(dst, map, 0, k, col >> 6, e, bar);
+    else tma_4d_pair(dst, map, 0, k, col >> 6, e, bar);
+  } else {
+    for (int h = 0; h < n; ++h) {
+      if (own) tma_3d(dst + h * 8192, map, col + 64 * h, k, e, bar);
+      else tma_3d_pair(dst + h * 8192, map, col + 64 * h, k, e, bar);
+    }
+  }
 }
 __device__ __forceinline__ void arrive_release_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
@@ -331,16 +369,24 @@ __device__ __forceinline__ void sts32(uint32_t at, uint32_t v) { asm volatile("s
 __device__ __forceinline__ void lds128(uint32_t at, uint4& v) {
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
 }
-// Where a chunk has the 4 scales `word` of row r: per word blocks of 128 rows, in which row r is at (r % 32) * 4 + r / 32.
-__device__ __forceinline__ uint32_t scales_at(uint32_t base, uint32_t word_stride, int r, int word) {
-  return base + word * word_stride + (r >> 7) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4;
+__device__ __forceinline__ void sts128(uint32_t at, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool read) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(read ? 4 : 0) : "memory");
+// 16 bytes of a row's scales, of which `left` >= 1 are there; `align`: what the address is a multiple of (and the row's length).
+__device__ __forceinline__ void load16(uint4& v, const uint8_t* at, int left, int align) {
+  if (align == 16) {
+    v = __ldg(reinterpret_cast<const uint4*>(at));
+  } else if (align == 8) {
+    const uint2 a = __ldg(reinterpret_cast<const uint2*>(at));
+    const uint2 b = left > 8 ? __ldg(reinterpret_cast<const uint2*>(at) + 1) : make_uint2(0, 0);
+    v = make_uint4(a.x, a.y, b.x, b.y);
+  } else {
+    v.x = load4_any(at, left);
+    v.y = left > 4 ? load4_any(at + 4, left - 4) : 0u;
+    v.z = left > 8 ? load4_any(at + 8, left - 8) : 0u;
+    v.w = left > 12 ? load4_any(at + 12, left - 12) : 0u;
+  }
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -382,7 +428,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
   constexpr int kSb = KIND == Kind::Mx ? 8 : 16;   // bytes of scales per row and stage
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t stage_bytes = kStageA + (uint32_t)p.NT * 64u;
+  const uint32_t stage_bytes = kStageA + (uint32_t)p.b_bytes;
   unsigned char* ring_sf = smem + (size_t)p.stages * stage_bytes;
   const uint32_t sf_bytes = kSf ? 4096u + (uint32_t)p.sfb_chunk : 0u;
   unsigned char* staging = ring_sf + kSfSlots * sf_bytes;
@@ -414,32 +460,31 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
     }
     const int per = (p.E + 31) / 32, lo = min(p.E, lane * per), hi = min(p.E, lo + per);
     bool bad = false;
-    long long rows = 0;
-    auto size_of = [&](int e) -> long long {
+    auto size_of = [&](int e) -> int {
       if (!p.sizes) return p.T;
-      const long long n = p.size_bytes == 8 ? static_cast<const long long*>(p.sizes)[e] : static_cast<const int*>(p.sizes)[e];
+      const long long n = p.size_bytes == 8 ? __ldg(static_cast<const long long*>(p.sizes) + e) : (long long)__ldg(static_cast<const int*>(p.sizes) + e);
       bad |= n < 0 || n > p.T;
-      return n < 0 ? 0 : (n > p.T ? p.T : n);
+      return n < 0 ? 0 : (n > p.T ? p.T : (int)n);
     };
-    for (int e = lo; e < hi; ++e) rows += size_of(e);
-    long long before = rows;
+    auto add = [&](int a, int b) { bad |= a + b > p.T; return min(a + b, p.T); };   // (T is at most 2^30)
+    int at = 0;
+    for (int e = lo; e < hi; ++e) at = add(at, size_of(e));
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-      const long long v = __shfl_up_sync(0xFFFFFFFFu, before, d);
-      if (lane >= d) before += v;
+      const int v = __shfl_up_sync(0xFFFFFFFFu, at, d);
+      if (lane >= d) at = add(at, v);
     }
-    before -= rows;
-    bad |= before + rows > p.T;
+    const int rows_end = __shfl_sync(0xFFFFFFFFu, at, 31);
+    at = __shfl_up_sync(0xFFFFFFFFu, at, 1);
+    if (lane == 0) at = 0;
     int units = 0, steps = 0;
-    long long at = before;
     for (int e = lo; e < hi; ++e) {
-      const int r0 = (int)min(at, (long long)p.T);
-      at += size_of(e);
-      const int len = (int)min(at, (long long)p.T) - r0;
-      const int2 tr = tiles_j<KIND>(p, len);
+      const int r0 = at;
+      at = add(at, size_of(e));
+      const int2 tr = tiles_j<KIND>(p, at - r0);
       tab[e] = make_int4(r0, units, steps, tr.y << 9 | tr.x);
       units += tr.y * p.i_tiles;
-      steps += tr.y * p.i_tiles * group_steps<KIND>(p, len);
+      steps += tr.y * p.i_tiles * group_steps<KIND>(p, at - r0);
     }
     int u0 = units, s0 = steps;
 #pragma unroll
@@ -451,22 +496,19 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
     u0 -= units;
     s0 -= steps;
     for (int e = lo; e < hi; ++e) { tab[e].y += u0; tab[e].z += s0; }
-    const int rows_end = (int)min(__shfl_sync(0xFFFFFFFFu, at, 31), (long long)p.T);
     bad = __any_sync(0xFFFFFFFFu, bad);
+    if (lane == 0) tab[p.E] = make_int4(rows_end, total, all_steps, 0);
     __syncwarp();
+    const int pairs = gridDim.x >> 1, full = (int)((uint32_t)total / (uint32_t)pairs) * pairs;
+    int cut_pairs = 0, base = 0, rest = 0;
+    if (full < total) {
+      int e = 0, h = p.E;   // the group in which the rest begins
+      while (h - e > 1) { const int m = (e + h) >> 1; if (tab[m].y <= full) e = m; else h = m; }
+      base = tab[e].z + (full - tab[e].y) * group_steps<KIND>(p, tab[e + 1].x - tab[e].x);
+      rest = all_steps - base;
+      cut_pairs = cut_for<KIND>(lane, total - full, rest, KIND == Kind::MM ? p.NT : (int)__fdividef((float)rows_end * (float)p.i_tiles, (float)total), pairs);
+    }
     if (lane == 0) {
-      tab[p.E] = make_int4(rows_end, total, all_steps, 0);
-      const int pairs = gridDim.x >> 1;
-      const int full = (int)((uint32_t)total / (uint32_t)pairs) * pairs;
-      int cut_pairs = 0, base = 0, rest = 0;
-      if (full < total) {
-        int e = 0, h = p.E;   // the group in which the rest begins
-        while (h - e > 1) { const int m = (e + h) >> 1; if (tab[m].y <= full) e = m; else h = m; }
-        const int x1 = tab[e + 1].x;
-        base = tab[e].z + (full - tab[e].y) * group_steps<KIND>(p, x1 - tab[e].x);
-        rest = all_steps - base;
-        cut_pairs = cut_for<KIND>(p, total - full, rest, KIND == Kind::MM ? p.NT : (int)__fdividef((float)rows_end * (float)p.i_tiles, (float)total), pairs);
-      }
       bars->rows = rows_end;
       bars->full_units = cut_pairs ? full : total;
       bars->cut_pairs = cut_pairs;
@@ -493,77 +535,47 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
     return __shfl_sync(0xFFFFFFFFu, more, 0);
   };
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ operands
+  if (warp == 0 || warp == 3) {
+    // ------------------------------------------------------------ operands: a warp for each
+    if (kSf && warp == 3) asm volatile("griddepcontrol.wait;" ::: "memory");   // 4 bits: the kernel that quantizes b may still be running
     if (elect_one()) {
+      const bool of_a = warp == 0;
       const uint32_t full = smem_u32(&bars->full[0]), lfull = leader_addr(full), empty = smem_u32(&bars->empty[0]), landed = smem_u32(&bars->landed[0]);
       uint32_t s = 0, ph = 1;
       bool ok = true;
-      bool begun = !kSf;
       while (ok && walk_next<KIND>(p, *bars, tab, walk)) {
         const Piece c = walk.c;
-        auto load_a = [&](int ks) {
-          const uint32_t a = ring + s * stage_bytes, bar = lfull + s * 8;
-          const int k = ks * (kSf ? 128 : 64);
-          if (rank == 0) mbar_expect_tx(full + s * 8, 2 * kStageA + (uint32_t)c.neff * 128u);
-          if constexpr (KIND == Kind::MK) {
-  #pragma unroll
-            for (int h = 0; h < 2; ++h) tma_3d_pair(a + h * 8192, &maps.a, c.i0 + rank * kLanes + 64 * h, k, c.e, bar);
-          } else {
-            tma_3d_pair(a, &maps.a, k, c.i0 + rank * kLanes, c.e, bar);
-          }
-        };
-        auto load_b = [&](int ks, uint32_t slot) {
-          const uint32_t b = ring + slot * stage_bytes + kStageA, bar = lfull + slot * 8;
-          const int k = ks * (kSf ? 128 : 64), half = c.neff >> 1, row = c.row0 + rank * half;
-          int r = 0;
-  #pragma unroll
-          for (int i = 0; i < 5; ++i) {
-            const int box = 128 >> i;
-            if (half & box) {
-              tma_3d_pair(b + r * 128, &maps.b[i], k, row + r, 0, bar);
-              r += box;
-            }
-          }
-        };
-        int ks = c.ks0;
-        if (!begun) {
-          // 4 bits: the kernel that quantizes b may still be running.  The first stages' weights are requested before it is
-          // waited for.
-          begun = true;
-          const int n = min(p.stages, c.ks1 - c.ks0);
-          for (; ks < c.ks0 + n; ++ks, ++s) load_a(ks);
-          asm volatile("griddepcontrol.wait;" ::: "memory");
-          for (int i = 0; i < n; ++i) load_b(c.ks0 + i, (uint32_t)i);
-          if (s == (uint32_t)p.stages) { s = 0; ph ^= 1; }
-        }
-        for (; ks < c.ks1; ++ks) {
+        const int half = c.neff >> 1, i = c.i0 + rank * kLanes, j = c.row0 + rank * half;
+        int box0 = 0;
+        const int rows = kSum ? half : box_rows(half, &box0);
+        const uint32_t bytes = kStageA + (uint32_t)rows * 128u;
+        for (int ks = c.ks0; ks < c.ks1; ++ks) {
           if (!wait_local(empty + s * 8, ph, abort_flag)) { ok = false; break; }
+          const uint32_t at = ring + s * stage_bytes + (of_a ? 0 : kStageA);
+          // A group's last stage (MM) is counted by this block, for the warp that zeroes foreign rows; any other by the pair's leader.
+          const bool ends = kSum && c.len - ks * 64 < 64;
+          const uint32_t bar = (ends ? landed : lfull) + s * 8;
+          if (of_a) {
+            if (ends) mbar_expect_tx(bar, bytes);
+            else if (rank == 0) mbar_expect_tx(full + s * 8, 2 * bytes);
+          }
           if constexpr (kSum) {
-            const uint32_t a = ring + s * stage_bytes, b = a + kStageA;
-            const int t = c.t0 + ks * 64, half = c.neff >> 1, i = c.i0 + rank * kLanes, j = c.row0 + rank * half;
-            if (c.len - ks * 64 >= 64) {
-              const uint32_t bar = lfull + s * 8;
-              if (rank == 0) mbar_expect_tx(full + s * 8, 2 * kStageA + (uint32_t)c.neff * 128u);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) tma_3d_pair(a + h * 8192, &maps.a, i + 64 * h, t, 0, bar);
-              for (int h = 0; h < half / 64; ++h) tma_3d_pair(b + h * 8192, &maps.b[0], j + 64 * h, t, 0, bar);
-            } else {
-              const uint32_t bar = landed + s * 8;
-              mbar_expect_tx(bar, kStageA + (uint32_t)half * 128u);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) tma_3d(a + h * 8192, &maps.a, i + 64 * h, t, 0, bar);
-              for (int h = 0; h < half / 64; ++h) tma_3d(b + h * 8192, &maps.b[0], j + 64 * h, t, 0, bar);
-            }
+            const CUtensorMap* map = of_a ? &maps.a : &maps.b[0];
+            const int col = of_a ? i : j, n = of_a ? 2 : half / 64, t = c.t0 + ks * 64;
+            load_columns(at, map, p.blocks & (of_a ? 1 : 2), n, col, t, 0, bar, ends);
+          } else if (of_a) {
+            if constexpr (KIND == Kind::MK) load_columns(at, &maps.a, p.blocks & 1, 2, i, ks * 64, c.e, bar, false);
+            else tma_3d_pair(at, &maps.a, ks * (kSf ? 128 : 64), i, c.e, bar);
           } else {
-            load_a(ks);
-            load_b(ks, s);
+            const int k = ks * (kSf ? 128 : 64);
+            const CUtensorMap* map = &maps.b[4 - (31 - __clz(box0 >> 3))];
+            tma_3d_pair(at, map, k, j, 0, bar);
+            if (rows > box0) tma_3d_pair(at + box0 * 128, &maps.b[4 - (31 - __clz((rows - box0) >> 3))], k, j + box0, 0, bar);
           }
           if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; }
         }
       }
-      if (!begun) asm volatile("griddepcontrol.wait;" ::: "memory");   // no block ends before that kernel has
-      if (!ok) for (int i = 0; i < 100; ++i) __nanosleep(1000);   // copies in flight land before the block ends
+      if (!ok) for (int n = 0; n < 100; ++n) __nanosleep(1000);   // copies in flight land before the block ends
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMAs (leader)
@@ -613,8 +625,10 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
             }
           } else {
             const int a_step = KIND == Kind::KK ? 2 : 128, b_step = kSum ? 128 : 2;
+            const int slices = ends ? max(1, (c.len - ks * 64 + 15) >> 4) : 4;   // of 16 k that hold any of the group's rows
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) tcgen05_mma_ss(acc, da + a_step * kk, db + b_step * kk, idesc, kk ? 1u : first);
+            for (int kk = 0; kk < 4; ++kk)
+              if (!kSum || kk < slices) tcgen05_mma_ss(acc, da + a_step * kk, db + b_step * kk, idesc, kk ? 1u : first);
           }
           first = 1;
           ++n_stage;
@@ -637,9 +651,9 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       if (!__all_sync(0xFFFFFFFFu, wait_local(landed + s * 8, (ph >> s) & 1, abort_flag))) break;
       ph ^= 1u << s;
       const int blocks = 2 + (c.neff >> 7);   // of 64 columns: two of a, one or two of b
-      const uint32_t tile = ring + s * stage_bytes;
+      const uint32_t tile = ring + s * stage_bytes, zero_end = max(16, (valid + 15) & ~15) * 128;   // the slice of 16 that it ends in
       for (int h = 0; h < blocks; ++h)
-        for (uint32_t o = max(valid, 0) * 128 + lane * 16; o < 8192; o += 512)
+        for (uint32_t o = max(valid, 0) * 128 + lane * 16; o < zero_end; o += 512)
           asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(tile + h * 8192 + o), "r"(0u) : "memory");
       fence_async_smem();
       __syncwarp();
@@ -648,63 +662,113 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
   } else if (kSf && warp >= kScaleWarp0) {
     // ------------------------------------------------------------ scales: an operand's two warps take chunks in turn
     const bool of_b = warp >= kScaleWarp0 + kScaleWarps;
-    const uint32_t mine = warp & 1, lsf = leader_addr(smem_u32(&bars->sf_full[0])), sf_empty = smem_u32(&bars->sf_empty[0]);
-    const uint32_t stride = of_b ? p.sfb_chunk / 8 : 512, base = smem_u32(ring_sf) + (of_b ? 4096 : 0);
-    const int word = lane & 7, r0 = lane >> 3;   // a lane has 4 of a row's 32 bytes
-    uint32_t chunk = 0, oldest = mine, pending = 0;
-    // The oldest chunk on its way is there: the tensor core may read it.
-    auto finish = [&]() {
+    const uint32_t lsf = leader_addr(smem_u32(&bars->sf_full[0])), sf_empty = smem_u32(&bars->sf_empty[0]);
+    const uint32_t base = smem_u32(ring_sf) + (of_b ? 4096 : 0);
+    const int blocks = p.sfb_chunk >> 12;   // of 128 rows of b: 1 or 2
+    uint32_t chunk = 0;                     // of the next one to be stored
+    bool ok = true;
+    // Scales are read before their slot is free, and stored after.
+    auto slot = [&](uint32_t n) -> uint32_t {
+      const uint32_t sl = n % kSfSlots;
+      ok = __all_sync(0xFFFFFFFFu, wait_local(sf_empty + sl * 8, (n / kSfSlots & 1) ^ 1, abort_flag));
+      return base + sl * sf_bytes;
+    };
+    auto stored = [&](uint32_t n) {
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) arrive_release_cluster(lsf + oldest % kSfSlots * 8);
-      oldest += kScaleWarps;
-      --pending;
+      if (lane == 0) arrive_release_cluster(lsf + n % kSfSlots * 8);
     };
-    bool ok = true;
-    if (of_b) asm volatile("griddepcontrol.wait;" ::: "memory");
-    while (ok && next_of_warp()) {
-      const Piece c = walk.c;
-      for (int ks = c.ks0; ks < c.ks1; ks += kSpc<KIND>, ++chunk) {
-        if ((chunk & (kScaleWarps - 1)) != mine) continue;
-        const uint32_t sl = chunk % kSfSlots, ph = (chunk / kSfSlots & 1) ^ 1, at = base + sl * sf_bytes;
-        if (pending && !__all_sync(0xFFFFFFFFu, mbar_test(sf_empty + sl * 8, ph))) {
-          // nobody waits for a slot while others wait for what is on its way
-          if (pending == 2) { cp_async_wait<1>(); finish(); }
-          cp_async_wait<0>();
-          finish();
-        }
-        ok = __all_sync(0xFFFFFFFFu, wait_local(sf_empty + sl * 8, ph, abort_flag));
-        if (!ok) break;
-        const int byte = ks * kSb + 4 * word;
-        if (of_b) {
-          // rows of the tile, 32 at a time (past the end of b: the last row's, for columns that nobody stores)
-          const uint32_t* from = p.sfb + (long long)(ks * kSb / 4) * p.T + c.row0;
-          const int most = p.T - 1 - c.row0;
-          for (int r = lane; r < ((c.neff + 31) & ~31); r += 32) {
-            const uint32_t* of_row = from + min(r, most);
+    if (of_b) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      while (ok && next_of_warp()) {
+        const Piece c = walk.c;
+        for (int ks = c.ks0; ks < c.ks1; ks += kSpc<KIND>, ++chunk) {
+          if ((chunk & (kScaleWarps - 1)) != (uint32_t)(warp & 1)) continue;
+          // a lane has rows lane, lane + 32, .. (past the end of b: the last row, for columns that nobody stores)
+          const uint32_t* from = p.sfb + (long long)(ks * kSb / 4) * p.T;
+          int row[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) cp_async4(scales_at(at, stride, r, k), of_row + (long long)k * p.T, true);
-          }
-        } else {
-          const int n0 = c.i0 + rank * kLanes, rows = p.I - n0, left = p.sf_row - byte;
-          const uint8_t* from = p.sfa + ((long long)c.e * p.I + n0) * p.sf_row + byte;
-          if (p.sfa4) {
-#pragma unroll 8
-            for (int r = r0; r < kLanes; r += 4) {
-              const bool in = r < rows && left > 0;
-              cp_async4(scales_at(at, 512, r, word), in ? from + (long long)r * p.sf_row : p.sfa, in);
+          for (int r = 0; r < 8; ++r) row[r] = min(c.row0 + lane + 32 * r, p.T - 1);
+          uint4 v[2][8];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (128 * h >= c.neff) break;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t* w = from + (long long)k * p.T;
+              v[h][k].x = __ldcg(w + row[4 * h]);
+              if (128 * h + 32 < c.neff) v[h][k].y = __ldcg(w + row[4 * h + 1]);
+              if (128 * h + 64 < c.neff) v[h][k].z = __ldcg(w + row[4 * h + 2]);
+              if (128 * h + 96 < c.neff) v[h][k].w = __ldcg(w + row[4 * h + 3]);
             }
-          } else {
-#pragma unroll 8
-            for (int r = r0; r < kLanes; r += 4)
-              sts32(scales_at(at, 512, r, word), r < rows && left > 0 ? load4_any(from + (long long)r * p.sf_row, left) : 0u);
           }
+          const uint32_t at = slot(chunk);
+          if (!ok) break;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (128 * h >= c.neff) break;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sts128(at + (k * blocks + h) * 512 + lane * 16, v[h][k]);
+          }
+          stored(chunk);
         }
-        cp_async_commit();
-        if (++pending == 2) { cp_async_wait<1>(); finish(); }
+      }
+    } else {
+      // Two chunks of each warp are on their way at a time: they come from HBM.
+      const int half = lane & 1, r0 = lane >> 1;   // a lane has 16 of a row's 32 bytes
+      Piece c;
+      int ks = 0;
+      uint32_t ahead = 0;   // of the next chunk to be read
+      bool more = next_of_warp();
+      if (more) { c = walk.c; ks = c.ks0; }
+      auto advance = [&]() {
+        ++ahead;
+        ks += kSpc<KIND>;
+        if (ks < c.ks1) return;
+        more = next_of_warp();
+        if (more) { c = walk.c; ks = c.ks0; }
+      };
+      // Reads this warp's next chunk; false: there is none.
+      auto read = [&](uint4 (&v)[kLanes / 16]) -> bool {
+        while (more && (ahead & (kScaleWarps - 1)) != (uint32_t)(warp & 1)) advance();
+        if (!more) return false;
+        const int n0 = c.i0 + rank * kLanes, byte = ks * kSb + 16 * half, left = p.sf_row - byte;
+        const uint8_t* from = p.sfa + ((long long)c.e * p.I + n0) * p.sf_row + byte;
+#pragma unroll
+        for (int i = 0; i < kLanes / 16; ++i) {
+          const int r = r0 + 16 * i;
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (n0 + r < p.I && left > 0) load16(v[i], from + (long long)r * p.sf_row, left, p.sfa_align);
+        }
+        advance();
+        return true;
+      };
+      auto store = [&](const uint4 (&v)[kLanes / 16]) {
+        const uint32_t at = slot(chunk);
+        if (!ok) return;
+#pragma unroll
+        for (int i = 0; i < kLanes / 16; ++i) {
+          const int r = r0 + 16 * i;
+          const uint32_t to = at + half * 2048 + (r & 31) * 16 + (r >> 5) * 4;
+          sts32(to, v[i].x);
+          sts32(to + 512, v[i].y);
+          sts32(to + 1024, v[i].z);
+          sts32(to + 1536, v[i].w);
+        }
+        stored(chunk);
+        chunk += kScaleWarps;
+      };
+      chunk = warp & 1;
+      uint4 v0[kLanes / 16], v1[kLanes / 16];
+      bool h0 = read(v0);
+      while (ok && h0) {
+        const bool h1 = read(v1);
+        store(v0);
+        if (!ok || !h1) break;
+        h0 = read(v0);
+        store(v1);
       }
     }
-    if (pending) { cp_async_wait<0>(); finish(); }
   } else if (warp >= kEpiWarp0 && warp < kEpiWarp0 + kEpiWarps) {
     // ------------------------------------------------------------ epilogue
     const int w = warp - kEpiWarp0, quad = warp & 3, chalf = w >> 2;
@@ -805,52 +869,55 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
           const uint32_t get = stg + (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
           const int i = i_warp + (lane & 3) * 8;
           T* dst = out_row<T, KIND>(p, c, 32 * p0 + (lane >> 2)) + i;
-          uint32_t r0[2][16], r1[2][16];
-          auto load = [&](int q, uint32_t (&v)[2][16]) {
-            load_16(acc + 32 * q, v[0]);
-            if (32 * q + 16 < c.neff) load_16(acc + 32 * q + 16, v[1]);
-          };
-          auto piece = [&](int q, uint32_t (&v)[2][16]) {
+          // Rounded and packed first, so that the accumulator is free for another tile's MMAs before (most of) it is stored.
+          // (4 bits: half at a time, for lack of registers)
+          constexpr int kBatch = kSf ? 2 : 4;
+          if (p0 == p1) release();
+          for (int b0 = p0; b0 < p1; b0 += kBatch) {
+            uint32_t packed[kBatch][2][8];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (h == 1 && 32 * q + 16 >= c.neff) break;
-              // 16 rows of 64 bytes, 16-byte chunks xor-ed with row / 2
-              auto f = [&](int k) { return __uint_as_float(v[h][k]) * alpha; };
+            for (int q = 0; q < kBatch; ++q) {
+              if (b0 + q >= p1) break;
+              const int col = 32 * (b0 + q);
+              const bool two = col + 16 < c.neff;
+              uint32_t v[2][16];
+              load_16(acc + col, v[0]);
+              if (two) load_16(acc + col + 16, v[1]);
+              tcgen05_wait_ld16(v[0]);
+              tcgen05_wait_ld16(v[1]);
 #pragma unroll
-              for (int x = 0; x < 2; ++x)
-                stmatrix_x4_trans(put + h * 1024 + x * 512, pack2<T>(f(4 * x), f(4 * x + 1)), pack2<T>(f(4 * x + 2), f(4 * x + 3)),
-                                  pack2<T>(f(8 + 4 * x), f(8 + 4 * x + 1)), pack2<T>(f(8 + 4 * x + 2), f(8 + 4 * x + 3)));
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  packed[q][h][k] = pack2<T>(__uint_as_float(v[h][2 * k]) * alpha, __uint_as_float(v[h][2 * k + 1]) * alpha);
             }
-            __syncwarp();
-            if (i < p.I) {   // (whole chunks: rows on 16-byte boundaries are whole eights long)
-              const int n = c.rows - 32 * q - (lane >> 2);
+            if (b0 + kBatch >= p1) release();
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                uint4 o;
-                lds128(get + k * 512, o);
-                if (8 * k < n) *reinterpret_cast<uint4*>(dst + (long long)(8 * k) * p.I) = o;
+            for (int q = 0; q < kBatch; ++q) {
+              if (b0 + q >= p1) break;
+              const int col = 32 * (b0 + q);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if (h == 1 && col + 16 >= c.neff) break;
+                // 16 rows of 64 bytes, 16-byte chunks xor-ed with row / 2
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                  stmatrix_x4_trans(put + h * 1024 + x * 512, packed[q][h][2 * x], packed[q][h][2 * x + 1], packed[q][h][4 + 2 * x], packed[q][h][5 + 2 * x]);
               }
-            }
-            dst += (long long)32 * p.I;
-            __syncwarp();
-          };
-          // the next piece is on its way while one is stored
-          if (p0 < p1) load(p0, r0);
-          for (int q = p0; q < p1; q += 2) {
-            tcgen05_wait_ld16(r0[0]);
-            tcgen05_wait_ld16(r0[1]);
-            if (q + 1 < p1) load(q + 1, r1);
-            else release();
-            piece(q, r0);
-            if (q + 1 < p1) {
-              tcgen05_wait_ld16(r1[0]);
-              tcgen05_wait_ld16(r1[1]);
-              if (q + 2 < p1) load(q + 2, r0);
-              else release();
-              piece(q + 1, r1);
+              __syncwarp();
+              if (i < p.I) {   // (whole chunks: rows on 16-byte boundaries are whole eights long)
+                const int n = c.rows - col - (lane >> 2);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  uint4 o;
+                  lds128(get + k * 512, o);
+                  if (8 * k < n) *reinterpret_cast<uint4*>(dst + (long long)(8 * k) * p.I) = o;
+                }
+              }
+              dst += (long long)32 * p.I;
+              __syncwarp();
             }
           }
-          if (p0 == p1) release();
           continue;
         }
       }
@@ -911,14 +978,16 @@ int sm_pairs() {
   return cached[dev];
 }
 
-// Rows of `cols` elements (bytes where esize is 1), `mid` of them per matrix; boxes of `box0` x `box1`.
-int encode(CUtensorMap* m, int dtype, int esize, const void* base, int64_t cols, int64_t pitch, int64_t mid, int64_t outer, int box0, int box1) {
-  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)mid, (cuuint64_t)outer};
-  const cuuint64_t strides[2] = {(cuuint64_t)pitch, (cuuint64_t)pitch * mid};
-  const cuuint32_t box[3] = {(cuuint32_t)box0, (cuuint32_t)box1, 1}, one[3] = {1, 1, 1};
+// Rows of `cols` elements (bytes where esize is 1), `mid` of them per matrix; boxes of `box0` x `box1`.  `blocks`: columns as
+// two dimensions, blocks of 64 and their number, of which a box has `blocks`.
+int encode(CUtensorMap* m, int dtype, int esize, const void* base, int64_t cols, int64_t pitch, int64_t mid, int64_t outer, int box0, int box1,
+           int blocks = 0) {
+  const cuuint64_t dims[4] = {(cuuint64_t)(blocks ? 64 : cols), (cuuint64_t)mid, (cuuint64_t)(blocks ? cols / 64 : outer), (cuuint64_t)outer};
+  const cuuint64_t strides[3] = {(cuuint64_t)pitch, (cuuint64_t)(blocks ? 128 : pitch * mid), (cuuint64_t)pitch * mid};
+  const cuuint32_t box[4] = {(cuuint32_t)box0, (cuuint32_t)box1, (cuuint32_t)(blocks ? blocks : 1), 1}, one[4] = {1, 1, 1, 1};
   const CUtensorMapDataType t = esize == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                 : dtype == B200Q_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const CUresult r = encode_fn()(m, t, 3, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const CUresult r = encode_fn()(m, t, blocks ? 4 : 3, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? B200Q_OK : fail(B200Q_ERR_CUDA, "[grouped product] a tensor map could not be encoded (%d)", (int)r);
 }
@@ -940,7 +1009,7 @@ int allow_smem(const void* kernel) {
 
 template <typename T, Kind KIND>
 int launch(const Maps& m, Params& p, cudaStream_t st) {
-  const size_t stage = kStageA + (size_t)p.NT * 64;
+  const size_t stage = kStageA + (size_t)p.b_bytes;
   const size_t fixed = 1024 + (kFp4<KIND> ? kSfSlots * (4096 + (size_t)p.sfb_chunk) : 0) + (sizeof(T) == 2 ? kEpiWarps * kStageOut : 0) +
                        sizeof(Bars) + (size_t)(p.E + 1) * sizeof(Group);
   p.stages = (int)((kSmemMax - fixed) / stage);
@@ -1002,25 +1071,30 @@ int grouped_tc(const GroupedTcArgs& a, cudaStream_t st) {
   p.status = a.status;
   p.sfb_chunk = p.NT > 128 ? 8192 : 4096;
   p.sfa = a.sfa; p.sfb = a.sfb; p.sf_row = (int)a.sf_row;
-  p.sfa4 = ((reinterpret_cast<uintptr_t>(a.sfa) | (uintptr_t)a.sf_row) & 3) == 0;
+  const uintptr_t sf_at = reinterpret_cast<uintptr_t>(a.sfa) | (uintptr_t)a.sf_row;
+  p.sfa_align = (sf_at & 15) == 0 ? 16 : ((sf_at & 7) == 0 ? 8 : 1);
   p.ga = a.ga; p.gb = a.gb; p.ga_each = a.ga_each;
+  if (a.T > (1 << 30) || a.J > (1 << 30))
+    return fail(B200Q_ERR_UNSUPPORTED, "[grouped product] No implementation for problem shape: more than 2^30 rows");
   // number of tiles and steps in 32 bits
   const int64_t tiles = ((sum ? (a.J + p.NT - 1) / p.NT * a.E : a.T / p.NT + a.E + 1)) * p.i_tiles;
   const int64_t steps = sum ? (a.T / 64 + 2 * a.E) * ((a.J + p.NT - 1) / p.NT) * p.i_tiles : tiles * ((a.K + 63) / 64);
   if (tiles >= INT32_MAX || steps >= INT32_MAX)
     return fail(B200Q_ERR_UNSUPPORTED, "[grouped product] No implementation for problem shape: too many tiles");
-  const int e_a = fp4 ? 1 : 2;
+  const int es_a = fp4 ? 1 : 2;
   const int64_t ka = fp4 ? a.K / 2 : a.K;
-  int rc = B200Q_OK;
+  int box0 = 0, rc = B200Q_OK;
+  p.b_bytes = (sum ? p.NT / 2 : box_rows(p.NT / 2, &box0)) * 128;
+  p.blocks = (a.form != GroupedForm::KK && !fp4 && a.I % 64 == 0 ? 1 : 0) | (sum && a.J % 256 == 0 ? 2 : 0);
   if (sum) {
-    rc = encode(&m.a, a.dtype, 2, a.a, a.I, a.a_pitch, a.T, 1, 64, 64);
-    if (!rc) rc = encode(&m.b[0], a.dtype, 2, a.b, a.J, a.b_pitch, a.T, 1, 64, 64);
+    rc = encode(&m.a, a.dtype, 2, a.a, a.I, a.a_pitch, a.T, 1, 64, 64, p.blocks & 1 ? 2 : 0);
+    if (!rc) rc = encode(&m.b[0], a.dtype, 2, a.b, a.J, a.b_pitch, a.T, 1, 64, 64, p.blocks & 2 ? 2 : 0);
   } else {
     const int box = fp4 ? 128 : 64;
-    if (a.form == GroupedForm::MK) rc = encode(&m.a, a.dtype, 2, a.a, a.I, a.a_pitch, a.K, a.E, 64, 64);
-    else rc = encode(&m.a, a.dtype, e_a, a.a, ka, a.a_pitch, a.I, a.E, box, kLanes);
+    if (a.form == GroupedForm::MK) rc = encode(&m.a, a.dtype, 2, a.a, a.I, a.a_pitch, a.K, a.E, 64, 64, p.blocks & 1 ? 2 : 0);
+    else rc = encode(&m.a, a.dtype, es_a, a.a, ka, a.a_pitch, a.I, a.E, box, kLanes);
     for (int i = 0; i < 5 && !rc; ++i)
-      if ((128 >> i) <= p.NT / 2) rc = encode(&m.b[i], a.dtype, e_a, a.b, ka, a.b_pitch, a.T, 1, box, 128 >> i);
+      if ((128 >> i) <= p.b_bytes / 128) rc = encode(&m.b[i], a.dtype, es_a, a.b, ka, a.b_pitch, a.T, 1, box, 128 >> i);
   }
   if (rc) return rc;
   switch (a.form) {
