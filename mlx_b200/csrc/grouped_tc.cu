@@ -12,8 +12,8 @@
 //
 //   warps 0, 3  TMA: a's and b's tile of a stage (128 bytes of k per row; MM and MK: 64 k)
 //   warp 1      tcgen05.mma, and for 4 bits tcgen05.cp of the stage's scales (leader block, one thread)
-//   warp 2      MM only: the stage that a group ends in has its foreign rows zeroed in shared memory (both operands: a foreign
-//               infinity times zero would be NaN).  Only those stages go through this warp: with all of them handed on by it
+//   warp 2      4 bits: hands the scales in shared memory to the tensor core.  MM: the stage that a group ends in has its foreign rows zeroed in shared memory (both operands: a foreign
+//               infinity times zero would be NaN); only those stages go through this warp: with all of them handed on by it
 //               a step of the ring took 1600 cycles instead of 700
 //   warps 4-11  epilogue: accumulator -> rounding -> stmatrix staging -> 16-byte stores
 //   warps 12-15 4 bits only: scales from global memory (row-major, a's at any alignment) into the order that tensor memory
@@ -120,6 +120,7 @@ struct __align__(16) Walk {
 struct __align__(16) Bars {
   uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t landed[kMaxStages], fixed[kMaxStages];  // MM, a group's last stage: this block's tiles are there; and without foreign rows, in both
+  uint64_t sf_stored[kSfSlots];                    // this block's scales of both operands are in shared memory
   uint64_t sf_full[kSfSlots], sf_empty[kSfSlots];
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem_base;
@@ -444,7 +445,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       mbar_init(smem_u32(&bars->empty[lane]), 1);
       if (kSum) { mbar_init(smem_u32(&bars->landed[lane]), 1); mbar_init(smem_u32(&bars->fixed[lane]), 2); }
     }
-    if (lane < kSfSlots) { mbar_init(smem_u32(&bars->sf_full[lane]), 4); mbar_init(smem_u32(&bars->sf_empty[lane]), 1); }
+    if (lane < kSfSlots) { mbar_init(smem_u32(&bars->sf_stored[lane]), 2); mbar_init(smem_u32(&bars->sf_full[lane]), 2); mbar_init(smem_u32(&bars->sf_empty[lane]), 1); }
     if (lane < 2) { mbar_init(smem_u32(&bars->acc_full[lane]), 1); mbar_init(smem_u32(&bars->acc_empty[lane]), 2 * kEpiWarps); }
     if (lane == 0) bars->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -659,10 +660,26 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       __syncwarp();
       if (lane == 0) arrive_release_cluster(lfixed + s * 8);
     }
+  } else if (kSf && warp == 2) {
+    // ------------------------------------------------------------ scales are handed to the tensor core
+    // (The warps that store them have loads on their way, which their own fence would wait for: 2000 cycles a chunk.)
+    if (lane == 0) {
+      const uint32_t sf_stored = smem_u32(&bars->sf_stored[0]), lsf = leader_addr(smem_u32(&bars->sf_full[0]));
+      uint32_t chunk = 0;
+      bool ok = true;
+      while (ok && walk_next<KIND>(p, *bars, tab, walk)) {
+        const int n = (walk.c.ks1 - walk.c.ks0 + kSpc<KIND> - 1) / kSpc<KIND>;
+        for (int i = 0; i < n; ++i, ++chunk) {
+          if (!wait_local(sf_stored + chunk % kSfSlots * 8, chunk / kSfSlots & 1, abort_flag)) { ok = false; break; }
+          fence_async_smem();
+          arrive_release_cluster(lsf + chunk % kSfSlots * 8);
+        }
+      }
+    }
   } else if (kSf && warp >= kScaleWarp0) {
     // ------------------------------------------------------------ scales: an operand's two warps take chunks in turn
     const bool of_b = warp >= kScaleWarp0 + kScaleWarps;
-    const uint32_t lsf = leader_addr(smem_u32(&bars->sf_full[0])), sf_empty = smem_u32(&bars->sf_empty[0]);
+    const uint32_t sf_stored = smem_u32(&bars->sf_stored[0]), sf_empty = smem_u32(&bars->sf_empty[0]);
     const uint32_t base = smem_u32(ring_sf) + (of_b ? 4096 : 0);
     const int blocks = p.sfb_chunk >> 12;   // of 128 rows of b: 1 or 2
     uint32_t chunk = 0;                     // of the next one to be stored
@@ -674,9 +691,8 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       return base + sl * sf_bytes;
     };
     auto stored = [&](uint32_t n) {
-      fence_async_smem();
       __syncwarp();
-      if (lane == 0) arrive_release_cluster(lsf + n % kSfSlots * 8);
+      if (lane == 0) mbar_arrive(sf_stored + n % kSfSlots * 8);
     };
     if (of_b) {
       asm volatile("griddepcontrol.wait;" ::: "memory");
