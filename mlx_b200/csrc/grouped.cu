@@ -61,11 +61,10 @@ int check_ws(const char* tag, const void* ws, size_t have, size_t need) {
 }
 uint32_t* status_word(void* ws, size_t bytes) { return reinterpret_cast<uint32_t*>(static_cast<char*>(ws) + bytes - kStatusBytes); }
 
-// Words of four scales per row of x, a multiple of 8.
-int64_t sf_words(int64_t K, int mode) { return (K / fp4_group(mode) + 31) / 32 * 8; }
-
+size_t sfx_bytes(int64_t T, int64_t K, int mode) { return up((size_t)T * fp4_words(K, mode) * 4); }
+size_t sfw_bytes(int64_t E, int64_t N, int64_t K, int mode) { return up((size_t)E * ((N + 127) / 128) * fp4_words(K, mode) * 512); }
 size_t qqmm_bytes(int64_t T, int64_t E, int64_t N, int64_t K, int mode) {
-  return up(grouped_tc_bytes(T, false)) + up((size_t)T * up16(K / 2)) + up((size_t)T * sf_words(K, mode) * 4) + packed_bytes(E * N, K / 2) + kStatusBytes;
+  return up(grouped_tc_bytes(T, false)) + up((size_t)T * up16(K / 2)) + sfx_bytes(T, K, mode) + sfw_bytes(E, N, K, mode) + packed_bytes(E * N, K / 2) + kStatusBytes;
 }
 size_t grouped_bytes(int64_t T, int64_t E, int64_t N, int64_t K, bool transpose) {
   return up(grouped_tc_bytes(T, false)) + packed_bytes(T, 2 * K) + (transpose ? packed_bytes(E * N, 2 * K) : packed_bytes(E * K, 2 * N)) + kStatusBytes;
@@ -138,10 +137,13 @@ extern "C" int b200q_grouped_qqmm(const void* x, const uint32_t* wq, const uint8
   uint8_t* codes = reinterpret_cast<uint8_t*>(at);
   at += up((size_t)T * up16(K / 2));
   uint32_t* sfx = reinterpret_cast<uint32_t*>(at);
-  at += up((size_t)T * sf_words(K, mode) * 4);
+  at += sfx_bytes(T, K, mode);
+  uint32_t* sfw = reinterpret_cast<uint32_t*>(at);
+  at += sfw_bytes(E, N, K, mode);
   Operand w;
   if (int rc = pack(wq, E * N, K / 2, at, &w, st)) return rc;
-  if (int rc = fp4_quantize_rows(x, dtype, T, K, mode, global_scale_x, codes, up16(K / 2), sfx, sf_words(K, mode), st)) return rc;
+  const Fp4Prepare pr{x, dtype, mode, T, E, N, K, global_scale_x, scales, sizes, size_bytes, codes, up16(K / 2), sfx, sfw};
+  if (int rc = fp4_prepare(pr, st)) return rc;
   GroupedTcArgs a{};
   a.form = mode == B200Q_MXFP4 ? GroupedForm::Mx : GroupedForm::Nv;
   a.a = w.at; a.a_pitch = w.pitch;
@@ -149,8 +151,7 @@ extern "C" int b200q_grouped_qqmm(const void* x, const uint32_t* wq, const uint8
   a.sizes = sizes; a.size_bytes = size_bytes;
   a.out = y; a.dtype = dtype;
   a.T = T; a.E = E; a.I = N; a.K = K;
-  a.sfa = scales; a.sf_row = K / fp4_group(mode);
-  a.sfb = sfx;
+  a.sfa = sfw; a.sfb = sfx; a.sf_words = fp4_words(K, mode);
   a.ga = global_scale_w; a.gb = global_scale_x; a.ga_each = scale_per_group;
   a.ws = ws; a.status = status_word(ws, ws_bytes);
   return grouped_tc(a, st);

@@ -12,12 +12,12 @@
 //
 //   warps 0, 3  TMA: a's and b's tile of a stage (128 bytes of k per row; MM and MK: 64 k)
 //   warp 1      tcgen05.mma, and for 4 bits tcgen05.cp of the stage's scales (leader block, one thread)
-//   warp 2      4 bits: hands the scales in shared memory to the tensor core.  MM: the stage that a group ends in has its foreign rows zeroed in shared memory (both operands: a foreign
-//               infinity times zero would be NaN); only those stages go through this warp: with all of them handed on by it
+//   warp 2      4 bits: TMA of a's scales.  MM: the stage that a group ends in has its foreign rows zeroed in shared memory (both operands: a foreign
+//               infinity times zero would be NaN).  Only those stages go through this warp: with all of them handed on by it
 //               a step of the ring took 1600 cycles instead of 700
 //   warps 4-11  epilogue: accumulator -> rounding -> stmatrix staging -> 16-byte stores
-//   warps 12-15 4 bits only: scales from global memory (row-major, a's at any alignment) into the order that tensor memory
-//               wants, word by word with cp.async, two warps for each operand
+//   warps 12-15 4 bits only: b's scales, from words in global memory into the order that tensor memory wants (a's are in that
+//               order already, fp4_prepare_kernel, and come by TMA: warp 2)
 //
 // The table of groups (first row, first tile, first step) is built in shared memory by every block from `sizes`, which the
 // host never reads: no launch in front and no synchronisation.
@@ -51,9 +51,9 @@ constexpr int kStageA = kLanes * 128;
 constexpr int kMaxStages = 12;
 constexpr int kSfSlots = 4;          // chunks of scales: 32 bytes per row each
 constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
-constexpr int kScaleWarp0 = 12, kScaleWarps = 2;   // of each operand's scales
-constexpr int kMaxWarps = kScaleWarp0 + 2 * kScaleWarps;
-template <Kind K> constexpr int kThreads = 32 * (kFp4<K> ? kScaleWarp0 + 2 * kScaleWarps : kScaleWarp0);
+constexpr int kScaleWarp0 = 12, kScaleWarps = 4;
+constexpr int kMaxWarps = kScaleWarp0 + kScaleWarps;
+template <Kind K> constexpr int kThreads = 32 * (kFp4<K> ? kMaxWarps : kScaleWarp0);
 constexpr int kStageOut = 2048;      // epilogue staging per warp: 32 rows of 64 bytes
 constexpr int kSfColumns = 96;       // two buffers of 16 (a) + 32 (b) columns
 constexpr size_t kSmemMax = 227 * 1024;
@@ -64,6 +64,7 @@ template <Kind K> constexpr int kSpc = K == Kind::Mx ? 4 : (K == Kind::Nv ? 2 : 
 
 struct Maps {
   CUtensorMap a;
+  CUtensorMap sfa;    // 4 bits: a's scales, rows of 1024 bytes
   CUtensorMap b[5];   // boxes of 128, 64, 32, 16 and 8 rows (MM: the first only, 64 x 64)
 };
 
@@ -78,10 +79,8 @@ struct Params {
   int sfb_chunk;           // 4 bits: bytes of a chunk of b's scales
   void* out;
   int vec;                 // rows of the output start on 16-byte boundaries
-  const uint8_t* sfa;      // scales [E * I, sf_row], and words of four of them [.., T]
-  const uint32_t* sfb;
-  int sf_row;
-  int sfa_align;           // rows of sfa start on multiples of 16, of 8, or anywhere (1)
+  const uint32_t* sfb;     // b's scales: words of four [.., T]
+  int sf_words, i_blocks;  // words of a's (and b's) scales per row, a multiple of 8; blocks of 128 i per group
   const float* ga;         // global scales: one, or (ga_each) one per group
   const float* gb;
   int ga_each;
@@ -120,7 +119,6 @@ struct __align__(16) Walk {
 struct __align__(16) Bars {
   uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t landed[kMaxStages], fixed[kMaxStages];  // MM, a group's last stage: this block's tiles are there; and without foreign rows, in both
-  uint64_t sf_stored[kSfSlots];                    // this block's scales of both operands are in shared memory
   uint64_t sf_full[kSfSlots], sf_empty[kSfSlots];
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem_base;
@@ -276,9 +274,6 @@ __device__ __forceinline__ void load_columns(uint32_t dst, const CUtensorMap* ma
     }
   }
 }
-__device__ __forceinline__ void arrive_release_cluster(uint32_t cluster_bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
-}
 // Bounded waits.  try_wait holds the thread back in hardware: a dozen warps that look again and again take issue slots and
 // shared-memory cycles from the tensor core's operands.
 constexpr long long kWaitMost = 1ll << 30;   // cycles, about half a second
@@ -358,37 +353,12 @@ __device__ __forceinline__ uint32_t make_idesc(int n) {
   return shape | (1u << 4) | (fmt << 7) | (fmt << 10) | (KIND != Kind::KK ? 1u << 15 : 0u) | (KIND == Kind::MM ? 1u << 16 : 0u);
 }
 
-// 4 bytes at any address, of which `left` >= 1 are there (and the rest are zeros): from the one or two words that hold them.
-__device__ __forceinline__ uint32_t load4_any(const uint8_t* at, int left) {
-  const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(at) & 3);
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(at - sh);
-  const uint32_t lo = __ldg(w), hi = sh && sh + min(left, 4) > 4 ? __ldg(w + 1) : 0u;
-  const uint32_t v = __funnelshift_r(lo, hi, 8 * sh);
-  return left >= 4 ? v : v & (0xFFFFFFFFu >> (32 - 8 * left));
-}
-__device__ __forceinline__ void sts32(uint32_t at, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
 __device__ __forceinline__ void lds128(uint32_t at, uint4& v) {
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
 }
 __device__ __forceinline__ void sts128(uint32_t at, const uint4& v) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-// 16 bytes of a row's scales, of which `left` >= 1 are there; `align`: what the address is a multiple of (and the row's length).
-__device__ __forceinline__ void load16(uint4& v, const uint8_t* at, int left, int align) {
-  if (align == 16) {
-    v = __ldg(reinterpret_cast<const uint4*>(at));
-  } else if (align == 8) {
-    const uint2 a = __ldg(reinterpret_cast<const uint2*>(at));
-    const uint2 b = left > 8 ? __ldg(reinterpret_cast<const uint2*>(at) + 1) : make_uint2(0, 0);
-    v = make_uint4(a.x, a.y, b.x, b.y);
-  } else {
-    v.x = load4_any(at, left);
-    v.y = left > 4 ? load4_any(at + 4, left - 4) : 0u;
-    v.z = left > 8 ? load4_any(at + 8, left - 8) : 0u;
-    v.w = left > 12 ? load4_any(at + 12, left - 12) : 0u;
-  }
-}
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   uint32_t d;
@@ -445,7 +415,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       mbar_init(smem_u32(&bars->empty[lane]), 1);
       if (kSum) { mbar_init(smem_u32(&bars->landed[lane]), 1); mbar_init(smem_u32(&bars->fixed[lane]), 2); }
     }
-    if (lane < kSfSlots) { mbar_init(smem_u32(&bars->sf_stored[lane]), 2); mbar_init(smem_u32(&bars->sf_full[lane]), 2); mbar_init(smem_u32(&bars->sf_empty[lane]), 1); }
+    if (lane < kSfSlots) { mbar_init(smem_u32(&bars->sf_full[lane]), 3); mbar_init(smem_u32(&bars->sf_empty[lane]), 1); }
     if (lane < 2) { mbar_init(smem_u32(&bars->acc_full[lane]), 1); mbar_init(smem_u32(&bars->acc_empty[lane]), 2 * kEpiWarps); }
     if (lane == 0) bars->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -658,131 +628,71 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
           asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(tile + h * 8192 + o), "r"(0u) : "memory");
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) arrive_release_cluster(lfixed + s * 8);
+      if (lane == 0) mbar_arrive_cluster(lfixed + s * 8);
     }
   } else if (kSf && warp == 2) {
-    // ------------------------------------------------------------ scales are handed to the tensor core
-    // (The warps that store them have loads on their way, which their own fence would wait for: 2000 cycles a chunk.)
-    if (lane == 0) {
-      const uint32_t sf_stored = smem_u32(&bars->sf_stored[0]), lsf = leader_addr(smem_u32(&bars->sf_full[0]));
-      uint32_t chunk = 0;
+    // ------------------------------------------------------------ a's scales
+    if (elect_one()) {
+      const uint32_t sf_full = smem_u32(&bars->sf_full[0]), lsf = leader_addr(sf_full), sf_empty = smem_u32(&bars->sf_empty[0]), at = smem_u32(ring_sf);
+      uint32_t sl = 0, ph = 1;
       bool ok = true;
+      asm volatile("griddepcontrol.wait;" ::: "memory");
       while (ok && walk_next<KIND>(p, *bars, tab, walk)) {
-        const int n = (walk.c.ks1 - walk.c.ks0 + kSpc<KIND> - 1) / kSpc<KIND>;
-        for (int i = 0; i < n; ++i, ++chunk) {
-          if (!wait_local(sf_stored + chunk % kSfSlots * 8, chunk / kSfSlots & 1, abort_flag)) { ok = false; break; }
-          fence_async_smem();
-          arrive_release_cluster(lsf + chunk % kSfSlots * 8);
+        const Piece c = walk.c;
+        // two words of 128 rows in 1024 bytes
+        const int row = (c.e * p.i_blocks + c.i0 / kLanes + rank) * (p.sf_words / 2);
+        for (int ks = c.ks0; ks < c.ks1; ks += kSpc<KIND>) {
+          if (!wait_local(sf_empty + sl * 8, ph, abort_flag)) { ok = false; break; }
+          if (rank == 0) mbar_expect_tx(sf_full + sl * 8, 2 * 4096);
+          tma_load_2d_pair(at + sl * sf_bytes, &maps.sfa, 0, row + ks * kSb / 8, lsf + sl * 8);
+          if (++sl == kSfSlots) { sl = 0; ph ^= 1; }
         }
       }
+      if (!ok) for (int n = 0; n < 100; ++n) __nanosleep(1000);
     }
   } else if (kSf && warp >= kScaleWarp0) {
-    // ------------------------------------------------------------ scales: an operand's two warps take chunks in turn
-    const bool of_b = warp >= kScaleWarp0 + kScaleWarps;
-    const uint32_t sf_stored = smem_u32(&bars->sf_stored[0]), sf_empty = smem_u32(&bars->sf_empty[0]);
-    const uint32_t base = smem_u32(ring_sf) + (of_b ? 4096 : 0);
-    const int blocks = p.sfb_chunk >> 12;   // of 128 rows of b: 1 or 2
-    uint32_t chunk = 0;                     // of the next one to be stored
+    // ------------------------------------------------------------ b's scales: warps take chunks in turn, each has its slot
+    const uint32_t sl = warp - kScaleWarp0, lsf = leader_addr(smem_u32(&bars->sf_full[sl])), sf_empty = smem_u32(&bars->sf_empty[sl]);
+    const uint32_t at = smem_u32(ring_sf) + sl * sf_bytes + 4096;
+    const int blocks = p.sfb_chunk >> 12;   // of 128 rows: 1 or 2
+    uint32_t chunk = 0, ph = 1;
     bool ok = true;
-    // Scales are read before their slot is free, and stored after.
-    auto slot = [&](uint32_t n) -> uint32_t {
-      const uint32_t sl = n % kSfSlots;
-      ok = __all_sync(0xFFFFFFFFu, wait_local(sf_empty + sl * 8, (n / kSfSlots & 1) ^ 1, abort_flag));
-      return base + sl * sf_bytes;
-    };
-    auto stored = [&](uint32_t n) {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(sf_stored + n % kSfSlots * 8);
-    };
-    if (of_b) {
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      while (ok && next_of_warp()) {
-        const Piece c = walk.c;
-        for (int ks = c.ks0; ks < c.ks1; ks += kSpc<KIND>, ++chunk) {
-          if ((chunk & (kScaleWarps - 1)) != (uint32_t)(warp & 1)) continue;
-          // a lane has rows lane, lane + 32, .. (past the end of b: the last row, for columns that nobody stores)
-          const uint32_t* from = p.sfb + (long long)(ks * kSb / 4) * p.T;
-          int row[8];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    while (ok && next_of_warp()) {
+      const Piece c = walk.c;
+      for (int ks = c.ks0; ks < c.ks1; ks += kSpc<KIND>, ++chunk) {
+        if ((chunk & (kScaleWarps - 1)) != sl) continue;
+        // a lane has rows lane, lane + 32, .. (past the end of b: the last row, for columns that nobody stores)
+        const uint32_t* from = p.sfb + (long long)(ks * kSb / 4) * p.T;
+        int row[8];
 #pragma unroll
-          for (int r = 0; r < 8; ++r) row[r] = min(c.row0 + lane + 32 * r, p.T - 1);
-          uint4 v[2][8];
+        for (int r = 0; r < 8; ++r) row[r] = min(c.row0 + lane + 32 * r, p.T - 1);
+        uint4 v[2][8];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (128 * h >= c.neff) break;
+        for (int h = 0; h < 2; ++h) {
+          if (128 * h >= c.neff) break;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint32_t* w = from + (long long)k * p.T;
-              v[h][k].x = __ldcg(w + row[4 * h]);
-              if (128 * h + 32 < c.neff) v[h][k].y = __ldcg(w + row[4 * h + 1]);
-              if (128 * h + 64 < c.neff) v[h][k].z = __ldcg(w + row[4 * h + 2]);
-              if (128 * h + 96 < c.neff) v[h][k].w = __ldcg(w + row[4 * h + 3]);
-            }
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t* w = from + (long long)k * p.T;
+            v[h][k].x = __ldcg(w + row[4 * h]);
+            if (128 * h + 32 < c.neff) v[h][k].y = __ldcg(w + row[4 * h + 1]);
+            if (128 * h + 64 < c.neff) v[h][k].z = __ldcg(w + row[4 * h + 2]);
+            if (128 * h + 96 < c.neff) v[h][k].w = __ldcg(w + row[4 * h + 3]);
           }
-          const uint32_t at = slot(chunk);
-          if (!ok) break;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (128 * h >= c.neff) break;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) sts128(at + (k * blocks + h) * 512 + lane * 16, v[h][k]);
-          }
-          stored(chunk);
         }
-      }
-    } else {
-      // Two chunks of each warp are on their way at a time: they come from HBM.
-      const int half = lane & 1, r0 = lane >> 1;   // a lane has 16 of a row's 32 bytes
-      Piece c;
-      int ks = 0;
-      uint32_t ahead = 0;   // of the next chunk to be read
-      bool more = next_of_warp();
-      if (more) { c = walk.c; ks = c.ks0; }
-      auto advance = [&]() {
-        ++ahead;
-        ks += kSpc<KIND>;
-        if (ks < c.ks1) return;
-        more = next_of_warp();
-        if (more) { c = walk.c; ks = c.ks0; }
-      };
-      // Reads this warp's next chunk; false: there is none.
-      auto read = [&](uint4 (&v)[kLanes / 16]) -> bool {
-        while (more && (ahead & (kScaleWarps - 1)) != (uint32_t)(warp & 1)) advance();
-        if (!more) return false;
-        const int n0 = c.i0 + rank * kLanes, byte = ks * kSb + 16 * half, left = p.sf_row - byte;
-        const uint8_t* from = p.sfa + ((long long)c.e * p.I + n0) * p.sf_row + byte;
+        // read before the slot is free, stored after
+        ok = __all_sync(0xFFFFFFFFu, wait_local(sf_empty, ph, abort_flag));
+        if (!ok) break;
+        ph ^= 1;
 #pragma unroll
-        for (int i = 0; i < kLanes / 16; ++i) {
-          const int r = r0 + 16 * i;
-          v[i] = make_uint4(0, 0, 0, 0);
-          if (n0 + r < p.I && left > 0) load16(v[i], from + (long long)r * p.sf_row, left, p.sfa_align);
-        }
-        advance();
-        return true;
-      };
-      auto store = [&](const uint4 (&v)[kLanes / 16]) {
-        const uint32_t at = slot(chunk);
-        if (!ok) return;
+        for (int h = 0; h < 2; ++h) {
+          if (128 * h >= c.neff) break;
 #pragma unroll
-        for (int i = 0; i < kLanes / 16; ++i) {
-          const int r = r0 + 16 * i;
-          const uint32_t to = at + half * 2048 + (r & 31) * 16 + (r >> 5) * 4;
-          sts32(to, v[i].x);
-          sts32(to + 512, v[i].y);
-          sts32(to + 1024, v[i].z);
-          sts32(to + 1536, v[i].w);
+          for (int k = 0; k < 8; ++k) sts128(at + (k * blocks + h) * 512 + lane * 16, v[h][k]);
         }
-        stored(chunk);
-        chunk += kScaleWarps;
-      };
-      chunk = warp & 1;
-      uint4 v0[kLanes / 16], v1[kLanes / 16];
-      bool h0 = read(v0);
-      while (ok && h0) {
-        const bool h1 = read(v1);
-        store(v0);
-        if (!ok || !h1) break;
-        h0 = read(v0);
-        store(v1);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(lsf);
       }
     }
   } else if (warp >= kEpiWarp0 && warp < kEpiWarp0 + kEpiWarps) {
@@ -1086,9 +996,8 @@ int grouped_tc(const GroupedTcArgs& a, cudaStream_t st) {
   p.partial = reinterpret_cast<float*>(static_cast<char*>(a.ws) + kCounterBytes);
   p.status = a.status;
   p.sfb_chunk = p.NT > 128 ? 8192 : 4096;
-  p.sfa = a.sfa; p.sfb = a.sfb; p.sf_row = (int)a.sf_row;
-  const uintptr_t sf_at = reinterpret_cast<uintptr_t>(a.sfa) | (uintptr_t)a.sf_row;
-  p.sfa_align = (sf_at & 15) == 0 ? 16 : ((sf_at & 7) == 0 ? 8 : 1);
+  p.sfb = a.sfb; p.sf_words = (int)a.sf_words;
+  p.i_blocks = (p.I + kLanes - 1) / kLanes;
   p.ga = a.ga; p.gb = a.gb; p.ga_each = a.ga_each;
   if (a.T > (1 << 30) || a.J > (1 << 30))
     return fail(B200Q_ERR_UNSUPPORTED, "[grouped product] No implementation for problem shape: more than 2^30 rows");
@@ -1111,6 +1020,16 @@ int grouped_tc(const GroupedTcArgs& a, cudaStream_t st) {
     else rc = encode(&m.a, a.dtype, es_a, a.a, ka, a.a_pitch, a.I, a.E, box, kLanes);
     for (int i = 0; i < 5 && !rc; ++i)
       if ((128 >> i) <= p.b_bytes / 128) rc = encode(&m.b[i], a.dtype, es_a, a.b, ka, a.b_pitch, a.T, 1, box, 128 >> i);
+  }
+  if (fp4 && !rc) {
+    const int64_t rows = a.E * p.i_blocks * (a.sf_words / 2);
+    const cuuint64_t dims[2] = {256, (cuuint64_t)rows}, strides[1] = {1024};
+    const cuuint32_t sbox[2] = {256, 4}, one[2] = {1, 1};
+    if (rows >= INT32_MAX) return fail(B200Q_ERR_UNSUPPORTED, "[grouped product] No implementation for problem shape: too many scales");
+    const CUresult r = encode_fn()(&m.sfa, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<uint32_t*>(a.sfa), dims, strides, sbox, one,
+                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(B200Q_ERR_CUDA, "[grouped product] a tensor map could not be encoded (%d)", (int)r);
   }
   if (rc) return rc;
   switch (a.form) {

@@ -178,9 +178,8 @@ struct GroupedTcArgs {
   void* out;                // [T, I], Sum: [E, J, I]
   int dtype;                // of out (and of 16-bit operands)
   int64_t T, E, I, J, K;
-  const uint8_t* sfa;               // 4 bits: scales, rows sf_row bytes apart
-  const uint32_t* sfb;              // and words of four consecutive ones: [words][T], zeros after the last up to a multiple of 8 words
-  int64_t sf_row;
+  const uint32_t *sfa, *sfb;        // 4 bits: scales as fp4_prepare leaves them
+  int64_t sf_words;                 // of four, per row
   const float *ga, *gb;             // global scales (null: 1); ga_each: one per group
   int ga_each;
   void* ws;                 // grouped_tc_bytes, zeroed once
@@ -195,9 +194,26 @@ int fp4_quantize(const void* w, int dtype, int64_t rows, int64_t K, int mode, co
                  uint32_t* wq, uint8_t* scales, cudaStream_t st);
 int fp4_dequantize(const uint32_t* wq, const uint8_t* scales, int mode, const float* global, int64_t rows_per_global, int dtype,
                    int64_t rows, int64_t K, void* out, cudaStream_t st);
-// Activations for grouped_tc: rows of codes with a pitch of their own, scales as [words][rows] words of four, zeros after the last.
-int fp4_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int mode, const float* global, uint8_t* codes,
-                      int64_t code_pitch, uint32_t* scales, int64_t words, cudaStream_t st);
+// Operands of a 4-bit product in the order that grouped_tc takes, in one launch (the one that its launch has to follow):
+//   codes  x quantized, rows code_pitch bytes apart
+//   sfx    its scales, words of four consecutive ones, [words][T]
+//   sfw    the weights' scales [E * N, K / group] by blocks of 128 rows, [E][blocks][words][32][4]: word (r % 32, r / 32) of a
+//          block and word index is row r's.  Groups without rows are left out.
+// words: fp4_words(K, mode), zeros after the last.
+constexpr int64_t fp4_words(int64_t K, int mode) { return (K / fp4_group(mode) + 31) / 32 * 8; }
+struct Fp4Prepare {
+  const void* x;
+  int dtype, mode;
+  int64_t T, E, N, K;
+  const float* global;      // x's
+  const uint8_t* scales;
+  const void* sizes;
+  int size_bytes;
+  uint8_t* codes;
+  int64_t code_pitch;
+  uint32_t *sfx, *sfw;
+};
+int fp4_prepare(const Fp4Prepare& a, cudaStream_t st);
 // dst rows of dst_pitch bytes (a multiple of 16) from src rows of src_bytes, padded with zeros.
 int repack_rows(const void* src, int64_t src_bytes, void* dst, int64_t dst_pitch, int64_t rows, cudaStream_t st);
 
