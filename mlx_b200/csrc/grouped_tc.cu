@@ -11,13 +11,14 @@
 // 64 bytes per clock and SM that way, the L2's rate, where a block of its own would need 94.
 //
 //   warps 0, 3  TMA: a's and b's tile of a stage (128 bytes of k per row; MM and MK: 64 k)
-//   warp 1      tcgen05.mma, and for 4 bits tcgen05.cp of the stage's scales (leader block, one thread)
-//   warp 2      4 bits: TMA of a's scales.  MM: the stage that a group ends in has its foreign rows zeroed in shared memory (both operands: a foreign
+//   warp 1      tcgen05.mma (leader block, one thread)
+//   warp 2      4 bits: tcgen05.cp of the scales, three per 4 k of 256 rows (leader, one thread: with them in warp 1 a stage's
+//               instructions took it longer than its MMAs take).  MM: the stage that a group ends in has its foreign rows zeroed in shared memory (both operands: a foreign
 //               infinity times zero would be NaN).  Only those stages go through this warp: with all of them handed on by it
 //               a step of the ring took 1600 cycles instead of 700
 //   warps 4-11  epilogue: accumulator -> rounding -> stmatrix staging -> 16-byte stores
 //   warps 12-15 4 bits only: b's scales, from words in global memory into the order that tensor memory wants (a's are in that
-//               order already, fp4_prepare_kernel, and come by TMA: warp 2)
+//               order already, fp4_prepare_kernel, and come by TMA: warp 3)
 //
 // The table of groups (first row, first tile, first step) is built in shared memory by every block from `sizes`, which the
 // host never reads: no launch in front and no synchronisation.
@@ -55,7 +56,8 @@ constexpr int kScaleWarp0 = 12, kScaleWarps = 4;
 constexpr int kMaxWarps = kScaleWarp0 + kScaleWarps;
 template <Kind K> constexpr int kThreads = 32 * (kFp4<K> ? kMaxWarps : kScaleWarp0);
 constexpr int kStageOut = 2048;      // epilogue staging per warp: 32 rows of 64 bytes
-constexpr int kSfColumns = 96;       // two buffers of 16 (a) + 32 (b) columns
+constexpr int kSfColumns = 48;       // tensor memory of a stage's scales: 16 (a) + 32 (b) columns
+constexpr int kSfBuffers = 4;        // at most
 constexpr size_t kSmemMax = 227 * 1024;
 
 // k per stage, and stages per step: the unit in which K is cut (4 bits: what a chunk of scales covers)
@@ -119,7 +121,8 @@ struct __align__(16) Walk {
 struct __align__(16) Bars {
   uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t landed[kMaxStages], fixed[kMaxStages];  // MM, a group's last stage: this block's tiles are there; and without foreign rows, in both
-  uint64_t sf_full[kSfSlots], sf_empty[kSfSlots];
+  uint64_t sf_full[kSfSlots], sf_empty[kSfSlots];  // chunks of scales in shared memory
+  uint64_t sf_ready[kSfBuffers];                   // a stage's scales in tensor memory
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem_base;
   int abort_flag, last, seen[2];
@@ -415,7 +418,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       mbar_init(smem_u32(&bars->empty[lane]), 1);
       if (kSum) { mbar_init(smem_u32(&bars->landed[lane]), 1); mbar_init(smem_u32(&bars->fixed[lane]), 2); }
     }
-    if (lane < kSfSlots) { mbar_init(smem_u32(&bars->sf_full[lane]), 3); mbar_init(smem_u32(&bars->sf_empty[lane]), 1); }
+    if (lane < kSfSlots) { mbar_init(smem_u32(&bars->sf_full[lane]), 3); mbar_init(smem_u32(&bars->sf_empty[lane]), 1); mbar_init(smem_u32(&bars->sf_ready[lane]), 1); }
     if (lane < 2) { mbar_init(smem_u32(&bars->acc_full[lane]), 1); mbar_init(smem_u32(&bars->acc_empty[lane]), 2 * kEpiWarps); }
     if (lane == 0) bars->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -493,8 +496,10 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
   cluster_sync();
   tcgen05_fence_after();
   const uint32_t tmem = bars->tmem_base;
-  const int nacc = 2 * p.NT + (kSf ? kSfColumns : 0) <= 512 ? 2 : 1;
+  const int nacc = 2 * p.NT + (kSf ? 2 * kSfColumns : 0) <= 512 ? 2 : 1;
   const uint32_t tmem_sf = tmem + nacc * p.NT;
+  // (fewer than the ring has stages: whoever waits for a stage's MMAs must not miss a turn of its barrier)
+  const uint32_t sf_buffers = kSfBuffers * kSfColumns + nacc * p.NT <= 512 && p.stages > kSfBuffers ? kSfBuffers : 2;
   const uint32_t ring = smem_u32(smem);
   Walk& walk = bars->walk[warp];
   if (lane == 0) walk_begin(*bars, walk);
@@ -512,7 +517,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
     if (elect_one()) {
       const bool of_a = warp == 0;
       const uint32_t full = smem_u32(&bars->full[0]), lfull = leader_addr(full), empty = smem_u32(&bars->empty[0]), landed = smem_u32(&bars->landed[0]);
-      uint32_t s = 0, ph = 1;
+      uint32_t s = 0, ph = 1, sl = 0, sl_ph = 1;
       bool ok = true;
       while (ok && walk_next<KIND>(p, *bars, tab, walk)) {
         const Piece c = walk.c;
@@ -521,6 +526,14 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
         const int rows = kSum ? half : box_rows(half, &box0);
         const uint32_t bytes = kStageA + (uint32_t)rows * 128u;
         for (int ks = c.ks0; ks < c.ks1; ++ks) {
+          if (kSf && !of_a && (ks - c.ks0) % kSpc<KIND> == 0) {   // a's scales of the chunk that begins here
+            if (!wait_local(smem_u32(&bars->sf_empty[sl]), sl_ph, abort_flag)) { ok = false; break; }
+            if (rank == 0) mbar_expect_tx(smem_u32(&bars->sf_full[sl]), 2 * 4096);
+            // (rows of 1024 bytes: two words of 128 rows)
+            tma_load_2d_pair(smem_u32(ring_sf) + sl * sf_bytes, &maps.sfa, 0, (c.e * p.i_blocks + c.i0 / kLanes + rank) * (p.sf_words / 2) + ks * kSb / 8,
+                             leader_addr(smem_u32(&bars->sf_full[sl])));
+            if (++sl == kSfSlots) { sl = 0; sl_ph ^= 1; }
+          }
           if (!wait_local(empty + s * 8, ph, abort_flag)) { ok = false; break; }
           const uint32_t at = ring + s * stage_bytes + (of_a ? 0 : kStageA);
           // A group's last stage (MM) is counted by this block, for the warp that zeroes foreign rows; any other by the pair's leader.
@@ -552,10 +565,10 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
     // ------------------------------------------------------------ MMAs (leader)
     if (rank == 0 && elect_one()) {
       const uint32_t full = smem_u32(&bars->full[0]), empty = smem_u32(&bars->empty[0]);
-      const uint32_t sf_full = smem_u32(&bars->sf_full[0]), sf_empty = smem_u32(&bars->sf_empty[0]), sf_ring = smem_u32(ring_sf);
+      const uint32_t sf_ready = smem_u32(&bars->sf_ready[0]);
       const uint32_t fixed = smem_u32(&bars->fixed[0]);
       // A bit per slot: the phase that its barriers `full` and `fixed` are in (MM uses one or the other)
-      uint32_t s = 0, full_ph = 0, fixed_ph = 0, sq = 0, sph = 0, n_piece = 0, n_stage = 0;
+      uint32_t s = 0, full_ph = 0, fixed_ph = 0, n_piece = 0, n_stage = 0;
       bool ok = true;
       while (ok && walk_next<KIND>(p, *bars, tab, walk)) {
         const Piece c = walk.c;
@@ -566,8 +579,6 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
         if (!wait_local(smem_u32(&bars->acc_empty[ab]), (an & 1) ^ 1, abort_flag)) break;
         uint32_t first = 0;
         for (int ks = c.ks0; ks < c.ks1; ++ks) {
-          const int in_chunk = kSf ? (ks - c.ks0) % kSpc<KIND> : 0;
-          if (kSf && in_chunk == 0 && !wait_cluster(sf_full + sq * 8, sph, abort_flag)) { ok = false; break; }
           const bool ends = kSum && c.len - ks * 64 < 64;
           if (!wait_cluster((ends ? fixed : full) + s * 8, ((ends ? fixed_ph : full_ph) >> s) & 1, abort_flag)) { ok = false; break; }
           if (ends) fixed_ph ^= 1u << s; else full_ph ^= 1u << s;
@@ -575,24 +586,13 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
           const uint64_t da = sw128_desc(ring + s * stage_bytes, KIND == Kind::MK || kSum);
           const uint64_t db = sw128_desc(ring + s * stage_bytes + kStageA, kSum);
           if constexpr (kSf) {
-            constexpr int kWords = kSb / 4;
-            const uint32_t kb = p.sfb_chunk / 8;   // bytes per word of k of b's scales: 512 or 1024
-            const uint32_t ta = tmem_sf + (n_stage & 1) * 48, tb = ta + 16;
-            const uint32_t sa = sf_ring + sq * sf_bytes + in_chunk * kWords * 512, sb = sf_ring + sq * sf_bytes + 4096 + in_chunk * kWords * kb;
-#pragma unroll
-            for (int w = 0; w < kWords; ++w) {
-              tcgen05_cp_scales(ta + 4 * w, scales_desc(sa + 512 * w));
-              tcgen05_cp_scales(tb + 8 * w, scales_desc(sb + kb * w));
-              if (c.neff > 128) tcgen05_cp_scales(tb + 8 * w + 4, scales_desc(sb + kb * w + 512));
-            }
+            const uint32_t buf = n_stage & (sf_buffers - 1), ta = tmem_sf + buf * kSfColumns, tb = ta + 16;
+            if (!wait_local(sf_ready + buf * 8, n_stage / sf_buffers & 1, abort_flag)) { ok = false; break; }
+            tcgen05_fence_after();
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
               const int w = KIND == Kind::Mx ? kk >> 1 : kk, id = KIND == Kind::Mx ? (kk & 1) * 2 : 0;
               mma_fp4<KIND>(acc, da + 2 * kk, db + 2 * kk, idesc | (uint32_t)id << 29 | (uint32_t)id << 4, ta + 4 * w, tb + 8 * w, kk ? 1u : first);
-            }
-            if (in_chunk == kSpc<KIND> - 1 || ks + 1 == c.ks1) {
-              tcgen05_commit_pair(sf_empty + sq * 8);
-              if (++sq == kSfSlots) { sq = 0; sph ^= 1; }
             }
           } else {
             const int a_step = KIND == Kind::KK ? 2 : 128, b_step = kSum ? 128 : 2;
@@ -631,24 +631,41 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       if (lane == 0) mbar_arrive_cluster(lfixed + s * 8);
     }
   } else if (kSf && warp == 2) {
-    // ------------------------------------------------------------ a's scales
-    if (elect_one()) {
-      const uint32_t sf_full = smem_u32(&bars->sf_full[0]), lsf = leader_addr(sf_full), sf_empty = smem_u32(&bars->sf_empty[0]), at = smem_u32(ring_sf);
-      uint32_t sl = 0, ph = 1;
+    // ------------------------------------------------------------ scales, from both blocks' shared memory into their tensor memories
+    if (rank == 0 && elect_one()) {
+      const uint32_t sf_full = smem_u32(&bars->sf_full[0]), sf_empty = smem_u32(&bars->sf_empty[0]), sf_ready = smem_u32(&bars->sf_ready[0]);
+      const uint32_t empty = smem_u32(&bars->empty[0]), at = smem_u32(ring_sf);
+      const uint32_t kb = p.sfb_chunk / 8;   // bytes per word of k of b's scales: 512 or 1024
+      constexpr int kWords = kSb / 4;
+      uint32_t sl = 0, ph = 0, n_stage = 0, done = 0, done_ph = 0;
       bool ok = true;
-      asm volatile("griddepcontrol.wait;" ::: "memory");
       while (ok && walk_next<KIND>(p, *bars, tab, walk)) {
         const Piece c = walk.c;
-        // two words of 128 rows in 1024 bytes
-        const int row = (c.e * p.i_blocks + c.i0 / kLanes + rank) * (p.sf_words / 2);
-        for (int ks = c.ks0; ks < c.ks1; ks += kSpc<KIND>) {
-          if (!wait_local(sf_empty + sl * 8, ph, abort_flag)) { ok = false; break; }
-          if (rank == 0) mbar_expect_tx(sf_full + sl * 8, 2 * 4096);
-          tma_load_2d_pair(at + sl * sf_bytes, &maps.sfa, 0, row + ks * kSb / 8, lsf + sl * 8);
+        for (int k0 = c.ks0; ok && k0 < c.ks1; k0 += kSpc<KIND>) {
+          if (!wait_cluster(sf_full + sl * 8, ph, abort_flag)) { ok = false; break; }
+          tcgen05_fence_after();
+          for (int j = 0; j < kSpc<KIND> && k0 + j < c.ks1; ++j, ++n_stage) {
+            const uint32_t buf = n_stage & (sf_buffers - 1);
+            if (n_stage >= sf_buffers) {   // the stage that used these columns last has been multiplied
+              if (!wait_local(empty + done * 8, done_ph, abort_flag)) { ok = false; break; }
+              if (++done == (uint32_t)p.stages) { done = 0; done_ph ^= 1; }
+              tcgen05_fence_after();
+            }
+            const uint32_t ta = tmem_sf + buf * kSfColumns, tb = ta + 16;
+            const uint32_t sa = at + sl * sf_bytes + j * kWords * 512, sb = at + sl * sf_bytes + 4096 + j * kWords * kb;
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) {
+              tcgen05_cp_scales(ta + 4 * w, scales_desc(sa + 512 * w));
+              tcgen05_cp_scales(tb + 8 * w, scales_desc(sb + kb * w));
+              if (c.neff > 128) tcgen05_cp_scales(tb + 8 * w + 4, scales_desc(sb + kb * w + 512));
+            }
+            tcgen05_commit_pair(sf_ready + buf * 8);
+          }
+          if (!ok) break;
+          tcgen05_commit_pair(sf_empty + sl * 8);
           if (++sl == kSfSlots) { sl = 0; ph ^= 1; }
         }
       }
-      if (!ok) for (int n = 0; n < 100; ++n) __nanosleep(1000);
     }
   } else if (kSf && warp >= kScaleWarp0) {
     // ------------------------------------------------------------ b's scales: warps take chunks in turn, each has its slot
@@ -940,6 +957,7 @@ int launch(const Maps& m, Params& p, cudaStream_t st) {
                        sizeof(Bars) + (size_t)(p.E + 1) * sizeof(Group);
   p.stages = (int)((kSmemMax - fixed) / stage);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
+  if (p.stages < 3) return fail(B200Q_ERR_UNSUPPORTED, "[grouped product] No implementation for problem shape: the table of %d groups leaves no shared memory", p.E);
   size_t smem = fixed + p.stages * stage;
   // One block per SM: the allocation of all of tensor memory never waits for another block of this kernel.
   if (smem < 120 * 1024) smem = 120 * 1024;
