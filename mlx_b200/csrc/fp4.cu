@@ -99,8 +99,26 @@ __device__ __forceinline__ uint32_t quantize_unit(float (&v)[kUnit], float G, ui
   } else {
     s = e4m3(fminf(__fdiv_rn(__uint_as_float(top), 6.0f * G), 448.0f));
     const float d = e4m3_value(s) * G;
+    if (d > 0x1p-100f && d < 0x1p100f && s < 0x7Eu) {
+      // Quotients rounded as a division rounds them (Markstein, 1990): with r the rounded reciprocal, q + (x - q d) r is the
+      // rounded quotient once q is within one unit of it, which the first correction makes it.  Not scaled down to 448, a
+      // quotient is at most 7.
+      const float r = __frcp_rn(d);
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i) v[i] = d == 0.0f ? copysignf(0.0f, v[i]) : __fdiv_rn(v[i], d);
+      for (int i = 0; i < kUnit; ++i) {
+        float q = v[i] * r;
+        q = fmaf(fmaf(-q, d, v[i]), r, q);
+        v[i] = fmaf(fmaf(-q, d, v[i]), r, q);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < kUnit; ++i) {
+        const float q = d == 0.0f ? copysignf(0.0f, v[0]) : __fdiv_rn(v[0], d);
+#pragma unroll
+        for (int j = 0; j + 1 < kUnit; ++j) v[j] = v[j + 1];   // (rolled: this path is rare and long)
+        v[kUnit - 1] = q;
+      }
+    }
     if (odd) s = 0x7Fu;
   }
   codes[0] = odd ? 0u : e2m1x8(v);
@@ -156,7 +174,7 @@ struct PrepareParams {
 };
 constexpr int kPrepareWords = 32;
 
-template <typename T, bool MX, bool ALIGNED>
+template <typename T, bool MX, bool ALIGNED, int ROWS>
 __global__ void __launch_bounds__(kQuantThreads)
 fp4_prepare_kernel(const T* __restrict__ x, const __grid_constant__ PrepareParams p) {
   __shared__ uint4 tile[kPrepareWords][32];
@@ -201,22 +219,30 @@ fp4_prepare_kernel(const T* __restrict__ x, const __grid_constant__ PrepareParam
     for (int i = t; i < n; i += kQuantThreads) out[i] = tile[i >> 5][i & 31];
     return;
   }
-  const int64_t b = blockIdx.x - p.scale_blocks, row = b / p.blocks_per_row;
-  const int64_t u = (b - row * p.blocks_per_row) * kQuantThreads + t, k = u * kUnit;
+  const int64_t b = blockIdx.x - p.scale_blocks, row0 = b / p.blocks_per_row * ROWS;
+  const int64_t u = (b % p.blocks_per_row) * kQuantThreads + t, k = u * kUnit;
   const bool in = k < p.K;
-  float v[kUnit];
-  if (in) load_unit<T, ALIGNED>(x + row * p.K + k, v);
-  else
-    for (int i = 0; i < kUnit; ++i) v[i] = 0.0f;
+  float v[ROWS][kUnit];
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+    if (in && row0 + j < p.T) load_unit<T, ALIGNED>(x + (row0 + j) * p.K + k, v[j]);
+    else
+      for (int i = 0; i < kUnit; ++i) v[j][i] = 0.0f;
+  }
   const float G = !MX && p.global ? __ldg(p.global) : 1.0f;
-  uint32_t codes[2];
-  uint32_t s = quantize_unit<MX>(v, G, codes);
-  if (in) *reinterpret_cast<uint2*>(p.codes + row * p.code_pitch + k / 2) = make_uint2(codes[0], codes[1]);
-  else s = 0;
-  constexpr int kShare = MX ? 8 : 4;   // lanes that share a word
-  s |= __shfl_down_sync(0xFFFFFFFFu, s, kShare / 4) << 8;
-  s |= __shfl_down_sync(0xFFFFFFFFu, s, kShare / 2) << 16;
-  if (t % kShare == 0 && u / kShare < p.words) p.sfx[(u / kShare) * p.T + row] = s;
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+    const int64_t row = row0 + j;
+    uint32_t codes[2];
+    uint32_t s = quantize_unit<MX>(v[j], G, codes);
+    if (row >= p.T) return;   // (of the whole block)
+    if (in) *reinterpret_cast<uint2*>(p.codes + row * p.code_pitch + k / 2) = make_uint2(codes[0], codes[1]);
+    else s = 0;
+    constexpr int kShare = MX ? 8 : 4;   // lanes that share a word
+    s |= __shfl_down_sync(0xFFFFFFFFu, s, kShare / 4) << 8;
+    s |= __shfl_down_sync(0xFFFFFFFFu, s, kShare / 2) << 16;
+    if (t % kShare == 0 && u / kShare < p.words) p.sfx[(u / kShare) * p.T + row] = s;
+  }
 }
 
 // A thread takes kAhead pieces of 8 values, kQuantThreads apart, whose codes and scales are all on their way before the first is
@@ -342,12 +368,14 @@ int fp4_prepare(const Fp4Prepare& a, cudaStream_t st) {
   const int64_t units = (int64_t)p.words * (a.mode == B200Q_MXFP4 ? 8 : 4);
   p.blocks_per_row = (int)((units + kQuantThreads - 1) / kQuantThreads);
   p.aligned = ((reinterpret_cast<uintptr_t>(a.scales) | (uintptr_t)p.sf_row) & 15) == 0;
-  const int64_t blocks = p.scale_blocks + a.T * p.blocks_per_row;
+  const int rows = a.T >= 1024 ? 2 : 1;   // of a block: with two on their way 4096 rows of 4096 take 6.3 us less, few rows end sooner with one
+  const int64_t blocks = p.scale_blocks + (a.T + rows - 1) / rows * p.blocks_per_row;
   if (blocks > kMostBlocks) return fail(B200Q_ERR_UNSUPPORTED, "[qqmm] No implementation for problem shape: too many values");
   return with_type(a.dtype, [&](auto t) {
     using T = decltype(t);
     return with_flags(a.mode, aligned16(a.x), [&](auto mx, auto al) {
-      fp4_prepare_kernel<T, decltype(mx)::value, decltype(al)::value><<<(unsigned)blocks, kQuantThreads, 0, st>>>(static_cast<const T*>(a.x), p);
+      if (rows == 2) fp4_prepare_kernel<T, decltype(mx)::value, decltype(al)::value, 2><<<(unsigned)blocks, kQuantThreads, 0, st>>>(static_cast<const T*>(a.x), p);
+      else fp4_prepare_kernel<T, decltype(mx)::value, decltype(al)::value, 1><<<(unsigned)blocks, kQuantThreads, 0, st>>>(static_cast<const T*>(a.x), p);
       B200Q_LAUNCH_OK("fp4_prepare_kernel");
       return B200Q_OK;
     });
