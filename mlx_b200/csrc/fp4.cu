@@ -108,7 +108,7 @@ __device__ __forceinline__ uint32_t quantize_unit(float (&v)[kUnit], float G, ui
       for (int i = 0; i < kUnit; ++i) {
         float q = v[i] * r;
         q = fmaf(fmaf(-q, d, v[i]), r, q);
-        v[i] = fmaf(fmaf(-q, d, v[i]), r, q);
+        v[i] = copysignf(fmaf(fmaf(-q, d, v[i]), r, q), v[i]);   // (of -0 too)
       }
     } else {
 #pragma unroll 1
