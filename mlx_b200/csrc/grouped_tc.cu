@@ -50,7 +50,7 @@ constexpr int kTileI = 2 * kLanes;
 constexpr int kMaxNT = 256;
 constexpr int kStageA = kLanes * 128;
 constexpr int kMaxStages = 12;
-constexpr int kSfSlots = 4;          // chunks of scales: 32 bytes per row each
+constexpr int kSfSlots = 8;          // at most, of chunks of scales: 32 bytes per row each
 constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
 constexpr int kScaleWarp0 = 12, kScaleWarps = 4;
 constexpr int kMaxWarps = kScaleWarp0 + kScaleWarps;
@@ -76,6 +76,7 @@ struct Params {
   int E, T;
   int I, J, K;             // output width; MM: output rows per group; length of the sum (MM: unused)
   int NT, i_tiles, stages;
+  int sf_slots;            // 8 up to 128 rows per tile, else 4
   int b_bytes;             // of a stage's b tile
   int blocks;              // MK, MM: a (b) comes in whole blocks of 64 columns, two in one copy (bit 0: a, bit 1: b)
   int sfb_chunk;           // 4 bits: bytes of a chunk of b's scales
@@ -155,15 +156,16 @@ __device__ __forceinline__ int2 tiles_j(const Params& p, int len) {
 }
 
 // Number of pairs that the n tiles (`rest` steps, `rows` rows each on average) left over from whole waves are cut for; 0: not
-// cut.  In cycles: a stage of n busy pairs takes its MMAs, its 16 KB of weights at their share of HBM, or at least 300; a cut
-// tile costs its writes (36 a row), the last arriver's reads (20 a row and part) and 4000 of fences and latencies.
+// cut.  In cycles: a stage of n busy pairs takes its MMAs, its 16 KB of weights at their share of HBM, or at least 300 (4
+// bits, whose scales pass more hands: 450); a cut tile costs its writes (36 a row), the last arriver's reads (20 a row and part)
+// and 4000 of fences and latencies.
 // The lanes of a warp try lane + 1 parts per tile (most: 8).
 template <Kind KIND>
 __device__ __forceinline__ int cut_for(int lane, int n, int rest, int rows, int pairs) {
   if ((long long)rest * (pairs + 1) >= INT32_MAX) return 0;
   const float r = (float)max(rows, 16), steps = (float)(rest * kSpc<KIND>);   // stages of all of them
   const int s = lane + 1, busy = min(min(n * s, pairs), rest);
-  const float stage = fmaxf(fmaxf(2.0f * r, 700.0f * (float)busy / (float)pairs), 300.0f);
+  const float stage = fmaxf(fmaxf(2.0f * r, 700.0f * (float)busy / (float)pairs), kFp4<KIND> ? 450.0f : 300.0f);
   float t = __fdividef(steps, (float)busy) * stage;
   if (s > 1) t += r * (36.0f + 20.0f * (__fdividef((float)busy, (float)n) + (n * s > pairs ? 1.0f : 0.0f))) + 4000.0f;
   if (s > 8 || n * (s - 1) >= pairs) t = 3.0e38f;
@@ -405,7 +407,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
   const uint32_t stage_bytes = kStageA + (uint32_t)p.b_bytes;
   unsigned char* ring_sf = smem + (size_t)p.stages * stage_bytes;
   const uint32_t sf_bytes = kSf ? 4096u + (uint32_t)p.sfb_chunk : 0u;
-  unsigned char* staging = ring_sf + kSfSlots * sf_bytes;
+  unsigned char* staging = ring_sf + (kSf ? p.sf_slots : 0) * sf_bytes;
   Bars* bars = reinterpret_cast<Bars*>(staging + (sizeof(T) == 2 ? kEpiWarps * kStageOut : 0));
   Group* tab = reinterpret_cast<Group*>(bars + 1);
   volatile int* abort_flag = &bars->abort_flag;
@@ -418,7 +420,8 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       mbar_init(smem_u32(&bars->empty[lane]), 1);
       if (kSum) { mbar_init(smem_u32(&bars->landed[lane]), 1); mbar_init(smem_u32(&bars->fixed[lane]), 2); }
     }
-    if (lane < kSfSlots) { mbar_init(smem_u32(&bars->sf_full[lane]), 3); mbar_init(smem_u32(&bars->sf_empty[lane]), 1); mbar_init(smem_u32(&bars->sf_ready[lane]), 1); }
+    if (lane < kSfSlots) { mbar_init(smem_u32(&bars->sf_full[lane]), 3); mbar_init(smem_u32(&bars->sf_empty[lane]), 1); }
+    if (lane < kSfBuffers) mbar_init(smem_u32(&bars->sf_ready[lane]), 1);
     if (lane < 2) { mbar_init(smem_u32(&bars->acc_full[lane]), 1); mbar_init(smem_u32(&bars->acc_empty[lane]), 2 * kEpiWarps); }
     if (lane == 0) bars->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -532,7 +535,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
             // (rows of 1024 bytes: two words of 128 rows)
             tma_load_2d_pair(smem_u32(ring_sf) + sl * sf_bytes, &maps.sfa, 0, (c.e * p.i_blocks + c.i0 / kLanes + rank) * (p.sf_words / 2) + ks * kSb / 8,
                              leader_addr(smem_u32(&bars->sf_full[sl])));
-            if (++sl == kSfSlots) { sl = 0; sl_ph ^= 1; }
+            if (++sl == (uint32_t)p.sf_slots) { sl = 0; sl_ph ^= 1; }
           }
           if (!wait_local(empty + s * 8, ph, abort_flag)) { ok = false; break; }
           const uint32_t at = ring + s * stage_bytes + (of_a ? 0 : kStageA);
@@ -663,22 +666,21 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
           }
           if (!ok) break;
           tcgen05_commit_pair(sf_empty + sl * 8);
-          if (++sl == kSfSlots) { sl = 0; ph ^= 1; }
+          if (++sl == (uint32_t)p.sf_slots) { sl = 0; ph ^= 1; }
         }
       }
     }
   } else if (kSf && warp >= kScaleWarp0) {
-    // ------------------------------------------------------------ b's scales: warps take chunks in turn, each has its slot
-    const uint32_t sl = warp - kScaleWarp0, lsf = leader_addr(smem_u32(&bars->sf_full[sl])), sf_empty = smem_u32(&bars->sf_empty[sl]);
-    const uint32_t at = smem_u32(ring_sf) + sl * sf_bytes + 4096;
+    // ------------------------------------------------------------ b's scales: warps take chunks in turn
+    const uint32_t first = warp - kScaleWarp0, sf_empty = smem_u32(&bars->sf_empty[0]), lsf = leader_addr(smem_u32(&bars->sf_full[0]));
     const int blocks = p.sfb_chunk >> 12;   // of 128 rows: 1 or 2
-    uint32_t chunk = 0, ph = 1;
+    uint32_t chunk = 0, sl = first, ph = 1;
     bool ok = true;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     while (ok && next_of_warp()) {
       const Piece c = walk.c;
       for (int ks = c.ks0; ks < c.ks1; ks += kSpc<KIND>, ++chunk) {
-        if ((chunk & (kScaleWarps - 1)) != sl) continue;
+        if ((chunk & (kScaleWarps - 1)) != first) continue;
         // a lane has rows lane, lane + 32, .. (past the end of b: the last row, for columns that nobody stores)
         const uint32_t* from = p.sfb + (long long)(ks * kSb / 4) * p.T;
         int row[8];
@@ -698,9 +700,9 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
           }
         }
         // read before the slot is free, stored after
-        ok = __all_sync(0xFFFFFFFFu, wait_local(sf_empty, ph, abort_flag));
+        ok = __all_sync(0xFFFFFFFFu, wait_local(sf_empty + sl * 8, ph, abort_flag));
         if (!ok) break;
-        ph ^= 1;
+        const uint32_t at = smem_u32(ring_sf) + sl * sf_bytes + 4096;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (128 * h >= c.neff) break;
@@ -709,7 +711,9 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(lsf);
+        if (lane == 0) mbar_arrive_cluster(lsf + sl * 8);
+        sl += kScaleWarps;
+        if (sl >= (uint32_t)p.sf_slots) { sl -= p.sf_slots; ph ^= 1; }
       }
     }
   } else if (warp >= kEpiWarp0 && warp < kEpiWarp0 + kEpiWarps) {
@@ -953,7 +957,7 @@ int allow_smem(const void* kernel) {
 template <typename T, Kind KIND>
 int launch(const Maps& m, Params& p, cudaStream_t st) {
   const size_t stage = kStageA + (size_t)p.b_bytes;
-  const size_t fixed = 1024 + (kFp4<KIND> ? kSfSlots * (4096 + (size_t)p.sfb_chunk) : 0) + (sizeof(T) == 2 ? kEpiWarps * kStageOut : 0) +
+  const size_t fixed = 1024 + (kFp4<KIND> ? p.sf_slots * (4096 + (size_t)p.sfb_chunk) : 0) + (sizeof(T) == 2 ? kEpiWarps * kStageOut : 0) +
                        sizeof(Bars) + (size_t)(p.E + 1) * sizeof(Group);
   p.stages = (int)((kSmemMax - fixed) / stage);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
@@ -1014,6 +1018,7 @@ int grouped_tc(const GroupedTcArgs& a, cudaStream_t st) {
   p.partial = reinterpret_cast<float*>(static_cast<char*>(a.ws) + kCounterBytes);
   p.status = a.status;
   p.sfb_chunk = p.NT > 128 ? 8192 : 4096;
+  p.sf_slots = p.NT > 128 ? 4 : 8;
   p.sfb = a.sfb; p.sf_words = (int)a.sf_words;
   p.i_blocks = (p.I + kLanes - 1) / kLanes;
   p.ga = a.ga; p.gb = a.gb; p.ga_each = a.ga_each;
