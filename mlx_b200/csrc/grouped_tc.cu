@@ -429,12 +429,13 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
   } else if (warp == 1) {
     tcgen05_alloc(smem_u32(&bars->tmem_base), 512);
     tcgen05_relinquish();
+  } else if (warp == 3) {
+    if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
+    if (kSf && lane == 1) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.sfa) : "memory");
+    if (lane >= 8 && lane < 13 && (kSum ? lane == 8 : (128 >> (lane - 8)) * 128 <= p.b_bytes))
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.b[lane - 8]) : "memory");
   } else if (warp == 2) {
     // The table: a lane takes E / 32 consecutive groups.
-    if (lane == 0) {
-      asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
-      asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.b[4]) : "memory");
-    }
     const int per = (p.E + 31) / 32, lo = min(p.E, lane * per), hi = min(p.E, lo + per);
     bool bad = false;
     auto size_of = [&](int e) -> int {
@@ -446,13 +447,16 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
     auto add = [&](int a, int b) { bad |= a + b > p.T; return min(a + b, p.T); };   // (T is at most 2^30)
     int at = 0;
     for (int e = lo; e < hi; ++e) at = add(at, size_of(e));
+    int rows_end = at, total, all_steps;   // sums over all groups; a lane keeps those of the lanes before it
+    if (p.E > 1) {
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int v = __shfl_up_sync(0xFFFFFFFFu, at, d);
-      if (lane >= d) at = add(at, v);
+      for (int d = 1; d < 32; d *= 2) {
+        const int v = __shfl_up_sync(0xFFFFFFFFu, at, d);
+        if (lane >= d) at = add(at, v);
+      }
+      rows_end = __shfl_sync(0xFFFFFFFFu, at, 31);
+      at = __shfl_up_sync(0xFFFFFFFFu, at, 1);
     }
-    const int rows_end = __shfl_sync(0xFFFFFFFFu, at, 31);
-    at = __shfl_up_sync(0xFFFFFFFFu, at, 1);
     if (lane == 0) at = 0;
     int units = 0, steps = 0;
     for (int e = lo; e < hi; ++e) {
@@ -463,16 +467,25 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       units += tr.y * p.i_tiles;
       steps += tr.y * p.i_tiles * group_steps<KIND>(p, at - r0);
     }
-    int u0 = units, s0 = steps;
+    total = units;
+    all_steps = steps;
+    if (p.E > 1) {
+      int u0 = units, s0 = steps;
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int a = __shfl_up_sync(0xFFFFFFFFu, u0, d), b = __shfl_up_sync(0xFFFFFFFFu, s0, d);
-      if (lane >= d) { u0 += a; s0 += b; }
+      for (int d = 1; d < 32; d *= 2) {
+        const int a = __shfl_up_sync(0xFFFFFFFFu, u0, d), b = __shfl_up_sync(0xFFFFFFFFu, s0, d);
+        if (lane >= d) { u0 += a; s0 += b; }
+      }
+      total = __shfl_sync(0xFFFFFFFFu, u0, 31);
+      all_steps = __shfl_sync(0xFFFFFFFFu, s0, 31);
+      u0 -= units;
+      s0 -= steps;
+      for (int e = lo; e < hi; ++e) { tab[e].y += u0; tab[e].z += s0; }
+    } else {   // one group, in lane 0
+      rows_end = __shfl_sync(0xFFFFFFFFu, rows_end, 0);
+      total = __shfl_sync(0xFFFFFFFFu, total, 0);
+      all_steps = __shfl_sync(0xFFFFFFFFu, all_steps, 0);
     }
-    const int total = __shfl_sync(0xFFFFFFFFu, u0, 31), all_steps = __shfl_sync(0xFFFFFFFFu, s0, 31);
-    u0 -= units;
-    s0 -= steps;
-    for (int e = lo; e < hi; ++e) { tab[e].y += u0; tab[e].z += s0; }
     bad = __any_sync(0xFFFFFFFFu, bad);
     if (lane == 0) tab[p.E] = make_int4(rows_end, total, all_steps, 0);
     __syncwarp();
@@ -495,8 +508,8 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
     }
   }
   tcgen05_fence_before();
-  __syncthreads();
-  cluster_sync();
+  __syncwarp();
+  cluster_sync();   // (every thread of both blocks: the block's own barrier too)
   tcgen05_fence_after();
   const uint32_t tmem = bars->tmem_base;
   const int nacc = 2 * p.NT + (kSf ? 2 * kSfColumns : 0) <= 512 ? 2 : 1;
