@@ -16,7 +16,8 @@
 //               instructions took it longer than its MMAs take).  MM: the stage that a group ends in has its foreign rows zeroed in shared memory (both operands: a foreign
 //               infinity times zero would be NaN).  Only those stages go through this warp: with all of them handed on by it
 //               a step of the ring took 1600 cycles instead of 700
-//   warps 4-11  epilogue: accumulator -> rounding -> stmatrix staging -> 16-byte stores
+//   warps 4-11  epilogue: accumulator -> rounding -> stmatrix staging -> 16-byte stores; MM, whose tiles have few stages and are
+//               stored as fast as they are multiplied: TMA stores of 128-byte rows
 //   warps 12-15 4 bits only: b's scales, from words in global memory into the order that tensor memory wants (a's are in that
 //               order already, fp4_prepare_kernel, and come by TMA: warp 3)
 //
@@ -67,6 +68,7 @@ template <Kind K> constexpr int kSpc = K == Kind::Mx ? 4 : (K == Kind::Nv ? 2 : 
 struct Maps {
   CUtensorMap a;
   CUtensorMap sfa;    // 4 bits: a's scales, rows of 1024 bytes
+  CUtensorMap out;    // MM, rows on 16-byte boundaries: the output, boxes of 64 i x 16 j
   CUtensorMap b[5];   // boxes of 128, 64, 32, 16 and 8 rows (MM: the first only, 64 x 64)
 };
 
@@ -265,6 +267,12 @@ __device__ __forceinline__ void tma_4d_pair(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
       ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(leader_bar)
       : "memory");
+}
+// Staged rows to global memory (what lies beyond the tensor is left out).
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];\n\tcp.async.bulk.commit_group;"
+               ::"l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
 }
 // n blocks of 64 columns and 64 rows, from column `col` and row `k` of matrix e: one copy where the map has blocks as a
 // dimension of their own (and the box both of them).
@@ -852,6 +860,30 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
                   packed[q][h][k] = pack2<T>(__uint_as_float(v[h][2 * k]) * alpha, __uint_as_float(v[h][2 * k + 1]) * alpha);
             }
             if (b0 + kBatch >= p1) release();
+            if constexpr (kSum) {
+              // Two warps (64 i) share rows of 128 bytes, 16 at a time in two buffers.  Whoever issues the stores comes to the
+              // pair's barrier when the store before has left its buffer, which then is the next to be written.
+              const uint32_t both = stg - (w & 1) * kStageOut, chunk0 = (w & 1) * 4 + (lane >> 3);
+              const bool issues = (w & 1) == 0 && lane == 0;
+              const int i64 = i_warp & ~63;
+#pragma unroll
+              for (int q = 0; q < 2 * kBatch; ++q) {
+                const int col = 32 * b0 + 16 * q;
+                if (col >= 32 * p1) break;
+                const uint32_t buf = both + (q & 1) * 2048;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                  const uint32_t row = 8 * x + (lane & 7);
+                  stmatrix_x4_trans(buf + row * 128 + ((chunk0 ^ (row & 7)) << 4), packed[q / 2][q & 1][2 * x], packed[q / 2][q & 1][2 * x + 1],
+                                    packed[q / 2][q & 1][4 + 2 * x], packed[q / 2][q & 1][5 + 2 * x]);
+                }
+                if (issues) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                fence_async_smem();
+                asm volatile("bar.sync %0, 64;" ::"r"(3 + (w >> 1)) : "memory");
+                if (issues && i64 < p.I) tma_store_3d(&maps.out, buf, i64, c.row0 + col, c.e);
+              }
+              continue;
+            }
 #pragma unroll
             for (int q = 0; q < kBatch; ++q) {
               if (b0 + q >= p1) break;
@@ -900,6 +932,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
     }
   }
 
+  if (kSum) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   __syncwarp();
   tcgen05_fence_before();
   __syncthreads();
@@ -1050,6 +1083,7 @@ int grouped_tc(const GroupedTcArgs& a, cudaStream_t st) {
   if (sum) {
     rc = encode(&m.a, a.dtype, 2, a.a, a.I, a.a_pitch, a.T, 1, 64, 64, p.blocks & 1 ? 2 : 0);
     if (!rc) rc = encode(&m.b[0], a.dtype, 2, a.b, a.J, a.b_pitch, a.T, 1, 64, 64, p.blocks & 2 ? 2 : 0);
+    if (!rc && p.vec) rc = encode(&m.out, a.dtype, 2, a.out, a.I, a.I * 2, a.J, a.E, 64, 16);
   } else {
     const int box = fp4 ? 128 : 64;
     if (a.form == GroupedForm::MK) rc = encode(&m.a, a.dtype, 2, a.a, a.I, a.a_pitch, a.K, a.E, 64, 64, p.blocks & 1 ? 2 : 0);
