@@ -56,7 +56,7 @@ constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
 constexpr int kScaleWarp0 = 12, kScaleWarps = 4;
 constexpr int kMaxWarps = kScaleWarp0 + kScaleWarps;
 template <Kind K> constexpr int kThreads = 32 * (kFp4<K> ? kMaxWarps : kScaleWarp0);
-constexpr int kStageOut = 2048;      // epilogue staging per warp: 32 rows of 64 bytes
+template <Kind K> constexpr int kStageOut = K == Kind::MM ? 4096 : 2048;   // epilogue staging per warp: 32 rows of 64 bytes; MM: twice
 constexpr int kSfColumns = 48;       // tensor memory of a stage's scales: 16 (a) + 32 (b) columns
 constexpr int kSfBuffers = 4;        // at most
 constexpr size_t kSmemMax = 227 * 1024;
@@ -68,7 +68,7 @@ template <Kind K> constexpr int kSpc = K == Kind::Mx ? 4 : (K == Kind::Nv ? 2 : 
 struct Maps {
   CUtensorMap a;
   CUtensorMap sfa;    // 4 bits: a's scales, rows of 1024 bytes
-  CUtensorMap out;    // MM, rows on 16-byte boundaries: the output, boxes of 64 i x 16 j
+  CUtensorMap out;    // MM, rows on 16-byte boundaries: the output, boxes of 64 i x 32 j
   CUtensorMap b[5];   // boxes of 128, 64, 32, 16 and 8 rows (MM: the first only, 64 x 64)
 };
 
@@ -416,7 +416,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
   unsigned char* ring_sf = smem + (size_t)p.stages * stage_bytes;
   const uint32_t sf_bytes = kSf ? 4096u + (uint32_t)p.sfb_chunk : 0u;
   unsigned char* staging = ring_sf + (kSf ? p.sf_slots : 0) * sf_bytes;
-  Bars* bars = reinterpret_cast<Bars*>(staging + (sizeof(T) == 2 ? kEpiWarps * kStageOut : 0));
+  Bars* bars = reinterpret_cast<Bars*>(staging + (sizeof(T) == 2 ? kEpiWarps * kStageOut<KIND> : 0));
   Group* tab = reinterpret_cast<Group*>(bars + 1);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -740,7 +740,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
   } else if (warp >= kEpiWarp0 && warp < kEpiWarp0 + kEpiWarps) {
     // ------------------------------------------------------------ epilogue
     const int w = warp - kEpiWarp0, quad = warp & 3, chalf = w >> 2;
-    const uint32_t stg = smem_u32(staging) + w * kStageOut;
+    const uint32_t stg = smem_u32(staging) + w * kStageOut<KIND>;
     const uint32_t lane_field = (uint32_t)(quad * 32) << 16;
     if (!kSum && bars->rows < p.T) {   // rows that belong to no group
       T* z = static_cast<T*>(p.out) + (long long)bars->rows * p.I;
@@ -861,26 +861,27 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
             }
             if (b0 + kBatch >= p1) release();
             if constexpr (kSum) {
-              // Two warps (64 i) share rows of 128 bytes, 16 at a time in two buffers.  Whoever issues the stores comes to the
-              // pair's barrier when the store before has left its buffer, which then is the next to be written.
-              const uint32_t both = stg - (w & 1) * kStageOut, chunk0 = (w & 1) * 4 + (lane >> 3);
+              // Two warps (64 i) share rows of 128 bytes, 32 at a time in two buffers.  Whoever issues the stores comes to the
+              // pair's barrier when the store before has left its buffer, which then is the next to be written.  (16 rows at a
+              // time: 1700 of a tile's 4900 cycles were spent waiting for that, 1400 issuing.)
+              const uint32_t both = stg - (w & 1) * kStageOut<KIND>, chunk0 = (w & 1) * 4 + (lane >> 3);
               const bool issues = (w & 1) == 0 && lane == 0;
               const int i64 = i_warp & ~63;
 #pragma unroll
-              for (int q = 0; q < 2 * kBatch; ++q) {
-                const int col = 32 * b0 + 16 * q;
-                if (col >= 32 * p1) break;
-                const uint32_t buf = both + (q & 1) * 2048;
+              for (int q = 0; q < kBatch; ++q) {
+                if (b0 + q >= p1) break;
+                const uint32_t buf = both + (q & 1) * 4096;
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
+                for (int x = 0; x < 4; ++x) {
                   const uint32_t row = 8 * x + (lane & 7);
-                  stmatrix_x4_trans(buf + row * 128 + ((chunk0 ^ (row & 7)) << 4), packed[q / 2][q & 1][2 * x], packed[q / 2][q & 1][2 * x + 1],
-                                    packed[q / 2][q & 1][4 + 2 * x], packed[q / 2][q & 1][5 + 2 * x]);
+                  const uint32_t (&v)[8] = packed[q][x >> 1];
+                  const int k = 2 * (x & 1);
+                  stmatrix_x4_trans(buf + row * 128 + ((chunk0 ^ (row & 7)) << 4), v[k], v[k + 1], v[4 + k], v[5 + k]);
                 }
                 if (issues) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 fence_async_smem();
                 asm volatile("bar.sync %0, 64;" ::"r"(3 + (w >> 1)) : "memory");
-                if (issues && i64 < p.I) tma_store_3d(&maps.out, buf, i64, c.row0 + col, c.e);
+                if (issues && i64 < p.I) tma_store_3d(&maps.out, buf, i64, c.row0 + 32 * (b0 + q), c.e);
               }
               continue;
             }
@@ -1003,7 +1004,7 @@ int allow_smem(const void* kernel) {
 template <typename T, Kind KIND>
 int launch(const Maps& m, Params& p, cudaStream_t st) {
   const size_t stage = kStageA + (size_t)p.b_bytes;
-  const size_t fixed = 1024 + (kFp4<KIND> ? p.sf_slots * (4096 + (size_t)p.sfb_chunk) : 0) + (sizeof(T) == 2 ? kEpiWarps * kStageOut : 0) +
+  const size_t fixed = 1024 + (kFp4<KIND> ? p.sf_slots * (4096 + (size_t)p.sfb_chunk) : 0) + (sizeof(T) == 2 ? kEpiWarps * kStageOut<KIND> : 0) +
                        sizeof(Bars) + (size_t)(p.E + 1) * sizeof(Group);
   p.stages = (int)((kSmemMax - fixed) / stage);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
@@ -1083,7 +1084,7 @@ int grouped_tc(const GroupedTcArgs& a, cudaStream_t st) {
   if (sum) {
     rc = encode(&m.a, a.dtype, 2, a.a, a.I, a.a_pitch, a.T, 1, 64, 64, p.blocks & 1 ? 2 : 0);
     if (!rc) rc = encode(&m.b[0], a.dtype, 2, a.b, a.J, a.b_pitch, a.T, 1, 64, 64, p.blocks & 2 ? 2 : 0);
-    if (!rc && p.vec) rc = encode(&m.out, a.dtype, 2, a.out, a.I, a.I * 2, a.J, a.E, 64, 16);
+    if (!rc && p.vec) rc = encode(&m.out, a.dtype, 2, a.out, a.I, a.I * 2, a.J, a.E, 64, 32);
   } else {
     const int box = fp4 ? 128 : 64;
     if (a.form == GroupedForm::MK) rc = encode(&m.a, a.dtype, 2, a.a, a.I, a.a_pitch, a.K, a.E, 64, 64, p.blocks & 1 ? 2 : 0);
