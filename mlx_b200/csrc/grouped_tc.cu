@@ -645,11 +645,11 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       const uint32_t s = (at - 1) % (uint32_t)p.stages;
       if (!__all_sync(0xFFFFFFFFu, wait_local(landed + s * 8, (ph >> s) & 1, abort_flag))) break;
       ph ^= 1u << s;
-      const int blocks = 2 + (c.neff >> 7);   // of 64 columns: two of a, one or two of b
-      const uint32_t tile = ring + s * stage_bytes, zero_end = max(16, (valid + 15) & ~15) * 128;   // the slice of 16 that it ends in
-      for (int h = 0; h < blocks; ++h)
-        for (uint32_t o = max(valid, 0) * 128 + lane * 16; o < zero_end; o += 512)
-          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(tile + h * 8192 + o), "r"(0u) : "memory");
+      // blocks of 64 columns: two of a, one or two of b; eight lanes for a row of each
+      const uint32_t tile = ring + s * stage_bytes + (lane >> 3) * 8192 + (lane & 7) * 16;
+      const int from = max(valid, 0), to = max(16, (valid + 15) & ~15);   // the slice of 16 that the group ends in
+      if ((lane >> 3) < 2 + (c.neff >> 7))
+        for (int r = from; r < to; ++r) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(tile + r * 128), "r"(0u) : "memory");
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(lfixed + s * 8);
