@@ -119,6 +119,7 @@ struct __align__(16) Walk {
   Piece c;        // where it is
   int u;          // next whole tile
   int pos, end;   // next step of the pair's range, and its end
+  int e;          // group
 };
 
 struct __align__(16) Bars {
@@ -129,6 +130,8 @@ struct __align__(16) Bars {
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem_base;
   int abort_flag, last, seen[2];
+  Piece piece[2];                                  // the epilogue's, by turns; what `more` says: whether there is one
+  int more[2];
   // schedule
   int full_units, cut_pairs, cut_steps;   // tiles in whole waves; pairs and steps of the rest
   int cut_base;                           // step at which the rest begins
@@ -182,7 +185,7 @@ __device__ __forceinline__ int cut_for(int lane, int n, int rest, int rows, int 
 __device__ __forceinline__ void walk_begin(const Bars& b, Walk& w) {
   const uint32_t pair = blockIdx.x >> 1;
   w.u = (int)pair;
-  w.pos = w.end = 0;
+  w.pos = w.end = w.e = 0;
   if ((int)pair < b.cut_pairs) {   // (cut_steps * pairs stays below 2^31)
     w.pos = b.cut_base + (int)((uint32_t)b.cut_steps * pair / (uint32_t)b.cut_pairs);
     w.end = b.cut_base + (int)((uint32_t)b.cut_steps * (pair + 1) / (uint32_t)b.cut_pairs);
@@ -196,10 +199,15 @@ __device__ __noinline__ bool walk_next(const Params& p, const Bars& b, const Gro
   const bool whole = w.u < b.full_units;
   if (!whole && w.pos >= w.end) return false;
   const int at = whole ? w.u : w.pos;
-  int e = 0, hi = p.E;   // the last group that begins at or before `at` is not empty
-  while (hi - e > 1) {
-    const int mid = (e + hi) >> 1;
-    if ((whole ? tab[mid].y : tab[mid].z) <= at) e = mid; else hi = mid;
+  auto begins = [&](int i) { return whole ? tab[i].y : tab[i].z; };
+  int e = w.e;   // the last group that begins at or before `at` is not empty; never one before the last piece's
+  if (begins(e + 1) <= at) {
+    int hi = p.E;
+    while (hi - e > 1) {
+      const int mid = (e + hi) >> 1;
+      if (begins(mid) <= at) e = mid; else hi = mid;
+    }
+    w.e = e;
   }
   const Group g = tab[e];
   const int len = tab[e + 1].x - g.x, steps = group_steps<KIND>(p, len), nj = g.w >> 9, tr = g.w & 511;
@@ -532,6 +540,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
     __syncwarp();   // everybody has read the last piece
     bool more = false;
     if (lane == 0) more = walk_next<KIND>(p, *bars, tab, walk);
+    __syncwarp();
     return __shfl_sync(0xFFFFFFFFu, more, 0);
   };
 
@@ -747,19 +756,25 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       const long long n = (long long)(p.T - bars->rows) * p.I, step = (long long)gridDim.x * kEpiWarps * 32;
       for (long long i = ((long long)blockIdx.x * kEpiWarps + w) * 32 + lane; i < n; i += step) z[i] = Elem<T>::from_float(0.0f);
     }
-    uint32_t n_piece = 0;
-    while (next_of_warp()) {
-      const Piece c = walk.c;
+    // One thread finds the pieces, the next one while a tile is stored.
+    auto find = [&](uint32_t n) {
+      const bool more = walk_next<KIND>(p, *bars, tab, walk);
+      if (more) bars->piece[n & 1] = walk.c;
+      bars->more[n & 1] = more;
+    };
+    if (w == 0 && lane == 0) find(0);
+    for (uint32_t n_piece = 0;; ++n_piece) {
       const uint32_t ab = nacc == 2 ? n_piece & 1 : 0, an = nacc == 2 ? n_piece >> 1 : n_piece;
       // One warp looks and all go by what it found: the abort flag may be raised between two warps' looks.
       if (w == 0) {
-        const bool seen = __all_sync(0xFFFFFFFFu, wait_local(smem_u32(&bars->acc_full[ab]), an & 1, abort_flag));
+        __syncwarp();
+        const bool seen = bars->more[n_piece & 1] && __all_sync(0xFFFFFFFFu, wait_local(smem_u32(&bars->acc_full[ab]), an & 1, abort_flag));
         if (lane == 0) bars->seen[n_piece & 1] = seen;
         __syncwarp();
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
       if (!bars->seen[n_piece & 1]) break;
-      ++n_piece;
+      const Piece c = bars->piece[n_piece & 1];
       tcgen05_fence_after();
       float alpha = 1.0f;
       if constexpr (kSf) {
@@ -771,7 +786,11 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       auto release = [&]() {
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(leader_addr(smem_u32(&bars->acc_empty[ab])));
+        if (lane == 0) {
+          mbar_arrive_cluster(leader_addr(smem_u32(&bars->acc_empty[ab])));
+          if (w == 0) find(n_piece + 1);
+        }
+        __syncwarp();
       };
       // this warp's columns: half of them, in pieces of 32
       const int pieces = (c.neff + 31) / 32, p0 = chalf ? (pieces + 1) / 2 : 0, p1 = chalf ? pieces : (pieces + 1) / 2;
