@@ -177,7 +177,6 @@ constexpr int kPrepareWords = 32;
 template <typename T, bool MX, bool ALIGNED, int ROWS>
 __global__ void __launch_bounds__(kQuantThreads)
 fp4_prepare_kernel(const T* __restrict__ x, const __grid_constant__ PrepareParams p) {
-  __shared__ uint4 tile[kPrepareWords][32];
   asm volatile("griddepcontrol.launch_dependents;");   // the product may set itself up; it waits for this grid before it reads
   const int t = threadIdx.x;
   if (blockIdx.x < p.scale_blocks) {
@@ -186,37 +185,33 @@ fp4_prepare_kernel(const T* __restrict__ x, const __grid_constant__ PrepareParam
       const long long n = p.size_bytes == 8 ? __ldg(static_cast<const long long*>(p.sizes) + e) : (long long)__ldg(static_cast<const int*>(p.sizes) + e);
       if (n <= 0) return;
     }
-    // two threads per row, 64 bytes each
-    const int r = t >> 1, w0 = wb * kPrepareWords + (t & 1) * 16;
+    // a thread: rows lane, lane + 32, lane + 64, lane + 96 of four words, which are the four 16-byte pieces that it writes
+    const int lane = t & 31, w0 = wb * kPrepareWords + (t >> 5) * 4;
     const int64_t left = p.sf_row - (int64_t)w0 * 4;
-    const uint8_t* from = p.scales + ((int64_t)e * p.N + n0 + r) * p.sf_row + (int64_t)w0 * 4;
     uint4 v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = make_uint4(0, 0, 0, 0);
-      if (n0 + r < p.N && left > 16 * i) {
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + 32 * j + lane;
+      v[j] = make_uint4(0, 0, 0, 0);
+      if (n < p.N && left > 0) {
+        const uint8_t* from = p.scales + ((int64_t)e * p.N + n) * p.sf_row + (int64_t)w0 * 4;
         if (p.aligned) {
-          v[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
+          v[j] = __ldg(reinterpret_cast<const uint4*>(from));
         } else {
-          uint32_t* word = &v[i].x;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (left > 16 * i + 4 * k) word[k] = load4_any(from + 16 * i + 4 * k, left - 16 * i - 4 * k);
+          v[j].x = load4_any(from, left);
+          if (left > 4) v[j].y = load4_any(from + 4, left - 4);
+          if (left > 8) v[j].z = load4_any(from + 8, left - 8);
+          if (left > 12) v[j].w = load4_any(from + 12, left - 12);
         }
       }
     }
-    uint32_t* put = reinterpret_cast<uint32_t*>(&tile[(t & 1) * 16][r & 31]) + (r >> 5);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      put[(4 * i) * 128] = v[i].x;
-      put[(4 * i + 1) * 128] = v[i].y;
-      put[(4 * i + 2) * 128] = v[i].z;
-      put[(4 * i + 3) * 128] = v[i].w;
+    uint4* out = reinterpret_cast<uint4*>(p.sfw) + ((int64_t)rb * p.words + w0) * 32 + lane;
+    if (w0 < p.words) {   // (a multiple of 8)
+      out[0] = make_uint4(v[0].x, v[1].x, v[2].x, v[3].x);
+      out[32] = make_uint4(v[0].y, v[1].y, v[2].y, v[3].y);
+      out[64] = make_uint4(v[0].z, v[1].z, v[2].z, v[3].z);
+      out[96] = make_uint4(v[0].w, v[1].w, v[2].w, v[3].w);
     }
-    __syncthreads();
-    uint4* out = reinterpret_cast<uint4*>(p.sfw) + ((int64_t)rb * p.words + wb * kPrepareWords) * 32;
-    const int n = min(kPrepareWords, p.words - wb * kPrepareWords) * 32;
-    for (int i = t; i < n; i += kQuantThreads) out[i] = tile[i >> 5][i & 31];
     return;
   }
   const int64_t b = blockIdx.x - p.scale_blocks, row0 = b / p.blocks_per_row * ROWS;
