@@ -1,6 +1,6 @@
 // C++ host shim over the C ABI of b200q.h with the shape of the reference's operator functions
 // (mlx/ops.cpp: quantize :5208-5245, dequantize :5465-5517, quantized_matmul :4784-4834,
-// gather_qmm :5553-5629): same argument meaning, same validation (mlx/ops.cpp:110-181,
+// gather_qmm :5553-5629; qqmm and the grouped products in the same manner): same argument meaning, same validation (mlx/ops.cpp:110-181,
 // 4704-4754), std::invalid_argument where the reference throws it and std::runtime_error for
 // everything the library reports later.  Arrays are non-owning views of row-contiguous device
 // memory; outputs and scratch are allocated by the caller (the reference's eval_gpu does that
@@ -17,17 +17,20 @@
 
 namespace b200q {
 
-enum class Dtype : int { float32 = B200Q_F32, float16 = B200Q_F16, bfloat16 = B200Q_BF16, uint32 = 100 };
+enum class Dtype : int { float32 = B200Q_F32, float16 = B200Q_F16, bfloat16 = B200Q_BF16, uint32 = 100, uint8 = 101, int32 = 102, int64 = 103 };
 
 inline const char* name(Dtype t) {
   switch (t) {
     case Dtype::float32: return "float32";
     case Dtype::float16: return "float16";
     case Dtype::bfloat16: return "bfloat16";
+    case Dtype::uint8: return "uint8";
+    case Dtype::int32: return "int32";
+    case Dtype::int64: return "int64";
     default: return "uint32";
   }
 }
-inline bool is_floating(Dtype t) { return t != Dtype::uint32; }
+inline bool is_floating(Dtype t) { return (int)t < (int)Dtype::uint32; }
 
 // Row-contiguous device array: shape + dtype + pointer.
 struct ArrayView {
@@ -195,6 +198,111 @@ inline void gather_qmm(const ArrayView& x, const ArrayView& w, const ArrayView& 
                                  static_cast<const uint32_t*>(lhs_indices.data), static_cast<const uint32_t*>(rhs_indices.data),
                                  lhs_indices.size(), out.data, (int)x.dtype, x_batch, E, M, N, K, group_size, bits, transpose ? 1 : 0,
                                  sorted_indices ? 3 : 0, ws.data, ws.bytes, stream));
+}
+
+// ---- microscaled 4-bit floating point (b200q_fp4_quantize says how values are rounded)
+enum class Fp4 : int { mxfp4 = B200Q_MXFP4, nvfp4 = B200Q_NVFP4 };
+namespace detail {
+inline int group(Fp4 mode) { return mode == Fp4::mxfp4 ? 32 : 16; }
+// wq [.., K/8] uint32 and scales [.., K/group] uint8
+inline void validate_fp4(const char* tag, const ArrayView& wq, const ArrayView& scales, Fp4 mode) {
+  if (wq.dtype != Dtype::uint32 || scales.dtype != Dtype::uint8)
+    throw std::invalid_argument(std::string("[") + tag + "] the weight matrix should be uint32 and its scales uint8 but are " + name(wq.dtype) +
+                                " and " + name(scales.dtype));
+  bool ok = wq.ndim() >= 2 && scales.ndim() == wq.ndim() && wq.dim(-1) * 8 == scales.dim(-1) * group(mode);
+  for (int i = 0; ok && i < wq.ndim() - 1; ++i) ok = wq.shape[i] == scales.shape[i];
+  if (!ok)
+    throw std::invalid_argument(std::string("[") + tag + "] The shapes of the weight and scales are incompatible: " + shape_str(wq.shape) + " and " +
+                                shape_str(scales.shape) + " with 4 bits in groups of " + std::to_string(group(mode)));
+}
+// A global scale (or an empty view: none): one float32, or one per matrix where `each` says how many there are.
+inline const float* global_scale(const char* tag, const ArrayView& g, Fp4 mode, int64_t each) {
+  if (!g.data) return nullptr;
+  if (mode != Fp4::nvfp4 || g.dtype != Dtype::float32 || (g.size() != 1 && g.size() != each))
+    throw std::invalid_argument(std::string("[") + tag + "] a global scale is one float32 (or one per matrix) and belongs to nvfp4");
+  return static_cast<const float*>(g.data);
+}
+inline int64_t matrices(const ArrayView& a) {
+  int64_t n = 1;
+  for (int i = 0; i < a.ndim() - 2; ++i) n *= a.shape[i];
+  return n;
+}
+inline int size_bytes(const char* tag, const ArrayView& sizes, int64_t groups) {
+  if ((sizes.dtype != Dtype::int32 && sizes.dtype != Dtype::int64) || sizes.ndim() != 1 || sizes.dim(0) != groups)
+    throw std::invalid_argument(std::string("[") + tag + "] one integral group size per expert is needed");
+  return sizes.dtype == Dtype::int64 ? 8 : 4;
+}
+}  // namespace detail
+
+// w [.., K] -> wq, scales
+inline void quantize(const ArrayView& w, ArrayView& wq, ArrayView& scales, Fp4 mode, const ArrayView& global_scale = {}, void* stream = nullptr) {
+  if (!is_floating(w.dtype))
+    throw std::invalid_argument(std::string("[quantize] Only real floating types can be quantized but w has type ") + name(w.dtype) + ".");
+  detail::validate_fp4("quantize", wq, scales, mode);
+  const int64_t K = w.dim(-1), rows = K ? w.size() / K : 0;
+  const float* g = detail::global_scale("quantize", global_scale, mode, detail::matrices(w));
+  detail::check(b200q_fp4_quantize(w.data, (int)w.dtype, rows, K, (int)mode, g, global_scale.size() == 1 || !g ? (rows ? rows : 1) : w.dim(-2),
+                                   static_cast<uint32_t*>(wq.data), static_cast<uint8_t*>(scales.data), stream));
+}
+
+// wq, scales -> out [.., K] in out's type
+inline void dequantize(const ArrayView& wq, const ArrayView& scales, ArrayView& out, Fp4 mode, const ArrayView& global_scale = {},
+                       void* stream = nullptr) {
+  detail::validate_fp4("dequantize", wq, scales, mode);
+  const int64_t K = wq.dim(-1) * 8, rows = wq.dim(-1) ? wq.size() / wq.dim(-1) : 0;
+  const float* g = detail::global_scale("dequantize", global_scale, mode, detail::matrices(wq));
+  detail::check(b200q_fp4_dequantize(static_cast<const uint32_t*>(wq.data), static_cast<const uint8_t*>(scales.data), (int)mode, g,
+                                     global_scale.size() == 1 || !g ? (rows ? rows : 1) : wq.dim(-2), (int)out.dtype, rows, K, out.data, stream));
+}
+
+// x [.., K] times the transpose of w [N, K/8], x quantized on the way
+inline void qqmm(const ArrayView& x, const ArrayView& w, const ArrayView& scales, ArrayView& out, const Workspace& ws, Fp4 mode,
+                 const ArrayView& global_scale_x = {}, const ArrayView& global_scale_w = {}, void* stream = nullptr) {
+  detail::validate_fp4("qqmm", w, scales, mode);
+  const int64_t K = w.dim(-1) * 8;
+  if (w.ndim() != 2 || x.ndim() < 1 || x.dim(-1) != K || !is_floating(x.dtype))
+    throw std::invalid_argument("[qqmm] x " + detail::shape_str(x.shape) + " does not match the matrix w " + detail::shape_str(w.shape));
+  detail::check(b200q_grouped_qqmm(x.data, static_cast<const uint32_t*>(w.data), static_cast<const uint8_t*>(scales.data), nullptr, 0, out.data,
+                                   (int)x.dtype, K ? x.size() / K : 0, 1, w.dim(0), K, (int)mode,
+                                   detail::global_scale("qqmm", global_scale_x, mode, 1), detail::global_scale("qqmm", global_scale_w, mode, 1), 0,
+                                   ws.data, ws.bytes, stream));
+}
+
+// Rows of x [T, K] sorted by expert, w [E, N, K/8]; sizes [E] on the device
+inline void grouped_qqmm(const ArrayView& x, const ArrayView& w, const ArrayView& scales, const ArrayView& sizes, ArrayView& out,
+                         const Workspace& ws, Fp4 mode, const ArrayView& global_scale_x = {}, const ArrayView& global_scale_w = {},
+                         void* stream = nullptr) {
+  detail::validate_fp4("grouped_qqmm", w, scales, mode);
+  if (w.ndim() != 3 || x.ndim() != 2 || x.dim(1) != w.dim(2) * 8 || !is_floating(x.dtype))
+    throw std::invalid_argument("[grouped_qqmm] x " + detail::shape_str(x.shape) + " does not match the matrices w " + detail::shape_str(w.shape));
+  const int bytes = detail::size_bytes("grouped_qqmm", sizes, w.dim(0));
+  detail::check(b200q_grouped_qqmm(x.data, static_cast<const uint32_t*>(w.data), static_cast<const uint8_t*>(scales.data), sizes.data, bytes,
+                                   out.data, (int)x.dtype, x.dim(0), w.dim(0), w.dim(1), x.dim(1), (int)mode,
+                                   detail::global_scale("grouped_qqmm", global_scale_x, mode, 1),
+                                   detail::global_scale("grouped_qqmm", global_scale_w, mode, w.dim(0)), global_scale_w.size() > 1, ws.data, ws.bytes,
+                                   stream));
+}
+
+// Rows of x [T, K] sorted by expert, 16-bit w [E, N, K] (transpose) or [E, K, N]; sizes [E] on the device.  The gradient with respect
+// to x is the same call on the cotangent with `transpose` inverted.
+inline void grouped_mm(const ArrayView& x, const ArrayView& w, const ArrayView& sizes, ArrayView& out, const Workspace& ws, bool transpose = true,
+                       void* stream = nullptr) {
+  if (w.ndim() != 3 || x.ndim() != 2 || x.dim(1) != w.dim(transpose ? 2 : 1) || x.dtype != w.dtype)
+    throw std::invalid_argument("[grouped_mm] x " + detail::shape_str(x.shape) + " does not match the matrices w " + detail::shape_str(w.shape));
+  const int bytes = detail::size_bytes("grouped_mm", sizes, w.dim(0));
+  detail::check(b200q_grouped_mm(x.data, w.data, sizes.data, bytes, out.data, (int)x.dtype, x.dim(0), w.dim(0), w.dim(transpose ? 1 : 2), x.dim(1),
+                                 transpose ? 1 : 0, ws.data, ws.bytes, stream));
+}
+
+// The gradient of grouped_mm with respect to w, in w's layout
+inline void grouped_mm_dw(const ArrayView& dy, const ArrayView& x, const ArrayView& sizes, ArrayView& dw, const Workspace& ws, bool transpose = true,
+                          void* stream = nullptr) {
+  if (dy.ndim() != 2 || x.ndim() != 2 || dy.dim(0) != x.dim(0) || dy.dtype != x.dtype || sizes.ndim() != 1)
+    throw std::invalid_argument("[grouped_mm_dw] dy and x must be matrices of one type with as many rows");
+  const int bytes = detail::size_bytes("grouped_mm_dw", sizes, sizes.dim(0));
+  const ArrayView &a = transpose ? dy : x, &b = transpose ? x : dy;
+  detail::check(b200q_grouped_mm_dw(a.data, b.data, sizes.data, bytes, dw.data, (int)x.dtype, x.dim(0), sizes.dim(0), a.dim(1), b.dim(1), ws.data,
+                                    ws.bytes, stream));
 }
 
 }  // namespace b200q

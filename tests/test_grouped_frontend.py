@@ -1,5 +1,8 @@
 """Refusals of the microscaled modes and the grouped products: ValueError before any device work, on the host alone."""
 import ctypes
+import os
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -110,3 +113,13 @@ def test_the_c_abi_refuses_before_any_cuda_call():
         d, wq, d, sizes, 8, d, _lib.BF16, 4, E, 8, K, mode, gx, None, 0, ws, 1 << 30, None)
     assert qq(E=2) == qq(wq=odd) == qq(K=33) == qq(mode=9) == qq(gx=d) == qq(wq=None) == bad
     assert qq(ws=None) == ws_err
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_the_cpp_shim_compiles_and_refuses(tmp_path):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe, libdir = str(tmp_path / "check"), os.path.dirname(_lib.LIB_PATH)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", os.path.join(root, "include"), os.path.join(root, "tests", "grouped_shim_check.cpp"), "-o", exe,
+                    "-L", libdir, "-lb200q", f"-Wl,-rpath,{libdir}"], check=True, capture_output=True, text=True)
+    res = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert res.returncode == 0 and "SHIM-OK" in res.stdout, res.stdout + res.stderr
