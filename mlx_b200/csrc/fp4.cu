@@ -278,26 +278,42 @@ fp4_dequantize_kernel(const uint32_t* __restrict__ wq, const uint8_t* __restrict
   }
 }
 
-// A thread makes 16 bytes of a destination row from the aligned words that hold them.
+// A thread makes kPacked times 16 bytes of destination rows, each from the aligned words that hold them.  Index: 32 bits where they
+// are enough (with a 64-bit division per 16 bytes the divisions took longer than the copy).
+constexpr int kPacked = 4;
+template <typename Index>
 __global__ void __launch_bounds__(256) repack_rows_kernel(const uint8_t* __restrict__ src, int64_t src_bytes, uint8_t* __restrict__ dst,
-                                                          int64_t dst_pitch, int64_t pieces_per_row, int64_t pieces) {
-  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (u >= pieces) return;
-  const int64_t row = u / pieces_per_row, at = (u - row * pieces_per_row) * 16;
-  const uint8_t* from = src + row * src_bytes + at;
-  const int64_t left = src_bytes - at;   // bytes of the row from here on
-  const int sh = (int)(reinterpret_cast<uintptr_t>(from) & 3);
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(from - sh);
-  uint32_t v[5], r[4];
+                                                          int64_t dst_pitch, Index pieces_per_row, Index pieces) {
+  const Index u0 = (Index)blockIdx.x * (256 * kPacked) + threadIdx.x;
+  uint32_t v[kPacked][5];
+  int sh[kPacked];
+  int64_t left[kPacked], to[kPacked];
 #pragma unroll
-  for (int i = 0; i < 5; ++i) v[i] = 4 * i - sh < left && 4 * i - sh < 16 ? __ldg(w + i) : 0u;   // words that hold a byte of the piece
+  for (int j = 0; j < kPacked; ++j) {
+    const Index u = u0 + j * 256;
+    if (u >= pieces) break;
+    const Index row = u / pieces_per_row;
+    const int64_t at = (int64_t)(u - row * pieces_per_row) * 16;
+    const uint8_t* from = src + (int64_t)row * src_bytes + at;
+    left[j] = src_bytes - at;   // bytes of the row from here on
+    to[j] = (int64_t)row * dst_pitch + at;
+    sh[j] = (int)(reinterpret_cast<uintptr_t>(from) & 3);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(from - sh[j]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t n = left - 4 * i;
-    r[i] = __funnelshift_r(v[i], v[i + 1], 8 * sh);
-    if (n < 4) r[i] = n <= 0 ? 0u : r[i] & (0xFFFFFFFFu >> (32 - 8 * (int)n));
+    for (int i = 0; i < 5; ++i) v[j][i] = 4 * i - sh[j] < left[j] && 4 * i - sh[j] < 16 ? __ldg(w + i) : 0u;   // words that hold a byte of the piece
   }
-  *reinterpret_cast<uint4*>(dst + row * dst_pitch + at) = make_uint4(r[0], r[1], r[2], r[3]);
+#pragma unroll
+  for (int j = 0; j < kPacked; ++j) {
+    if (u0 + j * 256 >= pieces) break;
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t n = left[j] - 4 * i;
+      r[i] = __funnelshift_r(v[j][i], v[j][i + 1], 8 * sh[j]);
+      if (n < 4) r[i] = n <= 0 ? 0u : r[i] & (0xFFFFFFFFu >> (32 - 8 * (int)n));
+    }
+    *reinterpret_cast<uint4*>(dst + to[j]) = make_uint4(r[0], r[1], r[2], r[3]);
+  }
 }
 
 template <class F>
@@ -378,10 +394,14 @@ int fp4_prepare(const Fp4Prepare& a, cudaStream_t st) {
 }
 
 int repack_rows(const void* src, int64_t src_bytes, void* dst, int64_t dst_pitch, int64_t rows, cudaStream_t st) {
-  const int64_t per = dst_pitch / 16, pieces = per * rows, blocks = (pieces + 255) / 256;
+  const int64_t per = dst_pitch / 16, pieces = per * rows, blocks = (pieces + 256 * kPacked - 1) / (256 * kPacked);
   if (blocks > kMostBlocks) return fail(B200Q_ERR_UNSUPPORTED, "[grouped product] No implementation for problem shape: too many values");
-  repack_rows_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const uint8_t*>(src), src_bytes, static_cast<uint8_t*>(dst), dst_pitch,
-                                                       per, pieces);
+  const uint8_t* from = static_cast<const uint8_t*>(src);
+  uint8_t* to = static_cast<uint8_t*>(dst);
+  if (pieces < (int64_t)UINT32_MAX - 256 * kPacked)
+    repack_rows_kernel<uint32_t><<<(unsigned)blocks, 256, 0, st>>>(from, src_bytes, to, dst_pitch, (uint32_t)per, (uint32_t)pieces);
+  else
+    repack_rows_kernel<uint64_t><<<(unsigned)blocks, 256, 0, st>>>(from, src_bytes, to, dst_pitch, (uint64_t)per, (uint64_t)pieces);
   B200Q_LAUNCH_OK("repack_rows_kernel");
   return B200Q_OK;
 }
