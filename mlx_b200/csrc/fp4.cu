@@ -18,9 +18,13 @@ namespace {
 
 constexpr int kUnit = 16;   // consecutive values of a thread: a whole nvfp4 group, half an mxfp4 one
 
-// 16 values at `at` (which is 16-byte aligned: ALIGNED; else aligned to its type only).
+// Bits of the larger magnitude (fp32 bits with the sign cleared are ordered as the numbers are, infinities and NaNs last).
+__device__ __forceinline__ uint32_t larger(uint32_t top, float v) { return max(top, __float_as_uint(v) & 0x7FFFFFFFu); }
+
+// 16 values at `at` (which is 16-byte aligned: ALIGNED; else aligned to its type only), and the largest magnitude's bits.
 template <typename T, bool ALIGNED>
-__device__ __forceinline__ void load_unit(const T* at, float (&v)[kUnit]) {
+__device__ __forceinline__ uint32_t load_unit(const T* at, float (&v)[kUnit]) {
+  uint32_t top = 0;
   if constexpr (ALIGNED) {
     uint4 raw[sizeof(T)];
 #pragma unroll
@@ -30,20 +34,32 @@ __device__ __forceinline__ void load_unit(const T* at, float (&v)[kUnit]) {
       const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
       if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[4 * i + j] = __uint_as_float(w[j]);
+        for (int j = 0; j < 4; ++j) {
+          v[4 * i + j] = __uint_as_float(w[j]);
+          top = larger(top, v[4 * i + j]);
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const T* e = reinterpret_cast<const T*>(&w[j]);
           v[8 * i + 2 * j] = Elem<T>::to_float(e[0]);
           v[8 * i + 2 * j + 1] = Elem<T>::to_float(e[1]);
+          top = __vmaxu2(top, w[j] & 0x7FFF7FFFu);   // two at a time, in their own bits
         }
       }
     }
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t most = max(top & 0xFFFFu, top >> 16);
+      top = __float_as_uint(Elem<T>::to_float(reinterpret_cast<const T&>(most))) & 0x7FFFFFFFu;
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i) v[i] = Elem<T>::to_float(at[i]);
+    for (int i = 0; i < kUnit; ++i) {
+      v[i] = Elem<T>::to_float(at[i]);
+      top = larger(top, v[i]);
+    }
   }
+  return top;
 }
 
 // Eight codes, lowest bits first.
@@ -81,11 +97,7 @@ __device__ __forceinline__ float e8m0_value(uint32_t code) {
 
 // Scale code and codes of a thread's 16 values.  MX: lanes 2i and 2i + 1 share a group; the whole warp calls.
 template <bool MX>
-__device__ __forceinline__ uint32_t quantize_unit(float (&v)[kUnit], float G, uint32_t (&codes)[2]) {
-  // The largest magnitude by its bits, which are ordered as the numbers are, infinities and NaNs last.
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < kUnit; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+__device__ __forceinline__ uint32_t quantize_unit(float (&v)[kUnit], uint32_t top, float G, uint32_t (&codes)[2]) {
   if constexpr (MX) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
   const bool odd = top >= 0x7F800000u;
   uint32_t s;
@@ -99,16 +111,15 @@ __device__ __forceinline__ uint32_t quantize_unit(float (&v)[kUnit], float G, ui
   } else {
     s = e4m3(fminf(__fdiv_rn(__uint_as_float(top), 6.0f * G), 448.0f));
     const float d = e4m3_value(s) * G;
-    if (d > 0x1p-100f && d < 0x1p100f && s < 0x7Eu) {
-      // Quotients rounded as a division rounds them (Markstein, 1990): with r the rounded reciprocal, q + (x - q d) r is the
-      // rounded quotient once q is within one unit of it, which the first correction makes it.  Not scaled down to 448, a
-      // quotient is at most 7.
+    if (d > 0x1p-100f && d < 0x1p100f && __uint_as_float(top) < 0x1p20f * d) {
+      // Quotients rounded as a division rounds them (Markstein, 1990): with r the rounded reciprocal, q - (q d - x) r is the
+      // rounded quotient once q is within one unit of it, which the first correction makes it.
       const float r = __frcp_rn(d);
 #pragma unroll
       for (int i = 0; i < kUnit; ++i) {
-        float q = v[i] * r;
-        q = fmaf(fmaf(-q, d, v[i]), r, q);
-        v[i] = copysignf(fmaf(fmaf(-q, d, v[i]), r, q), v[i]);   // (of -0 too)
+        float q = v[i] * r;                      // (the remainders' signs are such that -0 stays -0)
+        q = fmaf(-fmaf(q, d, -v[i]), r, q);
+        v[i] = fmaf(-fmaf(q, d, -v[i]), r, q);
       }
     } else {
 #pragma unroll 1
@@ -135,12 +146,13 @@ fp4_quantize_kernel(const T* __restrict__ w, int64_t units, const float* __restr
   const int64_t u = (int64_t)blockIdx.x * kQuantThreads + threadIdx.x;
   const bool in = u < units;
   float v[kUnit];
-  if (in) load_unit<T, ALIGNED>(w + u * kUnit, v);
+  uint32_t top = 0;
+  if (in) top = load_unit<T, ALIGNED>(w + u * kUnit, v);
   else
     for (int i = 0; i < kUnit; ++i) v[i] = 0.0f;
-  const float G = !MX && global && in ? __ldg(global + u / units_per_global) : 1.0f;
+  const float G = !MX && global && in ? __ldg(global + (units_per_global < units ? u / units_per_global : 0)) : 1.0f;
   uint32_t codes[2];
-  const uint32_t s = quantize_unit<MX>(v, G, codes);
+  const uint32_t s = quantize_unit<MX>(v, top, G, codes);
   if (!in) return;
   wq[u] = make_uint2(codes[0], codes[1]);
   if (!MX) scales[u] = (uint8_t)s;
@@ -218,9 +230,11 @@ fp4_prepare_kernel(const T* __restrict__ x, const __grid_constant__ PrepareParam
   const int64_t u = (b % p.blocks_per_row) * kQuantThreads + t, k = u * kUnit;
   const bool in = k < p.K;
   float v[ROWS][kUnit];
+  uint32_t top[ROWS];
 #pragma unroll
   for (int j = 0; j < ROWS; ++j) {
-    if (in && row0 + j < p.T) load_unit<T, ALIGNED>(x + (row0 + j) * p.K + k, v[j]);
+    top[j] = 0;
+    if (in && row0 + j < p.T) top[j] = load_unit<T, ALIGNED>(x + (row0 + j) * p.K + k, v[j]);
     else
       for (int i = 0; i < kUnit; ++i) v[j][i] = 0.0f;
   }
@@ -229,7 +243,7 @@ fp4_prepare_kernel(const T* __restrict__ x, const __grid_constant__ PrepareParam
   for (int j = 0; j < ROWS; ++j) {
     const int64_t row = row0 + j;
     uint32_t codes[2];
-    uint32_t s = quantize_unit<MX>(v[j], G, codes);
+    uint32_t s = quantize_unit<MX>(v[j], top[j], G, codes);
     if (row >= p.T) return;   // (of the whole block)
     if (in) *reinterpret_cast<uint2*>(p.codes + row * p.code_pitch + k / 2) = make_uint2(codes[0], codes[1]);
     else s = 0;
@@ -240,40 +254,43 @@ fp4_prepare_kernel(const T* __restrict__ x, const __grid_constant__ PrepareParam
   }
 }
 
-// A thread takes kAhead pieces of 8 values, kQuantThreads apart, whose codes and scales are all on their way before the first is
-// used: 16-byte stores, whole lines per warp.  (A thread per 16 values: 28672 x 8192 bf16 in 122 us.)
+// A thread takes kAhead pieces of 16 bytes of values, kQuantThreads apart, whose codes and scales are all on their way before the
+// first is used: whole lines per warp in every access.  (A thread per 16 values: 28672 x 8192 bf16 in 122 us, now 92; fp32 values
+// in pairs of stores 32 bytes apart: 4.4 TB/s.)
 constexpr int kAhead = 4;
 template <typename T, bool MX, bool ALIGNED>
 __global__ void __launch_bounds__(kQuantThreads)
 fp4_dequantize_kernel(const uint32_t* __restrict__ wq, const uint8_t* __restrict__ scales, int64_t pieces,
                       const float* __restrict__ global, int64_t pieces_per_global, T* __restrict__ out) {
+  constexpr int kValues = 16 / sizeof(T), kPerGroup = (MX ? 32 : 16) / kValues;
+  using Code = typename std::conditional<kValues == 8, uint32_t, uint16_t>::type;
   const int64_t p0 = (int64_t)blockIdx.x * (kQuantThreads * kAhead) + threadIdx.x;
   uint32_t c[kAhead], code[kAhead];
 #pragma unroll
   for (int j = 0; j < kAhead; ++j) {
     const int64_t p = p0 + j * kQuantThreads;
-    c[j] = p < pieces ? __ldg(wq + p) : 0u;
-    code[j] = p < pieces ? __ldg(scales + (MX ? p >> 2 : p >> 1)) : 0u;
+    c[j] = p < pieces ? __ldg(reinterpret_cast<const Code*>(wq) + p) : 0u;
+    code[j] = p < pieces ? __ldg(scales + p / kPerGroup) : 0u;
   }
 #pragma unroll
   for (int j = 0; j < kAhead; ++j) {
     const int64_t p = p0 + j * kQuantThreads;
     if (p >= pieces) return;
-    const float s = MX ? e8m0_value(code[j]) : e4m3_value(code[j]), G = !MX && global ? __ldg(global + p / pieces_per_global) : 1.0f;
-    alignas(16) T r[8];
+    const float s = MX ? e8m0_value(code[j]) : e4m3_value(code[j]);
+    const float G = !MX && global ? __ldg(global + (pieces_per_global < pieces ? p / pieces_per_global : 0)) : 1.0f;
+    alignas(16) T r[kValues];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kValues / 2; ++i) {
       const float2 q = e2m1x2_value(c[j] >> (8 * i));
       r[2 * i] = Elem<T>::from_float(q.x * s * G);
       r[2 * i + 1] = Elem<T>::from_float(q.y * s * G);
     }
-    T* at = out + p * 8;
+    T* at = out + p * kValues;
     if constexpr (ALIGNED) {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(at)[i] = reinterpret_cast<const uint4*>(r)[i];
+      *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(r);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) at[i] = r[i];
+      for (int i = 0; i < kValues; ++i) at[i] = r[i];
     }
   }
 }
@@ -353,13 +370,14 @@ int fp4_quantize(const void* w, int dtype, int64_t rows, int64_t K, int mode, co
 
 int fp4_dequantize(const uint32_t* wq, const uint8_t* scales, int mode, const float* global, int64_t rows_per_global, int dtype,
                    int64_t rows, int64_t K, void* out, cudaStream_t st) {
-  const int64_t pieces = rows * (K / 8), blocks = (pieces + kQuantThreads * kAhead - 1) / (kQuantThreads * kAhead);
+  const int values = 16 / (int)dtype_size(dtype);
+  const int64_t pieces = rows * (K / values), blocks = (pieces + kQuantThreads * kAhead - 1) / (kQuantThreads * kAhead);
   if (blocks > kMostBlocks) return fail(B200Q_ERR_UNSUPPORTED, "[dequantize] No implementation for problem shape: too many values");
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     return with_flags(mode, aligned16(out), [&](auto mx, auto al) {
       fp4_dequantize_kernel<T, decltype(mx)::value, decltype(al)::value><<<(unsigned)blocks, kQuantThreads, 0, st>>>(
-          wq, scales, pieces, global, rows_per_global * (K / 8), static_cast<T*>(out));
+          wq, scales, pieces, global, rows_per_global * (K / values), static_cast<T*>(out));
       B200Q_LAUNCH_OK("fp4_dequantize_kernel");
       return B200Q_OK;
     });
