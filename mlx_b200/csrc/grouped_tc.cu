@@ -2,31 +2,41 @@
 //   KK   out[t, i] = sum_k a[e, i, k] b[t, k]      the weights' reduced dimension is contiguous
 //   MK   out[t, i] = sum_k a[e, k, i] b[t, k]      the weights' output dimension is contiguous
 //   MM   out[e, j, i] = sum_t a[t, i] b[t, j]      gradient of the weights: the sum goes over the group's rows
-//   Mx, Nv  as KK, a and b in microscaled 4-bit floating point (fp4.cuh), times the operands' global scales
+//   Mx, Nv  as KK, a and b in microscaled 4-bit floating point (fp4.cu), times the operands' global scales
 // One group without sizes is the dense product.
 //
 // D[i, j] has the output's contiguous dimension on the accumulator's lanes (256 over a pair of thread blocks, cta_group::2)
 // and up to 256 rows of the output as columns: a tile costs what its rows cost, in steps of 16, so ragged groups and
-// single tokens need no other kernel.  Each block of the pair fetches 128 of the i and half of the j; 16-bit operands need
-// 64 bytes per clock and SM that way, the L2's rate, where a block of its own would need 94.
+// single tokens need no other kernel.  Each block of the pair fetches 128 of the i and half of the j: 64 bytes per clock
+// and SM at the tensor cores' full rate, where a block of its own would need 94.
 //
-//   warps 0, 3  TMA: a's and b's tile of a stage (128 bytes of k per row; MM and MK: 64 k)
+//   warps 0, 3  TMA: a's and b's tile of a stage (128 bytes of k per row; MM and MK: 64 k).  A copy costs its thread 100 to 200
+//               cycles, so that one warp for both was the bound of MM
 //   warp 1      tcgen05.mma (leader block, one thread)
-//   warp 2      4 bits: tcgen05.cp of the scales, three per 4 k of 256 rows (leader, one thread: with them in warp 1 a stage's
-//               instructions took it longer than its MMAs take).  MM: the stage that a group ends in has its foreign rows zeroed in shared memory (both operands: a foreign
-//               infinity times zero would be NaN).  Only those stages go through this warp: with all of them handed on by it
-//               a step of the ring took 1600 cycles instead of 700
-//   warps 4-11  epilogue: accumulator -> rounding -> stmatrix staging -> 16-byte stores; MM, whose tiles have few stages and are
-//               stored as fast as they are multiplied: TMA stores of 128-byte rows
+//   warp 2      4 bits: tcgen05.cp of the scales, two or three per 4 scales of 256 rows (leader, one thread: with them in warp
+//               1 a stage's instructions took it longer than its MMAs take).  MM: the stage that a group ends in has its
+//               foreign rows zeroed in shared memory, in both operands (a foreign infinity times zero would be NaN).  Only
+//               those stages go through this warp: with all of them handed on by it a step of the ring took 1600 cycles
+//               instead of 700
+//   warps 4-11  epilogue: the accumulator is rounded and packed in registers, which frees it for another tile, then goes through
+//               stmatrix staging to 16-byte stores.  MM, whose tiles have few stages and are stored as fast as they are
+//               multiplied: TMA stores of 32 whole lines
 //   warps 12-15 4 bits only: b's scales, from words in global memory into the order that tensor memory wants (a's are in that
 //               order already, fp4_prepare_kernel, and come by TMA: warp 3)
 //
 // The table of groups (first row, first tile, first step) is built in shared memory by every block from `sizes`, which the
-// host never reads: no launch in front and no synchronisation.
+// host never reads: no launch in front and no synchronisation.  The roles find their tiles in it through one function (walk_next).
 //
 // Tiles are dealt to the pairs in whole waves.  What is left over is laid end to end and cut into equal ranges of K where
 // that gains more than the partial sums cost; the last pair to arrive adds a tile's parts in order (no atomics on values,
-// the same bits every time), and nobody waits for another pair.
+// the same bits every time), and nobody waits for another pair.  (All tiles in equal ranges instead of whole waves: 5 to 40 %
+// slower, neighbours no longer share operands in L2.)
+//
+// What bounds it, measured (bf16 unless said): many rows, power and the tensor cores, 84 to 86 % of whose cycles are busy
+// (4096 rows of 8 experts [14336, 4096] 363 us, 1320 TFLOP/s; 8192^3 1476); its gradient of the weights the same with 940 MB written
+// (407 us); 4 bits, L2, which delivers 10.2 TB/s (4096 rows through nvfp4 [14336, 4096] 113 us in 124 with fp4_prepare_kernel;
+// half of the MMAs left out: 8 % less); few rows, HBM (8 rows of 5 or 6 experts, 0.95 of its rate) or, below some 20 us, latencies:
+// 4000 to 5000 cycles until the first copy is issued, 2500 until it lands, 4000 for a cut tile's end.
 //
 // Every wait is bounded: when one runs out, the role raises the block's abort flag and the status word, all roles leave, tensor
 // memory is freed and the kernel ends.
