@@ -174,7 +174,8 @@ __device__ __forceinline__ uint32_t load4_any(const uint8_t* at, int64_t left) {
 
 // Operands of a 4-bit product.  The first blocks bring the weights' scales into the order that tensor memory wants: a block
 // has 128 rows and up to 32 words of them.  (Inside the product, warps that read the scales as they lie took 1.3 to 1.6 times as
-// long as its MMAs; few rows of many experts would be 5 % faster that way.)  The others quantize x: up to kQuantThreads units of one row each; four scales become a word.
+// long as its MMAs; few rows of many experts would be 5 % faster that way.)  The others quantize x: up to kQuantThreads units
+// of one or two rows; four scales become a word.
 struct PrepareParams {
   const uint8_t* scales;
   const void* sizes;

@@ -88,7 +88,7 @@ struct Params {
   int E, T;
   int I, J, K;             // output width; MM: output rows per group; length of the sum (MM: unused)
   int NT, i_tiles, stages;
-  int sf_slots;            // 8 up to 128 rows per tile, else 4
+  int sf_slots;            // 8 up to 128 rows per tile, else 4 (less where the table of groups needs the room)
   int b_bytes;             // of a stage's b tile
   int blocks;              // MK, MM: a (b) comes in whole blocks of 64 columns, two in one copy (bit 0: a, bit 1: b)
   int sfb_chunk;           // 4 bits: bytes of a chunk of b's scales
@@ -712,15 +712,16 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
     }
   } else if (kSf && warp >= kScaleWarp0) {
     // ------------------------------------------------------------ b's scales: warps take chunks in turn
-    const uint32_t first = warp - kScaleWarp0, sf_empty = smem_u32(&bars->sf_empty[0]), lsf = leader_addr(smem_u32(&bars->sf_full[0]));
+    // (no more warps than slots, so that none is ahead of a slot's barrier by more than a turn)
+    const uint32_t first = warp - kScaleWarp0, turns = min(kScaleWarps, p.sf_slots), sf_empty = smem_u32(&bars->sf_empty[0]), lsf = leader_addr(smem_u32(&bars->sf_full[0]));
     const int blocks = p.sfb_chunk >> 12;   // of 128 rows: 1 or 2
     uint32_t chunk = 0, sl = first, ph = 1;
     bool ok = true;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    while (ok && next_of_warp()) {
+    while (ok && first < turns && next_of_warp()) {
       const Piece c = walk.c;
       for (int ks = c.ks0; ks < c.ks1; ks += kSpc<KIND>, ++chunk) {
-        if ((chunk & (kScaleWarps - 1)) != first) continue;
+        if ((chunk & (turns - 1)) != first) continue;
         // a lane has rows lane, lane + 32, .. (past the end of b: the last row, for columns that nobody stores)
         const uint32_t* from = p.sfb + (long long)(ks * kSb / 4) * p.T;
         int row[8];
@@ -752,7 +753,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(lsf + sl * 8);
-        sl += kScaleWarps;
+        sl += turns;
         if (sl >= (uint32_t)p.sf_slots) { sl -= p.sf_slots; ph ^= 1; }
       }
     }
@@ -1033,9 +1034,13 @@ int allow_smem(const void* kernel) {
 template <typename T, Kind KIND>
 int launch(const Maps& m, Params& p, cudaStream_t st) {
   const size_t stage = kStageA + (size_t)p.b_bytes;
-  const size_t fixed = 1024 + (kFp4<KIND> ? p.sf_slots * (4096 + (size_t)p.sfb_chunk) : 0) + (sizeof(T) == 2 ? kEpiWarps * kStageOut<KIND> : 0) +
-                       sizeof(Bars) + (size_t)(p.E + 1) * sizeof(Group);
-  p.stages = (int)((kSmemMax - fixed) / stage);
+  const size_t other = 1024 + (sizeof(T) == 2 ? kEpiWarps * kStageOut<KIND> : 0) + sizeof(Bars) + (size_t)(p.E + 1) * sizeof(Group);
+  size_t fixed;
+  for (;; p.sf_slots /= 2) {   // (thousands of groups leave room for fewer scales)
+    fixed = other + (kFp4<KIND> ? p.sf_slots * (4096 + (size_t)p.sfb_chunk) : 0);
+    p.stages = fixed < kSmemMax ? (int)((kSmemMax - fixed) / stage) : 0;
+    if (!kFp4<KIND> || p.stages >= 3 || p.sf_slots == 2) break;
+  }
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   if (p.stages < 3) return fail(B200Q_ERR_UNSUPPORTED, "[grouped product] No implementation for problem shape: the table of %d groups leaves no shared memory", p.E);
   size_t smem = fixed + p.stages * stage;

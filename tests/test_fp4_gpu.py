@@ -230,3 +230,10 @@ def test_grouped_qqmm_skips_experts_without_rows():
     y = mb.grouped_qqmm(x, wq, s, sizes, mode="mxfp4")
     s[1] = 255
     assert torch.equal(y, mb.grouped_qqmm(x, wq, s, sizes, mode="mxfp4")) and torch.isfinite(y).all()
+
+
+def test_grouped_qqmm_of_the_most_groups():
+    """The table of 4096 groups leaves room for few stages and few scales."""
+    E, N, K = 4096, 24, 1088
+    sizes = [3 if e % 13 == 0 else (300 if e == 2000 else 0) for e in range(E)]
+    check_qqmm(sum(sizes), N, K, "nvfp4", "bf16", sizes)
