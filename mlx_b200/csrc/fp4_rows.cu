@@ -1,0 +1,372 @@
+// 4-bit products of up to 16 rows, dense or grouped, in one launch: y[t] = Gx Gw[e] (quantized x[t]) (wq[e], scales[e])^T.
+//
+// Every block quantizes all of x into shared memory, as 16-bit numbers times their group's scale, and goes through its share of
+// the weights once, which lie as the caller has them.  A warp has 16 rows of weights and every 2^split-th piece of 256 k
+// (128 bytes of codes per row, two pieces ahead in registers); codes become 16-bit numbers in place:
+//   sign and three bits, shifted to sign and the lowest exponent and highest mantissa bits, are the f16 number q 2^-14 (bf16: q
+//   2^-126), subnormal 0.5 included; one multiplication by the scale makes it exact
+//   nvfp4  f16, q s 2^-7: at most 21, a multiple of 2^-17, four and two significant bits
+//   mxfp4  bf16, q 2^e; a warp that meets scales above 2 multiplies by 2^126 first, since 2^(e + 126) has no bf16 number then
+// mma.sync (m16n8k16) takes them as A and x as B, sums in fp32; k is in the order in which the codes fall out, for both alike.  Partial
+// sums of the warps that share rows go through shared memory and are added in order.
+//
+// Bound: latencies (launch, x, first weights, last sums) where the weights are few, then instructions and HBM alike.
+#include "fp4.cuh"
+
+namespace b200q {
+namespace {
+
+using namespace fp4;
+
+constexpr int kWarps = 16, kThreads = 32 * kWarps;
+constexpr int kMostRows = 8;       // of x: columns of one product
+constexpr int kPieceK = 256;
+constexpr int kPad = 20;            // floats from token to token of a partial sum: eight lanes of four tokens on 32 banks
+constexpr int kStages = 3;
+constexpr int kRowBytes = 144;      // of codes from row to row of a stage: eight rows' words on 32 banks
+constexpr int kStageBytes = 16 * kRowBytes + 16 * 16;
+constexpr size_t kSmemMax = 227 * 1024 - 1024;
+
+struct RowsParams {
+  const void* x;
+  const uint8_t* wq;
+  const uint8_t* scales;
+  const void* sizes;        // null: one group
+  void* y;
+  const float *gx, *gw;
+  uint32_t* status;
+  int T, E, N, K, size_bytes, gw_each;
+  int tiles;                // of 16 rows of weights, per group
+  int pieces;               // of K
+  int pitch;                // bytes of a row of x in shared memory
+  int x_stride;             // mxfp4: floats from group to group of x's scales there
+};
+
+__device__ __forceinline__ uint32_t times(uint32_t v, uint32_t m) {
+  const __half2 r = __hmul2(reinterpret_cast<const __half2&>(v), reinterpret_cast<const __half2&>(m));
+  return reinterpret_cast<const uint32_t&>(r);
+}
+// The eight codes of a word as four pairs of f16 numbers.
+__device__ __forceinline__ void spread(uint32_t w, uint32_t (&r)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+      : "r"(w));
+}
+// Two E4M3 scales as f16.
+__device__ __forceinline__ uint32_t nv_factors(uint32_t codes) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)codes));
+  return h;
+}
+// Byte q of four E8M0 scales: 2^(code - 127), 255 is NaN (infinity times zero).
+__device__ __forceinline__ float mx_factor(uint32_t codes, int q) {
+  const float f = __uint_as_float(q == 3 ? (codes >> 1) & 0x7F800000u : (codes << (23 - 8 * q)) & 0x7F800000u);
+  return fmaf(f, 0.0f, fmaxf(f, 0x1p-127f));
+}
+
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a0)[4], const uint32_t (&a8)[4], int j, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0[j]), "r"(a8[j]), "r"(a0[j + 1]), "r"(a8[j + 1]), "r"(b0), "r"(b1));
+}
+// N bytes into shared memory, zeros where there are none to read.
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from, bool there) {
+  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(N), "r"(there ? N : 0) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <typename T, bool MX>
+__global__ void __launch_bounds__(kThreads, 1) fp4_rows_kernel(const __grid_constant__ RowsParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int2 first[kMostRows];          // the group that begins with row r: its number and length
+  __shared__ int3 list[kMostRows];           // groups with rows: number, first row, length
+  __shared__ int totals[kWarps], count;
+  float* const sums = reinterpret_cast<float*>(smem + kWarps * kStages * kStageBytes);   // [2][warp][8][kPad]
+  constexpr int kSums = kWarps * 8 * kPad;
+  uint8_t* const xs = reinterpret_cast<uint8_t*>(sums + 2 * kSums);
+  float* const xscales = reinterpret_cast<float*>(xs + (size_t)p.T * p.pitch);   // mxfp4: [group of K][row]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* const stages = smem + warp * (kStages * kStageBytes);
+
+  // ---- groups ----
+  int rows_end = p.T, groups = 1;
+  if (p.sizes) {
+    bool bad = false;
+    auto size_of = [&](int e) -> int {
+      const long long n = p.size_bytes == 8 ? __ldg(static_cast<const long long*>(p.sizes) + e) : (long long)__ldg(static_cast<const int*>(p.sizes) + e);
+      bad |= n < 0 || n > p.T;
+      return n < 0 ? 0 : (n > p.T ? p.T : (int)n);
+    };
+    auto add = [&](int a, int b) { bad |= a + b > p.T; return min(a + b, p.T); };
+    if (tid < kMostRows) first[tid] = make_int2(0, 0);
+    const int per = (p.E + kThreads - 1) / kThreads, lo = min(p.E, tid * per), hi = min(p.E, lo + per);
+    int at = 0;
+    for (int e = lo; e < hi; ++e) at = add(at, size_of(e));
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, at, d);
+      if (lane >= d) at = add(at, v);
+    }
+    if (lane == 31) totals[warp] = at;
+    at = __shfl_up_sync(0xFFFFFFFFu, at, 1);
+    if (lane == 0) at = 0;
+    __syncthreads();
+    int before = 0;
+    rows_end = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp) before = rows_end;
+      rows_end = add(rows_end, totals[w]);
+    }
+    at = add(at, before);
+    for (int e = lo; e < hi; ++e) {
+      const int r0 = at;
+      at = add(at, size_of(e));
+      if (at > r0) first[r0] = make_int2(e, at - r0);
+    }
+    if (bad && blockIdx.x == 0) atomicMax(p.status, 9u);
+    __syncthreads();
+    if (warp == 0) {
+      const int2 f = lane < kMostRows ? first[lane] : make_int2(0, 0);
+      const uint32_t some = __ballot_sync(0xFFFFFFFFu, f.y > 0);
+      if (f.y > 0) list[__popc(some & ((1u << lane) - 1u))] = make_int3(f.x, lane, f.y);
+      if (lane == 0) count = __popc(some);
+    }
+    __syncthreads();
+    groups = count;
+  }
+
+  // ---- who does what: warps of a tile (a power of two), so that the longest way is shortest; a round's end counts as a piece ----
+  const int total = groups * p.tiles;
+  int split = 0, rounds = 0, best = INT_MAX;
+  for (int s = 0; s <= 4; ++s) {
+    const int at_once = (int)gridDim.x << (4 - s), r = (total + at_once - 1) / at_once, c = r * (((p.pieces - 1) >> s) + 2);
+    if (c < best) { best = c; split = s; rounds = r; }
+  }
+  const int part = warp & ((1 << split) - 1), stride = 1 << split;
+
+  // ---- the way through the weights, two pieces ahead: a lane copies 16 bytes of rows lane / 8 + {0, 4, 8, 12}, and scales ----
+  const int from_row = lane >> 3, from_byte = (lane & 7) * 16;
+  constexpr int kScaleCopy = MX ? 4 : 8;      // bytes of 128 k
+  int ahead_round = 0, ahead = part, ahead_slot = 0, rows_left = 0;
+  const uint8_t *w0 = nullptr, *s0 = nullptr;
+  auto tile_of = [&](int round) { return (round * (int)gridDim.x + (int)blockIdx.x) * (kWarps >> split) + (warp >> split); };
+  auto begin_tile = [&]() {
+    const int tile = tile_of(ahead_round);
+    rows_left = 0;
+    w0 = p.wq;
+    s0 = p.scales;
+    if (ahead_round >= rounds || tile >= total) return;
+    const int gi = tile / p.tiles, n = (tile - gi * p.tiles) * 16;
+    const int64_t row = (int64_t)(p.sizes ? list[gi].x : 0) * p.N + n;
+    rows_left = p.N - n;
+    w0 += (row + from_row) * (p.K / 2) + from_byte;
+    s0 += (row + (lane >> 1)) * (p.K / (MX ? 32 : 16)) + (lane & 1) * kScaleCopy;
+  };
+  auto load = [&]() {
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(stages + ahead_slot * kStageBytes);
+    const int k = ahead * kPieceK, left = p.K - k;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool there = from_row + 4 * i < rows_left && from_byte * 2 < left;
+      copy_async<16>(to + (from_row + 4 * i) * kRowBytes + from_byte, there ? w0 + k / 2 + (int64_t)i * 4 * (p.K / 2) : p.wq, there);
+    }
+    const bool there = (lane >> 1) < rows_left && (lane & 1) * 128 < left;
+    copy_async<kScaleCopy>(to + 16 * kRowBytes + lane * kScaleCopy, there ? s0 + k / (MX ? 32 : 16) : p.scales, there);
+    copies_done();
+    ahead_slot = ahead_slot == kStages - 1 ? 0 : ahead_slot + 1;
+    ahead += stride;
+    if (ahead >= p.pieces) {
+      ahead = part;
+      ++ahead_round;
+      begin_tile();
+    }
+  };
+  begin_tile();
+  if (part < p.pieces)
+    for (int i = 0; i < kStages - 1; ++i) load();
+
+  // ---- x ----
+  {
+    const int units = p.T * (p.pieces * (kPieceK / kUnit));
+    const float G = !MX && p.gx ? __ldg(p.gx) : 1.0f;
+    for (int u0 = 0; u0 < units; u0 += kThreads) {
+      const int u = u0 + tid, row = u / (p.pieces * (kPieceK / kUnit)), k = (u - row * (p.pieces * (kPieceK / kUnit))) * kUnit;
+      const bool in = u < units && k < p.K;
+      float v[kUnit];
+      uint32_t top = 0;
+      const T* from = static_cast<const T*>(p.x) + (int64_t)row * p.K + k;
+      if (in) top = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 ? load_unit<T, true>(from, v) : load_unit<T, false>(from, v);
+      else
+        for (int i = 0; i < kUnit; ++i) v[i] = 0.0f;
+      uint32_t codes[2];
+      const uint32_t s = quantize_unit<MX>(v, top, G, codes);
+      if (u >= units) break;
+      uint4* to = reinterpret_cast<uint4*>(xs + (size_t)row * p.pitch + k * 2);
+      const uint32_t f = MX ? 0u : nv_factors(s * 0x0101u);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t r[4];
+        spread(codes[i], r);
+        if (!MX)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) r[j] = times(r[j], f);
+        to[i] = in ? make_uint4(r[0], r[1], r[2], r[3]) : make_uint4(0, 0, 0, 0);
+      }
+      if (MX && (k & 16) == 0) xscales[(k >> 5) * p.x_stride + row] = in ? e8m0_value(s) : 0.0f;
+    }
+  }
+  // rows of no group
+  for (int64_t i = (int64_t)rows_end * p.N + (int64_t)blockIdx.x * kThreads + tid; i < (int64_t)p.T * p.N; i += (int64_t)gridDim.x * kThreads)
+    static_cast<T*>(p.y)[i] = Elem<T>::from_float(0.0f);
+  __syncthreads();
+
+  // ---- products ----
+  const float gx = !MX && p.gx ? __ldg(p.gx) : 1.0f;
+  int slot = 0;
+  for (int round = 0; round < rounds; ++round) {
+    const int tile = tile_of(round), gi = tile < total ? tile / p.tiles : 0, row0 = p.sizes ? list[gi].y : 0;
+    const int len = tile < total ? (p.sizes ? list[gi].z : p.T) : 0;
+    const uint8_t* xrow = xs + (size_t)(row0 + g) * p.pitch + t * 16;
+    const float* xscale = xscales + row0 + 2 * t;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int piece = part; piece < p.pieces; piece += stride) {
+      copies_wait<kStages - 2>();
+      __syncwarp();   // everybody's copies are there, and nobody reads the stage before any more
+      load();
+      const uint8_t* at = stages + slot * kStageBytes;
+      slot = slot == kStages - 1 ? 0 : slot + 1;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* xat = xrow + (piece * 2 + h) * 256;
+        uint32_t codes[2];      // mxfp4: four scales per row
+        uint32_t f[2][4];       // nvfp4: the factor of each word
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint8_t* sat = at + 16 * kRowBytes + (g + 8 * r) * (2 * kScaleCopy) + h * kScaleCopy;
+          if constexpr (MX) {
+            codes[r] = *reinterpret_cast<const uint32_t*>(sat);
+          } else {
+            const uint2 c = *reinterpret_cast<const uint2*>(sat);
+            const uint32_t lo = nv_factors(__byte_perm(c.x, 0, t >> 1 ? 0x31 : 0x20)), hi = nv_factors(__byte_perm(c.y, 0, t >> 1 ? 0x31 : 0x20));
+            f[r][0] = __byte_perm(lo, 0, 0x1010);
+            f[r][1] = __byte_perm(lo, 0, 0x3232);
+            f[r][2] = __byte_perm(hi, 0, 0x1010);
+            f[r][3] = __byte_perm(hi, 0, 0x3232);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t a[2][4];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            spread(*reinterpret_cast<const uint32_t*>(at + (g + 8 * r) * kRowBytes + h * 64 + q * 16 + t * 4), a[r]);
+            if constexpr (!MX)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) a[r][j] = times(a[r][j], f[r][q]);
+          }
+          uint4 b = make_uint4(0, 0, 0, 0);
+          if (g < len) b = *reinterpret_cast<const uint4*>(xat + q * 64);
+          if constexpr (MX) {
+            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma(d, a[0], a[1], 0, b.x, b.y);
+            mma(d, a[0], a[1], 2, b.z, b.w);
+            const float* sx = xscale + ((piece * 2 + h) * 4 + q) * p.x_stride;
+            const float lo = mx_factor(codes[0], q), hi = mx_factor(codes[1], q), x0 = sx[0], x1 = sx[1];
+            acc[0] = fmaf(d[0] * lo, x0, acc[0]);
+            acc[1] = fmaf(d[1] * lo, x1, acc[1]);
+            acc[2] = fmaf(d[2] * hi, x0, acc[2]);
+            acc[3] = fmaf(d[3] * hi, x1, acc[3]);
+          } else {
+            mma(acc, a[0], a[1], 0, b.x, b.y);
+            mma(acc, a[0], a[1], 2, b.z, b.w);
+          }
+        }
+      }
+    }
+    float* mine = sums + (round & 1) * kSums;
+    {
+      float* to = mine + (warp * 8 + 2 * t) * kPad + g;
+      to[0] = acc[0];
+      to[kPad] = acc[1];
+      to[8] = acc[2];
+      to[kPad + 8] = acc[3];
+    }
+    __syncthreads();   // (the next round writes the other half of `sums`)
+    for (int i = tid; i < (kWarps >> split) * 128; i += kThreads) {
+      const int sl = i / 128, token = i / 16 % 8, lane_n = i & 15;
+      const int tl = (round * (int)gridDim.x + (int)blockIdx.x) * (kWarps >> split) + sl;
+      if (tl >= total) break;
+      const int gj = tl / p.tiles, n = (tl - gj * p.tiles) * 16 + lane_n;
+      const int3 grp = p.sizes ? list[gj] : make_int3(0, 0, p.T);
+      if (token >= grp.z || n >= p.N) continue;
+      float v = 0.0f;
+      for (int w = 0; w < stride; ++w) v += mine[(((sl << split) + w) * 8 + token) * kPad + lane_n];
+      if constexpr (!MX) v *= (p.gw ? __ldg(p.gw + (p.gw_each ? grp.x : 0)) : 1.0f) * gx;
+      static_cast<T*>(p.y)[(int64_t)(grp.y + token) * p.N + n] = Elem<T>::from_float(v);
+    }
+  }
+  copies_wait<0>();
+}
+
+int sm_count() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!cached[dev]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    cached[dev] = n;
+  }
+  return cached[dev];
+}
+int row_pitch(int64_t K) { return (int)((K + kPieceK - 1) / kPieceK * kPieceK * 2 + 64); }   // eight lanes of two rows on 32 banks
+// Floats from group to group of x's scales: all rows, and what the lanes of columns without one read.
+int scale_stride(int64_t T) { return (int)T + 8; }
+size_t smem_bytes(int64_t T, int64_t K, int mode) {
+  const size_t xscales = mode == B200Q_MXFP4 ? (size_t)(K + kPieceK - 1) / kPieceK * (kPieceK / 32) * scale_stride(T) * 4 : 0;
+  return (size_t)kWarps * kStages * kStageBytes + 2 * (size_t)kWarps * 8 * kPad * 4 + (size_t)T * row_pitch(K) + xscales;
+}
+
+}  // namespace
+
+bool fp4_rows_supported(const Fp4Rows& a) {
+  const bool mx = a.mode == B200Q_MXFP4;
+  return a.T <= kMostRows && a.K % 128 == 0 && (reinterpret_cast<uintptr_t>(a.scales) & (mx ? 3 : 7)) == 0 && a.K <= 1 << 20 &&
+         smem_bytes(a.T, a.K, a.mode) <= kSmemMax && (a.N + 15) / 16 * (a.E < a.T ? a.E : a.T) < 1 << 24;
+}
+
+int fp4_rows(const Fp4Rows& a, cudaStream_t st) {
+  RowsParams p{};
+  p.x = a.x; p.wq = reinterpret_cast<const uint8_t*>(a.wq); p.scales = a.scales; p.sizes = a.sizes; p.size_bytes = a.size_bytes;
+  p.y = a.y; p.gx = a.gx; p.gw = a.gw; p.gw_each = a.gw_each; p.status = a.status;
+  p.T = (int)a.T; p.E = (int)a.E; p.N = (int)a.N; p.K = (int)a.K;
+  p.tiles = (p.N + 15) / 16;
+  p.pieces = (p.K + kPieceK - 1) / kPieceK;
+  p.pitch = row_pitch(a.K);
+  p.x_stride = scale_stride(a.T);
+  const size_t smem = smem_bytes(a.T, a.K, a.mode);
+  const int64_t most = (int64_t)p.tiles * (a.sizes ? (a.E < a.T ? a.E : a.T) : 1);
+  const unsigned grid = (unsigned)(most < sm_count() ? most : sm_count());
+  auto go = [&](auto kernel) -> int {
+    B200Q_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax));
+    kernel<<<grid, kThreads, smem, st>>>(p);
+    B200Q_LAUNCH_OK("fp4_rows_kernel");
+    return B200Q_OK;
+  };
+  auto typed = [&](auto t) -> int {
+    using T = decltype(t);
+    return a.mode == B200Q_MXFP4 ? go(fp4_rows_kernel<T, true>) : go(fp4_rows_kernel<T, false>);
+  };
+  switch (a.dtype) {
+    case B200Q_F32: return typed(float{});
+    case B200Q_F16: return typed(__half{});
+    default: return typed(__nv_bfloat16{});
+  }
+}
+
+}  // namespace b200q

@@ -133,6 +133,8 @@ extern "C" int b200q_grouped_qqmm(const void* x, const uint32_t* wq, const uint8
   if (!aligned16(wq)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] packed weights must be 16-byte aligned", tag);
   const size_t need = qqmm_bytes(T, E, N, K, mode);
   if (int rc = check_ws(tag, ws, ws_bytes, need)) return rc;
+  const Fp4Rows few{x, wq, scales, sizes, size_bytes, y, dtype, mode, T, E, N, K, global_scale_x, global_scale_w, scale_per_group, status_word(ws, ws_bytes)};
+  if (fp4_rows_supported(few)) return fp4_rows(few, st);
   char* at = static_cast<char*>(ws) + up(grouped_tc_bytes(T, false));
   uint8_t* codes = reinterpret_cast<uint8_t*>(at);
   at += up((size_t)T * up16(K / 2));

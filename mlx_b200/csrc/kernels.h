@@ -214,6 +214,22 @@ struct Fp4Prepare {
   uint32_t *sfx, *sfw;
 };
 int fp4_prepare(const Fp4Prepare& a, cudaStream_t st);
+// fp4_rows.cu : 4-bit products of up to 16 rows in one launch; operands as b200q_grouped_qqmm has them
+struct Fp4Rows {
+  const void* x;
+  const uint32_t* wq;
+  const uint8_t* scales;
+  const void* sizes;        // null: one group
+  int size_bytes;
+  void* y;
+  int dtype, mode;
+  int64_t T, E, N, K;
+  const float *gx, *gw;
+  int gw_each;
+  uint32_t* status;
+};
+bool fp4_rows_supported(const Fp4Rows& a);
+int fp4_rows(const Fp4Rows& a, cudaStream_t st);
 // dst rows of dst_pitch bytes (a multiple of 16) from src rows of src_bytes, padded with zeros.
 int repack_rows(const void* src, int64_t src_bytes, void* dst, int64_t dst_pitch, int64_t rows, cudaStream_t st);
 
