@@ -1,16 +1,15 @@
-// 4-bit products of up to 16 rows, dense or grouped, in one launch: y[t] = Gx Gw[e] (quantized x[t]) (wq[e], scales[e])^T.
+// 4-bit products of up to 8 rows, dense or grouped, in one launch: y[t] = Gx Gw[e] (quantized x[t]) (wq[e], scales[e])^T.
 //
-// Every block quantizes all of x into shared memory, as 16-bit numbers times their group's scale, and goes through its share of
-// the weights once, which lie as the caller has them.  A warp has 16 rows of weights and every 2^split-th piece of 256 k
-// (128 bytes of codes per row, two pieces ahead in registers); codes become 16-bit numbers in place:
-//   sign and three bits, shifted to sign and the lowest exponent and highest mantissa bits, are the f16 number q 2^-14 (bf16: q
-//   2^-126), subnormal 0.5 included; one multiplication by the scale makes it exact
-//   nvfp4  f16, q s 2^-7: at most 21, a multiple of 2^-17, four and two significant bits
-//   mxfp4  bf16, q 2^e; a warp that meets scales above 2 multiplies by 2^126 first, since 2^(e + 126) has no bf16 number then
-// mma.sync (m16n8k16) takes them as A and x as B, sums in fp32; k is in the order in which the codes fall out, for both alike.  Partial
-// sums of the warps that share rows go through shared memory and are added in order.
+// Every block quantizes all of x into shared memory and goes through its share of the weights once, which lie as the caller has them.  A
+// warp has 16 rows of weights and every 2^split-th piece of 256 k, fetched by asynchronous copies while the piece before is multiplied.
+// Codes become f16 numbers (e2m1 to f16 is one conversion per pair) for mma.sync (m16n8k16), weights as A and x as B, sums in fp32:
+//   nvfp4  times their E4M3 scale before, in both operands: at most 2688, a multiple of 2^-10 of six significant bits, so exact
+//   mxfp4  codes alone (a power of two of E8M0's range has no f16 number): a group's 32 products are summed from zero, then times
+//          the product of both scales in fp32
+// Sums of the warps that share rows go through shared memory and are added in order.  Rows beyond the sum of the sizes are zeroed.
 //
-// Bound: latencies (launch, x, first weights, last sums) where the weights are few, then instructions and HBM alike.
+// Bound: latencies up to some 10 million weights (4096^2, one row: 6.8 us, of which the launch, x, the first weights and the last sums
+// are 5), then instructions: 400 per piece and warp, ALU 61 % and issue slots 64 % busy, 3.6 TB/s (28672 x 8192: 36 us).
 #include "fp4.cuh"
 
 namespace b200q {
@@ -22,7 +21,7 @@ constexpr int kWarps = 16, kThreads = 32 * kWarps;
 constexpr int kMostRows = 8;       // of x: columns of one product
 constexpr int kPieceK = 256;
 constexpr int kPad = 20;            // floats from token to token of a partial sum: eight lanes of four tokens on 32 banks
-constexpr int kStages = 3;
+constexpr int kStages = 2;          // (three: the same; four: 15 % slower where the weights are many)
 constexpr int kRowBytes = 144;      // of codes from row to row of a stage: eight rows' words on 32 banks
 constexpr int kStageBytes = 16 * kRowBytes + 16 * 16;
 constexpr size_t kSmemMax = 227 * 1024 - 1024;
@@ -38,12 +37,13 @@ struct RowsParams {
   int T, E, N, K, size_bytes, gw_each;
   int tiles;                // of 16 rows of weights, per group
   int pieces;               // of K
+  int half;                 // the last piece has 128 k only
   int pitch;                // bytes of a row of x in shared memory
   int x_stride;             // mxfp4: floats from group to group of x's scales there
 };
 
-__device__ __forceinline__ uint32_t times(uint32_t v, uint32_t m) {
-  const __half2 r = __hmul2(reinterpret_cast<const __half2&>(v), reinterpret_cast<const __half2&>(m));
+__device__ __forceinline__ uint32_t times(uint32_t v, __half2 m) {
+  const __half2 r = __hmul2(reinterpret_cast<const __half2&>(v), m);
   return reinterpret_cast<const uint32_t&>(r);
 }
 // The eight codes of a word as four pairs of f16 numbers.
@@ -54,10 +54,10 @@ __device__ __forceinline__ void spread(uint32_t w, uint32_t (&r)[4]) {
       : "r"(w));
 }
 // Two E4M3 scales as f16.
-__device__ __forceinline__ uint32_t nv_factors(uint32_t codes) {
+__device__ __forceinline__ __half2 nv_factors(uint32_t codes) {
   uint32_t h;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)codes));
-  return h;
+  return reinterpret_cast<const __half2&>(h);
 }
 // Byte q of four E8M0 scales: 2^(code - 127), 255 is NaN (infinity times zero).
 __device__ __forceinline__ float mx_factor(uint32_t codes, int q) {
@@ -70,11 +70,16 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a0)[4], cons
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0[j]), "r"(a8[j]), "r"(a0[j + 1]), "r"(a8[j + 1]), "r"(b0), "r"(b1));
 }
-// N bytes into shared memory, zeros where there are none to read.
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a0)[4], const uint32_t (&a8)[4], int j, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0[j]), "r"(a8[j]), "r"(a0[j + 1]), "r"(a8[j + 1]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// N bytes into shared memory.
 template <int N>
-__device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from, bool there) {
-  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(N), "r"(there ? N : 0) : "memory");
+__device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from) {
+  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(N) : "memory");
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -149,37 +154,41 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_rows_kernel(const __grid_cons
   }
   const int part = warp & ((1 << split) - 1), stride = 1 << split;
 
-  // ---- the way through the weights, two pieces ahead: a lane copies 16 bytes of rows lane / 8 + {0, 4, 8, 12}, and scales ----
+  // ---- the way through the weights, a piece ahead: a lane copies 16 bytes of rows lane / 8 + {0, 4, 8, 12}, and scales ----
   const int from_row = lane >> 3, from_byte = (lane & 7) * 16;
   constexpr int kScaleCopy = MX ? 4 : 8;      // bytes of 128 k
-  int ahead_round = 0, ahead = part, ahead_slot = 0, rows_left = 0;
+  int ahead_round = 0, ahead = part, ahead_slot = 0;
+  const int64_t four_rows = (int64_t)p.K * 2;
+  bool there = false;
   const uint8_t *w0 = nullptr, *s0 = nullptr;
   auto tile_of = [&](int round) { return (round * (int)gridDim.x + (int)blockIdx.x) * (kWarps >> split) + (warp >> split); };
+  // first row of a tile: the last one of a group begins earlier where 16 do not divide N (some rows are computed twice, alike)
+  auto row_of = [&](int tile_in_group) { return min(tile_in_group * 16, p.N - 16); };
   auto begin_tile = [&]() {
     const int tile = tile_of(ahead_round);
-    rows_left = 0;
-    w0 = p.wq;
-    s0 = p.scales;
-    if (ahead_round >= rounds || tile >= total) return;
-    const int gi = tile / p.tiles, n = (tile - gi * p.tiles) * 16;
-    const int64_t row = (int64_t)(p.sizes ? list[gi].x : 0) * p.N + n;
-    rows_left = p.N - n;
-    w0 += (row + from_row) * (p.K / 2) + from_byte;
-    s0 += (row + (lane >> 1)) * (p.K / (MX ? 32 : 16)) + (lane & 1) * kScaleCopy;
+    there = ahead_round < rounds && tile < total;
+    if (!there) return;
+    const int gi = tile / p.tiles;
+    const int64_t row = (int64_t)(p.sizes ? list[gi].x : 0) * p.N + row_of(tile - gi * p.tiles);
+    w0 = p.wq + (row + from_row) * (p.K / 2) + from_byte + part * (kPieceK / 2);
+    s0 = p.scales + (row + (lane >> 1)) * (p.K / (MX ? 32 : 16)) + (lane & 1) * kScaleCopy + part * (kPieceK / (MX ? 32 : 16));
   };
   auto load = [&]() {
-    const uint32_t to = (uint32_t)__cvta_generic_to_shared(stages + ahead_slot * kStageBytes);
-    const int k = ahead * kPieceK, left = p.K - k;
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(stages + ahead_slot * kStageBytes) + from_row * kRowBytes + from_byte;
+    const uint32_t sto = (uint32_t)__cvta_generic_to_shared(stages + ahead_slot * kStageBytes) + 16 * kRowBytes + lane * kScaleCopy;
+    if (there) {
+      // the last piece may have one half: the other gets the same codes and scales, which meet zeros of x
+      const int half = ahead == p.pieces - 1 ? p.half : 0;
+      const uint8_t* at = w0 - ((lane & 4) ? half * 64 : 0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool there = from_row + 4 * i < rows_left && from_byte * 2 < left;
-      copy_async<16>(to + (from_row + 4 * i) * kRowBytes + from_byte, there ? w0 + k / 2 + (int64_t)i * 4 * (p.K / 2) : p.wq, there);
+      for (int i = 0; i < 4; ++i, at += four_rows) copy_async<16>(to + 4 * i * kRowBytes, at);
+      copy_async<kScaleCopy>(sto, s0 - ((lane & 1) ? half * kScaleCopy : 0));
     }
-    const bool there = (lane >> 1) < rows_left && (lane & 1) * 128 < left;
-    copy_async<kScaleCopy>(to + 16 * kRowBytes + lane * kScaleCopy, there ? s0 + k / (MX ? 32 : 16) : p.scales, there);
     copies_done();
     ahead_slot = ahead_slot == kStages - 1 ? 0 : ahead_slot + 1;
     ahead += stride;
+    w0 += stride * (kPieceK / 2);
+    s0 += stride * (kPieceK / (MX ? 32 : 16));
     if (ahead >= p.pieces) {
       ahead = part;
       ++ahead_round;
@@ -207,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_rows_kernel(const __grid_cons
       const uint32_t s = quantize_unit<MX>(v, top, G, codes);
       if (u >= units) break;
       uint4* to = reinterpret_cast<uint4*>(xs + (size_t)row * p.pitch + k * 2);
-      const uint32_t f = MX ? 0u : nv_factors(s * 0x0101u);
+      const __half2 f = nv_factors(s * 0x0101u);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t r[4];
@@ -233,6 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_rows_kernel(const __grid_cons
     const int len = tile < total ? (p.sizes ? list[gi].z : p.T) : 0;
     const uint8_t* xrow = xs + (size_t)(row0 + g) * p.pitch + t * 16;
     const float* xscale = xscales + row0 + 2 * t;
+    uint4 bs[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};   // columns without a row stay zero
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int piece = part; piece < p.pieces; piece += stride) {
       copies_wait<kStages - 2>();
@@ -244,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_rows_kernel(const __grid_cons
       for (int h = 0; h < 2; ++h) {
         const uint8_t* xat = xrow + (piece * 2 + h) * 256;
         uint32_t codes[2];      // mxfp4: four scales per row
-        uint32_t f[2][4];       // nvfp4: the factor of each word
+        __half2 f[2][4];        // nvfp4: the factor of each word
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const uint8_t* sat = at + 16 * kRowBytes + (g + 8 * r) * (2 * kScaleCopy) + h * kScaleCopy;
@@ -252,11 +262,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_rows_kernel(const __grid_cons
             codes[r] = *reinterpret_cast<const uint32_t*>(sat);
           } else {
             const uint2 c = *reinterpret_cast<const uint2*>(sat);
-            const uint32_t lo = nv_factors(__byte_perm(c.x, 0, t >> 1 ? 0x31 : 0x20)), hi = nv_factors(__byte_perm(c.y, 0, t >> 1 ? 0x31 : 0x20));
-            f[r][0] = __byte_perm(lo, 0, 0x1010);
-            f[r][1] = __byte_perm(lo, 0, 0x3232);
-            f[r][2] = __byte_perm(hi, 0, 0x1010);
-            f[r][3] = __byte_perm(hi, 0, 0x3232);
+            const __half2 lo = nv_factors(__byte_perm(c.x, 0, t >> 1 ? 0x31 : 0x20)), hi = nv_factors(__byte_perm(c.y, 0, t >> 1 ? 0x31 : 0x20));
+            f[r][0] = __low2half2(lo);
+            f[r][1] = __high2half2(lo);
+            f[r][2] = __low2half2(hi);
+            f[r][3] = __high2half2(hi);
           }
         }
 #pragma unroll
@@ -269,18 +279,18 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_rows_kernel(const __grid_cons
 #pragma unroll
               for (int j = 0; j < 4; ++j) a[r][j] = times(a[r][j], f[r][q]);
           }
-          uint4 b = make_uint4(0, 0, 0, 0);
+          uint4& b = bs[q & 1];
           if (g < len) b = *reinterpret_cast<const uint4*>(xat + q * 64);
           if constexpr (MX) {
-            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma(d, a[0], a[1], 0, b.x, b.y);
+            float d[4];
+            mma_first(d, a[0], a[1], 0, b.x, b.y);
             mma(d, a[0], a[1], 2, b.z, b.w);
             const float* sx = xscale + ((piece * 2 + h) * 4 + q) * p.x_stride;
             const float lo = mx_factor(codes[0], q), hi = mx_factor(codes[1], q), x0 = sx[0], x1 = sx[1];
-            acc[0] = fmaf(d[0] * lo, x0, acc[0]);
-            acc[1] = fmaf(d[1] * lo, x1, acc[1]);
-            acc[2] = fmaf(d[2] * hi, x0, acc[2]);
-            acc[3] = fmaf(d[3] * hi, x1, acc[3]);
+            acc[0] = fmaf(d[0], lo * x0, acc[0]);
+            acc[1] = fmaf(d[1], lo * x1, acc[1]);
+            acc[2] = fmaf(d[2], hi * x0, acc[2]);
+            acc[3] = fmaf(d[3], hi * x1, acc[3]);
           } else {
             mma(acc, a[0], a[1], 0, b.x, b.y);
             mma(acc, a[0], a[1], 2, b.z, b.w);
@@ -301,9 +311,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_rows_kernel(const __grid_cons
       const int sl = i / 128, token = i / 16 % 8, lane_n = i & 15;
       const int tl = (round * (int)gridDim.x + (int)blockIdx.x) * (kWarps >> split) + sl;
       if (tl >= total) break;
-      const int gj = tl / p.tiles, n = (tl - gj * p.tiles) * 16 + lane_n;
+      const int gj = tl / p.tiles, n = row_of(tl - gj * p.tiles) + lane_n;
       const int3 grp = p.sizes ? list[gj] : make_int3(0, 0, p.T);
-      if (token >= grp.z || n >= p.N) continue;
+      if (token >= grp.z) continue;
       float v = 0.0f;
       for (int w = 0; w < stride; ++w) v += mine[(((sl << split) + w) * 8 + token) * kPad + lane_n];
       if constexpr (!MX) v *= (p.gw ? __ldg(p.gw + (p.gw_each ? grp.x : 0)) : 1.0f) * gx;
@@ -334,10 +344,18 @@ size_t smem_bytes(int64_t T, int64_t K, int mode) {
 
 }  // namespace
 
+// Where this kernel is the faster one.  In us it takes about 5 + 0.15 per million weights that have rows + 0.1 per thousand values of x
+// (which every block quantizes); the tensor-core kernel behind the one that prepares its operands takes 11 at least and rises more
+// slowly, by 0.11 per million, but reorders every group's scales first.  nvfp4, here and there:
+//   dense, 1 and 8 rows   [4096, 4096] 6.8, 9.2 and 11.8, 12.1; [14336, 4096] 13.7, 16.7 and 15.7, 14.4; [28672, 8192] 36 and 37
+//   (mxfp4, 1 and 4 rows  [14336, 4096] 14.2, 14.9 and 14.3, 13.5; [4096, 14336] 13.7, 15.2 and 15.1, 15.4)
+//   grouped, 2 and 8 rows of 8 [14336, 4096] 22, 50 and 22.5, 44.5; of 256 [2048, 4096] 7.8, 18 and 24.5, 27
 bool fp4_rows_supported(const Fp4Rows& a) {
   const bool mx = a.mode == B200Q_MXFP4;
-  return a.T <= kMostRows && a.K % 128 == 0 && (reinterpret_cast<uintptr_t>(a.scales) & (mx ? 3 : 7)) == 0 && a.K <= 1 << 20 &&
-         smem_bytes(a.T, a.K, a.mode) <= kSmemMax && (a.N + 15) / 16 * (a.E < a.T ? a.E : a.T) < 1 << 24;
+  if (a.T > kMostRows || a.N < 16 || a.K % 128 != 0 || (reinterpret_cast<uintptr_t>(a.scales) & (mx ? 3 : 7)) != 0 || a.K > 1 << 20) return false;
+  const int64_t groups = a.sizes && a.E < a.T ? a.E : (a.sizes ? a.T : 1);
+  if (0.15e-6 * (double)groups * (double)a.N * (double)a.K + 0.1e-3 * (double)a.T * (double)a.K > (a.sizes ? 14.0 : 10.3)) return false;
+  return smem_bytes(a.T, a.K, a.mode) <= kSmemMax;
 }
 
 int fp4_rows(const Fp4Rows& a, cudaStream_t st) {
@@ -347,6 +365,7 @@ int fp4_rows(const Fp4Rows& a, cudaStream_t st) {
   p.T = (int)a.T; p.E = (int)a.E; p.N = (int)a.N; p.K = (int)a.K;
   p.tiles = (p.N + 15) / 16;
   p.pieces = (p.K + kPieceK - 1) / kPieceK;
+  p.half = p.K % kPieceK != 0;
   p.pitch = row_pitch(a.K);
   p.x_stride = scale_stride(a.T);
   const size_t smem = smem_bytes(a.T, a.K, a.mode);
