@@ -569,17 +569,24 @@ struct GroupedFn : public torch::autograd::Function<GroupedFn> {
     const bool transpose = ctx->saved_data["transpose"].toBool();
     Tensor dx, dw;
     if (!grads[0].defined()) return {dx, dw, Tensor(), Tensor(), Tensor()};
-    const Tensor dy = grads[0].contiguous();
+    const bool for_x = ctx->saved_data["dx"].toBool(), for_w = ctx->saved_data["dw"].toBool();
     pybind11::gil_scoped_acquire gil;   // the scratch table, and the Python forms
+    auto wrap = [](const Tensor& v) { return pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(v)); };
+    if (at::GradMode::is_enabled()) {   // a graph of the gradients is asked for: the Python form makes one
+      const pybind11::tuple r = pybind11::module_::import("mlx_b200.grad").attr("_grouped_mm_vjp")(
+          wrap(grads[0]), wrap(x), wrap(w), wrap(sizes), transpose, for_x, for_w);
+      if (for_x) dx = THPVariable_Unpack(r[0].ptr());
+      if (for_w) dw = THPVariable_Unpack(r[1].ptr());
+      return {dx, dw, Tensor(), Tensor(), Tensor()};
+    }
+    const Tensor dy = grads[0].contiguous();
     at::AutoDispatchBelowAutograd below;
     auto python = [&](const char* name, const Tensor& p, const Tensor& q, bool t) {
-      const auto ops = pybind11::module_::import("mlx_b200.ops");
-      auto wrap = [](const Tensor& v) { return pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(v)); };
-      pybind11::object r = ops.attr(name)(wrap(p), wrap(q), wrap(sizes), t);
+      pybind11::object r = pybind11::module_::import("mlx_b200.ops").attr(name)(wrap(p), wrap(q), wrap(sizes), t);
       return Tensor(THPVariable_Unpack(r.ptr()));
     };
-    if (ctx->saved_data["dx"].toBool() && !grouped_run(dy, w, sizes, !transpose, &dx)) dx = python("grouped_mm", dy, w, !transpose);
-    if (ctx->saved_data["dw"].toBool() && !grouped_dw_run(dy, x, sizes, transpose, &dw)) dw = python("grouped_mm_dw", dy, x, transpose);
+    if (for_x && !grouped_run(dy, w, sizes, !transpose, &dx)) dx = python("grouped_mm", dy, w, !transpose);
+    if (for_w && !grouped_dw_run(dy, x, sizes, transpose, &dw)) dw = python("grouped_mm_dw", dy, x, transpose);
     return {dx, dw, Tensor(), Tensor(), Tensor()};
   }
 };

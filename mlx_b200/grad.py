@@ -137,17 +137,39 @@ class _GroupedMmFn(torch.autograd.Function):
         return ops.grouped_mm(x, w, sizes, transpose)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w, sizes = ctx.saved_tensors
-        dy = dy.to(x.dtype)
-        dx = ops.grouped_mm(dy, w, sizes, not ctx.transpose) if ctx.needs_input_grad[0] else None
-        dw = ops.grouped_mm_dw(dy, x, sizes, ctx.transpose) if ctx.needs_input_grad[1] else None
-        return dx, dw, None, None
+        return (*_grouped_mm_vjp(dy, *ctx.saved_tensors, ctx.transpose, *ctx.needs_input_grad[:2]), None, None)
+
+
+class _GroupedMmDwFn(torch.autograd.Function):
+    """ops.grouped_mm_dw as a function of dy and x: both gradients are products with the cotangent as the experts' matrices."""
+
+    @staticmethod
+    def forward(ctx, dy, x, sizes, transpose):
+        ctx.save_for_backward(dy, x, sizes)
+        ctx.transpose = transpose
+        return ops.grouped_mm_dw(dy, x, sizes, transpose)
+
+    @staticmethod
+    def backward(ctx, g):
+        dy, x, sizes = ctx.saved_tensors
+        d_dy = grouped_mm(x, g, sizes, ctx.transpose) if ctx.needs_input_grad[0] else None
+        dx = grouped_mm(dy, g, sizes, not ctx.transpose) if ctx.needs_input_grad[1] else None
+        return d_dy, dx, None, None
+
+
+def _grouped_mm_vjp(dy, x, w, sizes, transpose, for_x, for_w):
+    """Gradients of grouped_mm with respect to x and w (None where not asked for), differentiable where a graph of them is asked for.
+    The native form, too, comes here for such a graph."""
+    graph = torch.is_grad_enabled()
+    dy = dy.to(x.dtype)
+    dx = (grouped_mm if graph else ops.grouped_mm)(dy, w, sizes, not transpose) if for_x else None
+    dw = (_GroupedMmDwFn.apply if graph else ops.grouped_mm_dw)(dy, x, sizes, transpose) if for_w else None
+    return dx, dw
 
 
 def grouped_mm(x: torch.Tensor, w: torch.Tensor, sizes: torch.Tensor, transpose: bool = True) -> torch.Tensor:
-    """ops.grouped_mm with autograd support for x and w."""
+    """ops.grouped_mm with autograd support for x and w, of any order."""
     y = ops._front.grouped_mm_grad(x, w, sizes, transpose)
     if y is not None:
         return y
