@@ -559,8 +559,6 @@ struct GroupedFn : public torch::autograd::Function<GroupedFn> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& sizes, bool transpose, Tensor* y) {
     ctx->save_for_backward({x, w, sizes});
     ctx->saved_data["transpose"] = transpose;
-    ctx->saved_data["dx"] = x.requires_grad();
-    ctx->saved_data["dw"] = w.requires_grad();
     return *y;   // by address: a result passed as a tensor would come back as a view of itself
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
@@ -569,7 +567,7 @@ struct GroupedFn : public torch::autograd::Function<GroupedFn> {
     const bool transpose = ctx->saved_data["transpose"].toBool();
     Tensor dx, dw;
     if (!grads[0].defined()) return {dx, dw, Tensor(), Tensor(), Tensor()};
-    const bool for_x = ctx->saved_data["dx"].toBool(), for_w = ctx->saved_data["dw"].toBool();
+    const bool for_x = ctx->needs_input_grad(0), for_w = ctx->needs_input_grad(1);   // of this pass, which may want one of the two only
     pybind11::gil_scoped_acquire gil;   // the scratch table, and the Python forms
     auto wrap = [](const Tensor& v) { return pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(v)); };
     if (at::GradMode::is_enabled()) {   // a graph of the gradients is asked for: the Python form makes one
