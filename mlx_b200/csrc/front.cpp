@@ -197,14 +197,19 @@ struct QmmFn : public torch::autograd::Function<QmmFn> {
     const auto saved = ctx->get_saved_variables();
     const bool transpose = ctx->saved_data["transpose"].toBool();
     const int64_t group = ctx->saved_data["group"].toInt(), bits = ctx->saved_data["bits"].toInt();
-    const Tensor dy = grads[0].contiguous();
     Tensor dx;
-    pybind11::gil_scoped_acquire gil;   // the scratch table, and the Python form
-    if (!qmm_run(dy, saved[0], saved[1], saved[2], !transpose, (int)group, (int)bits, &dx)) {
-      const auto ops = pybind11::module_::import("mlx_b200.ops");
+    pybind11::gil_scoped_acquire gil;   // the scratch table, and the Python forms
+    auto python = [&](const char* module, const Tensor& dy) {
       auto wrap = [](const Tensor& t) { return pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(t)); };
-      pybind11::object r = ops.attr("quantized_matmul")(wrap(dy), wrap(saved[0]), wrap(saved[1]), wrap(saved[2]), !transpose, group, bits);
-      dx = THPVariable_Unpack(r.ptr());
+      pybind11::object r = pybind11::module_::import(module).attr("quantized_matmul")(wrap(dy), wrap(saved[0]), wrap(saved[1]), wrap(saved[2]),
+                                                                                      !transpose, group, bits);
+      return Tensor(THPVariable_Unpack(r.ptr()));
+    };
+    if (at::GradMode::is_enabled()) {   // a graph of the gradient is asked for
+      dx = python("mlx_b200.grad", grads[0].contiguous());
+    } else {
+      const Tensor dy = grads[0].contiguous();
+      if (!qmm_run(dy, saved[0], saved[1], saved[2], !transpose, (int)group, (int)bits, &dx)) dx = python("mlx_b200.ops", dy);
     }
     return {dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }

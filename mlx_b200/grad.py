@@ -29,7 +29,8 @@ class _QuantizedMatmulFn(torch.autograd.Function):
         transpose, group_size, bits = ctx.cfg
         dx = ds = db = None
         if ctx.needs_input_grad[0]:
-            dx = ops.quantized_matmul(cotangent.contiguous(), w, scales, biases, not transpose, group_size, bits)
+            product = quantized_matmul if torch.is_grad_enabled() else ops.quantized_matmul   # (a graph of the gradient, or none)
+            dx = product(cotangent.contiguous(), w, scales, biases, not transpose, group_size, bits)
             dx = dx.to(x.dtype)
         if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
             if w.ndim != 2:
