@@ -88,7 +88,8 @@ class _GatherQmmFn(torch.autograd.Function):
         fc = cotangent.reshape((-1, M, cotangent.shape[-1])).contiguous()
         dx = ds = db = None
         if ctx.needs_input_grad[0]:
-            g = ops.gather_qmm(fc, w, scales, biases, None, rhs, not transpose, group_size, bits)   # [n_idx, M, K]
+            product = gather_qmm if torch.is_grad_enabled() else ops.gather_qmm   # (a graph of the gradient, or none)
+            g = product(fc, w, scales, biases, None, rhs, not transpose, group_size, bits)   # [n_idx, M, K]
             dx = torch.zeros((max(1, torch.Size(x_shape[:-2]).numel()),) + tuple(x_shape[-2:]), dtype=torch.float32,
                              device=g.device)
             dx.index_add_(0, lhs, g.float())
