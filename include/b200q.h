@@ -24,7 +24,9 @@
  *     with the matching *_workspace_bytes() query.  The first bytes of a workspace
  *     hold self-cleaning counters: zero the workspace once after allocating it
  *     (b200q_workspace_init) and never share one workspace between two calls that
- *     may overlap on the GPU.  b200q_qmm leaves its workspace zeroed again;
+ *     may overlap on the GPU.  Host threads may share a stream and its workspace: a call
+ *     whose kernels pass something on through the workspace holds a lock while it launches
+ *     them, so that no other call with that workspace comes between.  b200q_qmm leaves its workspace zeroed again;
  *     b200q_gather_qmm uses everything but the last 16 bytes as plain scratch and
  *     leaves arbitrary data there (it needs only those last 16 bytes to be zero), so
  *     keep a separate workspace for it or re-initialise before reusing the memory

@@ -50,6 +50,11 @@ int bind_context() {
 }
 
 namespace {
+std::mutex g_scratch[64];
+}  // namespace
+ScratchLock::ScratchLock(const void* ws) : held_(g_scratch[reinterpret_cast<uintptr_t>(ws) / 256 % 64]) {}
+
+namespace {
 
 enum class Path { QmvRows, Qmv, Tc, Qvm, Generic };
 

@@ -237,6 +237,7 @@ void set_matrix(RowsGroup& r, int i, const uint32_t* wq, const void* scales, con
 int run_grouped(const void* x, const uint32_t* wq, const void* scales, const void* biases, const Pairs& pairs, int64_t n_idx, void* y, const PeerOut* peers, int64_t x_batch, int64_t E_total,
                 int64_t e_lo, int64_t E_local, int64_t M, int64_t N, int64_t K, int group_size, int bits, void* ws,
                 size_t ws_bytes, cudaStream_t st) {
+  const ScratchLock lock(ws);
   uint32_t* status = reinterpret_cast<uint32_t*>(static_cast<char*>(ws) + ws_bytes - kStatusBytes);
   const FastLayout L = fast_layout(n_idx, E_total, M, K);
   char* base = static_cast<char*>(ws);
@@ -434,6 +435,7 @@ extern "C" int b200q_gather_qmm_chain(const void* x, const uint32_t* wq1, const 
   const size_t need = b200q_gather_qmm_chain_workspace_bytes(n_idx, E, M, N1, K1);
   if (!ws || ws_bytes < need)
     return fail(B200Q_ERR_WORKSPACE, "[gather_qmm_chain] workspace of %zu bytes required, %zu given", need, ws_bytes);
+  const ScratchLock lock(ws);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint32_t* status = reinterpret_cast<uint32_t*>(static_cast<char*>(ws) + ws_bytes - kStatusBytes);
   const FastLayout L = fast_layout(n_idx, E, M, K1);
@@ -532,6 +534,7 @@ int swiglu_impl(const void* x, const uint32_t* wq_gate, const void* scales_gate,
   const size_t need = b200q_gather_qmm_swiglu_workspace_bytes(n_idx, E, M, H, K1);
   if (!ws || ws_bytes < need)
     return fail(B200Q_ERR_WORKSPACE, "[gather_qmm_swiglu] workspace of %zu bytes required, %zu given", need, ws_bytes);
+  const ScratchLock lock(ws);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint32_t* status = reinterpret_cast<uint32_t*>(static_cast<char*>(ws) + ws_bytes - kStatusBytes);
   const FastLayout L = fast_layout(n_idx, E, M, K1);

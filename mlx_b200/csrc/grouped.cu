@@ -135,6 +135,7 @@ extern "C" int b200q_grouped_qqmm(const void* x, const uint32_t* wq, const uint8
   if (int rc = check_ws(tag, ws, ws_bytes, need)) return rc;
   const Fp4Rows few{x, wq, scales, sizes, size_bytes, y, dtype, mode, T, E, N, K, global_scale_x, global_scale_w, scale_per_group, status_word(ws, ws_bytes)};
   if (fp4_rows_supported(few)) return fp4_rows(few, st);
+  const ScratchLock lock(ws);
   char* at = static_cast<char*>(ws) + up(grouped_tc_bytes(T, false));
   uint8_t* codes = reinterpret_cast<uint8_t*>(at);
   at += up((size_t)T * up16(K / 2));
@@ -181,6 +182,7 @@ extern "C" int b200q_grouped_mm(const void* x, const void* w, const void* sizes,
   if (!aligned16(x) || !aligned16(w)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] x and w must be 16-byte aligned", tag);
   const size_t need = grouped_bytes(T, E, N, K, transpose != 0);
   if (int rc = check_ws(tag, ws, ws_bytes, need)) return rc;
+  const ScratchLock lock(ws);
   char* at = static_cast<char*>(ws) + up(grouped_tc_bytes(T, false));
   Operand xo, wo;
   if (int rc = pack(x, T, 2 * K, at, &xo, st)) return rc;
@@ -218,6 +220,7 @@ extern "C" int b200q_grouped_mm_dw(const void* dy, const void* x, const void* si
   if (!aligned16(dy) || !aligned16(x)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] dy and x must be 16-byte aligned", tag);
   const size_t need = dw_bytes(T, N, K);
   if (int rc = check_ws(tag, ws, ws_bytes, need)) return rc;
+  const ScratchLock lock(ws);
   char* at = static_cast<char*>(ws) + up(grouped_tc_bytes(T, true));
   Operand yo, xo;
   if (int rc = pack(dy, T, 2 * N, at, &yo, st)) return rc;

@@ -5,10 +5,21 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <mutex>
 
 #include "../../include/b200q.h"
 
 namespace b200q {
+
+// Held while a call launches kernels that pass something on through its workspace.  Stream order keeps one thread's calls apart;
+// another thread's launches on the same stream could come between this call's.  (Locks of a small set, by address: 20 ns.)
+class ScratchLock {
+ public:
+  explicit ScratchLock(const void* ws);
+
+ private:
+  std::lock_guard<std::mutex> held_;
+};
 
 // Output replicated into the buffers of several GPUs (N-sharded linear with the all_gather
 // fused into the epilogue): element (m, n) of the local [M, N] result goes to
