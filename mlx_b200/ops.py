@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 from typing import Optional, Tuple
 
 import torch
@@ -65,20 +66,25 @@ class _Workspaces:
     def __init__(self):
         self._bufs = {}
         self._outgrown = []   # (key, buffer)
+        self._making = threading.RLock()   # one buffer at a time: of two made at once the native form could keep the one that is dropped
 
     def get(self, dev: torch.device, nbytes: int, op: str) -> torch.Tensor:
         key = (dev.index, torch.cuda.current_stream(dev).cuda_stream, op)
         buf = self._bufs.get(key)
-        if buf is None or buf.numel() < nbytes:
-            nbytes = max(nbytes, 256)
-            if buf is not None:
-                self._outgrown.append((key, buf))
-                nbytes = max(nbytes, 2 * buf.numel())
-            with torch.cuda.device(dev):
-                buf = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
-            self._bufs[key] = buf
-            _front.scratch(dev.index, key[1], _SCRATCH_OPS[op], buf.data_ptr(), buf.numel())
-        return buf
+        if buf is not None and buf.numel() >= nbytes:
+            return buf
+        with self._making:
+            buf = self._bufs.get(key)
+            if buf is None or buf.numel() < nbytes:
+                nbytes = max(nbytes, 256)
+                if buf is not None:
+                    self._outgrown.append((key, buf))
+                    nbytes = max(nbytes, 2 * buf.numel())
+                with torch.cuda.device(dev):
+                    buf = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+                self._bufs[key] = buf
+                _front.scratch(dev.index, key[1], _SCRATCH_OPS[op], buf.data_ptr(), buf.numel())
+            return buf
 
     def all(self):
         """Every (key, buffer) that a kernel may still be using."""
