@@ -5,7 +5,7 @@
 // Codes become f16 numbers (e2m1 to f16 is one conversion per pair) for mma.sync (m16n8k16), weights as A and x as B, sums in fp32:
 //   nvfp4  times their E4M3 scale before, in both operands: at most 2688, a multiple of 2^-10 of six significant bits, so exact
 //   mxfp4  codes alone (a power of two of E8M0's range has no f16 number): a group's 32 products are summed from zero, then times
-//          the product of both scales in fp32
+//          both scales in fp32 (one product where fp32 holds it whatever the weights' scale is, else two factors: kXScale)
 // Sums of the warps that share rows go through shared memory and are added in order.  Rows beyond the sum of the sizes are zeroed.
 //
 // Bound: latencies up to some 10 million weights (4096^2, one row: 6.8 us, of which the launch, x, the first weights and the last sums
@@ -21,6 +21,12 @@ constexpr int kWarps = 16, kThreads = 32 * kWarps;
 constexpr int kMostRows = 8;       // of x: columns of one product
 constexpr int kPieceK = 256;
 constexpr int kPad = 20;            // floats from token to token of a partial sum: eight lanes of four tokens on 32 banks
+// mxfp4: x's scales are kept times 2^-6.  Times a scale of the weights (2^-127 to 2^127) that is a fp32 number without loss as long as x's
+// own lies between 2^-14 and 2^6 (groups whose largest magnitude is 2^-12 to 512), and all products of a group's sum with it are multiples
+// of 2^-149.  Where one of x's scales lies outside, both factors are applied one after the other, the smaller one of x's and 1 first, so
+// that nothing passes fp32's range but a result that does (one row: [14336, 4096] 16.0 for 14.0 us).
+constexpr float kXScale = 0x1p-6f;
+constexpr uint32_t kLeastX = 127 - 14, kMostX = 127 + 6;
 constexpr int kStages = 2;          // (three: the same; four: 15 % slower where the weights are many)
 constexpr int kRowBytes = 144;      // of codes from row to row of a stage: eight rows' words on 32 banks
 constexpr int kStageBytes = 16 * kRowBytes + 16 * 16;
@@ -200,6 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_rows_kernel(const __grid_cons
     for (int i = 0; i < kStages - 1; ++i) load();
 
   // ---- x ----
+  int far = 0;   // mxfp4: a group of x that is not zero (or NaN) has a scale outside the range above
   {
     const int units = p.T * (p.pieces * (kPieceK / kUnit));
     const float G = !MX && p.gx ? __ldg(p.gx) : 1.0f;
@@ -226,13 +233,14 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_rows_kernel(const __grid_cons
           for (int j = 0; j < 4; ++j) r[j] = times(r[j], f);
         to[i] = in ? make_uint4(r[0], r[1], r[2], r[3]) : make_uint4(0, 0, 0, 0);
       }
-      if (MX && (k & 16) == 0) xscales[(k >> 5) * p.x_stride + row] = in ? e8m0_value(s) : 0.0f;
+      if (MX && (k & 16) == 0) xscales[(k >> 5) * p.x_stride + row] = in ? e8m0_value(s) * kXScale : 0.0f;
+      if (MX) far |= in && (codes[0] | codes[1]) != 0 && (s > kMostX || s < kLeastX);
     }
   }
   // rows of no group
   for (int64_t i = (int64_t)rows_end * p.N + (int64_t)blockIdx.x * kThreads + tid; i < (int64_t)p.T * p.N; i += (int64_t)gridDim.x * kThreads)
     static_cast<T*>(p.y)[i] = Elem<T>::from_float(0.0f);
-  __syncthreads();
+  const bool wide = __syncthreads_or(far) != 0;
 
   // ---- products ----
   const float gx = !MX && p.gx ? __ldg(p.gx) : 1.0f;
@@ -244,60 +252,74 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_rows_kernel(const __grid_cons
     const float* xscale = xscales + row0 + 2 * t;
     uint4 bs[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};   // columns without a row stay zero
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int piece = part; piece < p.pieces; piece += stride) {
-      copies_wait<kStages - 2>();
-      __syncwarp();   // everybody's copies are there, and nobody reads the stage before any more
-      load();
-      const uint8_t* at = stages + slot * kStageBytes;
-      slot = slot == kStages - 1 ? 0 : slot + 1;
+    auto pieces = [&](auto form) {
+      constexpr bool WIDE = decltype(form)::value;
+      for (int piece = part; piece < p.pieces; piece += stride) {
+        copies_wait<kStages - 2>();
+        __syncwarp();   // everybody's copies are there, and nobody reads the stage before any more
+        load();
+        const uint8_t* at = stages + slot * kStageBytes;
+        slot = slot == kStages - 1 ? 0 : slot + 1;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint8_t* xat = xrow + (piece * 2 + h) * 256;
-        uint32_t codes[2];      // mxfp4: four scales per row
-        __half2 f[2][4];        // nvfp4: the factor of each word
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint8_t* sat = at + 16 * kRowBytes + (g + 8 * r) * (2 * kScaleCopy) + h * kScaleCopy;
-          if constexpr (MX) {
-            codes[r] = *reinterpret_cast<const uint32_t*>(sat);
-          } else {
-            const uint2 c = *reinterpret_cast<const uint2*>(sat);
-            const __half2 lo = nv_factors(__byte_perm(c.x, 0, t >> 1 ? 0x31 : 0x20)), hi = nv_factors(__byte_perm(c.y, 0, t >> 1 ? 0x31 : 0x20));
-            f[r][0] = __low2half2(lo);
-            f[r][1] = __high2half2(lo);
-            f[r][2] = __low2half2(hi);
-            f[r][3] = __high2half2(hi);
-          }
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t a[2][4];
+        for (int h = 0; h < 2; ++h) {
+          const uint8_t* xat = xrow + (piece * 2 + h) * 256;
+          uint32_t codes[2];      // mxfp4: four scales per row
+          __half2 f[2][4];        // nvfp4: the factor of each word
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            spread(*reinterpret_cast<const uint32_t*>(at + (g + 8 * r) * kRowBytes + h * 64 + q * 16 + t * 4), a[r]);
-            if constexpr (!MX)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) a[r][j] = times(a[r][j], f[r][q]);
+            const uint8_t* sat = at + 16 * kRowBytes + (g + 8 * r) * (2 * kScaleCopy) + h * kScaleCopy;
+            if constexpr (MX) {
+              codes[r] = *reinterpret_cast<const uint32_t*>(sat);
+            } else {
+              const uint2 c = *reinterpret_cast<const uint2*>(sat);
+              const __half2 lo = nv_factors(__byte_perm(c.x, 0, t >> 1 ? 0x31 : 0x20)), hi = nv_factors(__byte_perm(c.y, 0, t >> 1 ? 0x31 : 0x20));
+              f[r][0] = __low2half2(lo);
+              f[r][1] = __high2half2(lo);
+              f[r][2] = __low2half2(hi);
+              f[r][3] = __high2half2(hi);
+            }
           }
-          uint4& b = bs[q & 1];
-          if (g < len) b = *reinterpret_cast<const uint4*>(xat + q * 64);
-          if constexpr (MX) {
-            float d[4];
-            mma_first(d, a[0], a[1], 0, b.x, b.y);
-            mma(d, a[0], a[1], 2, b.z, b.w);
-            const float* sx = xscale + ((piece * 2 + h) * 4 + q) * p.x_stride;
-            const float lo = mx_factor(codes[0], q), hi = mx_factor(codes[1], q), x0 = sx[0], x1 = sx[1];
-            acc[0] = fmaf(d[0], lo * x0, acc[0]);
-            acc[1] = fmaf(d[1], lo * x1, acc[1]);
-            acc[2] = fmaf(d[2], hi * x0, acc[2]);
-            acc[3] = fmaf(d[3], hi * x1, acc[3]);
-          } else {
-            mma(acc, a[0], a[1], 0, b.x, b.y);
-            mma(acc, a[0], a[1], 2, b.z, b.w);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t a[2][4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              spread(*reinterpret_cast<const uint32_t*>(at + (g + 8 * r) * kRowBytes + h * 64 + q * 16 + t * 4), a[r]);
+              if constexpr (!MX)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) a[r][j] = times(a[r][j], f[r][q]);
+            }
+            uint4& b = bs[q & 1];
+            if (g < len) b = *reinterpret_cast<const uint4*>(xat + q * 64);
+            if constexpr (MX) {
+              float d[4];
+              mma_first(d, a[0], a[1], 0, b.x, b.y);
+              mma(d, a[0], a[1], 2, b.z, b.w);
+              const float* sx = xscale + ((piece * 2 + h) * 4 + q) * p.x_stride;
+              const float lo = mx_factor(codes[0], q), hi = mx_factor(codes[1], q), x0 = sx[0], x1 = sx[1];
+              if constexpr (WIDE) {
+                const float f0 = x0 / kXScale, f1 = x1 / kXScale;
+              const float s0 = f0 < 1.0f ? f0 : 1.0f, s1 = f1 < 1.0f ? f1 : 1.0f, b0 = f0 < 1.0f ? 1.0f : f0, b1 = f1 < 1.0f ? 1.0f : f1;
+                acc[0] = fmaf(d[0] * s0 * lo, b0, acc[0]);
+                acc[1] = fmaf(d[1] * s1 * lo, b1, acc[1]);
+                acc[2] = fmaf(d[2] * s0 * hi, b0, acc[2]);
+                acc[3] = fmaf(d[3] * s1 * hi, b1, acc[3]);
+              } else {
+                acc[0] = fmaf(d[0], lo * x0, acc[0]);
+                acc[1] = fmaf(d[1], lo * x1, acc[1]);
+                acc[2] = fmaf(d[2], hi * x0, acc[2]);
+                acc[3] = fmaf(d[3], hi * x1, acc[3]);
+              }
+            } else {
+              mma(acc, a[0], a[1], 0, b.x, b.y);
+              mma(acc, a[0], a[1], 2, b.z, b.w);
+            }
           }
         }
       }
-    }
+    };
+    if (MX && wide) pieces(std::true_type{});
+    else pieces(std::false_type{});
     float* mine = sums + (round & 1) * kSums;
     {
       float* to = mine + (warp * 8 + 2 * t) * kPad + g;
@@ -316,7 +338,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_rows_kernel(const __grid_cons
       if (token >= grp.z) continue;
       float v = 0.0f;
       for (int w = 0; w < stride; ++w) v += mine[(((sl << split) + w) * 8 + token) * kPad + lane_n];
-      if constexpr (!MX) v *= (p.gw ? __ldg(p.gw + (p.gw_each ? grp.x : 0)) : 1.0f) * gx;
+      if constexpr (MX) v *= wide ? 1.0f : 1.0f / kXScale;
+      else v *= (p.gw ? __ldg(p.gw + (p.gw_each ? grp.x : 0)) : 1.0f) * gx;
       static_cast<T*>(p.y)[(int64_t)(grp.y + token) * p.N + n] = Elem<T>::from_float(v);
     }
   }
