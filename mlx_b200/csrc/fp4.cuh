@@ -87,6 +87,13 @@ __device__ __forceinline__ float e8m0_value(uint32_t code) {
   return __uint_as_float(code == 255u ? 0x7FC00000u : (code == 0u ? 0x00400000u : code << 23));
 }
 
+// A product's sum is multiplied with the product of the two global scales; where that is no normal fp32 number, with the larger scale and
+// then the smaller one, so that only a result passes fp32's range.
+__device__ __forceinline__ bool one_factor(float both) { return !(both < 0x1p-126f || both > 0x1.FFFFFEp127f); }
+__device__ __forceinline__ float times_scales(float v, float gx, float gw) {
+  return one_factor(gx * gw) ? v * (gx * gw) : v * fmaxf(gx, gw) * fminf(gx, gw);
+}
+
 // Scale code and codes of a thread's 16 values.  MX: lanes 2i and 2i + 1 share a group; the whole warp calls.
 template <bool MX>
 __device__ __forceinline__ uint32_t quantize_unit(float (&v)[kUnit], uint32_t top, float G, uint32_t (&codes)[2]) {

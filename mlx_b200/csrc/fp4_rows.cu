@@ -338,8 +338,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_rows_kernel(const __grid_cons
       if (token >= grp.z) continue;
       float v = 0.0f;
       for (int w = 0; w < stride; ++w) v += mine[(((sl << split) + w) * 8 + token) * kPad + lane_n];
-      if constexpr (MX) v *= wide ? 1.0f : 1.0f / kXScale;
-      else v *= (p.gw ? __ldg(p.gw + (p.gw_each ? grp.x : 0)) : 1.0f) * gx;
+      if constexpr (MX) {
+        v *= wide ? 1.0f : 1.0f / kXScale;
+      } else {
+        v = times_scales(v, gx, p.gw ? __ldg(p.gw + (p.gw_each ? grp.x : 0)) : 1.0f);
+      }
       static_cast<T*>(p.y)[(int64_t)(grp.y + token) * p.N + n] = Elem<T>::from_float(v);
     }
   }

@@ -45,6 +45,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "fp4.cuh"
 #include "kernels.h"
 #include "tc_ptx.cuh"
 
@@ -423,6 +424,29 @@ __device__ __forceinline__ void store4(T* dst, int left, bool vec, float a, floa
   }
 }
 
+// nvfp4, global scales whose product is no normal fp32 number (rare, so out of line: a second factor in the kernel
+// costs 4 %, the calls 0 to 1.5 %): both
+// scales one after the other.  A warp's columns q0 to q1 (of 32) of a tile that is not cut, a lane per i;
+template <typename T>
+__device__ __noinline__ void store_far(const Params& p, const Piece& c, uint32_t acc, int i, int q0, int q1) {
+  const float gx = p.gb ? __ldg(p.gb) : 1.0f, gw = p.ga ? __ldg(p.ga + (p.ga_each ? c.e : 0)) : 1.0f;
+  for (int q = q0; q < q1; ++q) {
+    uint32_t v[32];
+    tcgen05_ld_x32(acc + 32 * q, v);
+    tcgen05_wait_ld();
+    T* y = static_cast<T*>(p.out) + (long long)(c.row0 + 32 * q) * p.I + i;
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (i < p.I && 32 * q + j < c.rows) y[(long long)j * p.I] = Elem<T>::from_float(fp4::times_scales(__uint_as_float(v[j]), gx, gw));
+  }
+}
+// and four i of one row of a cut one.
+template <typename T>
+__device__ __noinline__ void store4_far(const Params& p, int e, T* dst, int left, float a, float b, float c, float d) {
+  const float gx = p.gb ? __ldg(p.gb) : 1.0f, gw = p.ga ? __ldg(p.ga + (p.ga_each ? e : 0)) : 1.0f;
+  store4(dst, left, p.vec != 0, fp4::times_scales(a, gx, gw), fp4::times_scales(b, gx, gw), fp4::times_scales(c, gx, gw), fp4::times_scales(d, gx, gw));
+}
+
 template <typename T, Kind KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<KIND>, 1)
 grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
@@ -792,6 +816,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
         if (p.ga) alpha = __ldg(p.ga + (p.ga_each ? c.e : 0));
         if (p.gb) alpha *= __ldg(p.gb);
       }
+      const bool far = KIND == Kind::Nv && !fp4::one_factor(alpha);
       const uint32_t acc = tmem + ab * p.NT + lane_field;
       const int i_warp = c.i0 + rank * kLanes + quad * 32;
       auto release = [&]() {
@@ -854,11 +879,19 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              if (h < rows && i < p.I)
-                store4(out_row<T, KIND>(p, c, r + h * kEpiWarps) + i, p.I - i, p.vec != 0, sum[h].x * alpha, sum[h].y * alpha, sum[h].z * alpha, sum[h].w * alpha);
+              if (h < rows && i < p.I) {
+                T* dst = out_row<T, KIND>(p, c, r + h * kEpiWarps) + i;
+                if (far) store4_far(p, c.e, dst, p.I - i, sum[h].x, sum[h].y, sum[h].z, sum[h].w);
+                else store4(dst, p.I - i, p.vec != 0, sum[h].x * alpha, sum[h].y * alpha, sum[h].z * alpha, sum[h].w * alpha);
+              }
           }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");   // `last` may be written again
+        continue;
+      }
+      if (far) {
+        store_far<T>(p, bars->piece[n_piece & 1], acc, i_warp + lane, p0, p1);
+        release();
         continue;
       }
       if constexpr (sizeof(T) == 2) {
