@@ -400,7 +400,8 @@ int b200q_fp4_dequantize(const uint32_t* wq, const uint8_t* scales, int mode, co
  *   b200q_grouped_qqmm   y[t] = Gx Gw[e] (quantized x[t]) (wq[e], scales[e])^T: x is quantized on the way in the weights'
  *                        mode (b200q_fp4_quantize) and both go through the 4-bit tensor cores; every dtype.  sizes NULL and
  *                        E == 1: the dense product.  scale_per_group: global_scale_w has E entries, else one.
- * Sums are fp32, results are rounded once.  x, dy and w 16-byte aligned (qqmm: wq only); at most 4096 groups.
+ * Sums are fp32, results are rounded once.  x, dy and w 16-byte aligned (qqmm: wq only); at most 4096 groups, 2^30 - 256 rows of x
+ * (dw: and of a matrix, N) and widths of 2^31 - 256.
  */
 size_t b200q_grouped_mm_workspace_bytes(int64_t T, int64_t E, int64_t N, int64_t K, int transpose);
 int b200q_grouped_mm(const void* x, const void* w, const void* sizes, int size_bytes, void* y, int dtype, int64_t T, int64_t E,

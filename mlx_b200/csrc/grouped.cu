@@ -6,6 +6,9 @@ namespace b200q {
 namespace {
 
 constexpr int64_t kMostGroups = 4096;   // the table of groups is in shared memory (16 bytes each)
+// Rows of x, and of a matrix in the weights' gradient: the kernel's table holds the number of tiles of 256 of them in 22 bits, and adds two such
+// numbers in 31.  Widths: what 256 less one may be added to in 32 bits.
+constexpr int64_t kMostRows = (1 << 30) - 256, kMostWidth = INT32_MAX - 255;
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
@@ -24,8 +27,9 @@ int check_dtype(const char* tag, int dtype, bool f32) {
 }
 int check_dims(const char* tag, int64_t T, int64_t E, int64_t N, int64_t K) {
   if (T < 0 || E < 0 || N < 0 || K < 0) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] negative dimension.", tag);
-  if (T > INT32_MAX || N > INT32_MAX || K > INT32_MAX)
-    return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: dimension exceeds 2^31-1.", tag);
+  if (T > kMostRows) return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than 2^30 - 256 rows.", tag);
+  if (N > kMostWidth || K > kMostWidth)
+    return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: dimension exceeds 2^31 - 256.", tag);
   if (E > kMostGroups)
     return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than %lld groups.", tag, (long long)kMostGroups);
   return B200Q_OK;
@@ -208,6 +212,7 @@ extern "C" int b200q_grouped_mm_dw(const void* dy, const void* x, const void* si
   const char* tag = "grouped_mm_dw";
   if (int rc = check_dtype(tag, dtype, false)) return rc;
   if (int rc = check_dims(tag, T, E, N, K)) return rc;
+  if (N > kMostRows) return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than 2^30 - 256 rows per matrix.", tag);
   if (E == 0 || N == 0 || K == 0) return B200Q_OK;
   if (!dw) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -494,7 +494,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       bad |= n < 0 || n > p.T;
       return n < 0 ? 0 : (n > p.T ? p.T : (int)n);
     };
-    auto add = [&](int a, int b) { bad |= a + b > p.T; return min(a + b, p.T); };   // (T is at most 2^30)
+    auto add = [&](int a, int b) { bad |= a + b > p.T; return min(a + b, p.T); };   // (T is below 2^30)
     int at = 0;
     for (int e = lo; e < hi; ++e) at = add(at, size_of(e));
     int rows_end = at, total, all_steps;   // sums over all groups; a lane keeps those of the lanes before it
@@ -1136,8 +1136,6 @@ int grouped_tc(const GroupedTcArgs& a, cudaStream_t st) {
   p.sfb = a.sfb; p.sf_words = (int)a.sf_words;
   p.i_blocks = (p.I + kLanes - 1) / kLanes;
   p.ga = a.ga; p.gb = a.gb; p.ga_each = a.ga_each;
-  if (a.T > (1 << 30) || a.J > (1 << 30))
-    return fail(B200Q_ERR_UNSUPPORTED, "[grouped product] No implementation for problem shape: more than 2^30 rows");
   // number of tiles and steps in 32 bits
   const int64_t tiles = ((sum ? (a.J + p.NT - 1) / p.NT * a.E : a.T / p.NT + a.E + 1)) * p.i_tiles;
   const int64_t steps = sum ? (a.T / 64 + 2 * a.E) * ((a.J + p.NT - 1) / p.NT) * p.i_tiles : tiles * ((a.K + 63) / 64);

@@ -188,7 +188,7 @@ struct GroupedTcArgs {
   int size_bytes;
   void* out;                // [T, I], Sum: [E, J, I]
   int dtype;                // of out (and of 16-bit operands)
-  int64_t T, E, I, J, K;
+  int64_t T, E, I, J, K;    // T, J at most 2^30 - 256; I, K 2^31 - 256
   const uint32_t *sfa, *sfb;        // 4 bits: scales as fp4_prepare leaves them
   int64_t sf_words;                 // of four, per row
   const float *ga, *gb;             // global scales (null: 1); ga_each: one per group
