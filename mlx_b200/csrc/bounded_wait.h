@@ -43,4 +43,9 @@ B200Q_WAIT_FN void end_of_role(Last last, const volatile int* abort_flag, uint32
   }
 }
 
+// How many times 2^30 cycles (half a second) a role of the grouped kernel may wait for a whole tile: once, or more where the tile's sum has so
+// many stages (of 64 or 256 k) that twice what each takes at its slowest is longer: 1400 cycles, 64 KB per pair of blocks at a pair's
+// share of memory.
+inline int wait_times(int64_t stages) { return 1 + (int)(2 * 1400 * stages >> 30); }
+
 }  // namespace b200q

@@ -44,6 +44,7 @@
 
 #include <type_traits>
 
+#include "bounded_wait.h"
 #include "common.cuh"
 #include "fp4.cuh"
 #include "kernels.h"
@@ -102,6 +103,7 @@ struct Params {
   int ga_each;
   float* partial;          // [2 * pairs][block of the pair][NT][128]; null: no tile is cut
   uint32_t* counters;      // [pairs][block of the pair]
+  int wait_times;          // how many times kWaitMost a wait for a whole tile may last
   uint32_t* status;
 };
 
@@ -315,6 +317,19 @@ __device__ __forceinline__ bool wait_local(uint32_t bar, uint32_t parity, volati
   while (!mbar_try(bar, parity)) {
     if (*abort_flag) return false;
     if (clock64() - t0 > kWaitMost) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
+}
+// For a whole tile, as many times as long as its sum may take.
+__device__ __forceinline__ bool wait_tile(uint32_t bar, uint32_t parity, volatile int* abort_flag, int times) {
+  if (mbar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try(bar, parity)) {
+    if (*abort_flag) return false;
+    if ((int)((clock64() - t0) >> 30) >= times) {
       *abort_flag = 1;
       return false;
     }
@@ -686,7 +701,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       const int valid = c.len - (c.ks1 - 1) * 64;
       if (valid >= 64) continue;
       const uint32_t s = (at - 1) % (uint32_t)p.stages;
-      if (!__all_sync(0xFFFFFFFFu, wait_local(landed + s * 8, (ph >> s) & 1, abort_flag))) break;
+      if (!__all_sync(0xFFFFFFFFu, wait_tile(landed + s * 8, (ph >> s) & 1, abort_flag, p.wait_times))) break;
       ph ^= 1u << s;
       // blocks of 64 columns: two of a, one or two of b; eight lanes for a row of each
       const uint32_t tile = ring + s * stage_bytes + (lane >> 3) * 8192 + (lane & 7) * 16;
@@ -803,7 +818,7 @@ grouped_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Par
       // One warp looks and all go by what it found: the abort flag may be raised between two warps' looks.
       if (w == 0) {
         __syncwarp();
-        const bool seen = bars->more[n_piece & 1] && __all_sync(0xFFFFFFFFu, wait_local(smem_u32(&bars->acc_full[ab]), an & 1, abort_flag));
+        const bool seen = bars->more[n_piece & 1] && __all_sync(0xFFFFFFFFu, wait_tile(smem_u32(&bars->acc_full[ab]), an & 1, abort_flag, p.wait_times));
         if (lane == 0) bars->seen[n_piece & 1] = seen;
         __syncwarp();
       }
@@ -1131,6 +1146,7 @@ int grouped_tc(const GroupedTcArgs& a, cudaStream_t st) {
   p.counters = static_cast<uint32_t*>(a.ws);
   p.partial = reinterpret_cast<float*>(static_cast<char*>(a.ws) + kCounterBytes);
   p.status = a.status;
+  p.wait_times = wait_times(sum ? a.T / 64 + 1 : (a.K + (fp4 ? 255 : 63)) / (fp4 ? 256 : 64));
   p.sfb_chunk = p.NT > 128 ? 8192 : 4096;
   p.sf_slots = p.NT > 128 ? 4 : 8;
   p.sfb = a.sfb; p.sf_words = (int)a.sf_words;
