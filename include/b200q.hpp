@@ -222,6 +222,13 @@ inline const float* global_scale(const char* tag, const ArrayView& g, Fp4 mode, 
     throw std::invalid_argument(std::string("[") + tag + "] a global scale is one float32 (or one per matrix) and belongs to nvfp4");
   return static_cast<const float*>(g.data);
 }
+// A result that the library will write: as many elements of the right type as it writes.
+inline void validate_result(const char* tag, const ArrayView& out, int64_t size, Dtype type) {
+  if (out.dtype != type)
+    throw std::invalid_argument(std::string("[") + tag + "] unsupported dtype of the result: " + name(out.dtype) + " instead of " + name(type));
+  if (out.size() != size)
+    throw std::invalid_argument(std::string("[") + tag + "] the result's shape " + shape_str(out.shape) + " does not have " + std::to_string(size) + " elements");
+}
 inline int64_t matrices(const ArrayView& a) {
   int64_t n = 1;
   for (int i = 0; i < a.ndim() - 2; ++i) n *= a.shape[i];
@@ -239,6 +246,10 @@ inline void quantize(const ArrayView& w, ArrayView& wq, ArrayView& scales, Fp4 m
   if (!is_floating(w.dtype))
     throw std::invalid_argument(std::string("[quantize] Only real floating types can be quantized but w has type ") + name(w.dtype) + ".");
   detail::validate_fp4("quantize", wq, scales, mode);
+  bool ok = w.ndim() == wq.ndim() && w.dim(-1) == wq.dim(-1) * 8;
+  for (int i = 0; ok && i < w.ndim() - 1; ++i) ok = w.shape[i] == wq.shape[i];
+  if (!ok)
+    throw std::invalid_argument("[quantize] w " + detail::shape_str(w.shape) + " does not match the packed matrix " + detail::shape_str(wq.shape));
   const int64_t K = w.dim(-1), rows = K ? w.size() / K : 0;
   const float* g = detail::global_scale("quantize", global_scale, mode, detail::matrices(w));
   detail::check(b200q_fp4_quantize(w.data, (int)w.dtype, rows, K, (int)mode, g, global_scale.size() == 1 || !g ? (rows ? rows : 1) : w.dim(-2),
@@ -250,6 +261,7 @@ inline void dequantize(const ArrayView& wq, const ArrayView& scales, ArrayView& 
                        void* stream = nullptr) {
   detail::validate_fp4("dequantize", wq, scales, mode);
   const int64_t K = wq.dim(-1) * 8, rows = wq.dim(-1) ? wq.size() / wq.dim(-1) : 0;
+  if (is_floating(out.dtype)) detail::validate_result("dequantize", out, rows * K, out.dtype);   // (any other type the library refuses)
   const float* g = detail::global_scale("dequantize", global_scale, mode, detail::matrices(wq));
   detail::check(b200q_fp4_dequantize(static_cast<const uint32_t*>(wq.data), static_cast<const uint8_t*>(scales.data), (int)mode, g,
                                      global_scale.size() == 1 || !g ? (rows ? rows : 1) : wq.dim(-2), (int)out.dtype, rows, K, out.data, stream));
@@ -262,6 +274,7 @@ inline void qqmm(const ArrayView& x, const ArrayView& w, const ArrayView& scales
   const int64_t K = w.dim(-1) * 8;
   if (w.ndim() != 2 || x.ndim() < 1 || x.dim(-1) != K || !is_floating(x.dtype))
     throw std::invalid_argument("[qqmm] x " + detail::shape_str(x.shape) + " does not match the matrix w " + detail::shape_str(w.shape));
+  detail::validate_result("qqmm", out, (K ? x.size() / K : 0) * w.dim(0), x.dtype);
   detail::check(b200q_grouped_qqmm(x.data, static_cast<const uint32_t*>(w.data), static_cast<const uint8_t*>(scales.data), nullptr, 0, out.data,
                                    (int)x.dtype, K ? x.size() / K : 0, 1, w.dim(0), K, (int)mode,
                                    detail::global_scale("qqmm", global_scale_x, mode, 1), detail::global_scale("qqmm", global_scale_w, mode, 1), 0,
@@ -276,6 +289,7 @@ inline void grouped_qqmm(const ArrayView& x, const ArrayView& w, const ArrayView
   if (w.ndim() != 3 || x.ndim() != 2 || x.dim(1) != w.dim(2) * 8 || !is_floating(x.dtype))
     throw std::invalid_argument("[grouped_qqmm] x " + detail::shape_str(x.shape) + " does not match the matrices w " + detail::shape_str(w.shape));
   const int bytes = detail::size_bytes("grouped_qqmm", sizes, w.dim(0));
+  detail::validate_result("grouped_qqmm", out, x.dim(0) * w.dim(1), x.dtype);
   detail::check(b200q_grouped_qqmm(x.data, static_cast<const uint32_t*>(w.data), static_cast<const uint8_t*>(scales.data), sizes.data, bytes,
                                    out.data, (int)x.dtype, x.dim(0), w.dim(0), w.dim(1), x.dim(1), (int)mode,
                                    detail::global_scale("grouped_qqmm", global_scale_x, mode, 1),
@@ -290,6 +304,7 @@ inline void grouped_mm(const ArrayView& x, const ArrayView& w, const ArrayView& 
   if (w.ndim() != 3 || x.ndim() != 2 || x.dim(1) != w.dim(transpose ? 2 : 1) || x.dtype != w.dtype)
     throw std::invalid_argument("[grouped_mm] x " + detail::shape_str(x.shape) + " does not match the matrices w " + detail::shape_str(w.shape));
   const int bytes = detail::size_bytes("grouped_mm", sizes, w.dim(0));
+  detail::validate_result("grouped_mm", out, x.dim(0) * w.dim(transpose ? 1 : 2), x.dtype);
   detail::check(b200q_grouped_mm(x.data, w.data, sizes.data, bytes, out.data, (int)x.dtype, x.dim(0), w.dim(0), w.dim(transpose ? 1 : 2), x.dim(1),
                                  transpose ? 1 : 0, ws.data, ws.bytes, stream));
 }
@@ -300,6 +315,7 @@ inline void grouped_mm_dw(const ArrayView& dy, const ArrayView& x, const ArrayVi
   if (dy.ndim() != 2 || x.ndim() != 2 || dy.dim(0) != x.dim(0) || dy.dtype != x.dtype || sizes.ndim() != 1)
     throw std::invalid_argument("[grouped_mm_dw] dy and x must be matrices of one type with as many rows");
   const int bytes = detail::size_bytes("grouped_mm_dw", sizes, sizes.dim(0));
+  detail::validate_result("grouped_mm_dw", dw, sizes.dim(0) * dy.dim(1) * x.dim(1), x.dtype);
   const ArrayView &a = transpose ? dy : x, &b = transpose ? x : dy;
   detail::check(b200q_grouped_mm_dw(a.data, b.data, sizes.data, bytes, dw.data, (int)x.dtype, x.dim(0), sizes.dim(0), a.dim(1), b.dim(1), ws.data,
                                     ws.bytes, stream));
