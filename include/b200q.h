@@ -414,6 +414,9 @@ int b200q_grouped_qqmm(const void* x, const uint32_t* wq, const uint8_t* scales,
                        int64_t T, int64_t E, int64_t N, int64_t K, int mode, const float* global_scale_x,
                        const float* global_scale_w, int scale_per_group, void* ws, size_t ws_bytes, void* stream);
 
+/* Which kernel b200q_grouped_qqmm takes for operands on 16-byte boundaries ("fp4_rows", "grouped_tc"); grouped: with sizes. */
+const char* b200q_grouped_qqmm_kernel_name(int64_t T, int64_t E, int64_t N, int64_t K, int mode, int grouped);
+
 /*
  * Introspection for tests and benchmarks: name of the kernel family b200q_qmm would
  * launch for this problem ("qmv_rows", "qmv_mma", "qmm_tcgen05", "qvm",

@@ -68,6 +68,7 @@ SIGNATURES = {
     "b200q_grouped_mm_dw": (_i, [_vp, _vp, _vp, _i, _vp, _i, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
     "b200q_grouped_qqmm_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i]),
     "b200q_grouped_qqmm": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _i64, _i64, _i64, _i64, _i, _vp, _vp, _i, _vp, _sz, _vp]),
+    "b200q_grouped_qqmm_kernel_name": (ctypes.c_char_p, [_i64, _i64, _i64, _i64, _i, _i]),
     "b200q_qmm_kernel_name": (ctypes.c_char_p, [_i, _i64, _i64, _i64, _i64, _i, _i, _i]),
     "b200q_launch_count": (ctypes.c_uint64, []),
     "b200q_set_weights_constant": (None, [_i]),

@@ -164,6 +164,15 @@ extern "C" int b200q_grouped_qqmm(const void* x, const uint32_t* wq, const uint8
   return grouped_tc(a, st);
 }
 
+extern "C" const char* b200q_grouped_qqmm_kernel_name(int64_t T, int64_t E, int64_t N, int64_t K, int mode, int grouped) {
+  if (check_mode("qqmm", mode, K) || check_dims("qqmm", T, E, N, K) || (!grouped && E != 1)) return "invalid";
+  Fp4Rows few{};
+  few.mode = mode;
+  few.T = T; few.E = E; few.N = N; few.K = K;
+  few.sizes = grouped ? &few : nullptr;   // (whether there are any is all that matters)
+  return fp4_rows_supported(few) ? "fp4_rows" : "grouped_tc";
+}
+
 extern "C" size_t b200q_grouped_mm_workspace_bytes(int64_t T, int64_t E, int64_t N, int64_t K, int transpose) {
   if (T <= 0 || E <= 0 || N <= 0 || K <= 0) return 0;
   return grouped_bytes(T, E, N, K, transpose != 0);

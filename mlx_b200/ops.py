@@ -743,6 +743,12 @@ def grouped_qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, sizes: 
     return y if y is not None else _qqmm("grouped_qqmm", x, w, scales, sizes, group_size, bits, mode, global_scale_x, global_scale_w)
 
 
+def qqmm_kernel_name(M: int, N: int, K: int, mode: str = "nvfp4", experts: Optional[int] = None) -> str:
+    """Which kernel qqmm (experts: grouped_qqmm) launches for M rows of x and operands on 16-byte boundaries."""
+    code, _ = _fp4_params("qqmm_kernel_name", mode, None, None)
+    return _lib.load().b200q_grouped_qqmm_kernel_name(M, 1 if experts is None else experts, N, K, code, int(experts is not None)).decode()
+
+
 def _grouped_operands(tag, x, w, sizes, transpose):
     if x.dtype not in (torch.float16, torch.bfloat16) or w.dtype != x.dtype:
         raise ValueError(f"[{tag}] x and w must both be float16 or bfloat16 but are {x.dtype} and {w.dtype}.")
