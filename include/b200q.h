@@ -398,7 +398,8 @@ int b200q_fp4_dequantize(const uint32_t* wq, const uint8_t* scales, int mode, co
  *   b200q_grouped_mm_dw  dw[e] = sum over the rows of e of dy[t]^T x[t]  [E, N, K] (dy [T, N], x [T, K]): the gradient of
  *                        transpose-form weights; with dy and x (and N, K) exchanged that of the others.  No rows: zeros.
  *   b200q_grouped_qqmm   y[t] = Gx Gw[e] (quantized x[t]) (wq[e], scales[e])^T: x is quantized on the way in the weights'
- *                        mode (b200q_fp4_quantize) and both go through the 4-bit tensor cores; every dtype.  sizes NULL and
+ *                        mode (b200q_fp4_quantize); every dtype.  The codes are multiplied by the 4-bit tensor cores, those of
+ *                        up to 8 rows, where that is faster, as f16 numbers, which hold them exactly.  sizes NULL and
  *                        E == 1: the dense product.  scale_per_group: global_scale_w has E entries, else one.
  * Sums are fp32, results are rounded once.  x, dy and w 16-byte aligned (qqmm: wq only); at most 4096 groups, 2^30 - 256 rows of x
  * (dw: and of a matrix, N) and widths of 2^31 - 256.

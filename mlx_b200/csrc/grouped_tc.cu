@@ -34,12 +34,17 @@
 //
 // What bounds it, measured (bf16 unless said): many rows, power and the tensor cores, 84 to 86 % of whose cycles are busy
 // (4096 rows of 8 experts [14336, 4096] 363 us, 1320 TFLOP/s; 8192^3 1476); its gradient of the weights the same with 940 MB written
-// (407 us); 4 bits, L2, which delivers 10.2 TB/s (4096 rows through nvfp4 [14336, 4096] 113 us in 124 with fp4_prepare_kernel;
-// half of the MMAs left out: 8 % less); few rows, HBM (8 rows of 5 or 6 experts, 0.95 of its rate) or, below some 20 us, latencies:
+// (407 us); 4 bits, what is not hidden behind a quarter of the MMA time: of 165,000 cycles that the MMA thread of a pair takes for its 12 tiles of
+// 4096 rows through nvfp4 [14336, 4096] (113 us in 124 with fp4_prepare_kernel) it waits 23 % for the epilogue, since tiles of more than
+// 128 rows leave tensor memory for one accumulator only (3200 cycles a tile; 60 in bf16, which has two), 26 % for scales in tensor memory
+// and 9 % for operands (K = 16384: 8, 38 and 11 %; mxfp4: 25, 23 and 10 %).  L2 gives the bf16 form more (11.3 TB/s against 9.2).  From 19 groups on
+// their table leaves four stages instead of five and with them two buffers of scales instead of four: a stage takes 1130 cycles instead of 1020
+// (256 rows of each through nvfp4 [6144, 4096]).  Few rows, HBM (8 rows of 5 or 6 experts, 0.95 of its rate) or, below some 20 us, latencies:
 // 4000 to 5000 cycles until the first copy is issued, 2500 until it lands, 4000 for a cut tile's end.
 //
-// Every wait is bounded: when one runs out, the role raises the block's abort flag and the status word, all roles leave, tensor
-// memory is freed and the kernel ends.
+// Every wait on an mbarrier is bounded: when one runs out, the role raises the block's abort flag and the status word, all roles leave,
+// tensor memory is freed and the kernel ends.  What else waits ends by itself: the allocation of tensor memory (for other kernels'
+// blocks), the pair's barriers (for its own roles) and the wait for the kernel in front.
 #include <cuda.h>
 
 #include <type_traits>
@@ -101,7 +106,7 @@ struct Params {
   const float* ga;         // global scales: one, or (ga_each) one per group
   const float* gb;
   int ga_each;
-  float* partial;          // [2 * pairs][block of the pair][NT][128]; null: no tile is cut
+  float* partial;          // [2 * pairs][block of the pair][NT][128]
   uint32_t* counters;      // [pairs][block of the pair]
   int wait_times;          // how many times kWaitMost a wait for a whole tile may last
   uint32_t* status;

@@ -225,7 +225,7 @@ struct Fp4Prepare {
   uint32_t *sfx, *sfw;
 };
 int fp4_prepare(const Fp4Prepare& a, cudaStream_t st);
-// fp4_rows.cu : 4-bit products of up to 16 rows in one launch; operands as b200q_grouped_qqmm has them
+// fp4_rows.cu : 4-bit products of up to 8 rows in one launch; operands as b200q_grouped_qqmm has them
 struct Fp4Rows {
   const void* x;
   const uint32_t* wq;

@@ -727,7 +727,8 @@ def qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, group_size: Opt
          global_scale_w: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [..., K] times the transpose of a quantized matrix (w uint32 [N, K/8], scales uint8 [N, K/g]), both in 4-bit
     floating point: x is quantized on the way, as quantize(x, mode=mode, global_scale=global_scale_x) does, and the codes of
-    both go through the 4-bit tensor cores with their scales.  Sums in float32, the result [..., N] in x's type.
+    both are multiplied with their scales, by the 4-bit tensor cores or (up to 8 rows, where that is faster) as float16, which
+    holds them exactly.  Sums in float32, the result [..., N] in x's type.
     global_scale_w: what `w` was quantized with.  (QQMatmul of the reference, mlx/backend/cuda/quantized/qqmm.cpp.)"""
     y = _front.qqmm(x, w, scales, None, group_size, bits, mode, global_scale_x, global_scale_w)
     return y if y is not None else _qqmm("qqmm", x, w, scales, None, group_size, bits, mode, global_scale_x, global_scale_w)
