@@ -419,6 +419,73 @@ int b200q_grouped_qqmm(const void* x, const uint32_t* wq, const uint8_t* scales,
 const char* b200q_grouped_qqmm_kernel_name(int64_t T, int64_t E, int64_t N, int64_t K, int mode, int grouped);
 
 /*
+ * Routing of T tokens to experts.  logits [T, E] dtype; scores s are their softmax or sigmoid; keys are the logits, with a
+ * bias (float32 [E] on the device, or NULL) s + bias, in the order that 64 bits give them.  groups > 1: the experts are groups of
+ * E / groups consecutive ones, which are ranked by the sum of their best group_best (1 or 2) keys (without a bias: scores; one that is off adds
+ * nothing); the top_groups best stay.  Of what is left the `top` largest keys are taken in falling order.  Ties go to the lowest index, NaN
+ * is larger than every number.  An expert whose key is -inf is off; where too few are on, the last pairs have no expert.
+ *   weights [T, top] float32: the scores of the experts taken (renormalize: divided by their sum) times scale; no expert: 0
+ *   experts [T, top]: their indices; no expert: -1
+ *   sizes   [E]: pairs per expert
+ *   places  [T, top]: where a pair stands when pairs are sorted by expert (stably, pair p = t * top + j); no expert: -1
+ *   order   [T * top]: the pair at every place; behind the last pair with an expert -1 - p of those without
+ * b200q_route_dlogits: the gradient with respect to the logits (dtype) of the weights' gradient dw; none flows to the choice or the bias.
+ * At most 1024 experts, 32 of them per token, 32 groups and 2^31 - 1 pairs.  ws: plain scratch, 4-byte aligned.
+ */
+#define B200Q_SOFTMAX 0
+#define B200Q_SIGMOID 1
+size_t b200q_route_workspace_bytes(int64_t T, int64_t E, int64_t top);
+int b200q_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t top, int scoring, const float* bias, int64_t groups,
+                int64_t top_groups, int group_best, int renormalize, float scale, float* weights, int32_t* experts, int32_t* sizes,
+                int32_t* places, int32_t* order, void* ws, size_t ws_bytes, void* stream);
+int b200q_route_dlogits(const float* dw, const void* logits, int dtype, const int32_t* experts, int64_t T, int64_t E, int64_t top,
+                        int scoring, int renormalize, float scale, void* dlogits, void* stream);
+
+/*
+ * Rows between the tokens' order and the experts', every dtype.  places and order: as b200q_route leaves them; a place outside
+ * [0, T * top) is a pair without a row.
+ *   b200q_dispatch_rows      xs[places[t, j]] = x[t]   (x [T, D], xs [T * top, D]; rows whose order is negative: zeros)
+ *   b200q_combine_rows       out[t] = sum over j of weights[t, j] y[places[t, j]]   (weights NULL: 1, the gradient of dispatch)
+ *   b200q_combine_rows_grad  dys[places[t, j]] = weights[t, j] dy[t] (other rows: zeros),  dw[t, j] = <dy[t], y[places[t, j]]>;
+ *                            either may be NULL
+ * Sums are fp32, in the order of j, rounded once.  No workspace.
+ */
+int b200q_dispatch_rows(const void* x, int dtype, int64_t T, int64_t top, int64_t D, const int32_t* places, const int32_t* order,
+                        void* xs, void* stream);
+int b200q_combine_rows(const void* y, int dtype, int64_t T, int64_t top, int64_t D, const int32_t* places, const float* weights,
+                       void* out, void* stream);
+int b200q_combine_rows_grad(const void* dy, const void* y, int dtype, int64_t T, int64_t top, int64_t D, const int32_t* places,
+                            const int32_t* order, const float* weights, void* dys, float* dw, void* stream);
+
+/*
+ * Rows sorted by group (adapter): ids [T] integers of id_bytes (4 or 8) on the device; outside [0, n): no group.
+ *   sizes [n], starts [n + 1]: rows per group, and where each group (and behind them the rows without one) starts in the order
+ *   order [T]: rows by group, stably; those without a group last, as -1 - row
+ *   tiles [b200q_group_rows_tiles(T, n)][4] (16-byte aligned): what b200q_add_adapters reads: up to 64 places of one group each
+ * At most 4096 groups.  ws: plain scratch, 4-byte aligned.
+ */
+int64_t b200q_group_rows_tiles(int64_t T, int64_t n);
+size_t b200q_group_rows_workspace_bytes(int64_t T, int64_t n);
+int b200q_group_rows(const void* ids, int id_bytes, int64_t T, int64_t n, int32_t* sizes, int32_t* starts, int32_t* order, int32_t* tiles,
+                     void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * Low-rank adapters beside a shared projection: out[t] = y[t] + scales[l] b[l] (a[l] x[t]), l being row t's adapter; a row without one:
+ * y[t].  bf16 and f16; sums and the inner product in fp32, rounded once.
+ *   y, out [T, N] (out may be y), x [T, K], a [L, r, K], b [L, N, r] dtype; scales [L] float32 (NULL: 1)
+ *   order, starts, tiles: b200q_group_rows over L groups
+ *   h [T, r] float32: left with a[l] x in the order of the places, which the gradient takes (else scratch); the rows without adapter are not written
+ * b200q_add_adapters_grad: from dy [T, N] the gradients dx [T, K], da, db, each NULL where not wanted (that of y is dy); g [T, r]
+ * float32 is scratch, needed for dx and da.  h is needed for db, x for da, a for dx, b for dx and da.
+ * At most 4096 adapters, ranks of 4096 and widths of 2^24.
+ */
+int b200q_add_adapters(const void* y, const void* x, const void* a, const void* b, int dtype, int64_t T, int64_t L, int64_t N, int64_t K,
+                       int64_t r, const int32_t* order, const int32_t* tiles, const float* scales, float* h, void* out, void* stream);
+int b200q_add_adapters_grad(const void* dy, const void* x, const void* a, const void* b, int dtype, int64_t T, int64_t L, int64_t N,
+                            int64_t K, int64_t r, const int32_t* order, const int32_t* starts, const int32_t* tiles, const float* scales,
+                            const float* h, float* g, void* dx, void* da, void* db, void* stream);
+
+/*
  * Introspection for tests and benchmarks: name of the kernel family b200q_qmm would
  * launch for this problem ("qmv_rows", "qmv_mma", "qmm_tcgen05", "qvm",
  * "qmm_generic").

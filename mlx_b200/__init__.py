@@ -6,6 +6,8 @@ Drop-in for the reference's ``quantize`` / ``dequantize`` / ``quantized_matmul``
 """
 __all__ = ["quantize", "dequantize", "quantized_matmul", "gather_qmm", "gather_qmm_chain", "gather_qmm_swiglu",
            "quantized_embedding", "qqmm", "grouped_mm", "grouped_mm_dw", "grouped_qqmm",
+           "Routing", "route_experts", "route_dlogits", "dispatch_rows", "combine_rows", "combine_rows_grad",
+           "RowGroups", "group_rows", "add_adapters", "add_adapters_grad",
            "qmm_kernel_name", "qqmm_kernel_name", "set_weights_constant"]
 
 

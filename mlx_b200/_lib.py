@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(_HERE, "libb200q.so")
 
 F32, F16, BF16 = 0, 1, 2
 MXFP4, NVFP4 = 0, 1
+SOFTMAX, SIGMOID = 0, 1
 OK = 0
 ERR_INVALID_ARGUMENT = -1
 ERR_UNSUPPORTED = -2
@@ -69,6 +70,17 @@ SIGNATURES = {
     "b200q_grouped_qqmm_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i]),
     "b200q_grouped_qqmm": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _i64, _i64, _i64, _i64, _i, _vp, _vp, _i, _vp, _sz, _vp]),
     "b200q_grouped_qqmm_kernel_name": (ctypes.c_char_p, [_i64, _i64, _i64, _i64, _i, _i]),
+    "b200q_route_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "b200q_route": (_i, [_vp, _i, _i64, _i64, _i64, _i, _vp, _i64, _i64, _i, _i, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "b200q_route_dlogits": (_i, [_vp, _vp, _i, _vp, _i64, _i64, _i64, _i, _i, ctypes.c_float, _vp, _vp]),
+    "b200q_dispatch_rows": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "b200q_combine_rows": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "b200q_combine_rows_grad": (_i, [_vp, _vp, _i, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "b200q_group_rows_tiles": (_i64, [_i64, _i64]),
+    "b200q_group_rows_workspace_bytes": (_sz, [_i64, _i64]),
+    "b200q_group_rows": (_i, [_vp, _i, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "b200q_add_adapters": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "b200q_add_adapters_grad": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _i64] + [_vp] * 10),
     "b200q_qmm_kernel_name": (ctypes.c_char_p, [_i, _i64, _i64, _i64, _i64, _i, _i, _i]),
     "b200q_launch_count": (ctypes.c_uint64, []),
     "b200q_set_weights_constant": (None, [_i]),

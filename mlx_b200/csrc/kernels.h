@@ -241,6 +241,8 @@ struct Fp4Rows {
 };
 bool fp4_rows_supported(const Fp4Rows& a);
 int fp4_rows(const Fp4Rows& a, cudaStream_t st);
+// Rows per entry of the tile table that b200q_group_rows writes (group or -1, first position, rows, number of rows with a group).
+constexpr int kAdapterRows = 64;
 // dst rows of dst_pitch bytes (a multiple of 16) from src rows of src_bytes, padded with zeros.
 int repack_rows(const void* src, int64_t src_bytes, void* dst, int64_t dst_pitch, int64_t rows, cudaStream_t st);
 

@@ -1,0 +1,724 @@
+// Routing to experts (route, its gradient) and the order of rows by group (group_rows).
+//
+// Of every token's logits l [E]: scores s = softmax(l) or sigmoid(l); keys l, or s + bias where there is a bias.  Groups of
+// consecutive experts are ranked by the sum of their best one or two keys (of their scores without a bias) and the first top_groups of
+// them stay; of what is left the `top` largest keys are taken, ties to the lowest index.  Weights are the scores of the experts taken,
+// divided by their sum if asked for, times `scale`.  An expert whose key is -inf is off: it is never taken, and where too few are on,
+// a pair has expert -1, weight 0 and place -1.
+//
+// A warp has a token, a lane every 32nd expert.  Keys are compared as 32-bit integers of the same order (NaN above everything, 0:
+// not to be taken), so that a choice is two warp-wide integer reductions.  Which experts a token gets is decided in 64 bits: keys that
+// are logits need no rounding, and sums of rounded scores are taken in 32 bits only where neighbours are further apart than the
+// rounding can be; else the token's keys are computed again in 64 bits (choose64), for about a token in a thousand.
+//
+// The pairs (token, choice) are then counting-sorted by expert, stably: every warp has a contiguous range of tokens and counts into a
+// histogram of its own, so that a pair's rank among its warp's is known as it is chosen; sums over warps and blocks follow, the latter
+// in a second launch where there is more than one block.  No atomics: the order is the same every time.
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace b200q {
+namespace {
+
+constexpr int kMaxWarps = 32;
+constexpr uint32_t kFull = 0xffffffffu;
+
+// Integers in the order of the numbers; NaN above all, -0 as 0.  0 is below every number.
+__device__ __forceinline__ uint32_t code32(float f) {
+  if (f != f) return kFull;
+  const uint32_t b = __float_as_uint(f + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value32(uint32_t c) { return c == kFull ? __uint_as_float(0x7fffffffu) : __uint_as_float(c & 0x80000000u ? c ^ 0x80000000u : ~c); }
+__device__ __forceinline__ unsigned long long code64(double f) {
+  if (f != f) return ~0ull;
+  const unsigned long long b = (unsigned long long)__double_as_longlong(f + 0.0);
+  return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double value64(unsigned long long c) {
+  if (c == ~0ull) return __longlong_as_double(0x7fffffffffffffffll);
+  return __longlong_as_double((long long)(c >> 63 ? c ^ 0x8000000000000000ull : ~c));
+}
+__device__ __forceinline__ float warp_max(float v) {
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+template <typename F>
+__device__ __forceinline__ F warp_sum(F v) {
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+// Of the lanes' (code, index) the largest code's, at the lowest index.
+__device__ __forceinline__ void warp_best64(unsigned long long& c, int& i) {
+  for (int o = 16; o; o >>= 1) {
+    const unsigned long long c2 = __shfl_xor_sync(kFull, c, o);
+    const int i2 = __shfl_xor_sync(kFull, i, o);
+    if (c2 > c || (c2 == c && i2 < i)) { c = c2; i = i2; }
+  }
+}
+__device__ __forceinline__ float sigmoid(float l) { return 1.0f / (1.0f + expf(-l)); }
+
+struct RouteParams {
+  const void* logits;
+  const float* bias;
+  float* weights;
+  int *experts, *sizes, *places, *order;
+  uint32_t* hist;      // [blocks][E + 1]; one block: not used
+  int64_t T, per_block, per_warp;
+  int E, top, groups, top_groups, best, sigmoid, renormalize;
+  float scale;
+};
+
+// One token's experts, in 64 bits: lane j gets the j-th (-1: none).  `row` holds E numbers in shared memory.
+template <typename T>
+__device__ __noinline__ int choose64(const RouteParams& p, const T* logits, unsigned long long* row, int lane) {
+  const int E = p.E;
+  double m = -INFINITY, z = 1.0;
+  if (!p.sigmoid) {
+    for (int i = lane; i < E; i += 32) m = fmax(m, (double)Elem<T>::to_float(logits[i]));
+    for (int o = 16; o; o >>= 1) m = fmax(m, __shfl_xor_sync(kFull, m, o));
+    z = 0.0;
+    for (int i = lane; i < E; i += 32) z += exp((double)Elem<T>::to_float(logits[i]) - m);
+    z = warp_sum(z);
+  }
+  for (int i = lane; i < E; i += 32) {
+    const double l = (double)Elem<T>::to_float(logits[i]);
+    const double s = p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - m) / z;
+    const double key = p.bias ? s + (double)p.bias[i] : s;
+    row[i] = l == -INFINITY || key == -INFINITY ? 0 : code64(key);
+  }
+  __syncwarp();
+  uint32_t on = kFull;
+  const int size = E / p.groups;
+  if (p.groups > 1) {
+    unsigned long long rank = 0;
+    if (lane < p.groups) {
+      unsigned long long a = 0, b = 0;   // the best two
+      for (int i = lane * size; i < (lane + 1) * size; ++i) {
+        const unsigned long long c = row[i];
+        if (c > a) { b = a; a = c; } else if (c > b) b = c;
+      }
+      rank = a;
+      if (p.best == 2 && b != 0) rank = code64(value64(a) + value64(b));
+    }
+    on = 0;
+    for (int k = 0; k < p.top_groups; ++k) {
+      unsigned long long c = rank;
+      int i = lane;
+      warp_best64(c, i);
+      if (c == 0) break;
+      on |= 1u << i;
+      if (lane == i) rank = 0;
+    }
+  }
+  for (int i = lane; i < E; i += 32) {
+    if (!p.bias) {   // among experts the logits decide
+      const double l = (double)Elem<T>::to_float(logits[i]);
+      row[i] = l == -INFINITY ? 0 : code64(l);
+    }
+    if (p.groups > 1 && !(on >> (i / size) & 1)) row[i] = 0;
+  }
+  __syncwarp();
+  int mine = -1;
+  for (int j = 0; j < p.top; ++j) {
+    unsigned long long c = 0;
+    int at = E;
+    for (int i = lane; i < E; i += 32)
+      if (row[i] > c) { c = row[i]; at = i; }
+    warp_best64(c, at);
+    if (c == 0) break;
+    if (lane == j) mine = at;
+    if (lane == (at & 31)) row[at] = 0;
+    __syncwarp();
+  }
+  return mine;
+}
+
+// One token: lane j < top gets its j-th expert (-1: none) and the weight.  V = experts per lane.
+template <typename T, int V>
+__device__ __forceinline__ void route_token(const RouteParams& p, const T* logits, unsigned long long* row, int lane, int* expert, float* weight) {
+  const int E = p.E;
+  float l[V];
+  uint32_t u[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) l[v] = v * 32 + lane < E ? Elem<T>::to_float(logits[v * 32 + lane]) : -INFINITY;
+  const bool sums = p.groups > 1 && p.best == 2;
+  const bool scores = p.bias != nullptr || sums;
+  float m = -INFINITY, rz = 0.0f;   // softmax: the largest logit, 1 over the sum of exp(l - m)
+  if (!p.sigmoid && (scores || !p.renormalize)) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) m = fmaxf(m, l[v]);
+    m = warp_max(m);
+    if (m > -INFINITY) {
+      float z = 0.0f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) z += expf(l[v] - m);
+      rz = 1.0f / warp_sum(z);
+    }
+  }
+  uint32_t* row32 = reinterpret_cast<uint32_t*>(row);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int i = v * 32 + lane;
+    float key = l[v];
+    if (scores) {
+      const float s = p.sigmoid ? sigmoid(l[v]) : expf(l[v] - m) * rz;
+      if (p.bias && i < E) key = l[v] == -INFINITY ? -INFINITY : s + p.bias[i];
+      if (sums && i < E) {
+        const float k = p.bias ? key : s;
+        row32[i] = key == -INFINITY ? 0 : code32(k);
+      }
+    }
+    u[v] = i >= E || key == -INFINITY ? 0 : code32(key);
+    if (p.groups > 1 && !sums && i < E) row32[i] = u[v];
+  }
+  // how far two keys have to be apart for their rounded forms to be in the right order: 88 half units of the largest score
+  // (a sum of up to 37 terms, exp, the argument's rounding, a division), one of the sum with the bias; rounded up
+  const float room = p.sigmoid ? 0x1p-17f : 0x1p-17f * rz;
+  bool unsure = false;
+  if (p.groups > 1) {
+    __syncwarp();
+    const int size = E / p.groups;
+    uint32_t rank = 0;
+    if (lane < p.groups) {
+      uint32_t a = 0, b = 0;
+      int i = lane % size;   // lanes start at different places: no bank is asked twice
+      for (int n = 0; n < size; ++n) {
+        const uint32_t c = row32[lane * size + i];
+        if (c > a) { b = a; a = c; } else if (c > b) b = c;
+        i = i + 1 == size ? 0 : i + 1;
+      }
+      rank = a;
+      if (sums && b != 0) rank = code32(value32(a) + value32(b));
+    }
+    __syncwarp();
+    uint32_t on = 0, last = 0;
+    for (int k = 0; k < p.top_groups; ++k) {
+      const uint32_t c = __reduce_max_sync(kFull, rank);
+      if (c == 0) break;
+      const int i = __ffs(__ballot_sync(kFull, rank == c)) - 1;
+      on |= 1u << i;
+      last = c;
+      if (lane == i) rank = 0;
+    }
+    const uint32_t next = __reduce_max_sync(kFull, rank);
+    if (scores && next != 0 && last != 0) {
+      const float a = value32(last), b = value32(next);
+      unsure = a - b <= 2 * room + 0x1p-21f * fmaxf(fabsf(a), fabsf(b));
+    }
+    const uint32_t inv = ((1u << 20) + size - 1) / size;   // i / size for i < 1024
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (!(on >> (((v * 32 + lane) * inv >> 20) & 31) & 1)) u[v] = 0;
+  }
+  uint32_t best = 0;
+  int at = 0;
+  auto find = [&] {
+    best = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (u[v] > best) { best = u[v]; at = v; }
+  };
+  find();
+  int mine = -1;
+  uint32_t code = 0;   // lane j: the j-th key's
+  const int count = p.top + (p.bias ? 1 : 0);   // with a bias the first one left out has to be far enough away, too (lane `top`, if there is one)
+  for (int j = 0; j < count; ++j) {
+    const uint32_t c = __reduce_max_sync(kFull, best);
+    if (c == 0) break;
+    const int i = __reduce_min_sync(kFull, best == c ? at * 32 + lane : INT32_MAX);
+    if (lane == j) { mine = i; code = c; }
+    if (j == 32 && lane == 31) {   // (the 33rd has no lane)
+      const float a = value32(code), b = value32(c);
+      unsure |= a - b <= room + 0x1p-22f * fmaxf(fabsf(a), fabsf(b));
+    }
+    if (lane == (i & 31)) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (v == i >> 5) u[v] = 0;
+      find();
+    }
+  }
+  float lj = mine >= 0 ? Elem<T>::to_float(logits[mine]) : -INFINITY;
+  if (p.bias) {
+    const float bj = mine >= 0 ? p.bias[mine] : 0.0f;
+    const uint32_t c2 = __shfl_down_sync(kFull, code, 1);
+    const float l2 = __shfl_down_sync(kFull, lj, 1), b2 = __shfl_down_sync(kFull, bj, 1);
+    if (lane < 31 && code != 0 && c2 != 0 && !(lj == l2 && bj == b2)) {   // (the same numbers make the same key)
+      const float a = value32(code), b = value32(c2);
+      unsure |= a - b <= room + 0x1p-22f * fmaxf(fabsf(a), fabsf(b));
+    }
+  }
+  if (scores && __any_sync(kFull, unsure)) {
+    mine = choose64(p, logits, row, lane);
+    lj = mine >= 0 ? Elem<T>::to_float(logits[mine]) : -INFINITY;
+  }
+  if (lane >= p.top) { mine = -1; lj = -INFINITY; }
+  float w;
+  if (p.renormalize) {   // ratios, which neither the other experts nor small scores touch
+    const float top = warp_max(lj);
+    if (p.sigmoid) {
+      const float far = fminf(top, 0.0f);   // sigmoid(l) exp(-far) = exp(l - far) / (1 + exp(l))
+      w = lj > 0.0f ? sigmoid(lj) : expf(lj - far) / (1.0f + expf(lj));
+    } else {
+      w = expf(lj - top);
+    }
+    if (mine < 0) w = 0.0f;
+    else if (lj != lj) w = lj;
+    const float sum = warp_sum(w);
+    w = mine < 0 ? 0.0f : w / sum;
+  } else {
+    w = p.sigmoid ? sigmoid(lj) : expf(lj - m) * rz;
+    if (mine < 0) w = 0.0f;
+  }
+  *expert = mine;
+  *weight = w * p.scale;
+}
+
+// Exclusive sums of a[0, n) in shared memory, by the whole block.
+__device__ void block_scan(uint32_t* a, int n, uint32_t* warp_sums) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  const int each = (n + blockDim.x - 1) / blockDim.x, lo = min(tid * each, n), hi = min(lo + each, n);
+  uint32_t sum = 0;
+  for (int i = lo; i < hi; ++i) sum += a[i];
+  uint32_t before = sum;
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(kFull, before, o);
+    if (lane >= o) before += v;
+  }
+  if (lane == 31) warp_sums[warp] = before;
+  __syncthreads();
+  if (warp == 0) {
+    uint32_t v = lane < warps ? warp_sums[lane] : 0;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t q = __shfl_up_sync(kFull, v, o);
+      if (lane >= o) v += q;
+    }
+    warp_sums[lane] = v;
+  }
+  __syncthreads();
+  uint32_t run = before - sum + (warp ? warp_sums[warp - 1] : 0);
+  for (int i = lo; i < hi; ++i) {
+    const uint32_t v = a[i];
+    a[i] = run;
+    run += v;
+  }
+  __syncthreads();
+}
+
+// What the sort reads and writes; the last bin, n, is that of pairs without a group.
+struct SortParams {
+  const void* ids;     // of `bytes` each
+  int bytes;
+  uint32_t* rank;      // of every pair among its block's of the same group
+  uint32_t* hist;      // [blocks][n + 1]
+  int *sizes, *starts, *places, *order;   // starts and places may be null
+  int4* tiles;         // may be null
+  int64_t max_tiles, P, per_block;        // pairs
+  int n, blocks;
+};
+__device__ __forceinline__ int bin_of(const SortParams& p, int64_t i) {
+  const int64_t e = p.bytes == 8 ? static_cast<const int64_t*>(p.ids)[i] : static_cast<const int*>(p.ids)[i];
+  return e >= 0 && e < p.n ? (int)e : p.n;
+}
+// base: where the block's first pair of every bin goes; total: the bins' sizes (block 0 alone needs them, its own base being the bins' starts)
+__device__ void sort_finish(const SortParams& p, int block, const uint32_t* base, uint32_t* total, uint32_t* warp_sums) {
+  const int64_t lo = block * p.per_block, hi = min(lo + p.per_block, p.P);
+  for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) {
+    const int e = bin_of(p, i);
+    const uint32_t at = p.rank[i] + base[e];
+    if (p.places) p.places[i] = e < p.n ? (int)at : -1;
+    p.order[at] = e < p.n ? (int)i : (int)(-1 - i);
+  }
+  if (block != 0) return;
+  for (int e = threadIdx.x; e <= p.n; e += blockDim.x) {
+    if (e < p.n) p.sizes[e] = (int)total[e];
+    if (p.starts) p.starts[e] = (int)base[e];
+  }
+  if (p.tiles == nullptr) return;
+  const int bins = p.n + 1;
+  __syncthreads();
+  for (int e = threadIdx.x; e < bins; e += blockDim.x) total[e] = (total[e] + kAdapterRows - 1) / kAdapterRows;
+  __syncthreads();
+  block_scan(total, bins, warp_sums);
+  const uint32_t starts_of_none = base[p.n], rows = (uint32_t)p.P;
+  for (int64_t k = threadIdx.x; k < p.max_tiles; k += blockDim.x) {
+    int a = 0, b = bins;   // the last bin whose first tile is at or before k
+    while (b - a > 1) {
+      const int c = (a + b) / 2;
+      if (total[c] <= k) a = c; else b = c;
+    }
+    const uint32_t end = a < p.n ? base[a + 1] : rows, first = base[a] + (uint32_t)(k - total[a]) * kAdapterRows;
+    const int have = first < end ? (int)min(end - first, (uint32_t)kAdapterRows) : 0;
+    p.tiles[k] = make_int4(a < p.n ? a : -1, (int)first, have, (int)starts_of_none);
+  }
+}
+
+// hist: of every warp of the block [warps][bins].  Becomes the sums before every warp; the block's own sums go to `sums`.
+__device__ void sum_over_warps(uint32_t* hist, int bins, uint32_t* sums) {
+  const int warps = blockDim.x >> 5;
+  for (int e = threadIdx.x; e < bins; e += blockDim.x) {
+    uint32_t run = 0;
+    for (int w = 0; w < warps; ++w) {
+      const uint32_t v = hist[w * bins + e];
+      hist[w * bins + e] = run;
+      run += v;
+    }
+    sums[e] = run;
+  }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(V > 16 ? 512 : 1024) route_kernel(const RouteParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ uint32_t warp_sums[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, bins = p.E + 1;
+  const bool rows = p.bias != nullptr || p.groups > 1;
+  unsigned long long* row = reinterpret_cast<unsigned long long*>(smem) + (size_t)warp * p.E;
+  uint32_t* hist = reinterpret_cast<uint32_t*>(smem + (rows ? (size_t)warps * p.E * 8 : 0));
+  uint32_t* mine = hist + (size_t)warp * bins;
+  for (int e = lane; e < bins; e += 32) mine[e] = 0;
+  __syncwarp();
+  const int64_t block_lo = blockIdx.x * p.per_block, block_hi = min(block_lo + p.per_block, p.T);
+  const int64_t lo = min(block_lo + warp * p.per_warp, block_hi), hi = min(lo + p.per_warp, block_hi);
+  uint32_t* rank = reinterpret_cast<uint32_t*>(p.places);
+  for (int64_t t = lo; t < hi; ++t) {
+    int e;
+    float w;
+    route_token<T, V>(p, static_cast<const T*>(p.logits) + t * p.E, row, lane, &e, &w);
+    const uint32_t none = __ballot_sync(kFull, lane < p.top && e < 0);
+    if (lane < p.top) {
+      const int bin = e < 0 ? p.E : e;
+      const uint32_t r = mine[bin] + (e < 0 ? __popc(none & ((1u << lane) - 1)) : 0);
+      p.weights[t * p.top + lane] = w;
+      p.experts[t * p.top + lane] = e;
+      rank[t * p.top + lane] = r;
+    }
+    __syncwarp();
+    if (lane < p.top) {   // a token's experts are different ones
+      if (e >= 0) mine[e] += 1;
+      else if (lane == __ffs(none) - 1) mine[p.E] += __popc(none);
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  uint32_t* sums = hist + (size_t)warps * bins;
+  sum_over_warps(hist, bins, sums);
+  __syncthreads();
+  for (int64_t i = lo * p.top + lane; i < hi * p.top; i += 32) {
+    const int e = p.experts[i];
+    rank[i] += mine[e < 0 ? p.E : e];
+  }
+  if (gridDim.x > 1) {
+    for (int e = threadIdx.x; e < bins; e += blockDim.x) p.hist[(size_t)blockIdx.x * bins + e] = sums[e];
+    return;
+  }
+  uint32_t* total = sums + bins;
+  for (int e = threadIdx.x; e < bins; e += blockDim.x) total[e] = sums[e];
+  __syncthreads();
+  block_scan(sums, bins, warp_sums);
+  const SortParams s{p.experts, 4, rank, nullptr, p.sizes, nullptr, p.places, p.order, nullptr, 0, p.T * p.top, p.T * p.top, p.E, 1};
+  sort_finish(s, 0, sums, total, warp_sums);
+}
+
+__global__ void __launch_bounds__(1024) group_kernel(const SortParams p, int64_t per_warp) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ uint32_t warp_sums[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, bins = p.n + 1;
+  uint32_t* hist = reinterpret_cast<uint32_t*>(smem);
+  uint32_t* mine = hist + (size_t)warp * bins;
+  for (int e = lane; e < bins; e += 32) mine[e] = 0;
+  __syncwarp();
+  const int64_t block_lo = blockIdx.x * p.per_block, block_hi = min(block_lo + p.per_block, p.P);
+  const int64_t lo = min(block_lo + warp * per_warp, block_hi), hi = min(lo + per_warp, block_hi);
+  for (int64_t i0 = lo; i0 < hi; i0 += 32) {
+    const int64_t i = i0 + lane;
+    const int e = i < hi ? bin_of(p, i) : -1;
+    const uint32_t same = __match_any_sync(kFull, e);
+    if (e >= 0) p.rank[i] = mine[e] + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  uint32_t* sums = hist + (size_t)warps * bins;
+  sum_over_warps(hist, bins, sums);
+  __syncthreads();
+  for (int64_t i = lo + lane; i < hi; i += 32) p.rank[i] += mine[bin_of(p, i)];
+  if (gridDim.x > 1) {
+    for (int e = threadIdx.x; e < bins; e += blockDim.x) p.hist[(size_t)blockIdx.x * bins + e] = sums[e];
+    return;
+  }
+  uint32_t* total = sums + bins;
+  for (int e = threadIdx.x; e < bins; e += blockDim.x) total[e] = sums[e];
+  __syncthreads();
+  block_scan(sums, bins, warp_sums);
+  sort_finish(p, 0, sums, total, warp_sums);
+}
+
+// The second launch: every block adds up the histograms of those before it.
+__global__ void __launch_bounds__(1024) place_kernel(const SortParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ uint32_t warp_sums[32];
+  const int bins = p.n + 1;
+  uint32_t *base = reinterpret_cast<uint32_t*>(smem), *total = base + bins, *before = total + bins;
+  for (int e = threadIdx.x; e < bins; e += blockDim.x) { total[e] = 0; before[e] = 0; }
+  __syncthreads();
+  // threads by (part of the blocks, bin); sums of integers in shared memory, whose order does not matter
+  const int parts = max(1, (int)blockDim.x / bins);
+  for (int i = threadIdx.x; i < parts * bins; i += blockDim.x) {
+    const int part = i / bins, e = i % bins;
+    uint32_t all = 0, mine = 0;
+#pragma unroll 8
+    for (int b = part; b < p.blocks; b += parts) {
+      const uint32_t v = p.hist[(size_t)b * bins + e];
+      all += v;
+      if (b < (int)blockIdx.x) mine += v;
+    }
+    atomicAdd(&total[e], all);
+    atomicAdd(&before[e], mine);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < bins; e += blockDim.x) base[e] = total[e];
+  __syncthreads();
+  block_scan(base, bins, warp_sums);
+  for (int e = threadIdx.x; e < bins; e += blockDim.x) base[e] += before[e];
+  __syncthreads();
+  sort_finish(p, blockIdx.x, base, total, warp_sums);
+}
+
+template <typename K>
+int allow_smem(K kern, size_t bytes) {
+  if (bytes > 48 * 1024) B200Q_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  return B200Q_OK;
+}
+
+int place(const SortParams& s, cudaStream_t st) {
+  const size_t smem = (size_t)3 * (s.n + 1) * 4;
+  if (int rc = allow_smem(place_kernel, smem)) return rc;
+  place_kernel<<<s.blocks, 1024, smem, st>>>(s);
+  B200Q_LAUNCH_OK("place_kernel");
+  return B200Q_OK;
+}
+
+// ---- the gradient of the weights with respect to the logits.  A warp has a token.
+struct DlogitsParams {
+  const float* dw;
+  const void* logits;
+  const int* experts;
+  void* dlogits;
+  int64_t T;
+  int E, top, sigmoid, renormalize;
+  float scale;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) dlogits_kernel(const DlogitsParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (t >= p.T) return;
+  const T* l = static_cast<const T*>(p.logits) + t * p.E;
+  T* d = static_cast<T*>(p.dlogits) + t * p.E;
+  int e = lane < p.top ? p.experts[t * p.top + lane] : -1;
+  if (e >= p.E) e = -1;
+  const float lj = e >= 0 ? Elem<T>::to_float(l[e]) : -INFINITY;
+  const float g = e >= 0 ? p.dw[t * p.top + lane] * p.scale : 0.0f;
+  float dj;   // of lane j's expert
+  if (!p.sigmoid && !p.renormalize) {
+    float m = -INFINITY, z = 0.0f;
+    for (int i = lane; i < p.E; i += 32) m = fmaxf(m, Elem<T>::to_float(l[i]));
+    m = warp_max(m);
+    for (int i = lane; i < p.E; i += 32) z += m > -INFINITY ? expf(Elem<T>::to_float(l[i]) - m) : 0.0f;
+    z = warp_sum(z);
+    const float rz = z > 0.0f || z != z ? 1.0f / z : 0.0f;
+    const float pj = e >= 0 ? expf(lj - m) * rz : 0.0f;
+    const float mean = warp_sum(g * pj);
+    dj = pj * (g - mean);
+    for (int i = lane; i < p.E; i += 32) {
+      const float li = Elem<T>::to_float(l[i]);
+      d[i] = Elem<T>::from_float(li > -INFINITY || li != li ? -expf(li - m) * rz * mean : 0.0f);
+    }
+  } else {
+    float q = 0.0f;
+    if (p.renormalize) {
+      const float top = warp_max(lj);
+      if (p.sigmoid) q = lj > 0.0f ? sigmoid(lj) : expf(lj - fminf(top, 0.0f)) / (1.0f + expf(lj));
+      else q = expf(lj - top);
+      if (e < 0) q = 0.0f;
+      else if (lj != lj) q = lj;
+      const float sum = warp_sum(q);
+      q = e < 0 ? 0.0f : q / sum;
+      dj = q * (g - warp_sum(g * q));
+    } else {
+      dj = sigmoid(lj) * g;
+    }
+    if (p.sigmoid) dj *= sigmoid(-lj);
+    for (int i = lane; i < p.E; i += 32) d[i] = Elem<T>::from_float(0.0f);
+  }
+  __syncwarp();   // the row's stores before those of its experts
+  if (e >= 0) d[e] = Elem<T>::from_float(dj);
+}
+
+template <typename T>
+int launch_route(const RouteParams& p, int blocks, int warps, cudaStream_t st) {
+  const bool rows = p.bias != nullptr || p.groups > 1;
+  const size_t smem = (rows ? (size_t)warps * p.E * 8 : 0) + (size_t)(warps + 2) * (p.E + 1) * 4;
+  auto go = [&](auto kern) {
+    if (int rc = allow_smem(kern, smem)) return rc;
+    kern<<<blocks, warps * 32, smem, st>>>(p);
+    B200Q_LAUNCH_OK("route_kernel");
+    return (int)B200Q_OK;
+  };
+  if (p.E <= 32) return go(route_kernel<T, 1>);
+  if (p.E <= 64) return go(route_kernel<T, 2>);
+  if (p.E <= 128) return go(route_kernel<T, 4>);
+  if (p.E <= 256) return go(route_kernel<T, 8>);
+  if (p.E <= 512) return go(route_kernel<T, 16>);
+  return go(route_kernel<T, 32>);
+}
+
+// Blocks and warps: a decode batch in one block (one launch), else 16 tokens or more per block, two blocks per SM.
+struct Split { int blocks, warps; int64_t per_block, per_warp; };
+Split route_split(int64_t T, int64_t E) {
+  Split s{};
+  const int most = E > 512 ? 16 : kMaxWarps;
+  if (T <= 2 * most) {
+    s.blocks = 1;
+    s.warps = (int)std::min<int64_t>(T, most);
+  } else {
+    s.warps = 16;
+    s.blocks = (int)std::min<int64_t>((T + 15) / 16, 2 * 148);
+  }
+  s.per_block = (T + s.blocks - 1) / s.blocks;
+  s.per_warp = (s.per_block + s.warps - 1) / s.warps;
+  s.blocks = (int)((T + s.per_block - 1) / s.per_block);
+  return s;
+}
+Split group_split(int64_t T, int64_t n) {
+  Split s{};
+  s.warps = n <= 512 ? 32 : (n <= 1024 ? 16 : 8);   // their histograms share 132 KB at most
+  s.blocks = T <= 4096 ? 1 : (int)std::min<int64_t>((T + 2047) / 2048, 148);
+  if (s.blocks == 1) s.warps = (int)std::max<int64_t>(1, std::min<int64_t>(s.warps, (T + 31) / 32));
+  s.per_block = (T + s.blocks - 1) / s.blocks;
+  s.per_warp = ((s.per_block + s.warps - 1) / s.warps + 31) / 32 * 32;
+  s.blocks = (int)((T + s.per_block - 1) / s.per_block);
+  return s;
+}
+
+constexpr int64_t kMostPairs = INT32_MAX;   // places are 32-bit integers
+constexpr int64_t kMostExperts = 1024, kMostTop = 32, kMostGroups = 32, kMostRowGroups = 4096;
+
+int check_route(const char* tag, int dtype, int64_t T, int64_t E, int64_t top, int scoring) {
+  if (dtype != B200Q_F32 && dtype != B200Q_F16 && dtype != B200Q_BF16)
+    return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] unsupported dtype code %d", tag, dtype);
+  if (T < 0 || E < 1) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] no experts, or a negative number of tokens.", tag);
+  if (top < 1 || top > E) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] cannot take %lld of %lld experts.", tag, (long long)top, (long long)E);
+  if (scoring != B200Q_SOFTMAX && scoring != B200Q_SIGMOID) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] unknown scoring code %d", tag, scoring);
+  if (E > kMostExperts || top > kMostTop || T > kMostPairs / top)
+    return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than %lld experts, %lld of them per token or 2^31 - 1 pairs.", tag,
+                (long long)kMostExperts, (long long)kMostTop);
+  return B200Q_OK;
+}
+
+}  // namespace
+}  // namespace b200q
+
+using namespace b200q;
+
+extern "C" size_t b200q_route_workspace_bytes(int64_t T, int64_t E, int64_t top) {
+  if (T <= 0 || E <= 0 || top <= 0) return 0;
+  const Split s = route_split(T, E);
+  return s.blocks == 1 ? 0 : (size_t)s.blocks * (E + 1) * 4;
+}
+
+extern "C" int b200q_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t top, int scoring, const float* bias, int64_t groups,
+                           int64_t top_groups, int group_best, int renormalize, float scale, float* weights, int32_t* experts, int32_t* sizes,
+                           int32_t* places, int32_t* order, void* ws, size_t ws_bytes, void* stream) {
+  const char* tag = "route_experts";
+  if (int rc = check_route(tag, dtype, T, E, top, scoring)) return rc;
+  if (groups < 1 || E % groups != 0 || top_groups < 1 || top_groups > groups)
+    return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] cannot take %lld of %lld groups of %lld experts.", tag, (long long)top_groups, (long long)groups, (long long)E);
+  if (top > E / groups * top_groups)
+    return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] cannot take %lld experts out of %lld groups of %lld.", tag, (long long)top, (long long)top_groups, (long long)(E / groups));
+  if (group_best != 1 && group_best != 2) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] a group is ranked by its best 1 or 2 experts, not %d.", tag, group_best);
+  if (groups > kMostGroups) return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than %lld groups.", tag, (long long)kMostGroups);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (!sizes) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
+  if (T == 0) {
+    B200Q_CUDA_OK(cudaMemsetAsync(sizes, 0, (size_t)E * 4, st));
+    return B200Q_OK;
+  }
+  if (!logits || !weights || !experts || !places || !order) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
+  const Split s = route_split(T, E);
+  const size_t need = b200q_route_workspace_bytes(T, E, top);
+  if (need > 0 && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 4 != 0))
+    return fail(B200Q_ERR_WORKSPACE, "[%s] an aligned workspace of %zu bytes required, %zu given", tag, need, ws ? ws_bytes : (size_t)0);
+  if (top_groups == groups) groups = top_groups = 1;   // nothing to leave out
+  const RouteParams p{logits, bias, weights, experts, sizes, places, order, static_cast<uint32_t*>(ws), T, s.per_block, s.per_warp,
+                      (int)E, (int)top, (int)groups, (int)top_groups, group_best, scoring == B200Q_SIGMOID, renormalize != 0, scale};
+  const ScratchLock lock(ws);
+  int rc = dtype == B200Q_F32 ? launch_route<float>(p, s.blocks, s.warps, st)
+                              : (dtype == B200Q_F16 ? launch_route<__half>(p, s.blocks, s.warps, st) : launch_route<__nv_bfloat16>(p, s.blocks, s.warps, st));
+  if (rc || s.blocks == 1) return rc;
+  const SortParams sp{experts, 4, reinterpret_cast<uint32_t*>(places), static_cast<uint32_t*>(ws), sizes, nullptr, places, order, nullptr, 0, T * top, s.per_block * top, (int)E, s.blocks};
+  return place(sp, st);
+}
+
+extern "C" int b200q_route_dlogits(const float* dw, const void* logits, int dtype, const int32_t* experts, int64_t T, int64_t E, int64_t top, int scoring,
+                                   int renormalize, float scale, void* dlogits, void* stream) {
+  const char* tag = "route_experts";
+  if (int rc = check_route(tag, dtype, T, E, top, scoring)) return rc;
+  if (T == 0) return B200Q_OK;
+  if (!dw || !logits || !experts || !dlogits) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
+  const DlogitsParams p{dw, logits, experts, dlogits, T, (int)E, (int)top, scoring == B200Q_SIGMOID, renormalize != 0, scale};
+  const unsigned blocks = (unsigned)((T + 7) / 8);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == B200Q_F32) dlogits_kernel<float><<<blocks, 256, 0, st>>>(p);
+  else if (dtype == B200Q_F16) dlogits_kernel<__half><<<blocks, 256, 0, st>>>(p);
+  else dlogits_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(p);
+  B200Q_LAUNCH_OK("dlogits_kernel");
+  return B200Q_OK;
+}
+
+extern "C" int64_t b200q_group_rows_tiles(int64_t T, int64_t n) {
+  if (T <= 0 || n < 0) return 0;
+  return std::min(T, n + 1) + T / kAdapterRows;
+}
+extern "C" size_t b200q_group_rows_workspace_bytes(int64_t T, int64_t n) {
+  if (T <= 0 || n < 0) return 0;
+  const Split s = group_split(T, n);
+  return (size_t)T * 4 + (s.blocks == 1 ? 0 : (size_t)s.blocks * (n + 1) * 4);
+}
+
+extern "C" int b200q_group_rows(const void* ids, int id_bytes, int64_t T, int64_t n, int32_t* sizes, int32_t* starts, int32_t* order, int32_t* tiles,
+                                void* ws, size_t ws_bytes, void* stream) {
+  const char* tag = "group_rows";
+  if (T < 0 || n < 0) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] negative dimension.", tag);
+  if ((id_bytes != 4 && id_bytes != 8) || (ids && reinterpret_cast<uintptr_t>(ids) % id_bytes != 0))
+    return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] ids are aligned 4- or 8-byte integers", tag);
+  if (T > kMostPairs - 64 || n > kMostRowGroups)
+    return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than 2^31 - 65 rows or %lld groups.", tag, (long long)kMostRowGroups);
+  if (!starts || (n > 0 && !sizes)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (T == 0) {
+    if (n > 0) B200Q_CUDA_OK(cudaMemsetAsync(sizes, 0, (size_t)n * 4, st));
+    B200Q_CUDA_OK(cudaMemsetAsync(starts, 0, (size_t)(n + 1) * 4, st));
+    return B200Q_OK;
+  }
+  if (!ids || !order || !tiles) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
+  if (reinterpret_cast<uintptr_t>(tiles) % 16 != 0) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] tiles must be 16-byte aligned", tag);
+  const size_t need = b200q_group_rows_workspace_bytes(T, n);
+  if (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 4 != 0)
+    return fail(B200Q_ERR_WORKSPACE, "[%s] an aligned workspace of %zu bytes required, %zu given", tag, need, ws ? ws_bytes : (size_t)0);
+  const Split s = group_split(T, n);
+  uint32_t* rank = static_cast<uint32_t*>(ws);
+  const SortParams p{ids, id_bytes, rank, rank + T, sizes, starts, nullptr, order, reinterpret_cast<int4*>(tiles), b200q_group_rows_tiles(T, n), T, s.per_block, (int)n, s.blocks};
+  const size_t smem = (size_t)(s.warps + 2) * (n + 1) * 4;
+  const ScratchLock lock(ws);
+  if (int rc = allow_smem(group_kernel, smem)) return rc;
+  group_kernel<<<s.blocks, s.warps * 32, smem, st>>>(p, s.per_warp);
+  B200Q_LAUNCH_OK("group_kernel");
+  return s.blocks == 1 ? B200Q_OK : place(p, st);
+}

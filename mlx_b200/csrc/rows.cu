@@ -1,0 +1,205 @@
+// Rows between the tokens' order and the experts': dispatch_rows, combine_rows and their gradients.
+//
+//   dispatch  xs[places[t, j]] = x[t]
+//   combine   y[t] = sum over j of w[t, j] ys[places[t, j]]   (without w: the gradient of dispatch)
+//   its gradients  d ys[places[t, j]] = w[t, j] dy[t],  d w[t, j] = <dy[t], ys[places[t, j]]>
+//
+// Everything is bound by HBM, so every kernel goes by tokens: a token's row is read (or written) once, the experts' rows once each,
+// in pieces of 16 bytes.  Sums are fp32 in the order of j, rounded once.  A place outside [0, T top) is a pair without a row:
+// it adds nothing and gets nothing.  Rows that no pair has are those whose `order` is negative, the last ones; they get zeros.
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace b200q {
+namespace {
+
+template <typename T, int VEC>
+struct alignas(VEC * sizeof(T)) Vec {
+  T v[VEC];
+};
+constexpr int kThreads = 256;
+
+struct RowsParams {
+  const void *x, *y;       // tokens' rows; experts' rows
+  void* out;
+  const int *places, *order;
+  const float* weights;
+  float* dw;
+  int64_t T, R;            // tokens, rows (T * top)
+  int64_t D, pieces;       // width, pieces of VEC elements per row
+  int top;
+};
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) dispatch_kernel(const RowsParams p) {
+  using V = Vec<T, VEC>;
+  const V* x = static_cast<const V*>(p.x);
+  V* xs = static_cast<V*>(p.out);
+  const int64_t n = p.T * p.pieces, step = (int64_t)gridDim.x * kThreads;
+  const bool left = p.order[p.R - 1] < 0;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) {
+    const int64_t t = i / p.pieces, c = i - t * p.pieces;
+    const V v = x[i];
+    for (int j = 0; j < p.top; ++j) {
+      const int64_t at = p.places[t * p.top + j];
+      if (at >= 0 && at < p.R) xs[at * p.pieces + c] = v;
+    }
+    if (left)
+      for (int64_t r = t * p.top; r < (t + 1) * p.top; ++r)
+        if (p.order[r] < 0) xs[r * p.pieces + c] = V{};
+  }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) combine_kernel(const RowsParams p) {
+  using V = Vec<T, VEC>;
+  const V* y = static_cast<const V*>(p.y);
+  V* out = static_cast<V*>(p.out);
+  const int64_t n = p.T * p.pieces, step = (int64_t)gridDim.x * kThreads;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) {
+    const int64_t t = i / p.pieces, c = i - t * p.pieces;
+    float acc[VEC] = {};
+#pragma unroll 4
+    for (int j = 0; j < p.top; ++j) {
+      const int64_t at = p.places[t * p.top + j];
+      if (at < 0 || at >= p.R) continue;
+      const float w = p.weights ? p.weights[t * p.top + j] : 1.0f;
+      const V v = y[at * p.pieces + c];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] = fmaf(w, Elem<T>::to_float(v.v[k]), acc[k]);
+    }
+    V o;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) o.v[k] = Elem<T>::from_float(acc[k]);
+    out[i] = o;
+  }
+}
+
+// A block has a token.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) combine_grad_kernel(const RowsParams p) {
+  using V = Vec<T, VEC>;
+  __shared__ float part[32][kThreads / 32];
+  const int64_t t = blockIdx.x;
+  const V* dy = static_cast<const V*>(p.x) + t * p.pieces;
+  const V* y = static_cast<const V*>(p.y);
+  V* dys = static_cast<V*>(p.out);
+  for (int j = 0; j < p.top; ++j) {
+    const int64_t at = p.places[t * p.top + j];
+    const bool has = at >= 0 && at < p.R;
+    const float w = p.weights[t * p.top + j];
+    float dot = 0.0f;
+    if (has)
+      for (int64_t c = threadIdx.x; c < p.pieces; c += kThreads) {
+        const V g = dy[c];
+        if (p.dw) {
+          const V v = y[at * p.pieces + c];
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) dot = fmaf(Elem<T>::to_float(g.v[k]), Elem<T>::to_float(v.v[k]), dot);
+        }
+        if (dys) {
+          V o;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) o.v[k] = Elem<T>::from_float(w * Elem<T>::to_float(g.v[k]));
+          dys[at * p.pieces + c] = o;
+        }
+      }
+    for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if ((threadIdx.x & 31) == 0) part[j & 31][threadIdx.x >> 5] = dot;
+    if ((j & 31) == 31 || j == p.top - 1) {
+      __syncthreads();
+      const int j0 = j & ~31;
+      if (p.dw && threadIdx.x <= (unsigned)(j - j0)) {
+        float s = 0.0f;
+        for (int q = 0; q < kThreads / 32; ++q) s += part[threadIdx.x][q];
+        p.dw[t * p.top + j0 + threadIdx.x] = s;
+      }
+      __syncthreads();
+    }
+  }
+  if (dys && p.order[p.R - 1] < 0)
+    for (int64_t r = t * p.top; r < (t + 1) * p.top; ++r)
+      if (p.order[r] < 0)
+        for (int64_t c = threadIdx.x; c < p.pieces; c += kThreads) dys[r * p.pieces + c] = V{};
+}
+
+enum class Kind { Dispatch, Combine, Grad };
+
+template <typename T, int VEC>
+int launch(Kind kind, RowsParams p, cudaStream_t st) {
+  p.pieces = p.D / VEC;
+  const int64_t n = p.T * p.pieces;
+  const unsigned blocks = (unsigned)std::min<int64_t>((n + kThreads - 1) / kThreads, 148 * 8 * 16);
+  switch (kind) {
+    case Kind::Dispatch: dispatch_kernel<T, VEC><<<blocks, kThreads, 0, st>>>(p); break;
+    case Kind::Combine: combine_kernel<T, VEC><<<blocks, kThreads, 0, st>>>(p); break;
+    case Kind::Grad: combine_grad_kernel<T, VEC><<<(unsigned)p.T, kThreads, 0, st>>>(p); break;
+  }
+  B200Q_LAUNCH_OK("rows kernel");
+  return B200Q_OK;
+}
+
+int run(Kind kind, const RowsParams& p, int dtype, cudaStream_t st) {
+  const uintptr_t all = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.D * dtype_size(dtype));
+  const bool whole = all % 16 == 0;   // every piece of 16 bytes on its boundary
+  switch (dtype) {
+    case B200Q_F32: return whole ? launch<float, 4>(kind, p, st) : launch<float, 1>(kind, p, st);
+    case B200Q_F16: return whole ? launch<__half, 8>(kind, p, st) : launch<__half, 1>(kind, p, st);
+    default: return whole ? launch<__nv_bfloat16, 8>(kind, p, st) : launch<__nv_bfloat16, 1>(kind, p, st);
+  }
+}
+
+int check(const char* tag, int dtype, int64_t T, int64_t top, int64_t D) {
+  if (dtype != B200Q_F32 && dtype != B200Q_F16 && dtype != B200Q_BF16)
+    return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] unsupported dtype code %d", tag, dtype);
+  if (T < 0 || top < 0 || D < 0) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] negative dimension.", tag);
+  if (top > INT32_MAX || D > INT32_MAX || (top > 0 && T > INT32_MAX / top))
+    return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than 2^31 - 1 rows or elements in one.", tag);
+  return B200Q_OK;
+}
+bool aligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % dtype_size(dtype) == 0; }
+
+}  // namespace
+}  // namespace b200q
+
+using namespace b200q;
+
+extern "C" int b200q_dispatch_rows(const void* x, int dtype, int64_t T, int64_t top, int64_t D, const int32_t* places, const int32_t* order, void* xs,
+                                   void* stream) {
+  const char* tag = "dispatch_rows";
+  if (int rc = check(tag, dtype, T, top, D)) return rc;
+  if (T == 0 || top == 0 || D == 0) return B200Q_OK;
+  if (!x || !places || !order || !xs) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
+  if (!aligned(x, dtype) || !aligned(xs, dtype)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
+  const RowsParams p{x, nullptr, xs, places, order, nullptr, nullptr, T, T * top, D, 0, (int)top};
+  return run(Kind::Dispatch, p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b200q_combine_rows(const void* y, int dtype, int64_t T, int64_t top, int64_t D, const int32_t* places, const float* weights, void* out,
+                                  void* stream) {
+  const char* tag = "combine_rows";
+  if (int rc = check(tag, dtype, T, top, D)) return rc;
+  if (T == 0 || D == 0) return B200Q_OK;
+  if (!out || (top > 0 && (!y || !places))) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
+  if (!aligned(y, dtype) || !aligned(out, dtype)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
+  const RowsParams p{nullptr, y, out, places, nullptr, weights, nullptr, T, T * top, D, 0, (int)top};
+  return run(Kind::Combine, p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b200q_combine_rows_grad(const void* dy, const void* y, int dtype, int64_t T, int64_t top, int64_t D, const int32_t* places,
+                                       const int32_t* order, const float* weights, void* dys, float* dw, void* stream) {
+  const char* tag = "combine_rows";
+  if (int rc = check(tag, dtype, T, top, D)) return rc;
+  if (T == 0 || top == 0 || (!dys && !dw)) return B200Q_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (D == 0) {
+    if (dw) B200Q_CUDA_OK(cudaMemsetAsync(dw, 0, (size_t)T * top * 4, st));
+    return B200Q_OK;
+  }
+  if (!dy || (dw && !y) || !places || !order || !weights) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
+  if (!aligned(dy, dtype) || !aligned(y, dtype) || !aligned(dys, dtype)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
+  const RowsParams p{dy, y, dys, places, order, weights, dw, T, T * top, D, 0, (int)top};
+  return run(Kind::Grad, p, dtype, st);
+}

@@ -12,6 +12,7 @@ dW is a plain dense product (torch.matmul, a library GEMM) followed by group sum
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -176,3 +177,85 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, sizes: torch.Tensor, transpose:
     if y is not None:
         return y
     return _GroupedMmFn.apply(x, w, sizes, bool(transpose))
+
+
+class _RouteFn(torch.autograd.Function):
+    """The weights' gradient; the choice of the experts is constant."""
+
+    @staticmethod
+    def forward(ctx, logits, top, scoring, bias, groups, top_groups, group_best, renormalize, scale):
+        routing = ops.route_experts(logits, top, scoring, bias, groups, top_groups, group_best, renormalize, scale)
+        ctx.save_for_backward(logits, routing.experts)
+        ctx.cfg = (scoring, renormalize, scale)
+        ctx.mark_non_differentiable(*routing[1:])
+        return tuple(routing)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dw, *_):
+        logits, experts = ctx.saved_tensors
+        return (ops.route_dlogits(dw, logits, experts, *ctx.cfg),) + (None,) * 8
+
+
+def route_experts(logits: torch.Tensor, top: int, scoring: str = "softmax", bias: Optional[torch.Tensor] = None, groups: int = 1,
+                  top_groups: Optional[int] = None, group_best: int = 1, renormalize: bool = False, scale: float = 1.0) -> ops.Routing:
+    """ops.route_experts whose weights have a gradient with respect to the logits (of first order).  The bias gets none."""
+    return ops.Routing(*_RouteFn.apply(logits, top, scoring, None if bias is None else bias.detach(), groups, top_groups, group_best, renormalize, scale))
+
+
+class _DispatchFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, places, order):
+        ctx.save_for_backward(places, order)
+        return ops.dispatch_rows(x, ops.Routing(None, None, None, places, order))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dxs):
+        return ops.combine_rows(dxs, ops.Routing(None, None, None, *ctx.saved_tensors), weighted=False), None, None
+
+
+def dispatch_rows(x: torch.Tensor, routing: ops.Routing) -> torch.Tensor:
+    """ops.dispatch_rows with a gradient for x (of first order)."""
+    return _DispatchFn.apply(x, routing.places, routing.order)
+
+
+class _CombineFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, places, order):
+        ctx.save_for_backward(y, weights, places, order)
+        return ops.combine_rows(y, ops.Routing(weights, None, None, places, order))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        y, weights, places, order = ctx.saved_tensors
+        dys, dw = ops.combine_rows_grad(dy, y, ops.Routing(weights, None, None, places, order), *ctx.needs_input_grad[:2])
+        return dys, dw if dw is None else dw.to(weights.dtype), None, None
+
+
+def combine_rows(y: torch.Tensor, routing: ops.Routing) -> torch.Tensor:
+    """ops.combine_rows with gradients for y and routing.weights (of first order)."""
+    return _CombineFn.apply(y, routing.weights, routing.places, routing.order)
+
+
+class _AdaptersFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, x, a, b, scales, *groups):
+        out, h = ops._add_adapters(y, x, a, b, ops.RowGroups(*groups), scales)
+        ctx.save_for_backward(x, a, b, scales, h, *groups)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, a, b, scales, h, *groups = ctx.saved_tensors
+        for_y, *wanted = ctx.needs_input_grad[:4]
+        grads = ops.add_adapters_grad(dy, x, a, b, ops.RowGroups(*groups), h, scales, *wanted) if any(wanted) else (None,) * 3
+        return (dy if for_y else None, *grads) + (None,) * 5
+
+
+def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, groups: ops.RowGroups,
+                 scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """ops.add_adapters with gradients for y, x, a and b (of first order); the scales are constants."""
+    return _AdaptersFn.apply(y, x, a, b, None if scales is None else scales.detach(), *groups)

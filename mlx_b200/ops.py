@@ -12,9 +12,10 @@ Invalid arguments raise ``ValueError`` (the reference's std::invalid_argument).
 from __future__ import annotations
 
 import ctypes
+import operator
 import os
 import threading
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -815,3 +816,265 @@ def grouped_mm_dw(dy: torch.Tensor, x: torch.Tensor, sizes: torch.Tensor, transp
     if _checked():
         read_workspace_status(ws, torch.cuda.current_stream(dev).cuda_stream, "grouped")
     return dw
+
+
+# ------------------------------------------------------------------- routing, rows between tokens and experts, adapters
+class Routing(NamedTuple):
+    """What route_experts decides; pair p = token * top + choice.  weights float32 and experts int32 [..., top] (-1: no expert),
+    sizes int32 [E]: pairs per expert, as the grouped products take them; places int32 [..., top]: where a pair stands in the experts'
+    order (-1: nowhere); order int32 [tokens * top]: the pair at every place, behind the last one -1 - p of the pairs without an expert."""
+    weights: torch.Tensor
+    experts: torch.Tensor
+    sizes: torch.Tensor
+    places: torch.Tensor
+    order: torch.Tensor
+
+
+class RowGroups(NamedTuple):
+    """Rows sorted by group, as group_rows leaves them: sizes int32 [n], starts int32 [n + 1], order int32 [rows] (rows without a group last,
+    as -1 - row) and the table of tiles that add_adapters reads."""
+    sizes: torch.Tensor
+    starts: torch.Tensor
+    order: torch.Tensor
+    tiles: torch.Tensor
+
+
+_SCORING = {"softmax": _lib.SOFTMAX, "sigmoid": _lib.SIGMOID}
+
+
+def _scratch(nbytes: int, dev: torch.device) -> torch.Tensor:
+    """Plain scratch of one call: the allocator keeps it apart from every other call's, captured ones included."""
+    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+
+
+def _route_args(tag, logits, top, scoring, groups, top_groups, group_best):
+    if logits.dtype not in _DT:
+        raise ValueError(f"[{tag}] Only real floating types are supported but logits.dtype() == {logits.dtype}.")
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"[{tag}] logits must have a last dimension of experts but have shape {tuple(logits.shape)}.")
+    if scoring not in _SCORING:
+        raise ValueError(f"[{tag}] scoring is 'softmax' or 'sigmoid', not '{scoring}'.")
+    E = logits.shape[-1]
+    top, groups = operator.index(top), operator.index(groups)
+    top_groups = groups if top_groups is None else operator.index(top_groups)
+    if groups < 1 or E % groups != 0 or not 1 <= top_groups <= groups:
+        raise ValueError(f"[{tag}] cannot take {top_groups} of {groups} groups of {E} experts.")
+    if not 1 <= top <= E // groups * top_groups:
+        raise ValueError(f"[{tag}] cannot take {top} experts out of {top_groups} groups of {E // groups}.")
+    if group_best not in (1, 2):
+        raise ValueError(f"[{tag}] a group is ranked by its best 1 or 2 experts, not {group_best}.")
+    return E, top, groups, top_groups
+
+
+def route_experts(logits: torch.Tensor, top: int, scoring: str = "softmax", bias: Optional[torch.Tensor] = None, groups: int = 1,
+                  top_groups: Optional[int] = None, group_best: int = 1, renormalize: bool = False, scale: float = 1.0) -> Routing:
+    """Chooses `top` experts for every token from its router logits [..., E], and sorts the pairs by expert.
+
+    Scores are the logits' softmax or sigmoid.  Experts are taken by falling logit, or by falling score + bias where there is a bias
+    (float [E], which balances the experts' load and does not enter the weights), ties to the lowest index; the order is that of 64-bit
+    arithmetic.  groups > 1: of the groups of E / groups consecutive experts only the top_groups best stay, ranked by the sum of their
+    group_best (1 or 2) best.  Weights are the scores, renormalized to a sum of 1 over the experts taken if asked for, times scale.
+    An expert with a logit (or bias) of -inf is off and never taken: a token with too few experts on has pairs without one (expert
+    -1, weight 0, place -1), a token of padding none at all.  grad.route_experts is the same with the weights' gradient."""
+    tag = "route_experts"
+    E, top, groups, top_groups = _route_args(tag, logits, top, scoring, groups, top_groups, group_best)
+    if bias is not None and (not bias.dtype.is_floating_point or tuple(bias.shape) != (E,)):
+        raise ValueError(f"[{tag}] the bias is a floating-point tensor of {E} elements.")
+    dev = _require_cuda(tag, logits) if bias is None else _require_cuda(tag, logits, bias)
+    logits = logits.detach().contiguous()
+    bias = None if bias is None else bias.detach().to(torch.float32).contiguous()
+    lead, T = tuple(logits.shape[:-1]), torch.Size(logits.shape[:-1]).numel()
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=dev)
+        weights = torch.empty(lead + (top,), dtype=torch.float32, device=dev)
+        experts, sizes, places, order = new(*lead, top), new(E), new(*lead, top), new(T * top)
+        need = lib.b200q_route_workspace_bytes(T, E, top)
+        ws = _scratch(need, dev) if need else None
+        rc = lib.b200q_route(_ptr(logits), _DT[logits.dtype], T, E, top, _SCORING[scoring], _ptr(bias), groups, top_groups, group_best,
+                             int(bool(renormalize)), float(scale), _ptr(weights), _ptr(experts), _ptr(sizes), _ptr(places), _ptr(order),
+                             _ptr(ws), need, _stream(logits))
+    _lib.check(rc)
+    return Routing(weights, experts, sizes, places, order)
+
+
+def route_dlogits(dw: torch.Tensor, logits: torch.Tensor, experts: torch.Tensor, scoring: str = "softmax", renormalize: bool = False,
+                  scale: float = 1.0) -> torch.Tensor:
+    """The gradient with respect to the logits, in their type, of a loss whose gradient with respect to route_experts' weights is dw."""
+    tag = "route_dlogits"
+    if logits.dtype not in _DT or scoring not in _SCORING:
+        raise ValueError(f"[{tag}] unsupported logits.dtype() == {logits.dtype} or scoring '{scoring}'.")
+    if experts.dtype != torch.int32 or experts.ndim != logits.ndim or experts.shape[:-1] != logits.shape[:-1] or dw.shape != experts.shape:
+        raise ValueError(f"[{tag}] dw and experts (int32) must have one entry per pair, but have shapes {tuple(dw.shape)} and "
+                         f"{tuple(experts.shape)} with logits {tuple(logits.shape)}.")
+    dev = _require_cuda(tag, logits, dw, experts)
+    logits, dw, experts = logits.detach().contiguous(), dw.detach().to(torch.float32).contiguous(), experts.contiguous()
+    with torch.cuda.device(dev):
+        dl = torch.empty_like(logits)
+        rc = _lib.load().b200q_route_dlogits(_ptr(dw), _ptr(logits), _DT[logits.dtype], _ptr(experts), torch.Size(logits.shape[:-1]).numel(),
+                                             logits.shape[-1], experts.shape[-1], _SCORING[scoring], int(bool(renormalize)), float(scale),
+                                             _ptr(dl), _stream(logits))
+    _lib.check(rc)
+    return dl
+
+
+def _plan(tag, places, order):
+    if places.dtype != torch.int32 or order.dtype != torch.int32 or places.ndim < 1 or tuple(order.shape) != (places.numel(),):
+        raise ValueError(f"[{tag}] places and order are int32, with one entry per pair each, but have shapes {tuple(places.shape)} and {tuple(order.shape)}.")
+    return places.contiguous(), order.contiguous()
+
+
+def dispatch_rows(x: torch.Tensor, routing: Routing) -> torch.Tensor:
+    """The tokens' rows x [..., D] in the experts' order, [tokens * top, D]: the rows that grouped_mm and grouped_qqmm take with routing.sizes.
+    Rows behind the last pair with an expert are zeros."""
+    tag = "dispatch_rows"
+    if x.dtype not in _DT:
+        raise ValueError(f"[{tag}] Only real floating types are supported but x.dtype() == {x.dtype}.")
+    places, order = _plan(tag, routing.places, routing.order)
+    if x.ndim < 1 or x.shape[:-1] != places.shape[:-1]:
+        raise ValueError(f"[{tag}] x {tuple(x.shape)} does not have a row for every token of the routing {tuple(places.shape)}.")
+    dev = _require_cuda(tag, x, places, order)
+    x = x.detach().contiguous()
+    with torch.cuda.device(dev):
+        xs = torch.empty((order.shape[0], x.shape[-1]), dtype=x.dtype, device=dev)
+        rc = _lib.load().b200q_dispatch_rows(_ptr(x), _DT[x.dtype], torch.Size(x.shape[:-1]).numel(), places.shape[-1], x.shape[-1], _ptr(places),
+                                             _ptr(order), _ptr(xs), _stream(x))
+    _lib.check(rc)
+    return xs
+
+
+def _combine(tag, y, places, order, weights):
+    if y.dtype not in _DT:
+        raise ValueError(f"[{tag}] Only real floating types are supported but y.dtype() == {y.dtype}.")
+    places, order = _plan(tag, places, order)
+    if y.ndim != 2 or y.shape[0] != order.shape[0]:
+        raise ValueError(f"[{tag}] y {tuple(y.shape)} does not have a row for every pair of the routing {tuple(places.shape)}.")
+    if weights is not None and (not weights.dtype.is_floating_point or weights.shape != places.shape):
+        raise ValueError(f"[{tag}] the weights must be one floating-point number per pair but have shape {tuple(weights.shape)}.")
+    dev = _require_cuda(tag, y, places, order) if weights is None else _require_cuda(tag, y, places, order, weights)
+    return dev, y.detach().contiguous(), places, order, None if weights is None else weights.detach().to(torch.float32).contiguous()
+
+
+def combine_rows(y: torch.Tensor, routing: Routing, weighted: bool = True) -> torch.Tensor:
+    """The experts' results y [tokens * top, D], in their order, back to the tokens: out[t] = sum of weights[t, j] y[places[t, j]], [..., D];
+    weighted=False: the plain sum, which is the gradient of dispatch_rows.  Sums in float32, in the order of the choices."""
+    dev, y, places, _, weights = _combine("combine_rows", y, routing.places, routing.order, routing.weights if weighted else None)
+    with torch.cuda.device(dev):
+        out = torch.empty(tuple(places.shape[:-1]) + (y.shape[1],), dtype=y.dtype, device=dev)
+        rc = _lib.load().b200q_combine_rows(_ptr(y), _DT[y.dtype], torch.Size(places.shape[:-1]).numel(), places.shape[-1], y.shape[1], _ptr(places),
+                                            _ptr(weights), _ptr(out), _stream(y))
+    _lib.check(rc)
+    return out
+
+
+def combine_rows_grad(dy: torch.Tensor, y: torch.Tensor, routing: Routing, for_y: bool = True, for_weights: bool = True):
+    """-> gradients of combine_rows with respect to y and to the weights (None where not asked for)."""
+    tag = "combine_rows_grad"
+    if dy.dtype != y.dtype or y.ndim != 2 or tuple(dy.shape) != tuple(routing.places.shape[:-1]) + (y.shape[1],):
+        raise ValueError(f"[{tag}] dy {tuple(dy.shape)} ({dy.dtype}) does not match the result of combine_rows.")
+    dev, y, places, order, weights = _combine(tag, y, routing.places, routing.order, routing.weights)
+    _require_cuda(tag, y, dy)
+    dy = dy.detach().contiguous()
+    with torch.cuda.device(dev):
+        dys = torch.empty_like(y) if for_y else None
+        dw = torch.empty_like(weights) if for_weights else None
+        rc = _lib.load().b200q_combine_rows_grad(_ptr(dy), _ptr(y), _DT[y.dtype], torch.Size(places.shape[:-1]).numel(), places.shape[-1], y.shape[1],
+                                                 _ptr(places), _ptr(order), _ptr(weights), _ptr(dys), _ptr(dw), _stream(y))
+    _lib.check(rc)
+    return dys, dw
+
+
+def group_rows(ids: torch.Tensor, n: int) -> RowGroups:
+    """Rows sorted by group: ids, any integers, name every row's group (adapter); outside [0, n): none.  Computed once for a batch
+    and used beside all its projections."""
+    tag = "group_rows"
+    if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
+        raise ValueError(f"[{tag}] ids must be integral but are {ids.dtype}.")
+    n = operator.index(n)
+    if n < 0:
+        raise ValueError(f"[{tag}] there cannot be {n} groups.")
+    dev = _require_cuda(tag, ids)
+    ids = (ids if ids.dtype in (torch.int32, torch.int64) else ids.to(torch.int64)).contiguous()
+    T = ids.numel()
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=dev)
+        sizes, starts, order, tiles = new(n), new(n + 1), new(T), new(lib.b200q_group_rows_tiles(T, n), 4)
+        need = lib.b200q_group_rows_workspace_bytes(T, n)
+        ws = _scratch(need, dev)
+        rc = lib.b200q_group_rows(_ptr(ids), ids.element_size(), T, n, _ptr(sizes), _ptr(starts), _ptr(order), _ptr(tiles), _ptr(ws), need, _stream(ids))
+    _lib.check(rc)
+    return RowGroups(sizes, starts, order, tiles)
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    end = lambda t: t.data_ptr() + t.numel() * t.element_size()
+    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
+def _adapter_args(tag, y, x, a, b, groups, scales):
+    if x.dtype not in (torch.float16, torch.bfloat16) or any(t.dtype != x.dtype for t in (y, a, b)):
+        raise ValueError(f"[{tag}] y, x, a and b must all be float16 or bfloat16 but are {y.dtype}, {x.dtype}, {a.dtype} and {b.dtype}.")
+    if a.ndim != 3 or b.ndim != 3 or x.ndim < 1 or y.ndim < 1:
+        raise ValueError(f"[{tag}] a and b must have three dimensions and x and y one at least, but they have {a.ndim}, {b.ndim}, {x.ndim} and {y.ndim}.")
+    L, r, K, N = *a.shape, b.shape[1]
+    if b.shape[0] != L or b.shape[2] != r or x.shape[-1] != K or y.shape[-1] != N or x.shape[:-1] != y.shape[:-1]:
+        raise ValueError(f"[{tag}] The shapes of y {tuple(y.shape)}, x {tuple(x.shape)}, a {tuple(a.shape)} and b {tuple(b.shape)} do not match: "
+                         "[..., N], [..., K], [adapters, rank, K] and [adapters, N, rank] are needed")
+    T = torch.Size(x.shape[:-1]).numel()
+    if any(t.dtype != torch.int32 for t in groups) or tuple(groups.sizes.shape) != (L,) or tuple(groups.starts.shape) != (L + 1,) or \
+            tuple(groups.order.shape) != (T,) or tuple(groups.tiles.shape) != (_lib.load().b200q_group_rows_tiles(T, L), 4):
+        raise ValueError(f"[{tag}] the groups are not those of group_rows for {T} rows and {L} adapters.")
+    if scales is not None and (not scales.dtype.is_floating_point or tuple(scales.shape) != (L,)):
+        raise ValueError(f"[{tag}] the scales are one floating-point number per adapter.")
+    dev = _require_cuda(tag, y, x, a, b, *groups, *(() if scales is None else (scales,)))
+    scales = None if scales is None else scales.detach().to(torch.float32).contiguous()
+    return dev, T, L, N, K, r, RowGroups(*(t.contiguous() for t in groups)), scales
+
+
+def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, groups: RowGroups, scales: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Low-rank adapters of many requests at once beside a shared projection: y [..., N], what the projection (quantized_matmul, qqmm, ...)
+    made of x [..., K], plus scales[l] b[l] (a[l] x[t]) for every row t with an adapter l.  a [adapters, rank, K], b [adapters, N, rank],
+    scales [adapters] (None: 1); groups: group_rows of the rows' adapters.  bfloat16 and float16; sums and the inner product in float32,
+    rounded once.  out: where the sum goes, y itself for a sum in place.  grad.add_adapters is the same with gradients."""
+    return _add_adapters(y, x, a, b, groups, scales, out)[0]
+
+
+def _add_adapters(y, x, a, b, groups, scales=None, out=None):
+    """-> add_adapters' result and the inner products, float32 [rows, rank] in the order of the groups."""
+    tag = "add_adapters"
+    dev, T, L, N, K, rank, groups, scales = _adapter_args(tag, y, x, a, b, groups, scales)
+    if out is not None:
+        if out.dtype != y.dtype or out.shape != y.shape or out.device != y.device or not out.is_contiguous():
+            raise ValueError(f"[{tag}] out must be a contiguous tensor like y.")
+        if any(_overlap(out, t) for t in (x, a, b)) or (_overlap(out, y) and (out.data_ptr() != y.data_ptr() or not y.is_contiguous())):
+            raise ValueError(f"[{tag}] out must be y itself or not overlap the operands.")
+    y, x, a, b = (t.detach().contiguous() for t in (y, x, a, b))
+    with torch.cuda.device(dev):
+        out = torch.empty_like(y) if out is None else out
+        h = torch.empty((T, rank), dtype=torch.float32, device=dev)
+        rc = _lib.load().b200q_add_adapters(_ptr(y), _ptr(x), _ptr(a), _ptr(b), _DT[x.dtype], T, L, N, K, rank, _ptr(groups.order), _ptr(groups.tiles),
+                                            _ptr(scales), _ptr(h), _ptr(out), _stream(x))
+    _lib.check(rc)
+    return out, h
+
+
+def add_adapters_grad(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, groups: RowGroups, h: torch.Tensor,
+                      scales: Optional[torch.Tensor] = None, for_x: bool = True, for_a: bool = True, for_b: bool = True):
+    """-> gradients of add_adapters with respect to x, a and b (None where not asked for; that of y is dy).  h: a[l] x in float32, as the
+    forward pass leaves it."""
+    tag = "add_adapters_grad"
+    dev, T, L, N, K, rank, groups, scales = _adapter_args(tag, dy, x, a, b, groups, scales)
+    if h.dtype != torch.float32 or tuple(h.shape) != (T, rank):
+        raise ValueError(f"[{tag}] h must be float32 [{T}, {rank}].")
+    _require_cuda(tag, x, h)
+    dy, x, a, b, h = (t.detach().contiguous() for t in (dy, x, a, b, h))
+    with torch.cuda.device(dev):
+        dx, da, db = (torch.empty_like(t) if wanted else None for t, wanted in ((x, for_x), (a, for_a), (b, for_b)))
+        g = torch.empty((T, rank), dtype=torch.float32, device=dev) if for_x or for_a else None
+        rc = _lib.load().b200q_add_adapters_grad(_ptr(dy), _ptr(x), _ptr(a), _ptr(b), _DT[x.dtype], T, L, N, K, rank, _ptr(groups.order),
+                                                 _ptr(groups.starts), _ptr(groups.tiles), _ptr(scales), _ptr(h), _ptr(g), _ptr(dx), _ptr(da), _ptr(db),
+                                                 _stream(x))
+    _lib.check(rc)
+    return dx, da, db
