@@ -609,6 +609,413 @@ PyObject* py_grouped_mm_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {   //
   END_HANDLE_TH_ERRORS
 }
 
+// ---- routing, rows between tokens and experts, adapters.  None of them uses the scratch table: what scratch they need is allocated per call.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void* stream_of(at::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+Tensor fresh(at::IntArrayRef size, at::ScalarType t, at::Device dev) { return at::detail::empty_cuda(size, t, dev, std::nullopt); }
+bool plain(const Tensor& t, at::ScalarType type, at::Device dev) { return t.scalar_type() == type && t.device() == dev && t.is_contiguous(); }
+int64_t lead_of(const Tensor& t) { return product(t.sizes().slice(0, t.dim() - 1)); }
+bool tangent(const Tensor& t) { return t._fw_grad(0).defined(); }   // forward mode: the Python form says that there is none
+bool number(PyObject* o, float* out) {
+  if (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o)) return false;
+  const double v = PyFloat_AsDouble(o);
+  if (PyErr_Occurred()) { PyErr_Clear(); return false; }
+  *out = (float)v;
+  return true;
+}
+// The tensors of a tuple (a NamedTuple, too).
+template <int N>
+bool members(PyObject* o, const Tensor* (&t)[N]) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != N) return false;
+  for (int i = 0; i < N; ++i) t[i] = tensor(PyTuple_GET_ITEM(o, i));
+  return true;
+}
+PyObject* pack(variable_list&& ts) {
+  PyObject* out = PyTuple_New((Py_ssize_t)ts.size());
+  if (!out) return nullptr;
+  for (size_t i = 0; i < ts.size(); ++i) PyTuple_SET_ITEM(out, (Py_ssize_t)i, THPVariable_Wrap(std::move(ts[i])));
+  return out;
+}
+pybind11::object wrapped(const Tensor& t) { return pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(t)); }
+pybind11::object python(const char* module, const char* name) { return pybind11::module_::import(module).attr(name); }
+Tensor unwrapped(const pybind11::handle& o) { return o.is_none() ? Tensor() : Tensor(THPVariable_Unpack(o.ptr())); }
+// Gradients of first order: where a graph of them is asked for, one whose backward pass says so.
+void first_order(std::initializer_list<Tensor*> grads) {
+  if (!at::GradMode::is_enabled()) return;
+  pybind11::gil_scoped_acquire gil;
+  for (Tensor* g : grads)
+    if (g->defined()) *g = unwrapped(python("mlx_b200.grad", "_first_order")(wrapped(*g)));
+}
+
+struct Route {
+  int top, groups, top_groups, best, scoring;
+  bool renormalize;
+  float scale;
+  const Tensor* bias;
+};
+// (logits, top, scoring, bias, groups, top_groups, group_best, renormalize, scale)
+bool route_args(PyObject* const* a, Py_ssize_t n, const Tensor** logits, Route* r) {
+  if (n != 9 || !(*logits = tensor(a[0])) || !PyLong_CheckExact(a[1]) || !integer(a[1], 0, &r->top) || !index_arg(a[3], &r->bias) || !PyLong_CheckExact(a[4]) ||
+      !integer(a[4], 1, &r->groups) || !integer(a[5], r->groups, &r->top_groups) || !PyLong_CheckExact(a[6]) || !integer(a[6], 1, &r->best) ||
+      !PyBool_Check(a[7]) || !number(a[8], &r->scale) || !PyUnicode_Check(a[2]))
+    return false;
+  r->renormalize = a[7] == Py_True;
+  if (PyUnicode_CompareWithASCIIString(a[2], "softmax") == 0) r->scoring = B200Q_SOFTMAX;
+  else if (PyUnicode_CompareWithASCIIString(a[2], "sigmoid") == 0) r->scoring = B200Q_SIGMOID;
+  else return false;
+  return true;
+}
+bool route_run(const Tensor& l, const Route& r, variable_list* out) {
+  const int dt = dtype_code(l.scalar_type());
+  const at::Device dev = l.device();
+  if (dt < 0 || !current(dev) || l.dim() < 1 || !l.is_contiguous() || l.numel() == 0) return false;
+  const int64_t E = l.size(-1), T = lead_of(l);
+  if (r.top < 1 || r.top > E || (r.bias && (!plain(*r.bias, at::kFloat, dev) || r.bias->dim() != 1 || r.bias->size(0) != E))) return false;
+  c10::SmallVector<int64_t, 6> size(l.sizes().begin(), l.sizes().end());
+  size.back() = r.top;
+  Tensor w = fresh(size, at::kFloat, dev), e = fresh(size, at::kInt, dev), s = fresh({E}, at::kInt, dev), p = fresh(size, at::kInt, dev),
+         o = fresh({T * r.top}, at::kInt, dev), ws;
+  const size_t need = b200q_route_workspace_bytes(T, E, r.top);
+  if (need) ws = fresh({(int64_t)need}, at::kByte, dev);
+  auto at = [](const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
+  if (b200q_route(l.data_ptr(), dt, T, E, r.top, r.scoring, r.bias ? static_cast<const float*>(r.bias->data_ptr()) : nullptr, r.groups, r.top_groups, r.best,
+                  r.renormalize, r.scale, static_cast<float*>(w.data_ptr()), at(e), at(s), at(p), at(o), need ? ws.data_ptr() : nullptr, need,
+                  stream_of(dev)) != B200Q_OK)
+    return false;
+  *out = {w, e, s, p, o};
+  return true;
+}
+PyObject* py_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor* l;
+  Route r;
+  variable_list out;
+  if (!route_args(a, n, &l, &r) || !route_run(*l, r, &out)) return none();
+  return pack(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+struct RouteFn : public torch::autograd::Function<RouteFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Route* r, variable_list* out) {
+    ctx->save_for_backward({logits, (*out)[1]});
+    ctx->saved_data["scoring"] = (int64_t)r->scoring;
+    ctx->saved_data["renormalize"] = r->renormalize;
+    ctx->saved_data["scale"] = (double)r->scale;
+    ctx->mark_non_differentiable({(*out)[1], (*out)[2], (*out)[3], (*out)[4]});
+    return *out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &l = saved[0], &e = saved[1];
+    Tensor dl;
+    if (!grads[0].defined()) return {dl, Tensor(), Tensor()};
+    const int scoring = (int)ctx->saved_data["scoring"].toInt();
+    const bool renormalize = ctx->saved_data["renormalize"].toBool();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const at::Device dev = l.device();
+    {
+      at::AutoDispatchBelowAutograd below;
+      const Tensor dw = grads[0].contiguous();
+      if (current(dev) && l.is_contiguous() && e.is_contiguous() && e.device() == dev && plain(dw, at::kFloat, dev)) {
+        dl = fresh(l.sizes(), l.scalar_type(), dev);
+        if (b200q_route_dlogits(static_cast<const float*>(dw.data_ptr()), l.data_ptr(), dtype_code(l.scalar_type()), static_cast<const int32_t*>(e.data_ptr()),
+                                lead_of(l), l.size(-1), e.size(-1), scoring, renormalize, (float)scale, dl.data_ptr(), stream_of(dev)) != B200Q_OK)
+          dl = Tensor();
+      }
+      if (!dl.defined()) {
+        pybind11::gil_scoped_acquire gil;
+        dl = unwrapped(python("mlx_b200.ops", "route_dlogits")(wrapped(dw), wrapped(l.detach()), wrapped(e), scoring == B200Q_SOFTMAX ? "softmax" : "sigmoid",
+                                                               renormalize, scale));
+      }
+    }
+    first_order({&dl});
+    return {dl, Tensor(), Tensor()};
+  }
+};
+PyObject* py_route_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor* l;
+  Route r;
+  variable_list out;
+  if (!route_args(a, n, &l, &r) || tangent(*l) || (r.bias && tangent(*r.bias)) || !route_run(*l, r, &out)) return none();
+  if (l->requires_grad() && at::GradMode::is_enabled()) out = RouteFn::apply(*l, &r, &out);
+  return pack(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// The tables of a routing (weights, experts, sizes, places, order) that fit T = the tokens of `places`.
+bool plan_ok(const Tensor* places, const Tensor* order, at::Device dev) {
+  return places && order && plain(*places, at::kInt, dev) && plain(*order, at::kInt, dev) && places->dim() >= 1 && order->dim() == 1 &&
+         order->size(0) == places->numel() && places->numel() > 0;
+}
+const int32_t* ints(const Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
+bool dispatch_run(const Tensor& x, const Tensor* places, const Tensor* order, Tensor* xs) {
+  const int dt = dtype_code(x.scalar_type());
+  const at::Device dev = x.device();
+  if (dt < 0 || !current(dev) || !x.is_contiguous() || x.numel() == 0 || !plan_ok(places, order, dev) || x.dim() != places->dim()) return false;
+  for (int64_t i = 0; i < x.dim() - 1; ++i)
+    if (x.size(i) != places->size(i)) return false;
+  *xs = fresh({order->size(0), x.size(-1)}, x.scalar_type(), dev);
+  return b200q_dispatch_rows(x.data_ptr(), dt, lead_of(x), places->size(-1), x.size(-1), ints(*places), ints(*order), xs->data_ptr(), stream_of(dev)) == B200Q_OK;
+}
+bool rows_ok(const Tensor& y, const Tensor* places, const Tensor* order, const Tensor* weights, at::Device dev) {
+  return dtype_code(y.scalar_type()) >= 0 && current(dev) && y.is_contiguous() && y.dim() == 2 && y.numel() > 0 && plan_ok(places, order, dev) &&
+         y.size(0) == order->size(0) && (!weights || (plain(*weights, at::kFloat, dev) && weights->sizes() == places->sizes()));
+}
+bool combine_run(const Tensor& y, const Tensor* places, const Tensor* order, const Tensor* weights, Tensor* out) {
+  const at::Device dev = y.device();
+  if (!rows_ok(y, places, order, weights, dev)) return false;
+  c10::SmallVector<int64_t, 6> size(places->sizes().begin(), places->sizes().end());
+  size.back() = y.size(1);
+  *out = fresh(size, y.scalar_type(), dev);
+  return b200q_combine_rows(y.data_ptr(), dtype_code(y.scalar_type()), lead_of(*places), places->size(-1), y.size(1), ints(*places),
+                            weights ? static_cast<const float*>(weights->data_ptr()) : nullptr, out->data_ptr(), stream_of(dev)) == B200Q_OK;
+}
+pybind11::object routing_of(const Tensor* weights, const Tensor& places, const Tensor& order) {
+  const pybind11::object no = pybind11::none();
+  return python("mlx_b200.ops", "Routing")(weights ? wrapped(*weights) : no, no, no, wrapped(places), wrapped(order));
+}
+
+PyObject* py_dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {   // (x, routing)
+  HANDLE_TH_ERRORS
+  const Tensor *x, *r[5];
+  Tensor xs;
+  if (n != 2 || !(x = tensor(a[0])) || !members(a[1], r) || !dispatch_run(*x, r[3], r[4], &xs)) return none();
+  return THPVariable_Wrap(std::move(xs));
+  END_HANDLE_TH_ERRORS
+}
+struct DispatchFn : public torch::autograd::Function<DispatchFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor* places, const Tensor* order, Tensor* xs) {
+    ctx->save_for_backward({*places, *order});
+    return *xs;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    Tensor dx;
+    if (grads[0].defined()) {
+      {
+        at::AutoDispatchBelowAutograd below;
+        const Tensor g = grads[0].contiguous();
+        if (!combine_run(g, &saved[0], &saved[1], nullptr, &dx)) {
+          pybind11::gil_scoped_acquire gil;
+          dx = unwrapped(python("mlx_b200.ops", "combine_rows")(wrapped(g), routing_of(nullptr, saved[0], saved[1]), false));
+        }
+      }
+      first_order({&dx});
+    }
+    return {dx, Tensor(), Tensor(), Tensor()};
+  }
+};
+PyObject* py_dispatch_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {   // (x, routing)
+  HANDLE_TH_ERRORS
+  const Tensor *x, *r[5];
+  Tensor xs;
+  if (n != 2 || !(x = tensor(a[0])) || !members(a[1], r) || tangent(*x) || !dispatch_run(*x, r[3], r[4], &xs)) return none();
+  if (x->requires_grad() && at::GradMode::is_enabled()) xs = DispatchFn::apply(*x, r[3], r[4], &xs);
+  return THPVariable_Wrap(std::move(xs));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_combine(PyObject*, PyObject* const* a, Py_ssize_t n) {   // (y, routing, weighted)
+  HANDLE_TH_ERRORS
+  const Tensor *y, *r[5];
+  Tensor out;
+  bool weighted;
+  if (n != 3 || !(y = tensor(a[0])) || !members(a[1], r) || !boolean(a[2], &weighted) || (weighted && !r[0]) ||
+      !combine_run(*y, r[3], r[4], weighted ? r[0] : nullptr, &out))
+    return none();
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+struct CombineFn : public torch::autograd::Function<CombineFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& weights, const Tensor* places, const Tensor* order, Tensor* out) {
+    ctx->save_for_backward({y, weights, *places, *order});
+    return *out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &y = saved[0], &w = saved[1], &places = saved[2], &order = saved[3];
+    Tensor dys, dw;
+    const bool for_y = ctx->needs_input_grad(0), for_w = ctx->needs_input_grad(1);
+    if (grads[0].defined()) {
+      {
+        at::AutoDispatchBelowAutograd below;
+        const Tensor dy = grads[0].contiguous();
+        const at::Device dev = y.device();
+        bool done = rows_ok(y, &places, &order, &w, dev) && plain(dy, y.scalar_type(), dev);
+        if (done) {
+          if (for_y) dys = fresh(y.sizes(), y.scalar_type(), dev);
+          if (for_w) dw = fresh(w.sizes(), at::kFloat, dev);
+          done = b200q_combine_rows_grad(dy.data_ptr(), y.data_ptr(), dtype_code(y.scalar_type()), lead_of(places), places.size(-1), y.size(1), ints(places),
+                                         ints(order), static_cast<const float*>(w.data_ptr()), for_y ? dys.data_ptr() : nullptr,
+                                         for_w ? static_cast<float*>(dw.data_ptr()) : nullptr, stream_of(dev)) == B200Q_OK;
+        }
+        if (!done) {
+          pybind11::gil_scoped_acquire gil;
+          const Tensor wd = w.detach();
+          const pybind11::tuple r = python("mlx_b200.ops", "combine_rows_grad")(wrapped(dy), wrapped(y.detach()), routing_of(&wd, places, order), for_y, for_w);
+          dys = unwrapped(r[0]);
+          dw = unwrapped(r[1]);
+        }
+      }
+      first_order({&dys, &dw});
+    }
+    return {dys, dw, Tensor(), Tensor(), Tensor()};
+  }
+};
+PyObject* py_combine_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {   // (y, routing)
+  HANDLE_TH_ERRORS
+  const Tensor *y, *r[5];
+  Tensor out;
+  if (n != 2 || !(y = tensor(a[0])) || !members(a[1], r) || !r[0] || tangent(*y) || tangent(*r[0]) || !combine_run(*y, r[3], r[4], r[0], &out)) return none();
+  if ((y->requires_grad() || r[0]->requires_grad()) && at::GradMode::is_enabled()) out = CombineFn::apply(*y, *r[0], r[3], r[4], &out);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_group_rows(PyObject*, PyObject* const* a, Py_ssize_t nargs) {   // (ids, n)
+  HANDLE_TH_ERRORS
+  const Tensor* ids;
+  int n;
+  if (nargs != 2 || !(ids = tensor(a[0])) || !PyLong_CheckExact(a[1]) || !integer(a[1], 0, &n) || n < 0) return none();
+  const at::Device dev = ids->device();
+  const at::ScalarType t = ids->scalar_type();
+  if ((t != at::kInt && t != at::kLong) || !current(dev) || !ids->is_contiguous() || ids->numel() == 0) return none();
+  const int64_t T = ids->numel();
+  const size_t need = b200q_group_rows_workspace_bytes(T, n);
+  Tensor sizes = fresh({n}, at::kInt, dev), starts = fresh({n + 1}, at::kInt, dev), order = fresh({T}, at::kInt, dev),
+         tiles = fresh({b200q_group_rows_tiles(T, n), 4}, at::kInt, dev), ws = fresh({(int64_t)need}, at::kByte, dev);
+  auto at = [](const Tensor& v) { return static_cast<int32_t*>(v.data_ptr()); };
+  if (b200q_group_rows(ids->data_ptr(), t == at::kLong ? 8 : 4, T, n, at(sizes), at(starts), at(order), at(tiles), ws.data_ptr(), need, stream_of(dev)) != B200Q_OK)
+    return none();
+  return pack({sizes, starts, order, tiles});
+  END_HANDLE_TH_ERRORS
+}
+
+struct Adapters {
+  const Tensor *y, *x, *a, *b, *g[4], *scales;   // g: sizes, starts, order, tiles
+  int64_t T, L, N, K, r;
+};
+bool adapters_ok(Adapters* p, const Tensor& y) {   // y: what is added to, or the result's gradient
+  const at::ScalarType t = p->x->scalar_type();
+  const at::Device dev = p->x->device();
+  if ((t != at::kHalf && t != at::kBFloat16) || !current(dev)) return false;
+  for (const Tensor* v : {&y, p->x, p->a, p->b})
+    if (!plain(*v, t, dev) || v->numel() == 0) return false;
+  if (p->a->dim() != 3 || p->b->dim() != 3 || p->x->dim() < 1 || y.dim() != p->x->dim()) return false;
+  for (int64_t i = 0; i < y.dim() - 1; ++i)
+    if (y.size(i) != p->x->size(i)) return false;
+  p->T = lead_of(y); p->L = p->a->size(0); p->r = p->a->size(1); p->K = p->a->size(2); p->N = p->b->size(1);
+  if (p->b->size(0) != p->L || p->b->size(2) != p->r || p->x->size(-1) != p->K || y.size(-1) != p->N) return false;
+  for (const Tensor* v : p->g)
+    if (!v || !plain(*v, at::kInt, dev)) return false;
+  if (p->g[0]->dim() != 1 || p->g[0]->size(0) != p->L || p->g[1]->dim() != 1 || p->g[1]->size(0) != p->L + 1 || p->g[2]->dim() != 1 || p->g[2]->size(0) != p->T ||
+      p->g[3]->dim() != 2 || p->g[3]->size(0) != b200q_group_rows_tiles(p->T, p->L) || p->g[3]->size(1) != 4)
+    return false;
+  return !p->scales || (plain(*p->scales, at::kFloat, dev) && p->scales->dim() == 1 && p->scales->size(0) == p->L);
+}
+const float* floats(const Tensor* t) { return t ? static_cast<const float*>(t->data_ptr()) : nullptr; }
+bool adapters_run(Adapters* p, Tensor* out, Tensor* h) {
+  if (!adapters_ok(p, *p->y)) return false;
+  const at::Device dev = p->x->device();
+  if (!out->defined()) *out = fresh(p->y->sizes(), p->y->scalar_type(), dev);
+  *h = fresh({p->T, p->r}, at::kFloat, dev);
+  return b200q_add_adapters(p->y->data_ptr(), p->x->data_ptr(), p->a->data_ptr(), p->b->data_ptr(), dtype_code(p->x->scalar_type()), p->T, p->L, p->N, p->K, p->r,
+                            ints(*p->g[2]), ints(*p->g[3]), floats(p->scales), static_cast<float*>(h->data_ptr()), out->data_ptr(), stream_of(dev)) == B200Q_OK;
+}
+bool overlap(const Tensor& a, const Tensor& b) {
+  const char *p = static_cast<const char*>(a.data_ptr()), *q = static_cast<const char*>(b.data_ptr());
+  return p < q + b.nbytes() && q < p + a.nbytes();
+}
+bool adapters_args(PyObject* const* a, Adapters* p) {   // (y, x, a, b, groups, scales)
+  return (p->y = tensor(a[0])) && (p->x = tensor(a[1])) && (p->a = tensor(a[2])) && (p->b = tensor(a[3])) && members(a[4], p->g) && index_arg(a[5], &p->scales);
+}
+PyObject* py_add_adapters(PyObject*, PyObject* const* a, Py_ssize_t n) {   // (..., out): out is None or y itself
+  HANDLE_TH_ERRORS
+  Adapters p;
+  Tensor out, h;
+  if (n != 7 || !adapters_args(a, &p) || (a[6] != Py_None && a[6] != a[0])) return none();
+  if (a[6] != Py_None) {
+    out = *p.y;
+    for (const Tensor* v : {p.x, p.a, p.b})
+      if (overlap(out, *v)) return none();
+  }
+  if (!adapters_run(&p, &out, &h)) return none();
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) return nullptr;
+  if (a[6] != Py_None) { Py_INCREF(a[6]); PyTuple_SET_ITEM(pair, 0, a[6]); }
+  else PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(h)));
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+struct AdaptersFn : public torch::autograd::Function<AdaptersFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& x, const Tensor& a, const Tensor& b, const Adapters* p, const Tensor* h, Tensor* out) {
+    variable_list saved{x, a, b, *h, *p->g[0], *p->g[1], *p->g[2], *p->g[3]};
+    if (p->scales) saved.push_back(*p->scales);
+    ctx->save_for_backward(std::move(saved));
+    return *out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    Tensor d_y, dx, da, db;
+    if (grads[0].defined()) {
+      const bool for_y = ctx->needs_input_grad(0), for_x = ctx->needs_input_grad(1), for_a = ctx->needs_input_grad(2), for_b = ctx->needs_input_grad(3);
+      if (for_x || for_a || for_b) {
+        {
+          at::AutoDispatchBelowAutograd below;
+          const Tensor dy = grads[0].contiguous();
+          Adapters p{nullptr, &saved[0], &saved[1], &saved[2], {&saved[4], &saved[5], &saved[6], &saved[7]}, saved.size() > 8 ? &saved[8] : nullptr};
+          const Tensor& h = saved[3];
+          const at::Device dev = saved[0].device();
+          bool done = adapters_ok(&p, dy) && plain(h, at::kFloat, dev);
+          if (done) {
+            Tensor g;
+            if (for_x) dx = fresh(p.x->sizes(), p.x->scalar_type(), dev);
+            if (for_a) da = fresh(p.a->sizes(), p.x->scalar_type(), dev);
+            if (for_b) db = fresh(p.b->sizes(), p.x->scalar_type(), dev);
+            if (for_x || for_a) g = fresh({p.T, p.r}, at::kFloat, dev);
+            auto at = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+            done = b200q_add_adapters_grad(dy.data_ptr(), p.x->data_ptr(), p.a->data_ptr(), p.b->data_ptr(), dtype_code(p.x->scalar_type()), p.T, p.L, p.N, p.K, p.r,
+                                           ints(*p.g[2]), ints(*p.g[1]), ints(*p.g[3]), floats(p.scales), floats(&h), static_cast<float*>(at(g)), at(dx), at(da),
+                                           at(db), stream_of(dev)) == B200Q_OK;
+          }
+          if (!done) {
+            pybind11::gil_scoped_acquire gil;
+            const pybind11::object groups = python("mlx_b200.ops", "RowGroups")(wrapped(saved[4]), wrapped(saved[5]), wrapped(saved[6]), wrapped(saved[7]));
+            const pybind11::object scales = p.scales ? wrapped(*p.scales) : pybind11::object(pybind11::none());
+            const pybind11::tuple r = python("mlx_b200.ops", "add_adapters_grad")(wrapped(dy), wrapped(saved[0].detach()), wrapped(saved[1].detach()),
+                                                                                 wrapped(saved[2].detach()), groups, wrapped(h), scales, for_x, for_a, for_b);
+            dx = unwrapped(r[0]);
+            da = unwrapped(r[1]);
+            db = unwrapped(r[2]);
+          }
+        }
+        first_order({&dx, &da, &db});
+      }
+      if (for_y) d_y = grads[0];
+    }
+    return {d_y, dx, da, db, Tensor(), Tensor(), Tensor()};
+  }
+};
+PyObject* py_add_adapters_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {   // (y, x, a, b, groups, scales)
+  HANDLE_TH_ERRORS
+  Adapters p;
+  Tensor out, h;
+  if (n != 6 || !adapters_args(a, &p)) return none();
+  bool graph = false;
+  for (const Tensor* v : {p.y, p.x, p.a, p.b}) {
+    if (tangent(*v)) return none();
+    graph = graph || v->requires_grad();
+  }
+  if (p.scales && tangent(*p.scales)) return none();
+  if (!adapters_run(&p, &out, &h)) return none();
+  if (graph && at::GradMode::is_enabled()) out = AdaptersFn::apply(*p.y, *p.x, *p.a, *p.b, &p, &h, &out);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // (device index, stream, operator, address, bytes): ops._workspaces has a new buffer
 PyObject* py_scratch(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 5) { PyErr_SetString(PyExc_TypeError, "scratch takes five arguments"); return nullptr; }
@@ -633,6 +1040,15 @@ PyMethodDef methods[] = {
     {"grouped_mm", (PyCFunction)(void (*)(void))py_grouped_mm, METH_FASTCALL, nullptr},
     {"grouped_mm_dw", (PyCFunction)(void (*)(void))py_grouped_mm_dw, METH_FASTCALL, nullptr},
     {"grouped_mm_grad", (PyCFunction)(void (*)(void))py_grouped_mm_grad, METH_FASTCALL, nullptr},
+    {"route", (PyCFunction)(void (*)(void))py_route, METH_FASTCALL, nullptr},
+    {"route_grad", (PyCFunction)(void (*)(void))py_route_grad, METH_FASTCALL, nullptr},
+    {"dispatch", (PyCFunction)(void (*)(void))py_dispatch, METH_FASTCALL, nullptr},
+    {"dispatch_grad", (PyCFunction)(void (*)(void))py_dispatch_grad, METH_FASTCALL, nullptr},
+    {"combine", (PyCFunction)(void (*)(void))py_combine, METH_FASTCALL, nullptr},
+    {"combine_grad", (PyCFunction)(void (*)(void))py_combine_grad, METH_FASTCALL, nullptr},
+    {"group_rows", (PyCFunction)(void (*)(void))py_group_rows, METH_FASTCALL, nullptr},
+    {"add_adapters", (PyCFunction)(void (*)(void))py_add_adapters, METH_FASTCALL, nullptr},
+    {"add_adapters_grad", (PyCFunction)(void (*)(void))py_add_adapters_grad, METH_FASTCALL, nullptr},
     {"scratch", (PyCFunction)(void (*)(void))py_scratch, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_front", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

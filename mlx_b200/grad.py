@@ -179,6 +179,21 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, sizes: torch.Tensor, transpose:
     return _GroupedMmFn.apply(x, w, sizes, bool(transpose))
 
 
+class _FirstOrder(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, _, g):
+        return g.detach()
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("the gradients of route_experts, dispatch_rows, combine_rows and add_adapters have none themselves")
+
+
+def _first_order(g: torch.Tensor) -> torch.Tensor:
+    """A gradient that is final, in a graph that was asked for: its own backward pass is refused."""
+    return _FirstOrder.apply(torch.empty(0, requires_grad=True), g)
+
+
 class _RouteFn(torch.autograd.Function):
     """The weights' gradient; the choice of the experts is constant."""
 
@@ -200,6 +215,9 @@ class _RouteFn(torch.autograd.Function):
 def route_experts(logits: torch.Tensor, top: int, scoring: str = "softmax", bias: Optional[torch.Tensor] = None, groups: int = 1,
                   top_groups: Optional[int] = None, group_best: int = 1, renormalize: bool = False, scale: float = 1.0) -> ops.Routing:
     """ops.route_experts whose weights have a gradient with respect to the logits (of first order).  The bias gets none."""
+    r = ops._front.route_grad(logits, top, scoring, bias, groups, top_groups, group_best, renormalize, scale)
+    if r is not None:
+        return ops.Routing(*r)
     return ops.Routing(*_RouteFn.apply(logits, top, scoring, None if bias is None else bias.detach(), groups, top_groups, group_best, renormalize, scale))
 
 
@@ -217,7 +235,8 @@ class _DispatchFn(torch.autograd.Function):
 
 def dispatch_rows(x: torch.Tensor, routing: ops.Routing) -> torch.Tensor:
     """ops.dispatch_rows with a gradient for x (of first order)."""
-    return _DispatchFn.apply(x, routing.places, routing.order)
+    xs = ops._front.dispatch_grad(x, routing)
+    return xs if xs is not None else _DispatchFn.apply(x, routing.places, routing.order)
 
 
 class _CombineFn(torch.autograd.Function):
@@ -236,7 +255,8 @@ class _CombineFn(torch.autograd.Function):
 
 def combine_rows(y: torch.Tensor, routing: ops.Routing) -> torch.Tensor:
     """ops.combine_rows with gradients for y and routing.weights (of first order)."""
-    return _CombineFn.apply(y, routing.weights, routing.places, routing.order)
+    out = ops._front.combine_grad(y, routing)
+    return out if out is not None else _CombineFn.apply(y, routing.weights, routing.places, routing.order)
 
 
 class _AdaptersFn(torch.autograd.Function):
@@ -258,4 +278,5 @@ class _AdaptersFn(torch.autograd.Function):
 def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, groups: ops.RowGroups,
                  scales: Optional[torch.Tensor] = None) -> torch.Tensor:
     """ops.add_adapters with gradients for y, x, a and b (of first order); the scales are constants."""
-    return _AdaptersFn.apply(y, x, a, b, None if scales is None else scales.detach(), *groups)
+    out = ops._front.add_adapters_grad(y, x, a, b, groups, scales)
+    return out if out is not None else _AdaptersFn.apply(y, x, a, b, None if scales is None else scales.detach(), *groups)

@@ -876,6 +876,9 @@ def route_experts(logits: torch.Tensor, top: int, scoring: str = "softmax", bias
     group_best (1 or 2) best.  Weights are the scores, renormalized to a sum of 1 over the experts taken if asked for, times scale.
     An expert with a logit (or bias) of -inf is off and never taken: a token with too few experts on has pairs without one (expert
     -1, weight 0, place -1), a token of padding none at all.  grad.route_experts is the same with the weights' gradient."""
+    r = _front.route(logits, top, scoring, bias, groups, top_groups, group_best, renormalize, scale)
+    if r is not None:
+        return Routing(*r)
     tag = "route_experts"
     E, top, groups, top_groups = _route_args(tag, logits, top, scoring, groups, top_groups, group_best)
     if bias is not None and (not bias.dtype.is_floating_point or tuple(bias.shape) != (E,)):
@@ -927,6 +930,9 @@ def _plan(tag, places, order):
 def dispatch_rows(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     """The tokens' rows x [..., D] in the experts' order, [tokens * top, D]: the rows that grouped_mm and grouped_qqmm take with routing.sizes.
     Rows behind the last pair with an expert are zeros."""
+    xs = _front.dispatch(x, routing)
+    if xs is not None:
+        return xs
     tag = "dispatch_rows"
     if x.dtype not in _DT:
         raise ValueError(f"[{tag}] Only real floating types are supported but x.dtype() == {x.dtype}.")
@@ -958,6 +964,9 @@ def _combine(tag, y, places, order, weights):
 def combine_rows(y: torch.Tensor, routing: Routing, weighted: bool = True) -> torch.Tensor:
     """The experts' results y [tokens * top, D], in their order, back to the tokens: out[t] = sum of weights[t, j] y[places[t, j]], [..., D];
     weighted=False: the plain sum, which is the gradient of dispatch_rows.  Sums in float32, in the order of the choices."""
+    out = _front.combine(y, routing, weighted)
+    if out is not None:
+        return out
     dev, y, places, _, weights = _combine("combine_rows", y, routing.places, routing.order, routing.weights if weighted else None)
     with torch.cuda.device(dev):
         out = torch.empty(tuple(places.shape[:-1]) + (y.shape[1],), dtype=y.dtype, device=dev)
@@ -987,6 +996,9 @@ def combine_rows_grad(dy: torch.Tensor, y: torch.Tensor, routing: Routing, for_y
 def group_rows(ids: torch.Tensor, n: int) -> RowGroups:
     """Rows sorted by group: ids, any integers, name every row's group (adapter); outside [0, n): none.  Computed once for a batch
     and used beside all its projections."""
+    g = _front.group_rows(ids, n)
+    if g is not None:
+        return RowGroups(*g)
     tag = "group_rows"
     if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
         raise ValueError(f"[{tag}] ids must be integral but are {ids.dtype}.")
@@ -1043,6 +1055,9 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
 
 def _add_adapters(y, x, a, b, groups, scales=None, out=None):
     """-> add_adapters' result and the inner products, float32 [rows, rank] in the order of the groups."""
+    r = _front.add_adapters(y, x, a, b, groups, scales, out)
+    if r is not None:
+        return r
     tag = "add_adapters"
     dev, T, L, N, K, rank, groups, scales = _adapter_args(tag, y, x, a, b, groups, scales)
     if out is not None:
