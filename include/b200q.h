@@ -471,19 +471,21 @@ int b200q_group_rows(const void* ids, int id_bytes, int64_t T, int64_t n, int32_
 
 /*
  * Low-rank adapters beside a shared projection: out[t] = y[t] + scales[l] b[l] (a[l] x[t]), l being row t's adapter; a row without one:
- * y[t].  bf16 and f16; sums and the inner product in fp32, rounded once.
+ * y[t].  bf16 and f16; sums in fp32, the inner product to 2^-17, the result rounded once.
  *   y, out [T, N] (out may be y), x [T, K], a [L, r, K], b [L, N, r] dtype; scales [L] float32 (NULL: 1)
  *   order, starts, tiles: b200q_group_rows over L groups
- *   h [T, r] float32: left with a[l] x in the order of the places, which the gradient takes (else scratch); the rows without adapter are not written
- * b200q_add_adapters_grad: from dy [T, N] the gradients dx [T, K], da, db, each NULL where not wanted (that of y is dy); g [T, r]
- * float32 is scratch, needed for dx and da.  h is needed for db, x for da, a for dx, b for dx and da.
+ *   h: b200q_add_adapters_inner_bytes(T, r) bytes on a 16-byte boundary, left with a[l] x, by place, as two bf16 numbers per value,
+ *   which the gradient takes (else scratch); rows without an adapter have none
+ * b200q_add_adapters_grad: from dy [T, N] the gradients dx [T, K], da, db, each NULL where not wanted (that of y is dy); g, as
+ * large as h, is scratch, needed for dx and da.  h is needed for db, x for da, a for dx, b for dx and da.
  * At most 4096 adapters, ranks of 4096 and widths of 2^24.
  */
+size_t b200q_add_adapters_inner_bytes(int64_t T, int64_t r);
 int b200q_add_adapters(const void* y, const void* x, const void* a, const void* b, int dtype, int64_t T, int64_t L, int64_t N, int64_t K,
-                       int64_t r, const int32_t* order, const int32_t* tiles, const float* scales, float* h, void* out, void* stream);
+                       int64_t r, const int32_t* order, const int32_t* tiles, const float* scales, void* h, void* out, void* stream);
 int b200q_add_adapters_grad(const void* dy, const void* x, const void* a, const void* b, int dtype, int64_t T, int64_t L, int64_t N,
                             int64_t K, int64_t r, const int32_t* order, const int32_t* starts, const int32_t* tiles, const float* scales,
-                            const float* h, float* g, void* dx, void* da, void* db, void* stream);
+                            const void* h, void* g, void* dx, void* da, void* db, void* stream);
 
 /*
  * Introspection for tests and benchmarks: name of the kernel family b200q_qmm would

@@ -79,6 +79,7 @@ SIGNATURES = {
     "b200q_group_rows_tiles": (_i64, [_i64, _i64]),
     "b200q_group_rows_workspace_bytes": (_sz, [_i64, _i64]),
     "b200q_group_rows": (_i, [_vp, _i, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "b200q_add_adapters_inner_bytes": (_sz, [_i64, _i64]),
     "b200q_add_adapters": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
     "b200q_add_adapters_grad": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _i64] + [_vp] * 10),
     "b200q_qmm_kernel_name": (ctypes.c_char_p, [_i, _i64, _i64, _i64, _i64, _i, _i, _i]),

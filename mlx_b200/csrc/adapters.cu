@@ -6,13 +6,13 @@
 //
 // Rows come sorted by adapter (b200q_group_rows), in tiles of up to 64 rows of one adapter.  A rank of 8 to 64 makes r operations per
 // byte of activations, far below what the tensor cores do per byte of HBM, so the kernels are built for the memory: activations are read
-// once, straight from HBM into the fragments of mma.sync (no shared memory, no transposed copies), 16 bytes per lane.  That works because
-// the k index of a product may be permuted as long as both operands agree, and the columns of its result as long as the stores do:
-// a lane's 8 consecutive values are its fragments of four (or two) steps.  Operands that lie the other way round are transposed 8 x 8 in
-// registers (movmatrix).
+// once, straight into the fragments of mma.sync, 16 bytes per lane, without transposed copies.  That works because the k index of a product
+// may be permuted as long as both operands agree, and the columns of its result as long as the stores do: a lane's 8 consecutive values are
+// its fragments of several steps.  Operands that lie the other way round are transposed 8 x 8 in registers (movmatrix).
 //
-// h and g are kept in fp32.  As operands of the second product they are split into two bf16 numbers, high and low part (2^-17 of the
-// value is lost), and multiplied as such; 16-bit floats of type f16 are split too, exactly, so that no value leaves a type's range.
+// h and g, summed in fp32, are kept as two bf16 numbers each, high and low part (2^-17 of the value is lost, a 32nd of what the
+// result's rounding to f16 loses), since that is how the second products take them; 16-bit floats of type f16 are split too, exactly, so that
+// no value leaves a type's range (the product of two low parts, 2^-17, is left out).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -30,16 +30,16 @@ constexpr int kRows = kAdapterRows, kWarps = 8, kThreads = 32 * kWarps;
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (sizeof(T) == 2 && std::is_same_v<T, __half>)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // An 8 x 8 matrix of 16-bit values, lane (i, q) having (i, 2q) and (i, 2q + 1): afterwards (2q, i) and (2q + 1, i).
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {   // two bf16, the first in the lower half
@@ -112,18 +112,50 @@ __device__ __forceinline__ void load_few(const T* p, int64_t have, int width, ui
   }
 }
 
+__device__ __forceinline__ uint32_t shared(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// BYTES (4, 8, 16) to shared memory, asynchronously; zeros where there is nothing (p is not read then).
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* p, bool there) {
+  const int n = there ? BYTES : 0;
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared(dst)), "l"(p), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(shared(dst)), "l"(p), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_all_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// N consecutive values (4, 8 or 16) in the widest pieces that the rows' alignment allows.  base: an address that may be named.
+template <int N, typename T>
+__device__ __forceinline__ void copy_few(void* dst, const T* p, int64_t have, int width, const void* base) {
+  char* d = static_cast<char*>(dst);
+  const char* q = reinterpret_cast<const char*>(p);
+  if (N >= 8 && width == 16) {
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i) copy_async<16>(d + 512 * i, 8 * i < have ? q + 16 * i : base, 8 * i < have);   // (pieces of 16 bytes are 512 apart)
+  } else if (width >= 8) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) copy_async<8>(d + 512 * (i / 2) + 8 * (i & 1), 4 * i < have ? q + 8 * i : base, 4 * i < have);
+  } else if (width == 4) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) copy_async<4>(d + 512 * (i / 4) + 4 * (i & 3), 2 * i < have ? q + 4 * i : base, 2 * i < have);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      *reinterpret_cast<uint16_t*>(d + 512 * (i / 8) + 2 * (i & 7)) = i < have ? __ldg(reinterpret_cast<const uint16_t*>(p) + i) : (uint16_t)0;
+  }
+}
+
 struct Params {
   const void *x, *w;       // activations; weights of all adapters
-  const float* h;          // up, outer: [T, r]
+  uint16_t* h;             // inner products, by place: [T][high, low][r16] bf16
   const void* y;           // up: what is added to (null: zeros)
-  void* out;               // down: float [T, r]
+  void* out;
   const float* scales;     // null: 1
-  const int *order, *sizes, *starts;
+  const int *order, *starts;
   const int4* tiles;
   int64_t T, C;            // rows; the long dimension (K or N)
   int64_t tiles_n;
-  int L, r, width;         // width: bytes that a row of weights' pieces are aligned to
-  int split;               // blocks per cluster
+  int L, r, r16, width;    // r16: r in whole 16s; width: bytes that the pieces of short rows of weights are aligned to
+  int split, each;         // blocks per cluster; tiles per block
 };
 
 // A tile, or none (rows == 0) where the table does not fit the operands.
@@ -139,12 +171,23 @@ __device__ __forceinline__ int64_t row_at(const Params& p, int64_t place) {
   return row < p.T ? row : -1;
 }
 
-// ---- h[place] = (c) sum over the long dimension of x[row] w.  Blocks by (tile, part of the long dimension, 8 NT ranks); the parts are a cluster.
+// ---- h[place] = (c) sum over the long dimension of x[row] w.  Blocks by (tile, part of the long dimension, 8 NT ranks); the parts are a cluster
+// whose blocks add up their sums through distributed shared memory.  Warps take every 64th (of their cluster) 32 columns of x.
 // TALL: weights [C, r], else [r, C].
+//
+// Bound by the latency of its loads.  They go through a ring in shared memory, several steps ahead; every lane copies and reads its own
+// 16-byte pieces only, so that the ring needs no barrier, just the lane's own count of finished copies.
+template <bool TALL, int NT>
+struct Down {
+  static constexpr int kRanks = 8 * NT, kW = TALL ? (NT == 8 ? 8 : 4) : NT, kPieces = 8 + kW, kStages = NT == 8 ? 3 : 2;
+  static constexpr size_t kBytes = (size_t)kWarps * kStages * kPieces * 512;
+  static_assert(kBytes >= (size_t)kWarps * kRows * kRanks * 4, "the sums lie where the ring was");
+};
 template <typename T, bool TALL, bool WHOLE, int NT>
-__global__ void __launch_bounds__(kThreads) down_kernel(const Params p) {
-  constexpr int kRanks = 8 * NT;
-  extern __shared__ __align__(16) float red[];   // [kWarps][kRows][kRanks]
+__global__ void __launch_bounds__(kThreads, NT == 8 ? 1 : 2) down_kernel(const Params p) {
+  using D = Down<TALL, NT>;
+  constexpr int kRanks = D::kRanks, kStages = D::kStages;
+  extern __shared__ __align__(16) unsigned char smem[];
   cg::cluster_group cluster = cg::this_cluster();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
   const int part = (int)(blockIdx.x % p.split);
@@ -162,68 +205,88 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const Params p) {
       x[m][i] = at < 0 ? nullptr : static_cast<const T*>(p.x) + at * C;
     }
   const T* w = static_cast<const T*>(p.w) + (int64_t)tile.x * p.r * C;
-  float acc[4][NT][4] = {};
-  struct Stage {
-    uint4 x[4][2];
-    uint32_t w[TALL ? 4 : NT][TALL ? NT : 4];
-  };
-  auto load = [&](int64_t k0, Stage& s) {
+  unsigned char* ring = smem + (size_t)warp * kStages * D::kPieces * 512 + lane * 16;
+  auto slot = [&](int stage, int piece) { return ring + (stage * D::kPieces + piece) * 512; };
+  auto load = [&](int64_t k0, int stage) {
     const int64_t k = k0 + q * 8;
 #pragma unroll
     for (int m = 0; m < 4; ++m)
       if (m < subs) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) s.x[m][i] = x[m][i] ? load8<WHOLE>(x[m][i] + k, C - k) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 2; ++i) {
+          unsigned char* d = slot(stage, m * 2 + i);
+          const bool there = x[m][i] && k < C;
+          if constexpr (WHOLE) copy_async<16>(d, there ? x[m][i] + k : p.x, there);
+          else *reinterpret_cast<uint4*>(d) = there ? load8<false>(x[m][i] + k, C - k) : make_uint4(0, 0, 0, 0);
+        }
       }
     if constexpr (TALL) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {   // rows of pair j of every lane's 8
         const int64_t kr = k0 + (g >> 1) * 8 + j * 2 + (g & 1);
         const int rank = r0 + q * 2 * NT;
-        load_few<2 * NT>(w + kr * p.r + rank, kr < C ? p.r - rank : 0, p.width, s.w[j]);
+        copy_few<2 * NT>(slot(stage, 8 + j * (D::kW / 4)), w + kr * p.r + rank, kr < C ? p.r - rank : 0, p.width, p.w);
       }
     } else {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int rank = r0 + (g >> 1) * 2 * NT + t * 2 + (g & 1);
-        const uint4 v = rank < p.r ? load8<WHOLE>(w + (int64_t)rank * C + k, C - k) : make_uint4(0, 0, 0, 0);
-        s.w[t][0] = v.x; s.w[t][1] = v.y; s.w[t][2] = v.z; s.w[t][3] = v.w;
+        unsigned char* d = slot(stage, 8 + t);
+        const bool there = rank < p.r && k < C;
+        if constexpr (WHOLE) copy_async<16>(d, there ? w + (int64_t)rank * C + k : p.w, there);
+        else *reinterpret_cast<uint4*>(d) = there ? load8<false>(w + (int64_t)rank * C + k, C - k) : make_uint4(0, 0, 0, 0);
       }
     }
   };
-  auto multiply = [&](Stage& s) {
-    uint32_t b[NT][4];   // pair j of the lane's 8, of column tile t
+  float acc[4][NT][4] = {};
+  const int64_t step = (int64_t)p.split * kWarps * 32;
+  int64_t k = ((int64_t)part * kWarps + warp) * 32;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+  for (int s = 0; s < kStages - 1; ++s) {
+    if (k + s * step < C) load(k + s * step, s);
+    commit();
+  }
+  for (int stage = 0; k < C; k += step) {
+    const int64_t ahead = k + (kStages - 1) * step;
+    if (ahead < C) load(ahead, stage == 0 ? kStages - 1 : stage - 1);
+    commit();
+    wait_all_but<kStages - 1>();
+    uint32_t b[NT][4];   // pair j of the lane's 8, of column tile t
+    if constexpr (TALL) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if constexpr (TALL) b[t][j] = transposed(s.w[j][t]);
-        else b[t][j] = s.w[t][j];
+#pragma unroll
+        for (int i = 0; i < (NT + 3) / 4; ++i) {
+          const uint4 v = *reinterpret_cast<const uint4*>(slot(stage, 8 + j * (D::kW / 4) + i));
+          b[i * 4][j] = transposed(v.x);
+          b[i * 4 + 1][j] = transposed(v.y);
+          if constexpr (NT > 2) {
+            b[(i * 4 + 2) % NT][j] = transposed(v.z);
+            b[(i * 4 + 3) % NT][j] = transposed(v.w);
+          }
+        }
       }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const uint4 v = *reinterpret_cast<const uint4*>(slot(stage, 8 + t));
+        b[t][0] = v.x; b[t][1] = v.y; b[t][2] = v.z; b[t][3] = v.w;
+      }
+    }
 #pragma unroll
     for (int m = 0; m < 4; ++m)
       if (m < subs) {
-        const uint4 u = s.x[m][0], v = s.x[m][1];
+        const uint4 u = *reinterpret_cast<const uint4*>(slot(stage, m * 2)), v = *reinterpret_cast<const uint4*>(slot(stage, m * 2 + 1));
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          mma<T>(acc[m][t], u.x, v.x, u.y, v.y, b[t][0], b[t][1]);
-          mma<T>(acc[m][t], u.z, v.z, u.w, v.w, b[t][2], b[t][3]);
-        }
+        for (int t = 0; t < NT; ++t) mma<T>(acc[m][t], u.x, v.x, u.y, v.y, b[t][0], b[t][1]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma<T>(acc[m][t], u.z, v.z, u.w, v.w, b[t][2], b[t][3]);
       }
-  };
-  const int64_t step = (int64_t)p.split * kWarps * 32;
-  int64_t k = ((int64_t)part * kWarps + warp) * 32;
-  Stage a, b;
-  if (k < C) load(k, a);
-  while (k < C) {
-    if (k + step < C) load(k + step, b);
-    multiply(a);
-    k += step;
-    if (k >= C) break;
-    if (k + step < C) load(k + step, a);
-    multiply(b);
-    k += step;
+    stage = stage == kStages - 1 ? 0 : stage + 1;
   }
+  wait_all_but<0>();
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(smem);   // [kWarps][kRows][kRanks]
 #pragma unroll
   for (int m = 0; m < 4; ++m)
     if (m < subs) {
@@ -234,124 +297,154 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const Params p) {
           *reinterpret_cast<float2*>(&red[(warp * kRows + m * 16 + i * 8 + g) * kRanks + q * 2 * NT + t * 2]) = make_float2(acc[m][t][2 * i], acc[m][t][2 * i + 1]);
     }
   __syncthreads();
-  const int n = tile.z * kRanks;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    float s = red[i];
+  const int pairs = tile.z * kRanks / 2;
+  float2* red2 = reinterpret_cast<float2*>(red);
+  for (int i = threadIdx.x; i < pairs; i += kThreads) {
+    float2 s = red2[i];
 #pragma unroll
-    for (int v = 1; v < kWarps; ++v) s += red[v * kRows * kRanks + i];
-    red[i] = s;
+    for (int v = 1; v < kWarps; ++v) {
+      const float2 a = red2[v * kRows * kRanks / 2 + i];
+      s.x += a.x;
+      s.y += a.y;
+    }
+    red2[i] = s;
   }
   cluster.sync();
   const float c = p.scales ? p.scales[tile.x] : 1.0f;
-  float* h = static_cast<float*>(p.out);
-  for (int i = threadIdx.x * p.split + part; i < n; i += kThreads * p.split) {
-    float s = 0.0f;
-    for (int v = 0; v < p.split; ++v) s += cluster.map_shared_rank(red, v)[i];
-    const int rank = r0 + i % kRanks;
-    if (rank < p.r) h[(int64_t)(tile.y + i / kRanks) * p.r + rank] = c * s;
+  for (int i = threadIdx.x * p.split + part; i < pairs; i += kThreads * p.split) {
+    float2 s = make_float2(0.0f, 0.0f);
+    for (int v = 0; v < p.split; ++v) {
+      const float2 a = cluster.map_shared_rank(red2, v)[i];
+      s.x += a.x;
+      s.y += a.y;
+    }
+    const int rank = r0 + i % (kRanks / 2) * 2;
+    if (rank < p.r16) {   // (ranks from r on: their weights were zeros)
+      uint32_t hi, lo;
+      split(rank < p.r ? c * s.x : 0.0f, rank + 1 < p.r ? c * s.y : 0.0f, &hi, &lo);
+      uint16_t* h = p.h + (int64_t)(tile.y + i / (kRanks / 2)) * 2 * p.r16 + rank;
+      *reinterpret_cast<uint32_t*>(h) = hi;
+      *reinterpret_cast<uint32_t*>(h + p.r16) = lo;
+    }
   }
   cluster.sync();   // no block leaves while others read its sums
 }
 
-// ---- out[row] = y[row] + (c) sum over ranks of h[place] w.  Blocks by (tile, 256 columns), warps by 32 columns; ranks in chunks of 64.
+// ---- out[row] = y[row] + (c) sum over ranks of h[place] w.  Warps by (tiles, 32 columns), each on its own; ranks in steps of 16, of which KS
+// have their weights in registers (up to 64 ranks: all, over all rows that an adapter has among the warp's tiles).
 // WIDE: weights [r, C], else [C, r].
-constexpr int kChunk = 64, kPitch = kChunk + 16;
-template <typename T, bool WIDE, bool WHOLE>
-__global__ void __launch_bounds__(kThreads) up_kernel(const Params p) {
+template <typename T, bool WIDE, bool WHOLE, int KS>
+__global__ void __launch_bounds__(kThreads, KS == 4 ? 2 : 3) up_kernel(const Params p) {
   constexpr bool kSplitW = std::is_same_v<T, __half>;
-  __shared__ __align__(16) uint16_t hi[kRows * kPitch], lo[kRows * kPitch];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
   const int64_t C = p.C, blocks = (C + 255) / 256;
-  const int4 tile = tile_of(p, blockIdx.x / blocks);
-  if (tile.z == 0) return;
   const int64_t n0 = (blockIdx.x % blocks) * 256 + warp * 32, n = n0 + q * 8;   // the lane's columns are n .. n + 7
   const int64_t have = C - n;
-  const int subs = (tile.z + 15) / 16;
+  if (n0 >= C) return;
   const T* y = static_cast<const T*>(p.y);
   T* out = static_cast<T*>(p.out);
-  const bool plain = tile.x < 0;   // rows without an adapter
-  if (plain && p.y == p.out) return;
-  float acc[4][4][4] = {};
-  if (!plain) {
-    const T* w = static_cast<const T*>(p.w) + (int64_t)tile.x * p.r * C;
-    const float c = p.scales ? p.scales[tile.x] : 1.0f;
-    for (int r0 = 0; r0 < p.r; r0 += kChunk) {
-      const int ranks = min(kChunk, p.r - r0), steps = (ranks + 15) / 16;
-      if (r0) __syncthreads();
-      for (int i = threadIdx.x; i < kRows * (kChunk / 2); i += kThreads) {
-        const int row = i / (kChunk / 2), k = i % (kChunk / 2) * 2;
-        float a = 0.0f, b = 0.0f;
-        if (row < tile.z) {
-          const float* h = p.h + (int64_t)(tile.y + row) * p.r + r0 + k;
-          if (k < ranks) a = c * h[0];
-          if (k + 1 < ranks) b = c * h[1];
+  const int64_t first = blockIdx.x / blocks * p.each, last = min(first + p.each, p.tiles_n);
+  uint32_t bh[KS][4][2], bl[kSplitW ? KS : 1][4][2];   // rank step, column tile, pair of the lane's 4 ranks
+  const T* w = nullptr;
+  auto weights = [&](int r0) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      uint32_t b[4][2];
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int rank = r0 + s * 16 + (g >> 1) * 4 + j * 2 + (g & 1);
+          const uint4 v = rank < p.r ? load8<WHOLE>(w + (int64_t)rank * C + n, have) : make_uint4(0, 0, 0, 0);
+          b[0][j] = v.x; b[1][j] = v.y; b[2][j] = v.z; b[3][j] = v.w;
         }
-        split(a, b, reinterpret_cast<uint32_t*>(&hi[row * kPitch + k]), reinterpret_cast<uint32_t*>(&lo[row * kPitch + k]));
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int64_t col = n0 + (g >> 1) * 8 + t * 2 + (g & 1);
+          const int rank = r0 + s * 16 + q * 4;
+          load_few<4>(w + col * p.r + rank, col < C ? p.r - rank : 0, p.width, b[t]);
+        }
       }
-      __syncthreads();
 #pragma unroll
-      for (int s = 0; s < kChunk / 16; ++s) {
-        if (s >= steps) break;
-        uint32_t b[4][2];   // column tile, pair of the lane's 4 ranks
-        if constexpr (WIDE) {
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int rank = r0 + s * 16 + (g >> 1) * 4 + j * 2 + (g & 1);
-            const uint4 v = rank < p.r ? load8<WHOLE>(w + (int64_t)rank * C + n, have) : make_uint4(0, 0, 0, 0);
-            b[0][j] = transposed(v.x); b[1][j] = transposed(v.y); b[2][j] = transposed(v.z); b[3][j] = transposed(v.w);
+        for (int j = 0; j < 2; ++j) {
+          uint32_t lo;
+          as_bf16<T>(WIDE ? transposed(b[t][j]) : b[t][j], &bh[s][t][j], &lo);
+          if constexpr (kSplitW) bl[s][t][j] = lo;
+        }
+    }
+  };
+  int loaded = -1;
+  for (int64_t k = first; k < last; ++k) {
+    const int4 tile = tile_of(p, k);
+    if (tile.z == 0) continue;
+    const bool plain = tile.x < 0;   // rows without an adapter
+    if (plain && p.y == p.out) continue;
+    float c = 0.0f;
+    if (!plain) {
+      c = p.scales ? p.scales[tile.x] : 1.0f;
+      w = static_cast<const T*>(p.w) + (int64_t)tile.x * p.r * C;
+      if (p.r16 <= 16 * KS && loaded != tile.x) {
+        weights(0);
+        loaded = tile.x;
+      }
+    }
+    for (int m0 = 0; m0 < tile.z; m0 += 16) {
+      int64_t at[2];
+      uint4 v[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = m0 + i * 8 + g;
+        at[i] = row < tile.z ? row_at(p, tile.y + row) : -1;
+        v[i] = y && at[i] >= 0 ? load8<WHOLE, false>(y + at[i] * C + n, have) : make_uint4(0, 0, 0, 0);
+      }
+      float acc[4][4] = {};
+      if (!plain) {
+        for (int r0 = 0; r0 < p.r16; r0 += 16 * KS) {
+          if (p.r16 > 16 * KS) weights(r0);
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            const int rank = r0 + s * 16;
+            if (KS > 1 && rank >= p.r16) break;
+            uint2 h[2][2];   // row, part
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint16_t* src = p.h + (int64_t)(tile.y + m0 + i * 8 + g) * 2 * p.r16 + rank + q * 4;
+              const bool there = m0 + i * 8 + g < tile.z;
+              h[i][0] = there ? *reinterpret_cast<const uint2*>(src) : make_uint2(0, 0);
+              h[i][1] = there ? *reinterpret_cast<const uint2*>(src + p.r16) : make_uint2(0, 0);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], h[0][0].x, h[1][0].x, h[0][0].y, h[1][0].y, bh[s][t][0], bh[s][t][1]);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], h[0][1].x, h[1][1].x, h[0][1].y, h[1][1].y, bh[s][t][0], bh[s][t][1]);
+            if constexpr (kSplitW) {
+#pragma unroll
+              for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], h[0][0].x, h[1][0].x, h[0][0].y, h[1][0].y, bl[s][t][0], bl[s][t][1]);
+            }
           }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (at[i] < 0 || have <= 0) continue;
+        T o[8];
+        *reinterpret_cast<uint4*>(o) = v[i];
+        if (!plain) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = Elem<T>::from_float(fmaf(c, acc[e / 2][2 * i + (e & 1)], Elem<T>::to_float(o[e])));
+        }
+        if constexpr (WHOLE) {
+          *reinterpret_cast<uint4*>(out + at[i] * C + n) = *reinterpret_cast<const uint4*>(o);
         } else {
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const int64_t col = n0 + (g >> 1) * 8 + t * 2 + (g & 1);
-            const int rank = r0 + s * 16 + q * 4;
-            load_few<4>(w + col * p.r + rank, col < C ? p.r - rank : 0, p.width, b[t]);
-          }
-        }
-        uint32_t bh[4][2], bl[4][2];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) as_bf16<T>(b[t][j], &bh[t][j], &bl[t][j]);
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          if (m >= subs) break;
-          const int at = (m * 16 + g) * kPitch + s * 16 + q * 4;
-          const uint2 h0 = *reinterpret_cast<const uint2*>(&hi[at]), h1 = *reinterpret_cast<const uint2*>(&hi[at + 8 * kPitch]);
-          const uint2 l0 = *reinterpret_cast<const uint2*>(&lo[at]), l1 = *reinterpret_cast<const uint2*>(&lo[at + 8 * kPitch]);
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            mma<__nv_bfloat16>(acc[m][t], h0.x, h1.x, h0.y, h1.y, bh[t][0], bh[t][1]);
-            mma<__nv_bfloat16>(acc[m][t], l0.x, l1.x, l0.y, l1.y, bh[t][0], bh[t][1]);
-            if constexpr (kSplitW) mma<__nv_bfloat16>(acc[m][t], h0.x, h1.x, h0.y, h1.y, bl[t][0], bl[t][1]);
-          }
+          for (int e = 0; e < 8; ++e)
+            if (e < have) out[at[i] * C + n + e] = o[e];
         }
       }
     }
   }
-  if (have <= 0) return;
-#pragma unroll
-  for (int m = 0; m < 4; ++m)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = m * 16 + i * 8 + g;
-      const int64_t at = row < tile.z ? row_at(p, tile.y + row) : -1;
-      if (at < 0) continue;
-      const uint4 v = y ? load8<WHOLE, false>(y + at * C + n, have) : make_uint4(0, 0, 0, 0);
-      T o[8];
-      *reinterpret_cast<uint4*>(o) = v;
-      if (!plain) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = Elem<T>::from_float(Elem<T>::to_float(o[k]) + acc[m][k / 2][2 * i + (k & 1)]);
-      }
-      if constexpr (WHOLE) {
-        *reinterpret_cast<uint4*>(out + at * C + n) = *reinterpret_cast<const uint4*>(o);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (k < have) out[at * C + n + k] = o[k];
-      }
-    }
 }
 
 // ---- out_l = (c) sum over l's rows of h[place] x[row]^T.  Blocks by (64 columns, part of the rows; adapter; 16 MT ranks), the parts are a
@@ -369,22 +462,30 @@ __global__ void __launch_bounds__(kThreads) outer_kernel(const Params p) {
   float acc[MT][4][4] = {};
   struct Stage {
     uint4 x[2];
-    float h[MT][8];
+    uint2 h[MT][2][2];   // rank step, place (+ 8), part
   };
-  auto load = [&](int64_t t0, Stage& s) {
+  struct Index {
+    int64_t row[2];
+  };
+  auto index = [&](int64_t t0) {
+    Index v;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) v.row[i] = t0 + i * 8 + g < hi ? row_at(p, t0 + i * 8 + g) : -1;
+    return v;
+  };
+  auto load = [&](int64_t t0, const Index& at, Stage& s) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t at = t0 + i * 8 + g, row = at < hi ? row_at(p, at) : -1;
-      s.x[i] = row >= 0 ? load8<WHOLE>(x + row * C + col, C - col) : make_uint4(0, 0, 0, 0);
+      const int64_t place = t0 + i * 8 + g;
+      s.x[i] = at.row[i] >= 0 ? load8<WHOLE>(x + at.row[i] * C + col, C - col) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const int rank = r0 + m * 16;
+          s.h[m][i][v] = place < hi && rank < p.r16 ? *reinterpret_cast<const uint2*>(p.h + (place * 2 + v) * p.r16 + rank + q * 4) : make_uint2(0, 0);
+        }
     }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {   // places 2q, 2q + 1, the same + 8; ranks g, g + 8
-        const int64_t at = t0 + q * 2 + (i & 1) + (i & 2 ? 8 : 0);
-        const int rank = r0 + m * 16 + g + (i & 4 ? 8 : 0);
-        s.h[m][i] = at < hi && rank < p.r ? p.h[at * p.r + rank] : 0.0f;
-      }
   };
   auto multiply = [&](const Stage& s) {
     uint32_t bh[4][2], bl[4][2];
@@ -397,29 +498,39 @@ __global__ void __launch_bounds__(kThreads) outer_kernel(const Params p) {
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      uint32_t ah[4], al[4];
-      split(s.h[m][0], s.h[m][1], &ah[0], &al[0]);
-      split(s.h[m][4], s.h[m][5], &ah[1], &al[1]);
-      split(s.h[m][2], s.h[m][3], &ah[2], &al[2]);
-      split(s.h[m][6], s.h[m][7], &ah[3], &al[3]);
+      if (MT > 1 && r0 + m * 16 >= p.r16) break;
+      uint32_t a[2][4];   // part; rows of the product: of a lane's 4 ranks the first two are in its upper half
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        mma<__nv_bfloat16>(acc[m][t], ah[0], ah[1], ah[2], ah[3], bh[t][0], bh[t][1]);
-        mma<__nv_bfloat16>(acc[m][t], al[0], al[1], al[2], al[3], bh[t][0], bh[t][1]);
-        if constexpr (std::is_same_v<T, __half>) mma<__nv_bfloat16>(acc[m][t], ah[0], ah[1], ah[2], ah[3], bl[t][0], bl[t][1]);
+      for (int v = 0; v < 2; ++v) {
+        a[v][0] = transposed(s.h[m][0][v].x);
+        a[v][1] = transposed(s.h[m][0][v].y);
+        a[v][2] = transposed(s.h[m][1][v].x);
+        a[v][3] = transposed(s.h[m][1][v].y);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[m][t], a[0][0], a[0][1], a[0][2], a[0][3], bh[t][0], bh[t][1]);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[m][t], a[1][0], a[1][1], a[1][2], a[1][3], bh[t][0], bh[t][1]);
+      if constexpr (std::is_same_v<T, __half>) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[m][t], a[0][0], a[0][1], a[0][2], a[0][3], bl[t][0], bl[t][1]);
       }
     }
   };
   const int64_t step = (int64_t)p.split * 64;
   int64_t t = lo + ((int64_t)part * 4 + slot) * 16;
   Stage a, b;
-  if (t < hi) load(t, a);
+  Index at = index(t);
+  if (t < hi) load(t, at, a);
+  at = index(t + step);
   while (t < hi) {
-    if (t + step < hi) load(t + step, b);
+    if (t + step < hi) load(t + step, at, b);
+    at = index(t + 2 * step);
     multiply(a);
     t += step;
     if (t >= hi) break;
-    if (t + step < hi) load(t + step, a);
+    if (t + step < hi) load(t + step, at, a);
+    at = index(t + 2 * step);
     multiply(b);
     t += step;
   }
@@ -429,7 +540,8 @@ __global__ void __launch_bounds__(kThreads) outer_kernel(const Params p) {
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<float2*>(&red[(slot * kRanks + m * 16 + i * 8 + g) * kLine + (warp & 1) * 32 + q * 8 + t * 2]) = make_float2(acc[m][t][2 * i], acc[m][t][2 * i + 1]);
+        *reinterpret_cast<float2*>(&red[(slot * kRanks + m * 16 + (g >> 1) * 4 + i * 2 + (g & 1)) * kLine + (warp & 1) * 32 + q * 8 + t * 2]) =
+            make_float2(acc[m][t][2 * i], acc[m][t][2 * i + 1]);
   __syncthreads();
   for (int i = threadIdx.x; i < kRanks * kCols; i += kThreads) {
     const int at = i / kCols * kLine + i % kCols;
@@ -488,11 +600,21 @@ int launch(K kern, const Params& p, dim3 grid, size_t smem, bool cluster, cudaSt
 
 template <typename T, bool TALL, bool WHOLE>
 int down(Params p, cudaStream_t st) {
-  const int nt = p.r <= 16 ? 2 : 4, chunks = (p.r + 8 * nt - 1) / (8 * nt);
+  const int nt = p.r <= 16 ? 2 : (p.r <= 32 ? 4 : 8), chunks = (p.r + 8 * nt - 1) / (8 * nt);
   p.split = split_of(p.tiles_n * chunks, p.C / (kWarps * 32));
   const dim3 grid((unsigned)(p.tiles_n * p.split), chunks);
-  const size_t smem = (size_t)kWarps * kRows * 8 * nt * 4;
-  return nt == 2 ? launch(down_kernel<T, TALL, WHOLE, 2>, p, grid, smem, true, st) : launch(down_kernel<T, TALL, WHOLE, 4>, p, grid, smem, true, st);
+  if (nt == 2) return launch(down_kernel<T, TALL, WHOLE, 2>, p, grid, Down<TALL, 2>::kBytes, true, st);
+  if (nt == 4) return launch(down_kernel<T, TALL, WHOLE, 4>, p, grid, Down<TALL, 4>::kBytes, true, st);
+  return launch(down_kernel<T, TALL, WHOLE, 8>, p, grid, Down<TALL, 8>::kBytes, true, st);
+}
+template <typename T, bool WIDE, bool WHOLE>
+int up(Params p, cudaStream_t st) {
+  const int64_t cols = (p.C + 255) / 256;
+  p.each = (int)std::max<int64_t>(1, std::min<int64_t>(8, p.tiles_n * cols / (148 * 8)));   // a block's tiles share their weights' loads
+  const dim3 grid((unsigned)((p.tiles_n + p.each - 1) / p.each * cols));
+  if (p.r <= 16) return launch(up_kernel<T, WIDE, WHOLE, 1>, p, grid, 0, false, st);
+  if (p.r <= 32) return launch(up_kernel<T, WIDE, WHOLE, 2>, p, grid, 0, false, st);
+  return launch(up_kernel<T, WIDE, WHOLE, 4>, p, grid, 0, false, st);
 }
 template <typename T, bool TALL, bool WHOLE>
 int outer(Params p, cudaStream_t st) {
@@ -510,12 +632,11 @@ int outer(Params p, cudaStream_t st) {
 enum class Step { Down, DownTall, Up, UpWide, Outer, OuterTall };
 template <typename T, bool WHOLE>
 int run(Step step, const Params& p, cudaStream_t st) {
-  const dim3 grid((unsigned)(p.tiles_n * ((p.C + 255) / 256)));
   switch (step) {
     case Step::Down: return down<T, false, WHOLE>(p, st);
     case Step::DownTall: return down<T, true, WHOLE>(p, st);
-    case Step::Up: return launch(up_kernel<T, false, WHOLE>, p, grid, 0, false, st);
-    case Step::UpWide: return launch(up_kernel<T, true, WHOLE>, p, grid, 0, false, st);
+    case Step::Up: return up<T, false, WHOLE>(p, st);
+    case Step::UpWide: return up<T, true, WHOLE>(p, st);
     case Step::Outer: return outer<T, false, WHOLE>(p, st);
     default: return outer<T, true, WHOLE>(p, st);
   }
@@ -545,8 +666,10 @@ int check(const char* tag, int dtype, int64_t T, int64_t L, int64_t N, int64_t K
 
 using namespace b200q;
 
+extern "C" size_t b200q_add_adapters_inner_bytes(int64_t T, int64_t r) { return T <= 0 || r <= 0 ? 0 : (size_t)T * ((r + 15) / 16 * 16) * 4; }
+
 extern "C" int b200q_add_adapters(const void* y, const void* x, const void* a, const void* b, int dtype, int64_t T, int64_t L, int64_t N, int64_t K,
-                                  int64_t r, const int32_t* order, const int32_t* tiles, const float* scales, float* h, void* out, void* stream) {
+                                  int64_t r, const int32_t* order, const int32_t* tiles, const float* scales, void* h, void* out, void* stream) {
   const char* tag = "add_adapters";
   if (int rc = check(tag, dtype, T, L, N, K, r)) return rc;
   if (T == 0 || N == 0) return B200Q_OK;
@@ -559,20 +682,20 @@ extern "C" int b200q_add_adapters(const void* y, const void* x, const void* a, c
   if (!x || !a || !b || !order || !tiles || !h) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
   for (const void* q : {y, x, a, b, static_cast<const void*>(out)})
     if (!aligned(q, 2)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
-  if (!aligned(tiles, 16)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] tiles must be 16-byte aligned", tag);
+  if (!aligned(tiles, 16) || !aligned(h, 16)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] tiles and h must be 16-byte aligned", tag);
   Params p{};
-  p.x = x; p.w = a; p.out = h;
+  p.x = x; p.w = a; p.h = static_cast<uint16_t*>(h); p.r16 = (int)(r + 15) / 16 * 16;
   p.order = order; p.tiles = reinterpret_cast<const int4*>(tiles); p.tiles_n = b200q_group_rows_tiles(T, L);
   p.T = T; p.C = K; p.L = (int)L; p.r = (int)r;
   const ScratchLock lock(h);
   if (int rc = run(Step::Down, p, dtype, st)) return rc;
-  p.x = nullptr; p.w = b; p.h = h; p.y = y; p.out = out; p.scales = scales; p.C = N;
+  p.x = nullptr; p.w = b; p.y = y; p.out = out; p.scales = scales; p.C = N;
   return run(Step::Up, p, dtype, st);
 }
 
 extern "C" int b200q_add_adapters_grad(const void* dy, const void* x, const void* a, const void* b, int dtype, int64_t T, int64_t L, int64_t N, int64_t K,
-                                       int64_t r, const int32_t* order, const int32_t* starts, const int32_t* tiles, const float* scales, const float* h,
-                                       float* g, void* dx, void* da, void* db, void* stream) {
+                                       int64_t r, const int32_t* order, const int32_t* starts, const int32_t* tiles, const float* scales, const void* h,
+                                       void* g, void* dx, void* da, void* db, void* stream) {
   const char* tag = "add_adapters";
   if (int rc = check(tag, dtype, T, L, N, K, r)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -586,29 +709,30 @@ extern "C" int b200q_add_adapters_grad(const void* dy, const void* x, const void
     return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
   for (const void* q : {dy, x, a, b, static_cast<const void*>(dx), static_cast<const void*>(da), static_cast<const void*>(db)})
     if (!aligned(q, 2)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
-  if (!aligned(tiles, 16)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] tiles must be 16-byte aligned", tag);
+  if (!aligned(tiles, 16) || !aligned(h, 16) || !aligned(g, 16)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] tiles, h and g must be 16-byte aligned", tag);
   Params p{};
+  p.h = static_cast<uint16_t*>(g); p.r16 = (int)(r + 15) / 16 * 16;
   p.order = order; p.starts = starts; p.tiles = reinterpret_cast<const int4*>(tiles); p.tiles_n = b200q_group_rows_tiles(T, L);
   p.T = T; p.L = (int)L; p.r = (int)r;
   const ScratchLock lock(g);
   if (dx || da) {
     Params d = p;
-    d.x = dy; d.w = b; d.out = g; d.scales = scales; d.C = N;
+    d.x = dy; d.w = b; d.scales = scales; d.C = N;
     if (int rc = run(Step::DownTall, d, dtype, st)) return rc;
   }
   if (dx) {
     Params d = p;
-    d.w = a; d.h = g; d.out = dx; d.C = K;
+    d.w = a; d.out = dx; d.C = K;
     if (int rc = run(Step::UpWide, d, dtype, st)) return rc;
   }
   if (da) {
     Params d = p;
-    d.x = x; d.h = g; d.out = da; d.C = K;
+    d.x = x; d.out = da; d.C = K;
     if (int rc = run(Step::Outer, d, dtype, st)) return rc;
   }
   if (db) {
     Params d = p;
-    d.x = dy; d.h = h; d.out = db; d.scales = scales; d.C = N;
+    d.x = dy; d.h = static_cast<uint16_t*>(const_cast<void*>(h)); d.out = db; d.scales = scales; d.C = N;
     if (int rc = run(Step::OuterTall, d, dtype, st)) return rc;
   }
   return B200Q_OK;

@@ -920,9 +920,9 @@ bool adapters_run(Adapters* p, Tensor* out, Tensor* h) {
   if (!adapters_ok(p, *p->y)) return false;
   const at::Device dev = p->x->device();
   if (!out->defined()) *out = fresh(p->y->sizes(), p->y->scalar_type(), dev);
-  *h = fresh({p->T, p->r}, at::kFloat, dev);
+  *h = fresh({p->T, 2, (p->r + 15) / 16 * 16}, at::kBFloat16, dev);
   return b200q_add_adapters(p->y->data_ptr(), p->x->data_ptr(), p->a->data_ptr(), p->b->data_ptr(), dtype_code(p->x->scalar_type()), p->T, p->L, p->N, p->K, p->r,
-                            ints(*p->g[2]), ints(*p->g[3]), floats(p->scales), static_cast<float*>(h->data_ptr()), out->data_ptr(), stream_of(dev)) == B200Q_OK;
+                            ints(*p->g[2]), ints(*p->g[3]), floats(p->scales), h->data_ptr(), out->data_ptr(), stream_of(dev)) == B200Q_OK;
 }
 bool overlap(const Tensor& a, const Tensor& b) {
   const char *p = static_cast<const char*>(a.data_ptr()), *q = static_cast<const char*>(b.data_ptr());
@@ -969,16 +969,16 @@ struct AdaptersFn : public torch::autograd::Function<AdaptersFn> {
           Adapters p{nullptr, &saved[0], &saved[1], &saved[2], {&saved[4], &saved[5], &saved[6], &saved[7]}, saved.size() > 8 ? &saved[8] : nullptr};
           const Tensor& h = saved[3];
           const at::Device dev = saved[0].device();
-          bool done = adapters_ok(&p, dy) && plain(h, at::kFloat, dev);
+          bool done = adapters_ok(&p, dy) && plain(h, at::kBFloat16, dev) && on16(h);
           if (done) {
             Tensor g;
             if (for_x) dx = fresh(p.x->sizes(), p.x->scalar_type(), dev);
             if (for_a) da = fresh(p.a->sizes(), p.x->scalar_type(), dev);
             if (for_b) db = fresh(p.b->sizes(), p.x->scalar_type(), dev);
-            if (for_x || for_a) g = fresh({p.T, p.r}, at::kFloat, dev);
+            if (for_x || for_a) g = fresh(h.sizes(), at::kBFloat16, dev);
             auto at = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
             done = b200q_add_adapters_grad(dy.data_ptr(), p.x->data_ptr(), p.a->data_ptr(), p.b->data_ptr(), dtype_code(p.x->scalar_type()), p.T, p.L, p.N, p.K, p.r,
-                                           ints(*p.g[2]), ints(*p.g[1]), ints(*p.g[3]), floats(p.scales), floats(&h), static_cast<float*>(at(g)), at(dx), at(da),
+                                           ints(*p.g[2]), ints(*p.g[1]), ints(*p.g[3]), floats(p.scales), h.data_ptr(), at(g), at(dx), at(da),
                                            at(db), stream_of(dev)) == B200Q_OK;
           }
           if (!done) {

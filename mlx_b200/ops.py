@@ -1044,17 +1044,21 @@ def _adapter_args(tag, y, x, a, b, groups, scales):
     return dev, T, L, N, K, r, RowGroups(*(t.contiguous() for t in groups)), scales
 
 
+def _inner(T: int, rank: int) -> Tuple[int, int, int]:
+    return T, 2, (rank + 15) // 16 * 16
+
+
 def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, groups: RowGroups, scales: Optional[torch.Tensor] = None,
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Low-rank adapters of many requests at once beside a shared projection: y [..., N], what the projection (quantized_matmul, qqmm, ...)
     made of x [..., K], plus scales[l] b[l] (a[l] x[t]) for every row t with an adapter l.  a [adapters, rank, K], b [adapters, N, rank],
-    scales [adapters] (None: 1); groups: group_rows of the rows' adapters.  bfloat16 and float16; sums and the inner product in float32,
-    rounded once.  out: where the sum goes, y itself for a sum in place.  grad.add_adapters is the same with gradients."""
+    scales [adapters] (None: 1); groups: group_rows of the rows' adapters.  bfloat16 and float16; sums in float32, the
+    inner product to 2^-17, the result rounded once.  out: where the sum goes, y itself for a sum in place.  grad.add_adapters is the same with gradients."""
     return _add_adapters(y, x, a, b, groups, scales, out)[0]
 
 
 def _add_adapters(y, x, a, b, groups, scales=None, out=None):
-    """-> add_adapters' result and the inner products, float32 [rows, rank] in the order of the groups."""
+    """-> add_adapters' result and the inner products, two bfloat16 parts per value [rows, 2, rank in whole 16s] in the order of the groups."""
     r = _front.add_adapters(y, x, a, b, groups, scales, out)
     if r is not None:
         return r
@@ -1068,7 +1072,7 @@ def _add_adapters(y, x, a, b, groups, scales=None, out=None):
     y, x, a, b = (t.detach().contiguous() for t in (y, x, a, b))
     with torch.cuda.device(dev):
         out = torch.empty_like(y) if out is None else out
-        h = torch.empty((T, rank), dtype=torch.float32, device=dev)
+        h = torch.empty(_inner(T, rank), dtype=torch.bfloat16, device=dev)
         rc = _lib.load().b200q_add_adapters(_ptr(y), _ptr(x), _ptr(a), _ptr(b), _DT[x.dtype], T, L, N, K, rank, _ptr(groups.order), _ptr(groups.tiles),
                                             _ptr(scales), _ptr(h), _ptr(out), _stream(x))
     _lib.check(rc)
@@ -1077,17 +1081,18 @@ def _add_adapters(y, x, a, b, groups, scales=None, out=None):
 
 def add_adapters_grad(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, groups: RowGroups, h: torch.Tensor,
                       scales: Optional[torch.Tensor] = None, for_x: bool = True, for_a: bool = True, for_b: bool = True):
-    """-> gradients of add_adapters with respect to x, a and b (None where not asked for; that of y is dy).  h: a[l] x in float32, as the
-    forward pass leaves it."""
+    """-> gradients of add_adapters with respect to x, a and b (None where not asked for; that of y is dy).  h: the inner products, as the
+    forward pass leaves them."""
     tag = "add_adapters_grad"
     dev, T, L, N, K, rank, groups, scales = _adapter_args(tag, dy, x, a, b, groups, scales)
-    if h.dtype != torch.float32 or tuple(h.shape) != (T, rank):
-        raise ValueError(f"[{tag}] h must be float32 [{T}, {rank}].")
+    if h.dtype != torch.bfloat16 or tuple(h.shape) != _inner(T, rank):
+        raise ValueError(f"[{tag}] h must be bfloat16 {_inner(T, rank)}.")
     _require_cuda(tag, x, h)
-    dy, x, a, b, h = (t.detach().contiguous() for t in (dy, x, a, b, h))
+    dy, x, a, b = (t.detach().contiguous() for t in (dy, x, a, b))
+    h = _aligned(h)
     with torch.cuda.device(dev):
         dx, da, db = (torch.empty_like(t) if wanted else None for t, wanted in ((x, for_x), (a, for_a), (b, for_b)))
-        g = torch.empty((T, rank), dtype=torch.float32, device=dev) if for_x or for_a else None
+        g = torch.empty_like(h) if for_x or for_a else None
         rc = _lib.load().b200q_add_adapters_grad(_ptr(dy), _ptr(x), _ptr(a), _ptr(b), _DT[x.dtype], T, L, N, K, rank, _ptr(groups.order),
                                                  _ptr(groups.starts), _ptr(groups.tiles), _ptr(scales), _ptr(h), _ptr(g), _ptr(dx), _ptr(da), _ptr(db),
                                                  _stream(x))

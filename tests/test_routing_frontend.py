@@ -78,7 +78,7 @@ def test_adapters():
                    dict(groups=g._replace(order=i32(5).long())), dict(groups=g._replace(tiles=i32(n + 1, 4))), dict(groups=g._replace(starts=i32(2))),
                    dict(scales=torch.zeros(3)), dict(scales=i32(2))):
             refused(f, **{**args, **kw})
-    refused(mb.add_adapters_grad, bf(5, 8), bf(5, 16), bf(2, 4, 16), bf(2, 8, 4), g, torch.zeros(5, 4), error=RuntimeError)
+    refused(mb.add_adapters_grad, bf(5, 8), bf(5, 16), bf(2, 4, 16), bf(2, 8, 4), g, bf(5, 2, 16), error=RuntimeError)
 
 
 def test_the_c_abi_refuses_before_any_cuda_call():
