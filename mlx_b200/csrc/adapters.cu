@@ -146,7 +146,7 @@ __device__ __forceinline__ void copy_few(void* dst, const T* p, int64_t have, in
 
 struct Params {
   const void *x, *w;       // activations; weights of all adapters
-  uint16_t* h;             // inner products, by place: [T][high, low][r16] bf16
+  uint16_t* h;             // inner products, by place: [T][r16 / 16][4][high, low][4] bf16
   const void* y;           // up: what is added to (null: zeros)
   void* out;
   const float* scales;     // null: 1
@@ -322,115 +322,186 @@ __global__ void __launch_bounds__(kThreads, NT == 8 ? 1 : 2) down_kernel(const P
     if (rank < p.r16) {   // (ranks from r on: their weights were zeros)
       uint32_t hi, lo;
       split(rank < p.r ? c * s.x : 0.0f, rank + 1 < p.r ? c * s.y : 0.0f, &hi, &lo);
-      uint16_t* h = p.h + (int64_t)(tile.y + i / (kRanks / 2)) * 2 * p.r16 + rank;
+      uint16_t* h = p.h + (int64_t)(tile.y + i / (kRanks / 2)) * 2 * p.r16 + rank / 4 * 8 + rank % 4;
       *reinterpret_cast<uint32_t*>(h) = hi;
-      *reinterpret_cast<uint32_t*>(h + p.r16) = lo;
+      *reinterpret_cast<uint32_t*>(h + 4) = lo;
     }
   }
   cluster.sync();   // no block leaves while others read its sums
 }
 
-// ---- out[row] = y[row] + (c) sum over ranks of h[place] w.  Warps by (tiles, 32 columns), each on its own; ranks in steps of 16, of which KS
-// have their weights in registers (up to 64 ranks: all, over all rows that an adapter has among the warp's tiles).
+// ---- out[row] = y[row] + (c) sum over ranks of h[place] w.  Blocks by (tiles, 256 columns), warps by 32 columns; steps of 16 rows and, inside, 16
+// ranks.  Up to 64 ranks (KS steps) have their weights in registers, over all rows that an adapter has among the block's tiles, and h in shared
+// memory; more (CHUNKED) take both from the caches again for every 16 rows.
 // WIDE: weights [r, C], else [C, r].
-template <typename T, bool WIDE, bool WHOLE, int KS>
+//
+// Bound by the latency of y: every lane copies its own pieces of it, three steps of rows ahead, into a ring in shared memory.
+constexpr int kUpStages = 4, kUpTiles = 8;
+template <int KS>
+struct Up {
+  static constexpr int kPitch = 64 * (KS | 1);   // bytes of h per row: eight lanes' 16-byte reads are in different banks
+  static constexpr size_t kBytes = (size_t)kWarps * kUpStages * 1024 + 2 * kRows * kPitch;
+};
+template <typename T, bool WIDE, bool WHOLE, int KS, bool CHUNKED>
 __global__ void __launch_bounds__(kThreads, KS == 4 ? 2 : 3) up_kernel(const Params p) {
   constexpr bool kSplitW = std::is_same_v<T, __half>;
+  constexpr int kPitch = Up<KS>::kPitch;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ int4 tiles[kUpTiles];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
   const int64_t C = p.C, blocks = (C + 255) / 256;
   const int64_t n0 = (blockIdx.x % blocks) * 256 + warp * 32, n = n0 + q * 8;   // the lane's columns are n .. n + 7
   const int64_t have = C - n;
-  if (n0 >= C) return;
   const T* y = static_cast<const T*>(p.y);
   T* out = static_cast<T*>(p.out);
-  const int64_t first = blockIdx.x / blocks * p.each, last = min(first + p.each, p.tiles_n);
+  if (threadIdx.x < kUpTiles) {
+    const int64_t k = blockIdx.x / blocks * p.each + threadIdx.x;
+    int4 t = make_int4(-1, 0, 0, 0);
+    if (threadIdx.x < p.each && k < p.tiles_n) t = tile_of(p, k);
+    if (t.x < 0 && p.y == p.out) t.z = 0;   // rows without an adapter are there already
+    tiles[threadIdx.x] = t;
+  }
+  __syncthreads();
+  unsigned char *ring = smem + warp * kUpStages * 1024 + lane * 16, *hs = smem + kWarps * kUpStages * 1024;
+  auto next_tile = [&](int k) {
+    while (k < p.each && tiles[k].z == 0) ++k;
+    return k;
+  };
+  // y of the steps ahead
+  int ik = next_tile(0), im = 0, stage_in = 0;
+  int64_t rows[2];
+  auto look = [&] {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) rows[i] = ik < p.each && im + i * 8 + g < tiles[ik].z ? row_at(p, tiles[ik].y + im + i * 8 + g) : -1;
+  };
+  auto issue = [&] {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      unsigned char* d = ring + stage_in * 1024 + i * 512;
+      const bool there = y != nullptr && rows[i] >= 0 && have > 0;
+      if constexpr (WHOLE) copy_async<16>(d, there ? y + rows[i] * C + n : p.out, there);
+      else *reinterpret_cast<uint4*>(d) = there ? load8<false, false>(y + rows[i] * C + n, have) : make_uint4(0, 0, 0, 0);
+    }
+    commit();
+    stage_in = stage_in == kUpStages - 1 ? 0 : stage_in + 1;
+    if (ik < p.each && (im += 16) >= tiles[ik].z) {
+      ik = next_tile(ik + 1);
+      im = 0;
+    }
+    look();
+  };
+  auto copy_h = [&](int k, int buffer) {
+    if (CHUNKED || k >= p.each || tiles[k].x < 0) return;
+    const int per_row = p.r16 / 4, n16 = tiles[k].z * per_row;   // pieces of 16 bytes
+    const uint16_t* src = p.h + (int64_t)tiles[k].y * 2 * p.r16;
+    for (int i = threadIdx.x; i < n16; i += kThreads)
+      copy_async<16>(hs + (buffer * kRows + i / per_row) * kPitch + i % per_row * 16, src + i * 8, true);
+  };
   uint32_t bh[KS][4][2], bl[kSplitW ? KS : 1][4][2];   // rank step, column tile, pair of the lane's 4 ranks
   const T* w = nullptr;
   auto weights = [&](int r0) {
+    uint32_t b[KS][4][2];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      uint32_t b[4][2];
       if constexpr (WIDE) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int rank = r0 + s * 16 + (g >> 1) * 4 + j * 2 + (g & 1);
           const uint4 v = rank < p.r ? load8<WHOLE>(w + (int64_t)rank * C + n, have) : make_uint4(0, 0, 0, 0);
-          b[0][j] = v.x; b[1][j] = v.y; b[2][j] = v.z; b[3][j] = v.w;
+          b[s][0][j] = v.x; b[s][1][j] = v.y; b[s][2][j] = v.z; b[s][3][j] = v.w;
         }
       } else {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const int64_t col = n0 + (g >> 1) * 8 + t * 2 + (g & 1);
           const int rank = r0 + s * 16 + q * 4;
-          load_few<4>(w + col * p.r + rank, col < C ? p.r - rank : 0, p.width, b[t]);
+          load_few<4>(w + col * p.r + rank, col < C ? p.r - rank : 0, p.width, b[s][t]);
         }
       }
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           uint32_t lo;
-          as_bf16<T>(WIDE ? transposed(b[t][j]) : b[t][j], &bh[s][t][j], &lo);
+          as_bf16<T>(WIDE ? transposed(b[s][t][j]) : b[s][t][j], &bh[s][t][j], &lo);
           if constexpr (kSplitW) bl[s][t][j] = lo;
         }
-    }
   };
-  int loaded = -1;
-  for (int64_t k = first; k < last; ++k) {
-    const int4 tile = tile_of(p, k);
-    if (tile.z == 0) continue;
+  int k = ik, buffer = 0, loaded = -1, stage = 0;
+  look();
+  copy_h(k, 0);
+#pragma unroll
+  for (int i = 0; i < kUpStages - 1; ++i) issue();   // the first group has the first tile's h
+  bool short_tile = false;
+  for (bool start = true; k < p.each; start = false) {
+    const int4 tile = tiles[k];
     const bool plain = tile.x < 0;   // rows without an adapter
-    if (plain && p.y == p.out) continue;
     float c = 0.0f;
     if (!plain) {
       c = p.scales ? p.scales[tile.x] : 1.0f;
       w = static_cast<const T*>(p.w) + (int64_t)tile.x * p.r * C;
-      if (p.r16 <= 16 * KS && loaded != tile.x) {
+      if (!CHUNKED && loaded != tile.x) {
         weights(0);
         loaded = tile.x;
       }
     }
+    // the group with this tile's h was issued with the first step of the tile before, four steps ago if that was a whole one
+    if (start) wait_all_but<kUpStages - 2>();
+    else if (short_tile) wait_all_but<0>();
+    __syncthreads();
+    const int after = next_tile(k + 1);
+    copy_h(after, buffer ^ 1);
+    short_tile = tile.z <= 48;
     for (int m0 = 0; m0 < tile.z; m0 += 16) {
+      issue();
       int64_t at[2];
-      uint4 v[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = m0 + i * 8 + g;
-        at[i] = row < tile.z ? row_at(p, tile.y + row) : -1;
-        v[i] = y && at[i] >= 0 ? load8<WHOLE, false>(y + at[i] * C + n, have) : make_uint4(0, 0, 0, 0);
-      }
+      for (int i = 0; i < 2; ++i) at[i] = m0 + i * 8 + g < tile.z ? row_at(p, tile.y + m0 + i * 8 + g) : -1;
       float acc[4][4] = {};
+      auto step = [&](int s, const uint4& h0, const uint4& h1) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], h0.x, h1.x, h0.y, h1.y, bh[s][t][0], bh[s][t][1]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], h0.z, h1.z, h0.w, h1.w, bh[s][t][0], bh[s][t][1]);
+        if constexpr (kSplitW) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], h0.x, h1.x, h0.y, h1.y, bl[s][t][0], bl[s][t][1]);
+        }
+      };
       if (!plain) {
-        for (int r0 = 0; r0 < p.r16; r0 += 16 * KS) {
-          if (p.r16 > 16 * KS) weights(r0);
+        if constexpr (CHUNKED) {
+          for (int r0 = 0; r0 < p.r16; r0 += 16 * KS) {
+            weights(r0);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              if (r0 + s * 16 >= p.r16) break;
+              uint4 h[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                h[i] = m0 + i * 8 + g < tile.z ? *reinterpret_cast<const uint4*>(p.h + (int64_t)(tile.y + m0 + i * 8 + g) * 2 * p.r16 + (r0 + s * 16) * 2 + q * 8)
+                                               : make_uint4(0, 0, 0, 0);
+              step(s, h[0], h[1]);
+            }
+          }
+        } else {
+          // (rows behind the tile's last one have what was there before; their products are not stored)
+          const unsigned char* src = hs + (buffer * kRows + m0 + g) * kPitch + q * 16;
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
-            const int rank = r0 + s * 16;
-            if (KS > 1 && rank >= p.r16) break;
-            uint2 h[2][2];   // row, part
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint16_t* src = p.h + (int64_t)(tile.y + m0 + i * 8 + g) * 2 * p.r16 + rank + q * 4;
-              const bool there = m0 + i * 8 + g < tile.z;
-              h[i][0] = there ? *reinterpret_cast<const uint2*>(src) : make_uint2(0, 0);
-              h[i][1] = there ? *reinterpret_cast<const uint2*>(src + p.r16) : make_uint2(0, 0);
-            }
-#pragma unroll
-            for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], h[0][0].x, h[1][0].x, h[0][0].y, h[1][0].y, bh[s][t][0], bh[s][t][1]);
-#pragma unroll
-            for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], h[0][1].x, h[1][1].x, h[0][1].y, h[1][1].y, bh[s][t][0], bh[s][t][1]);
-            if constexpr (kSplitW) {
-#pragma unroll
-              for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], h[0][0].x, h[1][0].x, h[0][0].y, h[1][0].y, bl[s][t][0], bl[s][t][1]);
-            }
+            if (KS > 1 && s * 16 >= p.r16) break;
+            step(s, *reinterpret_cast<const uint4*>(src + s * 64), *reinterpret_cast<const uint4*>(src + 8 * kPitch + s * 64));
           }
         }
       }
+      wait_all_but<kUpStages - 1>();
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (at[i] < 0 || have <= 0) continue;
         T o[8];
-        *reinterpret_cast<uint4*>(o) = v[i];
+        *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(ring + stage * 1024 + i * 512);
         if (!plain) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[e] = Elem<T>::from_float(fmaf(c, acc[e / 2][2 * i + (e & 1)], Elem<T>::to_float(o[e])));
@@ -443,8 +514,12 @@ __global__ void __launch_bounds__(kThreads, KS == 4 ? 2 : 3) up_kernel(const Par
             if (e < have) out[at[i] * C + n + e] = o[e];
         }
       }
+      stage = stage == kUpStages - 1 ? 0 : stage + 1;
     }
+    buffer ^= 1;
+    k = after;
   }
+  wait_all_but<0>();
 }
 
 // ---- out_l = (c) sum over l's rows of h[place] x[row]^T.  Blocks by (64 columns, part of the rows; adapter; 16 MT ranks), the parts are a
@@ -462,7 +537,7 @@ __global__ void __launch_bounds__(kThreads) outer_kernel(const Params p) {
   float acc[MT][4][4] = {};
   struct Stage {
     uint4 x[2];
-    uint2 h[MT][2][2];   // rank step, place (+ 8), part
+    uint4 h[MT][2];   // rank step, place (+ 8): a lane's 4 ranks' high and low parts
   };
   struct Index {
     int64_t row[2];
@@ -479,12 +554,10 @@ __global__ void __launch_bounds__(kThreads) outer_kernel(const Params p) {
       const int64_t place = t0 + i * 8 + g;
       s.x[i] = at.row[i] >= 0 ? load8<WHOLE>(x + at.row[i] * C + col, C - col) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const int rank = r0 + m * 16;
-          s.h[m][i][v] = place < hi && rank < p.r16 ? *reinterpret_cast<const uint2*>(p.h + (place * 2 + v) * p.r16 + rank + q * 4) : make_uint2(0, 0);
-        }
+      for (int m = 0; m < MT; ++m) {
+        const int rank = r0 + m * 16;
+        s.h[m][i] = place < hi && rank < p.r16 ? *reinterpret_cast<const uint4*>(p.h + place * 2 * p.r16 + rank * 2 + q * 8) : make_uint4(0, 0, 0, 0);
+      }
     }
   };
   auto multiply = [&](const Stage& s) {
@@ -501,11 +574,11 @@ __global__ void __launch_bounds__(kThreads) outer_kernel(const Params p) {
       if (MT > 1 && r0 + m * 16 >= p.r16) break;
       uint32_t a[2][4];   // part; rows of the product: of a lane's 4 ranks the first two are in its upper half
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        a[v][0] = transposed(s.h[m][0][v].x);
-        a[v][1] = transposed(s.h[m][0][v].y);
-        a[v][2] = transposed(s.h[m][1][v].x);
-        a[v][3] = transposed(s.h[m][1][v].y);
+      for (int i = 0; i < 2; ++i) {
+        a[0][2 * i] = transposed(s.h[m][i].x);
+        a[0][2 * i + 1] = transposed(s.h[m][i].y);
+        a[1][2 * i] = transposed(s.h[m][i].z);
+        a[1][2 * i + 1] = transposed(s.h[m][i].w);
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[m][t], a[0][0], a[0][1], a[0][2], a[0][3], bh[t][0], bh[t][1]);
@@ -570,12 +643,14 @@ int width_of(const void* p, int64_t pitch) {
   while (w > 2 && (!aligned(p, w) || pitch % w != 0)) w /= 2;
   return w;
 }
-// Blocks per cluster: enough for two blocks per SM, a power of two up to 8, with work for everyone.
-int split_of(int64_t blocks, int64_t most) {
+// Blocks per cluster: a power of two up to 8, as many as fit on the SMs at once, with work for everyone.
+int split_of(int64_t blocks, int64_t slots, int64_t most) {
   int s = 1;
-  while (s < 8 && blocks * s < 2 * 148 && 2 * s <= most) s *= 2;
+  while (s < 8 && blocks * 2 * s <= slots && 2 * s <= most) s *= 2;
   return s;
 }
+// Tiles that there will be, about: the table has room for the most that there can be.
+int64_t likely_tiles(const Params& p) { return std::min<int64_t>(p.T, p.T / kRows + (std::min<int64_t>(p.T, p.L) + 1) / 2); }
 
 template <typename K>
 int launch(K kern, const Params& p, dim3 grid, size_t smem, bool cluster, cudaStream_t st) {
@@ -601,7 +676,7 @@ int launch(K kern, const Params& p, dim3 grid, size_t smem, bool cluster, cudaSt
 template <typename T, bool TALL, bool WHOLE>
 int down(Params p, cudaStream_t st) {
   const int nt = p.r <= 16 ? 2 : (p.r <= 32 ? 4 : 8), chunks = (p.r + 8 * nt - 1) / (8 * nt);
-  p.split = split_of(p.tiles_n * chunks, p.C / (kWarps * 32));
+  p.split = split_of(likely_tiles(p) * chunks, 148 * (nt == 8 ? 1 : 2), p.C / (kWarps * 32));
   const dim3 grid((unsigned)(p.tiles_n * p.split), chunks);
   if (nt == 2) return launch(down_kernel<T, TALL, WHOLE, 2>, p, grid, Down<TALL, 2>::kBytes, true, st);
   if (nt == 4) return launch(down_kernel<T, TALL, WHOLE, 4>, p, grid, Down<TALL, 4>::kBytes, true, st);
@@ -610,17 +685,18 @@ int down(Params p, cudaStream_t st) {
 template <typename T, bool WIDE, bool WHOLE>
 int up(Params p, cudaStream_t st) {
   const int64_t cols = (p.C + 255) / 256;
-  p.each = (int)std::max<int64_t>(1, std::min<int64_t>(8, p.tiles_n * cols / (148 * 8)));   // a block's tiles share their weights' loads
+  p.each = (int)std::max<int64_t>(1, std::min<int64_t>(kUpTiles, p.tiles_n * cols / (148 * 8)));   // a block's tiles share their weights' loads
   const dim3 grid((unsigned)((p.tiles_n + p.each - 1) / p.each * cols));
-  if (p.r <= 16) return launch(up_kernel<T, WIDE, WHOLE, 1>, p, grid, 0, false, st);
-  if (p.r <= 32) return launch(up_kernel<T, WIDE, WHOLE, 2>, p, grid, 0, false, st);
-  return launch(up_kernel<T, WIDE, WHOLE, 4>, p, grid, 0, false, st);
+  if (p.r <= 16) return launch(up_kernel<T, WIDE, WHOLE, 1, false>, p, grid, Up<1>::kBytes, false, st);
+  if (p.r <= 32) return launch(up_kernel<T, WIDE, WHOLE, 2, false>, p, grid, Up<2>::kBytes, false, st);
+  if (p.r <= 64) return launch(up_kernel<T, WIDE, WHOLE, 4, false>, p, grid, Up<4>::kBytes, false, st);
+  return launch(up_kernel<T, WIDE, WHOLE, 4, true>, p, grid, kWarps * kUpStages * 1024, false, st);
 }
 template <typename T, bool TALL, bool WHOLE>
 int outer(Params p, cudaStream_t st) {
   const int mt = p.r <= 16 ? 1 : (p.r <= 32 ? 2 : 4), chunks = (p.r + 16 * mt - 1) / (16 * mt);
   const int64_t cols = (p.C + 63) / 64;
-  p.split = split_of(cols * p.L * chunks, p.T / 64);
+  p.split = split_of(cols * p.L * chunks, 148 * 4, p.T / 64);
   const dim3 grid((unsigned)(cols * p.split), p.L, chunks);
   const size_t smem = (size_t)4 * 16 * mt * 68 * 4;
   if (mt == 1) return launch(outer_kernel<T, TALL, WHOLE, 1>, p, grid, smem, true, st);
