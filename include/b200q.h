@@ -462,7 +462,7 @@ int b200q_combine_rows_grad(const void* dy, const void* y, int dtype, int64_t T,
  *   sizes [n], starts [n + 1]: rows per group, and where each group (and behind them the rows without one) starts in the order
  *   order [T]: rows by group, stably; those without a group last, as -1 - row
  *   tiles [b200q_group_rows_tiles(T, n)][4] (16-byte aligned): what b200q_add_adapters reads: up to 64 places of one group each
- * At most 4096 groups.  ws: plain scratch, 4-byte aligned.
+ * At most 4096 groups and 2^30 rows.  ws: plain scratch, 4-byte aligned.
  */
 int64_t b200q_group_rows_tiles(int64_t T, int64_t n);
 size_t b200q_group_rows_workspace_bytes(int64_t T, int64_t n);
@@ -478,7 +478,7 @@ int b200q_group_rows(const void* ids, int id_bytes, int64_t T, int64_t n, int32_
  *   which the gradient takes (else scratch); rows without an adapter have none
  * b200q_add_adapters_grad: from dy [T, N] the gradients dx [T, K], da, db, each NULL where not wanted (that of y is dy); g, as
  * large as h, is scratch, needed for dx and da.  h is needed for db, x for da, a for dx, b for dx and da.
- * At most 4096 adapters, ranks of 4096 and widths of 2^24.
+ * At most 2^30 rows, 4096 adapters, ranks of 4096 and widths of 2^24.
  */
 size_t b200q_add_adapters_inner_bytes(int64_t T, int64_t r);
 int b200q_add_adapters(const void* y, const void* x, const void* a, const void* b, int dtype, int64_t T, int64_t L, int64_t N, int64_t K,

@@ -113,35 +113,62 @@ __device__ __forceinline__ void load_few(const T* p, int64_t have, int width, ui
 }
 
 __device__ __forceinline__ uint32_t shared(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// BYTES (4, 8, 16) to shared memory, asynchronously; zeros where there is nothing (p is not read then).
+// BYTES (4, 8, 16) to shared memory, asynchronously; of them the first n (0: p is not read) from p on, then zeros.
 template <int BYTES>
-__device__ __forceinline__ void copy_async(void* dst, const void* p, bool there) {
-  const int n = there ? BYTES : 0;
-  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared(dst)), "l"(p), "r"(n) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(shared(dst)), "l"(p), "n"(BYTES), "r"(n) : "memory");
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* p, int n) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(p), "n"(BYTES), "r"(n) : "memory");
 }
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void wait_all_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-// N consecutive values (4, 8 or 16) in the widest pieces that the rows' alignment allows.  base: an address that may be named.
+// N consecutive values (4, 8 or 16) in the widest pieces that the rows' alignment allows, to shared memory; pieces of 16 bytes are 512 apart.
 template <int N, typename T>
-__device__ __forceinline__ void copy_few(void* dst, const T* p, int64_t have, int width, const void* base) {
-  char* d = static_cast<char*>(dst);
+__device__ __forceinline__ void copy_few(uint32_t dst, const T* p, int have, int width) {
   const char* q = reinterpret_cast<const char*>(p);
   if (N >= 8 && width == 16) {
 #pragma unroll
-    for (int i = 0; i < N / 8; ++i) copy_async<16>(d + 512 * i, 8 * i < have ? q + 16 * i : base, 8 * i < have);   // (pieces of 16 bytes are 512 apart)
+    for (int i = 0; i < N / 8; ++i) copy_async<16>(dst + 512 * i, q + 16 * i, 8 * i < have ? 16 : 0);
   } else if (width >= 8) {
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) copy_async<8>(d + 512 * (i / 2) + 8 * (i & 1), 4 * i < have ? q + 8 * i : base, 4 * i < have);
+    for (int i = 0; i < N / 4; ++i) copy_async<8>(dst + 512 * (i / 2) + 8 * (i & 1), q + 8 * i, 4 * i < have ? 8 : 0);
   } else if (width == 4) {
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) copy_async<4>(d + 512 * (i / 4) + 4 * (i & 3), 2 * i < have ? q + 4 * i : base, 2 * i < have);
+    for (int i = 0; i < N / 2; ++i) copy_async<4>(dst + 512 * (i / 4) + 4 * (i & 3), q + 4 * i, 2 * i < have ? 4 : 0);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      *reinterpret_cast<uint16_t*>(d + 512 * (i / 8) + 2 * (i & 7)) = i < have ? __ldg(reinterpret_cast<const uint16_t*>(p) + i) : (uint16_t)0;
+    for (int i = 0; i < N; ++i) {
+      const uint16_t v = i < have ? __ldg(reinterpret_cast<const uint16_t*>(p) + i) : (uint16_t)0;
+      asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + 512 * (i / 8) + 2 * (i & 7)), "h"(v) : "memory");
+    }
   }
+}
+__device__ __forceinline__ void store16(uint32_t dst, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// (volatile: after the wait for the copy)
+__device__ __forceinline__ uint4 load16(uint32_t src) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
+  return v;
+}
+// a + c * b for eight values of T
+template <typename T>
+__device__ __forceinline__ uint4 add8(const uint4& a, float c, const float (&b)[8]) {
+  uint4 o;
+  const uint32_t* in = &a.x;
+  uint32_t* to = &o.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 f;
+    if constexpr (std::is_same_v<T, __half>) f = __half22float2(*reinterpret_cast<const __half2*>(&in[i]));
+    else f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&in[i]));
+    f.x = fmaf(c, b[2 * i], f.x);
+    f.y = fmaf(c, b[2 * i + 1], f.y);
+    if constexpr (std::is_same_v<T, __half>) { const __half2 h = __float22half2_rn(f); to[i] = *reinterpret_cast<const uint32_t*>(&h); }
+    else { const __nv_bfloat162 h = __float22bfloat162_rn(f); to[i] = *reinterpret_cast<const uint32_t*>(&h); }
+  }
+  return o;
 }
 
 struct Params {
@@ -165,10 +192,10 @@ __device__ __forceinline__ int4 tile_of(const Params& p, int64_t k) {
   return t;
 }
 // The row at a place of the order; -1 where there is none.
-__device__ __forceinline__ int64_t row_at(const Params& p, int64_t place) {
-  int64_t row = p.order[place];
-  if (row < 0) row = -1 - row;
-  return row < p.T ? row : -1;
+__device__ __forceinline__ int row_at(const Params& p, int64_t place) {
+  int row = p.order[place];
+  row = row < 0 ? ~row : row;
+  return row < (int)p.T ? row : -1;
 }
 
 // ---- h[place] = (c) sum over the long dimension of x[row] w.  Blocks by (tile, part of the long dimension, 8 NT ranks); the parts are a cluster
@@ -180,75 +207,79 @@ __device__ __forceinline__ int64_t row_at(const Params& p, int64_t place) {
 template <bool TALL, int NT>
 struct Down {
   static constexpr int kRanks = 8 * NT, kW = TALL ? (NT == 8 ? 8 : 4) : NT, kPieces = 8 + kW, kStages = NT == 8 ? 3 : 2;
+  static constexpr int kLine = kRanks + 8;   // floats per row of the sums: lanes' pairs are in different banks
   static constexpr size_t kBytes = (size_t)kWarps * kStages * kPieces * 512;
-  static_assert(kBytes >= (size_t)kWarps * kRows * kRanks * 4, "the sums lie where the ring was");
+  static_assert(kBytes >= (size_t)kWarps * kRows * kLine * 4, "the sums lie where the ring was");
 };
 template <typename T, bool TALL, bool WHOLE, int NT>
 __global__ void __launch_bounds__(kThreads, NT == 8 ? 1 : 2) down_kernel(const Params p) {
   using D = Down<TALL, NT>;
-  constexpr int kRanks = D::kRanks, kStages = D::kStages;
+  constexpr int kRanks = D::kRanks, kStages = D::kStages, kLine = D::kLine, kStageBytes = D::kPieces * 512;
   extern __shared__ __align__(16) unsigned char smem[];
   cg::cluster_group cluster = cg::this_cluster();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
   const int part = (int)(blockIdx.x % p.split);
   const int4 tile = tile_of(p, blockIdx.x / p.split);
   if (tile.z == 0 || tile.x < 0) return;   // the whole cluster
-  const int subs = (tile.z + 15) / 16, r0 = blockIdx.y * kRanks;
-  const int64_t C = p.C;
+  const int subs = (tile.z + 15) / 16, r0 = blockIdx.y * kRanks, C = (int)p.C, step = p.split * kWarps * 32;
+  int k = (part * kWarps + warp) * 32;     // of the step that is multiplied
+  int kl = k + q * 8;                      // the lane's, of the step that is loaded
   const T* x[4][2];
+  int xn[4][2];   // bytes to copy: 0 where there is no row
 #pragma unroll
   for (int m = 0; m < 4; ++m)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int row = m * 16 + i * 8 + g;
-      const int64_t at = row < tile.z ? row_at(p, tile.y + row) : -1;
-      x[m][i] = at < 0 ? nullptr : static_cast<const T*>(p.x) + at * C;
+      const int row = m * 16 + i * 8 + g, at = row < tile.z ? row_at(p, tile.y + row) : -1;
+      x[m][i] = static_cast<const T*>(p.x) + (int64_t)max(at, 0) * C + kl;
+      xn[m][i] = at < 0 ? 0 : 16;
     }
   const T* w = static_cast<const T*>(p.w) + (int64_t)tile.x * p.r * C;
-  unsigned char* ring = smem + (size_t)warp * kStages * D::kPieces * 512 + lane * 16;
-  auto slot = [&](int stage, int piece) { return ring + (stage * D::kPieces + piece) * 512; };
-  auto load = [&](int64_t k0, int stage) {
-    const int64_t k = k0 + q * 8;
+  const int first = r0 + (TALL ? q * 2 * NT : (g >> 1) * 2 * NT + (g & 1));   // the lane's first rank
+  int kr = k + (g >> 1) * 8 + (g & 1);
+  w += TALL ? (int64_t)kr * p.r + first : (int64_t)first * C + kl;
+  const uint32_t ring = shared(smem) + warp * kStages * kStageBytes + lane * 16;
+  auto load = [&](uint32_t to) {   // the next step
+    const bool in = kl < C;
 #pragma unroll
     for (int m = 0; m < 4; ++m)
       if (m < subs) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          unsigned char* d = slot(stage, m * 2 + i);
-          const bool there = x[m][i] && k < C;
-          if constexpr (WHOLE) copy_async<16>(d, there ? x[m][i] + k : p.x, there);
-          else *reinterpret_cast<uint4*>(d) = there ? load8<false>(x[m][i] + k, C - k) : make_uint4(0, 0, 0, 0);
+          if constexpr (WHOLE) copy_async<16>(to + (m * 2 + i) * 512, x[m][i], in ? xn[m][i] : 0);
+          else store16(to + (m * 2 + i) * 512, xn[m][i] ? load8<false>(x[m][i], C - kl) : make_uint4(0, 0, 0, 0));
+          x[m][i] += step;
         }
       }
     if constexpr (TALL) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {   // rows of pair j of every lane's 8
-        const int64_t kr = k0 + (g >> 1) * 8 + j * 2 + (g & 1);
-        const int rank = r0 + q * 2 * NT;
-        copy_few<2 * NT>(slot(stage, 8 + j * (D::kW / 4)), w + kr * p.r + rank, kr < C ? p.r - rank : 0, p.width, p.w);
-      }
+      for (int j = 0; j < 4; ++j)   // rows of pair j of every lane's 8
+        copy_few<2 * NT>(to + (8 + j * (D::kW / 4)) * 512, w + j * 2 * p.r, kr + 2 * j < C ? p.r - first : 0, p.width);
+      w += (int64_t)step * p.r;
+      kr += step;
     } else {
+      const T* v = w;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const int rank = r0 + (g >> 1) * 2 * NT + t * 2 + (g & 1);
-        unsigned char* d = slot(stage, 8 + t);
-        const bool there = rank < p.r && k < C;
-        if constexpr (WHOLE) copy_async<16>(d, there ? w + (int64_t)rank * C + k : p.w, there);
-        else *reinterpret_cast<uint4*>(d) = there ? load8<false>(w + (int64_t)rank * C + k, C - k) : make_uint4(0, 0, 0, 0);
+        const bool there = in && first + t * 2 < p.r;
+        if constexpr (WHOLE) copy_async<16>(to + (8 + t) * 512, v, there ? 16 : 0);
+        else store16(to + (8 + t) * 512, there ? load8<false>(v, C - kl) : make_uint4(0, 0, 0, 0));
+        v += 2 * C;
       }
+      w += step;
     }
+    kl += step;
   };
   float acc[4][NT][4] = {};
-  const int64_t step = (int64_t)p.split * kWarps * 32;
-  int64_t k = ((int64_t)part * kWarps + warp) * 32;
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
-    if (k + s * step < C) load(k + s * step, s);
+    if (k + s * step < C) load(ring + s * kStageBytes);
     commit();
   }
-  for (int stage = 0; k < C; k += step) {
-    const int64_t ahead = k + (kStages - 1) * step;
-    if (ahead < C) load(ahead, stage == 0 ? kStages - 1 : stage - 1);
+  uint32_t from = ring, to = ring + (kStages - 1) * kStageBytes;
+  const uint32_t end = ring + kStages * kStageBytes;
+  for (; k < C; k += step) {
+    if (k + (kStages - 1) * step < C) load(to);
     commit();
     wait_all_but<kStages - 1>();
     uint32_t b[NT][4];   // pair j of the lane's 8, of column tile t
@@ -257,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, NT == 8 ? 1 : 2) down_kernel(const P
       for (int j = 0; j < 4; ++j) {
 #pragma unroll
         for (int i = 0; i < (NT + 3) / 4; ++i) {
-          const uint4 v = *reinterpret_cast<const uint4*>(slot(stage, 8 + j * (D::kW / 4) + i));
+          const uint4 v = load16(from + (8 + j * (D::kW / 4) + i) * 512);
           b[i * 4][j] = transposed(v.x);
           b[i * 4 + 1][j] = transposed(v.y);
           if constexpr (NT > 2) {
@@ -269,24 +300,25 @@ __global__ void __launch_bounds__(kThreads, NT == 8 ? 1 : 2) down_kernel(const P
     } else {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const uint4 v = *reinterpret_cast<const uint4*>(slot(stage, 8 + t));
+        const uint4 v = load16(from + (8 + t) * 512);
         b[t][0] = v.x; b[t][1] = v.y; b[t][2] = v.z; b[t][3] = v.w;
       }
     }
 #pragma unroll
     for (int m = 0; m < 4; ++m)
       if (m < subs) {
-        const uint4 u = *reinterpret_cast<const uint4*>(slot(stage, m * 2)), v = *reinterpret_cast<const uint4*>(slot(stage, m * 2 + 1));
+        const uint4 u = load16(from + m * 1024), v = load16(from + m * 1024 + 512);
 #pragma unroll
         for (int t = 0; t < NT; ++t) mma<T>(acc[m][t], u.x, v.x, u.y, v.y, b[t][0], b[t][1]);
 #pragma unroll
         for (int t = 0; t < NT; ++t) mma<T>(acc[m][t], u.z, v.z, u.w, v.w, b[t][2], b[t][3]);
       }
-    stage = stage == kStages - 1 ? 0 : stage + 1;
+    to = from;
+    from = from + kStageBytes == end ? ring : from + kStageBytes;
   }
   wait_all_but<0>();
   __syncthreads();
-  float* red = reinterpret_cast<float*>(smem);   // [kWarps][kRows][kRanks]
+  float* red = reinterpret_cast<float*>(smem);   // [kWarps][kRows][kLine], columns as the products have them: 8 t + 2 q + (0, 1)
 #pragma unroll
   for (int m = 0; m < 4; ++m)
     if (m < subs) {
@@ -294,40 +326,47 @@ __global__ void __launch_bounds__(kThreads, NT == 8 ? 1 : 2) down_kernel(const P
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          *reinterpret_cast<float2*>(&red[(warp * kRows + m * 16 + i * 8 + g) * kRanks + q * 2 * NT + t * 2]) = make_float2(acc[m][t][2 * i], acc[m][t][2 * i + 1]);
+          *reinterpret_cast<float2*>(&red[(warp * kRows + m * 16 + i * 8 + g) * kLine + t * 8 + q * 2]) = make_float2(acc[m][t][2 * i], acc[m][t][2 * i + 1]);
     }
   __syncthreads();
-  const int pairs = tile.z * kRanks / 2;
+  constexpr int kPairs = kRanks / 2;   // per row
+  const int pairs = tile.z * kPairs;
   float2* red2 = reinterpret_cast<float2*>(red);
   for (int i = threadIdx.x; i < pairs; i += kThreads) {
-    float2 s = red2[i];
+    const int at = i / kPairs * (kLine / 2) + i % kPairs;
+    float2 s = red2[at];
 #pragma unroll
     for (int v = 1; v < kWarps; ++v) {
-      const float2 a = red2[v * kRows * kRanks / 2 + i];
+      const float2 a = red2[v * kRows * kLine / 2 + at];
       s.x += a.x;
       s.y += a.y;
     }
-    red2[i] = s;
+    red2[at] = s;
   }
-  cluster.sync();
+  if (p.split > 1) cluster.sync();
+  else __syncthreads();
   const float c = p.scales ? p.scales[tile.x] : 1.0f;
   for (int i = threadIdx.x * p.split + part; i < pairs; i += kThreads * p.split) {
-    float2 s = make_float2(0.0f, 0.0f);
-    for (int v = 0; v < p.split; ++v) {
-      const float2 a = cluster.map_shared_rank(red2, v)[i];
-      s.x += a.x;
-      s.y += a.y;
+    const int row = i / kPairs, pair = i % kPairs, at = row * (kLine / 2) + pair;
+    float2 s = red2[at];
+    if (p.split > 1) {
+      s = make_float2(0.0f, 0.0f);
+      for (int v = 0; v < p.split; ++v) {
+        const float2 a = cluster.map_shared_rank(red2, v)[at];
+        s.x += a.x;
+        s.y += a.y;
+      }
     }
-    const int rank = r0 + i % (kRanks / 2) * 2;
-    if (rank < p.r16) {   // (ranks from r on: their weights were zeros)
+    const int rank = r0 + pair % 4 * 2 * NT + pair / 4 * 2;
+    if (rank < p.r16) {
       uint32_t hi, lo;
       split(rank < p.r ? c * s.x : 0.0f, rank + 1 < p.r ? c * s.y : 0.0f, &hi, &lo);
-      uint16_t* h = p.h + (int64_t)(tile.y + i / (kRanks / 2)) * 2 * p.r16 + rank / 4 * 8 + rank % 4;
+      uint16_t* h = p.h + (int64_t)(tile.y + row) * 2 * p.r16 + rank / 4 * 8 + rank % 4;
       *reinterpret_cast<uint32_t*>(h) = hi;
       *reinterpret_cast<uint32_t*>(h + 4) = lo;
     }
   }
-  cluster.sync();   // no block leaves while others read its sums
+  if (p.split > 1) cluster.sync();   // no block leaves while others read its sums
 }
 
 // ---- out[row] = y[row] + (c) sum over ranks of h[place] w.  Blocks by (tiles, 256 columns), warps by 32 columns; steps of 16 rows and, inside, 16
@@ -335,67 +374,52 @@ __global__ void __launch_bounds__(kThreads, NT == 8 ? 1 : 2) down_kernel(const P
 // memory; more (CHUNKED) take both from the caches again for every 16 rows.
 // WIDE: weights [r, C], else [C, r].
 //
-// Bound by the latency of y: every lane copies its own pieces of it, three steps of rows ahead, into a ring in shared memory.
-constexpr int kUpStages = 4, kUpTiles = 8;
+// Bound by the latency of y: every lane copies its own pieces of it, three steps of rows ahead, into a ring in shared memory.  The steps' rows
+// are looked up once per block.
+constexpr int kUpStages = 4, kUpTiles = 8, kUpSteps = kUpTiles * kRows / 16;
 template <int KS>
 struct Up {
   static constexpr int kPitch = 64 * (KS | 1);   // bytes of h per row: eight lanes' 16-byte reads are in different banks
   static constexpr size_t kBytes = (size_t)kWarps * kUpStages * 1024 + 2 * kRows * kPitch;
 };
 template <typename T, bool WIDE, bool WHOLE, int KS, bool CHUNKED>
-__global__ void __launch_bounds__(kThreads, KS == 4 ? 2 : 3) up_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, (KS == 4 ? 2 : 3) - std::is_same_v<T, __half>) up_kernel(const Params p) {
   constexpr bool kSplitW = std::is_same_v<T, __half>;
   constexpr int kPitch = Up<KS>::kPitch;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int4 tiles[kUpTiles];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-  const int64_t C = p.C, blocks = (C + 255) / 256;
-  const int64_t n0 = (blockIdx.x % blocks) * 256 + warp * 32, n = n0 + q * 8;   // the lane's columns are n .. n + 7
-  const int64_t have = C - n;
-  const T* y = static_cast<const T*>(p.y);
-  T* out = static_cast<T*>(p.out);
+  __shared__ int rows[kUpSteps + kUpStages][16];   // of every step (-1: none); behind the last one some without any
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3, C = (int)p.C;
+  const int blocks = (C + 255) / 256, n0 = (int)(blockIdx.x % blocks) * 256 + warp * 32, n = n0 + q * 8;   // the lane's columns are n .. n + 7
+  const int have = C - n;
+  const bool in = have > 0, add = p.y != nullptr && in;
+  const T* y = static_cast<const T*>(p.y) + n;
+  T* out = static_cast<T*>(p.out) + n;
   if (threadIdx.x < kUpTiles) {
-    const int64_t k = blockIdx.x / blocks * p.each + threadIdx.x;
+    const int64_t k = (int64_t)(blockIdx.x / blocks) * p.each + threadIdx.x;
     int4 t = make_int4(-1, 0, 0, 0);
     if (threadIdx.x < p.each && k < p.tiles_n) t = tile_of(p, k);
     if (t.x < 0 && p.y == p.out) t.z = 0;   // rows without an adapter are there already
     tiles[threadIdx.x] = t;
   }
+  for (int i = threadIdx.x; i < (kUpSteps + kUpStages) * 16; i += kThreads) rows[i / 16][i % 16] = -1;
   __syncthreads();
-  unsigned char *ring = smem + warp * kUpStages * 1024 + lane * 16, *hs = smem + kWarps * kUpStages * 1024;
+  int steps = 0;
+  for (int k = 0; k < p.each; ++k) {
+    const int4 t = tiles[k];
+    for (int i = threadIdx.x; i < t.z; i += kThreads) rows[steps + i / 16][i % 16] = row_at(p, t.y + i);
+    steps += (t.z + 15) / 16;
+  }
+  const uint32_t ring = shared(smem) + warp * kUpStages * 1024 + lane * 16, hs = shared(smem) + kWarps * kUpStages * 1024;
   auto next_tile = [&](int k) {
     while (k < p.each && tiles[k].z == 0) ++k;
     return k;
-  };
-  // y of the steps ahead
-  int ik = next_tile(0), im = 0, stage_in = 0;
-  int64_t rows[2];
-  auto look = [&] {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) rows[i] = ik < p.each && im + i * 8 + g < tiles[ik].z ? row_at(p, tiles[ik].y + im + i * 8 + g) : -1;
-  };
-  auto issue = [&] {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      unsigned char* d = ring + stage_in * 1024 + i * 512;
-      const bool there = y != nullptr && rows[i] >= 0 && have > 0;
-      if constexpr (WHOLE) copy_async<16>(d, there ? y + rows[i] * C + n : p.out, there);
-      else *reinterpret_cast<uint4*>(d) = there ? load8<false, false>(y + rows[i] * C + n, have) : make_uint4(0, 0, 0, 0);
-    }
-    commit();
-    stage_in = stage_in == kUpStages - 1 ? 0 : stage_in + 1;
-    if (ik < p.each && (im += 16) >= tiles[ik].z) {
-      ik = next_tile(ik + 1);
-      im = 0;
-    }
-    look();
   };
   auto copy_h = [&](int k, int buffer) {
     if (CHUNKED || k >= p.each || tiles[k].x < 0) return;
     const int per_row = p.r16 / 4, n16 = tiles[k].z * per_row;   // pieces of 16 bytes
     const uint16_t* src = p.h + (int64_t)tiles[k].y * 2 * p.r16;
-    for (int i = threadIdx.x; i < n16; i += kThreads)
-      copy_async<16>(hs + (buffer * kRows + i / per_row) * kPitch + i % per_row * 16, src + i * 8, true);
+    for (int i = threadIdx.x; i < n16; i += kThreads) copy_async<16>(hs + (buffer * kRows + i / per_row) * kPitch + i % per_row * 16, src + i * 8, 16);
   };
   uint32_t bh[KS][4][2], bl[kSplitW ? KS : 1][4][2];   // rank step, column tile, pair of the lane's 4 ranks
   const T* w = nullptr;
@@ -413,9 +437,8 @@ __global__ void __launch_bounds__(kThreads, KS == 4 ? 2 : 3) up_kernel(const Par
       } else {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const int64_t col = n0 + (g >> 1) * 8 + t * 2 + (g & 1);
-          const int rank = r0 + s * 16 + q * 4;
-          load_few<4>(w + col * p.r + rank, col < C ? p.r - rank : 0, p.width, b[s][t]);
+          const int col = n0 + (g >> 1) * 8 + t * 2 + (g & 1), rank = r0 + s * 16 + q * 4;
+          load_few<4>(w + (int64_t)col * p.r + rank, col < C ? p.r - rank : 0, p.width, b[s][t]);
         }
       }
     }
@@ -430,13 +453,23 @@ __global__ void __launch_bounds__(kThreads, KS == 4 ? 2 : 3) up_kernel(const Par
           if constexpr (kSplitW) bl[s][t][j] = lo;
         }
   };
-  int k = ik, buffer = 0, loaded = -1, stage = 0;
-  look();
+  int k = next_tile(0), buffer = 0, loaded = -1, ahead = 0, now = 0;
+  auto issue = [&] {   // y of the next step
+    const uint32_t to = ring + (ahead % kUpStages) * 1024;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = rows[ahead][i * 8 + g];
+      if constexpr (WHOLE) copy_async<16>(to + i * 512, y + (int64_t)row * C, add && row >= 0 ? 16 : 0);
+      else store16(to + i * 512, add && row >= 0 ? load8<false, false>(y + (int64_t)row * C, have) : make_uint4(0, 0, 0, 0));
+    }
+    commit();
+    ++ahead;
+  };
   copy_h(k, 0);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < kUpStages - 1; ++i) issue();   // the first group has the first tile's h
-  bool short_tile = false;
-  for (bool start = true; k < p.each; start = false) {
+  for (int last = 4; k < p.each;) {
     const int4 tile = tiles[k];
     const bool plain = tile.x < 0;   // rows without an adapter
     float c = 0.0f;
@@ -449,17 +482,16 @@ __global__ void __launch_bounds__(kThreads, KS == 4 ? 2 : 3) up_kernel(const Par
       }
     }
     // the group with this tile's h was issued with the first step of the tile before, four steps ago if that was a whole one
-    if (start) wait_all_but<kUpStages - 2>();
-    else if (short_tile) wait_all_but<0>();
+    if (now == 0) wait_all_but<kUpStages - 2>();
+    else if (last < 4) wait_all_but<0>();
     __syncthreads();
     const int after = next_tile(k + 1);
     copy_h(after, buffer ^ 1);
-    short_tile = tile.z <= 48;
-    for (int m0 = 0; m0 < tile.z; m0 += 16) {
+    last = (tile.z + 15) / 16;
+    // (rows behind the tile's last one have what was there before; their products are not stored)
+    uint32_t src = hs + (buffer * kRows + g) * kPitch + q * 16;
+    for (int m = 0; m < last; ++m, ++now, src += 16 * kPitch) {
       issue();
-      int64_t at[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) at[i] = m0 + i * 8 + g < tile.z ? row_at(p, tile.y + m0 + i * 8 + g) : -1;
       float acc[4][4] = {};
       auto step = [&](int s, const uint4& h0, const uint4& h1) {
 #pragma unroll
@@ -480,41 +512,41 @@ __global__ void __launch_bounds__(kThreads, KS == 4 ? 2 : 3) up_kernel(const Par
               if (r0 + s * 16 >= p.r16) break;
               uint4 h[2];
 #pragma unroll
-              for (int i = 0; i < 2; ++i)
-                h[i] = m0 + i * 8 + g < tile.z ? *reinterpret_cast<const uint4*>(p.h + (int64_t)(tile.y + m0 + i * 8 + g) * 2 * p.r16 + (r0 + s * 16) * 2 + q * 8)
-                                               : make_uint4(0, 0, 0, 0);
+              for (int i = 0; i < 2; ++i) {
+                const int row = m * 16 + i * 8 + g;
+                h[i] = row < tile.z ? *reinterpret_cast<const uint4*>(p.h + (int64_t)(tile.y + row) * 2 * p.r16 + (r0 + s * 16) * 2 + q * 8) : make_uint4(0, 0, 0, 0);
+              }
               step(s, h[0], h[1]);
             }
           }
         } else {
-          // (rows behind the tile's last one have what was there before; their products are not stored)
-          const unsigned char* src = hs + (buffer * kRows + m0 + g) * kPitch + q * 16;
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
             if (KS > 1 && s * 16 >= p.r16) break;
-            step(s, *reinterpret_cast<const uint4*>(src + s * 64), *reinterpret_cast<const uint4*>(src + 8 * kPitch + s * 64));
+            step(s, load16(src + s * 64), load16(src + 8 * kPitch + s * 64));
           }
         }
       }
       wait_all_but<kUpStages - 1>();
+      const uint32_t from = ring + (now % kUpStages) * 1024;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (at[i] < 0 || have <= 0) continue;
-        T o[8];
-        *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(ring + stage * 1024 + i * 512);
-        if (!plain) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = Elem<T>::from_float(fmaf(c, acc[e / 2][2 * i + (e & 1)], Elem<T>::to_float(o[e])));
-        }
+        const int row = rows[now][i * 8 + g];
+        if (row < 0 || !in) continue;
+        const float sum[8] = {acc[0][2 * i], acc[0][2 * i + 1], acc[1][2 * i], acc[1][2 * i + 1], acc[2][2 * i], acc[2][2 * i + 1], acc[3][2 * i], acc[3][2 * i + 1]};
+        uint4 v = load16(from + i * 512);
+        if (!plain) v = add8<T>(v, c, sum);
+        T* o = out + (int64_t)row * C;
         if constexpr (WHOLE) {
-          *reinterpret_cast<uint4*>(out + at[i] * C + n) = *reinterpret_cast<const uint4*>(o);
+          *reinterpret_cast<uint4*>(o) = v;
         } else {
+          T e[8];
+          *reinterpret_cast<uint4*>(e) = v;
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < have) out[at[i] * C + n + e] = o[e];
+          for (int j = 0; j < 8; ++j)
+            if (j < have) o[j] = e[j];
         }
       }
-      stage = stage == kUpStages - 1 ? 0 : stage + 1;
     }
     buffer ^= 1;
     k = after;
@@ -526,39 +558,42 @@ __global__ void __launch_bounds__(kThreads, KS == 4 ? 2 : 3) up_kernel(const Par
 // cluster; warps by (32 columns, quarter of the rows).  TALL: out [C, r], else [r, C].
 template <typename T, bool TALL, bool WHOLE, int MT>
 __global__ void __launch_bounds__(kThreads) outer_kernel(const Params p) {
-  constexpr int kRanks = 16 * MT, kCols = 64, kLine = kCols + 4;
+  constexpr int kRanks = 16 * MT, kCols = 64, kLine = kCols + 8;
   extern __shared__ __align__(16) float red[];   // [4][kRanks][kLine]
   cg::cluster_group cluster = cg::this_cluster();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3, slot = warp >> 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3, slot = warp >> 1, C = (int)p.C;
   const int part = (int)(blockIdx.x % p.split), l = blockIdx.y, r0 = blockIdx.z * kRanks;
-  const int64_t C = p.C, c0 = (int64_t)(blockIdx.x / p.split) * kCols, col = c0 + (warp & 1) * 32 + q * 8;
-  const int64_t lo = max(p.starts[l], 0), hi = min((int64_t)p.starts[l + 1], p.T);
-  const T* x = static_cast<const T*>(p.x);
+  const int c0 = (int)(blockIdx.x / p.split) * kCols, col = c0 + (warp & 1) * 32 + q * 8, have = C - col;
+  const int lo = max(p.starts[l], 0), hi = min(p.starts[l + 1], (int)p.T);
+  const T* x = static_cast<const T*>(p.x) + col;
+  const int step = p.split * 64;
+  int t = lo + (part * 4 + slot) * 16;   // of the step that is multiplied
+  int place = t + g;                     // the lane's, of the step that is loaded
+  const uint16_t* h = p.h + (int64_t)place * 2 * p.r16 + r0 * 2 + q * 8;
   float acc[MT][4][4] = {};
   struct Stage {
     uint4 x[2];
     uint4 h[MT][2];   // rank step, place (+ 8): a lane's 4 ranks' high and low parts
   };
-  struct Index {
-    int64_t row[2];
-  };
-  auto index = [&](int64_t t0) {
-    Index v;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) v.row[i] = t0 + i * 8 + g < hi ? row_at(p, t0 + i * 8 + g) : -1;
-    return v;
-  };
-  auto load = [&](int64_t t0, const Index& at, Stage& s) {
+  int row[2];
+  auto look = [&](int at) {   // at: the lane's place
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t place = t0 + i * 8 + g;
-      s.x[i] = at.row[i] >= 0 ? load8<WHOLE>(x + at.row[i] * C + col, C - col) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int rank = r0 + m * 16;
-        s.h[m][i] = place < hi && rank < p.r16 ? *reinterpret_cast<const uint4*>(p.h + place * 2 * p.r16 + rank * 2 + q * 8) : make_uint4(0, 0, 0, 0);
-      }
+      row[i] = at + i * 8 < hi ? p.order[at + i * 8] : -1;
+      if (row[i] >= (int)p.T) row[i] = -1;
     }
+  };
+  auto load = [&](Stage& s) {   // the next step, whose rows have been looked up
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s.x[i] = row[i] >= 0 ? load8<WHOLE>(x + (int64_t)row[i] * C, have) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        s.h[m][i] = place + i * 8 < hi && (MT == 1 || r0 + m * 16 < p.r16) ? *reinterpret_cast<const uint4*>(h + i * 16 * p.r16 + m * 32) : make_uint4(0, 0, 0, 0);
+    }
+    place += step;
+    h += (int64_t)step * 2 * p.r16;
+    look(place);
   };
   auto multiply = [&](const Stage& s) {
     uint32_t bh[4][2], bl[4][2];
@@ -581,40 +616,35 @@ __global__ void __launch_bounds__(kThreads) outer_kernel(const Params p) {
         a[1][2 * i + 1] = transposed(s.h[m][i].w);
       }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[m][t], a[0][0], a[0][1], a[0][2], a[0][3], bh[t][0], bh[t][1]);
+      for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a[0][0], a[0][1], a[0][2], a[0][3], bh[v][0], bh[v][1]);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[m][t], a[1][0], a[1][1], a[1][2], a[1][3], bh[t][0], bh[t][1]);
+      for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a[1][0], a[1][1], a[1][2], a[1][3], bh[v][0], bh[v][1]);
       if constexpr (std::is_same_v<T, __half>) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[m][t], a[0][0], a[0][1], a[0][2], a[0][3], bl[t][0], bl[t][1]);
+        for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a[0][0], a[0][1], a[0][2], a[0][3], bl[v][0], bl[v][1]);
       }
     }
   };
-  const int64_t step = (int64_t)p.split * 64;
-  int64_t t = lo + ((int64_t)part * 4 + slot) * 16;
   Stage a, b;
-  Index at = index(t);
-  if (t < hi) load(t, at, a);
-  at = index(t + step);
+  look(place);
+  if (t < hi) load(a);
   while (t < hi) {
-    if (t + step < hi) load(t + step, at, b);
-    at = index(t + 2 * step);
+    if (t + step < hi) load(b);
     multiply(a);
     t += step;
     if (t >= hi) break;
-    if (t + step < hi) load(t + step, at, a);
-    at = index(t + 2 * step);
+    if (t + step < hi) load(a);
     multiply(b);
     t += step;
   }
+  // rows and columns as the products have them: 16 m + 8 i + g is rank 16 m + 4 (g / 2) + 2 i + g % 2, 32 half + 8 v + 2 q is column 32 half + 8 q + 2 v
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int v = 0; v < 4; ++v)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<float2*>(&red[(slot * kRanks + m * 16 + (g >> 1) * 4 + i * 2 + (g & 1)) * kLine + (warp & 1) * 32 + q * 8 + t * 2]) =
-            make_float2(acc[m][t][2 * i], acc[m][t][2 * i + 1]);
+        *reinterpret_cast<float2*>(&red[(slot * kRanks + m * 16 + i * 8 + g) * kLine + (warp & 1) * 32 + v * 8 + q * 2]) = make_float2(acc[m][v][2 * i], acc[m][v][2 * i + 1]);
   __syncthreads();
   for (int i = threadIdx.x; i < kRanks * kCols; i += kThreads) {
     const int at = i / kCols * kLine + i % kCols;
@@ -623,17 +653,22 @@ __global__ void __launch_bounds__(kThreads) outer_kernel(const Params p) {
     for (int v = 1; v < 4; ++v) s += red[v * kRanks * kLine + at];
     red[at] = s;
   }
-  cluster.sync();
+  if (p.split > 1) cluster.sync();
+  else __syncthreads();
   const float c = p.scales ? p.scales[l] : 1.0f;
   T* out = static_cast<T*>(p.out) + (int64_t)l * p.r * C;
   const int each = kRanks * kCols / p.split;   // of the tile's elements: this block's
   for (int i = threadIdx.x; i < each; i += kThreads) {
     const int e = part * each + i, rank = TALL ? e % kRanks : e / kCols, cc = TALL ? e / kRanks : e % kCols;
-    float s = 0.0f;
-    for (int v = 0; v < p.split; ++v) s += cluster.map_shared_rank(red, v)[rank * kLine + cc];
-    if (r0 + rank < p.r && c0 + cc < C) out[TALL ? (c0 + cc) * p.r + r0 + rank : (int64_t)(r0 + rank) * C + c0 + cc] = Elem<T>::from_float(c * s);
+    const int at = (rank / 16 * 16 + rank / 2 % 2 * 8 + rank / 4 % 4 * 2 + rank % 2) * kLine + cc / 32 * 32 + cc / 2 % 4 * 8 + cc / 8 % 4 * 2 + cc % 2;
+    float s = red[at];
+    if (p.split > 1) {
+      s = 0.0f;
+      for (int v = 0; v < p.split; ++v) s += cluster.map_shared_rank(red, v)[at];
+    }
+    if (r0 + rank < p.r && c0 + cc < C) out[TALL ? (int64_t)(c0 + cc) * p.r + r0 + rank : (int64_t)(r0 + rank) * C + c0 + cc] = Elem<T>::from_float(c * s);
   }
-  cluster.sync();
+  if (p.split > 1) cluster.sync();
 }
 
 bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -653,7 +688,7 @@ int split_of(int64_t blocks, int64_t slots, int64_t most) {
 int64_t likely_tiles(const Params& p) { return std::min<int64_t>(p.T, p.T / kRows + (std::min<int64_t>(p.T, p.L) + 1) / 2); }
 
 template <typename K>
-int launch(K kern, const Params& p, dim3 grid, size_t smem, bool cluster, cudaStream_t st) {
+int launch(K kern, const Params& p, dim3 grid, size_t smem, cudaStream_t st) {
   if (smem > 48 * 1024) B200Q_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
@@ -661,7 +696,7 @@ int launch(K kern, const Params& p, dim3 grid, size_t smem, bool cluster, cudaSt
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
-  if (cluster) {
+  if (p.split > 1) {
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = p.split;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
@@ -678,19 +713,20 @@ int down(Params p, cudaStream_t st) {
   const int nt = p.r <= 16 ? 2 : (p.r <= 32 ? 4 : 8), chunks = (p.r + 8 * nt - 1) / (8 * nt);
   p.split = split_of(likely_tiles(p) * chunks, 148 * (nt == 8 ? 1 : 2), p.C / (kWarps * 32));
   const dim3 grid((unsigned)(p.tiles_n * p.split), chunks);
-  if (nt == 2) return launch(down_kernel<T, TALL, WHOLE, 2>, p, grid, Down<TALL, 2>::kBytes, true, st);
-  if (nt == 4) return launch(down_kernel<T, TALL, WHOLE, 4>, p, grid, Down<TALL, 4>::kBytes, true, st);
-  return launch(down_kernel<T, TALL, WHOLE, 8>, p, grid, Down<TALL, 8>::kBytes, true, st);
+  if (nt == 2) return launch(down_kernel<T, TALL, WHOLE, 2>, p, grid, Down<TALL, 2>::kBytes, st);
+  if (nt == 4) return launch(down_kernel<T, TALL, WHOLE, 4>, p, grid, Down<TALL, 4>::kBytes, st);
+  return launch(down_kernel<T, TALL, WHOLE, 8>, p, grid, Down<TALL, 8>::kBytes, st);
 }
 template <typename T, bool WIDE, bool WHOLE>
 int up(Params p, cudaStream_t st) {
+  p.split = 1;
   const int64_t cols = (p.C + 255) / 256;
   p.each = (int)std::max<int64_t>(1, std::min<int64_t>(kUpTiles, p.tiles_n * cols / (148 * 8)));   // a block's tiles share their weights' loads
   const dim3 grid((unsigned)((p.tiles_n + p.each - 1) / p.each * cols));
-  if (p.r <= 16) return launch(up_kernel<T, WIDE, WHOLE, 1, false>, p, grid, Up<1>::kBytes, false, st);
-  if (p.r <= 32) return launch(up_kernel<T, WIDE, WHOLE, 2, false>, p, grid, Up<2>::kBytes, false, st);
-  if (p.r <= 64) return launch(up_kernel<T, WIDE, WHOLE, 4, false>, p, grid, Up<4>::kBytes, false, st);
-  return launch(up_kernel<T, WIDE, WHOLE, 4, true>, p, grid, kWarps * kUpStages * 1024, false, st);
+  if (p.r <= 16) return launch(up_kernel<T, WIDE, WHOLE, 1, false>, p, grid, Up<1>::kBytes, st);
+  if (p.r <= 32) return launch(up_kernel<T, WIDE, WHOLE, 2, false>, p, grid, Up<2>::kBytes, st);
+  if (p.r <= 64) return launch(up_kernel<T, WIDE, WHOLE, 4, false>, p, grid, Up<4>::kBytes, st);
+  return launch(up_kernel<T, WIDE, WHOLE, 4, true>, p, grid, kWarps * kUpStages * 1024, st);
 }
 template <typename T, bool TALL, bool WHOLE>
 int outer(Params p, cudaStream_t st) {
@@ -698,10 +734,10 @@ int outer(Params p, cudaStream_t st) {
   const int64_t cols = (p.C + 63) / 64;
   p.split = split_of(cols * p.L * chunks, 148 * 4, p.T / 64);
   const dim3 grid((unsigned)(cols * p.split), p.L, chunks);
-  const size_t smem = (size_t)4 * 16 * mt * 68 * 4;
-  if (mt == 1) return launch(outer_kernel<T, TALL, WHOLE, 1>, p, grid, smem, true, st);
-  if (mt == 2) return launch(outer_kernel<T, TALL, WHOLE, 2>, p, grid, smem, true, st);
-  return launch(outer_kernel<T, TALL, WHOLE, 4>, p, grid, smem, true, st);
+  const size_t smem = (size_t)4 * 16 * mt * 72 * 4;
+  if (mt == 1) return launch(outer_kernel<T, TALL, WHOLE, 1>, p, grid, smem, st);
+  if (mt == 2) return launch(outer_kernel<T, TALL, WHOLE, 2>, p, grid, smem, st);
+  return launch(outer_kernel<T, TALL, WHOLE, 4>, p, grid, smem, st);
 }
 
 // Of a call: which form of a kernel.
@@ -729,8 +765,8 @@ int run(Step step, Params p, int dtype, cudaStream_t st) {
 int check(const char* tag, int dtype, int64_t T, int64_t L, int64_t N, int64_t K, int64_t r) {
   if (dtype != B200Q_F16 && dtype != B200Q_BF16) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] unsupported dtype code %d", tag, dtype);
   if (T < 0 || L < 0 || N < 0 || K < 0 || r < 0) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] negative dimension.", tag);
-  if (T > INT32_MAX - 64 || L > 4096 || N > (1 << 24) || K > (1 << 24) || r > 4096)
-    return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than 2^31 - 65 rows, 4096 adapters, widths of 2^24 or ranks of 4096.", tag);
+  if (T > (1 << 30) || L > 4096 || N > (1 << 24) || K > (1 << 24) || r > 4096)
+    return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than 2^30 rows, 4096 adapters, widths of 2^24 or ranks of 4096.", tag);
   const int64_t tiles = b200q_group_rows_tiles(T, L), most = INT32_MAX;
   if (tiles * 8 > most || tiles > most / ((N + 255) / 256 + 1) || tiles > most / ((K + 255) / 256 + 1))
     return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than 2^31 - 1 blocks.", tag);
@@ -760,6 +796,7 @@ extern "C" int b200q_add_adapters(const void* y, const void* x, const void* a, c
     if (!aligned(q, 2)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
   if (!aligned(tiles, 16) || !aligned(h, 16)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] tiles and h must be 16-byte aligned", tag);
   Params p{};
+  p.split = 1;
   p.x = x; p.w = a; p.h = static_cast<uint16_t*>(h); p.r16 = (int)(r + 15) / 16 * 16;
   p.order = order; p.tiles = reinterpret_cast<const int4*>(tiles); p.tiles_n = b200q_group_rows_tiles(T, L);
   p.T = T; p.C = K; p.L = (int)L; p.r = (int)r;
@@ -787,6 +824,7 @@ extern "C" int b200q_add_adapters_grad(const void* dy, const void* x, const void
     if (!aligned(q, 2)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
   if (!aligned(tiles, 16) || !aligned(h, 16) || !aligned(g, 16)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] tiles, h and g must be 16-byte aligned", tag);
   Params p{};
+  p.split = 1;
   p.h = static_cast<uint16_t*>(g); p.r16 = (int)(r + 15) / 16 * 16;
   p.order = order; p.starts = starts; p.tiles = reinterpret_cast<const int4*>(tiles); p.tiles_n = b200q_group_rows_tiles(T, L);
   p.T = T; p.L = (int)L; p.r = (int)r;

@@ -698,8 +698,8 @@ extern "C" int b200q_group_rows(const void* ids, int id_bytes, int64_t T, int64_
   if (T < 0 || n < 0) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] negative dimension.", tag);
   if ((id_bytes != 4 && id_bytes != 8) || (ids && reinterpret_cast<uintptr_t>(ids) % id_bytes != 0))
     return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] ids are aligned 4- or 8-byte integers", tag);
-  if (T > kMostPairs - 64 || n > kMostRowGroups)
-    return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than 2^31 - 65 rows or %lld groups.", tag, (long long)kMostRowGroups);
+  if (T > (1 << 30) || n > kMostRowGroups)
+    return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than 2^30 rows or %lld groups.", tag, (long long)kMostRowGroups);
   if (!starts || (n > 0 && !sizes)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (T == 0) {
