@@ -16,6 +16,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "common.cuh"
@@ -55,12 +56,16 @@ __device__ __forceinline__ void split(float a, float b, uint32_t* hi, uint32_t* 
   *hi = pack(fa, fb);
   *lo = pack(isinf(fa) ? 0.0f : a - fa, isinf(fb) ? 0.0f : b - fb);
 }
-// A pair of T as bf16 numbers: itself, or (f16) high and low part.
+// A pair of T as bf16 numbers: itself, or (f16) high and low part: the upper 8 bits of the 11, and the rest, exactly (0 of what is not finite).
 template <typename T>
 __device__ __forceinline__ void as_bf16(uint32_t v, uint32_t* hi, uint32_t* lo) {
   if constexpr (std::is_same_v<T, __half>) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
-    split(f.x, f.y, hi, lo);
+    const __half2 h = *reinterpret_cast<const __half2*>(&v);
+    const float2 f = __half22float2(h);
+    const uint32_t a = __float_as_uint(f.x), b = __float_as_uint(f.y);
+    *hi = __byte_perm(a, b, 0x7632);
+    const float la = f.x - __uint_as_float(a & 0xffff0000u), lb = f.y - __uint_as_float(b & 0xffff0000u);
+    *lo = __byte_perm(__float_as_uint(la), __float_as_uint(lb), 0x7632) & __hlt2_mask(__habs2(h), __half2half2(__ushort_as_half(0x7c00)));
   } else {
     *hi = v;
     *lo = 0;
@@ -113,11 +118,13 @@ __device__ __forceinline__ void load_few(const T* p, int64_t have, int width, ui
 }
 
 __device__ __forceinline__ uint32_t shared(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// BYTES (4, 8, 16) to shared memory, asynchronously; of them the first n (0: p is not read) from p on, then zeros.
+// BYTES (4, 8, 16) to shared memory, asynchronously; zeros where there is nothing (p is not read then).
 template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* p, int n) {
-  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p), "r"(n) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(p), "n"(BYTES), "r"(n) : "memory");
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* p, bool there) {
+  if constexpr (BYTES == 16)
+    asm volatile("{\n.reg .pred none;\nsetp.eq.s32 none, %2, 0;\ncp.async.cg.shared.global [%0], [%1], 16, none;\n}" ::"r"(dst), "l"(p), "r"((int)there) : "memory");
+  else
+    asm volatile("{\n.reg .pred none;\nsetp.eq.s32 none, %3, 0;\ncp.async.ca.shared.global [%0], [%1], %2, none;\n}" ::"r"(dst), "l"(p), "n"(BYTES), "r"((int)there) : "memory");
 }
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -128,13 +135,13 @@ __device__ __forceinline__ void copy_few(uint32_t dst, const T* p, int have, int
   const char* q = reinterpret_cast<const char*>(p);
   if (N >= 8 && width == 16) {
 #pragma unroll
-    for (int i = 0; i < N / 8; ++i) copy_async<16>(dst + 512 * i, q + 16 * i, 8 * i < have ? 16 : 0);
+    for (int i = 0; i < N / 8; ++i) copy_async<16>(dst + 512 * i, q + 16 * i, 8 * i < have);
   } else if (width >= 8) {
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) copy_async<8>(dst + 512 * (i / 2) + 8 * (i & 1), q + 8 * i, 4 * i < have ? 8 : 0);
+    for (int i = 0; i < N / 4; ++i) copy_async<8>(dst + 512 * (i / 2) + 8 * (i & 1), q + 8 * i, 4 * i < have);
   } else if (width == 4) {
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) copy_async<4>(dst + 512 * (i / 4) + 4 * (i & 3), q + 4 * i, 2 * i < have ? 4 : 0);
+    for (int i = 0; i < N / 2; ++i) copy_async<4>(dst + 512 * (i / 4) + 4 * (i & 3), q + 4 * i, 2 * i < have);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -150,6 +157,14 @@ __device__ __forceinline__ void store16(uint32_t dst, const uint4& v) {
 __device__ __forceinline__ uint4 load16(uint32_t src) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
+  return v;
+}
+// Four 8 x 8 matrices of 16-bit values, lane 8 i + j naming row j of the i-th: lane (g, q) gets (g, 2q) and (g, 2q + 1) of each, TRANS: (2q, g), (2q + 1, g).
+template <bool TRANS>
+__device__ __forceinline__ uint4 load_matrices(uint32_t row) {
+  uint4 v;
+  if constexpr (TRANS) asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(row) : "memory");
+  else asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(row) : "memory");
   return v;
 }
 // a + c * b for eight values of T
@@ -198,22 +213,24 @@ __device__ __forceinline__ int row_at(const Params& p, int64_t place) {
   return row < (int)p.T ? row : -1;
 }
 
-// ---- h[place] = (c) sum over the long dimension of x[row] w.  Blocks by (tile, part of the long dimension, 8 NT ranks); the parts are a cluster
-// whose blocks add up their sums through distributed shared memory.  Warps take every 64th (of their cluster) 32 columns of x.
+// ---- h[place] = (c) sum over the long dimension of x[row] w.  Blocks by (tile, part of the long dimension, 16 MT ranks); the parts are a cluster
+// whose blocks add up their sums through distributed shared memory.  Warps take every 8th (of their cluster: 8 split-th) 32 columns of x.
+// Ranks are the rows of the products and activations their columns: a column's operands are two registers out of one 16-byte load, where a
+// row's would have to be brought together from two.
 // TALL: weights [C, r], else [r, C].
 //
-// Bound by the latency of its loads.  They go through a ring in shared memory, several steps ahead; every lane copies and reads its own
-// 16-byte pieces only, so that the ring needs no barrier, just the lane's own count of finished copies.
-template <bool TALL, int NT>
+// Bound by the latency of its loads (with 64 ranks: by the products, too).  Every warp has a ring of its own in shared memory, filled some steps
+// ahead, in pieces of 16 bytes whose places are swizzled so that eight rows of a matrix are in different banks; no barrier but the warp's.
+template <bool TALL, int MT>
 struct Down {
-  static constexpr int kRanks = 8 * NT, kW = TALL ? (NT == 8 ? 8 : 4) : NT, kPieces = 8 + kW, kStages = NT == 8 ? 3 : 2;
-  static constexpr int kLine = kRanks + 8;   // floats per row of the sums: lanes' pairs are in different banks
-  static constexpr size_t kBytes = (size_t)kWarps * kStages * kPieces * 512;
-  static_assert(kBytes >= (size_t)kWarps * kRows * kLine * 4, "the sums lie where the ring was");
+  static constexpr int kRanks = 16 * MT, kW = 2 * MT, kPieces = 8 + kW, kStages = MT == 4 ? 3 : 2;
+  static constexpr int kLine = kRows + 8;   // floats per rank of the sums: lanes' pairs are in different banks
+  static constexpr size_t kRing = (size_t)kWarps * kStages * kPieces * 512, kSums = (size_t)kWarps * kRanks * kLine * 4;
+  static constexpr size_t kBytes = kRing > kSums ? kRing : kSums;   // the sums lie where the ring was
 };
-template <typename T, bool TALL, bool WHOLE, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 8 ? 1 : 2) down_kernel(const Params p) {
-  using D = Down<TALL, NT>;
+template <typename T, bool TALL, bool WHOLE, int MT>
+__global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) down_kernel(const Params p) {
+  using D = Down<TALL, MT>;
   constexpr int kRanks = D::kRanks, kStages = D::kStages, kLine = D::kLine, kStageBytes = D::kPieces * 512;
   extern __shared__ __align__(16) unsigned char smem[];
   cg::cluster_group cluster = cg::this_cluster();
@@ -221,146 +238,139 @@ __global__ void __launch_bounds__(kThreads, NT == 8 ? 1 : 2) down_kernel(const P
   const int part = (int)(blockIdx.x % p.split);
   const int4 tile = tile_of(p, blockIdx.x / p.split);
   if (tile.z == 0 || tile.x < 0) return;   // the whole cluster
-  const int subs = (tile.z + 15) / 16, r0 = blockIdx.y * kRanks, C = (int)p.C, step = p.split * kWarps * 32;
+  const int eights = (tile.z + 7) / 8, r0 = blockIdx.y * kRanks, C = (int)p.C, step = p.split * kWarps * 32;
   int k = (part * kWarps + warp) * 32;     // of the step that is multiplied
+  // Rows along the long dimension (x, weights [r, C]) are copied eight at a time, 8 k per lane: lane (g, q) has k 8 q of row g, which goes to
+  // piece 4 g + (q ^ g / 2) of the eight rows' 32.
   int kl = k + q * 8;                      // the lane's, of the step that is loaded
-  const T* x[4][2];
-  int xn[4][2];   // bytes to copy: 0 where there is no row
+  const uint32_t own = (g * 4 + (q ^ (g >> 1))) * 16;
+  const T* x[8];
+  bool has[8];
 #pragma unroll
-  for (int m = 0; m < 4; ++m)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = m * 16 + i * 8 + g, at = row < tile.z ? row_at(p, tile.y + row) : -1;
-      x[m][i] = static_cast<const T*>(p.x) + (int64_t)max(at, 0) * C + kl;
-      xn[m][i] = at < 0 ? 0 : 16;
-    }
+  for (int n = 0; n < 8; ++n) {
+    const int row = n * 8 + g, at = row < tile.z ? row_at(p, tile.y + row) : -1;
+    x[n] = static_cast<const T*>(p.x) + (int64_t)max(at, 0) * C + kl;
+    has[n] = at >= 0;
+  }
+  // TALL: 32 rows of 2 MT pieces, one after the other, piece c of row i at c ^ tall(i).
+  auto tall = [](int i) { return MT == 4 ? i & 7 : (MT == 2 ? i >> 1 & 3 : i >> 2 & 1); };
   const T* w = static_cast<const T*>(p.w) + (int64_t)tile.x * p.r * C;
-  const int first = r0 + (TALL ? q * 2 * NT : (g >> 1) * 2 * NT + (g & 1));   // the lane's first rank
-  int kr = k + (g >> 1) * 8 + (g & 1);
-  w += TALL ? (int64_t)kr * p.r + first : (int64_t)first * C + kl;
-  const uint32_t ring = shared(smem) + warp * kStages * kStageBytes + lane * 16;
+  int kw = k;                              // TALL: of the step that is loaded
+  if constexpr (!TALL) w += (int64_t)(r0 + g) * C + kl;
+  const uint32_t ring = shared(smem) + warp * kStages * kStageBytes;
   auto load = [&](uint32_t to) {   // the next step
     const bool in = kl < C;
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
-      if (m < subs) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if constexpr (WHOLE) copy_async<16>(to + (m * 2 + i) * 512, x[m][i], in ? xn[m][i] : 0);
-          else store16(to + (m * 2 + i) * 512, xn[m][i] ? load8<false>(x[m][i], C - kl) : make_uint4(0, 0, 0, 0));
-          x[m][i] += step;
-        }
+    for (int n = 0; n < 8; ++n)
+      if (n < eights) {
+        if constexpr (WHOLE) copy_async<16>(to + n * 512 + own, x[n], in && has[n]);
+        else store16(to + n * 512 + own, has[n] ? load8<false>(x[n], C - kl) : make_uint4(0, 0, 0, 0));
+        x[n] += step;
       }
     if constexpr (TALL) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)   // rows of pair j of every lane's 8
-        copy_few<2 * NT>(to + (8 + j * (D::kW / 4)) * 512, w + j * 2 * p.r, kr + 2 * j < C ? p.r - first : 0, p.width);
-      w += (int64_t)step * p.r;
-      kr += step;
+      for (int i = 0; i < 2 * MT; ++i) {
+        const int row = (i * 32 + lane) / (2 * MT), c = lane % (2 * MT), rank = r0 + c * 8;
+        copy_few<8>(to + 4096 + (row * 2 * MT + (c ^ tall(row))) * 16, w + (int64_t)(kw + row) * p.r + rank, kw + row < C ? p.r - rank : 0, p.width);
+      }
+      kw += step;
     } else {
       const T* v = w;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const bool there = in && first + t * 2 < p.r;
-        if constexpr (WHOLE) copy_async<16>(to + (8 + t) * 512, v, there ? 16 : 0);
-        else store16(to + (8 + t) * 512, there ? load8<false>(v, C - kl) : make_uint4(0, 0, 0, 0));
-        v += 2 * C;
+      for (int t = 0; t < 2 * MT; ++t) {
+        const bool there = in && r0 + t * 8 + g < p.r;
+        if constexpr (WHOLE) copy_async<16>(to + 4096 + t * 512 + own, v, there);
+        else store16(to + 4096 + t * 512 + own, there ? load8<false>(v, C - kl) : make_uint4(0, 0, 0, 0));
+        v += 8 * C;
       }
       w += step;
     }
     kl += step;
   };
-  float acc[4][NT][4] = {};
+  float acc[MT][8][4] = {};
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
     if (k + s * step < C) load(ring + s * kStageBytes);
     commit();
   }
+  // Rows that the lane names: of x, 8 k per matrix; of weights [r, C], two times eight ranks by two times 8 k; of TALL ones, 16 k by two times eight ranks.
+  const int mr = lane & 7, mi = lane >> 3;
+  const uint32_t x_row = (mr * 4 + (mi ^ (mr >> 1))) * 16;
+  const uint32_t w_row[2] = {4096u + (mi & 1) * 512 + (mr * 4 + ((mi >> 1) ^ (mr >> 1))) * 16, 4096u + (mi & 1) * 512 + (mr * 4 + ((mi >> 1 | 2) ^ (mr >> 1))) * 16};
   uint32_t from = ring, to = ring + (kStages - 1) * kStageBytes;
   const uint32_t end = ring + kStages * kStageBytes;
   for (; k < C; k += step) {
+    __syncwarp();   // everyone has read the stage that is filled now
     if (k + (kStages - 1) * step < C) load(to);
     commit();
     wait_all_but<kStages - 1>();
-    uint32_t b[NT][4];   // pair j of the lane's 8, of column tile t
-    if constexpr (TALL) {
+    __syncwarp();
+    uint4 a[MT][2];   // of the first and the second 16 k
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < (NT + 3) / 4; ++i) {
-          const uint4 v = load16(from + (8 + j * (D::kW / 4) + i) * 512);
-          b[i * 4][j] = transposed(v.x);
-          b[i * 4 + 1][j] = transposed(v.y);
-          if constexpr (NT > 2) {
-            b[(i * 4 + 2) % NT][j] = transposed(v.z);
-            b[(i * 4 + 3) % NT][j] = transposed(v.w);
-          }
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (TALL) {
+          const int row = h * 16 + (mi >> 1) * 8 + mr;
+          a[m][h] = load_matrices<true>(from + 4096 + (row * 2 * MT + ((2 * m + (mi & 1)) ^ tall(row))) * 16);
+        } else {
+          a[m][h] = load_matrices<false>(from + m * 1024 + w_row[h]);
         }
       }
-    } else {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const uint4 v = load16(from + (8 + t) * 512);
-        b[t][0] = v.x; b[t][1] = v.y; b[t][2] = v.z; b[t][3] = v.w;
-      }
-    }
+    for (int n = 0; n < 8; ++n)
+      if (n < eights) {
+        const uint4 v = load_matrices<false>(from + n * 512 + x_row);
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
-      if (m < subs) {
-        const uint4 u = load16(from + m * 1024), v = load16(from + m * 1024 + 512);
+        for (int m = 0; m < MT; ++m) mma<T>(acc[m][n], a[m][0].x, a[m][0].y, a[m][0].z, a[m][0].w, v.x, v.y);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) mma<T>(acc[m][t], u.x, v.x, u.y, v.y, b[t][0], b[t][1]);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) mma<T>(acc[m][t], u.z, v.z, u.w, v.w, b[t][2], b[t][3]);
+        for (int m = 0; m < MT; ++m) mma<T>(acc[m][n], a[m][1].x, a[m][1].y, a[m][1].z, a[m][1].w, v.z, v.w);
       }
     to = from;
     from = from + kStageBytes == end ? ring : from + kStageBytes;
   }
   wait_all_but<0>();
   __syncthreads();
-  float* red = reinterpret_cast<float*>(smem);   // [kWarps][kRows][kLine], columns as the products have them: 8 t + 2 q + (0, 1)
+  float* red = reinterpret_cast<float*>(smem);   // [kWarps][kRanks][kLine]
 #pragma unroll
-  for (int m = 0; m < 4; ++m)
-    if (m < subs) {
+  for (int n = 0; n < 8; ++n)
+    if (n < eights) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          *reinterpret_cast<float2*>(&red[(warp * kRows + m * 16 + i * 8 + g) * kLine + t * 8 + q * 2]) = make_float2(acc[m][t][2 * i], acc[m][t][2 * i + 1]);
+          *reinterpret_cast<float2*>(&red[(warp * kRanks + m * 16 + i * 8 + g) * kLine + n * 8 + q * 2]) = make_float2(acc[m][n][2 * i], acc[m][n][2 * i + 1]);
     }
   __syncthreads();
-  constexpr int kPairs = kRanks / 2;   // per row
-  const int pairs = tile.z * kPairs;
-  float2* red2 = reinterpret_cast<float2*>(red);
-  for (int i = threadIdx.x; i < pairs; i += kThreads) {
-    const int at = i / kPairs * (kLine / 2) + i % kPairs;
-    float2 s = red2[at];
+  // sums over the block's warps, then over the cluster's blocks; two ranks of a row per thread, rows next to each other
+  const int n = kRanks / 2 * (eights * 8);
+  auto at = [&](int i) { return i / (eights * 8) * 2 * kLine + i % (eights * 8); };
+  for (int i = threadIdx.x; i < n; i += kThreads) {
 #pragma unroll
-    for (int v = 1; v < kWarps; ++v) {
-      const float2 a = red2[v * kRows * kLine / 2 + at];
-      s.x += a.x;
-      s.y += a.y;
+    for (int e = 0; e < 2; ++e) {
+      float s = red[at(i) + e * kLine];
+#pragma unroll
+      for (int v = 1; v < kWarps; ++v) s += red[v * kRanks * kLine + at(i) + e * kLine];
+      red[at(i) + e * kLine] = s;
     }
-    red2[at] = s;
   }
   if (p.split > 1) cluster.sync();
   else __syncthreads();
   const float c = p.scales ? p.scales[tile.x] : 1.0f;
-  for (int i = threadIdx.x * p.split + part; i < pairs; i += kThreads * p.split) {
-    const int row = i / kPairs, pair = i % kPairs, at = row * (kLine / 2) + pair;
-    float2 s = red2[at];
+  for (int i = threadIdx.x * p.split + part; i < n; i += kThreads * p.split) {
+    float s[2] = {red[at(i)], red[at(i) + kLine]};
     if (p.split > 1) {
-      s = make_float2(0.0f, 0.0f);
+      s[0] = s[1] = 0.0f;
       for (int v = 0; v < p.split; ++v) {
-        const float2 a = cluster.map_shared_rank(red2, v)[at];
-        s.x += a.x;
-        s.y += a.y;
+        const float* other = cluster.map_shared_rank(red, v);
+        s[0] += other[at(i)];
+        s[1] += other[at(i) + kLine];
       }
     }
-    const int rank = r0 + pair % 4 * 2 * NT + pair / 4 * 2;
-    if (rank < p.r16) {
+    const int row = i % (eights * 8), rank = r0 + i / (eights * 8) * 2;
+    if (rank < p.r16 && row < tile.z) {
       uint32_t hi, lo;
-      split(rank < p.r ? c * s.x : 0.0f, rank + 1 < p.r ? c * s.y : 0.0f, &hi, &lo);
+      split(rank < p.r ? c * s[0] : 0.0f, rank + 1 < p.r ? c * s[1] : 0.0f, &hi, &lo);
       uint16_t* h = p.h + (int64_t)(tile.y + row) * 2 * p.r16 + rank / 4 * 8 + rank % 4;
       *reinterpret_cast<uint32_t*>(h) = hi;
       *reinterpret_cast<uint32_t*>(h + 4) = lo;
@@ -374,18 +384,19 @@ __global__ void __launch_bounds__(kThreads, NT == 8 ? 1 : 2) down_kernel(const P
 // memory; more (CHUNKED) take both from the caches again for every 16 rows.
 // WIDE: weights [r, C], else [C, r].
 //
-// Bound by the latency of y: every lane copies its own pieces of it, three steps of rows ahead, into a ring in shared memory.  The steps' rows
-// are looked up once per block.
+// Bound by the latency of y and by instructions: every lane copies its own pieces of y, three steps of rows ahead, into a ring in shared memory; the steps'
+// rows are looked up once per block; h lies in shared memory as the products' operands want it, so that one load brings four registers that are next to each
+// other (two rows loaded apart would have to be moved together for every product: half of all instructions).
 constexpr int kUpStages = 4, kUpTiles = 8, kUpSteps = kUpTiles * kRows / 16;
-template <int KS>
+template <int KS, bool CHUNKED>
 struct Up {
-  static constexpr int kPitch = 64 * (KS | 1);   // bytes of h per row: eight lanes' 16-byte reads are in different banks
-  static constexpr size_t kBytes = (size_t)kWarps * kUpStages * 1024 + 2 * kRows * kPitch;
+  static constexpr int kStep = KS * 1024;   // bytes of h per step of 16 rows: [rank step][part][lane][4]
+  static constexpr size_t kBytes = (size_t)kWarps * kUpStages * 1024 + (CHUNKED ? 0 : 8 * kStep);
 };
 template <typename T, bool WIDE, bool WHOLE, int KS, bool CHUNKED>
 __global__ void __launch_bounds__(kThreads, (KS == 4 ? 2 : 3) - std::is_same_v<T, __half>) up_kernel(const Params p) {
   constexpr bool kSplitW = std::is_same_v<T, __half>;
-  constexpr int kPitch = Up<KS>::kPitch;
+  constexpr int kStep = Up<KS, CHUNKED>::kStep;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int4 tiles[kUpTiles];
   __shared__ int rows[kUpSteps + kUpStages][16];   // of every step (-1: none); behind the last one some without any
@@ -417,9 +428,22 @@ __global__ void __launch_bounds__(kThreads, (KS == 4 ? 2 : 3) - std::is_same_v<T
   };
   auto copy_h = [&](int k, int buffer) {
     if (CHUNKED || k >= p.each || tiles[k].x < 0) return;
-    const int per_row = p.r16 / 4, n16 = tiles[k].z * per_row;   // pieces of 16 bytes
-    const uint16_t* src = p.h + (int64_t)tiles[k].y * 2 * p.r16;
-    for (int i = threadIdx.x; i < n16; i += kThreads) copy_async<16>(hs + (buffer * kRows + i / per_row) * kPitch + i % per_row * 16, src + i * 8, 16);
+    constexpr int kPer = 4 * KS, kSweep = kThreads / kPer;   // pieces of 16 bytes per row; rows that the block copies at once
+    const int piece = threadIdx.x % kPer, row = threadIdx.x / kPer, z = tiles[k].z;
+    if (piece * 4 >= p.r16) return;
+    const uint16_t* src = p.h + (int64_t)(tiles[k].y + row) * 2 * p.r16 + piece * 8;
+    const uint32_t to = hs + buffer * 4 * kStep + piece / 4 * 1024 + piece % 4 * 16;
+#pragma unroll
+    for (int i = 0; i < kRows / kSweep; ++i) {
+      const int at = row + i * kSweep;
+      if (at >= z) break;
+      const uint32_t d = to + at / 16 * kStep + at % 8 * 64 + at / 8 % 2 * 4;
+      copy_async<4>(d, src, true);             // high part, first pair of ranks
+      copy_async<4>(d + 8, src + 2, true);     // second pair
+      copy_async<4>(d + 512, src + 4, true);   // low part
+      copy_async<4>(d + 520, src + 6, true);
+      src += (int64_t)kSweep * 2 * p.r16;
+    }
   };
   uint32_t bh[KS][4][2], bl[kSplitW ? KS : 1][4][2];   // rank step, column tile, pair of the lane's 4 ranks
   const T* w = nullptr;
@@ -459,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, (KS == 4 ? 2 : 3) - std::is_same_v<T
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = rows[ahead][i * 8 + g];
-      if constexpr (WHOLE) copy_async<16>(to + i * 512, y + (int64_t)row * C, add && row >= 0 ? 16 : 0);
+      if constexpr (WHOLE) copy_async<16>(to + i * 512, y + (int64_t)row * C, add && row >= 0);
       else store16(to + i * 512, add && row >= 0 ? load8<false, false>(y + (int64_t)row * C, have) : make_uint4(0, 0, 0, 0));
     }
     commit();
@@ -489,18 +513,18 @@ __global__ void __launch_bounds__(kThreads, (KS == 4 ? 2 : 3) - std::is_same_v<T
     copy_h(after, buffer ^ 1);
     last = (tile.z + 15) / 16;
     // (rows behind the tile's last one have what was there before; their products are not stored)
-    uint32_t src = hs + (buffer * kRows + g) * kPitch + q * 16;
-    for (int m = 0; m < last; ++m, ++now, src += 16 * kPitch) {
+    uint32_t src = hs + buffer * 4 * kStep + lane * 16;
+    for (int m = 0; m < last; ++m, ++now, src += kStep) {
       issue();
       float acc[4][4] = {};
-      auto step = [&](int s, const uint4& h0, const uint4& h1) {
+      auto step = [&](int s, const uint4& hi, const uint4& lo) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], h0.x, h1.x, h0.y, h1.y, bh[s][t][0], bh[s][t][1]);
+        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], hi.x, hi.y, hi.z, hi.w, bh[s][t][0], bh[s][t][1]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], h0.z, h1.z, h0.w, h1.w, bh[s][t][0], bh[s][t][1]);
+        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], lo.x, lo.y, lo.z, lo.w, bh[s][t][0], bh[s][t][1]);
         if constexpr (kSplitW) {
 #pragma unroll
-          for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], h0.x, h1.x, h0.y, h1.y, bl[s][t][0], bl[s][t][1]);
+          for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], hi.x, hi.y, hi.z, hi.w, bl[s][t][0], bl[s][t][1]);
         }
       };
       if (!plain) {
@@ -516,14 +540,14 @@ __global__ void __launch_bounds__(kThreads, (KS == 4 ? 2 : 3) - std::is_same_v<T
                 const int row = m * 16 + i * 8 + g;
                 h[i] = row < tile.z ? *reinterpret_cast<const uint4*>(p.h + (int64_t)(tile.y + row) * 2 * p.r16 + (r0 + s * 16) * 2 + q * 8) : make_uint4(0, 0, 0, 0);
               }
-              step(s, h[0], h[1]);
+              step(s, make_uint4(h[0].x, h[1].x, h[0].y, h[1].y), make_uint4(h[0].z, h[1].z, h[0].w, h[1].w));
             }
           }
         } else {
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
             if (KS > 1 && s * 16 >= p.r16) break;
-            step(s, load16(src + s * 64), load16(src + 8 * kPitch + s * 64));
+            step(s, load16(src + s * 1024), load16(src + s * 1024 + 512));
           }
         }
       }
@@ -684,15 +708,31 @@ int split_of(int64_t blocks, int64_t slots, int64_t most) {
   while (s < 8 && blocks * 2 * s <= slots && 2 * s <= most) s *= 2;
   return s;
 }
-// Tiles that there will be, about: the table has room for the most that there can be.
-int64_t likely_tiles(const Params& p) { return std::min<int64_t>(p.T, p.T / kRows + (std::min<int64_t>(p.T, p.L) + 1) / 2); }
+// Tiles that there will be, about (the table has room for the most that there can be): rows that choose their adapters at random.
+int64_t likely_tiles(const Params& p) {
+  const double used = p.L * (1.0 - exp(-(double)p.T / p.L)), rows = p.T / used;
+  return std::max<int64_t>(1, std::min<int64_t>(p.T, p.T / kRows + (int64_t)(used * (1.0 - 0.5 * std::min(1.0, rows / kRows)))));
+}
+// Tiles per block of the second product.  A block takes about as long as its tiles and three quarters of one more; blocks run in waves.  (By graph
+// replay, both products, us, with 1, 2, 3, 4, 5, 6, 8 tiles: 57 rows of 40 adapters of rank 20, f16, [11008, 4096] 26 23 22 25 21 22 26; 4096 rows of rank 64,
+// [14336, 4096] 119 104 102 103 100 111 111; 2048 rows of rank 16 41 40 40 40 38 39 41: the rule takes 6, 5 and 5.)
+int tiles_per_block(const Params& p, int64_t cols, int64_t slots) {
+  const int64_t tiles = likely_tiles(p);
+  double best = 0;
+  int each = 1;
+  for (int e = 1; e <= kUpTiles; ++e) {
+    const double time = (double)(((tiles + e - 1) / e * cols + slots - 1) / slots) * (e + 0.75);
+    if (e == 1 || time < best) { best = time; each = e; }
+  }
+  return each;
+}
 
 template <typename K>
-int launch(K kern, const Params& p, dim3 grid, size_t smem, cudaStream_t st) {
-  if (smem > 48 * 1024) B200Q_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+int launch(K kern, const Params& p, dim3 grid, int threads, size_t smem, cudaStream_t st) {
+  if (smem > 40 * 1024) B200Q_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -710,23 +750,23 @@ int launch(K kern, const Params& p, dim3 grid, size_t smem, cudaStream_t st) {
 
 template <typename T, bool TALL, bool WHOLE>
 int down(Params p, cudaStream_t st) {
-  const int nt = p.r <= 16 ? 2 : (p.r <= 32 ? 4 : 8), chunks = (p.r + 8 * nt - 1) / (8 * nt);
-  p.split = split_of(likely_tiles(p) * chunks, 148 * (nt == 8 ? 1 : 2), p.C / (kWarps * 32));
+  const int mt = p.r <= 16 ? 1 : (p.r <= 32 ? 2 : 4), chunks = (p.r + 16 * mt - 1) / (16 * mt);
+  p.split = split_of(likely_tiles(p) * chunks, 148 * (mt == 4 ? 1 : 2), p.C / (kWarps * 32));
   const dim3 grid((unsigned)(p.tiles_n * p.split), chunks);
-  if (nt == 2) return launch(down_kernel<T, TALL, WHOLE, 2>, p, grid, Down<TALL, 2>::kBytes, st);
-  if (nt == 4) return launch(down_kernel<T, TALL, WHOLE, 4>, p, grid, Down<TALL, 4>::kBytes, st);
-  return launch(down_kernel<T, TALL, WHOLE, 8>, p, grid, Down<TALL, 8>::kBytes, st);
+  if (mt == 1) return launch(down_kernel<T, TALL, WHOLE, 1>, p, grid, kThreads, Down<TALL, 1>::kBytes, st);
+  if (mt == 2) return launch(down_kernel<T, TALL, WHOLE, 2>, p, grid, kThreads, Down<TALL, 2>::kBytes, st);
+  return launch(down_kernel<T, TALL, WHOLE, 4>, p, grid, kThreads, Down<TALL, 4>::kBytes, st);
 }
 template <typename T, bool WIDE, bool WHOLE>
 int up(Params p, cudaStream_t st) {
   p.split = 1;
   const int64_t cols = (p.C + 255) / 256;
-  p.each = (int)std::max<int64_t>(1, std::min<int64_t>(kUpTiles, p.tiles_n * cols / (148 * 8)));   // a block's tiles share their weights' loads
+  p.each = tiles_per_block(p, cols, 148 * ((p.r > 32 ? 2 : 3) - std::is_same_v<T, __half>));
   const dim3 grid((unsigned)((p.tiles_n + p.each - 1) / p.each * cols));
-  if (p.r <= 16) return launch(up_kernel<T, WIDE, WHOLE, 1, false>, p, grid, Up<1>::kBytes, st);
-  if (p.r <= 32) return launch(up_kernel<T, WIDE, WHOLE, 2, false>, p, grid, Up<2>::kBytes, st);
-  if (p.r <= 64) return launch(up_kernel<T, WIDE, WHOLE, 4, false>, p, grid, Up<4>::kBytes, st);
-  return launch(up_kernel<T, WIDE, WHOLE, 4, true>, p, grid, kWarps * kUpStages * 1024, st);
+  if (p.r <= 16) return launch(up_kernel<T, WIDE, WHOLE, 1, false>, p, grid, kThreads, Up<1, false>::kBytes, st);
+  if (p.r <= 32) return launch(up_kernel<T, WIDE, WHOLE, 2, false>, p, grid, kThreads, Up<2, false>::kBytes, st);
+  if (p.r <= 64) return launch(up_kernel<T, WIDE, WHOLE, 4, false>, p, grid, kThreads, Up<4, false>::kBytes, st);
+  return launch(up_kernel<T, WIDE, WHOLE, 4, true>, p, grid, kThreads, Up<4, true>::kBytes, st);
 }
 template <typename T, bool TALL, bool WHOLE>
 int outer(Params p, cudaStream_t st) {
@@ -735,9 +775,9 @@ int outer(Params p, cudaStream_t st) {
   p.split = split_of(cols * p.L * chunks, 148 * 4, p.T / 64);
   const dim3 grid((unsigned)(cols * p.split), p.L, chunks);
   const size_t smem = (size_t)4 * 16 * mt * 72 * 4;
-  if (mt == 1) return launch(outer_kernel<T, TALL, WHOLE, 1>, p, grid, smem, st);
-  if (mt == 2) return launch(outer_kernel<T, TALL, WHOLE, 2>, p, grid, smem, st);
-  return launch(outer_kernel<T, TALL, WHOLE, 4>, p, grid, smem, st);
+  if (mt == 1) return launch(outer_kernel<T, TALL, WHOLE, 1>, p, grid, kThreads, smem, st);
+  if (mt == 2) return launch(outer_kernel<T, TALL, WHOLE, 2>, p, grid, kThreads, smem, st);
+  return launch(outer_kernel<T, TALL, WHOLE, 4>, p, grid, kThreads, smem, st);
 }
 
 // Of a call: which form of a kernel.
