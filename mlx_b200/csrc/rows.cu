@@ -28,10 +28,11 @@ struct RowsParams {
   const float* weights;
   float* dw;
   int64_t T, R;            // tokens, rows (T * top)
-  int64_t D, pieces;       // width, pieces of VEC elements per row
+  int64_t D, pieces;       // width, pieces of 16 bytes per row
   int top;
 };
 
+// ---- rows that are whole pieces of 16 bytes on their boundaries
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) dispatch_kernel(const RowsParams p) {
   using V = Vec<T, VEC>;
@@ -81,7 +82,7 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const RowsParams p) {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const RowsParams p) {
   using V = Vec<T, VEC>;
-  __shared__ float part[32][kThreads / 32];
+  __shared__ float part[32][kThreads / 32];   // of d w, for 32 choices at a time
   const int64_t t = blockIdx.x;
   const V* dy = static_cast<const V*>(p.x) + t * p.pieces;
   const V* y = static_cast<const V*>(p.y);
@@ -125,29 +126,178 @@ __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const RowsParams
         for (int64_t c = threadIdx.x; c < p.pieces; c += kThreads) dys[r * p.pieces + c] = V{};
 }
 
+// ---- rows that start anywhere.  A block has a token.  What is written to a row goes by the pieces of 16 bytes of memory that it covers: whole ones by
+// one store, those at its ends value by value.  What is read for a whole piece is 16 bytes from any address: two pieces of memory and a shift.  (Both hold bytes of
+// the row, and memory is mapped by more than 16 bytes, so that nothing outside is touched that is not there.)
+template <typename T>
+__device__ __forceinline__ Vec<T, 16 / sizeof(T)> load_any(const T* p) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  const uint32_t off = a & 15;
+  const uint4* q = reinterpret_cast<const uint4*>(a - off);
+  const uint4 lo = q[0];
+  uint4 hi = lo;
+  if (off) hi = q[1];
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  if (off & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (off & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  union {
+    uint32_t u[4];
+    Vec<T, 16 / sizeof(T)> v;
+  } r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.u[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
+  return r.v;
+}
+// For the row at `row`: whole(first column) for the pieces that this thread of a group has, one(column) for its values at the ends.
+template <typename T, typename F, typename G>
+__device__ __forceinline__ void for_pieces(const T* row, int64_t D, int id, int group, F whole, G one) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int64_t head = min((int64_t)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) % 16 / sizeof(T)), D), tail = head + (D - head) / VEC * VEC;
+  for (int64_t c = head + id * VEC; c < tail; c += group * VEC) whole(c);
+  // the ends' values: with the last threads, which have the fewest pieces
+  const int64_t ends = head + D - tail;
+  for (int64_t i = group - 1 - id; i < ends; i += group) one(i < head ? i : tail + i - head);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) dispatch_any_kernel(const RowsParams p) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int64_t t = blockIdx.x;
+  const T* x = static_cast<const T*>(p.x) + t * p.D;
+  T* xs = static_cast<T*>(p.out);
+  const bool left = p.order[p.R - 1] < 0;
+  for (int j = 0; j < p.top; ++j) {
+    const int64_t at = p.places[t * p.top + j];
+    if (at >= 0 && at < p.R)
+      for_pieces(xs + at * p.D, p.D, threadIdx.x, blockDim.x, [&](int64_t c) { *reinterpret_cast<Vec<T, VEC>*>(xs + at * p.D + c) = load_any(x + c); },
+                 [&](int64_t c) { xs[at * p.D + c] = x[c]; });
+  }
+  if (left)
+    for (int64_t r = t * p.top; r < (t + 1) * p.top; ++r)
+      if (p.order[r] < 0)
+        for (int64_t c = threadIdx.x; c < p.D; c += blockDim.x) xs[r * p.D + c] = Elem<T>::from_float(0.0f);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) combine_any_kernel(const RowsParams p) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int64_t t = blockIdx.x;
+  const T* y = static_cast<const T*>(p.y);
+  T* out = static_cast<T*>(p.out) + t * p.D;
+  for_pieces(out, p.D, threadIdx.x, blockDim.x, [&](int64_t c) {
+    float acc[VEC] = {};
+#pragma unroll 4
+    for (int j = 0; j < p.top; ++j) {
+      const int64_t at = p.places[t * p.top + j];
+      if (at < 0 || at >= p.R) continue;
+      const float w = p.weights ? p.weights[t * p.top + j] : 1.0f;
+      const auto v = load_any(y + at * p.D + c);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] = fmaf(w, Elem<T>::to_float(v.v[k]), acc[k]);
+    }
+    Vec<T, VEC> o;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) o.v[k] = Elem<T>::from_float(acc[k]);
+    *reinterpret_cast<Vec<T, VEC>*>(out + c) = o;
+  }, [&](int64_t c) {
+    float acc = 0.0f;
+    for (int j = 0; j < p.top; ++j) {
+      const int64_t at = p.places[t * p.top + j];
+      if (at >= 0 && at < p.R) acc = fmaf(p.weights ? p.weights[t * p.top + j] : 1.0f, Elem<T>::to_float(y[at * p.D + c]), acc);
+    }
+    out[c] = Elem<T>::from_float(acc);
+  });
+}
+
+// A group of threads has a pair (token, choice): a warp, or the block where there are few pairs.  dy's row is read once from HBM and for the token's other
+// pairs from L2.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) combine_grad_any_kernel(const RowsParams p, int group) {
+  constexpr int VEC = 16 / sizeof(T);
+  using V = Vec<T, VEC>;
+  __shared__ float part[kThreads / 32];
+  const int id = threadIdx.x % group;
+  const int64_t pair = (int64_t)blockIdx.x * (kThreads / group) + threadIdx.x / group;
+  if (pair >= p.R) return;   // (a whole warp; blocks of one pair have none such)
+  const int64_t at = p.places[pair];
+  const T *dy = static_cast<const T*>(p.x) + pair / p.top * p.D, *y = static_cast<const T*>(p.y) + at * p.D;
+  T *dys = static_cast<T*>(p.out), *d = dys + at * p.D;
+  float dot = 0.0f;
+  if (at >= 0 && at < p.R) {
+    const float w = p.weights[pair];
+    auto whole = [&](int64_t c) {
+      const V g = load_any(dy + c);
+      if (p.dw) {
+        const V v = load_any(y + c);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) dot = fmaf(Elem<T>::to_float(g.v[k]), Elem<T>::to_float(v.v[k]), dot);
+      }
+      if (dys) {
+        V o;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) o.v[k] = Elem<T>::from_float(w * Elem<T>::to_float(g.v[k]));
+        *reinterpret_cast<V*>(d + c) = o;
+      }
+    };
+    for_pieces(dys ? d : const_cast<T*>(y), p.D, id, group, whole, [&](int64_t c) {
+      const float g = Elem<T>::to_float(dy[c]);
+      if (p.dw) dot = fmaf(g, Elem<T>::to_float(y[c]), dot);
+      if (dys) d[c] = Elem<T>::from_float(w * g);
+    });
+  }
+  if (p.dw) {
+    for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (group > 32) {
+      if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
+      __syncthreads();
+      if (id == 0)
+        for (int q = 1; q < kThreads / 32; ++q) dot += part[q];
+    }
+    if (id == 0) p.dw[pair] = dot;
+  }
+  if (dys && p.order[pair] < 0)   // a row that no pair has
+    for (int64_t c = id; c < p.D; c += group) dys[pair * p.D + c] = Elem<T>::from_float(0.0f);
+}
+
 enum class Kind { Dispatch, Combine, Grad };
 
-template <typename T, int VEC>
+template <typename T>
 int launch(Kind kind, RowsParams p, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(T);
+  const uintptr_t all = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.D * sizeof(T));
   p.pieces = p.D / VEC;
-  const int64_t n = p.T * p.pieces;
-  const unsigned blocks = (unsigned)std::min<int64_t>((n + kThreads - 1) / kThreads, 148 * 8 * 16);
-  switch (kind) {
-    case Kind::Dispatch: dispatch_kernel<T, VEC><<<blocks, kThreads, 0, st>>>(p); break;
-    case Kind::Combine: combine_kernel<T, VEC><<<blocks, kThreads, 0, st>>>(p); break;
-    case Kind::Grad: combine_grad_kernel<T, VEC><<<(unsigned)p.T, kThreads, 0, st>>>(p); break;
+  const unsigned tokens = (unsigned)p.T, threads = (unsigned)std::min<int64_t>(kThreads, (p.pieces + 32) / 32 * 32);
+  const int group = p.R < 148 * 8 ? kThreads : 32;
+  const unsigned pairs = (unsigned)((p.R + kThreads / group - 1) / (kThreads / group));
+  if (all % 16 == 0) {   // every piece of 16 bytes on its boundary
+    const unsigned blocks = (unsigned)std::min<int64_t>((p.T * p.pieces + kThreads - 1) / kThreads, 148 * 8 * 16);
+    switch (kind) {
+      case Kind::Dispatch: dispatch_kernel<T, VEC><<<blocks, kThreads, 0, st>>>(p); break;
+      case Kind::Combine: combine_kernel<T, VEC><<<blocks, kThreads, 0, st>>>(p); break;
+      case Kind::Grad: combine_grad_kernel<T, VEC><<<tokens, kThreads, 0, st>>>(p); break;
+    }
+  } else {
+    switch (kind) {
+      case Kind::Dispatch: dispatch_any_kernel<T><<<tokens, threads, 0, st>>>(p); break;
+      case Kind::Combine: combine_any_kernel<T><<<tokens, threads, 0, st>>>(p); break;
+      case Kind::Grad: combine_grad_any_kernel<T><<<pairs, kThreads, 0, st>>>(p, group); break;
+    }
   }
   B200Q_LAUNCH_OK("rows kernel");
   return B200Q_OK;
 }
 
 int run(Kind kind, const RowsParams& p, int dtype, cudaStream_t st) {
-  const uintptr_t all = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.D * dtype_size(dtype));
-  const bool whole = all % 16 == 0;   // every piece of 16 bytes on its boundary
   switch (dtype) {
-    case B200Q_F32: return whole ? launch<float, 4>(kind, p, st) : launch<float, 1>(kind, p, st);
-    case B200Q_F16: return whole ? launch<__half, 8>(kind, p, st) : launch<__half, 1>(kind, p, st);
-    default: return whole ? launch<__nv_bfloat16, 8>(kind, p, st) : launch<__nv_bfloat16, 1>(kind, p, st);
+    case B200Q_F32: return launch<float>(kind, p, st);
+    case B200Q_F16: return launch<__half>(kind, p, st);
+    default: return launch<__nv_bfloat16>(kind, p, st);
   }
 }
 
