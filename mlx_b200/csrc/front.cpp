@@ -703,6 +703,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
     ctx->saved_data["renormalize"] = r->renormalize;
     ctx->saved_data["scale"] = (double)r->scale;
     ctx->mark_non_differentiable({(*out)[1], (*out)[2], (*out)[3], (*out)[4]});
+    ctx->set_materialize_grads(false);   // (no zeros for the four that have none)
     return *out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {

@@ -203,11 +203,14 @@ class _RouteFn(torch.autograd.Function):
         ctx.save_for_backward(logits, routing.experts)
         ctx.cfg = (scoring, renormalize, scale)
         ctx.mark_non_differentiable(*routing[1:])
+        ctx.set_materialize_grads(False)   # (no zeros for the four that have none)
         return tuple(routing)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dw, *_):
+        if dw is None:
+            return (None,) * 9
         logits, experts = ctx.saved_tensors
         return (ops.route_dlogits(dw, logits, experts, *ctx.cfg),) + (None,) * 8
 
