@@ -430,7 +430,7 @@ const char* b200q_grouped_qqmm_kernel_name(int64_t T, int64_t E, int64_t N, int6
  *   places  [T, top]: where a pair stands when pairs are sorted by expert (stably, pair p = t * top + j); no expert: -1
  *   order   [T * top]: the pair at every place; behind the last pair with an expert -1 - p of those without
  * b200q_route_dlogits: the gradient with respect to the logits (dtype) of the weights' gradient dw; none flows to the choice or the bias.
- * At most 1024 experts, 32 of them per token, 32 groups and 2^31 - 1 pairs.  ws: plain scratch, 4-byte aligned.
+ * At most 1024 experts, 32 of them per token, 32 groups and 2^31 - 1 pairs.  ws: plain scratch, 16-byte aligned.
  */
 #define B200Q_SOFTMAX 0
 #define B200Q_SIGMOID 1
@@ -462,7 +462,7 @@ int b200q_combine_rows_grad(const void* dy, const void* y, int dtype, int64_t T,
  *   sizes [n], starts [n + 1]: rows per group, and where each group (and behind them the rows without one) starts in the order
  *   order [T]: rows by group, stably; those without a group last, as -1 - row
  *   tiles [b200q_group_rows_tiles(T, n)][4] (16-byte aligned): what b200q_add_adapters reads: up to 64 places of one group each
- * At most 4096 groups and 2^30 rows.  ws: plain scratch, 4-byte aligned.
+ * At most 4096 groups and 2^30 rows.  ws: plain scratch, 16-byte aligned.
  */
 int64_t b200q_group_rows_tiles(int64_t T, int64_t n);
 size_t b200q_group_rows_workspace_bytes(int64_t T, int64_t n);

@@ -24,6 +24,8 @@ namespace {
 
 constexpr int kMaxWarps = 32;
 constexpr uint32_t kFull = 0xffffffffu;
+// Bins of a histogram in memory: whole pieces of 16 bytes.
+constexpr __host__ __device__ int pitch(int64_t bins) { return (int)(bins + 3) / 4 * 4; }
 
 // Integers in the order of the numbers; NaN above all, -0 as 0.  0 is below every number.
 __device__ __forceinline__ uint32_t code32(float f) {
@@ -59,15 +61,17 @@ __device__ __forceinline__ void warp_best64(unsigned long long& c, int& i) {
   }
 }
 __device__ __forceinline__ float sigmoid(float l) { return 1.0f / (1.0f + expf(-l)); }
+// For keys, whose roundings have room: off by less than a unit of the largest score (the exponential by 2 + 1.2 |x| units, times s (1 - s)).
+__device__ __forceinline__ float sigmoid_near(float l) { return __fdividef(1.0f, 1.0f + __expf(-l)); }
 
 struct RouteParams {
   const void* logits;
   const float* bias;
   float* weights;
   int *experts, *sizes, *places, *order;
-  uint32_t* hist;      // [blocks][E + 1]; one block: not used
+  uint32_t* hist;      // [blocks][pitch(E + 1)]; one block: not used
   int64_t T, per_block, per_warp;
-  int E, top, groups, top_groups, best, sigmoid, renormalize;
+  int E, top, groups, log_groups, top_groups, best, sigmoid, renormalize;   // log_groups: rounded up
   float scale;
 };
 
@@ -154,7 +158,7 @@ __device__ __forceinline__ void route_token(const RouteParams& p, const T* logit
     if (m > -INFINITY) {
       float z = 0.0f;
 #pragma unroll
-      for (int v = 0; v < V; ++v) z += expf(l[v] - m);
+      for (int v = 0; v < V; ++v) z += p.renormalize ? __expf(l[v] - m) : expf(l[v] - m);   // (then only keys need it)
       rz = 1.0f / warp_sum(z);
     }
   }
@@ -164,7 +168,7 @@ __device__ __forceinline__ void route_token(const RouteParams& p, const T* logit
     const int i = v * 32 + lane;
     float key = l[v];
     if (scores) {
-      const float s = p.sigmoid ? sigmoid(l[v]) : expf(l[v] - m) * rz;
+      const float s = p.sigmoid ? sigmoid_near(l[v]) : __expf(l[v] - m) * rz;
       if (p.bias && i < E) key = l[v] == -INFINITY ? -INFINITY : s + p.bias[i];
       if (sums && i < E) {
         const float k = p.bias ? key : s;
@@ -174,32 +178,39 @@ __device__ __forceinline__ void route_token(const RouteParams& p, const T* logit
     u[v] = i >= E || key == -INFINITY ? 0 : code32(key);
     if (p.groups > 1 && !sums && i < E) row32[i] = u[v];
   }
-  // how far two keys have to be apart for their rounded forms to be in the right order: 88 half units of the largest score
+  // how far two keys have to be apart for their rounded forms to be in the right order: 90 half units of the largest score
   // (a sum of up to 37 terms, exp, the argument's rounding, a division), one of the sum with the bias; rounded up
   const float room = p.sigmoid ? 0x1p-17f : 0x1p-17f * rz;
   bool unsure = false;
   if (p.groups > 1) {
     __syncwarp();
-    const int size = E / p.groups;
-    uint32_t rank = 0;
-    if (lane < p.groups) {
-      uint32_t a = 0, b = 0;
-      int i = lane % size;   // lanes start at different places: no bank is asked twice
-      for (int n = 0; n < size; ++n) {
-        const uint32_t c = row32[lane * size + i];
-        if (c > a) { b = a; a = c; } else if (c > b) b = c;
-        i = i + 1 == size ? 0 : i + 1;
+    // several lanes scan a group, each from another place on, so that no bank is asked twice; then they put their best two together
+    const int size = E / p.groups, lanes = 32 >> p.log_groups, group = lane >> (5 - p.log_groups), each = (size + lanes - 1) / lanes;
+    uint32_t rank = 0, b = 0;   // the group's best, the second
+    if (group < p.groups) {
+      int k = group % each;
+      for (int n = 0; n < each; ++n) {
+        const int i = k * lanes + (lane & (lanes - 1));
+        const uint32_t c = i < size ? row32[group * size + i] : 0;
+        b = max(b, min(rank, c));
+        rank = max(rank, c);
+        k = k + 1 == each ? 0 : k + 1;
       }
-      rank = a;
-      if (sums && b != 0) rank = code32(value32(a) + value32(b));
     }
+    for (int o = 1; o < lanes; o *= 2) {
+      const uint32_t c = __shfl_xor_sync(kFull, rank, o), c2 = __shfl_xor_sync(kFull, b, o);
+      b = max(max(b, c2), min(rank, c));
+      rank = max(rank, c);
+    }
+    if (sums && b != 0) rank = code32(value32(rank) + value32(b));
+    if (lane & (lanes - 1)) rank = 0;   // the group's first lane stands for it
     __syncwarp();
     uint32_t on = 0, last = 0;
     for (int k = 0; k < p.top_groups; ++k) {
       const uint32_t c = __reduce_max_sync(kFull, rank);
       if (c == 0) break;
       const int i = __ffs(__ballot_sync(kFull, rank == c)) - 1;
-      on |= 1u << i;
+      on |= 1u << (i / lanes);
       last = c;
       if (lane == i) rank = 0;
     }
@@ -313,7 +324,7 @@ struct SortParams {
   const void* ids;     // of `bytes` each
   int bytes;
   uint32_t* rank;      // of every pair among its block's of the same group
-  uint32_t* hist;      // [blocks][n + 1]
+  uint32_t* hist;      // [blocks][pitch(n + 1)]
   int *sizes, *starts, *places, *order;   // starts and places may be null
   int4* tiles;         // may be null
   int64_t max_tiles, P, per_block;        // pairs
@@ -374,6 +385,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(V > 16 ? 512 : 1024) route_kernel(const RouteParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ uint32_t warp_sums[32];
+  asm volatile("griddepcontrol.launch_dependents;");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, bins = p.E + 1;
   const bool rows = p.bias != nullptr || p.groups > 1;
   unsigned long long* row = reinterpret_cast<unsigned long long*>(smem) + (size_t)warp * p.E;
@@ -412,7 +424,7 @@ __global__ void __launch_bounds__(V > 16 ? 512 : 1024) route_kernel(const RouteP
     rank[i] += mine[e < 0 ? p.E : e];
   }
   if (gridDim.x > 1) {
-    for (int e = threadIdx.x; e < bins; e += blockDim.x) p.hist[(size_t)blockIdx.x * bins + e] = sums[e];
+    for (int e = threadIdx.x; e < bins; e += blockDim.x) p.hist[(size_t)blockIdx.x * pitch(bins) + e] = sums[e];
     return;
   }
   uint32_t* total = sums + bins;
@@ -426,6 +438,7 @@ __global__ void __launch_bounds__(V > 16 ? 512 : 1024) route_kernel(const RouteP
 __global__ void __launch_bounds__(1024) group_kernel(const SortParams p, int64_t per_warp) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ uint32_t warp_sums[32];
+  asm volatile("griddepcontrol.launch_dependents;");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, bins = p.n + 1;
   uint32_t* hist = reinterpret_cast<uint32_t*>(smem);
   uint32_t* mine = hist + (size_t)warp * bins;
@@ -448,7 +461,7 @@ __global__ void __launch_bounds__(1024) group_kernel(const SortParams p, int64_t
   __syncthreads();
   for (int64_t i = lo + lane; i < hi; i += 32) p.rank[i] += mine[bin_of(p, i)];
   if (gridDim.x > 1) {
-    for (int e = threadIdx.x; e < bins; e += blockDim.x) p.hist[(size_t)blockIdx.x * bins + e] = sums[e];
+    for (int e = threadIdx.x; e < bins; e += blockDim.x) p.hist[(size_t)blockIdx.x * pitch(bins) + e] = sums[e];
     return;
   }
   uint32_t* total = sums + bins;
@@ -462,23 +475,24 @@ __global__ void __launch_bounds__(1024) group_kernel(const SortParams p, int64_t
 __global__ void __launch_bounds__(1024) place_kernel(const SortParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ uint32_t warp_sums[32];
-  const int bins = p.n + 1;
-  uint32_t *base = reinterpret_cast<uint32_t*>(smem), *total = base + bins, *before = total + bins;
-  for (int e = threadIdx.x; e < bins; e += blockDim.x) { total[e] = 0; before[e] = 0; }
+  const int bins = p.n + 1, quads = pitch(bins) / 4;
+  uint32_t *base = reinterpret_cast<uint32_t*>(smem), *total = base + 4 * quads, *before = total + 4 * quads;
+  for (int e = threadIdx.x; e < 4 * quads; e += blockDim.x) { total[e] = 0; before[e] = 0; }
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the first launch's results
   __syncthreads();
-  // threads by (part of the blocks, bin); sums of integers in shared memory, whose order does not matter
-  const int parts = max(1, (int)blockDim.x / bins);
-  for (int i = threadIdx.x; i < parts * bins; i += blockDim.x) {
-    const int part = i / bins, e = i % bins;
-    uint32_t all = 0, mine = 0;
-#pragma unroll 8
+  // threads by (part of the blocks, four bins); sums of integers in shared memory, whose order does not matter
+  const int parts = max(1, (int)blockDim.x / quads);
+  for (int i = threadIdx.x; i < parts * quads; i += blockDim.x) {
+    const int part = i / quads, e = i % quads;
+    uint4 all = make_uint4(0, 0, 0, 0), mine = all;
+#pragma unroll 4
     for (int b = part; b < p.blocks; b += parts) {
-      const uint32_t v = p.hist[(size_t)b * bins + e];
-      all += v;
-      if (b < (int)blockIdx.x) mine += v;
+      const uint4 v = reinterpret_cast<const uint4*>(p.hist)[(size_t)b * quads + e];
+      all.x += v.x; all.y += v.y; all.z += v.z; all.w += v.w;
+      if (b < (int)blockIdx.x) { mine.x += v.x; mine.y += v.y; mine.z += v.z; mine.w += v.w; }
     }
-    atomicAdd(&total[e], all);
-    atomicAdd(&before[e], mine);
+    atomicAdd(&total[4 * e], all.x); atomicAdd(&total[4 * e + 1], all.y); atomicAdd(&total[4 * e + 2], all.z); atomicAdd(&total[4 * e + 3], all.w);
+    atomicAdd(&before[4 * e], mine.x); atomicAdd(&before[4 * e + 1], mine.y); atomicAdd(&before[4 * e + 2], mine.z); atomicAdd(&before[4 * e + 3], mine.w);
   }
   __syncthreads();
   for (int e = threadIdx.x; e < bins; e += blockDim.x) base[e] = total[e];
@@ -495,10 +509,21 @@ int allow_smem(K kern, size_t bytes) {
   return B200Q_OK;
 }
 
+// Launched while the first kernel runs, whose last blocks it waits for.
 int place(const SortParams& s, cudaStream_t st) {
-  const size_t smem = (size_t)3 * (s.n + 1) * 4;
+  const size_t smem = (size_t)3 * pitch(s.n + 1) * 4;
   if (int rc = allow_smem(place_kernel, smem)) return rc;
-  place_kernel<<<s.blocks, 1024, smem, st>>>(s);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(s.blocks);
+  cfg.blockDim = dim3(1024);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  B200Q_CUDA_OK(cudaLaunchKernelEx(&cfg, place_kernel, s));
   B200Q_LAUNCH_OK("place_kernel");
   return B200Q_OK;
 }
@@ -579,21 +604,18 @@ int launch_route(const RouteParams& p, int blocks, int warps, cudaStream_t st) {
   return go(route_kernel<T, 32>);
 }
 
-// Blocks and warps: a decode batch in one block (one launch), else 16 tokens or more per block, two blocks per SM.
+// Blocks and warps: up to 16 tokens in one block, one launch; else 8 tokens or more per block, one block of up to 32 warps per SM, whose histograms the
+// second launch reads.  (64 tokens of 256 experts in groups: 29 us in one block of 32 warps, which share an SM's instructions.)
 struct Split { int blocks, warps; int64_t per_block, per_warp; };
 Split route_split(int64_t T, int64_t E) {
   Split s{};
   const int most = E > 512 ? 16 : kMaxWarps;
-  if (T <= 2 * most) {
-    s.blocks = 1;
-    s.warps = (int)std::min<int64_t>(T, most);
-  } else {
-    s.warps = 16;
-    s.blocks = (int)std::min<int64_t>((T + 15) / 16, 2 * 148);
-  }
+  s.blocks = T <= 16 ? 1 : (int)std::min<int64_t>((T + 7) / 8, 148);
   s.per_block = (T + s.blocks - 1) / s.blocks;
-  s.per_warp = (s.per_block + s.warps - 1) / s.warps;
   s.blocks = (int)((T + s.per_block - 1) / s.per_block);
+  s.warps = (int)std::min<int64_t>(s.per_block, most);
+  s.per_warp = (s.per_block + s.warps - 1) / s.warps;
+  s.warps = (int)((s.per_block + s.per_warp - 1) / s.per_warp);
   return s;
 }
 Split group_split(int64_t T, int64_t n) {
@@ -630,7 +652,7 @@ using namespace b200q;
 extern "C" size_t b200q_route_workspace_bytes(int64_t T, int64_t E, int64_t top) {
   if (T <= 0 || E <= 0 || top <= 0) return 0;
   const Split s = route_split(T, E);
-  return s.blocks == 1 ? 0 : (size_t)s.blocks * (E + 1) * 4;
+  return s.blocks == 1 ? 0 : (size_t)s.blocks * pitch(E + 1) * 4;
 }
 
 extern "C" int b200q_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t top, int scoring, const float* bias, int64_t groups,
@@ -653,11 +675,13 @@ extern "C" int b200q_route(const void* logits, int dtype, int64_t T, int64_t E, 
   if (!logits || !weights || !experts || !places || !order) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
   const Split s = route_split(T, E);
   const size_t need = b200q_route_workspace_bytes(T, E, top);
-  if (need > 0 && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 4 != 0))
+  if (need > 0 && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16 != 0))
     return fail(B200Q_ERR_WORKSPACE, "[%s] an aligned workspace of %zu bytes required, %zu given", tag, need, ws ? ws_bytes : (size_t)0);
   if (top_groups == groups) groups = top_groups = 1;   // nothing to leave out
+  int log_groups = 0;
+  while (1 << log_groups < groups) ++log_groups;
   const RouteParams p{logits, bias, weights, experts, sizes, places, order, static_cast<uint32_t*>(ws), T, s.per_block, s.per_warp,
-                      (int)E, (int)top, (int)groups, (int)top_groups, group_best, scoring == B200Q_SIGMOID, renormalize != 0, scale};
+                      (int)E, (int)top, (int)groups, log_groups, (int)top_groups, group_best, scoring == B200Q_SIGMOID, renormalize != 0, scale};
   const ScratchLock lock(ws);
   int rc = dtype == B200Q_F32 ? launch_route<float>(p, s.blocks, s.warps, st)
                               : (dtype == B200Q_F16 ? launch_route<__half>(p, s.blocks, s.warps, st) : launch_route<__nv_bfloat16>(p, s.blocks, s.warps, st));
@@ -689,7 +713,7 @@ extern "C" int64_t b200q_group_rows_tiles(int64_t T, int64_t n) {
 extern "C" size_t b200q_group_rows_workspace_bytes(int64_t T, int64_t n) {
   if (T <= 0 || n < 0) return 0;
   const Split s = group_split(T, n);
-  return (size_t)T * 4 + (s.blocks == 1 ? 0 : (size_t)s.blocks * (n + 1) * 4);
+  return (size_t)pitch(T) * 4 + (s.blocks == 1 ? 0 : (size_t)s.blocks * pitch(n + 1) * 4);
 }
 
 extern "C" int b200q_group_rows(const void* ids, int id_bytes, int64_t T, int64_t n, int32_t* sizes, int32_t* starts, int32_t* order, int32_t* tiles,
@@ -710,11 +734,11 @@ extern "C" int b200q_group_rows(const void* ids, int id_bytes, int64_t T, int64_
   if (!ids || !order || !tiles) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
   if (reinterpret_cast<uintptr_t>(tiles) % 16 != 0) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] tiles must be 16-byte aligned", tag);
   const size_t need = b200q_group_rows_workspace_bytes(T, n);
-  if (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 4 != 0)
+  if (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16 != 0)
     return fail(B200Q_ERR_WORKSPACE, "[%s] an aligned workspace of %zu bytes required, %zu given", tag, need, ws ? ws_bytes : (size_t)0);
   const Split s = group_split(T, n);
   uint32_t* rank = static_cast<uint32_t*>(ws);
-  const SortParams p{ids, id_bytes, rank, rank + T, sizes, starts, nullptr, order, reinterpret_cast<int4*>(tiles), b200q_group_rows_tiles(T, n), T, s.per_block, (int)n, s.blocks};
+  const SortParams p{ids, id_bytes, rank, rank + pitch(T), sizes, starts, nullptr, order, reinterpret_cast<int4*>(tiles), b200q_group_rows_tiles(T, n), T, s.per_block, (int)n, s.blocks};
   const size_t smem = (size_t)(s.warps + 2) * (n + 1) * 4;
   const ScratchLock lock(ws);
   if (int rc = allow_smem(group_kernel, smem)) return rc;
