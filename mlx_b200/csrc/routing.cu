@@ -7,7 +7,8 @@
 // a pair has expert -1, weight 0 and place -1.
 //
 // A warp has a token, a lane every 32nd expert.  Keys are compared as 32-bit integers of the same order (NaN above everything, 0:
-// not to be taken), so that a choice is two warp-wide integer reductions.  Which experts a token gets is decided in 64 bits: keys that
+// not to be taken).  The chain of dependent steps is what costs time, so nothing is chosen one by one: of the lanes' best keys the top-th is a bound that
+// what is taken has to reach; the few keys that do are put side by side, and each counts those before it.  Which experts a token gets is decided in 64 bits: keys that
 // are logits need no rounding, and sums of rounded scores are taken in 32 bits only where neighbours are further apart than the
 // rounding can be; else the token's keys are computed again in 64 bits (choose64), for about a token in a thousand.
 //
@@ -27,13 +28,12 @@ constexpr uint32_t kFull = 0xffffffffu;
 // Bins of a histogram in memory: whole pieces of 16 bytes.
 constexpr __host__ __device__ int pitch(int64_t bins) { return (int)(bins + 3) / 4 * 4; }
 
-// Integers in the order of the numbers; NaN above all, -0 as 0.  0 is below every number.
+// Integers in the order of the numbers; NaN above all, -0 as 0 (the sum with 0 makes them the one NaN and 0 that arithmetic gives).  0 is below every number.
 __device__ __forceinline__ uint32_t code32(float f) {
-  if (f != f) return kFull;
-  const uint32_t b = __float_as_uint(f + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const int b = __float_as_int(f + 0.0f);
+  return (uint32_t)(b ^ (b >> 31 | (int)0x80000000));
 }
-__device__ __forceinline__ float value32(uint32_t c) { return c == kFull ? __uint_as_float(0x7fffffffu) : __uint_as_float(c & 0x80000000u ? c ^ 0x80000000u : ~c); }
+__device__ __forceinline__ float value32(uint32_t c) { return __uint_as_float(c & 0x80000000u ? c ^ 0x80000000u : ~c); }
 __device__ __forceinline__ unsigned long long code64(double f) {
   if (f != f) return ~0ull;
   const unsigned long long b = (unsigned long long)__double_as_longlong(f + 0.0);
@@ -52,6 +52,28 @@ __device__ __forceinline__ F warp_sum(F v) {
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
   return v;
 }
+// Over the first `lanes` lanes (a power of two), each of which gets the result.
+__device__ __forceinline__ float first_max(float v, int lanes) {
+  for (int o = 1; o < lanes; o *= 2) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+__device__ __forceinline__ float first_sum(float v, int lanes) {
+  for (int o = 1; o < lanes; o *= 2) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+// How many of n codes (in shared memory; zeros up to a multiple of 4) are before the lane's own, which is the lane-th: larger ones, and equal ones of
+// lower lanes.
+__device__ __forceinline__ int place_among(const uint32_t* codes, int n, uint32_t own, int lane) {
+  int before = 0;
+  for (int j = 0; j < n; j += 4) {
+    const uint4 c = *reinterpret_cast<const uint4*>(codes + j);
+    before += c.x > own || (c.x == own && j < lane);
+    before += c.y > own || (c.y == own && j + 1 < lane);
+    before += c.z > own || (c.z == own && j + 2 < lane);
+    before += c.w > own || (c.w == own && j + 3 < lane);
+  }
+  return before;
+}
 // Of the lanes' (code, index) the largest code's, at the lowest index.
 __device__ __forceinline__ void warp_best64(unsigned long long& c, int& i) {
   for (int o = 16; o; o >>= 1) {
@@ -61,6 +83,11 @@ __device__ __forceinline__ void warp_best64(unsigned long long& c, int& i) {
   }
 }
 __device__ __forceinline__ float sigmoid(float l) { return 1.0f / (1.0f + expf(-l)); }
+// sigmoid(l) exp(-far) for far <= 0 and l <= far, or far = 0: scores that would underflow, relative to the largest.
+__device__ __forceinline__ float sigmoid_over(float l, float far) {
+  const float e = expf(-fabsf(l));
+  return (l > 0.0f ? 1.0f : (far < 0.0f ? expf(l - far) : e)) / (1.0f + e);
+}
 // For keys, whose roundings have room: off by less than a unit of the largest score (the exponential by 2 + 1.2 |x| units, times s (1 - s)).
 __device__ __forceinline__ float sigmoid_near(float l) { return __fdividef(1.0f, 1.0f + __expf(-l)); }
 
@@ -71,61 +98,110 @@ struct RouteParams {
   int *experts, *sizes, *places, *order;
   uint32_t* hist;      // [blocks][pitch(E + 1)]; one block: not used
   int64_t T, per_block, per_warp;
-  int E, top, groups, log_groups, top_groups, best, sigmoid, renormalize;   // log_groups: rounded up
+  int E, top, top2, groups, log_groups, top_groups, best, sigmoid, renormalize;   // top2: top as a power of two, log_groups: both rounded up
   float scale;
 };
 
-// One token's experts, in 64 bits: lane j gets the j-th (-1: none).  `row` holds E numbers in shared memory.
-template <typename T>
-__device__ __noinline__ int choose64(const RouteParams& p, const T* logits, unsigned long long* row, int lane) {
+// One token's experts, in 64 bits: lane j gets the j-th (-1: none).  `row` holds E numbers in shared memory, `few` 96 words.  (The other tokens' warps wait
+// for this one at the end of the block, so it has to be quick, too.)
+template <typename T, int V>
+__device__ __noinline__ int choose64(const RouteParams& p, const T* logits, unsigned long long* row, uint32_t* few, int lane) {
   const int E = p.E;
   double m = -INFINITY, z = 1.0;
   if (!p.sigmoid) {
     for (int i = lane; i < E; i += 32) m = fmax(m, (double)Elem<T>::to_float(logits[i]));
     for (int o = 16; o; o >>= 1) m = fmax(m, __shfl_xor_sync(kFull, m, o));
     z = 0.0;
-    for (int i = lane; i < E; i += 32) z += exp((double)Elem<T>::to_float(logits[i]) - m);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (v * 32 + lane < E) z += exp((double)Elem<T>::to_float(logits[v * 32 + lane]) - m);
     z = warp_sum(z);
   }
-  for (int i = lane; i < E; i += 32) {
-    const double l = (double)Elem<T>::to_float(logits[i]);
-    const double s = p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - m) / z;
-    const double key = p.bias ? s + (double)p.bias[i] : s;
-    row[i] = l == -INFINITY || key == -INFINITY ? 0 : code64(key);
+  constexpr int U = V < 8 ? V : 8;   // at once: an exponential and a division are chains of some 40 steps each
+  for (int v0 = 0; v0 < V; v0 += U) {
+    double key[U];
+#pragma unroll
+    for (int v = 0; v < U; ++v) {
+      const int i = (v0 + v) * 32 + lane;
+      const double l = i < E ? (double)Elem<T>::to_float(logits[i]) : -INFINITY;
+      const double e = exp(p.sigmoid ? -l : l - m);
+      key[v] = (p.sigmoid ? 1.0 : e) / (p.sigmoid ? 1.0 + e : z) + (p.bias && i < E ? (double)p.bias[i] : 0.0);
+      if (l == -INFINITY) key[v] = -INFINITY;
+    }
+#pragma unroll
+    for (int v = 0; v < U; ++v)
+      if ((v0 + v) * 32 + lane < E) row[(v0 + v) * 32 + lane] = key[v] == -INFINITY ? 0 : code64(key[v]);
   }
   __syncwarp();
   uint32_t on = kFull;
   const int size = E / p.groups;
   if (p.groups > 1) {
-    unsigned long long rank = 0;
-    if (lane < p.groups) {
-      unsigned long long a = 0, b = 0;   // the best two
-      for (int i = lane * size; i < (lane + 1) * size; ++i) {
-        const unsigned long long c = row[i];
-        if (c > a) { b = a; a = c; } else if (c > b) b = c;
+    const int lanes = 32 >> p.log_groups, group = lane >> (5 - p.log_groups);
+    unsigned long long a = 0, b = 0;   // the best two
+    if (group < p.groups)
+      for (int i = lane & (lanes - 1); i < size; i += lanes) {
+        const unsigned long long c = row[group * size + i];
+        b = max(b, min(a, c));
+        a = max(a, c);
       }
-      rank = a;
-      if (p.best == 2 && b != 0) rank = code64(value64(a) + value64(b));
+    for (int o = 1; o < lanes; o *= 2) {
+      const unsigned long long c = __shfl_xor_sync(kFull, a, o), c2 = __shfl_xor_sync(kFull, b, o);
+      b = max(max(b, c2), min(a, c));
+      a = max(a, c);
     }
+    const unsigned long long rank = p.best == 2 && b != 0 ? code64(value64(a) + value64(b)) : a;
+    int before = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const unsigned long long c = __shfl_sync(kFull, rank, g * lanes);
+      before += c > rank || (c == rank && g < group);
+    }
+    uint32_t taken = __ballot_sync(kFull, group < p.groups && (lane & (lanes - 1)) == 0 && rank != 0 && before < p.top_groups);
     on = 0;
-    for (int k = 0; k < p.top_groups; ++k) {
-      unsigned long long c = rank;
-      int i = lane;
-      warp_best64(c, i);
-      if (c == 0) break;
-      on |= 1u << i;
-      if (lane == i) rank = 0;
-    }
+    for (; taken; taken &= taken - 1) on |= 1u << ((__ffs(taken) - 1) / lanes);
   }
+  uint32_t best = 0;   // upper words, which are in the same order
   for (int i = lane; i < E; i += 32) {
     if (!p.bias) {   // among experts the logits decide
       const double l = (double)Elem<T>::to_float(logits[i]);
       row[i] = l == -INFINITY ? 0 : code64(l);
     }
     if (p.groups > 1 && !(on >> (i / size) & 1)) row[i] = 0;
+    best = max(best, (uint32_t)(row[i] >> 32));
+  }
+  uint32_t bound = 1;
+  for (int j = 0; j < p.top; ++j) {
+    const uint32_t c = __reduce_max_sync(kFull, best);
+    if (c == 0) { bound = 1; break; }
+    bound = c;
+    if (best == c) best = 0;
+  }
+  unsigned long long* codes = reinterpret_cast<unsigned long long*>(few);
+  int n = 0;
+  __syncwarp();
+  for (int i0 = 0; i0 < E; i0 += 32) {
+    const unsigned long long c = i0 + lane < E ? row[i0 + lane] : 0;
+    const uint32_t has = __ballot_sync(kFull, (uint32_t)(c >> 32) >= bound);   // (a code's upper word is 0 for no number)
+    const int to = n + __popc(has & ((1u << lane) - 1));
+    if ((has >> lane & 1) && to < 32) {
+      codes[to] = c;
+      few[64 + to] = i0 + lane;
+    }
+    n += __popc(has);
   }
   __syncwarp();
   int mine = -1;
+  if (n <= 32) {
+    const unsigned long long own = lane < n ? codes[lane] : 0;
+    const int index = lane < n ? (int)few[64 + lane] : -1;
+    int before = 0;
+    for (int j = 0; j < n; ++j) before += codes[j] > own || (codes[j] == own && j < lane);
+    __syncwarp();
+    if (lane < n) few[before] = index;
+    __syncwarp();
+    if (lane < min(n, p.top)) mine = (int)few[lane];
+    __syncwarp();
+    return mine;
+  }
   for (int j = 0; j < p.top; ++j) {
     unsigned long long c = 0;
     int at = E;
@@ -140,14 +216,50 @@ __device__ __noinline__ int choose64(const RouteParams& p, const T* logits, unsi
   return mine;
 }
 
-// One token: lane j < top gets its j-th expert (-1: none) and the weight.  V = experts per lane.
+// The same for n candidates, the j-th in lane j, in the order of their indices, among which the experts are (a token in a thousand: 2 us instead of 9, for which
+// a call of many tokens waits).
+template <typename T>
+__device__ __noinline__ int order64(const RouteParams& p, const T* logits, int candidate, int n, uint32_t* few, int lane) {
+  double m = 0.0, z = 1.0;
+  if (!p.sigmoid) {
+    m = -INFINITY;
+    for (int i = lane; i < p.E; i += 32) m = fmax(m, (double)Elem<T>::to_float(logits[i]));
+    for (int o = 16; o; o >>= 1) m = fmax(m, __shfl_xor_sync(kFull, m, o));
+    z = 0.0;
+    for (int i = lane; i < p.E; i += 32) z += exp((double)Elem<T>::to_float(logits[i]) - m);
+    z = warp_sum(z);
+  }
+  unsigned long long* codes = reinterpret_cast<unsigned long long*>(few);
+  unsigned long long own = 0;
+  if (candidate >= 0) {
+    const double l = (double)Elem<T>::to_float(logits[candidate]), e = exp(p.sigmoid ? -l : l - m);
+    own = code64((p.sigmoid ? 1.0 : e) / (p.sigmoid ? 1.0 + e : z) + (double)p.bias[candidate]);
+  }
+  codes[lane] = own;
+  __syncwarp();
+  int before = 0;
+  for (int j = 0; j < n; ++j) {
+    const unsigned long long c = codes[j];
+    before += c > own || (c == own && j < lane);
+  }
+  if (candidate >= 0) few[64 + before] = candidate;
+  __syncwarp();
+  const int mine = lane < min(n, p.top) ? (int)few[64 + lane] : -1;
+  __syncwarp();
+  return mine;
+}
+
+// One token: lane j < top gets its j-th expert (-1: none) and the weight.  V = experts per lane; few: 96 words in shared memory.
 template <typename T, int V>
-__device__ __forceinline__ void route_token(const RouteParams& p, const T* logits, unsigned long long* row, int lane, int* expert, float* weight) {
+__device__ __forceinline__ void route_token(const RouteParams& p, const T* logits, unsigned long long* row, uint32_t* few, int lane, int* expert, float* weight) {
   const int E = p.E;
   float l[V];
   uint32_t u[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) l[v] = v * 32 + lane < E ? Elem<T>::to_float(logits[v * 32 + lane]) : -INFINITY;
+  float bias[V];   // (before anything is stored: the loads then wait together)
+#pragma unroll
+  for (int v = 0; v < V; ++v) bias[v] = p.bias && v * 32 + lane < E ? p.bias[v * 32 + lane] : 0.0f;
   const bool sums = p.groups > 1 && p.best == 2;
   const bool scores = p.bias != nullptr || sums;
   float m = -INFINITY, rz = 0.0f;   // softmax: the largest logit, 1 over the sum of exp(l - m)
@@ -169,7 +281,7 @@ __device__ __forceinline__ void route_token(const RouteParams& p, const T* logit
     float key = l[v];
     if (scores) {
       const float s = p.sigmoid ? sigmoid_near(l[v]) : __expf(l[v] - m) * rz;
-      if (p.bias && i < E) key = l[v] == -INFINITY ? -INFINITY : s + p.bias[i];
+      if (p.bias && i < E) key = l[v] == -INFINITY ? -INFINITY : s + bias[v];
       if (sums && i < E) {
         const float k = p.bias ? key : s;
         row32[i] = key == -INFINITY ? 0 : code32(k);
@@ -178,47 +290,48 @@ __device__ __forceinline__ void route_token(const RouteParams& p, const T* logit
     u[v] = i >= E || key == -INFINITY ? 0 : code32(key);
     if (p.groups > 1 && !sums && i < E) row32[i] = u[v];
   }
-  // how far two keys have to be apart for their rounded forms to be in the right order: 90 half units of the largest score
-  // (a sum of up to 37 terms, exp, the argument's rounding, a division), one of the sum with the bias; rounded up
-  const float room = p.sigmoid ? 0x1p-17f : 0x1p-17f * rz;
-  bool unsure = false;
+  // how far two keys have to be apart for their rounded forms to be in the right order.  Softmax: 90 half units of the largest score (a sum of up to 37
+  // terms, exp, the argument's rounding, a division; 2^-17).  Sigmoid: off by 2^-23 (s (1 - s) (2 + 1.2 |l|) + 2.5 s), at most 3.3 2^-23 (2^-20 for two).
+  // And one half unit of each sum with the bias, rounded up.
+  const float room = p.sigmoid ? 0x1p-20f : 0x1p-17f * rz;
+  bool unsure = false, unsure_group = false;
   if (p.groups > 1) {
     __syncwarp();
     // several lanes scan a group, each from another place on, so that no bank is asked twice; then they put their best two together
     const int size = E / p.groups, lanes = 32 >> p.log_groups, group = lane >> (5 - p.log_groups), each = (size + lanes - 1) / lanes;
     uint32_t rank = 0, b = 0;   // the group's best, the second
     if (group < p.groups) {
+      const uint32_t* at = row32 + group * size + (lane & (lanes - 1));
       int k = group % each;
       for (int n = 0; n < each; ++n) {
-        const int i = k * lanes + (lane & (lanes - 1));
-        const uint32_t c = i < size ? row32[group * size + i] : 0;
-        b = max(b, min(rank, c));
+        const uint32_t c = (k + 1) * lanes <= size || k * lanes + (lane & (lanes - 1)) < size ? at[k * lanes] : 0;
+        if (sums) b = max(b, min(rank, c));
         rank = max(rank, c);
         k = k + 1 == each ? 0 : k + 1;
       }
     }
     for (int o = 1; o < lanes; o *= 2) {
-      const uint32_t c = __shfl_xor_sync(kFull, rank, o), c2 = __shfl_xor_sync(kFull, b, o);
-      b = max(max(b, c2), min(rank, c));
+      const uint32_t c = __shfl_xor_sync(kFull, rank, o);
+      if (sums) b = max(max(b, __shfl_xor_sync(kFull, b, o)), min(rank, c));
       rank = max(rank, c);
     }
     if (sums && b != 0) rank = code32(value32(rank) + value32(b));
-    if (lane & (lanes - 1)) rank = 0;   // the group's first lane stands for it
+    if (lane < 32) few[lane] = 0;
     __syncwarp();
-    uint32_t on = 0, last = 0;
-    for (int k = 0; k < p.top_groups; ++k) {
-      const uint32_t c = __reduce_max_sync(kFull, rank);
-      if (c == 0) break;
-      const int i = __ffs(__ballot_sync(kFull, rank == c)) - 1;
-      on |= 1u << (i / lanes);
-      last = c;
-      if (lane == i) rank = 0;
+    if (group < p.groups) few[group] = rank;
+    __syncwarp();
+    // lane g looks after group g
+    rank = few[lane];
+    const int before = place_among(few, p.groups, rank, lane);
+    const uint32_t on = __ballot_sync(kFull, rank != 0 && before < p.top_groups);
+    if (scores) {
+      const uint32_t last = __ballot_sync(kFull, rank != 0 && before == p.top_groups - 1), next = __ballot_sync(kFull, rank != 0 && before == p.top_groups);
+      if (last && next) {
+        const float a = value32(__shfl_sync(kFull, rank, __ffs(last) - 1)), c = value32(__shfl_sync(kFull, rank, __ffs(next) - 1));
+        unsure_group = a - c <= 2 * room + 0x1p-21f * fmaxf(fabsf(a), fabsf(c));
+      }
     }
-    const uint32_t next = __reduce_max_sync(kFull, rank);
-    if (scores && next != 0 && last != 0) {
-      const float a = value32(last), b = value32(next);
-      unsure = a - b <= 2 * room + 0x1p-21f * fmaxf(fabsf(a), fabsf(b));
-    }
+    __syncwarp();
     const uint32_t inv = ((1u << 20) + size - 1) / size;   // i / size for i < 1024
 #pragma unroll
     for (int v = 0; v < V; ++v)
@@ -236,20 +349,65 @@ __device__ __forceinline__ void route_token(const RouteParams& p, const T* logit
   int mine = -1;
   uint32_t code = 0;   // lane j: the j-th key's
   const int count = p.top + (p.bias ? 1 : 0);   // with a bias the first one left out has to be far enough away, too (lane `top`, if there is one)
-  for (int j = 0; j < count; ++j) {
-    const uint32_t c = __reduce_max_sync(kFull, best);
-    if (c == 0) break;
-    const int i = __reduce_min_sync(kFull, best == c ? at * 32 + lane : INT32_MAX);
-    if (lane == j) { mine = i; code = c; }
-    if (j == 32 && lane == 31) {   // (the 33rd has no lane)
-      const float a = value32(code), b = value32(c);
-      unsure |= a - b <= room + 0x1p-22f * fmaxf(fabsf(a), fabsf(b));
+  int n = 33, candidate = -1;   // keys that reach the bound; lane j < n: the j-th of them
+  if (count <= 32) {
+    uint32_t bound = 1, left = best;
+    for (int j = 0; j < count; ++j) {   // (equal ones go together: the bound may then be lower than it could)
+      const uint32_t c = __reduce_max_sync(kFull, left);
+      if (c == 0) { bound = 1; break; }
+      bound = c;
+      if (left == c) left = 0;
     }
-    if (lane == (i & 31)) {
+    if (p.bias && bound != 1) {   // with all that could reach it, in 64 bits
+      const float b = value32(bound);
+      bound = max(1u, min(bound, code32(b - 2 * (room + 0x1p-22f * fabsf(b)))));
+    }
+    few[lane] = 0;
+    __syncwarp();
+    n = 0;
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (v == i >> 5) u[v] = 0;
-      find();
+    for (int v = 0; v < V; ++v) {   // in the order of their indices
+      const uint32_t has = __ballot_sync(kFull, u[v] >= bound);
+      const int to = n + __popc(has & ((1u << lane) - 1));
+      if (u[v] >= bound && to < 32) {
+        few[to] = u[v];
+        few[32 + to] = v * 32 + lane;
+      }
+      n += __popc(has);
+    }
+    __syncwarp();
+  }
+  if (n <= 32) {
+    const uint32_t own = few[lane];
+    const int before = place_among(few, n, own, lane);
+    candidate = lane < n ? (int)few[32 + lane] : -1;
+    __syncwarp();
+    if (lane < n) {
+      few[before] = own;
+      few[32 + before] = candidate;
+    }
+    __syncwarp();
+    if (lane < min(n, count)) {
+      code = few[lane];
+      mine = (int)few[32 + lane];
+    }
+    __syncwarp();
+  } else {   // many of them, or many to take: one by one
+    for (int j = 0; j < count; ++j) {
+      const uint32_t c = __reduce_max_sync(kFull, best);
+      if (c == 0) break;
+      const int i = __reduce_min_sync(kFull, best == c ? at * 32 + lane : INT32_MAX);
+      if (lane == j) { mine = i; code = c; }
+      if (j == 32 && lane == 31) {   // (the 33rd has no lane)
+        const float a = value32(code), b = value32(c);
+        unsure |= a - b <= room + 0x1p-22f * fmaxf(fabsf(a), fabsf(b));
+      }
+      if (lane == (i & 31)) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (v == i >> 5) u[v] = 0;
+        find();
+      }
     }
   }
   float lj = mine >= 0 ? Elem<T>::to_float(logits[mine]) : -INFINITY;
@@ -262,23 +420,23 @@ __device__ __forceinline__ void route_token(const RouteParams& p, const T* logit
       unsure |= a - b <= room + 0x1p-22f * fmaxf(fabsf(a), fabsf(b));
     }
   }
-  if (scores && __any_sync(kFull, unsure)) {
-    mine = choose64(p, logits, row, lane);
+  if (scores && __any_sync(kFull, unsure || unsure_group)) {
+    if (n <= 32 && !unsure_group) mine = order64<T>(p, logits, candidate, n, few, lane);
+    else mine = choose64<T, V>(p, logits, row, few, lane);
     lj = mine >= 0 ? Elem<T>::to_float(logits[mine]) : -INFINITY;
   }
   if (lane >= p.top) { mine = -1; lj = -INFINITY; }
   float w;
   if (p.renormalize) {   // ratios, which neither the other experts nor small scores touch
-    const float top = warp_max(lj);
+    const float top = first_max(lj, p.top2);
     if (p.sigmoid) {
-      const float far = fminf(top, 0.0f);   // sigmoid(l) exp(-far) = exp(l - far) / (1 + exp(l))
-      w = lj > 0.0f ? sigmoid(lj) : expf(lj - far) / (1.0f + expf(lj));
+      w = sigmoid_over(lj, fminf(top, 0.0f));
     } else {
       w = expf(lj - top);
     }
     if (mine < 0) w = 0.0f;
     else if (lj != lj) w = lj;
-    const float sum = warp_sum(w);
+    const float sum = first_sum(w, p.top2);
     w = mine < 0 ? 0.0f : w / sum;
   } else {
     w = p.sigmoid ? sigmoid(lj) : expf(lj - m) * rz;
@@ -388,8 +546,9 @@ __global__ void __launch_bounds__(V > 16 ? 512 : 1024) route_kernel(const RouteP
   asm volatile("griddepcontrol.launch_dependents;");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, bins = p.E + 1;
   const bool rows = p.bias != nullptr || p.groups > 1;
-  unsigned long long* row = reinterpret_cast<unsigned long long*>(smem) + (size_t)warp * p.E;
-  uint32_t* hist = reinterpret_cast<uint32_t*>(smem + (rows ? (size_t)warps * p.E * 8 : 0));
+  unsigned long long* row = reinterpret_cast<unsigned long long*>(smem) + (size_t)warp * (p.E + p.E % 2);
+  uint32_t* few = reinterpret_cast<uint32_t*>(smem + (rows ? (size_t)warps * (p.E + p.E % 2) * 8 : 0)) + warp * 96;
+  uint32_t* hist = few - warp * 96 + warps * 96;
   uint32_t* mine = hist + (size_t)warp * bins;
   for (int e = lane; e < bins; e += 32) mine[e] = 0;
   __syncwarp();
@@ -399,7 +558,7 @@ __global__ void __launch_bounds__(V > 16 ? 512 : 1024) route_kernel(const RouteP
   for (int64_t t = lo; t < hi; ++t) {
     int e;
     float w;
-    route_token<T, V>(p, static_cast<const T*>(p.logits) + t * p.E, row, lane, &e, &w);
+    route_token<T, V>(p, static_cast<const T*>(p.logits) + t * p.E, row, few, lane, &e, &w);
     const uint32_t none = __ballot_sync(kFull, lane < p.top && e < 0);
     if (lane < p.top) {
       const int bin = e < 0 ? p.E : e;
@@ -476,26 +635,33 @@ __global__ void __launch_bounds__(1024) place_kernel(const SortParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ uint32_t warp_sums[32];
   const int bins = p.n + 1, quads = pitch(bins) / 4;
-  uint32_t *base = reinterpret_cast<uint32_t*>(smem), *total = base + 4 * quads, *before = total + 4 * quads;
-  for (int e = threadIdx.x; e < 4 * quads; e += blockDim.x) { total[e] = 0; before[e] = 0; }
-  asm volatile("griddepcontrol.wait;" ::: "memory");   // the first launch's results
-  __syncthreads();
-  // threads by (part of the blocks, four bins); sums of integers in shared memory, whose order does not matter
+  // threads by (part of the blocks, four bins), then by bins
   const int parts = max(1, (int)blockDim.x / quads);
+  uint32_t *base = reinterpret_cast<uint32_t*>(smem), *total = base + 4 * quads, *before = total + 4 * quads;
+  uint4 *alls = reinterpret_cast<uint4*>(before + 4 * quads), *mines = alls + parts * quads;
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the first launch's results
   for (int i = threadIdx.x; i < parts * quads; i += blockDim.x) {
     const int part = i / quads, e = i % quads;
     uint4 all = make_uint4(0, 0, 0, 0), mine = all;
-#pragma unroll 4
+#pragma unroll 10
     for (int b = part; b < p.blocks; b += parts) {
       const uint4 v = reinterpret_cast<const uint4*>(p.hist)[(size_t)b * quads + e];
       all.x += v.x; all.y += v.y; all.z += v.z; all.w += v.w;
       if (b < (int)blockIdx.x) { mine.x += v.x; mine.y += v.y; mine.z += v.z; mine.w += v.w; }
     }
-    atomicAdd(&total[4 * e], all.x); atomicAdd(&total[4 * e + 1], all.y); atomicAdd(&total[4 * e + 2], all.z); atomicAdd(&total[4 * e + 3], all.w);
-    atomicAdd(&before[4 * e], mine.x); atomicAdd(&before[4 * e + 1], mine.y); atomicAdd(&before[4 * e + 2], mine.z); atomicAdd(&before[4 * e + 3], mine.w);
+    alls[i] = all;
+    mines[i] = mine;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < bins; e += blockDim.x) base[e] = total[e];
+  for (int e = threadIdx.x; e < bins; e += blockDim.x) {
+    uint32_t all = 0, mine = 0;
+    for (int k = 0; k < parts; ++k) {
+      all += reinterpret_cast<const uint32_t*>(alls)[k * 4 * quads + e];
+      mine += reinterpret_cast<const uint32_t*>(mines)[k * 4 * quads + e];
+    }
+    total[e] = base[e] = all;
+    before[e] = mine;
+  }
   __syncthreads();
   block_scan(base, bins, warp_sums);
   for (int e = threadIdx.x; e < bins; e += blockDim.x) base[e] += before[e];
@@ -511,7 +677,8 @@ int allow_smem(K kern, size_t bytes) {
 
 // Launched while the first kernel runs, whose last blocks it waits for.
 int place(const SortParams& s, cudaStream_t st) {
-  const size_t smem = (size_t)3 * pitch(s.n + 1) * 4;
+  const int quads = pitch(s.n + 1) / 4;
+  const size_t smem = (size_t)quads * 16 * (3 + 2 * std::max(1, 1024 / quads));
   if (int rc = allow_smem(place_kernel, smem)) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(s.blocks);
@@ -569,7 +736,7 @@ __global__ void __launch_bounds__(256) dlogits_kernel(const DlogitsParams p) {
     float q = 0.0f;
     if (p.renormalize) {
       const float top = warp_max(lj);
-      if (p.sigmoid) q = lj > 0.0f ? sigmoid(lj) : expf(lj - fminf(top, 0.0f)) / (1.0f + expf(lj));
+      if (p.sigmoid) q = sigmoid_over(lj, fminf(top, 0.0f));
       else q = expf(lj - top);
       if (e < 0) q = 0.0f;
       else if (lj != lj) q = lj;
@@ -589,7 +756,7 @@ __global__ void __launch_bounds__(256) dlogits_kernel(const DlogitsParams p) {
 template <typename T>
 int launch_route(const RouteParams& p, int blocks, int warps, cudaStream_t st) {
   const bool rows = p.bias != nullptr || p.groups > 1;
-  const size_t smem = (rows ? (size_t)warps * p.E * 8 : 0) + (size_t)(warps + 2) * (p.E + 1) * 4;
+  const size_t smem = (rows ? (size_t)warps * (p.E + p.E % 2) * 8 : 0) + warps * 384 + (size_t)(warps + 2) * (p.E + 1) * 4;
   auto go = [&](auto kern) {
     if (int rc = allow_smem(kern, smem)) return rc;
     kern<<<blocks, warps * 32, smem, st>>>(p);
@@ -678,10 +845,11 @@ extern "C" int b200q_route(const void* logits, int dtype, int64_t T, int64_t E, 
   if (need > 0 && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16 != 0))
     return fail(B200Q_ERR_WORKSPACE, "[%s] an aligned workspace of %zu bytes required, %zu given", tag, need, ws ? ws_bytes : (size_t)0);
   if (top_groups == groups) groups = top_groups = 1;   // nothing to leave out
-  int log_groups = 0;
+  int log_groups = 0, top2 = 1;
   while (1 << log_groups < groups) ++log_groups;
+  while (top2 < top) top2 *= 2;
   const RouteParams p{logits, bias, weights, experts, sizes, places, order, static_cast<uint32_t*>(ws), T, s.per_block, s.per_warp,
-                      (int)E, (int)top, (int)groups, log_groups, (int)top_groups, group_best, scoring == B200Q_SIGMOID, renormalize != 0, scale};
+                      (int)E, (int)top, top2, (int)groups, log_groups, (int)top_groups, group_best, scoring == B200Q_SIGMOID, renormalize != 0, scale};
   const ScratchLock lock(ws);
   int rc = dtype == B200Q_F32 ? launch_route<float>(p, s.blocks, s.warps, st)
                               : (dtype == B200Q_F16 ? launch_route<__half>(p, s.blocks, s.warps, st) : launch_route<__nv_bfloat16>(p, s.blocks, s.warps, st));
