@@ -234,6 +234,7 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) down_kernel(const P
   constexpr int kRanks = D::kRanks, kStages = D::kStages, kLine = D::kLine, kStageBytes = D::kPieces * 512;
   extern __shared__ __align__(16) unsigned char smem[];
   cg::cluster_group cluster = cg::this_cluster();
+  asm volatile("griddepcontrol.launch_dependents;");   // the second product's blocks begin with what does not depend on this one
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
   const int part = (int)(blockIdx.x % p.split);
   const int4 tile = tile_of(p, blockIdx.x / p.split);
@@ -489,10 +490,17 @@ __global__ void __launch_bounds__(kThreads, (KS == 4 ? 2 : 3) - std::is_same_v<T
     commit();
     ++ahead;
   };
-  copy_h(k, 0);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kUpStages - 1; ++i) issue();   // the first group has the first tile's h
+  for (int i = 0; i < kUpStages - 1; ++i) issue();
+  if (!CHUNKED && k < p.each && tiles[k].x >= 0) {
+    loaded = tiles[k].x;
+    w = static_cast<const T*>(p.w) + (int64_t)loaded * p.r * C;
+    weights(0);
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // all of h, of the launch before
+  copy_h(k, 0);
+  commit();
   for (int last = 4; k < p.each;) {
     const int4 tile = tiles[k];
     const bool plain = tile.x < 0;   // rows without an adapter
@@ -506,8 +514,7 @@ __global__ void __launch_bounds__(kThreads, (KS == 4 ? 2 : 3) - std::is_same_v<T
       }
     }
     // the group with this tile's h was issued with the first step of the tile before, four steps ago if that was a whole one
-    if (now == 0) wait_all_but<kUpStages - 2>();
-    else if (last < 4) wait_all_but<0>();
+    if (now == 0 || last < 4) wait_all_but<0>();
     __syncthreads();
     const int after = next_tile(k + 1);
     copy_h(after, buffer ^ 1);
@@ -728,7 +735,7 @@ int tiles_per_block(const Params& p, int64_t cols, int64_t slots) {
 }
 
 template <typename K>
-int launch(K kern, const Params& p, dim3 grid, int threads, size_t smem, cudaStream_t st) {
+int launch(K kern, const Params& p, dim3 grid, int threads, size_t smem, cudaStream_t st, bool beside = false) {
   if (smem > 40 * 1024) B200Q_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
@@ -736,11 +743,15 @@ int launch(K kern, const Params& p, dim3 grid, int threads, size_t smem, cudaStr
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
+  cfg.attrs = at;
   if (p.split > 1) {
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = p.split;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
+    cfg.numAttrs = 1;
+  } else if (beside) {   // may start while the launch before runs, whose results it waits for
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 1;
   }
   B200Q_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p));
@@ -763,10 +774,10 @@ int up(Params p, cudaStream_t st) {
   const int64_t cols = (p.C + 255) / 256;
   p.each = tiles_per_block(p, cols, 148 * ((p.r > 32 ? 2 : 3) - std::is_same_v<T, __half>));
   const dim3 grid((unsigned)((p.tiles_n + p.each - 1) / p.each * cols));
-  if (p.r <= 16) return launch(up_kernel<T, WIDE, WHOLE, 1, false>, p, grid, kThreads, Up<1, false>::kBytes, st);
-  if (p.r <= 32) return launch(up_kernel<T, WIDE, WHOLE, 2, false>, p, grid, kThreads, Up<2, false>::kBytes, st);
-  if (p.r <= 64) return launch(up_kernel<T, WIDE, WHOLE, 4, false>, p, grid, kThreads, Up<4, false>::kBytes, st);
-  return launch(up_kernel<T, WIDE, WHOLE, 4, true>, p, grid, kThreads, Up<4, true>::kBytes, st);
+  if (p.r <= 16) return launch(up_kernel<T, WIDE, WHOLE, 1, false>, p, grid, kThreads, Up<1, false>::kBytes, st, true);
+  if (p.r <= 32) return launch(up_kernel<T, WIDE, WHOLE, 2, false>, p, grid, kThreads, Up<2, false>::kBytes, st, true);
+  if (p.r <= 64) return launch(up_kernel<T, WIDE, WHOLE, 4, false>, p, grid, kThreads, Up<4, false>::kBytes, st, true);
+  return launch(up_kernel<T, WIDE, WHOLE, 4, true>, p, grid, kThreads, Up<4, true>::kBytes, st, true);
 }
 template <typename T, bool TALL, bool WHOLE>
 int outer(Params p, cudaStream_t st) {

@@ -492,16 +492,8 @@ __device__ __forceinline__ int bin_of(const SortParams& p, int64_t i) {
   const int64_t e = p.bytes == 8 ? static_cast<const int64_t*>(p.ids)[i] : static_cast<const int*>(p.ids)[i];
   return e >= 0 && e < p.n ? (int)e : p.n;
 }
-// base: where the block's first pair of every bin goes; total: the bins' sizes (block 0 alone needs them, its own base being the bins' starts)
-__device__ void sort_finish(const SortParams& p, int block, const uint32_t* base, uint32_t* total, uint32_t* warp_sums) {
-  const int64_t lo = block * p.per_block, hi = min(lo + p.per_block, p.P);
-  for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) {
-    const int e = bin_of(p, i);
-    const uint32_t at = p.rank[i] + base[e];
-    if (p.places) p.places[i] = e < p.n ? (int)at : -1;
-    p.order[at] = e < p.n ? (int)i : (int)(-1 - i);
-  }
-  if (block != 0) return;
+// The bins' sizes, starts and tiles, by one block.  base: the bins' starts; total: their sizes
+__device__ void sort_tables(const SortParams& p, const uint32_t* base, uint32_t* total, uint32_t* warp_sums) {
   for (int e = threadIdx.x; e <= p.n; e += blockDim.x) {
     if (e < p.n) p.sizes[e] = (int)total[e];
     if (p.starts) p.starts[e] = (int)base[e];
@@ -523,6 +515,18 @@ __device__ void sort_finish(const SortParams& p, int block, const uint32_t* base
     const int have = first < end ? (int)min(end - first, (uint32_t)kAdapterRows) : 0;
     p.tiles[k] = make_int4(a < p.n ? a : -1, (int)first, have, (int)starts_of_none);
   }
+}
+
+// base: where the block's first pair of every bin goes; total: the bins' sizes (block 0 alone needs them, its own base being the bins' starts)
+__device__ void sort_finish(const SortParams& p, int block, const uint32_t* base, uint32_t* total, uint32_t* warp_sums) {
+  const int64_t lo = block * p.per_block, hi = min(lo + p.per_block, p.P);
+  for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) {
+    const int e = bin_of(p, i);
+    const uint32_t at = p.rank[i] + base[e];
+    if (p.places) p.places[i] = e < p.n ? (int)at : -1;
+    p.order[at] = e < p.n ? (int)i : (int)(-1 - i);
+  }
+  if (block == 0) sort_tables(p, base, total, warp_sums);
 }
 
 // hist: of every warp of the block [warps][bins].  Becomes the sums before every warp; the block's own sums go to `sums`.
@@ -628,6 +632,45 @@ __global__ void __launch_bounds__(1024) group_kernel(const SortParams p, int64_t
   __syncthreads();
   block_scan(sums, bins, warp_sums);
   sort_finish(p, 0, sums, total, warp_sums);
+}
+
+// Up to 128 rows per warp in one block: ids and ranks stay in registers.
+__global__ void __launch_bounds__(1024) group_few_kernel(const SortParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ uint32_t warp_sums[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, bins = p.n + 1, rows = (int)p.P;
+  uint32_t* hist = reinterpret_cast<uint32_t*>(smem);
+  uint32_t* mine = hist + (size_t)warp * bins;
+  const int each = ((rows + warps - 1) / warps + 31) / 32, lo = warp * each * 32 + lane;
+  int e[4];
+  uint32_t rank[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) e[k] = k < each && lo + k * 32 < rows ? bin_of(p, lo + k * 32) : -1;
+  for (int i = lane; i < bins; i += 32) mine[i] = 0;
+  __syncwarp();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (k >= each) break;
+    const uint32_t same = __match_any_sync(kFull, e[k]);
+    if (e[k] >= 0) rank[k] = mine[e[k]] + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (e[k] >= 0 && lane == __ffs(same) - 1) mine[e[k]] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  uint32_t *base = hist + (size_t)warps * bins, *total = base + bins;
+  sum_over_warps(hist, bins, base);
+  __syncthreads();
+  for (int i = threadIdx.x; i < bins; i += blockDim.x) total[i] = base[i];
+  __syncthreads();
+  block_scan(base, bins, warp_sums);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (e[k] >= 0) {
+      const int i = lo + k * 32;
+      p.order[rank[k] + mine[e[k]] + base[e[k]]] = e[k] < p.n ? i : -1 - i;
+    }
+  sort_tables(p, base, total, warp_sums);
 }
 
 // The second launch: every block adds up the histograms of those before it.
@@ -908,6 +951,12 @@ extern "C" int b200q_group_rows(const void* ids, int id_bytes, int64_t T, int64_
   uint32_t* rank = static_cast<uint32_t*>(ws);
   const SortParams p{ids, id_bytes, rank, rank + pitch(T), sizes, starts, nullptr, order, reinterpret_cast<int4*>(tiles), b200q_group_rows_tiles(T, n), T, s.per_block, (int)n, s.blocks};
   const size_t smem = (size_t)(s.warps + 2) * (n + 1) * 4;
+  if (T <= 128 * s.warps && s.blocks == 1) {
+    if (int rc = allow_smem(group_few_kernel, smem)) return rc;
+    group_few_kernel<<<1, s.warps * 32, smem, st>>>(p);
+    B200Q_LAUNCH_OK("group_few_kernel");
+    return B200Q_OK;
+  }
   const ScratchLock lock(ws);
   if (int rc = allow_smem(group_kernel, smem)) return rc;
   group_kernel<<<s.blocks, s.warps * 32, smem, st>>>(p, s.per_warp);
