@@ -2,8 +2,8 @@
 
     python examples/moe_layer.py [--tokens 2048] [--experts 8] [--top 2] [--width 1024] [--hidden 2048] [--steps 20] [--mode nvfp4]
 
-Tokens are sorted by expert once; both projections, their gradients and the 4-bit products then work on rows sorted by
-expert with the experts' row counts on the device: no padding, no capacity, no synchronisation with the host.
+The router chooses every token's experts and sorts the pairs by expert once; both projections, their gradients and the 4-bit products then
+work on rows sorted by expert with the experts' row counts on the device: no padding, no capacity, no synchronisation with the host.
 """
 import argparse
 import os
@@ -16,15 +16,6 @@ import mlx_b200 as mb  # noqa: E402
 from mlx_b200 import grad  # noqa: E402
 
 
-def route(logits, top):
-    """-> (rows of the tokens in expert order, their weights, rows per expert)."""
-    weight, expert = torch.softmax(logits.float(), -1).topk(top, -1)
-    order = expert.flatten().argsort(stable=True)
-    sizes = torch.zeros(logits.shape[-1], dtype=torch.int64, device=logits.device)
-    sizes.scatter_add_(0, expert.flatten(), torch.ones_like(expert.flatten()))
-    return order // top, weight.flatten()[order], sizes
-
-
 class Layer:
     def __init__(self, experts, width, hidden, gen):
         def weights(*shape):
@@ -33,10 +24,9 @@ class Layer:
         self.router, self.up, self.down = weights(experts, width), weights(experts, hidden, width), weights(experts, width, hidden)
 
     def __call__(self, x, top):
-        rows, weight, sizes = route(x @ self.router.T, top)
-        h = torch.nn.functional.silu(grad.grouped_mm(x[rows], self.up, sizes))
-        y = grad.grouped_mm(h, self.down, sizes) * weight[:, None].to(x.dtype)
-        return torch.zeros_like(x).index_add(0, rows, y)
+        r = grad.route_experts(x @ self.router.T, top)
+        h = torch.nn.functional.silu(grad.grouped_mm(grad.dispatch_rows(x, r), self.up, r.sizes))
+        return grad.combine_rows(grad.grouped_mm(h, self.down, r.sizes), r)
 
     def parameters(self):
         return [self.router, self.up, self.down]
@@ -53,16 +43,15 @@ class Served:
             g = self.scale(w)
             self.weights.append((*mb.quantize(w.detach(), mode=mode, global_scale=g), g))
         # scales of the activations, as calibration on x finds them
-        rows, _, sizes = route(x @ self.router.T, 1)
+        r = mb.route_experts(x @ self.router.T, 1)
         self.gx = self.scale(x)
-        self.gh = self.scale(torch.nn.functional.silu(mb.grouped_mm(x[rows], layer.up.detach(), sizes)))
+        self.gh = self.scale(torch.nn.functional.silu(mb.grouped_mm(mb.dispatch_rows(x, r), layer.up.detach(), r.sizes)))
 
     def __call__(self, x, top):
-        rows, weight, sizes = route(x @ self.router.T, top)
+        r = mb.route_experts(x @ self.router.T, top)
         (uq, us, ug), (dq, ds, dg) = self.weights
-        h = torch.nn.functional.silu(mb.grouped_qqmm(x[rows], uq, us, sizes, mode=self.mode, global_scale_x=self.gx, global_scale_w=ug))
-        y = mb.grouped_qqmm(h, dq, ds, sizes, mode=self.mode, global_scale_x=self.gh, global_scale_w=dg) * weight[:, None].to(x.dtype)
-        return torch.zeros_like(x).index_add(0, rows, y)
+        h = torch.nn.functional.silu(mb.grouped_qqmm(mb.dispatch_rows(x, r), uq, us, r.sizes, mode=self.mode, global_scale_x=self.gx, global_scale_w=ug))
+        return mb.combine_rows(mb.grouped_qqmm(h, dq, ds, r.sizes, mode=self.mode, global_scale_x=self.gh, global_scale_w=dg), r)
 
 
 def run(tokens=2048, experts=8, top=2, width=1024, hidden=2048, steps=20, mode="nvfp4", seed=0):

@@ -1,6 +1,6 @@
 // C++ host shim over the C ABI of b200q.h with the shape of the reference's operator functions
 // (mlx/ops.cpp: quantize :5208-5245, dequantize :5465-5517, quantized_matmul :4784-4834,
-// gather_qmm :5553-5629; qqmm and the grouped products in the same manner): same argument meaning, same validation (mlx/ops.cpp:110-181,
+// gather_qmm :5553-5629; qqmm, the grouped products, routing and adapters in the same manner): same argument meaning, same validation (mlx/ops.cpp:110-181,
 // 4704-4754), std::invalid_argument where the reference throws it and std::runtime_error for
 // everything the library reports later.  Arrays are non-owning views of row-contiguous device
 // memory; outputs and scratch are allocated by the caller (the reference's eval_gpu does that
@@ -319,6 +319,152 @@ inline void grouped_mm_dw(const ArrayView& dy, const ArrayView& x, const ArrayVi
   const ArrayView &a = transpose ? dy : x, &b = transpose ? x : dy;
   detail::check(b200q_grouped_mm_dw(a.data, b.data, sizes.data, bytes, dw.data, (int)x.dtype, x.dim(0), sizes.dim(0), a.dim(1), b.dim(1), ws.data,
                                     ws.bytes, stream));
+}
+
+// ---- routing to experts, rows between tokens and experts, adapters (b200q_route and so on say what they compute)
+enum class Scoring : int { softmax = B200Q_SOFTMAX, sigmoid = B200Q_SIGMOID };
+// What route_experts writes: weights float32 [.., top]; experts, places int32 [.., top]; sizes int32 [E]; order int32 [tokens * top]
+struct Routing {
+  ArrayView weights, experts, sizes, places, order;
+};
+// What group_rows writes, int32: sizes [n], starts [n + 1], order [rows], tiles [b200q_group_rows_tiles(rows, n), 4]
+struct RowGroups {
+  ArrayView sizes, starts, order, tiles;
+};
+struct RouteOptions {
+  Scoring scoring = Scoring::softmax;
+  ArrayView bias = {};   // float32 [E]; empty: none
+  int64_t groups = 1, top_groups = 1;
+  int group_best = 1;
+  bool renormalize = false;
+  float scale = 1.0f;
+};
+namespace detail {
+inline int32_t* i32(const ArrayView& a) { return static_cast<int32_t*>(a.data); }
+inline float* f32(const ArrayView& a) { return static_cast<float*>(a.data); }
+inline int64_t rows_of(const ArrayView& a) {
+  int64_t n = 1;
+  for (int i = 0; i < a.ndim() - 1; ++i) n *= a.shape[i];
+  return n;
+}
+inline bool same_rows(const ArrayView& a, const ArrayView& b) {
+  bool ok = a.ndim() >= 1 && a.ndim() == b.ndim();
+  for (int i = 0; ok && i < a.ndim() - 1; ++i) ok = a.shape[i] == b.shape[i];
+  return ok;
+}
+// places [.., top] and order [tokens * top]; -> top
+inline int64_t plan(const char* tag, const Routing& r) {
+  if (r.places.dtype != Dtype::int32 || r.order.dtype != Dtype::int32 || r.places.ndim() < 1 || r.order.ndim() != 1 || r.order.dim(0) != r.places.size())
+    throw std::invalid_argument(std::string("[") + tag + "] places and order are int32, with one entry per pair each");
+  return r.places.dim(-1);
+}
+inline void row_groups(const char* tag, const RowGroups& g, int64_t rows, int64_t n) {
+  validate_result(tag, g.sizes, n, Dtype::int32);
+  validate_result(tag, g.starts, n + 1, Dtype::int32);
+  validate_result(tag, g.order, rows, Dtype::int32);
+  validate_result(tag, g.tiles, 4 * b200q_group_rows_tiles(rows, n), Dtype::int32);
+}
+struct AdapterDims {
+  int64_t T, L, N, K, r;
+};
+inline AdapterDims adapters(const char* tag, const ArrayView& y, const ArrayView& x, const ArrayView& a, const ArrayView& b, const RowGroups& g, const ArrayView& scales) {
+  if (a.ndim() != 3 || b.ndim() != 3 || !same_rows(x, y) || a.dim(0) != b.dim(0) || a.dim(1) != b.dim(2) || x.dim(-1) != a.dim(2) || y.dim(-1) != b.dim(1))
+    throw std::invalid_argument(std::string("[") + tag + "] The shapes of y " + shape_str(y.shape) + ", x " + shape_str(x.shape) + ", a " + shape_str(a.shape) + " and b " +
+                                shape_str(b.shape) + " do not match");
+  if (y.dtype != x.dtype || a.dtype != x.dtype || b.dtype != x.dtype) throw std::invalid_argument(std::string("[") + tag + "] y, x, a and b must be of one type");
+  const AdapterDims d{rows_of(x), a.dim(0), b.dim(1), a.dim(2), a.dim(1)};
+  row_groups(tag, g, d.T, d.L);
+  if (scales.data) validate_result(tag, scales, d.L, Dtype::float32);
+  return d;
+}
+inline void* inner(const char* tag, const Workspace& h, const AdapterDims& d) {
+  if (h.bytes < b200q_add_adapters_inner_bytes(d.T, d.r)) throw std::runtime_error(std::string("[") + tag + "] the buffer of inner products is too small");
+  return h.data;
+}
+}  // namespace detail
+
+// logits [.., E] -> out
+inline void route_experts(const ArrayView& logits, Routing& out, const Workspace& ws, const RouteOptions& o = {}, void* stream = nullptr) {
+  if (!is_floating(logits.dtype) || logits.ndim() < 1 || !detail::same_rows(logits, out.experts))
+    throw std::invalid_argument("[route_experts] logits " + detail::shape_str(logits.shape) + " do not match the experts " + detail::shape_str(out.experts.shape));
+  const int64_t T = detail::rows_of(logits), E = logits.dim(-1), top = out.experts.dim(-1);
+  detail::validate_result("route_experts", out.weights, T * top, Dtype::float32);
+  for (const ArrayView* v : {&out.experts, &out.places, &out.order}) detail::validate_result("route_experts", *v, T * top, Dtype::int32);
+  detail::validate_result("route_experts", out.sizes, E, Dtype::int32);
+  if (o.bias.data) detail::validate_result("route_experts", o.bias, E, Dtype::float32);
+  detail::check(b200q_route(logits.data, (int)logits.dtype, T, E, top, (int)o.scoring, detail::f32(o.bias), o.groups, o.top_groups, o.group_best, o.renormalize,
+                            o.scale, detail::f32(out.weights), detail::i32(out.experts), detail::i32(out.sizes), detail::i32(out.places), detail::i32(out.order),
+                            ws.data, ws.bytes, stream));
+}
+
+// The gradient with respect to the logits of the weights' gradient dw [.., top]
+inline void route_dlogits(const ArrayView& dw, const ArrayView& logits, const ArrayView& experts, ArrayView& dlogits, const RouteOptions& o = {}, void* stream = nullptr) {
+  if (!is_floating(logits.dtype) || logits.ndim() < 1 || !detail::same_rows(logits, experts) || experts.dtype != Dtype::int32)
+    throw std::invalid_argument("[route_dlogits] logits " + detail::shape_str(logits.shape) + " do not match the experts " + detail::shape_str(experts.shape));
+  detail::validate_result("route_dlogits", dw, experts.size(), Dtype::float32);
+  detail::validate_result("route_dlogits", dlogits, logits.size(), logits.dtype);
+  detail::check(b200q_route_dlogits(detail::f32(dw), logits.data, (int)logits.dtype, detail::i32(experts), detail::rows_of(logits), logits.dim(-1), experts.dim(-1),
+                                    (int)o.scoring, o.renormalize, o.scale, dlogits.data, stream));
+}
+
+// x [.., D] -> xs [tokens * top, D]
+inline void dispatch_rows(const ArrayView& x, const Routing& r, ArrayView& xs, void* stream = nullptr) {
+  const int64_t top = detail::plan("dispatch_rows", r);
+  if (!detail::same_rows(x, r.places)) throw std::invalid_argument("[dispatch_rows] x " + detail::shape_str(x.shape) + " does not have a row for every token");
+  if (is_floating(x.dtype)) detail::validate_result("dispatch_rows", xs, r.order.size() * x.dim(-1), x.dtype);
+  detail::check(b200q_dispatch_rows(x.data, (int)x.dtype, detail::rows_of(x), top, x.dim(-1), detail::i32(r.places), detail::i32(r.order), xs.data, stream));
+}
+
+// y [tokens * top, D] -> out [.., D]
+inline void combine_rows(const ArrayView& y, const Routing& r, ArrayView& out, bool weighted = true, void* stream = nullptr) {
+  const int64_t top = detail::plan("combine_rows", r);
+  if (y.ndim() != 2 || y.dim(0) != r.order.dim(0)) throw std::invalid_argument("[combine_rows] y " + detail::shape_str(y.shape) + " does not have a row for every pair");
+  if (weighted) detail::validate_result("combine_rows", r.weights, r.places.size(), Dtype::float32);
+  if (is_floating(y.dtype)) detail::validate_result("combine_rows", out, detail::rows_of(r.places) * y.dim(1), y.dtype);
+  detail::check(b200q_combine_rows(y.data, (int)y.dtype, detail::rows_of(r.places), top, y.dim(1), detail::i32(r.places), weighted ? detail::f32(r.weights) : nullptr,
+                                   out.data, stream));
+}
+
+// Gradients of combine_rows; dys and dw may be empty views: not wanted
+inline void combine_rows_grad(const ArrayView& dy, const ArrayView& y, const Routing& r, ArrayView& dys, ArrayView& dw, void* stream = nullptr) {
+  const int64_t top = detail::plan("combine_rows_grad", r);
+  if (y.ndim() != 2 || y.dim(0) != r.order.dim(0) || dy.dtype != y.dtype || dy.ndim() < 1 || dy.dim(-1) != y.dim(1) || !detail::same_rows(dy, r.places))
+    throw std::invalid_argument("[combine_rows_grad] dy " + detail::shape_str(dy.shape) + " does not match the result of combine_rows");
+  detail::validate_result("combine_rows_grad", r.weights, r.places.size(), Dtype::float32);
+  if (dys.data) detail::validate_result("combine_rows_grad", dys, y.size(), y.dtype);
+  if (dw.data) detail::validate_result("combine_rows_grad", dw, r.places.size(), Dtype::float32);
+  detail::check(b200q_combine_rows_grad(dy.data, y.data, (int)y.dtype, detail::rows_of(r.places), top, y.dim(1), detail::i32(r.places), detail::i32(r.order),
+                                        detail::f32(r.weights), dys.data, detail::f32(dw), stream));
+}
+
+// ids [..] int32 or int64 -> out
+inline void group_rows(const ArrayView& ids, int64_t n, RowGroups& out, const Workspace& ws, void* stream = nullptr) {
+  if (ids.dtype != Dtype::int32 && ids.dtype != Dtype::int64) throw std::invalid_argument(std::string("[group_rows] ids must be int32 or int64 but are ") + name(ids.dtype));
+  if (n < 0) throw std::invalid_argument("[group_rows] a negative number of groups");
+  detail::row_groups("group_rows", out, ids.size(), n);
+  detail::check(b200q_group_rows(ids.data, ids.dtype == Dtype::int64 ? 8 : 4, ids.size(), n, detail::i32(out.sizes), detail::i32(out.starts), detail::i32(out.order),
+                                 detail::i32(out.tiles), ws.data, ws.bytes, stream));
+}
+
+// y [.., N] + adapters of x [.., K] -> out (which may be y); a [L, r, K], b [L, N, r]; h: b200q_add_adapters_inner_bytes bytes, left for the gradient
+inline void add_adapters(const ArrayView& y, const ArrayView& x, const ArrayView& a, const ArrayView& b, const RowGroups& groups, const Workspace& h, ArrayView& out,
+                         const ArrayView& scales = {}, void* stream = nullptr) {
+  const auto d = detail::adapters("add_adapters", y, x, a, b, groups, scales);
+  if (is_floating(x.dtype)) detail::validate_result("add_adapters", out, d.T * d.N, x.dtype);
+  detail::check(b200q_add_adapters(y.data, x.data, a.data, b.data, (int)x.dtype, d.T, d.L, d.N, d.K, d.r, detail::i32(groups.order), detail::i32(groups.tiles),
+                                   detail::f32(scales), detail::inner("add_adapters", h, d), out.data, stream));
+}
+
+// Gradients of add_adapters (that of y is dy); dx, da and db may be empty views: not wanted.  g: scratch as large as h
+inline void add_adapters_grad(const ArrayView& dy, const ArrayView& x, const ArrayView& a, const ArrayView& b, const RowGroups& groups, const Workspace& h,
+                              const Workspace& g, ArrayView& dx, ArrayView& da, ArrayView& db, const ArrayView& scales = {}, void* stream = nullptr) {
+  const auto d = detail::adapters("add_adapters_grad", dy, x, a, b, groups, scales);
+  if (dx.data) detail::validate_result("add_adapters_grad", dx, x.size(), x.dtype);
+  if (da.data) detail::validate_result("add_adapters_grad", da, a.size(), x.dtype);
+  if (db.data) detail::validate_result("add_adapters_grad", db, b.size(), x.dtype);
+  detail::check(b200q_add_adapters_grad(dy.data, x.data, a.data, b.data, (int)x.dtype, d.T, d.L, d.N, d.K, d.r, detail::i32(groups.order), detail::i32(groups.starts),
+                                        detail::i32(groups.tiles), detail::f32(scales), detail::inner("add_adapters_grad", h, d),
+                                        dx.data || da.data ? detail::inner("add_adapters_grad", g, d) : nullptr, dx.data, da.data, db.data, stream));
 }
 
 }  // namespace b200q

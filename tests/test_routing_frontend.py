@@ -1,5 +1,8 @@
 """Refusals of the routing, of the rows' exchange and of the adapters: errors before any device work, on the host alone."""
 import ctypes
+import os
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -115,3 +118,13 @@ def test_the_c_abi_refuses_before_any_cuda_call():
         dy, x, a, b, dtype, 4, 2, 8, 16, 4, d, d, d, None, h, g, dx, da, db, None)
     assert g(dy=None) == g(x=None) == g(a=None) == g(b=None) == g(h=None) == g(g=None) == g(dtype=_lib.F32) == g(dx=odd) == bad
     assert g(dx=None, da=None, db=None, g=None) == 0
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_the_cpp_shim_compiles_and_refuses(tmp_path):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe, libdir = str(tmp_path / "check"), os.path.dirname(_lib.LIB_PATH)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", os.path.join(root, "include"), os.path.join(root, "tests", "routing_shim_check.cpp"), "-o", exe,
+                    "-L", libdir, "-lb200q", f"-Wl,-rpath,{libdir}"], check=True, capture_output=True, text=True)
+    res = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert res.returncode == 0 and "SHIM-OK" in res.stdout, res.stdout + res.stderr
