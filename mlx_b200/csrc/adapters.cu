@@ -736,7 +736,7 @@ int tiles_per_block(const Params& p, int64_t cols, int64_t slots) {
 
 template <typename K>
 int launch(K kern, const Params& p, dim3 grid, int threads, size_t smem, cudaStream_t st, bool beside = false) {
-  if (smem > 40 * 1024) B200Q_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (int rc = allow_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);

@@ -35,6 +35,19 @@ int fail(int code, const char* fmt, ...) {
 
 void count_launch(int n) { g_launches += (uint64_t)n; }
 
+int allow_smem(const void* kernel, size_t bytes) {
+  struct Known { const void* kernel; int device; size_t bytes; };
+  static thread_local Known known[64] = {};
+  if (bytes <= 40 * 1024) return B200Q_OK;   // (48 KB with what kernels have besides)
+  int device = 0;
+  B200Q_CUDA_OK(cudaGetDevice(&device));
+  Known& k = known[(reinterpret_cast<uintptr_t>(kernel) / 16 * 31 + device) % 64];
+  if (k.kernel == kernel && k.device == device && k.bytes >= bytes) return B200Q_OK;
+  B200Q_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  k = Known{kernel, device, bytes};
+  return B200Q_OK;
+}
+
 // cuTensorMapEncodeTiled is a driver call and needs a current context, which a thread that has not yet
 // made a runtime call that touches the device (an autograd worker) does not have.  cudaSetDevice makes one current; unlike
 // cudaFree(nullptr), the customary way, it may also be called while the thread's stream is being captured.

@@ -615,6 +615,14 @@ using torch::autograd::variable_list;
 
 void* stream_of(at::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 Tensor fresh(at::IntArrayRef size, at::ScalarType t, at::Device dev) { return at::detail::empty_cuda(size, t, dev, std::nullopt); }
+// A tensor of int32 at `offset` of a one-dimensional one: of what a call makes, the tables share one allocation.
+Tensor part(const Tensor& of, int64_t offset, at::IntArrayRef size) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(of.storage()), of.key_set(), of.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+  return t;
+}
+int64_t up4(int64_t n) { return (n + 3) / 4 * 4; }
 bool plain(const Tensor& t, at::ScalarType type, at::Device dev) { return t.scalar_type() == type && t.device() == dev && t.is_contiguous(); }
 int64_t lead_of(const Tensor& t) { return product(t.sizes().slice(0, t.dim() - 1)); }
 bool tangent(const Tensor& t) { return t._fw_grad(0).defined(); }   // forward mode: the Python form says that there is none
@@ -632,12 +640,18 @@ bool members(PyObject* o, const Tensor* (&t)[N]) {
   for (int i = 0; i < N; ++i) t[i] = tensor(PyTuple_GET_ITEM(o, i));
   return true;
 }
-PyObject* pack(variable_list&& ts) {
-  PyObject* out = PyTuple_New((Py_ssize_t)ts.size());
+// As a NamedTuple of ops.py.
+PyObject* pack(variable_list&& ts, const char* name, PyTypeObject** type) {
+  if (!*type) {
+    pybind11::object t = pybind11::module_::import("mlx_b200.ops").attr(name);
+    *type = reinterpret_cast<PyTypeObject*>(t.release().ptr());
+  }
+  PyObject* out = (*type)->tp_alloc(*type, (Py_ssize_t)ts.size());
   if (!out) return nullptr;
   for (size_t i = 0; i < ts.size(); ++i) PyTuple_SET_ITEM(out, (Py_ssize_t)i, THPVariable_Wrap(std::move(ts[i])));
   return out;
 }
+PyTypeObject *g_routing = nullptr, *g_row_groups = nullptr;   // (guarded by the GIL)
 pybind11::object wrapped(const Tensor& t) { return pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(t)); }
 pybind11::object python(const char* module, const char* name) { return pybind11::module_::import(module).attr(name); }
 Tensor unwrapped(const pybind11::handle& o) { return o.is_none() ? Tensor() : Tensor(THPVariable_Unpack(o.ptr())); }
@@ -675,8 +689,9 @@ bool route_run(const Tensor& l, const Route& r, variable_list* out) {
   if (r.top < 1 || r.top > E || (r.bias && (!plain(*r.bias, at::kFloat, dev) || r.bias->dim() != 1 || r.bias->size(0) != E))) return false;
   c10::SmallVector<int64_t, 6> size(l.sizes().begin(), l.sizes().end());
   size.back() = r.top;
-  Tensor w = fresh(size, at::kFloat, dev), e = fresh(size, at::kInt, dev), s = fresh({E}, at::kInt, dev), p = fresh(size, at::kInt, dev),
-         o = fresh({T * r.top}, at::kInt, dev), ws;
+  const int64_t P = T * r.top, P4 = up4(P);
+  const Tensor all = fresh({3 * P4 + E}, at::kInt, dev);
+  Tensor w = fresh(size, at::kFloat, dev), e = part(all, 0, size), p = part(all, P4, size), o = part(all, 2 * P4, {P}), s = part(all, 3 * P4, {E}), ws;
   const size_t need = b200q_route_workspace_bytes(T, E, r.top);
   if (need) ws = fresh({(int64_t)need}, at::kByte, dev);
   auto at = [](const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
@@ -693,7 +708,7 @@ PyObject* py_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Route r;
   variable_list out;
   if (!route_args(a, n, &l, &r) || !route_run(*l, r, &out)) return none();
-  return pack(std::move(out));
+  return pack(std::move(out), "Routing", &g_routing);
   END_HANDLE_TH_ERRORS
 }
 struct RouteFn : public torch::autograd::Function<RouteFn> {
@@ -741,7 +756,7 @@ PyObject* py_route_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   variable_list out;
   if (!route_args(a, n, &l, &r) || tangent(*l) || (r.bias && tangent(*r.bias)) || !route_run(*l, r, &out)) return none();
   if (l->requires_grad() && at::GradMode::is_enabled()) out = RouteFn::apply(*l, &r, &out);
-  return pack(std::move(out));
+  return pack(std::move(out), "Routing", &g_routing);
   END_HANDLE_TH_ERRORS
 }
 
@@ -885,12 +900,14 @@ PyObject* py_group_rows(PyObject*, PyObject* const* a, Py_ssize_t nargs) {   // 
   if ((t != at::kInt && t != at::kLong) || !current(dev) || !ids->is_contiguous() || ids->numel() == 0) return none();
   const int64_t T = ids->numel();
   const size_t need = b200q_group_rows_workspace_bytes(T, n);
-  Tensor sizes = fresh({n}, at::kInt, dev), starts = fresh({n + 1}, at::kInt, dev), order = fresh({T}, at::kInt, dev),
-         tiles = fresh({b200q_group_rows_tiles(T, n), 4}, at::kInt, dev), ws = fresh({(int64_t)need}, at::kByte, dev);
+  const int64_t t4 = b200q_group_rows_tiles(T, n);
+  const Tensor all = fresh({4 * t4 + up4(T) + up4(n) + n + 1}, at::kInt, dev);   // (tiles first: on 16 bytes)
+  Tensor tiles = part(all, 0, {t4, 4}), order = part(all, 4 * t4, {T}), sizes = part(all, 4 * t4 + up4(T), {n}), starts = part(all, 4 * t4 + up4(T) + up4(n), {n + 1}), ws;
+  if (need) ws = fresh({(int64_t)need}, at::kByte, dev);
   auto at = [](const Tensor& v) { return static_cast<int32_t*>(v.data_ptr()); };
-  if (b200q_group_rows(ids->data_ptr(), t == at::kLong ? 8 : 4, T, n, at(sizes), at(starts), at(order), at(tiles), ws.data_ptr(), need, stream_of(dev)) != B200Q_OK)
+  if (b200q_group_rows(ids->data_ptr(), t == at::kLong ? 8 : 4, T, n, at(sizes), at(starts), at(order), at(tiles), need ? ws.data_ptr() : nullptr, need, stream_of(dev)) != B200Q_OK)
     return none();
-  return pack({sizes, starts, order, tiles});
+  return pack({sizes, starts, order, tiles}, "RowGroups", &g_row_groups);
   END_HANDLE_TH_ERRORS
 }
 

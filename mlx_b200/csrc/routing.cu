@@ -712,17 +712,11 @@ __global__ void __launch_bounds__(1024) place_kernel(const SortParams p) {
   sort_finish(p, blockIdx.x, base, total, warp_sums);
 }
 
-template <typename K>
-int allow_smem(K kern, size_t bytes) {
-  if (bytes > 48 * 1024) B200Q_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  return B200Q_OK;
-}
-
 // Launched while the first kernel runs, whose last blocks it waits for.
 int place(const SortParams& s, cudaStream_t st) {
   const int quads = pitch(s.n + 1) / 4;
   const size_t smem = (size_t)quads * 16 * (3 + 2 * std::max(1, 1024 / quads));
-  if (int rc = allow_smem(place_kernel, smem)) return rc;
+  if (int rc = allow_smem(reinterpret_cast<const void*>(place_kernel), smem)) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(s.blocks);
   cfg.blockDim = dim3(1024);
@@ -801,7 +795,7 @@ int launch_route(const RouteParams& p, int blocks, int warps, cudaStream_t st) {
   const bool rows = p.bias != nullptr || p.groups > 1;
   const size_t smem = (rows ? (size_t)warps * (p.E + p.E % 2) * 8 : 0) + warps * 384 + (size_t)(warps + 2) * (p.E + 1) * 4;
   auto go = [&](auto kern) {
-    if (int rc = allow_smem(kern, smem)) return rc;
+    if (int rc = allow_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
     kern<<<blocks, warps * 32, smem, st>>>(p);
     B200Q_LAUNCH_OK("route_kernel");
     return (int)B200Q_OK;
@@ -921,9 +915,13 @@ extern "C" int64_t b200q_group_rows_tiles(int64_t T, int64_t n) {
   if (T <= 0 || n < 0) return 0;
   return std::min(T, n + 1) + T / kAdapterRows;
 }
+namespace {
+bool few_rows(int64_t T, const Split& s) { return s.blocks == 1 && T <= 128 * s.warps; }
+}  // namespace
 extern "C" size_t b200q_group_rows_workspace_bytes(int64_t T, int64_t n) {
   if (T <= 0 || n < 0) return 0;
   const Split s = group_split(T, n);
+  if (few_rows(T, s)) return 0;
   return (size_t)pitch(T) * 4 + (s.blocks == 1 ? 0 : (size_t)s.blocks * pitch(n + 1) * 4);
 }
 
@@ -945,20 +943,20 @@ extern "C" int b200q_group_rows(const void* ids, int id_bytes, int64_t T, int64_
   if (!ids || !order || !tiles) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
   if (reinterpret_cast<uintptr_t>(tiles) % 16 != 0) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] tiles must be 16-byte aligned", tag);
   const size_t need = b200q_group_rows_workspace_bytes(T, n);
-  if (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16 != 0)
+  if (need > 0 && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16 != 0))
     return fail(B200Q_ERR_WORKSPACE, "[%s] an aligned workspace of %zu bytes required, %zu given", tag, need, ws ? ws_bytes : (size_t)0);
   const Split s = group_split(T, n);
   uint32_t* rank = static_cast<uint32_t*>(ws);
-  const SortParams p{ids, id_bytes, rank, rank + pitch(T), sizes, starts, nullptr, order, reinterpret_cast<int4*>(tiles), b200q_group_rows_tiles(T, n), T, s.per_block, (int)n, s.blocks};
+  const SortParams p{ids, id_bytes, rank, need ? rank + pitch(T) : nullptr, sizes, starts, nullptr, order, reinterpret_cast<int4*>(tiles), b200q_group_rows_tiles(T, n), T, s.per_block, (int)n, s.blocks};
   const size_t smem = (size_t)(s.warps + 2) * (n + 1) * 4;
-  if (T <= 128 * s.warps && s.blocks == 1) {
-    if (int rc = allow_smem(group_few_kernel, smem)) return rc;
+  if (few_rows(T, s)) {
+    if (int rc = allow_smem(reinterpret_cast<const void*>(group_few_kernel), smem)) return rc;
     group_few_kernel<<<1, s.warps * 32, smem, st>>>(p);
     B200Q_LAUNCH_OK("group_few_kernel");
     return B200Q_OK;
   }
   const ScratchLock lock(ws);
-  if (int rc = allow_smem(group_kernel, smem)) return rc;
+  if (int rc = allow_smem(reinterpret_cast<const void*>(group_kernel), smem)) return rc;
   group_kernel<<<s.blocks, s.warps * 32, smem, st>>>(p, s.per_warp);
   B200Q_LAUNCH_OK("group_kernel");
   return s.blocks == 1 ? B200Q_OK : place(p, st);

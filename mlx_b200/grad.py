@@ -220,7 +220,7 @@ def route_experts(logits: torch.Tensor, top: int, scoring: str = "softmax", bias
     """ops.route_experts whose weights have a gradient with respect to the logits (of first order).  The bias gets none."""
     r = ops._front.route_grad(logits, top, scoring, bias, groups, top_groups, group_best, renormalize, scale)
     if r is not None:
-        return ops.Routing(*r)
+        return r
     return ops.Routing(*_RouteFn.apply(logits, top, scoring, None if bias is None else bias.detach(), groups, top_groups, group_best, renormalize, scale))
 
 

@@ -878,7 +878,7 @@ def route_experts(logits: torch.Tensor, top: int, scoring: str = "softmax", bias
     -1, weight 0, place -1), a token of padding none at all.  grad.route_experts is the same with the weights' gradient."""
     r = _front.route(logits, top, scoring, bias, groups, top_groups, group_best, renormalize, scale)
     if r is not None:
-        return Routing(*r)
+        return r
     tag = "route_experts"
     E, top, groups, top_groups = _route_args(tag, logits, top, scoring, groups, top_groups, group_best)
     if bias is not None and (not bias.dtype.is_floating_point or tuple(bias.shape) != (E,)):
@@ -998,7 +998,7 @@ def group_rows(ids: torch.Tensor, n: int) -> RowGroups:
     and used beside all its projections."""
     g = _front.group_rows(ids, n)
     if g is not None:
-        return RowGroups(*g)
+        return g
     tag = "group_rows"
     if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
         raise ValueError(f"[{tag}] ids must be integral but are {ids.dtype}.")
@@ -1013,7 +1013,7 @@ def group_rows(ids: torch.Tensor, n: int) -> RowGroups:
         new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=dev)
         sizes, starts, order, tiles = new(n), new(n + 1), new(T), new(lib.b200q_group_rows_tiles(T, n), 4)
         need = lib.b200q_group_rows_workspace_bytes(T, n)
-        ws = _scratch(need, dev)
+        ws = _scratch(need, dev) if need else None
         rc = lib.b200q_group_rows(_ptr(ids), ids.element_size(), T, n, _ptr(sizes), _ptr(starts), _ptr(order), _ptr(tiles), _ptr(ws), need, _stream(ids))
     _lib.check(rc)
     return RowGroups(sizes, starts, order, tiles)

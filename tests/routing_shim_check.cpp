@@ -52,7 +52,10 @@ int main() {
   auto a = view(bf, {3, 4, 16}), b = view(bf, {3, 32, 4}), base = view(bf, {6, 32});
   bad += refused("ids' type", "int32 or int64", [&] { group_rows(view(f32, {6}), 3, g, some); });
   bad += refused("number of ids", "does not have", [&] { group_rows(view(i32, {7}), 3, g, some); });
-  bad += refused("no workspace for groups", "workspace", [&] { group_rows(view(i32, {6}), 3, g, none); });
+  bad += refused("no workspace for groups", "workspace", [&] {
+    RowGroups q{view(i32, {3}), view(i32, {4}), view(i32, {5000}), view(i32, {b200q_group_rows_tiles(5000, 3), 4})};
+    group_rows(view(i32, {5000}), 3, q, none);
+  });
   bad += refused("width of x", "do not match", [&] { add_adapters(base, view(bf, {6, 15}), a, b, g, some, base); });
   bad += refused("types", "one type", [&] { add_adapters(base, view(Dtype::float16, {6, 16}), a, b, g, some, base); });
   bad += refused("float32", "unsupported dtype", [&] {

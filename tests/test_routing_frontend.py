@@ -108,7 +108,7 @@ def test_the_c_abi_refuses_before_any_cuda_call():
     assert both(dy=None) == both(y=None) == both(w=None) == both(dys=odd) == bad and both(dys=None, dw=None) == 0
     group = lambda ids=d, nb=8, T=4, n=3, ws=d, have=1 << 30, tiles=d: lib.b200q_group_rows(ids, nb, T, n, d, d, d, tiles, ws, have, None)
     assert group(ids=None) == group(nb=2) == group(ids=odd) == group(T=-1) == group(n=-1) == group(tiles=None) == group(tiles=ctypes.c_void_p(4104)) == bad
-    assert group(n=4097) == group(T=(1 << 31) - 1) == uns and group(ws=None) == group(have=4) == ws_err
+    assert group(n=4097) == group(T=(1 << 31) - 1) == uns and group(ws=None, T=5000) == group(have=4, T=5000) == ws_err
     add = lambda y=d, x=d, dtype=_lib.BF16, T=4, L=2, N=8, K=16, r=4, h=d, tiles=d, out=d: lib.b200q_add_adapters(
         y, x, d, d, dtype, T, L, N, K, r, d, tiles, None, h, out, None)
     assert add(y=None) == add(x=None) == add(h=None) == add(x=odd) == add(dtype=_lib.F32) == add(T=-1) == add(r=-1) == add(tiles=ctypes.c_void_p(4104)) == bad
