@@ -471,7 +471,8 @@ int b200q_group_rows(const void* ids, int id_bytes, int64_t T, int64_t n, int32_
 
 /*
  * Low-rank adapters beside a shared projection: out[t] = y[t] + scales[l] b[l] (a[l] x[t]), l being row t's adapter; a row without one:
- * y[t].  bf16 and f16; sums in fp32, the inner product to 2^-17, the result rounded once.
+ * y[t].  bf16 and f16; sums in fp32, the inner product to 2^-17, the result rounded once.  Inner products and f16 weights are multiplied as two
+ * parts each: where one of them is infinite, so that the sum would be, it may be a NaN.
  *   y, out [T, N] (out may be y), x [T, K], a [L, r, K], b [L, N, r] dtype; scales [L] float32 (NULL: 1)
  *   order, starts, tiles: b200q_group_rows over L groups
  *   h: b200q_add_adapters_inner_bytes(T, r) bytes on a 16-byte boundary, left with a[l] x, by place, as two bf16 numbers per value,

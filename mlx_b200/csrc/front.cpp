@@ -956,8 +956,10 @@ PyObject* py_add_adapters(PyObject*, PyObject* const* a, Py_ssize_t n) {   // (.
   if (n != 7 || !adapters_args(a, &p) || (a[6] != Py_None && a[6] != a[0])) return none();
   if (a[6] != Py_None) {
     out = *p.y;
+    if (out.requires_grad() && at::GradMode::is_enabled()) return none();
     for (const Tensor* v : {p.x, p.a, p.b})
       if (overlap(out, *v)) return none();
+    out.unsafeGetTensorImpl()->bump_version();   // whoever has kept it for a gradient hears of it
   }
   if (!adapters_run(&p, &out, &h)) return none();
   PyObject* pair = PyTuple_New(2);

@@ -1067,8 +1067,11 @@ def _add_adapters(y, x, a, b, groups, scales=None, out=None):
     if out is not None:
         if out.dtype != y.dtype or out.shape != y.shape or out.device != y.device or not out.is_contiguous():
             raise ValueError(f"[{tag}] out must be a contiguous tensor like y.")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"[{tag}] out must not be part of a graph.")
         if any(_overlap(out, t) for t in (x, a, b)) or (_overlap(out, y) and (out.data_ptr() != y.data_ptr() or not y.is_contiguous())):
             raise ValueError(f"[{tag}] out must be y itself or not overlap the operands.")
+        torch.autograd.graph.increment_version(out)   # whoever has kept it for a gradient hears of it
     y, x, a, b = (t.detach().contiguous() for t in (y, x, a, b))
     with torch.cuda.device(dev):
         out = torch.empty_like(y) if out is None else out

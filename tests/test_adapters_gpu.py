@@ -322,3 +322,31 @@ def test_beside_a_quantized_projection():
     groups = mb.group_rows(ids, 3)
     out = mb.add_adapters(y.clone(), x, a, b, groups, s)
     near(out, *exact(ids, y, x, a, b, s), 512 + 16)
+
+
+def test_sums_in_place_and_autograd():
+    """What is overwritten is noticed by a graph that has kept it; a sum in place of what is part of a graph is refused."""
+    ids = torch.tensor([1, 0, -1, 1], device="cuda")
+    y, x, a, b, s = problem(15, ids, 2, 8, 64, 72, torch.bfloat16)
+    groups = mb.group_rows(ids, 2)
+    ref = mb.add_adapters(y, x, a, b, groups, s)
+    for into in (lambda kept: kept, lambda kept: y):   # in place; another tensor's sum
+        for scales in (s, s.double()):
+            kept, w = y.clone(), torch.ones_like(y).requires_grad_()
+            z = kept * w
+            mb.add_adapters(into(kept), x, a, b, groups, scales, out=kept)
+            assert torch.equal(kept, ref)
+            with pytest.raises(RuntimeError):
+                z.sum().backward()
+    leaf = y.clone().requires_grad_()
+    for t in (leaf, leaf * 2):
+        with pytest.raises(ValueError):
+            mb.add_adapters(t, x, a, b, groups, s, out=t)
+        with pytest.raises(ValueError):
+            mb.add_adapters(y, x, a, b, groups, s, out=t)
+    assert torch.equal(leaf, y)
+    with torch.no_grad():
+        assert torch.equal(mb.add_adapters(leaf, x, a, b, groups, s, out=leaf), ref)
+    with torch.inference_mode():
+        t = y.clone()
+        assert torch.equal(mb.add_adapters(t, x, a, b, groups, s, out=t), ref)
