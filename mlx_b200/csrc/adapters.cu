@@ -395,7 +395,7 @@ struct Up {
   static constexpr size_t kBytes = (size_t)kWarps * kUpStages * 1024 + (CHUNKED ? 0 : 8 * kStep);
 };
 template <typename T, bool WIDE, bool WHOLE, int KS, bool CHUNKED>
-__global__ void __launch_bounds__(kThreads, (KS == 4 ? 2 : 3) - std::is_same_v<T, __half>) up_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - std::is_same_v<T, __half>) up_kernel(const Params p) {
   constexpr bool kSplitW = std::is_same_v<T, __half>;
   constexpr int kStep = Up<KS, CHUNKED>::kStep;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -521,43 +521,7 @@ __global__ void __launch_bounds__(kThreads, (KS == 4 ? 2 : 3) - std::is_same_v<T
     last = (tile.z + 15) / 16;
     // (rows behind the tile's last one have what was there before; their products are not stored)
     uint32_t src = hs + buffer * 4 * kStep + lane * 16;
-    for (int m = 0; m < last; ++m, ++now, src += kStep) {
-      issue();
-      float acc[4][4] = {};
-      auto step = [&](int s, const uint4& hi, const uint4& lo) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], hi.x, hi.y, hi.z, hi.w, bh[s][t][0], bh[s][t][1]);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], lo.x, lo.y, lo.z, lo.w, bh[s][t][0], bh[s][t][1]);
-        if constexpr (kSplitW) {
-#pragma unroll
-          for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], hi.x, hi.y, hi.z, hi.w, bl[s][t][0], bl[s][t][1]);
-        }
-      };
-      if (!plain) {
-        if constexpr (CHUNKED) {
-          for (int r0 = 0; r0 < p.r16; r0 += 16 * KS) {
-            weights(r0);
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-              if (r0 + s * 16 >= p.r16) break;
-              uint4 h[2];
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const int row = m * 16 + i * 8 + g;
-                h[i] = row < tile.z ? *reinterpret_cast<const uint4*>(p.h + (int64_t)(tile.y + row) * 2 * p.r16 + (r0 + s * 16) * 2 + q * 8) : make_uint4(0, 0, 0, 0);
-              }
-              step(s, make_uint4(h[0].x, h[1].x, h[0].y, h[1].y), make_uint4(h[0].z, h[1].z, h[0].w, h[1].w));
-            }
-          }
-        } else {
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            if (KS > 1 && s * 16 >= p.r16) break;
-            step(s, load16(src + s * 1024), load16(src + s * 1024 + 512));
-          }
-        }
-      }
+    auto finish = [&](const float (&acc)[4][4]) {   // the step's sums to its rows
       wait_all_but<kUpStages - 1>();
       const uint32_t from = ring + (now % kUpStages) * 1024;
 #pragma unroll
@@ -577,6 +541,57 @@ __global__ void __launch_bounds__(kThreads, (KS == 4 ? 2 : 3) - std::is_same_v<T
           for (int j = 0; j < 8; ++j)
             if (j < have) o[j] = e[j];
         }
+      }
+      ++now;
+    };
+    auto step = [&](float (&acc)[4][4], int s, const uint4& hi, const uint4& lo) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], hi.x, hi.y, hi.z, hi.w, bh[s][t][0], bh[s][t][1]);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], lo.x, lo.y, lo.z, lo.w, bh[s][t][0], bh[s][t][1]);
+      if constexpr (kSplitW) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], hi.x, hi.y, hi.z, hi.w, bl[s][t][0], bl[s][t][1]);
+      }
+    };
+    if constexpr (CHUNKED) {
+      float acc[kRows / 16][4][4] = {};
+      for (int r0 = 0; r0 < p.r16 && !plain; r0 += 16 * KS) {
+        weights(r0);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          if (r0 + s * 16 >= p.r16) break;
+#pragma unroll
+          for (int m = 0; m < kRows / 16; ++m)
+            if (m < last) {
+              uint4 h[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int row = m * 16 + i * 8 + g;
+                h[i] = row < tile.z ? *reinterpret_cast<const uint4*>(p.h + (int64_t)(tile.y + row) * 2 * p.r16 + (r0 + s * 16) * 2 + q * 8) : make_uint4(0, 0, 0, 0);
+              }
+              step(acc[m], s, make_uint4(h[0].x, h[1].x, h[0].y, h[1].y), make_uint4(h[0].z, h[1].z, h[0].w, h[1].w));
+            }
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < kRows / 16; ++m)
+        if (m < last) {
+          issue();
+          finish(acc[m]);
+        }
+    } else {
+      for (int m = 0; m < last; ++m, src += kStep) {
+        issue();
+        float acc[4][4] = {};
+        if (!plain) {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            if (KS > 1 && s * 16 >= p.r16) break;
+            step(acc, s, load16(src + s * 1024), load16(src + s * 1024 + 512));
+          }
+        }
+        finish(acc);
       }
     }
     buffer ^= 1;
@@ -772,12 +787,12 @@ template <typename T, bool WIDE, bool WHOLE>
 int up(Params p, cudaStream_t st) {
   p.split = 1;
   const int64_t cols = (p.C + 255) / 256;
-  p.each = tiles_per_block(p, cols, 148 * ((p.r > 32 ? 2 : 3) - std::is_same_v<T, __half>));
+  p.each = tiles_per_block(p, cols, 148 * (p.r > 64 ? 2 : (p.r > 32 ? 2 : 3) - std::is_same_v<T, __half>));
   const dim3 grid((unsigned)((p.tiles_n + p.each - 1) / p.each * cols));
   if (p.r <= 16) return launch(up_kernel<T, WIDE, WHOLE, 1, false>, p, grid, kThreads, Up<1, false>::kBytes, st, true);
   if (p.r <= 32) return launch(up_kernel<T, WIDE, WHOLE, 2, false>, p, grid, kThreads, Up<2, false>::kBytes, st, true);
   if (p.r <= 64) return launch(up_kernel<T, WIDE, WHOLE, 4, false>, p, grid, kThreads, Up<4, false>::kBytes, st, true);
-  return launch(up_kernel<T, WIDE, WHOLE, 4, true>, p, grid, kThreads, Up<4, true>::kBytes, st, true);
+  return launch(up_kernel<T, WIDE, WHOLE, 2, true>, p, grid, kThreads, Up<2, true>::kBytes, st, true);
 }
 template <typename T, bool TALL, bool WHOLE>
 int outer(Params p, cudaStream_t st) {
