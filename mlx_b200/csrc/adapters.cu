@@ -600,121 +600,154 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
   wait_all_but<0>();
 }
 
-// ---- out_l = (c) sum over l's rows of h[place] x[row]^T.  Blocks by (64 columns, part of the rows; adapter; 16 MT ranks), the parts are a
-// cluster; warps by (32 columns, quarter of the rows).  TALL: out [C, r], else [r, C].
+// ---- out_l = (c) sum over l's rows of h[place] x[row]^T.  Blocks by (128 columns, part of the rows; adapter; 16 MT ranks), the parts are a
+// cluster; warps by (32 columns, half of a step's 32 rows).  TALL: out [C, r], else [r, C].
+//
+// Rows lie in shared memory as they come, and matrix loads that transpose make both operands of them; h's two parts lie apart there.
+template <bool TALL, int MT>
+struct Outer {
+  static constexpr int kRanks = 16 * MT, kCols = 128, kSteps = 32, kStages = 3;
+  static constexpr int kXPitch = kCols * 2 + 16, kHPitch = kRanks * 2 + 16;   // (eight rows of a matrix are in different banks)
+  static constexpr int kStage = kSteps * (kXPitch + 2 * kHPitch);
+  static constexpr int kLine = kCols + (TALL ? 2 : 8);   // floats per rank of the sums
+  static constexpr size_t kRing = (size_t)kStages * kStage, kSums = (size_t)2 * kRanks * kLine * 4, kBytes = kRing > kSums ? kRing : kSums;
+};
 template <typename T, bool TALL, bool WHOLE, int MT>
-__global__ void __launch_bounds__(kThreads) outer_kernel(const Params p) {
-  constexpr int kRanks = 16 * MT, kCols = 64, kLine = kCols + 8;
-  extern __shared__ __align__(16) float red[];   // [4][kRanks][kLine]
+__global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) outer_kernel(const Params p) {
+  using O = Outer<TALL, MT>;
+  constexpr int kRanks = O::kRanks, kCols = O::kCols, kLine = O::kLine, kStages = O::kStages, kXPitch = O::kXPitch, kHPitch = O::kHPitch;
+  constexpr bool kSplitX = std::is_same_v<T, __half>;
+  extern __shared__ __align__(16) unsigned char smem[];
   cg::cluster_group cluster = cg::this_cluster();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3, slot = warp >> 1, C = (int)p.C;
-  const int part = (int)(blockIdx.x % p.split), l = blockIdx.y, r0 = blockIdx.z * kRanks;
-  const int c0 = (int)(blockIdx.x / p.split) * kCols, col = c0 + (warp & 1) * 32 + q * 8, have = C - col;
-  const int lo = max(p.starts[l], 0), hi = min(p.starts[l + 1], (int)p.T);
-  const T* x = static_cast<const T*>(p.x) + col;
-  const int step = p.split * 64;
-  int t = lo + (part * 4 + slot) * 16;   // of the step that is multiplied
-  int place = t + g;                     // the lane's, of the step that is loaded
-  const uint16_t* h = p.h + (int64_t)place * 2 * p.r16 + r0 * 2 + q * 8;
-  float acc[MT][4][4] = {};
-  struct Stage {
-    uint4 x[2];
-    uint4 h[MT][2];   // rank step, place (+ 8): a lane's 4 ranks' high and low parts
-  };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3, slot = warp >> 2, C = (int)p.C;
+  const int part = (int)(blockIdx.x % p.split), l = blockIdx.y, r0 = blockIdx.z * kRanks, c0 = (int)(blockIdx.x / p.split) * kCols;
+  const int lo = max(p.starts[l], 0), hi = min(p.starts[l + 1], (int)p.T), step = p.split * O::kSteps, first = lo + part * O::kSteps;
+  const int n = first < hi ? (hi - first + step - 1) / step : 0;
+  // Copied per step by a thread: 8 columns of two rows of x; of h, pieces of 4 ranks' two parts.
+  constexpr int kPer = 4 * MT, kHRows = kThreads / kPer, kH = O::kSteps > kHRows ? O::kSteps / kHRows : 1;   // pieces per row; rows at once; rows of a thread
+  const int xr = threadIdx.x / 16, xc = threadIdx.x % 16, hr = threadIdx.x / kPer, hc = threadIdx.x % kPer, have = C - c0 - xc * 8;
+  const T* x = static_cast<const T*>(p.x) + c0 + xc * 8;
+  const bool ranks = hr < O::kSteps && r0 + hc * 4 < p.r16;
+  int place = first;   // of the step that is loaded
   int row[2];
-  auto look = [&](int at) {   // at: the lane's place
+  auto look = [&] {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      row[i] = at + i * 8 < hi ? p.order[at + i * 8] : -1;
+      const int at = place + xr + i * 16;
+      row[i] = at < hi ? p.order[at] : -1;
       if (row[i] >= (int)p.T) row[i] = -1;
     }
   };
-  auto load = [&](Stage& s) {   // the next step, whose rows have been looked up
+  const uint32_t ring = shared(smem);
+  auto load = [&](int stage) {   // the next step, whose rows have been looked up
+    const uint32_t to = ring + stage * O::kStage;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      s.x[i] = row[i] >= 0 ? load8<WHOLE>(x + (int64_t)row[i] * C, have) : make_uint4(0, 0, 0, 0);
+      const uint32_t d = to + (xr + i * 16) * kXPitch + xc * 16;
+      const T* src = x + (int64_t)row[i] * C;
+      if constexpr (WHOLE) copy_async<16>(d, src, row[i] >= 0 && have > 0);
+      else store16(d, row[i] >= 0 ? load8<false>(src, have) : make_uint4(0, 0, 0, 0));
+    }
+    if (hr < O::kSteps) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-        s.h[m][i] = place + i * 8 < hi && (MT == 1 || r0 + m * 16 < p.r16) ? *reinterpret_cast<const uint4*>(h + i * 16 * p.r16 + m * 32) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < kH; ++i) {
+        const int at = hr + i * kHRows;
+        const uint32_t d = to + O::kSteps * kXPitch + at * kHPitch + hc * 8;
+        const uint16_t* src = p.h + (int64_t)(place + at) * 2 * p.r16 + r0 * 2 + hc * 8;
+        const bool there = ranks && place + at < hi;
+        copy_async<8>(d, src, there);
+        copy_async<8>(d + O::kSteps * kHPitch, src + 4, there);
+      }
     }
     place += step;
-    h += (int64_t)step * 2 * p.r16;
-    look(place);
+    look();
   };
-  auto multiply = [&](const Stage& s) {
+  float acc[MT][4][4] = {};
+  look();
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    if (s < n) load(s);
+    commit();
+  }
+  const int mr = lane & 7, mi = lane >> 3;
+  const uint32_t x_at = (slot * 16 + (mi & 1) * 8 + mr) * kXPitch + ((warp & 3) * 4 + (mi >> 1)) * 16;
+  const uint32_t h_at = O::kSteps * kXPitch + (slot * 16 + (mi >> 1) * 8 + mr) * kHPitch + (mi & 1) * 16;
+  int from = 0, to = kStages - 1;
+  for (int k = 0; k < n; ++k) {
+    wait_all_but<kStages - 2>();
+    __syncthreads();   // the step is there, and everyone has read the stage that is filled now
+    if (k + kStages - 1 < n) load(to);
+    commit();
+    const uint32_t src = ring + from * O::kStage;
     uint32_t bh[4][2], bl[4][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      as_bf16<T>(transposed(s.x[i].x), &bh[0][i], &bl[0][i]);
-      as_bf16<T>(transposed(s.x[i].y), &bh[1][i], &bl[1][i]);
-      as_bf16<T>(transposed(s.x[i].z), &bh[2][i], &bl[2][i]);
-      as_bf16<T>(transposed(s.x[i].w), &bh[3][i], &bl[3][i]);
+    for (int v = 0; v < 4; v += 2) {
+      const uint4 b = load_matrices<true>(src + x_at + v * 16);
+      as_bf16<T>(b.x, &bh[v][0], &bl[v][0]);
+      as_bf16<T>(b.y, &bh[v][1], &bl[v][1]);
+      as_bf16<T>(b.z, &bh[v + 1][0], &bl[v + 1][0]);
+      as_bf16<T>(b.w, &bh[v + 1][1], &bl[v + 1][1]);
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       if (MT > 1 && r0 + m * 16 >= p.r16) break;
-      uint32_t a[2][4];   // part; rows of the product: of a lane's 4 ranks the first two are in its upper half
+      const uint4 a = load_matrices<true>(src + h_at + m * 32), b = load_matrices<true>(src + h_at + m * 32 + O::kSteps * kHPitch);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        a[0][2 * i] = transposed(s.h[m][i].x);
-        a[0][2 * i + 1] = transposed(s.h[m][i].y);
-        a[1][2 * i] = transposed(s.h[m][i].z);
-        a[1][2 * i + 1] = transposed(s.h[m][i].w);
-      }
+      for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a.x, a.y, a.z, a.w, bh[v][0], bh[v][1]);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a[0][0], a[0][1], a[0][2], a[0][3], bh[v][0], bh[v][1]);
+      for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], b.x, b.y, b.z, b.w, bh[v][0], bh[v][1]);
+      if constexpr (kSplitX) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a[1][0], a[1][1], a[1][2], a[1][3], bh[v][0], bh[v][1]);
-      if constexpr (std::is_same_v<T, __half>) {
-#pragma unroll
-        for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a[0][0], a[0][1], a[0][2], a[0][3], bl[v][0], bl[v][1]);
+        for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a.x, a.y, a.z, a.w, bl[v][0], bl[v][1]);
       }
     }
-  };
-  Stage a, b;
-  look(place);
-  if (t < hi) load(a);
-  while (t < hi) {
-    if (t + step < hi) load(b);
-    multiply(a);
-    t += step;
-    if (t >= hi) break;
-    if (t + step < hi) load(a);
-    multiply(b);
-    t += step;
+    to = from;
+    from = from + 1 == kStages ? 0 : from + 1;
   }
-  // rows and columns as the products have them: 16 m + 8 i + g is rank 16 m + 4 (g / 2) + 2 i + g % 2, 32 half + 8 v + 2 q is column 32 half + 8 q + 2 v
+  wait_all_but<0>();
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(smem);   // [2][kRanks][kLine]
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int v = 0; v < 4; ++v)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<float2*>(&red[(slot * kRanks + m * 16 + i * 8 + g) * kLine + (warp & 1) * 32 + v * 8 + q * 2]) = make_float2(acc[m][v][2 * i], acc[m][v][2 * i + 1]);
+        *reinterpret_cast<float2*>(&red[(slot * kRanks + m * 16 + i * 8 + g) * kLine + (warp & 3) * 32 + v * 8 + q * 2]) = make_float2(acc[m][v][2 * i], acc[m][v][2 * i + 1]);
   __syncthreads();
-  for (int i = threadIdx.x; i < kRanks * kCols; i += kThreads) {
-    const int at = i / kCols * kLine + i % kCols;
-    float s = red[at];
-#pragma unroll
-    for (int v = 1; v < 4; ++v) s += red[v * kRanks * kLine + at];
-    red[at] = s;
+  if (p.split > 1) {
+    for (int i = threadIdx.x; i < kRanks * kCols; i += kThreads) {
+      const int at = i / kCols * kLine + i % kCols;
+      red[at] += red[kRanks * kLine + at];
+    }
+    cluster.sync();
   }
-  if (p.split > 1) cluster.sync();
-  else __syncthreads();
   const float c = p.scales ? p.scales[l] : 1.0f;
   T* out = static_cast<T*>(p.out) + (int64_t)l * p.r * C;
-  const int each = kRanks * kCols / p.split;   // of the tile's elements: this block's
+  const int each = kRanks * kCols / p.split, wide = kCols / p.split;   // of the tile's elements: this block's; TALL: its columns
+  if (TALL && p.split > 1) {   // the others' sums along their rows, then the block's own along its columns
+    for (int i = threadIdx.x; i < each; i += kThreads) {
+      const int at = i / wide * kLine + part * wide + i % wide;
+      float s = 0.0f;
+      for (int v = 0; v < p.split; ++v) s += cluster.map_shared_rank(red, v)[at];
+      red[kRanks * kLine + at] = s;
+    }
+    __syncthreads();
+  }
   for (int i = threadIdx.x; i < each; i += kThreads) {
-    const int e = part * each + i, rank = TALL ? e % kRanks : e / kCols, cc = TALL ? e / kRanks : e % kCols;
-    const int at = (rank / 16 * 16 + rank / 2 % 2 * 8 + rank / 4 % 4 * 2 + rank % 2) * kLine + cc / 32 * 32 + cc / 2 % 4 * 8 + cc / 8 % 4 * 2 + cc % 2;
-    float s = red[at];
-    if (p.split > 1) {
+    const int e = part * each + i, rank = TALL ? e % kRanks : e / kCols, cc = TALL ? e / kRanks : e % kCols, at = rank * kLine + cc;
+    float s;
+    if (p.split == 1) {
+      s = red[at] + red[kRanks * kLine + at];
+    } else if (TALL) {
+      s = red[kRanks * kLine + at];
+    } else {
       s = 0.0f;
       for (int v = 0; v < p.split; ++v) s += cluster.map_shared_rank(red, v)[at];
     }
     if (r0 + rank < p.r && c0 + cc < C) out[TALL ? (int64_t)(c0 + cc) * p.r + r0 + rank : (int64_t)(r0 + rank) * C + c0 + cc] = Elem<T>::from_float(c * s);
   }
-  if (p.split > 1) cluster.sync();
+  if (p.split > 1) cluster.sync();   // no block leaves while others read its sums
 }
 
 bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -797,13 +830,12 @@ int up(Params p, cudaStream_t st) {
 template <typename T, bool TALL, bool WHOLE>
 int outer(Params p, cudaStream_t st) {
   const int mt = p.r <= 16 ? 1 : (p.r <= 32 ? 2 : 4), chunks = (p.r + 16 * mt - 1) / (16 * mt);
-  const int64_t cols = (p.C + 63) / 64;
-  p.split = split_of(cols * p.L * chunks, 148 * 4, p.T / 64);
+  const int64_t cols = (p.C + 127) / 128;
+  p.split = split_of(cols * p.L * chunks, 148 * 2, p.T / 64);
   const dim3 grid((unsigned)(cols * p.split), p.L, chunks);
-  const size_t smem = (size_t)4 * 16 * mt * 72 * 4;
-  if (mt == 1) return launch(outer_kernel<T, TALL, WHOLE, 1>, p, grid, kThreads, smem, st);
-  if (mt == 2) return launch(outer_kernel<T, TALL, WHOLE, 2>, p, grid, kThreads, smem, st);
-  return launch(outer_kernel<T, TALL, WHOLE, 4>, p, grid, kThreads, smem, st);
+  if (mt == 1) return launch(outer_kernel<T, TALL, WHOLE, 1>, p, grid, kThreads, Outer<TALL, 1>::kBytes, st);
+  if (mt == 2) return launch(outer_kernel<T, TALL, WHOLE, 2>, p, grid, kThreads, Outer<TALL, 2>::kBytes, st);
+  return launch(outer_kernel<T, TALL, WHOLE, 4>, p, grid, kThreads, Outer<TALL, 4>::kBytes, st);
 }
 
 // Of a call: which form of a kernel.
