@@ -392,7 +392,7 @@ constexpr int kUpStages = 4, kUpTiles = 8, kUpSteps = kUpTiles * kRows / 16;
 template <int KS, bool CHUNKED>
 struct Up {
   static constexpr int kStep = KS * 1024;   // bytes of h per step of 16 rows: [rank step][part][lane][4]
-  static constexpr size_t kBytes = (size_t)kWarps * kUpStages * 1024 + (CHUNKED ? 0 : 8 * kStep);
+  static constexpr size_t kBytes = (size_t)kWarps * kUpStages * 1024 + 8 * kStep;
 };
 template <typename T, bool WIDE, bool WHOLE, int KS, bool CHUNKED>
 __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - std::is_same_v<T, __half>) up_kernel(const Params p) {
@@ -427,12 +427,12 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
     while (k < p.each && tiles[k].z == 0) ++k;
     return k;
   };
-  auto copy_h = [&](int k, int buffer) {
-    if (CHUNKED || k >= p.each || tiles[k].x < 0) return;
+  auto copy_h = [&](int k, int r0, int buffer) {
+    if (k >= p.each || tiles[k].x < 0) return;
     constexpr int kPer = 4 * KS, kSweep = kThreads / kPer;   // pieces of 16 bytes per row; rows that the block copies at once
     const int piece = threadIdx.x % kPer, row = threadIdx.x / kPer, z = tiles[k].z;
-    if (piece * 4 >= p.r16) return;
-    const uint16_t* src = p.h + (int64_t)(tiles[k].y + row) * 2 * p.r16 + piece * 8;
+    if (r0 + piece * 4 >= p.r16) return;
+    const uint16_t* src = p.h + (int64_t)(tiles[k].y + row) * 2 * p.r16 + r0 * 2 + piece * 8;
     const uint32_t to = hs + buffer * 4 * kStep + piece / 4 * 1024 + piece % 4 * 16;
 #pragma unroll
     for (int i = 0; i < kRows / kSweep; ++i) {
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
     weights(0);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");   // all of h, of the launch before
-  copy_h(k, 0);
+  copy_h(k, 0, 0);
   commit();
   for (int last = 4; k < p.each;) {
     const int4 tile = tiles[k];
@@ -513,14 +513,8 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
         loaded = tile.x;
       }
     }
-    // the group with this tile's h was issued with the first step of the tile before, four steps ago if that was a whole one
-    if (now == 0 || last < 4) wait_all_but<0>();
-    __syncthreads();
-    const int after = next_tile(k + 1);
-    copy_h(after, buffer ^ 1);
+    const int after = next_tile(k + 1), before = last;
     last = (tile.z + 15) / 16;
-    // (rows behind the tile's last one have what was there before; their products are not stored)
-    uint32_t src = hs + buffer * 4 * kStep + lane * 16;
     auto finish = [&](const float (&acc)[4][4]) {   // the step's sums to its rows
       wait_all_but<kUpStages - 1>();
       const uint32_t from = ring + (now % kUpStages) * 1024;
@@ -554,24 +548,26 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
         for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], hi.x, hi.y, hi.z, hi.w, bl[s][t][0], bl[s][t][1]);
       }
     };
+    // (rows behind the tile's last one have what was there before; their products are not stored)
     if constexpr (CHUNKED) {
       float acc[kRows / 16][4][4] = {};
-      for (int r0 = 0; r0 < p.r16 && !plain; r0 += 16 * KS) {
+      for (int r0 = 0; r0 == 0 || (r0 < p.r16 && !plain); r0 += 16 * KS, buffer ^= 1) {
+        // these ranks' h was issued before the last tile's four steps, or last
+        if (r0 == 0 && now != 0 && before == 4) wait_all_but<4>();
+        else wait_all_but<0>();
+        __syncthreads();
+        if (r0 + 16 * KS < p.r16 && !plain) copy_h(k, r0 + 16 * KS, buffer ^ 1);
+        else copy_h(after, 0, buffer ^ 1);
+        commit();
+        if (plain) continue;
         weights(r0);
+        const uint32_t src = hs + buffer * 4 * kStep + lane * 16;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           if (r0 + s * 16 >= p.r16) break;
 #pragma unroll
           for (int m = 0; m < kRows / 16; ++m)
-            if (m < last) {
-              uint4 h[2];
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const int row = m * 16 + i * 8 + g;
-                h[i] = row < tile.z ? *reinterpret_cast<const uint4*>(p.h + (int64_t)(tile.y + row) * 2 * p.r16 + (r0 + s * 16) * 2 + q * 8) : make_uint4(0, 0, 0, 0);
-              }
-              step(acc[m], s, make_uint4(h[0].x, h[1].x, h[0].y, h[1].y), make_uint4(h[0].z, h[1].z, h[0].w, h[1].w));
-            }
+            if (m < last) step(acc[m], s, load16(src + m * kStep + s * 1024), load16(src + m * kStep + s * 1024 + 512));
         }
       }
 #pragma unroll
@@ -581,6 +577,11 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
           finish(acc[m]);
         }
     } else {
+      // the group with this tile's h was issued with the first step of the tile before, four steps ago if that was a whole one
+      if (now == 0 || before < 4) wait_all_but<0>();
+      __syncthreads();
+      copy_h(after, 0, buffer ^ 1);
+      uint32_t src = hs + buffer * 4 * kStep + lane * 16;
       for (int m = 0; m < last; ++m, src += kStep) {
         issue();
         float acc[4][4] = {};
@@ -593,8 +594,8 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
         }
         finish(acc);
       }
+      buffer ^= 1;
     }
-    buffer ^= 1;
     k = after;
   }
   wait_all_but<0>();
