@@ -167,6 +167,20 @@ __device__ __forceinline__ uint4 load_matrices(uint32_t row) {
   else asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(row) : "memory");
   return v;
 }
+// Eight values of T, of which `have` are there; whole: on 16 bytes.
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int have, bool whole, const float (&v)[8]) {
+  alignas(16) T e[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) e[j] = Elem<T>::from_float(v[j]);
+  if (whole && have >= 8) {
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(e);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < have) p[j] = e[j];
+  }
+}
 // a + c * b for eight values of T
 template <typename T>
 __device__ __forceinline__ uint4 add8(const uint4& a, float c, const float (&b)[8]) {
@@ -196,7 +210,7 @@ struct Params {
   const int4* tiles;
   int64_t T, C;            // rows; the long dimension (K or N)
   int64_t tiles_n;
-  int L, r, r16, width;    // r16: r in whole 16s; width: bytes that the pieces of short rows of weights are aligned to
+  int L, r, r16, width;    // r16: r in whole 16s; width: bytes that the rows of weights [C, r] (or of their gradient) are aligned to
   int split, each;         // blocks per cluster; tiles per block
 };
 
@@ -725,28 +739,53 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) outer_kernel(const 
   }
   const float c = p.scales ? p.scales[l] : 1.0f;
   T* out = static_cast<T*>(p.out) + (int64_t)l * p.r * C;
-  const int each = kRanks * kCols / p.split, wide = kCols / p.split;   // of the tile's elements: this block's; TALL: its columns
-  if (TALL && p.split > 1) {   // the others' sums along their rows, then the block's own along its columns
+  float* sums = red + kRanks * kLine;   // with a cluster: what the block stores
+  const int wide = kCols / p.split;     // TALL: its columns
+  // A thread stores eight values at once: ranks of a column (lanes: 16 columns by twice 8 ranks, so that pairs fill a sector), or columns of a rank.
+  if constexpr (TALL) {
+    if (p.split > 1) {   // the others' sums along their rows, then the block's own along its columns
+      for (int i = threadIdx.x; i < kRanks * wide / 2; i += kThreads) {
+        const int at = i / (wide / 2) * kLine + part * wide + i % (wide / 2) * 2;
+        float2 s = make_float2(0.0f, 0.0f);
+        for (int v = 0; v < p.split; ++v) {
+          const float2 o = *reinterpret_cast<const float2*>(cluster.map_shared_rank(red, v) + at);
+          s.x += o.x;
+          s.y += o.y;
+        }
+        *reinterpret_cast<float2*>(sums + at) = s;
+      }
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < 2 * MT * wide; i += kThreads) {
+      const int cc = part * wide + i / (32 * MT) * 16 + i % 16, rank = (i / 32 % MT * 2 + i / 16 % 2) * 8;
+      float s[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = (rank + j) * kLine + cc;
+        s[j] = c * (p.split > 1 ? sums[at] : red[at] + sums[at]);
+      }
+      if (c0 + cc < C) store8(out + (int64_t)(c0 + cc) * p.r + r0 + rank, p.r - r0 - rank, p.width == 16, s);
+    }
+  } else {
+    const int each = kRanks * kCols / 8 / p.split;
     for (int i = threadIdx.x; i < each; i += kThreads) {
-      const int at = i / wide * kLine + part * wide + i % wide;
-      float s = 0.0f;
-      for (int v = 0; v < p.split; ++v) s += cluster.map_shared_rank(red, v)[at];
-      red[kRanks * kLine + at] = s;
+      const int rank = (part * each + i) / (kCols / 8), cc = (part * each + i) % (kCols / 8) * 8, at = rank * kLine + cc;
+      float s[8] = {};
+      auto add = [&](const float* o) {
+        const float4 u = *reinterpret_cast<const float4*>(o), w = *reinterpret_cast<const float4*>(o + 4);
+        s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w;
+        s[4] += w.x; s[5] += w.y; s[6] += w.z; s[7] += w.w;
+      };
+      if (p.split > 1) {
+        for (int v = 0; v < p.split; ++v) add(cluster.map_shared_rank(red, v) + at);
+      } else {
+        add(red + at);
+        add(sums + at);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] *= c;
+      if (r0 + rank < p.r) store8(out + (int64_t)(r0 + rank) * C + c0 + cc, C - c0 - cc, WHOLE, s);
     }
-    __syncthreads();
-  }
-  for (int i = threadIdx.x; i < each; i += kThreads) {
-    const int e = part * each + i, rank = TALL ? e % kRanks : e / kCols, cc = TALL ? e / kRanks : e % kCols, at = rank * kLine + cc;
-    float s;
-    if (p.split == 1) {
-      s = red[at] + red[kRanks * kLine + at];
-    } else if (TALL) {
-      s = red[kRanks * kLine + at];
-    } else {
-      s = 0.0f;
-      for (int v = 0; v < p.split; ++v) s += cluster.map_shared_rank(red, v)[at];
-    }
-    if (r0 + rank < p.r && c0 + cc < C) out[TALL ? (int64_t)(c0 + cc) * p.r + r0 + rank : (int64_t)(r0 + rank) * C + c0 + cc] = Elem<T>::from_float(c * s);
   }
   if (p.split > 1) cluster.sync();   // no block leaves while others read its sums
 }
@@ -855,8 +894,8 @@ int run(Step step, const Params& p, cudaStream_t st) {
 int run(Step step, Params p, int dtype, cudaStream_t st) {
   const bool lies = step == Step::Down || step == Step::UpWide;   // weights' rows are along the long dimension
   bool whole = p.C % 8 == 0;
-  for (const void* q : {p.x, p.y, lies ? p.w : nullptr, step == Step::Up || step == Step::UpWide ? static_cast<const void*>(p.out) : nullptr}) whole = whole && aligned(q, 16);
-  p.width = p.w && !lies ? width_of(p.w, 2 * p.r) : 2;
+  for (const void* q : {p.x, p.y, lies ? p.w : nullptr, step == Step::OuterTall ? nullptr : static_cast<const void*>(p.out)}) whole = whole && aligned(q, 16);
+  p.width = step == Step::OuterTall ? width_of(p.out, 2 * p.r) : (p.w && !lies ? width_of(p.w, 2 * p.r) : 2);
   if (dtype == B200Q_F16) return whole ? run<__half, true>(step, p, st) : run<__half, false>(step, p, st);
   return whole ? run<__nv_bfloat16, true>(step, p, st) : run<__nv_bfloat16, false>(step, p, st);
 }
