@@ -4,11 +4,10 @@
 //   backward  g = c B^T dy      down (weights [N, r], "tall")      dx = A^T g         up (weights [r, K], "wide")
 //             dA = sum g x^T    outer                              dB = c sum dy h^T  outer, transposed
 //
-// Rows come sorted by adapter (b200q_group_rows), in tiles of up to 64 rows of one adapter.  A rank of 8 to 64 makes r operations per
-// byte of activations, far below what the tensor cores do per byte of HBM, so the kernels are built for the memory: activations are read
-// once, straight into the fragments of mma.sync, 16 bytes per lane, without transposed copies.  That works because the k index of a product
-// may be permuted as long as both operands agree, and the columns of its result as long as the stores do: a lane's 8 consecutive values are
-// its fragments of several steps.  Operands that lie the other way round are transposed 8 x 8 in registers (movmatrix).
+// Rows come sorted by adapter (b200q_group_rows), in tiles of up to 64 rows of one adapter.  A rank of 8 to 64 makes r operations per byte of
+// activations, far below what the tensor cores do per byte of HBM, so the kernels are built for the memory: activations are read once per product and
+// nothing is written but h and the results.  The products are mma.sync (545 TFLOP/s measured here): tiles of a few rows whose number only the
+// device knows, operands that come in pieces from gathered rows and are split into two parts on the way; at rank 64 they take about as long as HBM does.
 //
 // h and g, summed in fp32, are kept as two bf16 numbers each, high and low part (2^-17 of the value is lost, a 32nd of what the
 // result's rounding to f16 loses), since that is how the second products take them; 16-bit floats of type f16 are split too, exactly, so that
@@ -233,8 +232,10 @@ __device__ __forceinline__ int row_at(const Params& p, int64_t place) {
 // row's would have to be brought together from two.
 // TALL: weights [C, r], else [r, C].
 //
-// Bound by the latency of its loads (with 64 ranks: by the products, too).  Every warp has a ring of its own in shared memory, filled some steps
-// ahead, in pieces of 16 bytes whose places are swizzled so that eight rows of a matrix are in different banks; no barrier but the warp's.
+// Every warp has a ring of its own in shared memory, filled some steps ahead, in pieces of 16 bytes whose places are swizzled so that eight rows of
+// a matrix are in different banks; no barrier but the warp's.  4096 rows of 16 adapters of rank 64, bf16: 21 us from K = 4096, 40 from K = 14336
+// (2.9 TB/s of x); what bounds it there is L2, from which the weights come again for every 64 rows, as many bytes as x has.  Few rows: latencies, 10 us for
+// 57 rows of 40 adapters of rank 20 (K 4096, f16).
 template <bool TALL, int MT>
 struct Down {
   static constexpr int kRanks = 16 * MT, kW = 2 * MT, kPieces = 8 + kW, kStages = MT == 4 ? 3 : 2;
@@ -395,13 +396,15 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) down_kernel(const P
 }
 
 // ---- out[row] = y[row] + (c) sum over ranks of h[place] w.  Blocks by (tiles, 256 columns), warps by 32 columns; steps of 16 rows and, inside, 16
-// ranks.  Up to 64 ranks (KS steps) have their weights in registers, over all rows that an adapter has among the block's tiles, and h in shared
-// memory; more (CHUNKED) take both from the caches again for every 16 rows.
+// ranks.  Up to 64 ranks (KS steps) have their weights in registers, over all rows that an adapter has among the block's tiles.  More (CHUNKED): the
+// sums of a tile stay in registers while its ranks come 32 at a time.  (4096 rows of rank 64, [14336, 4096], both products, us: 104, CHUNKED 119; rank 32: 72
+// and 86.  4096 rows of rank 128, [4096, 4096]: 66.)
 // WIDE: weights [r, C], else [C, r].
 //
 // Bound by the latency of y and by instructions: every lane copies its own pieces of y, three steps of rows ahead, into a ring in shared memory; the steps'
 // rows are looked up once per block; h lies in shared memory as the products' operands want it, so that one load brings four registers that are next to each
-// other (two rows loaded apart would have to be moved together for every product: half of all instructions).
+// other (two rows loaded apart would have to be moved together for every product: half of all instructions).  4096 rows of rank 64, bf16: 87 us for C = 14336 (2.7
+// TB/s), 31 for C = 4096 (3.2 TB/s).  The two parts' products alone would take 28 and 8, HBM 36 and 10.
 constexpr int kUpStages = 4, kUpTiles = 8, kUpSteps = kUpTiles * kRows / 16;
 template <int KS, bool CHUNKED>
 struct Up {
@@ -618,7 +621,9 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
 // ---- out_l = (c) sum over l's rows of h[place] x[row]^T.  Blocks by (128 columns, part of the rows; adapter; 16 MT ranks), the parts are a
 // cluster; warps by (32 columns, half of a step's 32 rows).  TALL: out [C, r], else [r, C].
 //
-// Rows lie in shared memory as they come, and matrix loads that transpose make both operands of them; h's two parts lie apart there.
+// Rows lie in shared memory as they come, and matrix loads that transpose make both operands of them; h's two parts lie apart there.  (Transposed in
+// registers for every 32 columns, 4096 rows of one adapter of rank 64 and 4096 columns took 90 us, now 27; HBM 5.)  Bound by latencies: a block has few steps,
+// and reads where its rows are before it reads them.  2048 rows of 4 adapters of rank 16: 17 us for 4096 columns, 26 for 14336 (2.3 TB/s).
 template <bool TALL, int MT>
 struct Outer {
   static constexpr int kRanks = 16 * MT, kCols = 128, kSteps = 32, kStages = 3;
@@ -797,7 +802,9 @@ int width_of(const void* p, int64_t pitch) {
   while (w > 2 && (!aligned(p, w) || pitch % w != 0)) w /= 2;
   return w;
 }
-// Blocks per cluster: a power of two up to 8, as many as fit on the SMs at once, with work for everyone.
+// Blocks per cluster: a power of two up to 8, as many as fit on the SMs at once, with work for everyone.  (With at most 1, 2, 4, 8, by graph replay, us: one row of
+// rank 16, [14336, 4096], forward 8.4 7.0 5.8 5.3, gradient of x 25.7 15.6 10.1 7.5; 57 rows of 40 adapters of rank 20, f16, [11008, 4096], gradient
+// of x 48 30 20 19; 4096 rows of rank 64 102 70 70 70.)
 int split_of(int64_t blocks, int64_t slots, int64_t most) {
   int s = 1;
   while (s < 8 && blocks * 2 * s <= slots && 2 * s <= most) s *= 2;

@@ -543,6 +543,9 @@ __device__ void sum_over_warps(uint32_t* hist, int bins, uint32_t* sums) {
   }
 }
 
+// A block has consecutive tokens, a warp a range of them.  Bound by the instructions of a token's dependent steps, HBM is idle: 8192 tokens, 8 of 256 experts in
+// groups with a bias, f32, 26 us with cold caches (320 GB/s; bytes would take 1.4) and 13 for the second launch, which begins beside it: 29 together in graph replay;
+// 16384 tokens, 8 of 128, bf16: 23 and 10, 22 together.  4 tokens: 4 us of latencies.
 template <typename T, int V>
 __global__ void __launch_bounds__(V > 16 ? 512 : 1024) route_kernel(const RouteParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -598,6 +601,7 @@ __global__ void __launch_bounds__(V > 16 ? 512 : 1024) route_kernel(const RouteP
   sort_finish(s, 0, sums, total, warp_sums);
 }
 
+// More rows: as route_kernel counts its pairs, 32 rows of a warp at a time.  Bound by the latency of ids, ranks and the second launch: 16384 rows of 40 groups 11 us.
 __global__ void __launch_bounds__(1024) group_kernel(const SortParams p, int64_t per_warp) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ uint32_t warp_sums[32];
@@ -634,7 +638,7 @@ __global__ void __launch_bounds__(1024) group_kernel(const SortParams p, int64_t
   sort_finish(p, 0, sums, total, warp_sums);
 }
 
-// Up to 128 rows per warp in one block: ids and ranks stay in registers.
+// Up to 128 rows per warp in one block: ids and ranks stay in registers.  (57 rows of 40 groups 3.9 us instead of 4.1, 1024 5.8 instead of 6.4, 4096 9.6 instead of 10.9.)
 __global__ void __launch_bounds__(1024) group_few_kernel(const SortParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ uint32_t warp_sums[32];
@@ -673,7 +677,8 @@ __global__ void __launch_bounds__(1024) group_few_kernel(const SortParams p) {
   sort_tables(p, base, total, warp_sums);
 }
 
-// The second launch: every block adds up the histograms of those before it.
+// The second launch: every block adds up the histograms of those before it, four bins at a time, by threads that share the blocks (148 KB from L2 for 256 bins), and
+// places its own pairs.  Bound by these two latencies: 10 to 13 us with cold caches, of which its start lies beside the first launch.
 __global__ void __launch_bounds__(1024) place_kernel(const SortParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ uint32_t warp_sums[32];
@@ -732,7 +737,9 @@ int place(const SortParams& s, cudaStream_t st) {
   return B200Q_OK;
 }
 
-// ---- the gradient of the weights with respect to the logits.  A warp has a token.
+// ---- the gradient of the weights with respect to the logits: d l = p (g - <g, p>) over all experts, or (renormalized) over those taken, where g = scale dw; sigmoid:
+// s (1 - s) g.  A warp has a token and reads its row again for each of three passes, from L1.  16384 tokens, 128 experts, bf16: 8 us in graph replay (1 TB/s of
+// logits and gradients; bytes would take 1.4): the chain of three sums over the warp.
 struct DlogitsParams {
   const float* dw;
   const void* logits;
@@ -809,7 +816,8 @@ int launch_route(const RouteParams& p, int blocks, int warps, cudaStream_t st) {
 }
 
 // Blocks and warps: up to 16 tokens in one block, one launch; else 8 tokens or more per block, one block of up to 32 warps per SM, whose histograms the
-// second launch reads.  (64 tokens of 256 experts in groups: 29 us in one block of 32 warps, which share an SM's instructions.)
+// second launch reads.  (One block / several, us: 16 tokens, 2 of 8 experts, 6.0 / 9.6, 8 of 256 in groups 9.6 / 11.1; 32 tokens 8.2 / 9.6 and 14.6 / 11.1; 64 tokens 9.9 / 9.6
+// and 22 / 11.1: many experts share one SM's instructions.)
 struct Split { int blocks, warps; int64_t per_block, per_warp; };
 Split route_split(int64_t T, int64_t E) {
   Split s{};
@@ -822,6 +830,7 @@ Split route_split(int64_t T, int64_t E) {
   s.warps = (int)((s.per_block + s.per_warp - 1) / s.per_warp);
   return s;
 }
+// Up to 4096 rows in one block.  (40 groups, one block / several, us: 4096 rows 9.6 / 11.0, 8192 16.6 / 10.9.)
 Split group_split(int64_t T, int64_t n) {
   Split s{};
   s.warps = n <= 512 ? 32 : (n <= 1024 ? 16 : 8);   // their histograms share 132 KB at most

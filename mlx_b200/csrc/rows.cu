@@ -4,7 +4,7 @@
 //   combine   y[t] = sum over j of w[t, j] ys[places[t, j]]   (without w: the gradient of dispatch)
 //   its gradients  d ys[places[t, j]] = w[t, j] dy[t],  d w[t, j] = <dy[t], ys[places[t, j]]>
 //
-// Everything is bound by HBM, so every kernel goes by tokens: a token's row is read (or written) once, the experts' rows once each,
+// Everything is bound by HBM, so a token's row is read from there (or written) once, the experts' rows once each,
 // in pieces of 16 bytes.  Sums are fp32 in the order of j, rounded once.  A place outside [0, T top) is a pair without a row:
 // it adds nothing and gets nothing.  Rows that no pair has are those whose `order` is negative, the last ones; they get zeros.
 #include <algorithm>
@@ -32,7 +32,8 @@ struct RowsParams {
   int top;
 };
 
-// ---- rows that are whole pieces of 16 bytes on their boundaries
+// ---- rows that are whole pieces of 16 bytes on their boundaries.  dispatch and combine: a thread has a piece of a token and its pairs' pieces.  4096 tokens, 2 of 8
+// experts, 4096 wide, bf16, by graph replay: dispatch 15.7 us (6.4 TB/s, 0.98 of the measured copy rate), combine 19.6 (5.1), without weights 19.0.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) dispatch_kernel(const RowsParams p) {
   using V = Vec<T, VEC>;
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const RowsParams p) {
   }
 }
 
-// A block has a token.
+// A block has a token, whose row stays in L1 for its pairs.  The same rows: 29.3 us (5.7 TB/s).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const RowsParams p) {
   using V = Vec<T, VEC>;
@@ -128,7 +129,8 @@ __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const RowsParams
 
 // ---- rows that start anywhere.  A block has a token.  What is written to a row goes by the pieces of 16 bytes of memory that it covers: whole ones by
 // one store, those at its ends value by value.  What is read for a whole piece is 16 bytes from any address: two pieces of memory and a shift.  (Both hold bytes of
-// the row, and memory is mapped by more than 16 bytes, so that nothing outside is touched that is not there.)
+// the row, and memory is mapped by more than 16 bytes, so that nothing outside is touched that is not there.)  1531 tokens, 6 of 64 experts, 2047 wide, f16, by graph
+// replay: dispatch 12.2 us (3.6 TB/s), combine 10.5, its gradients 18.2 (4.5); bound by instructions, the shifts and the rows' ends.
 template <typename T>
 __device__ __forceinline__ Vec<T, 16 / sizeof(T)> load_any(const T* p) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(p);
@@ -215,8 +217,8 @@ __global__ void __launch_bounds__(kThreads) combine_any_kernel(const RowsParams 
   });
 }
 
-// A group of threads has a pair (token, choice): a warp, or the block where there are few pairs.  dy's row is read once from HBM and for the token's other
-// pairs from L2.
+// A group of threads has a pair (token, choice): a warp, or the block where there are few pairs, up to a wave of blocks.  (Rows of 2047, f16, block / warp, us: 8 pairs 2.7 / 6.8,
+// 800 5.1 / 7.4, 1200 6.2 / 7.8, 9186 33.6 / 18.8.)  dy's row is read once from HBM and for the token's other pairs from L2.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) combine_grad_any_kernel(const RowsParams p, int group) {
   constexpr int VEC = 16 / sizeof(T);
