@@ -1,4 +1,4 @@
-"""mlx_b200 - B200-native (sm_100a) quantized matmul operators and products grouped by expert.
+"""mlx_b200 - B200-native (sm_100a) quantized matmul operators, products grouped by expert, routing and adapters.
 
 Drop-in for the reference's ``quantize`` / ``dequantize`` / ``quantized_matmul`` /
 ``gather_qmm`` operators; see ``mlx_b200.ops`` for the operator front-end and

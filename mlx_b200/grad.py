@@ -8,6 +8,9 @@ QuantizedMatmul::vjp (mlx/primitives.cpp:3532-3598):
 
 The product for d x runs on this library's kernels (the non-transposed form of the forward);
 dW is a plain dense product (torch.matmul, a library GEMM) followed by group sums.
+
+grouped_mm has gradients of any order; route_experts, dispatch_rows, combine_rows and add_adapters of first order, whose
+own backward passes are refused.
 """
 from typing import Optional
 

@@ -5,7 +5,8 @@ Same names, argument meaning and error behaviour as ``mlx.core.quantize``,
 quantized_matmul, :5208-5245 quantize, :5465-5517 dequantize, :5553-5629 gather_qmm;
 validation helpers :110-181, :4704-4754) in the affine mode.  ``quantize``, ``dequantize`` and ``qqmm`` have the
 microscaled 4-bit modes ``mxfp4`` and ``nvfp4`` too; ``grouped_mm`` and ``grouped_qqmm`` are products of rows that are
-already sorted by expert, with one size per expert.  Arrays are ``torch`` CUDA tensors: torch only
+already sorted by expert, with one size per expert; ``route_experts``, ``dispatch_rows`` and ``combine_rows`` bring tokens
+there and back, ``group_rows`` and ``add_adapters`` put low-rank adapters beside a shared projection.  Arrays are ``torch`` CUDA tensors: torch only
 supplies device memory and streams, every computation is a call into libb200q.so.
 Invalid arguments raise ``ValueError`` (the reference's std::invalid_argument).
 """
