@@ -210,7 +210,7 @@ struct Params {
   int64_t T, C;            // rows; the long dimension (K or N)
   int64_t tiles_n;
   int L, r, r16, width;    // r16: r in whole 16s; width: bytes that the rows of weights [C, r] (or of their gradient) are aligned to
-  int split, each;         // blocks per cluster; tiles per block
+  int split, each;         // blocks per cluster; tiles per block (0: the block counts them)
 };
 
 // A tile, or none (rows == 0) where the table does not fit the operands.
@@ -224,6 +224,26 @@ __device__ __forceinline__ int row_at(const Params& p, int64_t place) {
   int row = p.order[place];
   row = row < 0 ? ~row : row;
   return row < (int)p.T ? row : -1;
+}
+
+// How many tiles have rows (with_adapter: of an adapter); they come first in the table, so that a search by the whole block finds the end: 256 of them are looked
+// at at once.
+__device__ int64_t tiles_with_rows(const Params& p, bool with_adapter) {
+  int64_t lo = 0, n = p.tiles_n;   // all before lo have rows, none from lo + n on
+  while (n > 0) {
+    const int64_t each = (n + kThreads - 1) / kThreads, at = lo + threadIdx.x * each;   // of every part its first one
+    bool has = false;
+    if (threadIdx.x * each < n) {
+      const int4 t = p.tiles[at];
+      has = t.z > 0 && (!with_adapter || t.x >= 0);
+    }
+    const int parts = __syncthreads_count(has);
+    if (parts == 0) break;
+    const int64_t end = lo + n;
+    lo += (parts - 1) * each + 1;
+    n = min(each - 1, end - lo);
+  }
+  return lo;
 }
 
 // ---- h[place] = (c) sum over the long dimension of x[row] w.  Blocks by (tile, part of the long dimension, 16 MT ranks); the parts are a cluster
@@ -405,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) down_kernel(const P
 // rows are looked up once per block; h lies in shared memory as the products' operands want it, so that one load brings four registers that are next to each
 // other (two rows loaded apart would have to be moved together for every product: half of all instructions).  4096 rows of rank 64, bf16: 87 us for C = 14336 (2.7
 // TB/s), 31 for C = 4096 (3.2 TB/s).  The two parts' products alone would take 28 and 8, HBM 36 and 10.
-constexpr int kUpStages = 4, kUpTiles = 8, kUpSteps = kUpTiles * kRows / 16;
+constexpr int kUpStages = 4, kUpTiles = 16, kUpSteps = kUpTiles * kRows / 16;
 template <int KS, bool CHUNKED>
 struct Up {
   static constexpr int kStep = KS * 1024;   // bytes of h per step of 16 rows: [rank step][part][lane][4]
@@ -424,198 +444,205 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
   const bool in = have > 0, add = p.y != nullptr && in;
   const T* y = static_cast<const T*>(p.y) + n;
   T* out = static_cast<T*>(p.out) + n;
-  if (threadIdx.x < kUpTiles) {
-    const int64_t k = (int64_t)(blockIdx.x / blocks) * p.each + threadIdx.x;
-    int4 t = make_int4(-1, 0, 0, 0);
-    if (threadIdx.x < p.each && k < p.tiles_n) t = tile_of(p, k);
-    if (t.x < 0 && p.y == p.out) t.z = 0;   // rows without an adapter are there already
-    tiles[threadIdx.x] = t;
-  }
-  for (int i = threadIdx.x; i < (kUpSteps + kUpStages) * 16; i += kThreads) rows[i / 16][i % 16] = -1;
-  __syncthreads();
-  int steps = 0;
-  for (int k = 0; k < p.each; ++k) {
-    const int4 t = tiles[k];
-    for (int i = threadIdx.x; i < t.z; i += kThreads) rows[steps + i / 16][i % 16] = row_at(p, t.y + i);
-    steps += (t.z + 15) / 16;
-  }
-  const uint32_t ring = shared(smem) + warp * kUpStages * 1024 + lane * 16, hs = shared(smem) + kWarps * kUpStages * 1024;
-  auto next_tile = [&](int k) {
-    while (k < p.each && tiles[k].z == 0) ++k;
-    return k;
-  };
-  auto copy_h = [&](int k, int r0, int buffer) {
-    if (k >= p.each || tiles[k].x < 0) return;
-    constexpr int kPer = 4 * KS, kSweep = kThreads / kPer;   // pieces of 16 bytes per row; rows that the block copies at once
-    const int piece = threadIdx.x % kPer, row = threadIdx.x / kPer, z = tiles[k].z;
-    if (r0 + piece * 4 >= p.r16) return;
-    const uint16_t* src = p.h + (int64_t)(tiles[k].y + row) * 2 * p.r16 + r0 * 2 + piece * 8;
-    const uint32_t to = hs + buffer * 4 * kStep + piece / 4 * 1024 + piece % 4 * 16;
-#pragma unroll
-    for (int i = 0; i < kRows / kSweep; ++i) {
-      const int at = row + i * kSweep;
-      if (at >= z) break;
-      const uint32_t d = to + at / 16 * kStep + at % 8 * 64 + at / 8 % 2 * 4;
-      copy_async<4>(d, src, true);             // high part, first pair of ranks
-      copy_async<4>(d + 8, src + 2, true);     // second pair
-      copy_async<4>(d + 512, src + 4, true);   // low part
-      copy_async<4>(d + 520, src + 6, true);
-      src += (int64_t)kSweep * 2 * p.r16;
-    }
-  };
   uint32_t bh[KS][4][2], bl[kSplitW ? KS : 1][4][2];   // rank step, column tile, pair of the lane's 4 ranks
-  const T* w = nullptr;
-  auto weights = [&](int r0) {
-    uint32_t b[KS][4][2];
+  int loaded = -1;                                     // whose weights they are
+  const int64_t part = blockIdx.x / blocks, parts = gridDim.x / blocks, n_tiles = p.each ? p.tiles_n : tiles_with_rows(p, p.y == p.out);
+  const int64_t end = p.each ? min((part + 1) * p.each, n_tiles) : n_tiles * (part + 1) / parts;
+  for (int64_t first = p.each ? part * p.each : n_tiles * part / parts; first < end; first += kUpTiles) {
+    const int count = (int)min((int64_t)kUpTiles, end - first);
+    __syncthreads();   // everyone is through with the tiles before
+    if (threadIdx.x < count) {
+      int4 t = tile_of(p, first + threadIdx.x);
+      if (t.x < 0 && p.y == p.out) t.z = 0;   // rows without an adapter are there already
+      tiles[threadIdx.x] = t;
+    }
+    for (int i = threadIdx.x; i < (kUpSteps + kUpStages) * 16; i += kThreads) rows[i / 16][i % 16] = -1;
+    __syncthreads();
+    int steps = 0;
+    for (int k = 0; k < count; ++k) {   // (four tiles at once)
+      const int4 t = tiles[k];
+      const int i = threadIdx.x % kRows;
+      if (k % (kThreads / kRows) == threadIdx.x / kRows && i < t.z) rows[steps + i / 16][i % 16] = row_at(p, t.y + i);
+      steps += (t.z + 15) / 16;
+    }
+    const uint32_t ring = shared(smem) + warp * kUpStages * 1024 + lane * 16, hs = shared(smem) + kWarps * kUpStages * 1024;
+    auto next_tile = [&](int k) {
+      while (k < count && tiles[k].z == 0) ++k;
+      return k;
+    };
+    auto copy_h = [&](int k, int r0, int buffer) {
+      if (k >= count || tiles[k].x < 0) return;
+      constexpr int kPer = 4 * KS, kSweep = kThreads / kPer;   // pieces of 16 bytes per row; rows that the block copies at once
+      const int piece = threadIdx.x % kPer, row = threadIdx.x / kPer, z = tiles[k].z;
+      if (r0 + piece * 4 >= p.r16) return;
+      const uint16_t* src = p.h + (int64_t)(tiles[k].y + row) * 2 * p.r16 + r0 * 2 + piece * 8;
+      const uint32_t to = hs + buffer * 4 * kStep + piece / 4 * 1024 + piece % 4 * 16;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      if constexpr (WIDE) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int rank = r0 + s * 16 + (g >> 1) * 4 + j * 2 + (g & 1);
-          const uint4 v = rank < p.r ? load8<WHOLE>(w + (int64_t)rank * C + n, have) : make_uint4(0, 0, 0, 0);
-          b[s][0][j] = v.x; b[s][1][j] = v.y; b[s][2][j] = v.z; b[s][3][j] = v.w;
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int col = n0 + (g >> 1) * 8 + t * 2 + (g & 1), rank = r0 + s * 16 + q * 4;
-          load_few<4>(w + (int64_t)col * p.r + rank, col < C ? p.r - rank : 0, p.width, b[s][t]);
-        }
+      for (int i = 0; i < kRows / kSweep; ++i) {
+        const int at = row + i * kSweep;
+        if (at >= z) break;
+        const uint32_t d = to + at / 16 * kStep + at % 8 * 64 + at / 8 % 2 * 4;
+        copy_async<4>(d, src, true);             // high part, first pair of ranks
+        copy_async<4>(d + 8, src + 2, true);     // second pair
+        copy_async<4>(d + 512, src + 4, true);   // low part
+        copy_async<4>(d + 520, src + 6, true);
+        src += (int64_t)kSweep * 2 * p.r16;
       }
-    }
+    };
+    const T* w = nullptr;
+    auto weights = [&](int r0) {
+      uint32_t b[KS][4][2];
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+      for (int s = 0; s < KS; ++s) {
+        if constexpr (WIDE) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t lo;
-          as_bf16<T>(WIDE ? transposed(b[s][t][j]) : b[s][t][j], &bh[s][t][j], &lo);
-          if constexpr (kSplitW) bl[s][t][j] = lo;
-        }
-  };
-  int k = next_tile(0), buffer = 0, loaded = -1, ahead = 0, now = 0;
-  auto issue = [&] {   // y of the next step
-    const uint32_t to = ring + (ahead % kUpStages) * 1024;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = rows[ahead][i * 8 + g];
-      if constexpr (WHOLE) copy_async<16>(to + i * 512, y + (int64_t)row * C, add && row >= 0);
-      else store16(to + i * 512, add && row >= 0 ? load8<false, false>(y + (int64_t)row * C, have) : make_uint4(0, 0, 0, 0));
-    }
-    commit();
-    ++ahead;
-  };
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kUpStages - 1; ++i) issue();
-  if (!CHUNKED && k < p.each && tiles[k].x >= 0) {
-    loaded = tiles[k].x;
-    w = static_cast<const T*>(p.w) + (int64_t)loaded * p.r * C;
-    weights(0);
-  }
-  asm volatile("griddepcontrol.wait;" ::: "memory");   // all of h, of the launch before
-  copy_h(k, 0, 0);
-  commit();
-  for (int last = 4; k < p.each;) {
-    const int4 tile = tiles[k];
-    const bool plain = tile.x < 0;   // rows without an adapter
-    float c = 0.0f;
-    if (!plain) {
-      c = p.scales ? p.scales[tile.x] : 1.0f;
-      w = static_cast<const T*>(p.w) + (int64_t)tile.x * p.r * C;
-      if (!CHUNKED && loaded != tile.x) {
-        weights(0);
-        loaded = tile.x;
-      }
-    }
-    const int after = next_tile(k + 1), before = last;
-    last = (tile.z + 15) / 16;
-    auto finish = [&](const float (&acc)[4][4]) {   // the step's sums to its rows
-      wait_all_but<kUpStages - 1>();
-      const uint32_t from = ring + (now % kUpStages) * 1024;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = rows[now][i * 8 + g];
-        if (row < 0 || !in) continue;
-        const float sum[8] = {acc[0][2 * i], acc[0][2 * i + 1], acc[1][2 * i], acc[1][2 * i + 1], acc[2][2 * i], acc[2][2 * i + 1], acc[3][2 * i], acc[3][2 * i + 1]};
-        uint4 v = load16(from + i * 512);
-        if (!plain) v = add8<T>(v, c, sum);
-        T* o = out + (int64_t)row * C;
-        if constexpr (WHOLE) {
-          *reinterpret_cast<uint4*>(o) = v;
+          for (int j = 0; j < 2; ++j) {
+            const int rank = r0 + s * 16 + (g >> 1) * 4 + j * 2 + (g & 1);
+            const uint4 v = rank < p.r ? load8<WHOLE>(w + (int64_t)rank * C + n, have) : make_uint4(0, 0, 0, 0);
+            b[s][0][j] = v.x; b[s][1][j] = v.y; b[s][2][j] = v.z; b[s][3][j] = v.w;
+          }
         } else {
-          T e[8];
-          *reinterpret_cast<uint4*>(e) = v;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j < have) o[j] = e[j];
-        }
-      }
-      ++now;
-    };
-    auto step = [&](float (&acc)[4][4], int s, const uint4& hi, const uint4& lo) {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], hi.x, hi.y, hi.z, hi.w, bh[s][t][0], bh[s][t][1]);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], lo.x, lo.y, lo.z, lo.w, bh[s][t][0], bh[s][t][1]);
-      if constexpr (kSplitW) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], hi.x, hi.y, hi.z, hi.w, bl[s][t][0], bl[s][t][1]);
-      }
-    };
-    // (rows behind the tile's last one have what was there before; their products are not stored)
-    if constexpr (CHUNKED) {
-      float acc[kRows / 16][4][4] = {};
-      for (int r0 = 0; r0 == 0 || (r0 < p.r16 && !plain); r0 += 16 * KS, buffer ^= 1) {
-        // these ranks' h was issued before the last tile's four steps, or last
-        if (r0 == 0 && now != 0 && before == 4) wait_all_but<4>();
-        else wait_all_but<0>();
-        __syncthreads();
-        if (r0 + 16 * KS < p.r16 && !plain) copy_h(k, r0 + 16 * KS, buffer ^ 1);
-        else copy_h(after, 0, buffer ^ 1);
-        commit();
-        if (plain) continue;
-        weights(r0);
-        const uint32_t src = hs + buffer * 4 * kStep + lane * 16;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          if (r0 + s * 16 >= p.r16) break;
-#pragma unroll
-          for (int m = 0; m < kRows / 16; ++m)
-            if (m < last) step(acc[m], s, load16(src + m * kStep + s * 1024), load16(src + m * kStep + s * 1024 + 512));
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < kRows / 16; ++m)
-        if (m < last) {
-          issue();
-          finish(acc[m]);
-        }
-    } else {
-      // the group with this tile's h was issued with the first step of the tile before, four steps ago if that was a whole one
-      if (now == 0 || before < 4) wait_all_but<0>();
-      __syncthreads();
-      copy_h(after, 0, buffer ^ 1);
-      uint32_t src = hs + buffer * 4 * kStep + lane * 16;
-      for (int m = 0; m < last; ++m, src += kStep) {
-        issue();
-        float acc[4][4] = {};
-        if (!plain) {
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            if (KS > 1 && s * 16 >= p.r16) break;
-            step(acc, s, load16(src + s * 1024), load16(src + s * 1024 + 512));
+          for (int t = 0; t < 4; ++t) {
+            const int col = n0 + (g >> 1) * 8 + t * 2 + (g & 1), rank = r0 + s * 16 + q * 4;
+            load_few<4>(w + (int64_t)col * p.r + rank, col < C ? p.r - rank : 0, p.width, b[s][t]);
           }
         }
-        finish(acc);
       }
-      buffer ^= 1;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t lo;
+            as_bf16<T>(WIDE ? transposed(b[s][t][j]) : b[s][t][j], &bh[s][t][j], &lo);
+            if constexpr (kSplitW) bl[s][t][j] = lo;
+          }
+    };
+    int k = next_tile(0), buffer = 0, ahead = 0, now = 0;
+    auto issue = [&] {   // y of the next step
+      const uint32_t to = ring + (ahead % kUpStages) * 1024;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = rows[ahead][i * 8 + g];
+        if constexpr (WHOLE) copy_async<16>(to + i * 512, y + (int64_t)row * C, add && row >= 0);
+        else store16(to + i * 512, add && row >= 0 ? load8<false, false>(y + (int64_t)row * C, have) : make_uint4(0, 0, 0, 0));
+      }
+      commit();
+      ++ahead;
+    };
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kUpStages - 1; ++i) issue();
+    if (!CHUNKED && k < count && tiles[k].x >= 0 && loaded != tiles[k].x) {
+      loaded = tiles[k].x;
+      w = static_cast<const T*>(p.w) + (int64_t)loaded * p.r * C;
+      weights(0);
     }
-    k = after;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // all of h, of the launch before
+    copy_h(k, 0, 0);
+    commit();
+    for (int last = 4; k < count;) {
+      const int4 tile = tiles[k];
+      const bool plain = tile.x < 0;   // rows without an adapter
+      float c = 0.0f;
+      if (!plain) {
+        c = p.scales ? p.scales[tile.x] : 1.0f;
+        w = static_cast<const T*>(p.w) + (int64_t)tile.x * p.r * C;
+        if (!CHUNKED && loaded != tile.x) {
+          weights(0);
+          loaded = tile.x;
+        }
+      }
+      const int after = next_tile(k + 1), before = last;
+      last = (tile.z + 15) / 16;
+      auto finish = [&](const float (&acc)[4][4]) {   // the step's sums to its rows
+        wait_all_but<kUpStages - 1>();
+        const uint32_t from = ring + (now % kUpStages) * 1024;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = rows[now][i * 8 + g];
+          if (row < 0 || !in) continue;
+          const float sum[8] = {acc[0][2 * i], acc[0][2 * i + 1], acc[1][2 * i], acc[1][2 * i + 1], acc[2][2 * i], acc[2][2 * i + 1], acc[3][2 * i], acc[3][2 * i + 1]};
+          uint4 v = load16(from + i * 512);
+          if (!plain) v = add8<T>(v, c, sum);
+          T* o = out + (int64_t)row * C;
+          if constexpr (WHOLE) {
+            *reinterpret_cast<uint4*>(o) = v;
+          } else {
+            T e[8];
+            *reinterpret_cast<uint4*>(e) = v;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (j < have) o[j] = e[j];
+          }
+        }
+        ++now;
+      };
+      auto step = [&](float (&acc)[4][4], int s, const uint4& hi, const uint4& lo) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], hi.x, hi.y, hi.z, hi.w, bh[s][t][0], bh[s][t][1]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], lo.x, lo.y, lo.z, lo.w, bh[s][t][0], bh[s][t][1]);
+        if constexpr (kSplitW) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], hi.x, hi.y, hi.z, hi.w, bl[s][t][0], bl[s][t][1]);
+        }
+      };
+      // (rows behind the tile's last one have what was there before; their products are not stored)
+      if constexpr (CHUNKED) {
+        float acc[kRows / 16][4][4] = {};
+        for (int r0 = 0; r0 == 0 || (r0 < p.r16 && !plain); r0 += 16 * KS, buffer ^= 1) {
+          // these ranks' h was issued before the last tile's four steps, or last
+          if (r0 == 0 && now != 0 && before == 4) wait_all_but<4>();
+          else wait_all_but<0>();
+          __syncthreads();
+          if (r0 + 16 * KS < p.r16 && !plain) copy_h(k, r0 + 16 * KS, buffer ^ 1);
+          else copy_h(after, 0, buffer ^ 1);
+          commit();
+          if (plain) continue;
+          weights(r0);
+          const uint32_t src = hs + buffer * 4 * kStep + lane * 16;
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            if (r0 + s * 16 >= p.r16) break;
+#pragma unroll
+            for (int m = 0; m < kRows / 16; ++m)
+              if (m < last) step(acc[m], s, load16(src + m * kStep + s * 1024), load16(src + m * kStep + s * 1024 + 512));
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < kRows / 16; ++m)
+          if (m < last) {
+            issue();
+            finish(acc[m]);
+          }
+      } else {
+        // the group with this tile's h was issued with the first step of the tile before, four steps ago if that was a whole one
+        if (now == 0 || before < 4) wait_all_but<0>();
+        __syncthreads();
+        copy_h(after, 0, buffer ^ 1);
+        uint32_t src = hs + buffer * 4 * kStep + lane * 16;
+        for (int m = 0; m < last; ++m, src += kStep) {
+          issue();
+          float acc[4][4] = {};
+          if (!plain) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              if (KS > 1 && s * 16 >= p.r16) break;
+              step(acc, s, load16(src + s * 1024), load16(src + s * 1024 + 512));
+            }
+          }
+          finish(acc);
+        }
+        buffer ^= 1;
+      }
+      k = after;
+    }
+    wait_all_but<0>();
   }
-  wait_all_but<0>();
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // (blocks without work: who comes next waits for the first product through this one)
 }
 
 // ---- out_l = (c) sum over l's rows of h[place] x[row]^T.  Blocks by (128 columns, part of the rows; adapter; 16 MT ranks), the parts are a
@@ -822,7 +849,7 @@ int tiles_per_block(const Params& p, int64_t cols, int64_t slots) {
   const int64_t tiles = likely_tiles(p);
   double best = 0;
   int each = 1;
-  for (int e = 1; e <= kUpTiles; ++e) {
+  for (int e = 1; e <= 8; ++e) {
     const double time = (double)(((tiles + e - 1) / e * cols + slots - 1) / slots) * (e + 0.75);
     if (e == 1 || time < best) { best = time; each = e; }
   }
@@ -867,8 +894,13 @@ template <typename T, bool WIDE, bool WHOLE>
 int up(Params p, cudaStream_t st) {
   p.split = 1;
   const int64_t cols = (p.C + 255) / 256;
-  p.each = tiles_per_block(p, cols, 148 * (p.r > 64 ? 2 : (p.r > 32 ? 2 : 3) - std::is_same_v<T, __half>));
-  const dim3 grid((unsigned)((p.tiles_n + p.each - 1) / p.each * cols));
+  const int64_t slots = 148 * (p.r > 64 ? 2 : (p.r > 32 ? 2 : 3) - std::is_same_v<T, __half>);
+  // Blocks with 8 tiles or more each count the tiles that have rows and share them evenly, in one wave; for fewer the count costs more than a last wave.  (Counted /
+  // not, graph replay, us: 4096 rows of 5 of 16 adapters of rank 64, [14336, 4096] 96 / 104, 4096 rows of rank 64, [4096, 4096] 43.6 / 43.1, 16 rows of as many adapters 7.3 / 6.7, 57 rows
+  // of 40 adapters, f16, both projections 41.6 / 39.3.)
+  p.each = likely_tiles(p) * cols >= 8 * slots ? 0 : tiles_per_block(p, cols, slots);
+  const int64_t parts = p.each ? (p.tiles_n + p.each - 1) / p.each : std::max<int64_t>(1, slots / cols);
+  const dim3 grid((unsigned)(cols * parts));
   if (p.r <= 16) return launch(up_kernel<T, WIDE, WHOLE, 1, false>, p, grid, kThreads, Up<1, false>::kBytes, st, true);
   if (p.r <= 32) return launch(up_kernel<T, WIDE, WHOLE, 2, false>, p, grid, kThreads, Up<2, false>::kBytes, st, true);
   if (p.r <= 64) return launch(up_kernel<T, WIDE, WHOLE, 4, false>, p, grid, kThreads, Up<4, false>::kBytes, st, true);

@@ -350,3 +350,23 @@ def test_sums_in_place_and_autograd():
     with torch.inference_mode():
         t = y.clone()
         assert torch.equal(mb.add_adapters(t, x, a, b, groups, s, out=t), ref)
+
+
+@pytest.mark.parametrize("T,N,K,r,dtype", ((32000, 1032, 72, 33, "f16"), (16000, 1030, 64, 66, "f16"), (700, 38200, 64, 33, "f16"), (9000, 8200, 64, 4, "bf16")))
+@pytest.mark.parametrize("last", (0.0, 0.9))
+def test_many_tiles(T, N, K, r, dtype, last):
+    """Many tiles per block of the second product, and columns for more blocks than there is room for; with some rows or most of them without an adapter."""
+    g = torch.Generator().manual_seed(21)
+    ids = torch.randint(-1, 3, (T,), generator=g)
+    ids[torch.rand(T, generator=g) < last] = -1
+    ids = ids.cuda()
+    y, x, a, b, s = problem(22, ids, 4, r, N, K, DTYPES[dtype])
+    groups = mb.group_rows(ids, 4)
+    out = mb.add_adapters(y, x, a, b, groups, s)
+    near(out, *exact(ids, y, x, a, b, s), K + r)
+    y2 = y.clone()
+    mb.add_adapters(y2, x, a, b, groups, s, out=y2)
+    assert torch.equal(y2, out)
+    _, h = ops._add_adapters(y, x, a, b, groups, s)
+    dx, _, _ = mb.add_adapters_grad(y, x, a, b, groups, h, s, True, False, False)
+    assert (dx[ids < 0] == 0).all()
