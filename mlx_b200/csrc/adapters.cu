@@ -417,14 +417,15 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) down_kernel(const P
 
 // ---- out[row] = y[row] + (c) sum over ranks of h[place] w.  Blocks by (tiles, 256 columns), warps by 32 columns; steps of 16 rows and, inside, 16
 // ranks.  Up to 64 ranks (KS steps) have their weights in registers, over all rows that an adapter has among the block's tiles.  More (CHUNKED): the
-// sums of a tile stay in registers while its ranks come 32 at a time.  (4096 rows of rank 64, [14336, 4096], both products, us: 104, CHUNKED 119; rank 32: 72
-// and 86.  4096 rows of rank 128, [4096, 4096]: 66.)
+// sums of a tile stay in registers while its ranks come 32 at a time.  (4096 rows of rank 64, [14336, 4096], both products, before the tiles were shared evenly, us: 104, CHUNKED
+// 119; rank 32: 72 and 86.  4096 rows of rank 128, [4096, 4096]: 67.)
 // WIDE: weights [r, C], else [C, r].
 //
 // Bound by the latency of y and by instructions: every lane copies its own pieces of y, three steps of rows ahead, into a ring in shared memory; the steps'
 // rows are looked up once per block; h lies in shared memory as the products' operands want it, so that one load brings four registers that are next to each
-// other (two rows loaded apart would have to be moved together for every product: half of all instructions).  4096 rows of rank 64, bf16: 87 us for C = 14336 (2.7
-// TB/s), 31 for C = 4096 (3.2 TB/s).  The two parts' products alone would take 28 and 8, HBM 36 and 10.
+// other (two rows loaded apart would have to be moved together for every product: half of all instructions).  4096 rows of rank 64, bf16, cold: 84 us for C = 14336 (2.8
+// TB/s), 31 for C = 4096 (3.2 TB/s): tensor cores 33 %, loads and stores of shared memory 58 %, HBM 30 %, 16 warps on an SM for their registers; the two parts' products alone
+// would take 28 and 8, HBM 36 and 10.
 constexpr int kUpStages = 4, kUpTiles = 16, kUpSteps = kUpTiles * kRows / 16;
 template <int KS, bool CHUNKED>
 struct Up {
