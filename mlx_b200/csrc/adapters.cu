@@ -649,12 +649,14 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
 // ---- out_l = (c) sum over l's rows of h[place] x[row]^T.  Blocks by (128 columns, part of the rows; adapter; 16 MT ranks), the parts are a
 // cluster; warps by (32 columns, half of a step's 32 rows).  TALL: out [C, r], else [r, C].
 //
-// Rows lie in shared memory as they come, and matrix loads that transpose make both operands of them; h's two parts lie apart there.  (Transposed in
-// registers for every 32 columns, 4096 rows of one adapter of rank 64 and 4096 columns took 90 us, now 27; HBM 5.)  Bound by latencies: a block has few steps,
-// and reads where its rows are before it reads them.  2048 rows of 4 adapters of rank 16: 17 us for 4096 columns, 26 for 14336 (2.3 TB/s).
+// Rows lie in shared memory as they come, and matrix loads that transpose make both operands of them; h's two parts lie apart there.  Which rows come next is
+// copied there, too, a ring ahead, so that no step waits for it.  (4096 rows of one adapter of rank 64 and 4096 columns: 27 us, 90 when every 32 columns' h was
+// transposed in registers; HBM 5.  2048 rows of 4 adapters of rank 16, [14336, 4096], forward and all gradients: 98 us, 106 with three stages and rows looked up
+// one step ahead; 1000 adapters of a row each have no use for it: 229 and 215.)  Bound by latencies: a block has few steps, and reads where its rows are before it
+// reads them; with 64 ranks tensor cores and shared memory are at a third and two thirds.
 template <bool TALL, int MT>
 struct Outer {
-  static constexpr int kRanks = 16 * MT, kCols = 128, kSteps = 32, kStages = 3;
+  static constexpr int kRanks = 16 * MT, kCols = 128, kSteps = 32, kStages = MT == 1 ? 5 : 4;
   static constexpr int kXPitch = kCols * 2 + 16, kHPitch = kRanks * 2 + 16;   // (eight rows of a matrix are in different banks)
   static constexpr int kStage = kSteps * (kXPitch + 2 * kHPitch);
   static constexpr int kLine = kCols + (TALL ? 2 : 8);   // floats per rank of the sums
@@ -676,19 +678,17 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) outer_kernel(const 
   const int xr = threadIdx.x / 16, xc = threadIdx.x % 16, hr = threadIdx.x / kPer, hc = threadIdx.x % kPer, have = C - c0 - xc * 8;
   const T* x = static_cast<const T*>(p.x) + c0 + xc * 8;
   const bool ranks = hr < O::kSteps && r0 + hc * 4 < p.r16;
+  __shared__ int order[kStages][O::kSteps];   // of the steps that are loaded next: copied a ring ahead of their rows
   int place = first;   // of the step that is loaded
-  int row[2];
-  auto look = [&] {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int at = place + xr + i * 16;
-      row[i] = at < hi ? p.order[at] : -1;
-      if (row[i] >= (int)p.T) row[i] = -1;
-    }
+  auto row_of = [&](int at, int row) { return at < hi && row < (int)p.T ? row : -1; };
+  auto look_ahead = [&](int slot) {   // a ring less one ahead
+    const int at = place + (kStages - 1) * step + threadIdx.x;
+    if (threadIdx.x < O::kSteps) copy_async<4>(shared(&order[slot][threadIdx.x]), p.order + at, at < hi);
   };
   const uint32_t ring = shared(smem);
-  auto load = [&](int stage) {   // the next step, whose rows have been looked up
+  auto load = [&](int stage, const int (&row)[2]) {   // the next step
     const uint32_t to = ring + stage * O::kStage;
+    look_ahead(stage == 0 ? kStages - 1 : stage - 1);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint32_t d = to + (xr + i * 16) * kXPitch + xc * 16;
@@ -708,13 +708,19 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) outer_kernel(const 
       }
     }
     place += step;
-    look();
   };
   float acc[MT][4][4] = {};
-  look();
+  int begin[kStages - 1][2];
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = first + s * step + xr + i * 16;
+      begin[s][i] = row_of(at, at < hi ? p.order[at] : -1);
+    }
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
-    if (s < n) load(s);
+    if (s < n) load(s, begin[s]);
     commit();
   }
   const int mr = lane & 7, mi = lane >> 3;
@@ -724,7 +730,10 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) outer_kernel(const 
   for (int k = 0; k < n; ++k) {
     wait_all_but<kStages - 2>();
     __syncthreads();   // the step is there, and everyone has read the stage that is filled now
-    if (k + kStages - 1 < n) load(to);
+    if (k + kStages - 1 < n) {
+      const int row[2] = {row_of(place + xr, order[to][xr]), row_of(place + xr + 16, order[to][xr + 16])};
+      load(to, row);
+    }
     commit();
     const uint32_t src = ring + from * O::kStage;
     uint32_t bh[4][2], bl[4][2];
