@@ -36,15 +36,20 @@ int fail(int code, const char* fmt, ...) {
 void count_launch(int n) { g_launches += (uint64_t)n; }
 
 int allow_smem(const void* kernel, size_t bytes) {
-  struct Known { const void* kernel; int device; size_t bytes; };
+  struct Known { const void* kernel; int device; };
   static thread_local Known known[64] = {};
   if (bytes <= 40 * 1024) return B200Q_OK;   // (48 KB with what kernels have besides)
   int device = 0;
   B200Q_CUDA_OK(cudaGetDevice(&device));
   Known& k = known[(reinterpret_cast<uintptr_t>(kernel) / 16 * 31 + device) % 64];
-  if (k.kernel == kernel && k.device == device && k.bytes >= bytes) return B200Q_OK;
-  B200Q_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  k = Known{kernel, device, bytes};
+  if (k.kernel == kernel && k.device == device) return B200Q_OK;
+  // The limit belongs to the kernel, for all host threads: every one asks for the same, the most that there is, so that none takes from another what it relies on.
+  int most = 0;
+  cudaFuncAttributes a{};
+  B200Q_CUDA_OK(cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device));
+  B200Q_CUDA_OK(cudaFuncGetAttributes(&a, kernel));
+  B200Q_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)a.sharedSizeBytes));
+  k = Known{kernel, device};
   return B200Q_OK;
 }
 

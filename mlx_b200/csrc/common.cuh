@@ -18,7 +18,7 @@ namespace b200q {
 // Records a formatted message in the calling thread's error slot and returns `code`.
 int fail(int code, const char* fmt, ...);
 void count_launch(int n = 1);
-// Lets `kernel` have `bytes` of dynamic shared memory; asks the runtime once per thread, device and kernel (a call costs 1 us).
+// Lets `kernel` have `bytes` of dynamic shared memory (and all that there is, for every host thread); asks the runtime once per thread, device and kernel (a call costs 1 us).
 int allow_smem(const void* kernel, size_t bytes);
 // Makes the device's context current for the calling thread; to be called before cuTensorMapEncodeTiled.
 int bind_context();
