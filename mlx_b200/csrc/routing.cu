@@ -315,21 +315,29 @@ __device__ __forceinline__ void route_token(const RouteParams& p, const T* logit
       if (sums) b = max(max(b, __shfl_xor_sync(kFull, b, o)), min(rank, c));
       rank = max(rank, c);
     }
-    if (sums && b != 0) rank = code32(value32(rank) + value32(b));
+    float size_of = fabsf(value32(rank));   // the larger of the two, whose rounding the sum has, however small it is itself
+    if (sums && b != 0) {
+      size_of = fmaxf(size_of, fabsf(value32(b)));
+      rank = code32(value32(rank) + value32(b));
+    }
     if (lane < 32) few[lane] = 0;
     __syncwarp();
-    if (group < p.groups) few[group] = rank;
+    if (group < p.groups) {
+      few[group] = rank;
+      few[32 + group] = __float_as_uint(size_of);
+    }
     __syncwarp();
     // lane g looks after group g
     rank = few[lane];
     const int before = place_among(few, p.groups, rank, lane);
     const uint32_t on = __ballot_sync(kFull, rank != 0 && before < p.top_groups);
-    if (scores) {
-      const uint32_t last = __ballot_sync(kFull, rank != 0 && before == p.top_groups - 1), next = __ballot_sync(kFull, rank != 0 && before == p.top_groups);
-      if (last && next) {
-        const float a = value32(__shfl_sync(kFull, rank, __ffs(last) - 1)), c = value32(__shfl_sync(kFull, rank, __ffs(next) - 1));
-        unsure_group = a - c <= 2 * room + 0x1p-21f * fmaxf(fabsf(a), fabsf(c));
-      }
+    if (scores && __popc(on) == p.top_groups) {
+      // Where the ranks lie, with their errors, of those that stay and of those that do not: off by `room` and 2^-22 of the larger key (two keys' half units and
+      // their sum's, rounded up).  (An infinite sum of finite keys is no answer: its bounds are infinite, too.)
+      const float off = rank != 0 ? room + 0x1.2p-22f * __uint_as_float(few[32 + lane]) : 0.0f, r = value32(rank);
+      const uint32_t least = __reduce_min_sync(kFull, on >> lane & 1 ? code32(r - off) : kFull);
+      const uint32_t most = __reduce_max_sync(kFull, rank != 0 && !(on >> lane & 1) ? code32(r + off) : 0);
+      unsure_group = least <= most;
     }
     __syncwarp();
     const uint32_t inv = ((1u << 20) + size - 1) / size;   // i / size for i < 1024
