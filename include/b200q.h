@@ -471,11 +471,11 @@ int b200q_group_rows(const void* ids, int id_bytes, int64_t T, int64_t n, int32_
 
 /*
  * Low-rank adapters beside a shared projection: out[t] = y[t] + scales[l] b[l] (a[l] x[t]), l being row t's adapter; a row without one:
- * y[t].  bf16 and f16; sums in fp32, the inner product to 2^-17, the result rounded once.  Inner products and f16 weights are multiplied as two
- * parts each: where one of them is infinite, so that the sum would be, it may be a NaN.
+ * y[t].  bf16 and f16; sums and inner products in fp32, the result rounded once.  Inner products are multiplied as three parts each and 16-bit numbers of f16 as
+ * two: where what a finite inner product is multiplied with is infinite (b, in the gradients a, x or dy), so that the sum would be, it may be a NaN.
  *   y, out [T, N] (out may be y), x [T, K], a [L, r, K], b [L, N, r] dtype; scales [L] float32 (NULL: 1)
  *   order, starts, tiles: b200q_group_rows over L groups
- *   h: b200q_add_adapters_inner_bytes(T, r) bytes on a 16-byte boundary, left with a[l] x, by place, as two bf16 numbers per value,
+ *   h: b200q_add_adapters_inner_bytes(T, r) bytes on a 16-byte boundary, left with a[l] x, by place, as three bf16 numbers per value,
  *   which the gradient takes (else scratch); rows without an adapter have none
  * b200q_add_adapters_grad: from dy [T, N] the gradients dx [T, K], da, db, each NULL where not wanted (that of y is dy); g, as
  * large as h, is scratch, needed for dx and da.  h is needed for db, x for da, a for dx, b for dx and da.

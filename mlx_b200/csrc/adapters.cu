@@ -9,9 +9,9 @@
 // nothing is written but h and the results.  The products are mma.sync (545 TFLOP/s measured here): tiles of a few rows whose number only the
 // device knows, operands that come in pieces from gathered rows and are split into two parts on the way; at rank 64 they take about as long as HBM does.
 //
-// h and g, summed in fp32, are kept as two bf16 numbers each, high and low part (2^-17 of the value is lost, a 32nd of what the
-// result's rounding to f16 loses), since that is how the second products take them; 16-bit floats of type f16 are split too, exactly, so that
-// no value leaves a type's range (the product of two low parts, 2^-17, is left out).
+// h and g, summed in fp32, are kept as three bf16 numbers each that add up to them exactly, since that is how the second products take them: fp32's 24 bits are 8
+// and two times 8 more with signs.  16-bit floats of type f16 are split too, in two, exactly, so that no value leaves a type's range; of those six products
+// the smallest, below 2^-24 of the whole, is left out.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -46,14 +46,20 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {   // two bf16, th
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// The high part's rounding is away from infinity where the nearest bf16 would be one; what is not finite has no low part.
-__device__ __forceinline__ void split(float a, float b, uint32_t* hi, uint32_t* lo) {
-  __nv_bfloat16 ha = __float2bfloat16_rn(a), hb = __float2bfloat16_rn(b);
-  if (isinf(__bfloat162float(ha))) ha = __float2bfloat16_rz(a);
-  if (isinf(__bfloat162float(hb))) hb = __float2bfloat16_rz(b);
-  const float fa = __bfloat162float(ha), fb = __bfloat162float(hb);
-  *hi = pack(fa, fb);
-  *lo = pack(isinf(fa) ? 0.0f : a - fa, isinf(fb) ? 0.0f : b - fb);
+// The nearest bf16; toward zero where that would be infinite.
+__device__ __forceinline__ float near_bf16(float a) {
+  const float f = __bfloat162float(__float2bfloat16_rn(a));
+  return isinf(f) ? __bfloat162float(__float2bfloat16_rz(a)) : f;
+}
+// Two numbers as three bf16 each, exactly.  An infinity is the last one's, and the others have its sign: whatever finite numbers these are multiplied with, of two parts
+// of which the second may be zero, the sum is the infinity that it has to be.
+__device__ __forceinline__ void split(float a, float b, uint32_t (&part)[3]) {
+  const bool ia = isinf(a), ib = isinf(b);
+  const float ha = near_bf16(a), hb = near_bf16(b), ra = a - ha, rb = b - hb;
+  const float ma = ia ? copysignf(1.0f, a) : near_bf16(ra), mb = ib ? copysignf(1.0f, b) : near_bf16(rb);
+  part[0] = pack(ia ? ma : ha, ib ? mb : hb);
+  part[1] = pack(ma, mb);
+  part[2] = pack(ia ? a : ra - ma, ib ? b : rb - mb);
 }
 // A pair of T as bf16 numbers: itself, or (f16) high and low part: the upper 8 bits of the 11, and the rest, exactly (0 of what is not finite).
 template <typename T>
@@ -201,7 +207,7 @@ __device__ __forceinline__ uint4 add8(const uint4& a, float c, const float (&b)[
 
 struct Params {
   const void *x, *w;       // activations; weights of all adapters
-  uint16_t* h;             // inner products, by place: [T][r16 / 16][4][high, low][4] bf16
+  uint16_t* h;             // inner products, by place: [T][r16 / 16][3 parts][16] bf16; of 16 ranks 0 1 4 5 8 9 12 13 2 3 6 7 10 11 14 15, as the operands want them
   const void* y;           // up: what is added to (null: zeros)
   void* out;
   const float* scales;     // null: 1
@@ -405,11 +411,11 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) down_kernel(const P
     }
     const int row = i % (eights * 8), rank = r0 + i / (eights * 8) * 2;
     if (rank < p.r16 && row < tile.z) {
-      uint32_t hi, lo;
-      split(rank < p.r ? c * s[0] : 0.0f, rank + 1 < p.r ? c * s[1] : 0.0f, &hi, &lo);
-      uint16_t* h = p.h + (int64_t)(tile.y + row) * 2 * p.r16 + rank / 4 * 8 + rank % 4;
-      *reinterpret_cast<uint32_t*>(h) = hi;
-      *reinterpret_cast<uint32_t*>(h + 4) = lo;
+      uint32_t parts[3];
+      split(rank < p.r ? c * s[0] : 0.0f, rank + 1 < p.r ? c * s[1] : 0.0f, parts);
+      uint16_t* h = p.h + (int64_t)(tile.y + row) * 3 * p.r16 + rank / 16 * 48 + rank % 16 / 4 * 2 + (rank & 2) * 4;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) *reinterpret_cast<uint32_t*>(h + 16 * i) = parts[i];
     }
   }
   if (p.split > 1) cluster.sync();   // no block leaves while others read its sums
@@ -429,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) down_kernel(const P
 constexpr int kUpStages = 4, kUpTiles = 16, kUpSteps = kUpTiles * kRows / 16;
 template <int KS, bool CHUNKED>
 struct Up {
-  static constexpr int kStep = KS * 1024;   // bytes of h per step of 16 rows: [rank step][part][lane][4]
+  static constexpr int kStep = KS * 1536;   // bytes of h per step of 16 rows: [rank step][part][row][two pieces of 16, swapped in every other four rows]
   static constexpr size_t kBytes = (size_t)kWarps * kUpStages * 1024 + 8 * kStep;
 };
 template <typename T, bool WIDE, bool WHOLE, int KS, bool CHUNKED>
@@ -467,27 +473,20 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
       steps += (t.z + 15) / 16;
     }
     const uint32_t ring = shared(smem) + warp * kUpStages * 1024 + lane * 16, hs = shared(smem) + kWarps * kUpStages * 1024;
+    const uint32_t h_row = hs + (lane & 15) * 32 + ((lane >> 4 ^ lane >> 2) & 1) * 16;   // that the lane names: of two times eight rows by two times eight ranks
     auto next_tile = [&](int k) {
       while (k < count && tiles[k].z == 0) ++k;
       return k;
     };
     auto copy_h = [&](int k, int r0, int buffer) {
       if (k >= count || tiles[k].x < 0) return;
-      constexpr int kPer = 4 * KS, kSweep = kThreads / kPer;   // pieces of 16 bytes per row; rows that the block copies at once
-      const int piece = threadIdx.x % kPer, row = threadIdx.x / kPer, z = tiles[k].z;
-      if (r0 + piece * 4 >= p.r16) return;
-      const uint16_t* src = p.h + (int64_t)(tiles[k].y + row) * 2 * p.r16 + r0 * 2 + piece * 8;
-      const uint32_t to = hs + buffer * 4 * kStep + piece / 4 * 1024 + piece % 4 * 16;
-#pragma unroll
-      for (int i = 0; i < kRows / kSweep; ++i) {
-        const int at = row + i * kSweep;
-        if (at >= z) break;
-        const uint32_t d = to + at / 16 * kStep + at % 8 * 64 + at / 8 % 2 * 4;
-        copy_async<4>(d, src, true);             // high part, first pair of ranks
-        copy_async<4>(d + 8, src + 2, true);     // second pair
-        copy_async<4>(d + 512, src + 4, true);   // low part
-        copy_async<4>(d + 520, src + 6, true);
-        src += (int64_t)kSweep * 2 * p.r16;
+      constexpr int kPer = 6 * KS;   // pieces of 16 bytes per row
+      const int z = tiles[k].z;
+      const uint16_t* src = p.h + (int64_t)tiles[k].y * 3 * p.r16 + r0 * 3;
+      for (int i = threadIdx.x; i < z * kPer; i += kThreads) {
+        const int row = i / kPer, piece = i % kPer;
+        if (KS == 1 || r0 + piece / 6 * 16 < p.r16)
+          copy_async<16>(hs + buffer * 4 * kStep + row / 16 * kStep + piece / 2 * 512 + row % 16 * 32 + ((piece ^ row >> 2) & 1) * 16, src + row * 3 * p.r16 + piece * 8, true);
       }
     };
     const T* w = nullptr;
@@ -581,14 +580,18 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
         }
         ++now;
       };
-      auto step = [&](float (&acc)[4][4], int s, const uint4& hi, const uint4& lo) {
+      auto step = [&](float (&acc)[4][4], int s, uint32_t src) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], hi.x, hi.y, hi.z, hi.w, bh[s][t][0], bh[s][t][1]);
+        for (int i = 0; i < 3; ++i) {
+          const uint4 a = load_matrices<false>(src + i * 512);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], lo.x, lo.y, lo.z, lo.w, bh[s][t][0], bh[s][t][1]);
-        if constexpr (kSplitW) {
+          for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], a.x, a.y, a.z, a.w, bh[s][t][0], bh[s][t][1]);
+          if constexpr (kSplitW) {
+            if (i < 2) {
 #pragma unroll
-          for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], hi.x, hi.y, hi.z, hi.w, bl[s][t][0], bl[s][t][1]);
+              for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], a.x, a.y, a.z, a.w, bl[s][t][0], bl[s][t][1]);
+            }
+          }
         }
       };
       // (rows behind the tile's last one have what was there before; their products are not stored)
@@ -604,13 +607,13 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
           commit();
           if (plain) continue;
           weights(r0);
-          const uint32_t src = hs + buffer * 4 * kStep + lane * 16;
+          const uint32_t src = h_row + buffer * 4 * kStep;
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
             if (r0 + s * 16 >= p.r16) break;
 #pragma unroll
             for (int m = 0; m < kRows / 16; ++m)
-              if (m < last) step(acc[m], s, load16(src + m * kStep + s * 1024), load16(src + m * kStep + s * 1024 + 512));
+              if (m < last) step(acc[m], s, src + m * kStep + s * 1536);
           }
         }
 #pragma unroll
@@ -624,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
         if (now == 0 || before < 4) wait_all_but<0>();
         __syncthreads();
         copy_h(after, 0, buffer ^ 1);
-        uint32_t src = hs + buffer * 4 * kStep + lane * 16;
+        uint32_t src = h_row + buffer * 4 * kStep;
         for (int m = 0; m < last; ++m, src += kStep) {
           issue();
           float acc[4][4] = {};
@@ -632,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
               if (KS > 1 && s * 16 >= p.r16) break;
-              step(acc, s, load16(src + s * 1024), load16(src + s * 1024 + 512));
+              step(acc, s, src + s * 1536);
             }
           }
           finish(acc);
@@ -649,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
 // ---- out_l = (c) sum over l's rows of h[place] x[row]^T.  Blocks by (128 columns, part of the rows; adapter; 16 MT ranks), the parts are a
 // cluster; warps by (32 columns, half of a step's 32 rows).  TALL: out [C, r], else [r, C].
 //
-// Rows lie in shared memory as they come, and matrix loads that transpose make both operands of them; h's two parts lie apart there.  Which rows come next is
+// Rows lie in shared memory as they come, and matrix loads that transpose make both operands of them; h's parts lie apart there.  Which rows come next is
 // copied there, too, a ring ahead, so that no step waits for it.  (4096 rows of one adapter of rank 64 and 4096 columns: 27 us, 90 when every 32 columns' h was
 // transposed in registers; HBM 5.  2048 rows of 4 adapters of rank 16, [14336, 4096], forward and all gradients: 98 us, 106 with three stages and rows looked up
 // one step ahead; 1000 adapters of a row each have no use for it: 229 and 215.)  Bound by latencies: a block has few steps, and reads where its rows are before it
@@ -658,12 +661,12 @@ template <bool TALL, int MT>
 struct Outer {
   static constexpr int kRanks = 16 * MT, kCols = 128, kSteps = 32, kStages = MT == 1 ? 5 : 4;
   static constexpr int kXPitch = kCols * 2 + 16, kHPitch = kRanks * 2 + 16;   // (eight rows of a matrix are in different banks)
-  static constexpr int kStage = kSteps * (kXPitch + 2 * kHPitch);
+  static constexpr int kStage = kSteps * (kXPitch + 3 * kHPitch);
   static constexpr int kLine = kCols + (TALL ? 2 : 8);   // floats per rank of the sums
   static constexpr size_t kRing = (size_t)kStages * kStage, kSums = (size_t)2 * kRanks * kLine * 4, kBytes = kRing > kSums ? kRing : kSums;
 };
 template <typename T, bool TALL, bool WHOLE, int MT>
-__global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) outer_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 2) outer_kernel(const Params p) {
   using O = Outer<TALL, MT>;
   constexpr int kRanks = O::kRanks, kCols = O::kCols, kLine = O::kLine, kStages = O::kStages, kXPitch = O::kXPitch, kHPitch = O::kHPitch;
   constexpr bool kSplitX = std::is_same_v<T, __half>;
@@ -673,11 +676,10 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) outer_kernel(const 
   const int part = (int)(blockIdx.x % p.split), l = blockIdx.y, r0 = blockIdx.z * kRanks, c0 = (int)(blockIdx.x / p.split) * kCols;
   const int lo = max(p.starts[l], 0), hi = min(p.starts[l + 1], (int)p.T), step = p.split * O::kSteps, first = lo + part * O::kSteps;
   const int n = first < hi ? (hi - first + step - 1) / step : 0;
-  // Copied per step by a thread: 8 columns of two rows of x; of h, pieces of 4 ranks' two parts.
-  constexpr int kPer = 4 * MT, kHRows = kThreads / kPer, kH = O::kSteps > kHRows ? O::kSteps / kHRows : 1;   // pieces per row; rows at once; rows of a thread
-  const int xr = threadIdx.x / 16, xc = threadIdx.x % 16, hr = threadIdx.x / kPer, hc = threadIdx.x % kPer, have = C - c0 - xc * 8;
+  // Copied per step by a thread: 8 columns of two rows of x; of h, pieces of 8 ranks of a part.
+  constexpr int kPer = 6 * MT;   // pieces per row
+  const int xr = threadIdx.x / 16, xc = threadIdx.x % 16, have = C - c0 - xc * 8;
   const T* x = static_cast<const T*>(p.x) + c0 + xc * 8;
-  const bool ranks = hr < O::kSteps && r0 + hc * 4 < p.r16;
   __shared__ int order[kStages][O::kSteps];   // of the steps that are loaded next: copied a ring ahead of their rows
   int place = first;   // of the step that is loaded
   auto row_of = [&](int at, int row) { return at < hi && row < (int)p.T ? row : -1; };
@@ -696,16 +698,12 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) outer_kernel(const 
       if constexpr (WHOLE) copy_async<16>(d, src, row[i] >= 0 && have > 0);
       else store16(d, row[i] >= 0 ? load8<false>(src, have) : make_uint4(0, 0, 0, 0));
     }
-    if (hr < O::kSteps) {
 #pragma unroll
-      for (int i = 0; i < kH; ++i) {
-        const int at = hr + i * kHRows;
-        const uint32_t d = to + O::kSteps * kXPitch + at * kHPitch + hc * 8;
-        const uint16_t* src = p.h + (int64_t)(place + at) * 2 * p.r16 + r0 * 2 + hc * 8;
-        const bool there = ranks && place + at < hi;
-        copy_async<8>(d, src, there);
-        copy_async<8>(d + O::kSteps * kHPitch, src + 4, there);
-      }
+    for (int i = 0; i < (O::kSteps * kPer + kThreads - 1) / kThreads; ++i) {
+      const int id = threadIdx.x + i * kThreads, at = id / kPer, piece = id % kPer;
+      if (O::kSteps * kPer % kThreads != 0 && at >= O::kSteps) break;
+      copy_async<16>(to + O::kSteps * (kXPitch + piece / 2 % 3 * kHPitch) + at * kHPitch + piece / 6 * 32 + piece % 2 * 16,
+                     p.h + (int64_t)(place + at) * 3 * p.r16 + r0 * 3 + piece * 8, place + at < hi && r0 + piece / 6 * 16 < p.r16);
     }
     place += step;
   };
@@ -748,14 +746,17 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) outer_kernel(const 
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       if (MT > 1 && r0 + m * 16 >= p.r16) break;
-      const uint4 a = load_matrices<true>(src + h_at + m * 32), b = load_matrices<true>(src + h_at + m * 32 + O::kSteps * kHPitch);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a.x, a.y, a.z, a.w, bh[v][0], bh[v][1]);
+      for (int i = 0; i < 3; ++i) {
+        const uint4 a = load_matrices<true>(src + h_at + m * 32 + i * O::kSteps * kHPitch);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], b.x, b.y, b.z, b.w, bh[v][0], bh[v][1]);
-      if constexpr (kSplitX) {
+        for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a.x, a.y, a.z, a.w, bh[v][0], bh[v][1]);
+        if constexpr (kSplitX) {
+          if (i < 2) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a.x, a.y, a.z, a.w, bl[v][0], bl[v][1]);
+            for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a.x, a.y, a.z, a.w, bl[v][0], bl[v][1]);
+          }
+        }
       }
     }
     to = from;
@@ -770,7 +771,8 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) outer_kernel(const 
     for (int v = 0; v < 4; ++v)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<float2*>(&red[(slot * kRanks + m * 16 + i * 8 + g) * kLine + (warp & 3) * 32 + v * 8 + q * 2]) = make_float2(acc[m][v][2 * i], acc[m][v][2 * i + 1]);
+        *reinterpret_cast<float2*>(&red[(slot * kRanks + m * 16 + (g >> 1) * 4 + i * 2 + (g & 1)) * kLine + (warp & 3) * 32 + v * 8 + q * 2]) =
+            make_float2(acc[m][v][2 * i], acc[m][v][2 * i + 1]);   // (ranks back in their order)
   __syncthreads();
   if (p.split > 1) {
     for (int i = threadIdx.x; i < kRanks * kCols; i += kThreads) {
@@ -965,7 +967,7 @@ int check(const char* tag, int dtype, int64_t T, int64_t L, int64_t N, int64_t K
 
 using namespace b200q;
 
-extern "C" size_t b200q_add_adapters_inner_bytes(int64_t T, int64_t r) { return T <= 0 || r <= 0 ? 0 : (size_t)T * ((r + 15) / 16 * 16) * 4; }
+extern "C" size_t b200q_add_adapters_inner_bytes(int64_t T, int64_t r) { return T <= 0 || r <= 0 ? 0 : (size_t)T * ((r + 15) / 16 * 16) * 6; }
 
 extern "C" int b200q_add_adapters(const void* y, const void* x, const void* a, const void* b, int dtype, int64_t T, int64_t L, int64_t N, int64_t K,
                                   int64_t r, const int32_t* order, const int32_t* tiles, const float* scales, void* h, void* out, void* stream) {

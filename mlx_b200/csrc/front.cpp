@@ -938,7 +938,7 @@ bool adapters_run(Adapters* p, Tensor* out, Tensor* h) {
   if (!adapters_ok(p, *p->y)) return false;
   const at::Device dev = p->x->device();
   if (!out->defined()) *out = fresh(p->y->sizes(), p->y->scalar_type(), dev);
-  *h = fresh({p->T, 2, (p->r + 15) / 16 * 16}, at::kBFloat16, dev);
+  *h = fresh({p->T, 3, (p->r + 15) / 16 * 16}, at::kBFloat16, dev);
   return b200q_add_adapters(p->y->data_ptr(), p->x->data_ptr(), p->a->data_ptr(), p->b->data_ptr(), dtype_code(p->x->scalar_type()), p->T, p->L, p->N, p->K, p->r,
                             ints(*p->g[2]), ints(*p->g[3]), floats(p->scales), h->data_ptr(), out->data_ptr(), stream_of(dev)) == B200Q_OK;
 }

@@ -1046,20 +1046,20 @@ def _adapter_args(tag, y, x, a, b, groups, scales):
 
 
 def _inner(T: int, rank: int) -> Tuple[int, int, int]:
-    return T, 2, (rank + 15) // 16 * 16
+    return T, 3, (rank + 15) // 16 * 16
 
 
 def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, groups: RowGroups, scales: Optional[torch.Tensor] = None,
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Low-rank adapters of many requests at once beside a shared projection: y [..., N], what the projection (quantized_matmul, qqmm, ...)
     made of x [..., K], plus scales[l] b[l] (a[l] x[t]) for every row t with an adapter l.  a [adapters, rank, K], b [adapters, N, rank],
-    scales [adapters] (None: 1); groups: group_rows of the rows' adapters.  bfloat16 and float16; sums in float32, the
-    inner product to 2^-17, the result rounded once.  out: where the sum goes, y itself for a sum in place.  grad.add_adapters is the same with gradients."""
+    scales [adapters] (None: 1); groups: group_rows of the rows' adapters.  bfloat16 and float16; sums and inner products in
+    float32, the result rounded once.  out: where the sum goes, y itself for a sum in place.  grad.add_adapters is the same with gradients."""
     return _add_adapters(y, x, a, b, groups, scales, out)[0]
 
 
 def _add_adapters(y, x, a, b, groups, scales=None, out=None):
-    """-> add_adapters' result and the inner products, two bfloat16 parts per value [rows, 2, rank in whole 16s] in the order of the groups."""
+    """-> add_adapters' result and the inner products, three bfloat16 parts per value [rows, 3, rank in whole 16s] in the order of the groups."""
     r = _front.add_adapters(y, x, a, b, groups, scales, out)
     if r is not None:
         return r
