@@ -959,9 +959,9 @@ PyObject* py_add_adapters(PyObject*, PyObject* const* a, Py_ssize_t n) {   // (.
     if (out.requires_grad() && at::GradMode::is_enabled()) return none();
     for (const Tensor* v : {p.x, p.a, p.b})
       if (overlap(out, *v)) return none();
-    out.unsafeGetTensorImpl()->bump_version();   // whoever has kept it for a gradient hears of it
   }
   if (!adapters_run(&p, &out, &h)) return none();
+  if (a[6] != Py_None && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();   // whoever has kept it for a gradient hears of it
   PyObject* pair = PyTuple_New(2);
   if (!pair) return nullptr;
   if (a[6] != Py_None) { Py_INCREF(a[6]); PyTuple_SET_ITEM(pair, 0, a[6]); }

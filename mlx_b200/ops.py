@@ -1072,7 +1072,7 @@ def _add_adapters(y, x, a, b, groups, scales=None, out=None):
             raise ValueError(f"[{tag}] out must not be part of a graph.")
         if any(_overlap(out, t) for t in (x, a, b)) or (_overlap(out, y) and (out.data_ptr() != y.data_ptr() or not y.is_contiguous())):
             raise ValueError(f"[{tag}] out must be y itself or not overlap the operands.")
-        torch.autograd.graph.increment_version(out)   # whoever has kept it for a gradient hears of it
+    into = out
     y, x, a, b = (t.detach().contiguous() for t in (y, x, a, b))
     with torch.cuda.device(dev):
         out = torch.empty_like(y) if out is None else out
@@ -1080,6 +1080,8 @@ def _add_adapters(y, x, a, b, groups, scales=None, out=None):
         rc = _lib.load().b200q_add_adapters(_ptr(y), _ptr(x), _ptr(a), _ptr(b), _DT[x.dtype], T, L, N, K, rank, _ptr(groups.order), _ptr(groups.tiles),
                                             _ptr(scales), _ptr(h), _ptr(out), _stream(x))
     _lib.check(rc)
+    if into is not None:
+        torch.autograd.graph.increment_version(into)   # whoever has kept it for a gradient hears of it
     return out, h
 
 
