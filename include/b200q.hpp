@@ -455,7 +455,7 @@ inline void add_adapters(const ArrayView& y, const ArrayView& x, const ArrayView
                                    detail::f32(scales), detail::inner("add_adapters", h, d), out.data, stream));
 }
 
-// Gradients of add_adapters (that of y is dy); dx, da and db may be empty views: not wanted.  g: scratch as large as h
+// Gradients of add_adapters (that of y is dy); dx, da and db may be empty views: not wanted.  h: what add_adapters left, for db alone; g: scratch as large, for dx and da
 inline void add_adapters_grad(const ArrayView& dy, const ArrayView& x, const ArrayView& a, const ArrayView& b, const RowGroups& groups, const Workspace& h,
                               const Workspace& g, ArrayView& dx, ArrayView& da, ArrayView& db, const ArrayView& scales = {}, void* stream = nullptr) {
   const auto d = detail::adapters("add_adapters_grad", dy, x, a, b, groups, scales);
@@ -463,7 +463,7 @@ inline void add_adapters_grad(const ArrayView& dy, const ArrayView& x, const Arr
   if (da.data) detail::validate_result("add_adapters_grad", da, a.size(), x.dtype);
   if (db.data) detail::validate_result("add_adapters_grad", db, b.size(), x.dtype);
   detail::check(b200q_add_adapters_grad(dy.data, x.data, a.data, b.data, (int)x.dtype, d.T, d.L, d.N, d.K, d.r, detail::i32(groups.order), detail::i32(groups.starts),
-                                        detail::i32(groups.tiles), detail::f32(scales), detail::inner("add_adapters_grad", h, d),
+                                        detail::i32(groups.tiles), detail::f32(scales), db.data ? detail::inner("add_adapters_grad", h, d) : h.data,
                                         dx.data || da.data ? detail::inner("add_adapters_grad", g, d) : nullptr, dx.data, da.data, db.data, stream));
 }
 

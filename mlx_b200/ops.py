@@ -1085,20 +1085,22 @@ def _add_adapters(y, x, a, b, groups, scales=None, out=None):
     return out, h
 
 
-def add_adapters_grad(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, groups: RowGroups, h: torch.Tensor,
+def add_adapters_grad(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, groups: RowGroups, h: Optional[torch.Tensor] = None,
                       scales: Optional[torch.Tensor] = None, for_x: bool = True, for_a: bool = True, for_b: bool = True):
     """-> gradients of add_adapters with respect to x, a and b (None where not asked for; that of y is dy).  h: the inner products, as the
-    forward pass leaves them."""
+    forward pass leaves them for b's gradient; None: computed again where that is asked for."""
     tag = "add_adapters_grad"
     dev, T, L, N, K, rank, groups, scales = _adapter_args(tag, dy, x, a, b, groups, scales)
-    if h.dtype != torch.bfloat16 or tuple(h.shape) != _inner(T, rank):
+    if h is None and for_b:
+        h = _add_adapters(dy, x, a, b, groups, scales)[1]
+    if h is not None and (h.dtype != torch.bfloat16 or tuple(h.shape) != _inner(T, rank)):
         raise ValueError(f"[{tag}] h must be bfloat16 {_inner(T, rank)}.")
-    _require_cuda(tag, x, h)
+    _require_cuda(tag, x, *(() if h is None else (h,)))
     dy, x, a, b = (t.detach().contiguous() for t in (dy, x, a, b))
-    h = _aligned(h)
+    h = None if h is None else _aligned(h)
     with torch.cuda.device(dev):
         dx, da, db = (torch.empty_like(t) if wanted else None for t, wanted in ((x, for_x), (a, for_a), (b, for_b)))
-        g = torch.empty_like(h) if for_x or for_a else None
+        g = torch.empty(_inner(T, rank), dtype=torch.bfloat16, device=dev) if for_x or for_a else None
         rc = _lib.load().b200q_add_adapters_grad(_ptr(dy), _ptr(x), _ptr(a), _ptr(b), _DT[x.dtype], T, L, N, K, rank, _ptr(groups.order),
                                                  _ptr(groups.starts), _ptr(groups.tiles), _ptr(scales), _ptr(h), _ptr(g), _ptr(dx), _ptr(da), _ptr(db),
                                                  _stream(x))
