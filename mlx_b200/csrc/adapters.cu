@@ -93,31 +93,23 @@ __device__ __forceinline__ uint4 load8(const T* p, int64_t have) {
   }
   return v;
 }
-// N consecutive values (4 or 8) in the widest pieces that the rows' alignment allows (`width` bytes).
-template <int N, typename T>
-__device__ __forceinline__ void load_few(const T* p, int64_t have, int width, uint32_t (&w)[N / 2]) {
-#pragma unroll
-  for (int i = 0; i < N / 2; ++i) w[i] = 0;
-  if (N == 8 && width == 16) {
+// 4 consecutive values in the widest pieces that the rows' alignment allows (`width` bytes).
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, int64_t have, int width, uint32_t (&w)[2]) {
+  w[0] = w[1] = 0;
+  if (width >= 8) {
     if (have > 0) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-      w[0] = v.x; w[1] = v.y; w[N / 2 - 2] = v.z; w[N / 2 - 1] = v.w;
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = v.x; w[1] = v.y;
     }
-  } else if (width >= 8) {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i)
-      if (4 * i < have) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p) + i);
-        w[2 * i] = v.x; w[2 * i + 1] = v.y;
-      }
   } else if (width == 4) {
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i)
+    for (int i = 0; i < 2; ++i)
       if (2 * i < have) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
   } else {
     const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < 4; ++i)
       if (i < have) w[i / 2] |= (uint32_t)__ldg(q + i) << (16 * (i & 1));
   }
 }
@@ -134,24 +126,23 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* p, bool the
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void wait_all_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-// N consecutive values (4, 8 or 16) in the widest pieces that the rows' alignment allows, to shared memory; pieces of 16 bytes are 512 apart.
-template <int N, typename T>
-__device__ __forceinline__ void copy_few(uint32_t dst, const T* p, int have, int width) {
+// 8 consecutive values in the widest pieces that the rows' alignment allows, to shared memory.
+template <typename T>
+__device__ __forceinline__ void copy8(uint32_t dst, const T* p, int have, int width) {
   const char* q = reinterpret_cast<const char*>(p);
-  if (N >= 8 && width == 16) {
+  if (width == 16) {
+    copy_async<16>(dst, q, have > 0);
+  } else if (width == 8) {
 #pragma unroll
-    for (int i = 0; i < N / 8; ++i) copy_async<16>(dst + 512 * i, q + 16 * i, 8 * i < have);
-  } else if (width >= 8) {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) copy_async<8>(dst + 512 * (i / 2) + 8 * (i & 1), q + 8 * i, 4 * i < have);
+    for (int i = 0; i < 2; ++i) copy_async<8>(dst + 8 * i, q + 8 * i, 4 * i < have);
   } else if (width == 4) {
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) copy_async<4>(dst + 512 * (i / 4) + 4 * (i & 3), q + 4 * i, 2 * i < have);
+    for (int i = 0; i < 4; ++i) copy_async<4>(dst + 4 * i, q + 4 * i, 2 * i < have);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const uint16_t v = i < have ? __ldg(reinterpret_cast<const uint16_t*>(p) + i) : (uint16_t)0;
-      asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + 512 * (i / 8) + 2 * (i & 7)), "h"(v) : "memory");
+      asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + 2 * i), "h"(v) : "memory");
     }
   }
 }
@@ -313,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) down_kernel(const P
 #pragma unroll
       for (int i = 0; i < 2 * MT; ++i) {
         const int row = (i * 32 + lane) / (2 * MT), c = lane % (2 * MT), rank = r0 + c * 8;
-        copy_few<8>(to + 4096 + (row * 2 * MT + (c ^ tall(row))) * 16, w + (int64_t)(kw + row) * p.r + rank, kw + row < C ? p.r - rank : 0, p.width);
+        copy8(to + 4096 + (row * 2 * MT + (c ^ tall(row))) * 16, w + (int64_t)(kw + row) * p.r + rank, kw + row < C ? p.r - rank : 0, p.width);
       }
       kw += step;
     } else {
@@ -505,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
             const int col = n0 + (g >> 1) * 8 + t * 2 + (g & 1), rank = r0 + s * 16 + q * 4;
-            load_few<4>(w + (int64_t)col * p.r + rank, col < C ? p.r - rank : 0, p.width, b[s][t]);
+            load4(w + (int64_t)col * p.r + rank, col < C ? p.r - rank : 0, p.width, b[s][t]);
           }
         }
       }
