@@ -972,8 +972,7 @@ extern "C" int b200q_add_adapters(const void* y, const void* x, const void* a, c
     return B200Q_OK;
   }
   if (!x || !a || !b || !order || !tiles || !h) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
-  for (const void* q : {y, x, a, b, static_cast<const void*>(out)})
-    if (!aligned(q, 2)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
+  if (!on_boundaries({y, x, a, b, out}, 2) || !on_boundaries({order, scales}, 4)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
   if (!aligned(tiles, 16) || !aligned(h, 16)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] tiles and h must be 16-byte aligned", tag);
   Params p{};
   p.split = 1;
@@ -1000,8 +999,7 @@ extern "C" int b200q_add_adapters_grad(const void* dy, const void* x, const void
   }
   if (!dy || !order || !starts || !tiles || (dx && !a) || ((dx || da) && (!b || !g)) || (da && !x) || (db && !h))
     return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
-  for (const void* q : {dy, x, a, b, static_cast<const void*>(dx), static_cast<const void*>(da), static_cast<const void*>(db)})
-    if (!aligned(q, 2)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
+  if (!on_boundaries({dy, x, a, b, dx, da, db}, 2) || !on_boundaries({order, starts, scales}, 4)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
   if (!aligned(tiles, 16) || !aligned(h, 16) || !aligned(g, 16)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] tiles, h and g must be 16-byte aligned", tag);
   Params p{};
   p.split = 1;

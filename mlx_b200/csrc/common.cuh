@@ -8,6 +8,7 @@
 
 #include <cstdarg>
 #include <cstdint>
+#include <initializer_list>
 #include <cstdio>
 
 #include "../../include/b200q.h"
@@ -42,6 +43,12 @@ int bind_context();
 inline bool valid_group(int g) { return g == 32 || g == 64 || g == 128; }
 inline bool valid_bits(int b) { return b >= 2 && b <= 8 && b != 7; }
 inline size_t dtype_size(int dt) { return dt == B200Q_F32 ? 4 : 2; }
+// Whether all of these (null: none) are on boundaries of `bytes`.
+inline bool on_boundaries(std::initializer_list<const void*> pointers, size_t bytes) {
+  for (const void* p : pointers)
+    if (reinterpret_cast<uintptr_t>(p) % bytes != 0) return false;
+  return true;
+}
 
 // Workspace layout shared by the matmul kernels.  The trailing 16 bytes hold the
 // device status word (4 x uint32); counters and partial sums come first.

@@ -889,6 +889,8 @@ extern "C" int b200q_route(const void* logits, int dtype, int64_t T, int64_t E, 
   if (groups > kMostGroups) return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than %lld groups.", tag, (long long)kMostGroups);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!sizes) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
+  if (!on_boundaries({logits}, dtype_size(dtype)) || !on_boundaries({bias, weights, experts, sizes, places, order}, 4))
+    return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
   if (T == 0) {
     B200Q_CUDA_OK(cudaMemsetAsync(sizes, 0, (size_t)E * 4, st));
     return B200Q_OK;
@@ -918,6 +920,7 @@ extern "C" int b200q_route_dlogits(const float* dw, const void* logits, int dtyp
   if (int rc = check_route(tag, dtype, T, E, top, scoring)) return rc;
   if (T == 0) return B200Q_OK;
   if (!dw || !logits || !experts || !dlogits) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
+  if (!on_boundaries({logits, dlogits}, dtype_size(dtype)) || !on_boundaries({dw, experts}, 4)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
   const DlogitsParams p{dw, logits, experts, dlogits, T, (int)E, (int)top, scoring == B200Q_SIGMOID, renormalize != 0, scale};
   const unsigned blocks = (unsigned)((T + 7) / 8);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -951,6 +954,7 @@ extern "C" int b200q_group_rows(const void* ids, int id_bytes, int64_t T, int64_
   if (T > (1 << 30) || n > kMostRowGroups)
     return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than 2^30 rows or %lld groups.", tag, (long long)kMostRowGroups);
   if (!starts || (n > 0 && !sizes)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
+  if (!on_boundaries({sizes, starts, order}, 4)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (T == 0) {
     if (n > 0) B200Q_CUDA_OK(cudaMemsetAsync(sizes, 0, (size_t)n * 4, st));

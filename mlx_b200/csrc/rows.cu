@@ -311,7 +311,6 @@ int check(const char* tag, int dtype, int64_t T, int64_t top, int64_t D) {
     return fail(B200Q_ERR_UNSUPPORTED, "[%s] No implementation for problem shape: more than 2^31 - 1 rows or elements in one.", tag);
   return B200Q_OK;
 }
-bool aligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % dtype_size(dtype) == 0; }
 
 }  // namespace
 }  // namespace b200q
@@ -324,7 +323,7 @@ extern "C" int b200q_dispatch_rows(const void* x, int dtype, int64_t T, int64_t 
   if (int rc = check(tag, dtype, T, top, D)) return rc;
   if (T == 0 || top == 0 || D == 0) return B200Q_OK;
   if (!x || !places || !order || !xs) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
-  if (!aligned(x, dtype) || !aligned(xs, dtype)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
+  if (!on_boundaries({x, xs}, dtype_size(dtype)) || !on_boundaries({places, order}, 4)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
   const RowsParams p{x, nullptr, xs, places, order, nullptr, nullptr, T, T * top, D, 0, (int)top};
   return run(Kind::Dispatch, p, dtype, static_cast<cudaStream_t>(stream));
 }
@@ -335,7 +334,7 @@ extern "C" int b200q_combine_rows(const void* y, int dtype, int64_t T, int64_t t
   if (int rc = check(tag, dtype, T, top, D)) return rc;
   if (T == 0 || D == 0) return B200Q_OK;
   if (!out || (top > 0 && (!y || !places))) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
-  if (!aligned(y, dtype) || !aligned(out, dtype)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
+  if (!on_boundaries({y, out}, dtype_size(dtype)) || !on_boundaries({places, weights}, 4)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
   const RowsParams p{nullptr, y, out, places, nullptr, weights, nullptr, T, T * top, D, 0, (int)top};
   return run(Kind::Combine, p, dtype, static_cast<cudaStream_t>(stream));
 }
@@ -345,13 +344,13 @@ extern "C" int b200q_combine_rows_grad(const void* dy, const void* y, int dtype,
   const char* tag = "combine_rows";
   if (int rc = check(tag, dtype, T, top, D)) return rc;
   if (T == 0 || top == 0 || (!dys && !dw)) return B200Q_OK;
+  if (!on_boundaries({dy, y, dys}, dtype_size(dtype)) || !on_boundaries({places, order, weights, dw}, 4)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (D == 0) {
     if (dw) B200Q_CUDA_OK(cudaMemsetAsync(dw, 0, (size_t)T * top * 4, st));
     return B200Q_OK;
   }
   if (!dy || (dw && !y) || !places || !order || !weights) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] null pointer", tag);
-  if (!aligned(dy, dtype) || !aligned(y, dtype) || !aligned(dys, dtype)) return fail(B200Q_ERR_INVALID_ARGUMENT, "[%s] misaligned pointer", tag);
   const RowsParams p{dy, y, dys, places, order, weights, dw, T, T * top, D, 0, (int)top};
   return run(Kind::Grad, p, dtype, st);
 }
