@@ -500,8 +500,7 @@ bool pdl_enabled() {
 template <int BITS>
 int launch(const QmvPlan& pl, cudaStream_t st) {
   auto go = [&](auto kern) -> int {
-    if (pl.smem > 48 * 1024)
-      B200Q_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem));
+    if (int rc = allow_smem(reinterpret_cast<const void*>(kern), pl.smem)) return rc;
     if (pdl_enabled()) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(pl.grid);

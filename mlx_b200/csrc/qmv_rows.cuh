@@ -1016,8 +1016,7 @@ bool pdl_on();
 template <typename T, int BITS, bool RUNS, int SHAPE, int MT, Work W, bool WIDE = false>
 int launch(const RowsPlan& pl, cudaStream_t st) {
   auto kern = qmv_rows_kernel<T, BITS, RUNS, SHAPE, MT, W, WIDE>;
-  if (pl.smem > 48 * 1024)
-    B200Q_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem));
+  if (int rc = allow_smem(reinterpret_cast<const void*>(kern), pl.smem)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(pl.grid);
   cfg.blockDim = dim3(kThreads);

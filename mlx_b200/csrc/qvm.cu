@@ -186,15 +186,13 @@ size_t qvm_counters_bytes(int blocks_n) { return (size_t)((blocks_n * 4 + 255) /
 
 template <typename T>
 int launch_qvm(const QmmArgs& a, const QvmPlan& pl, cudaStream_t st) {
-  const size_t smem = (size_t)(kQvmMaxM * pl.slab + kQvmMaxM * kQvmCols) * sizeof(float);
+  const size_t smem = (size_t)(kQvmMaxM * pl.slab + kQvmMaxM * kQvmCols) * sizeof(float);   // 40 KB at most: within what every kernel may have
   uint32_t* counters = reinterpret_cast<uint32_t*>(a.ws);
   float* partial = reinterpret_cast<float*>(static_cast<char*>(a.ws) + qvm_counters_bytes(pl.blocks_n));
   const dim3 grid(pl.blocks_n, pl.slabs);
   int rc = B200Q_ERR_UNSUPPORTED;
 #define B200Q_QVM_LAUNCH2(BITS_, MM_)                                                                             \
   {                                                                                                               \
-    cudaError_t e = cudaFuncSetAttribute(qvm_kernel<T, BITS_, MM_>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
-    if (e != cudaSuccess) return fail(B200Q_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(e));   \
     qvm_kernel<T, BITS_, MM_><<<grid, kQvmThreads, smem, st>>>((const T*)a.x, a.wq, (const T*)a.scales,           \
                                                                (const T*)a.biases, (T*)a.y, partial, counters,    \
                                                                (int)a.M, (int)a.N, (int)a.K, a.group, pl.slab);   \
