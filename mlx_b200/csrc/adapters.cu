@@ -7,7 +7,7 @@
 // Rows come sorted by adapter (b200q_group_rows), in tiles of up to 64 rows of one adapter.  A rank of 8 to 64 makes r operations per byte of
 // activations, far below what the tensor cores do per byte of HBM, so the kernels are built for the memory: activations are read once per product and
 // nothing is written but h and the results.  The products are mma.sync (545 TFLOP/s measured here): tiles of a few rows whose number only the
-// device knows, operands that come in pieces from gathered rows and are split into two parts on the way; at rank 64 they take about as long as HBM does.
+// device knows, operands that come in pieces from gathered rows and are split into parts on the way; at rank 64 they take somewhat longer than HBM does.
 //
 // h and g, summed in fp32, are kept as three bf16 numbers each that add up to them exactly, since that is how the second products take them: fp32's 24 bits are 8
 // and two times 8 more with signs.  16-bit floats of type f16 are split too, in two, exactly, so that no value leaves a type's range; of those six products
@@ -250,7 +250,7 @@ __device__ int64_t tiles_with_rows(const Params& p, bool with_adapter) {
 // TALL: weights [C, r], else [r, C].
 //
 // Every warp has a ring of its own in shared memory, filled some steps ahead, in pieces of 16 bytes whose places are swizzled so that eight rows of
-// a matrix are in different banks; no barrier but the warp's.  4096 rows of 16 adapters of rank 64, bf16: 21 us from K = 4096, 40 from K = 14336
+// a matrix are in different banks; no barrier but the warp's.  4096 rows of 16 adapters of rank 64, bf16: 23 us from K = 4096, 41 from K = 14336
 // (2.9 TB/s of x); what bounds it there is L2, from which the weights come again for every 64 rows, as many bytes as x has.  Few rows: latencies, 10 us for
 // 57 rows of 40 adapters of rank 20 (K 4096, f16).
 template <bool TALL, int MT>
@@ -414,15 +414,14 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) down_kernel(const P
 
 // ---- out[row] = y[row] + (c) sum over ranks of h[place] w.  Blocks by (tiles, 256 columns), warps by 32 columns; steps of 16 rows and, inside, 16
 // ranks.  Up to 64 ranks (KS steps) have their weights in registers, over all rows that an adapter has among the block's tiles.  More (CHUNKED): the
-// sums of a tile stay in registers while its ranks come 32 at a time.  (4096 rows of rank 64, [14336, 4096], both products, before the tiles were shared evenly, us: 104, CHUNKED
-// 119; rank 32: 72 and 86.  4096 rows of rank 128, [4096, 4096]: 67.)
+// sums of a tile stay in registers while its ranks come 32 at a time.  (4096 rows of rank 64, [14336, 4096], both products, us: 110, CHUNKED 141; rank 32: 75 and 97.  4096 rows of rank
+// 128, [4096, 4096]: 84.)
 // WIDE: weights [r, C], else [C, r].
 //
 // Bound by the latency of y and by instructions: every lane copies its own pieces of y, three steps of rows ahead, into a ring in shared memory; the steps'
-// rows are looked up once per block; h lies in shared memory as the products' operands want it, so that one load brings four registers that are next to each
-// other (two rows loaded apart would have to be moved together for every product: half of all instructions).  4096 rows of rank 64, bf16, cold: 84 us for C = 14336 (2.8
-// TB/s), 31 for C = 4096 (3.2 TB/s): tensor cores 33 %, loads and stores of shared memory 58 %, HBM 30 %, 16 warps on an SM for their registers; the two parts' products alone
-// would take 28 and 8, HBM 36 and 10.
+// rows are looked up once per block; h lies in shared memory as one matrix load per part wants it.  4096 rows of rank 64, bf16, cold: 95 us for C = 14336 (2.1
+// TB/s of HBM), 34 for C = 4096: tensor cores 45 %, shared memory 39 %, HBM 26 %, 15 warps on an SM for their registers; a warp's issue waits for fixed latencies, shared memory and the
+// tensor cores in turn.  The three parts' products alone would take 41 and 12, HBM 36 and 10.  (Two parts of h, which lose 2^-17: 84 and 31.)
 constexpr int kUpStages = 4, kUpTiles = 16, kUpSteps = kUpTiles * kRows / 16;
 template <int KS, bool CHUNKED>
 struct Up {
@@ -646,8 +645,9 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
 // Rows lie in shared memory as they come, and matrix loads that transpose make both operands of them; h's parts lie apart there.  Which rows come next is
 // copied there, too, a ring ahead, so that no step waits for it.  (4096 rows of one adapter of rank 64 and 4096 columns: 27 us, 90 when every 32 columns' h was
 // transposed in registers; HBM 5.  2048 rows of 4 adapters of rank 16, [14336, 4096], forward and all gradients: 98 us, 106 with three stages and rows looked up
-// one step ahead; 1000 adapters of a row each have no use for it: 229 and 215.)  Bound by latencies: a block has few steps, and reads where its rows are before it
-// reads them; with 64 ranks tensor cores and shared memory are at a third and two thirds.
+// one step ahead; 1000 adapters of a row each have no use for it: 229 and 215; all these with two parts of h.  With three 36 us, and 99.)  Bound by latencies: a block has few steps, and reads where its rows are
+// before it reads them; with 64 ranks and 14336 columns (104 us cold) tensor cores are at 41 %, shared memory at 38, waits for it take a third of the time.  Two blocks on an SM (rank 64, f16: gradients
+// 223 us with one, 158 with two).
 template <bool TALL, int MT>
 struct Outer {
   static constexpr int kRanks = 16 * MT, kCols = 128, kSteps = 32, kStages = MT == 1 ? 5 : 4;
@@ -833,11 +833,12 @@ int width_of(const void* p, int64_t pitch) {
   return w;
 }
 // Blocks per cluster: a power of two up to 8, as many as fit on the SMs at once, with work for everyone.  (With at most 1, 2, 4, 8, by graph replay, us: one row of
-// rank 16, [14336, 4096], forward 8.4 7.0 5.8 5.3, gradient of x 25.7 15.6 10.1 7.5; 57 rows of 40 adapters of rank 20, f16, [11008, 4096], gradient
-// of x 48 30 20 19; 4096 rows of rank 64 102 70 70 70.)
-int split_of(int64_t blocks, int64_t slots, int64_t most) {
+// rank 16, [14336, 4096], forward 8.8 7.2 6.1 5.7, gradient of x 24.4 15.3 10.4 7.7; 57 rows that choose among 40 adapters of rank 20, f16, [11008, 4096], gradient
+// of x 46 29 21 19; 4096 rows of rank 64 110 77 77 77.)  Eight only where a sixth of the SMs is left to blocks of the product after it, which begin beside it: both projections of 2048 rows of 4 adapters of rank
+// 16 66 us with four, 70 with eight; 1024 rows of rank 64, [4096, 4096], 23 and 34.
+int split_of(int64_t blocks, int64_t slots, int64_t most, bool beside) {
   int s = 1;
-  while (s < 8 && blocks * 2 * s <= slots && 2 * s <= most) s *= 2;
+  while (s < 8 && blocks * 2 * s <= (beside && s == 4 ? slots * 5 / 6 : slots) && 2 * s <= most) s *= 2;
   return s;
 }
 // Tiles that there will be, about (the table has room for the most that there can be): rows that choose their adapters at random.
@@ -846,8 +847,8 @@ int64_t likely_tiles(const Params& p) {
   return std::max<int64_t>(1, std::min<int64_t>(p.T, p.T / kRows + (int64_t)(used * (1.0 - 0.5 * std::min(1.0, rows / kRows)))));
 }
 // Tiles per block of the second product.  A block takes about as long as its tiles and three quarters of one more; blocks run in waves.  (By graph
-// replay, both products, us, with 1, 2, 3, 4, 5, 6, 8 tiles: 57 rows of 40 adapters of rank 20, f16, [11008, 4096] 26 23 22 25 21 22 26; 4096 rows of rank 64,
-// [14336, 4096] 119 104 102 103 100 111 111; 2048 rows of rank 16 41 40 40 40 38 39 41: the rule takes 6, 5 and 5.)
+// replay, both products, us, with 1, 2, 3, 4, 5, 6, 8 tiles: 57 rows that choose among 40 adapters of rank 20, f16, [11008, 4096] 27 23 23 24 22 22 27; 4096 rows of rank 64,
+// [14336, 4096] 129 115 111 115 109 118 124; 2048 rows of rank 16 41 38 37 40 36 39 47: the rule takes 5 for all three.)
 int tiles_per_block(const Params& p, int64_t cols, int64_t slots) {
   const int64_t tiles = likely_tiles(p);
   double best = 0;
@@ -887,7 +888,7 @@ int launch(K kern, const Params& p, dim3 grid, int threads, size_t smem, cudaStr
 template <typename T, bool TALL, bool WHOLE>
 int down(Params p, cudaStream_t st) {
   const int mt = p.r <= 16 ? 1 : (p.r <= 32 ? 2 : 4), chunks = (p.r + 16 * mt - 1) / (16 * mt);
-  p.split = split_of(likely_tiles(p) * chunks, 148 * (mt == 4 ? 1 : 2), p.C / (kWarps * 32));
+  p.split = split_of(likely_tiles(p) * chunks, 148 * (mt == 4 ? 1 : 2), p.C / (kWarps * 32), true);
   const dim3 grid((unsigned)(p.tiles_n * p.split), chunks);
   if (mt == 1) return launch(down_kernel<T, TALL, WHOLE, 1>, p, grid, kThreads, Down<TALL, 1>::kBytes, st);
   if (mt == 2) return launch(down_kernel<T, TALL, WHOLE, 2>, p, grid, kThreads, Down<TALL, 2>::kBytes, st);
@@ -898,11 +899,13 @@ int up(Params p, cudaStream_t st) {
   p.split = 1;
   const int64_t cols = (p.C + 255) / 256;
   const int64_t slots = 148 * (p.r > 64 ? 2 : (p.r > 32 ? 2 : 3) - std::is_same_v<T, __half>);
-  // Blocks with 8 tiles or more each count the tiles that have rows and share them evenly, in one wave; for fewer the count costs more than a last wave.  (Counted /
-  // not, graph replay, us: 4096 rows of 5 of 16 adapters of rank 64, [14336, 4096] 96 / 104, 4096 rows of rank 64, [4096, 4096] 43.6 / 43.1, 16 rows of as many adapters 7.3 / 6.7, 57 rows
-  // of 40 adapters, f16, both projections 41.6 / 39.3.)
-  p.each = likely_tiles(p) * cols >= 8 * slots ? 0 : tiles_per_block(p, cols, slots);
-  const int64_t parts = p.each ? (p.tiles_n + p.each - 1) / p.each : std::max<int64_t>(1, slots / cols);
+  // Where blocks have 8 tiles or more each, those that fit on the SMs at once count the tiles that have rows and share them evenly, if that leaves hardly any SM without a block or if the sum
+  // is in place, where tiles of rows without an adapter are no work.  (Counted / not, graph replay, us: 16384 rows of 16 adapters, [4096, 4096], rank 64 155 / 155, 16 83 / 85, 128 306 / 310; 8192 rows of
+  // which 9 in 10 have no adapter, [14336, 2048], in place, rank 64 41 / 51, 16 22 / 26; with an eighth of the SMs left out: 8192 rows of rank 32, [14336, 4096], 142 / 128, of rank 64, f16, 191 / 176.  For
+  // fewer tiles the count costs more than a last wave: 16 rows of as many adapters 8.8 / 6.9.)
+  const int64_t even = std::max<int64_t>(1, slots / cols);
+  p.each = likely_tiles(p) * cols >= 8 * slots && (p.y == p.out || even * cols * 25 >= slots * 24) ? 0 : tiles_per_block(p, cols, slots);
+  const int64_t parts = p.each ? (p.tiles_n + p.each - 1) / p.each : even;
   const dim3 grid((unsigned)(cols * parts));
   if (p.r <= 16) return launch(up_kernel<T, WIDE, WHOLE, 1, false>, p, grid, kThreads, Up<1, false>::kBytes, st, true);
   if (p.r <= 32) return launch(up_kernel<T, WIDE, WHOLE, 2, false>, p, grid, kThreads, Up<2, false>::kBytes, st, true);
@@ -913,7 +916,7 @@ template <typename T, bool TALL, bool WHOLE>
 int outer(Params p, cudaStream_t st) {
   const int mt = p.r <= 16 ? 1 : (p.r <= 32 ? 2 : 4), chunks = (p.r + 16 * mt - 1) / (16 * mt);
   const int64_t cols = (p.C + 127) / 128;
-  p.split = split_of(cols * p.L * chunks, 148 * 2, p.T / 64);
+  p.split = split_of(cols * p.L * chunks, 148 * 2, p.T / 64, false);
   const dim3 grid((unsigned)(cols * p.split), p.L, chunks);
   if (mt == 1) return launch(outer_kernel<T, TALL, WHOLE, 1>, p, grid, kThreads, Outer<TALL, 1>::kBytes, st);
   if (mt == 2) return launch(outer_kernel<T, TALL, WHOLE, 2>, p, grid, kThreads, Outer<TALL, 2>::kBytes, st);

@@ -823,14 +823,14 @@ int launch_route(const RouteParams& p, int blocks, int warps, cudaStream_t st) {
   return go(route_kernel<T, 32>);
 }
 
-// Blocks and warps: up to 16 tokens in one block, one launch; else 8 tokens or more per block, one block of up to 32 warps per SM, whose histograms the
-// second launch reads.  (One block / several, us: 16 tokens, 2 of 8 experts, 6.0 / 9.6, 8 of 256 in groups 9.6 / 11.1; 32 tokens 8.2 / 9.6 and 14.6 / 11.1; 64 tokens 9.9 / 9.6
-// and 22 / 11.1: many experts share one SM's instructions.)
+// Blocks and warps: up to 16 tokens in one block, one launch (to 24 of up to 128 experts, to 48 of up to 32); else 8 tokens or more per block, one block of up to 32 warps per SM,
+// whose histograms the second launch reads.  (One block / several, us: 2 of 8 experts, 16 tokens 5.8 / 9.3, 48 8.4 / 9.6, 64 9.8 / 9.7; 8 of 128, 24 tokens 7.7 / 8.0, 32 9.3 / 8.1;
+// 8 of 256 in groups, 16 tokens 9.4 / 10.4, 24 11.6 / 10.5: many experts share one SM's instructions.)
 struct Split { int blocks, warps; int64_t per_block, per_warp; };
 Split route_split(int64_t T, int64_t E) {
   Split s{};
   const int most = E > 512 ? 16 : kMaxWarps;
-  s.blocks = T <= 16 ? 1 : (int)std::min<int64_t>((T + 7) / 8, 148);
+  s.blocks = T <= (E <= 32 ? 48 : (E <= 128 ? 24 : 16)) ? 1 : (int)std::min<int64_t>((T + 7) / 8, 148);
   s.per_block = (T + s.blocks - 1) / s.blocks;
   s.blocks = (int)((T + s.per_block - 1) / s.per_block);
   s.warps = (int)std::min<int64_t>(s.per_block, most);

@@ -217,8 +217,9 @@ __global__ void __launch_bounds__(kThreads) combine_any_kernel(const RowsParams 
   });
 }
 
-// A group of threads has a pair (token, choice): a warp, or the block where there are few pairs, up to a wave of blocks.  (Rows of 2047, f16, block / warp, us: 8 pairs 2.7 / 6.8,
-// 800 5.1 / 7.4, 1200 6.2 / 7.8, 9186 33.6 / 18.8.)  dy's row is read once from HBM and for the token's other pairs from L2.
+// A group of threads has a pair (token, choice): a warp, or the block where rows are long and pairs few: up to 12 pairs for every 16 bytes of a row.  (Inputs not in L2, block /
+// warp, us: rows of 2047, f16, 300 pairs 4.5 / 12.1, 2400 14.0 / 16.4, 3600 18.7 / 17.8, 9186 44.2 / 32.5; of 1023, f32, 2400 12.6 / 16.8, 3600 17.3 / 17.9, 4800 22.2 / 19.4; of 255,
+// bf16, 300 2.8 / 2.8, 800 4.2 / 2.8; of 8191, bf16, 300 8.6 / 43, 9186 101 / 109.)  dy's row is read once from HBM and for the token's other pairs from L2.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) combine_grad_any_kernel(const RowsParams p, int group) {
   constexpr int VEC = 16 / sizeof(T);
@@ -275,7 +276,7 @@ int launch(Kind kind, RowsParams p, cudaStream_t st) {
   const uintptr_t all = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.D * sizeof(T));
   p.pieces = p.D / VEC;
   const unsigned tokens = (unsigned)p.T, threads = (unsigned)std::min<int64_t>(kThreads, (p.pieces + 32) / 32 * 32);
-  const int group = p.R < 148 * 8 ? kThreads : 32;
+  const int group = p.R < 12 * p.pieces ? kThreads : 32;
   const unsigned pairs = (unsigned)((p.R + kThreads / group - 1) / (kThreads / group));
   if (all % 16 == 0) {   // every piece of 16 bytes on its boundary
     const unsigned blocks = (unsigned)std::min<int64_t>((p.T * p.pieces + kThreads - 1) / kThreads, 148 * 8 * 16);
