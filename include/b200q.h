@@ -471,7 +471,7 @@ int b200q_group_rows(const void* ids, int id_bytes, int64_t T, int64_t n, int32_
 
 /*
  * Low-rank adapters beside a shared projection: out[t] = y[t] + scales[l] b[l] (a[l] x[t]), l being row t's adapter; a row without one:
- * y[t].  bf16 and f16; sums and inner products in fp32, the result rounded once.  Inner products are multiplied as three parts each and 16-bit numbers of f16 as
+ * y[t].  bf16 and f16; sums and inner products in fp32 (short ones by the tensor cores, which truncate; these are added with the nearest rounding), the result rounded once.  Inner products are multiplied as three parts each and 16-bit numbers of f16 as
  * two: where what a finite inner product is multiplied with is infinite (b, in the gradients a, x or dy), so that the sum would be, it may be a NaN.
  *   y, out [T, N] (out may be y), x [T, K], a [L, r, K], b [L, N, r] dtype; scales [L] float32 (NULL: 1)
  *   order, starts, tiles: b200q_group_rows over L groups

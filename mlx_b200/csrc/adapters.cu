@@ -36,6 +36,11 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The matrix instructions truncate their sums: long ones are made of short ones, which are added here with the nearest rounding.
+__device__ __forceinline__ void add4(float (&d)[4], const float (&s)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d[i] += s[i];
+}
 // An 8 x 8 matrix of 16-bit values, lane (i, q) having (i, 2q) and (i, 2q + 1): afterwards (2q, i) and (2q + 1, i).
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t r;
@@ -250,9 +255,9 @@ __device__ int64_t tiles_with_rows(const Params& p, bool with_adapter) {
 // TALL: weights [C, r], else [r, C].
 //
 // Every warp has a ring of its own in shared memory, filled some steps ahead, in pieces of 16 bytes whose places are swizzled so that eight rows of
-// a matrix are in different banks; no barrier but the warp's.  4096 rows of 16 adapters of rank 64, bf16: 23 us from K = 4096, 41 from K = 14336
-// (2.9 TB/s of x); what bounds it there is L2, from which the weights come again for every 64 rows, as many bytes as x has.  Few rows: latencies, 10 us for
-// 57 rows of 40 adapters of rank 20 (K 4096, f16).
+// a matrix are in different banks; no barrier but the warp's.  4096 rows of 16 adapters of rank 64, bf16: 25 us from K = 4096, 46 from K = 14336
+// (2.6 TB/s of x); what bounds it there is L2, from which the weights come again for every 64 rows, as many bytes as x has.  Few rows: latencies, 10 us for
+// 57 rows of 40 adapters of rank 20 (K 4096, f16).  The additions of every step's sums in fp32 are 2 to 5 us of the 25 and 46.
 template <bool TALL, int MT>
 struct Down {
   static constexpr int kRanks = 16 * MT, kW = 2 * MT, kPieces = 8 + kW, kStages = MT == 4 ? 3 : 2;
@@ -354,10 +359,13 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) down_kernel(const P
     for (int n = 0; n < 8; ++n)
       if (n < eights) {
         const uint4 v = load_matrices<false>(from + n * 512 + x_row);
+        float sum[MT][4] = {};
 #pragma unroll
-        for (int m = 0; m < MT; ++m) mma<T>(acc[m][n], a[m][0].x, a[m][0].y, a[m][0].z, a[m][0].w, v.x, v.y);
+        for (int m = 0; m < MT; ++m) mma<T>(sum[m], a[m][0].x, a[m][0].y, a[m][0].z, a[m][0].w, v.x, v.y);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) mma<T>(acc[m][n], a[m][1].x, a[m][1].y, a[m][1].z, a[m][1].w, v.z, v.w);
+        for (int m = 0; m < MT; ++m) mma<T>(sum[m], a[m][1].x, a[m][1].y, a[m][1].z, a[m][1].w, v.z, v.w);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) add4(acc[m][n], sum[m]);
       }
     to = from;
     from = from + kStageBytes == end ? ring : from + kStageBytes;
@@ -414,13 +422,13 @@ __global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2) down_kernel(const P
 
 // ---- out[row] = y[row] + (c) sum over ranks of h[place] w.  Blocks by (tiles, 256 columns), warps by 32 columns; steps of 16 rows and, inside, 16
 // ranks.  Up to 64 ranks (KS steps) have their weights in registers, over all rows that an adapter has among the block's tiles.  More (CHUNKED): the
-// sums of a tile stay in registers while its ranks come 32 at a time.  (4096 rows of rank 64, [14336, 4096], both products, us: 110, CHUNKED 141; rank 32: 75 and 97.  4096 rows of rank
-// 128, [4096, 4096]: 84.)
+// sums of a tile stay in registers while its ranks come 32 (f16: 16) at a time.  (4096 rows of rank 64, [14336, 4096], both products, us: 115, CHUNKED 150; rank 32: 74 and 104.  4096 rows of rank
+// 128, [4096, 4096]: 93.)
 // WIDE: weights [r, C], else [C, r].
 //
 // Bound by the latency of y and by instructions: every lane copies its own pieces of y, three steps of rows ahead, into a ring in shared memory; the steps'
-// rows are looked up once per block; h lies in shared memory as one matrix load per part wants it.  4096 rows of rank 64, bf16, cold: 95 us for C = 14336 (2.1
-// TB/s of HBM), 34 for C = 4096: tensor cores 45 %, shared memory 39 %, HBM 26 %, 15 warps on an SM for their registers; a warp's issue waits for fixed latencies, shared memory and the
+// rows are looked up once per block; h lies in shared memory as one matrix load per part wants it.  4096 rows of rank 64, bf16, cold: 96 us for C = 14336 (2.1
+// TB/s of HBM), 34 for C = 4096: tensor cores 43 %, shared memory 38 %, HBM 26 %, 15 warps on an SM for their registers; a warp's issue waits for fixed latencies, shared memory and the
 // tensor cores in turn.  The three parts' products alone would take 41 and 12, HBM 36 and 10.  (Two parts of h, which lose 2^-17: 84 and 31.)
 constexpr int kUpStages = 4, kUpTiles = 16, kUpSteps = kUpTiles * kRows / 16;
 template <int KS, bool CHUNKED>
@@ -570,19 +578,23 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
         }
         ++now;
       };
-      auto step = [&](float (&acc)[4][4], int s, uint32_t src) {
+      // The ranks r0 .. r0 + 16 KS of 16 rows, whose h lies at src; the smallest parts first, so that few products are truncated at the whole sum's size.
+      auto products = [&](float (&acc)[4][4], int r0, uint32_t src) {
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          const uint4 a = load_matrices<false>(src + i * 512);
+        for (int i = 2; i >= 0; --i)
 #pragma unroll
-          for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], a.x, a.y, a.z, a.w, bh[s][t][0], bh[s][t][1]);
-          if constexpr (kSplitW) {
-            if (i < 2) {
+          for (int s = 0; s < KS; ++s) {
+            if (KS > 1 && r0 + s * 16 >= p.r16) break;
+            const uint4 a = load_matrices<false>(src + s * 1536 + i * 512);
+            if constexpr (kSplitW) {
+              if (i < 2) {
 #pragma unroll
-              for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], a.x, a.y, a.z, a.w, bl[s][t][0], bl[s][t][1]);
+                for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], a.x, a.y, a.z, a.w, bl[s][t][0], bl[s][t][1]);
+              }
             }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) mma<__nv_bfloat16>(acc[t], a.x, a.y, a.z, a.w, bh[s][t][0], bh[s][t][1]);
           }
-        }
       };
       // (rows behind the tile's last one have what was there before; their products are not stored)
       if constexpr (CHUNKED) {
@@ -599,12 +611,13 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
           weights(r0);
           const uint32_t src = h_row + buffer * 4 * kStep;
 #pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            if (r0 + s * 16 >= p.r16) break;
+          for (int m = 0; m < kRows / 16; ++m)
+            if (m < last) {
+              float sum[4][4] = {};
+              products(sum, r0, src + m * kStep);
 #pragma unroll
-            for (int m = 0; m < kRows / 16; ++m)
-              if (m < last) step(acc[m], s, src + m * kStep + s * 1536);
-          }
+              for (int t = 0; t < 4; ++t) add4(acc[m][t], sum[t]);
+            }
         }
 #pragma unroll
         for (int m = 0; m < kRows / 16; ++m)
@@ -621,13 +634,7 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
         for (int m = 0; m < last; ++m, src += kStep) {
           issue();
           float acc[4][4] = {};
-          if (!plain) {
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-              if (KS > 1 && s * 16 >= p.r16) break;
-              step(acc, s, src + s * 1536);
-            }
-          }
+          if (!plain) products(acc, 0, src);
           finish(acc);
         }
         buffer ^= 1;
@@ -645,8 +652,8 @@ __global__ void __launch_bounds__(kThreads, CHUNKED ? 2 : (KS == 4 ? 2 : 3) - st
 // Rows lie in shared memory as they come, and matrix loads that transpose make both operands of them; h's parts lie apart there.  Which rows come next is
 // copied there, too, a ring ahead, so that no step waits for it.  (4096 rows of one adapter of rank 64 and 4096 columns: 27 us, 90 when every 32 columns' h was
 // transposed in registers; HBM 5.  2048 rows of 4 adapters of rank 16, [14336, 4096], forward and all gradients: 98 us, 106 with three stages and rows looked up
-// one step ahead; 1000 adapters of a row each have no use for it: 229 and 215; all these with two parts of h.  With three 36 us, and 99.)  Bound by latencies: a block has few steps, and reads where its rows are
-// before it reads them; with 64 ranks and 14336 columns (104 us cold) tensor cores are at 41 %, shared memory at 38, waits for it take a third of the time.  Two blocks on an SM (rank 64, f16: gradients
+// one step ahead; 1000 adapters of a row each have no use for it: 229 and 215; all these with two parts of h.  With three, and every step's sums added in fp32, 39 us, and 99.)  Bound by latencies: a block has few steps, and reads where its rows are
+// before it reads them; with 64 ranks and 14336 columns (107 us cold) tensor cores are at 38 %, shared memory at 36.  Two blocks on an SM (rank 64, f16: all gradients
 // 223 us with one, 158 with two).
 template <bool TALL, int MT>
 struct Outer {
@@ -737,18 +744,21 @@ __global__ void __launch_bounds__(kThreads, 2) outer_kernel(const Params p) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       if (MT > 1 && r0 + m * 16 >= p.r16) break;
+      float sum[4][4] = {};
 #pragma unroll
-      for (int i = 0; i < 3; ++i) {
+      for (int i = 2; i >= 0; --i) {   // (the smallest products first)
         const uint4 a = load_matrices<true>(src + h_at + m * 32 + i * O::kSteps * kHPitch);
-#pragma unroll
-        for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a.x, a.y, a.z, a.w, bh[v][0], bh[v][1]);
         if constexpr (kSplitX) {
           if (i < 2) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(acc[m][v], a.x, a.y, a.z, a.w, bl[v][0], bl[v][1]);
+            for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(sum[v], a.x, a.y, a.z, a.w, bl[v][0], bl[v][1]);
           }
         }
+#pragma unroll
+        for (int v = 0; v < 4; ++v) mma<__nv_bfloat16>(sum[v], a.x, a.y, a.z, a.w, bh[v][0], bh[v][1]);
       }
+#pragma unroll
+      for (int v = 0; v < 4; ++v) add4(acc[m][v], sum[v]);
     }
     to = from;
     from = from + 1 == kStages ? 0 : from + 1;
@@ -833,9 +843,9 @@ int width_of(const void* p, int64_t pitch) {
   return w;
 }
 // Blocks per cluster: a power of two up to 8, as many as fit on the SMs at once, with work for everyone.  (With at most 1, 2, 4, 8, by graph replay, us: one row of
-// rank 16, [14336, 4096], forward 8.8 7.2 6.1 5.7, gradient of x 24.4 15.3 10.4 7.7; 57 rows that choose among 40 adapters of rank 20, f16, [11008, 4096], gradient
-// of x 46 29 21 19; 4096 rows of rank 64 110 77 77 77.)  Eight only where a sixth of the SMs is left to blocks of the product after it, which begin beside it: both projections of 2048 rows of 4 adapters of rank
-// 16 66 us with four, 70 with eight; 1024 rows of rank 64, [4096, 4096], 23 and 34.
+// rank 16, [14336, 4096], forward 8.6 7.2 6.2 5.7, gradient of x 23.9 14.7 10.0 7.7; 57 rows that choose among 40 adapters of rank 20, f16, [11008, 4096], gradient
+// of x 40 26 20 19; 4096 rows of rank 64 123 83 83 83.)  Eight only where a sixth of the SMs is left to blocks of the product after it, which begin beside it: both projections of 2048 rows of 4 adapters of rank
+// 16 68 us with four, 70 with eight; 1024 rows of rank 64, [4096, 4096], 24 and 34.
 int split_of(int64_t blocks, int64_t slots, int64_t most, bool beside) {
   int s = 1;
   while (s < 8 && blocks * 2 * s <= (beside && s == 4 ? slots * 5 / 6 : slots) && 2 * s <= most) s *= 2;
@@ -847,8 +857,8 @@ int64_t likely_tiles(const Params& p) {
   return std::max<int64_t>(1, std::min<int64_t>(p.T, p.T / kRows + (int64_t)(used * (1.0 - 0.5 * std::min(1.0, rows / kRows)))));
 }
 // Tiles per block of the second product.  A block takes about as long as its tiles and three quarters of one more; blocks run in waves.  (By graph
-// replay, both products, us, with 1, 2, 3, 4, 5, 6, 8 tiles: 57 rows that choose among 40 adapters of rank 20, f16, [11008, 4096] 27 23 23 24 22 22 27; 4096 rows of rank 64,
-// [14336, 4096] 129 115 111 115 109 118 124; 2048 rows of rank 16 41 38 37 40 36 39 47: the rule takes 5 for all three.)
+// replay, both products, us, with 1, 2, 3, 4, 5, 6, 8 tiles: 57 rows that choose among 40 adapters of rank 20, f16, [11008, 4096] 27 23 23 24 21 24 28; 4096 rows of rank 64,
+// [14336, 4096] 135 120 116 120 115 123 127; 2048 rows of rank 16 41 39 37 40 37 40 48: the rule takes 5 for all three.)
 int tiles_per_block(const Params& p, int64_t cols, int64_t slots) {
   const int64_t tiles = likely_tiles(p);
   double best = 0;
@@ -900,8 +910,8 @@ int up(Params p, cudaStream_t st) {
   const int64_t cols = (p.C + 255) / 256;
   const int64_t slots = 148 * (p.r > 64 ? 2 : (p.r > 32 ? 2 : 3) - std::is_same_v<T, __half>);
   // Where blocks have 8 tiles or more each, those that fit on the SMs at once count the tiles that have rows and share them evenly, if that leaves hardly any SM without a block or if the sum
-  // is in place, where tiles of rows without an adapter are no work.  (Counted / not, graph replay, us: 16384 rows of 16 adapters, [4096, 4096], rank 64 155 / 155, 16 83 / 85, 128 306 / 310; 8192 rows of
-  // which 9 in 10 have no adapter, [14336, 2048], in place, rank 64 41 / 51, 16 22 / 26; with an eighth of the SMs left out: 8192 rows of rank 32, [14336, 4096], 142 / 128, of rank 64, f16, 191 / 176.  For
+  // is in place, where tiles of rows without an adapter are no work.  (Counted / not, graph replay, us: 16384 rows of 16 adapters, [4096, 4096], rank 64 160 / 162, 16 83 / 85, 128 342 / 347; 8192 rows of
+  // which 9 in 10 have no adapter, [14336, 2048], in place, rank 64 42 / 54, 16 22 / 27; with an eighth of the SMs left out: 8192 rows of rank 32, [14336, 4096], 143 / 130; a quarter: 4096 of rank 64, f16, 202 / 185.  For
   // fewer tiles the count costs more than a last wave: 16 rows of as many adapters 8.8 / 6.9.)
   const int64_t even = std::max<int64_t>(1, slots / cols);
   p.each = likely_tiles(p) * cols >= 8 * slots && (p.y == p.out || even * cols * 25 >= slots * 24) ? 0 : tiles_per_block(p, cols, slots);
@@ -910,7 +920,8 @@ int up(Params p, cudaStream_t st) {
   if (p.r <= 16) return launch(up_kernel<T, WIDE, WHOLE, 1, false>, p, grid, kThreads, Up<1, false>::kBytes, st, true);
   if (p.r <= 32) return launch(up_kernel<T, WIDE, WHOLE, 2, false>, p, grid, kThreads, Up<2, false>::kBytes, st, true);
   if (p.r <= 64) return launch(up_kernel<T, WIDE, WHOLE, 4, false>, p, grid, kThreads, Up<4, false>::kBytes, st, true);
-  return launch(up_kernel<T, WIDE, WHOLE, 2, true>, p, grid, kThreads, Up<2, true>::kBytes, st, true);
+  constexpr int kChunk = std::is_same_v<T, __half> ? 1 : 2;   // (f16: weights of 32 ranks in two parts would be spilled; 4096 rows of rank 128, [4096, 4096], 133 us instead of 115)
+  return launch(up_kernel<T, WIDE, WHOLE, kChunk, true>, p, grid, kThreads, Up<kChunk, true>::kBytes, st, true);
 }
 template <typename T, bool TALL, bool WHOLE>
 int outer(Params p, cudaStream_t st) {
