@@ -552,8 +552,8 @@ __device__ void sum_over_warps(uint32_t* hist, int bins, uint32_t* sums) {
 }
 
 // A block has consecutive tokens, a warp a range of them.  Bound by the instructions of a token's dependent steps, HBM is idle: 8192 tokens, 8 of 256 experts in
-// groups with a bias, f32, 26 us with cold caches (320 GB/s; bytes would take 1.4) and 13 for the second launch, which begins beside it: 29 together in graph replay;
-// 16384 tokens, 8 of 128, bf16: 23 and 10, 22 together.  4 tokens: 4 us of latencies.
+// groups with a bias, f32, 26 us with cold caches (320 GB/s; bytes would take 1.4) and 13 for the second launch, which begins beside it: 33 together in graph replay, inputs not in L2;
+// 16384 tokens, 8 of 128, bf16: 21 and 10, 26 together.  4 tokens: 4 us of latencies.
 template <typename T, int V>
 __global__ void __launch_bounds__(V > 16 ? 512 : 1024) route_kernel(const RouteParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
